@@ -357,6 +357,84 @@ MOM_API int mom_gumbel(const float *u, int64_t n, float noise_scale, float *out,
  * both. n % 4 == 0, dk / dv 16-byte and out 8-byte aligned. */
 MOM_API int mom_kv_pack_bf16(const float *dk, const float *dv, int64_t L, int64_t n, void *out, void *stream);
 
+/* ------------------------------------------------------------------ serving
+ * The decoder answering instead of training: no counterpart in the reference,
+ * whose model recomputes the whole prefix for each new token. bf16 throughout
+ * (fp32 sums, maxima and products), head_dim 64 or 128, H query heads on Hk key
+ * heads (H a multiple of Hk; query head h reads key head h / (H / Hk)). Pointers
+ * 16-byte aligned, row pitches (in elements) multiples of 8.
+ *
+ * The cache: k_pages, v_pages (num_pages, Hk, page_size, hd), page_size a power
+ * of two in [8, 256]; a token's slot is page * page_size + its offset there.
+ *
+ * mom_rope_append: qkv (T, [q | k | v] heads) of row pitch qkv_ld, the fused
+ * projection's output; cos, sin (n_pos, hd) fp32; positions, slots (T) I32 or
+ * I64. Writes q (T, H, hd) rotated, the rotated keys and the values into their
+ * slots and, when k is not NULL, the rotated keys (T, Hk, hd) side by side. The
+ * rotation is mom_rope_qkv_fwd's, bit for bit. A slot outside
+ * [0, num_pages * page_size) is not written (padding: -1); a position outside
+ * [0, n_pos) makes the token's q and k NaN. Two tokens of a call must not share
+ * a slot. */
+MOM_API int mom_rope_append(const void *qkv, int64_t qkv_ld, const float *cos, const float *sin, int64_t n_pos,
+                            const void *positions, int pos_dtype, const void *slots, int slot_dtype, int64_t T,
+                            int64_t H, int64_t Hk, int64_t head_dim, int64_t num_pages, int64_t page_size,
+                            void *k_pages, void *v_pages, void *q, void *k, void *stream);
+
+/* Attention of one new token per sequence over its cached keys: q (B, H, hd) of
+ * row pitch q_ld; block_table (B, table_ld) I32, the pages of each sequence in
+ * order; seq_lens (B) I32 on the device, the keys of each sequence (the new
+ * token's own among them). out (B, H, hd) = softmax(scale q.k) v. max_len: an
+ * upper bound of seq_lens known to the host (at most table_ld * page_size); the
+ * work is split over it, and a workspace of mom_decode_attn_workspace_size bytes
+ * joins the parts. A sequence of length <= 0 gets zeros; one longer than max_len,
+ * or with a page outside [0, num_pages) among its keys, gets NaN. What the pages
+ * hold behind a sequence's end is not read into the result, NaN neither. */
+MOM_API size_t mom_decode_attn_workspace_size(int64_t B, int64_t H, int64_t Hk, int64_t head_dim, int64_t max_len);
+MOM_API int mom_decode_attn(const void *q, int64_t q_ld, const void *k_pages, const void *v_pages, int64_t num_pages,
+                            int64_t page_size, const int32_t *block_table, int64_t table_ld, const int32_t *seq_lens,
+                            int64_t max_len, int64_t B, int64_t H, int64_t Hk, int64_t head_dim, double scale,
+                            void *out, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Causal attention over packed prompts: n sequences one after another in q
+ * (Tq, H, hd) and k, v (Tk, Hk, hd), rows of pitch q_ld, k_ld, v_ld; out
+ * (Tq, H, hd) contiguous. A sequence may have more keys than queries (its prefix
+ * is cached): the mask is aligned at the end, row r of Lq sees keys
+ * 0 .. Lk - Lq + r; a row that sees none (Lk < Lq) gets zeros. Values that the
+ * mask hides from a row do not reach it, NaN and infinities neither.
+ *
+ * The plan depends on the lengths alone and serves every layer of a model:
+ * mom_prompt_plan fills mom_prompt_plan_size bytes of HOST memory (k_lens may be
+ * NULL: k_lens = q_lens), which the caller copies to the device; mom_prompt_attn
+ * takes the device copy and its size. mom_prompt_plan_check reads and clears the
+ * plan's device error word (it synchronises `stream`). */
+MOM_API size_t mom_prompt_plan_size(const int64_t *q_lens, int64_t n);
+MOM_API int mom_prompt_plan(const int64_t *q_lens, const int64_t *k_lens, int64_t n, void *plan_host,
+                            size_t plan_bytes);
+MOM_API int mom_prompt_attn(const void *q, int64_t q_ld, const void *k, int64_t k_ld, const void *v, int64_t v_ld,
+                            int64_t Tq, int64_t Tk, int64_t H, int64_t Hk, int64_t head_dim, double scale, void *plan,
+                            size_t plan_bytes, void *out, void *stream);
+MOM_API int mom_prompt_plan_check(void *plan, void *stream);
+
+/* ------------------------------------------------------------------ scoring
+ * Log probabilities of given tokens (no counterpart in the reference, which has
+ * only the summed training loss): logits (R, V) F32 or BF16 of row pitch ld,
+ * y = logits / temperature; targets (R) int64. logprob (R) = log_softmax(y)[t]
+ * (0 where t == ignore_index, NaN where t is outside [0, V)), entropy (R) of
+ * softmax(y), and the top_k (<= 32) greatest logits in order, ties to the lowest
+ * index, NaN above all: top_idx (R, top_k) int64 and their top_logprob. All fp32.
+ * A logit of -inf has probability 0; a row with a NaN or +inf, or of nothing but
+ * -inf, gets NaN. stats (R, 4) fp32 for the backward, or NULL.
+ * mom_logprobs_bwd: dlogits (R, V) in the logits' dtype, contiguous, from the
+ * gradients of logprob (R), entropy (R) and top_logprob (R, top_k), each of which
+ * may be NULL (none); ignored rows have no gradient from their logprob. */
+MOM_API int mom_logprobs_fwd(const void *logits, int dtype, int64_t ld, const int64_t *targets, int64_t R, int64_t V,
+                             int64_t ignore_index, double temperature, int64_t top_k, float *logprob, float *entropy,
+                             float *top_logprob, int64_t *top_idx, float *stats, void *stream);
+MOM_API int mom_logprobs_bwd(const void *logits, int dtype, int64_t ld, const int64_t *targets, const float *stats,
+                             const int64_t *top_idx, int64_t top_k, const float *g_logprob, const float *g_entropy,
+                             const float *g_top, int64_t R, int64_t V, int64_t ignore_index, double temperature,
+                             void *dlogits, void *stream);
+
 /* Reads (and clears) the device error word of a plan: MOM_OK, or
  * MOM_ERR_DEVICE_INDEX when mom_bucket saw an index outside [0, nb).
  * Synchronises `stream`. */

@@ -84,6 +84,20 @@ SIGNATURES = {
     "mom_read_bwd_noalloc_max_bytes": (_sz, []),
     "mom_read_bwd_noalloc": (_int, [_vp, _vp, _vp, _vp, _vp, _fp, _int, _i64, _i64, _i64, _i64, _i64,
                                     _i64, _i64, _vp, _vp, _vp, _fp, _fp, _fp, _vp]),
+    "mom_rope_append": (_int, [_vp, _i64, _fp, _fp, _i64, _vp, _int, _vp, _int, _i64, _i64, _i64, _i64, _i64, _i64,
+                               _vp, _vp, _vp, _vp, _vp]),
+    "mom_decode_attn_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64]),
+    "mom_decode_attn": (_int, [_vp, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64,
+                               _c.c_double, _vp, _vp, _sz, _vp]),
+    "mom_prompt_plan_size": (_sz, [_vp, _i64]),
+    "mom_prompt_plan": (_int, [_vp, _vp, _i64, _vp, _sz]),
+    "mom_prompt_attn": (_int, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _c.c_double, _vp, _sz,
+                               _vp, _vp]),
+    "mom_prompt_plan_check": (_int, [_vp, _vp]),
+    "mom_logprobs_fwd": (_int, [_vp, _int, _i64, _vp, _i64, _i64, _i64, _c.c_double, _i64, _fp, _fp, _fp, _vp, _fp,
+                                _vp]),
+    "mom_logprobs_bwd": (_int, [_vp, _int, _i64, _vp, _fp, _vp, _i64, _fp, _fp, _fp, _i64, _i64, _i64, _c.c_double,
+                                _vp, _vp]),
 }
 
 _lock = threading.Lock()

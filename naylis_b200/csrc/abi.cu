@@ -857,6 +857,207 @@ int mom_xent_bwd(const void *logits, const int64_t *labels, const float *lse, co
     return e == cudaSuccess ? MOM_OK : cuda_fail(e, "xent_bwd");
 }
 
+// ------------------------------------------------------------------ serving
+namespace {
+int page_shift_of(int64_t page_size) {
+    int sh = 0;
+    while ((int64_t(1) << sh) < page_size) ++sh;
+    return sh;
+}
+bool aligned(const void *p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+int check_attn_geometry(int64_t H, int64_t Hk, int64_t hd) {
+    MOM_REQUIRE(H > 0 && Hk > 0 && H % Hk == 0 && H <= 65535, "n_heads (%lld) must be a positive multiple of n_kv_heads (%lld)",
+                (long long)H, (long long)Hk);
+    if (hd != 64 && hd != 128) return fail(MOM_ERR_UNSUPPORTED, "head_dim %lld: 64 or 128", (long long)hd);
+    return MOM_OK;
+}
+int check_cache_geometry(int64_t num_pages, int64_t page_size) {
+    MOM_REQUIRE(num_pages >= 0, "num_pages must be >= 0");
+    MOM_REQUIRE(page_size >= 8 && page_size <= 256 && (page_size & (page_size - 1)) == 0,
+                "page_size must be a power of two in [8, 256] (got %lld)", (long long)page_size);
+    MOM_REQUIRE(num_pages <= INT32_MAX, "num_pages too large");
+    return MOM_OK;
+}
+}  // namespace
+
+int mom_rope_append(const void *qkv, int64_t qkv_ld, const float *cosv, const float *sinv, int64_t n_pos,
+                    const void *positions, int pos_dtype, const void *slots, int slot_dtype, int64_t T, int64_t H,
+                    int64_t Hk, int64_t hd, int64_t num_pages, int64_t page_size, void *k_pages, void *v_pages,
+                    void *q, void *k, void *stream) {
+    int rc = check_attn_geometry(H, Hk, hd);
+    if (rc) return rc;
+    if ((rc = check_cache_geometry(num_pages, page_size))) return rc;
+    MOM_REQUIRE(is_idx_dtype(pos_dtype) && is_idx_dtype(slot_dtype), "positions and slots must be I32 or I64");
+    MOM_REQUIRE(T >= 0 && n_pos >= 0 && T < (int64_t(1) << 31), "bad token or position count");
+    MOM_REQUIRE(qkv_ld >= (H + 2 * Hk) * hd && qkv_ld % 8 == 0, "qkv row pitch must hold all heads and be a multiple of 8");
+    if (T == 0) return MOM_OK;
+    MOM_REQUIRE(qkv && cosv && sinv && positions && slots && q, "null pointer argument");
+    MOM_REQUIRE(num_pages == 0 || (k_pages && v_pages), "null pointer argument");
+    MOM_REQUIRE(aligned(qkv, 16) && aligned(cosv, 16) && aligned(sinv, 16) && aligned(k_pages, 16) &&
+                    aligned(v_pages, 16) && aligned(q, 16) && aligned(k, 16),
+                "buffers must be 16-byte aligned");
+    if ((rc = check_current_device())) return rc;
+    cudaError_t e = mom::launch_rope_append(qkv, qkv_ld, cosv, sinv, n_pos, positions, pos_dtype == MOM_I64, slots,
+                                            slot_dtype == MOM_I64, T, (int)H, (int)Hk, (int)hd, num_pages,
+                                            page_shift_of(page_size), k_pages, v_pages, q, k,
+                                            static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? MOM_OK : cuda_fail(e, "rope_append");
+}
+
+size_t mom_decode_attn_workspace_size(int64_t B, int64_t H, int64_t Hk, int64_t hd, int64_t max_len) {
+    if (B <= 0 || H <= 0 || Hk <= 0 || hd <= 0 || max_len <= 0) return 0;
+    const mom::DecodeSplit s = mom::decode_split(B, H, Hk, max_len);
+    return s.n_chunks == 1 ? 0 : static_cast<size_t>(B) * H * s.n_chunks * (hd + 2) * sizeof(float);
+}
+
+int mom_decode_attn(const void *q, int64_t q_ld, const void *k_pages, const void *v_pages, int64_t num_pages,
+                    int64_t page_size, const int32_t *block_table, int64_t table_ld, const int32_t *seq_lens,
+                    int64_t max_len, int64_t B, int64_t H, int64_t Hk, int64_t hd, double scale, void *out,
+                    void *workspace, size_t workspace_bytes, void *stream) {
+    int rc = check_attn_geometry(H, Hk, hd);
+    if (rc) return rc;
+    if ((rc = check_cache_geometry(num_pages, page_size))) return rc;
+    MOM_REQUIRE(B >= 0 && B <= 65535, "B must be in [0, 65535] (got %lld)", (long long)B);
+    MOM_REQUIRE(max_len >= 0 && max_len <= INT32_MAX, "max_len out of range");
+    MOM_REQUIRE(table_ld >= 0 && max_len <= table_ld * page_size, "max_len exceeds the block table (%lld pages of %lld)",
+                (long long)table_ld, (long long)page_size);
+    MOM_REQUIRE(q_ld >= H * hd && q_ld % 8 == 0, "q row pitch must hold all heads and be a multiple of 8");
+    MOM_REQUIRE(std::isfinite(scale), "scale must be finite");
+    if (B == 0) return MOM_OK;
+    MOM_REQUIRE(q && seq_lens && out, "null pointer argument");
+    MOM_REQUIRE(max_len == 0 || (block_table && (num_pages == 0 || (k_pages && v_pages))), "null pointer argument");
+    MOM_REQUIRE(aligned(q, 16) && aligned(k_pages, 16) && aligned(v_pages, 16) && aligned(out, 16) &&
+                    aligned(workspace, 16),
+                "buffers must be 16-byte aligned");
+    const size_t need = mom_decode_attn_workspace_size(B, H, Hk, hd, max_len);
+    if (need > 0 && (!workspace || workspace_bytes < need))
+        return fail(MOM_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    if ((rc = check_current_device())) return rc;
+    cudaError_t e = mom::launch_decode_attn(q, q_ld, k_pages, v_pages, num_pages, page_shift_of(page_size),
+                                            block_table, table_ld, seq_lens, max_len, B, (int)H, (int)Hk, (int)hd,
+                                            (float)scale, out, static_cast<float *>(workspace),
+                                            static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? MOM_OK : cuda_fail(e, "decode_attn");
+}
+
+namespace {
+int check_prompt_lens(const int64_t *q_lens, const int64_t *k_lens, int64_t n) {
+    MOM_REQUIRE(n >= 0 && n < (int64_t(1) << 31) && (n == 0 || q_lens), "bad sequence count or null lengths");
+    int64_t tq = 0, tk = 0;
+    for (int64_t i = 0; i < n; ++i) {
+        const int64_t lk = k_lens ? k_lens[i] : q_lens[i];
+        MOM_REQUIRE(q_lens[i] >= 0 && lk >= 0 && q_lens[i] <= (1 << 30) && lk <= (1 << 30),
+                    "sequence %lld: lengths must be in [0, 2^30]", (long long)i);
+        tq += q_lens[i];
+        tk += lk;
+        MOM_REQUIRE(tq <= (1 << 30) && tk <= (1 << 30), "packed rows out of range (2^30)");
+    }
+    return MOM_OK;
+}
+}  // namespace
+
+size_t mom_prompt_plan_size(const int64_t *q_lens, int64_t n) {
+    if (check_prompt_lens(q_lens, nullptr, n) != MOM_OK) return 0;
+    return mom::kPromptHeader + static_cast<size_t>(mom::prompt_tiles(q_lens, n)) * sizeof(mom::PromptTile);
+}
+
+int mom_prompt_plan(const int64_t *q_lens, const int64_t *k_lens, int64_t n, void *plan_host, size_t plan_bytes) {
+    int rc = check_prompt_lens(q_lens, k_lens, n);
+    if (rc) return rc;
+    MOM_REQUIRE(plan_host, "null pointer argument");
+    const size_t need = mom_prompt_plan_size(q_lens, n);
+    if (plan_bytes < need) return fail(MOM_ERR_WORKSPACE, "plan of %zu bytes, %zu needed", plan_bytes, need);
+    std::memset(plan_host, 0, mom::kPromptHeader);
+    mom::prompt_plan(q_lens, k_lens, n,
+                     reinterpret_cast<mom::PromptTile *>(static_cast<char *>(plan_host) + mom::kPromptHeader));
+    return MOM_OK;
+}
+
+int mom_prompt_attn(const void *q, int64_t q_ld, const void *k, int64_t k_ld, const void *v, int64_t v_ld, int64_t Tq,
+                    int64_t Tk, int64_t H, int64_t Hk, int64_t hd, double scale, void *plan, size_t plan_bytes,
+                    void *out, void *stream) {
+    int rc = check_attn_geometry(H, Hk, hd);
+    if (rc) return rc;
+    MOM_REQUIRE(Tq >= 0 && Tk >= 0 && Tq <= (1 << 30) && Tk <= (1 << 30), "packed rows out of range (2^30)");
+    MOM_REQUIRE(q_ld >= H * hd && q_ld % 8 == 0 && k_ld >= Hk * hd && k_ld % 8 == 0 && v_ld >= Hk * hd && v_ld % 8 == 0,
+                "row pitches must hold all heads and be multiples of 8");
+    MOM_REQUIRE(std::isfinite(scale), "scale must be finite");
+    if (Tq == 0) return MOM_OK;
+    MOM_REQUIRE(q && plan && out && (Tk == 0 || (k && v)), "null pointer argument");
+    MOM_REQUIRE(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 16) && aligned(plan, 16),
+                "buffers must be 16-byte aligned");
+    MOM_REQUIRE(plan_bytes > mom::kPromptHeader && (plan_bytes - mom::kPromptHeader) % sizeof(mom::PromptTile) == 0,
+                "plan_bytes is not a plan's size");
+    const int64_t n_tiles = (plan_bytes - mom::kPromptHeader) / sizeof(mom::PromptTile);
+    MOM_REQUIRE(n_tiles * H < (int64_t(1) << 31), "too many tiles");
+    if ((rc = check_current_device())) return rc;
+    cudaError_t e = mom::launch_prompt_attn(
+        q, q_ld, k, k_ld, v, v_ld, Tq, Tk,
+        reinterpret_cast<const mom::PromptTile *>(static_cast<const char *>(plan) + mom::kPromptHeader), n_tiles,
+        static_cast<int *>(plan), (int)H, (int)Hk, (int)hd, (float)scale, out, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? MOM_OK : cuda_fail(e, "prompt_attn");
+}
+
+int mom_prompt_plan_check(void *plan, void *stream) {
+    MOM_REQUIRE(plan, "null pointer argument");
+    int err = 0;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaError_t e = cudaMemcpyAsync(&err, plan, sizeof(int), cudaMemcpyDeviceToHost, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    if (e == cudaSuccess && err) e = cudaMemsetAsync(plan, 0, sizeof(int), st);
+    if (e != cudaSuccess) return cuda_fail(e, "prompt_plan_check");
+    if (err & 2) return fail(MOM_ERR_DEVICE_TIMEOUT, "a bounded device-side wait gave up");
+    return MOM_OK;
+}
+
+// ------------------------------------------------------------------ scoring
+namespace {
+int check_logprobs(int dtype, int64_t ld, int64_t R, int64_t V, double temperature, int64_t top) {
+    MOM_REQUIRE(is_float_dtype(dtype), "logits must be F32 or BF16");
+    MOM_REQUIRE(R >= 0 && R < (int64_t(1) << 31) && V > 0 && V < (int64_t(1) << 31), "bad logits geometry");
+    MOM_REQUIRE(ld >= V, "row pitch smaller than the vocabulary");
+    MOM_REQUIRE(std::isfinite(temperature) && temperature > 0.0 && std::isfinite(1.0f / (float)temperature),
+                "temperature must be positive");
+    MOM_REQUIRE(top >= 0 && top <= mom::kMaxTopLogprobs && top <= V, "top_k must be in [0, min(%d, vocabulary)]",
+                mom::kMaxTopLogprobs);
+    return MOM_OK;
+}
+}  // namespace
+
+int mom_logprobs_fwd(const void *logits, int dtype, int64_t ld, const int64_t *targets, int64_t R, int64_t V,
+                     int64_t ignore_index, double temperature, int64_t top_k, float *logprob, float *entropy,
+                     float *top_logprob, int64_t *top_idx, float *stats, void *stream) {
+    int rc = check_logprobs(dtype, ld, R, V, temperature, top_k);
+    if (rc) return rc;
+    if (R == 0) return MOM_OK;
+    MOM_REQUIRE(logits && targets && logprob && entropy && (top_k == 0 || (top_logprob && top_idx)),
+                "null pointer argument");
+    MOM_REQUIRE(aligned(logits, dt_size(dtype)) && aligned(stats, 16), "logits or stats misaligned");
+    if ((rc = check_current_device())) return rc;
+    cudaError_t e = mom::launch_logprobs_fwd(logits, dtype, ld, targets, R, (int)V, ignore_index,
+                                             (float)(1.0 / temperature), (int)top_k, logprob, entropy, top_logprob,
+                                             top_idx, stats, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? MOM_OK : cuda_fail(e, "logprobs_fwd");
+}
+
+int mom_logprobs_bwd(const void *logits, int dtype, int64_t ld, const int64_t *targets, const float *stats,
+                     const int64_t *top_idx, int64_t top_k, const float *g_logprob, const float *g_entropy,
+                     const float *g_top, int64_t R, int64_t V, int64_t ignore_index, double temperature,
+                     void *dlogits, void *stream) {
+    int rc = check_logprobs(dtype, ld, R, V, temperature, top_k);
+    if (rc) return rc;
+    if (R == 0) return MOM_OK;
+    MOM_REQUIRE(logits && targets && stats && dlogits && (top_k == 0 || !g_top || top_idx), "null pointer argument");
+    MOM_REQUIRE(aligned(logits, dt_size(dtype)) && aligned(dlogits, dt_size(dtype)) && aligned(stats, 16),
+                "logits, dlogits or stats misaligned");
+    if ((rc = check_current_device())) return rc;
+    cudaError_t e = mom::launch_logprobs_bwd(logits, dtype, ld, targets, stats, top_idx, (int)top_k, g_logprob,
+                                             g_entropy, g_top, R, (int)V, ignore_index, (float)(1.0 / temperature),
+                                             dlogits, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? MOM_OK : cuda_fail(e, "logprobs_bwd");
+}
+
 // ------------------------------------------------- read backward, no allocation
 // mom_read_bwd_noalloc runs mom_read_bwd with its workspace (the per-row delta,
 // H x B*S fp32) in a fixed device array of this library instead of caller

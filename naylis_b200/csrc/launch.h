@@ -214,4 +214,47 @@ cudaError_t launch_xent_fwd(const void *logits, const int64_t *labels, int64_t R
 cudaError_t launch_xent_bwd(const void *logits, const int64_t *labels, const float *lse, const float *grad, int64_t R,
                             int V, int64_t ignore_index, void *dlogits, cudaStream_t st);
 
+// Serving (serve.cu): rotary embedding by explicit positions of a fused projection's
+// heads with the cache write, and one new token's attention over paged K / V
+// (n_pages, Hk, 1 << page_shift, hd) bf16. `part` holds the chunks' partial sums:
+// decode_split says how many chunks a call of these sizes takes.
+cudaError_t launch_rope_append(const void *qkv, int64_t ld, const float *cosv, const float *sinv, int64_t n_pos,
+                               const void *positions, int pos64, const void *slots, int slot64, int64_t T, int H,
+                               int Hk, int hd, int64_t n_pages, int page_shift, void *kp, void *vp, void *q, void *k,
+                               cudaStream_t st);
+struct DecodeSplit {
+    int chunk = 0;      // keys of a chunk
+    int n_chunks = 1;   // chunks of the longest sequence the call may hold
+};
+DecodeSplit decode_split(int64_t B, int64_t H, int64_t Hk, int64_t max_len);
+cudaError_t launch_decode_attn(const void *q, int64_t q_ld, const void *kp, const void *vp, int64_t n_pages,
+                               int page_shift, const int32_t *table, int64_t table_ld, const int32_t *seq_lens,
+                               int64_t max_len, int64_t B, int H, int Hk, int hd, float scale, void *out, float *part,
+                               cudaStream_t st);
+
+// Packed prompts (prompt.cu): the plan's tiles of query rows, costliest first.
+constexpr int kPromptRows = 256;
+struct PromptTile {
+    int32_t q0;     // first query row (packed)
+    int32_t rows;   // 1 .. kPromptRows
+    int32_t k0;     // the sequence's first key row (packed)
+    int32_t vis;    // keys the first row sees (<= 0: none); row r sees vis + r
+};
+constexpr int kPromptHeader = 16;   // bytes before the tiles in a plan: the error word
+int64_t prompt_tiles(const int64_t *q_lens, int64_t n);
+void prompt_plan(const int64_t *q_lens, const int64_t *k_lens, int64_t n, PromptTile *tiles);
+cudaError_t launch_prompt_attn(const void *q, int64_t q_ld, const void *k, int64_t k_ld, const void *v, int64_t v_ld,
+                               int64_t Tq, int64_t Tk, const PromptTile *tiles, int64_t n_tiles, int *err, int H,
+                               int Hk, int hd, float scale, void *out, cudaStream_t st);
+
+// Token log probabilities (scoring.cu): logits (R, V) of row pitch ld; stats (R, 4).
+constexpr int kMaxTopLogprobs = 32;
+cudaError_t launch_logprobs_fwd(const void *logits, int dt, int64_t ld, const int64_t *targets, int64_t R, int V,
+                                int64_t ignore, float inv_t, int top, float *logprob, float *entropy, float *top_lp,
+                                int64_t *top_idx, float *stats, cudaStream_t st);
+cudaError_t launch_logprobs_bwd(const void *logits, int dt, int64_t ld, const int64_t *targets, const float *stats,
+                                const int64_t *top_idx, int top, const float *g_lp, const float *g_ent,
+                                const float *g_top, int64_t R, int V, int64_t ignore, float inv_t, void *dlogits,
+                                cudaStream_t st);
+
 }  // namespace mom

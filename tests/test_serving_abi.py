@@ -1,0 +1,119 @@
+"""CPU tests of the serving and scoring entry points of the C ABI: the prompt plan
+(host code) and the arguments they reject before any device work."""
+import ctypes
+
+import numpy as np
+import pytest
+
+P = ctypes.c_void_p
+OK, INVALID, UNSUPPORTED, WORKSPACE = 0, 1, 2, 4
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from naylis_b200 import _lib, build
+    build.build()
+    return _lib.load()
+
+
+def _plan(lib, ql, kl=None):
+    q = np.asarray(ql, dtype=np.int64)
+    k = None if kl is None else np.asarray(kl, dtype=np.int64)
+    size = lib.mom_prompt_plan_size(q.ctypes.data, len(ql))
+    buf = np.full(size, 0xAB, dtype=np.uint8)
+    rc = lib.mom_prompt_plan(q.ctypes.data, None if k is None else k.ctypes.data, len(ql), buf.ctypes.data, size)
+    assert rc == OK
+    return buf[:16], buf[16:].view(np.int32).reshape(-1, 4)
+
+
+@pytest.mark.parametrize("ql,kl", [([1], None), ([256, 257, 0, 1, 1000], None), ([5, 300], [400, 10]), ([0, 0], None)])
+def test_plan_covers_every_row_once_and_puts_the_costliest_first(lib, ql, kl):
+    head, tiles = _plan(lib, ql, kl)
+    assert not head.any()
+    seen = np.zeros(sum(ql), dtype=int)
+    q0 = np.concatenate([[0], np.cumsum(ql)])
+    k0 = np.concatenate([[0], np.cumsum(kl or ql)])
+    for a, rows, k, vis in tiles:
+        assert 1 <= rows <= 256
+        seen[a:a + rows] += 1
+        i = int(np.searchsorted(q0, a, side="right") - 1)
+        assert a + rows <= q0[i + 1] and k == k0[i]
+        assert vis == (kl or ql)[i] - ql[i] + (a - q0[i]) + 1
+    assert (seen == 1).all()
+    last = tiles[:, 3] + tiles[:, 1]
+    assert (np.diff(last) <= 0).all()
+
+
+def test_plan_refuses(lib):
+    one = np.asarray([-1], dtype=np.int64)
+    assert lib.mom_prompt_plan_size(one.ctypes.data, 1) == 0 and b"lengths" in lib.mom_last_error_string()
+    big = np.asarray([1 << 30, 1 << 30], dtype=np.int64)
+    assert lib.mom_prompt_plan_size(big.ctypes.data, 2) == 0
+    two = np.asarray([300, 4], dtype=np.int64)
+    buf = np.zeros(64, dtype=np.uint8)
+    assert lib.mom_prompt_plan(two.ctypes.data, None, 2, buf.ctypes.data, 32) == WORKSPACE
+    assert lib.mom_prompt_plan(two.ctypes.data, None, 2, None, 64) == INVALID
+
+
+def _rope(lib, **kw):
+    a = dict(qkv=P(256), ld=384, cos=P(256), sin=P(256), n_pos=8, pos=P(256), pt=3, slots=P(256), st=3, T=2, H=2, Hk=2,
+             hd=64, pages=4, page=16, kp=P(256), vp=P(256), q=P(256), k=None, stream=None)
+    a.update(kw)
+    return lib.mom_rope_append(*a.values())
+
+
+def _decode(lib, **kw):
+    a = dict(q=P(256), ld=128, kp=P(256), vp=P(256), pages=4, page=16, table=P(256), tld=4, lens=P(256), max_len=64,
+             B=2, H=2, Hk=2, hd=64, scale=0.1, out=P(256), ws=P(256), wsb=1 << 30, stream=None)
+    a.update(kw)
+    return lib.mom_decode_attn(*a.values())
+
+
+def _prompt(lib, **kw):
+    a = dict(q=P(256), qld=128, k=P(256), kld=128, v=P(256), vld=128, Tq=3, Tk=3, H=2, Hk=2, hd=64, scale=0.1,
+             plan=P(256), bytes=32, out=P(256), stream=None)
+    a.update(kw)
+    return lib.mom_prompt_attn(*a.values())
+
+
+def _lp(lib, **kw):
+    a = dict(x=P(256), dt=1, ld=20, t=P(256), R=2, V=20, ignore=-100, T=1.0, top=2, lp=P(256), ent=P(256), tl=P(256),
+             ti=P(256), stats=P(256), stream=None)
+    a.update(kw)
+    return lib.mom_logprobs_fwd(*a.values())
+
+
+def _lpb(lib, **kw):
+    a = dict(x=P(256), dt=1, ld=20, t=P(256), stats=P(256), ti=P(256), top=2, g=P(256), h=P(256), a=P(256), R=2, V=20,
+             ignore=-100, T=1.0, dx=P(256), stream=None)
+    a.update(kw)
+    return lib.mom_logprobs_bwd(*a.values())
+
+
+def test_bad_arguments_fail_before_device_work(lib):
+    for kw in (dict(H=3), dict(Hk=0), dict(ld=383), dict(ld=376), dict(page=12), dict(page=4), dict(page=512), dict(T=-1),
+               dict(pt=0), dict(st=1), dict(qkv=P(264)), dict(qkv=None), dict(kp=None), dict(q=None), dict(n_pos=-1)):
+        assert _rope(lib, **kw) == INVALID, kw
+    assert _rope(lib, hd=96) == UNSUPPORTED
+    assert _rope(lib, T=0, qkv=None) == OK
+    for kw in (dict(H=3), dict(B=-1), dict(B=70000), dict(max_len=65), dict(max_len=-1), dict(ld=120), dict(ld=132),
+               dict(scale=float("nan")), dict(q=None), dict(lens=None), dict(table=None), dict(out=P(260)), dict(page=20)):
+        assert _decode(lib, **kw) == INVALID, kw
+    assert _decode(lib, hd=32) == UNSUPPORTED
+    assert _decode(lib, B=0, q=None) == OK
+    long = dict(tld=1 << 16, max_len=1 << 20)
+    need = lib.mom_decode_attn_workspace_size(2, 2, 2, 64, 1 << 20)
+    assert need > 0 and _decode(lib, **long, ws=None, wsb=0) == WORKSPACE
+    assert _decode(lib, **long, wsb=need - 1) == WORKSPACE
+    for kw in (dict(H=3), dict(Tq=-1), dict(kld=64), dict(vld=132), dict(scale=float("inf")), dict(plan=None),
+               dict(bytes=16), dict(bytes=40), dict(q=P(264)), dict(out=None), dict(v=None)):
+        assert _prompt(lib, **kw) == INVALID, kw
+    assert _prompt(lib, hd=256) == UNSUPPORTED
+    assert _prompt(lib, Tq=0, q=None) == OK
+    for kw in (dict(dt=2), dict(ld=19), dict(V=0), dict(R=-1), dict(T=0.0), dict(T=float("nan")), dict(T=1e-60),
+               dict(top=33), dict(top=21), dict(top=-1), dict(x=None), dict(t=None), dict(ti=None), dict(x=P(257)),
+               dict(stats=P(264))):
+        assert _lp(lib, **kw) == INVALID, kw
+    assert _lp(lib, R=0, x=None) == OK
+    for kw in (dict(stats=None), dict(dx=None), dict(ti=None), dict(dx=P(257)), dict(T=-1.0)):
+        assert _lpb(lib, **kw) == INVALID, kw
