@@ -162,7 +162,7 @@ def prompt_attention(q, k, v, plan: PromptPlan, *, scale=None):
     bf16, the plan's sequences one after another (token strides may be a fused
     projection's); query head h reads key head h // (H // Hk). Row r of a sequence
     of Lq queries and Lk keys sees its keys 0 .. Lk - Lq + r; one that sees none
-    gets zeros. scale defaults to hd ** -0.5. Returns (Tq, H, hd) bf16."""
+    gets zeros. scale (> 0) defaults to hd ** -0.5. Returns (Tq, H, hd) bf16."""
     _check("prompt_attention", q, k, v)
     q, q_ld = _rows("prompt_attention", q, "q")
     k, k_ld = _rows("prompt_attention", k, "k")

@@ -923,7 +923,7 @@ int mom_decode_attn(const void *q, int64_t q_ld, const void *k_pages, const void
     MOM_REQUIRE(table_ld >= 0 && max_len <= table_ld * page_size, "max_len exceeds the block table (%lld pages of %lld)",
                 (long long)table_ld, (long long)page_size);
     MOM_REQUIRE(q_ld >= H * hd && q_ld % 8 == 0, "q row pitch must hold all heads and be a multiple of 8");
-    MOM_REQUIRE(std::isfinite(scale), "scale must be finite");
+    MOM_REQUIRE(std::isfinite(scale) && scale > 0.0, "scale must be positive");
     if (B == 0) return MOM_OK;
     MOM_REQUIRE(q && seq_lens && out, "null pointer argument");
     MOM_REQUIRE(max_len == 0 || (block_table && (num_pages == 0 || (k_pages && v_pages))), "null pointer argument");
@@ -982,7 +982,7 @@ int mom_prompt_attn(const void *q, int64_t q_ld, const void *k, int64_t k_ld, co
     MOM_REQUIRE(Tq >= 0 && Tk >= 0 && Tq <= (1 << 30) && Tk <= (1 << 30), "packed rows out of range (2^30)");
     MOM_REQUIRE(q_ld >= H * hd && q_ld % 8 == 0 && k_ld >= Hk * hd && k_ld % 8 == 0 && v_ld >= Hk * hd && v_ld % 8 == 0,
                 "row pitches must hold all heads and be multiples of 8");
-    MOM_REQUIRE(std::isfinite(scale), "scale must be finite");
+    MOM_REQUIRE(std::isfinite(scale) && scale > 0.0, "scale must be positive");
     if (Tq == 0) return MOM_OK;
     MOM_REQUIRE(q && plan && out && (Tk == 0 || (k && v)), "null pointer argument");
     MOM_REQUIRE(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 16) && aligned(plan, 16),

@@ -1,6 +1,7 @@
 // Host-side launchers shared between the kernel files and the C ABI layer.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -213,6 +214,12 @@ cudaError_t launch_xent_fwd(const void *logits, const int64_t *labels, int64_t R
                             float *row_loss, float *lse, cudaStream_t st);
 cudaError_t launch_xent_bwd(const void *logits, const int64_t *labels, const float *lse, const float *grad, int64_t R,
                             int V, int64_t ignore_index, void *dlogits, cudaStream_t st);
+
+// Tensor maps (read_fwd_tc.cu): false when the driver has no encoder or refuses.
+// bf16 rows of `cols` elements, `pitch` elements apart; box 64 columns x box_rows, 128-B swizzle.
+bool make_bf16_map_pitched(CUtensorMap *map, const void *ptr, uint64_t rows, uint64_t cols, uint64_t pitch,
+                           uint32_t box_rows);
+int device_sm_count();
 
 // Serving (serve.cu): rotary embedding by explicit positions of a fused projection's
 // heads with the cache write, and one new token's attention over paged K / V

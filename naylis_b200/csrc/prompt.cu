@@ -5,10 +5,10 @@
 //
 // The plan lists tiles of up to kPromptRows query rows, the costliest first.
 #include <algorithm>
-#include <vector>
+#include <climits>
 
-#include "common.cuh"
 #include "launch.h"
+#include "tc_common.cuh"
 
 namespace mom {
 
@@ -38,63 +38,507 @@ void prompt_plan(const int64_t *q_lens, const int64_t *k_lens, int64_t n, Prompt
 
 namespace {
 
-// One warp per (row, head): 32 keys at a time, lane = key for the scores and
-// lane = hd/32 dimensions for the sum over values.
+constexpr int kM = 128;                        // query rows of a half (TMEM lanes)
+constexpr int kN = 128;                        // keys of a tile
+constexpr int kThreads = 512;
+constexpr uint32_t kBox = 128 * 128;           // one TMA box: 128 rows x 64 bf16 columns
+constexpr uint32_t kTmemCols = 512;            // S of half A, S of half B, O of A, O of B
+constexpr uint32_t kSCol = 0, kOCol = 256;     // P (bf16 pairs) takes the first 64 columns of its S
+constexpr int kFix = 8;
+constexpr float kRescale = 8.0f;               // log2 growth of a row maximum that O is rescaled for
+
 template <int HD>
-__global__ void __launch_bounds__(128)
-prompt_kernel(const uint16_t *__restrict__ q, int64_t q_ld, const uint16_t *__restrict__ k, int64_t k_ld,
-              const uint16_t *__restrict__ v, int64_t v_ld, const PromptTile *__restrict__ tiles, int64_t n_tiles,
-              int H, int Hk, float scale_log2, uint16_t *__restrict__ out) {
-    constexpr int kD = HD / 32;
-    __shared__ float sq[4][HD];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t item = blockIdx.x;
-    const PromptTile t = tiles[item / H];
-    const int h = static_cast<int>(item % H), hk = h / (H / Hk);
-    for (int r = warp; r < t.rows; r += 4) {
-        const int64_t row = t.q0 + r;
-        const int n = t.vis + r;
-        __syncwarp();
-        for (int d = lane; d < HD; d += 32) sq[warp][d] = bf16_bits_to_f32(q[row * q_ld + h * HD + d]);
-        __syncwarp();
-        float m = -INFINITY, l = 0.0f, acc[kD] = {};
-        for (int j0 = 0; j0 < n; j0 += 32) {
-            const int j = j0 + lane;
-            float s = -INFINITY;
-            if (j < n) {
-                const uint4 *kr = reinterpret_cast<const uint4 *>(k + (static_cast<int64_t>(t.k0) + j) * k_ld + hk * HD);
-                s = 0.0f;
-                for (int d = 0; d < HD / 8; ++d) {
-                    const uint4 w = kr[d];
-                    const uint32_t a[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        s += sq[warp][8 * d + 2 * e] * __uint_as_float(a[e] << 16) +
-                             sq[warp][8 * d + 2 * e + 1] * __uint_as_float(a[e] & 0xFFFF0000u);
-                }
-                s *= scale_log2;
-            }
-            float mx = s;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            const float mn = fmaxf(m, mx), mr = mn == -INFINITY ? 0.0f : mn;
-            const float f = exp2f(m - mr), p = j < n ? exp2f(s - mr) : 0.0f;
-            l = l * f + warp_sum(p);
-#pragma unroll
-            for (int d = 0; d < kD; ++d) acc[d] *= f;
-            const int cnt = min(32, n - j0);
-            for (int e = 0; e < cnt; ++e) {
-                const float pe = __shfl_sync(0xffffffffu, p, e);
-                const uint16_t *vr = v + (static_cast<int64_t>(t.k0) + j0 + e) * v_ld + hk * HD + lane * kD;
-#pragma unroll
-                for (int d = 0; d < kD; ++d) acc[d] += pe * bf16_bits_to_f32(vr[d]);
-            }
-            m = mn;
-        }
-        uint16_t *dst = out + (row * H + h) * HD + lane * kD;
-#pragma unroll
-        for (int d = 0; d < kD; ++d) dst[d] = f32_to_bf16_bits(n > 0 ? acc[d] / l : 0.0f);
+struct Cfg {
+    static constexpr int kBoxes = HD / 64;
+    static constexpr uint32_t kTile = kN * HD * 2;            // a K, V or Q tile
+    static constexpr int kStages = HD == 64 ? 8 : 4;          // K and V tiles in turn
+    static constexpr uint32_t kRing = kStages * kTile;
+    static constexpr uint32_t kSum = 2 * 2 * kM * 4;          // row sums [item parity][half][row]
+    static constexpr uint32_t kSmem = 2 * kTile + kRing + kSum + 1024 /*barriers*/ + 1024 /*align*/;
+    static_assert(kSmem <= 227 * 1024, "shared memory");
+};
+
+struct Bars {
+    uint64_t q_full[2], q_empty[2], kv_full[8], kv_empty[8], v_ready[8], s_full[2], p_full[2], o_full[2], o_free[2],
+        l_full[2], drain;
+    uint32_t tmem_base;
+    int abort;
+    int fix[kFix];      // item whose values needed the slow path, in slot item % kFix
+};
+static_assert(sizeof(Bars) <= 1024, "barrier block");
+
+struct Params {
+    const PromptTile *tiles;
+    int n_items, H, Hk, hd, pair;      // pair: the halves are two heads of a group, else two runs of rows
+    float scale_log2;
+    const uint16_t *v;
+    int64_t v_ld;
+    uint16_t *out;
+    int *err;
+};
+
+struct Half {
+    int q0, rows, vis, head, n;    // n: key tiles the half has to see
+};
+struct Item {
+    Half h[2];
+    int k0, hk, n;
+    bool work;
+    __device__ __forceinline__ int last() const {      // keys any row sees
+        return max(h[0].rows > 0 ? h[0].vis + h[0].rows - 1 : 0, h[1].rows > 0 ? h[1].vis + h[1].rows - 1 : 0);
     }
+    __device__ __forceinline__ int first() const {     // keys every row sees
+        return min(h[0].rows > 0 ? h[0].vis : INT_MAX, h[1].rows > 0 ? h[1].vis : INT_MAX);
+    }
+};
+
+// Item of this CTA in round i: the costliest items come first in the list and the
+// CTAs take them in turn, every other round backwards, so their sums stay close.
+__device__ __forceinline__ int item_id(int i) {
+    const int g = static_cast<int>(gridDim.x), c = static_cast<int>(blockIdx.x);
+    return i * g + ((i & 1) ? g - 1 - c : c);
+}
+
+__device__ __forceinline__ Item make_item(const Params &p, int id) {
+    Item it;
+    it.work = id < p.n_items;
+    if (!it.work) return it;
+    const PromptTile t = p.tiles[id / p.H];
+    const int rem = id % p.H;
+    it.k0 = t.k0;
+    if (p.pair) {
+        const int per = p.H / 2, sub = 1 - rem / per, hp = rem % per;
+        const int rows = min(max(t.rows - sub * kM, 0), kM);
+#pragma unroll
+        for (int a = 0; a < 2; ++a) it.h[a] = Half{t.q0 + sub * kM, rows, t.vis + sub * kM, 2 * hp + a, 0};
+    } else {
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+            it.h[a] = Half{t.q0 + a * kM, min(max(t.rows - a * kM, 0), kM), t.vis + a * kM, rem, 0};
+    }
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+        it.h[a].n = it.h[a].rows > 0 ? max(0, (it.h[a].vis + it.h[a].rows - 1 + kN - 1) / kN) : 0;
+    it.hk = it.h[0].head / (p.H / p.Hk);
+    it.n = max(it.h[0].n, it.h[1].n);
+    it.work = it.h[0].rows > 0;
+    return it;
+}
+
+// The non-finite values that were taken out of an item's cut tiles, back into 32
+// columns of a row that sees `seen` keys: each makes its sum NaN or infinite.
+__device__ __noinline__ void add_hidden_at(const uint16_t *v, int64_t v_ld, int j0, int seen, float *o) {
+    for (int j = j0; j < seen; ++j)
+        for (int e = 0; e < 32; ++e) {
+            const uint16_t x = v[j * v_ld + e];
+            if ((x & 0x7f80) == 0x7f80) o[e] += bf16_bits_to_f32(x);
+        }
+}
+__device__ __forceinline__ void add_hidden(const Params &P, const Item &it, int seen, int c, uint32_t (&o)[32]) {
+    float f[32];
+#pragma unroll
+    for (int e = 0; e < 32; ++e) f[e] = 0.0f;
+    const int hd = P.hd;
+    add_hidden_at(P.v + static_cast<int64_t>(it.k0) * P.v_ld + it.hk * hd + 32 * c, P.v_ld,
+                  max(it.first(), 0) / kN * kN, seen, f);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) + f[e]);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 1)
+prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                 const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ Params P) {
+    using C = Cfg<HD>;
+    constexpr int kStages = C::kStages;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    unsigned char *sbase = smem_raw + (base - raw);
+    const uint32_t ring = base + 2 * C::kTile;
+    float *sSum = reinterpret_cast<float *>(sbase + 2 * C::kTile + C::kRing);
+    Bars *bars = reinterpret_cast<Bars *>(sbase + 2 * C::kTile + C::kRing + C::kSum);
+    volatile int *abort_flag = &bars->abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rounds = (P.n_items + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+
+    if (threadIdx.x == 0) {
+        for (int a = 0; a < 2; ++a) {
+            tc::mbar_init(&bars->q_full[a], 1);
+            tc::mbar_init(&bars->q_empty[a], 1);
+            tc::mbar_init(&bars->s_full[a], 1);
+            tc::mbar_init(&bars->p_full[a], kM);
+            tc::mbar_init(&bars->o_full[a], 1);
+            tc::mbar_init(&bars->o_free[a], kM);
+            tc::mbar_init(&bars->l_full[a], kM);
+        }
+        for (int s = 0; s < kStages; ++s) {
+            tc::mbar_init(&bars->kv_full[s], 1);
+            tc::mbar_init(&bars->kv_empty[s], 1);
+            tc::mbar_init(&bars->v_ready[s], 2);
+        }
+        tc::mbar_init(&bars->drain, 1);
+        bars->abort = 0;
+        for (int i = 0; i < kFix; ++i) bars->fix[i] = -1;
+    }
+    if (warp == 12) {
+        tc::tmem_alloc(&bars->tmem_base, kTmemCols);
+        tc::tmem_relinquish();
+    }
+    if (warp == 13 && lane == 0) {
+        tc::prefetch_tensormap(&tmap_q);
+        tc::prefetch_tensormap(&tmap_k);
+        tc::prefetch_tensormap(&tmap_v);
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    const uint32_t tmem = bars->tmem_base;
+    auto wait = [&](uint64_t *bar, uint32_t parity) {
+        return tc::mbar_wait_warp(bar, parity, P.err, 2, abort_flag);
+    };
+
+    if (warp < 8) {
+        // ------------------------------------------------------------ softmax
+        // Warps 0-3: half A, 4-7: half B; a thread holds one row of scores.
+        tc::regs_inc<184>();
+        const int a = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+        const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+        const uint32_t tS = tmem + kSCol + a * kN + lanes, tO = tmem + kOCol + a * HD + lanes;
+        const uint64_t sc2 = tc::f2(P.scale_log2, P.scale_log2);
+        int phase = 0, par = 0;
+        bool ok = true;
+        for (int i = 0; ok && i < rounds; ++i) {
+            const Item it = make_item(P, item_id(i));
+            if (!it.work) continue;
+            const Half h = it.h[a];
+            float m = -INFINITY, l = 0.0f;
+            for (int j = 0; j < h.n; ++j) {
+                if (!(ok = wait(&bars->s_full[a], phase & 1))) break;
+                ++phase;
+                tc::tc_fence_after();
+                uint32_t v[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tc::tmem_ld32(tS + 32 * c, v[c]);
+                tc::tmem_ld_wait();
+                // keys of this tile that the row sees; warp-uniform test whether any row is cut
+                const int seen = h.vis + r - j * kN;
+                if (h.vis + quarter * 32 - j * kN < kN) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (32 * c + e >= seen) v[c][e] = __float_as_uint(-INFINITY);
+                }
+                float mx[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    mx[c] = __uint_as_float(v[c][0]);
+#pragma unroll
+                    for (int e = 1; e < 31; e += 2)
+                        mx[c] = tc::fmax3_nan(mx[c], __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
+                }
+                float top = tc::fmax3_nan(mx[0], mx[1], __uint_as_float(v[0][31]));
+                top = tc::fmax3_nan(top, mx[2], __uint_as_float(v[1][31]));
+                top = tc::fmax3_nan(top, mx[3], __uint_as_float(v[2][31]));
+                top = tc::fmax3_nan(top, top, __uint_as_float(v[3][31]));
+                // a score of NaN or +inf makes the row NaN (the polynomial below would lose it)
+                if (!(top < INFINITY)) l = __int_as_float(0x7fc00000);
+                const float mn = fmaxf(m, top * P.scale_log2);
+                if (j == 0) {
+                    m = mn;
+                } else if (__any_sync(0xffffffffu, mn > m + kRescale)) {
+                    // S(j) was issued behind PV(j-1): O is complete here
+                    const float mo = m == -INFINITY ? mn : m;
+                    const float f = mn > m + kRescale ? (mn == INFINITY ? 1.0f : tc::ex2(mo - mn)) : 1.0f;
+                    if (mn > m + kRescale) m = mn;
+                    l *= f;
+#pragma unroll
+                    for (int c = 0; c < HD / 16; ++c) {
+                        uint32_t o[16];
+                        tc::tmem_ld16(tO + 16 * c, o);
+                        tc::tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tc::tmem_st16(tO + 16 * c, o);
+                    }
+                }
+                const float mref = m == -INFINITY ? 0.0f : m;
+                const uint64_t nm2 = tc::f2(-mref, -mref);
+                uint64_t l2[2] = {tc::f2(0.0f, 0.0f), tc::f2(0.0f, 0.0f)};
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const uint32_t *s = &v[2 * c + (e >> 4)][2 * (e & 15)];
+                        const uint64_t x2 = tc::fma2(tc::f2_bits(s[0], s[1]), sc2, nm2);
+                        const uint64_t p2 = (e & 3) == 3 ? tc::ex2_poly2(x2) : tc::ex2_pair(x2);
+                        l2[e & 1] = tc::add2(l2[e & 1], p2);
+                        const float2 p = tc::f2_split(p2);
+                        pk[e] = pack_bf16x2(p.x, p.y);
+                    }
+                    tc::tmem_st32(tS + 32 * c, pk);
+                }
+                const float2 ls = tc::f2_split(tc::add2(l2[0], l2[1]));
+                l += ls.x + ls.y;
+                tc::tmem_st_wait();
+                tc::tc_fence_before();
+                tc::mbar_arrive(&bars->p_full[a]);
+            }
+            if (!ok) break;
+            if (h.n > 0) {
+                sSum[(par * 2 + a) * kM + r] = l;
+                tc::mbar_arrive(&bars->l_full[a]);
+                par ^= 1;
+            }
+        }
+    } else if (warp < 12) {
+        // ------------------------------------------------------------ epilogue
+        // One item behind the softmax: O / l to global, each thread one row.
+        tc::regs_dec<80>();
+        const int quarter = warp & 3, r = quarter * 32 + lane;
+        const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+        int phase[2] = {0, 0};
+        bool ok = true;
+        for (int i = 0; ok && i < rounds; ++i) {
+            const Item it = make_item(P, item_id(i));
+            if (!it.work) continue;
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                const Half h = it.h[a];
+                uint16_t *dst = P.out + (static_cast<int64_t>(h.q0 + r) * P.H + h.head) * HD;
+                if (h.n == 0) {
+                    if (r < h.rows)
+#pragma unroll
+                        for (int c = 0; c < HD / 8; ++c) reinterpret_cast<uint4 *>(dst)[c] = make_uint4(0, 0, 0, 0);
+                    continue;
+                }
+                const int ph = phase[a]++;
+                if (!(ok = wait(&bars->l_full[a], ph & 1) && wait(&bars->o_full[a], ph & 1))) break;
+                tc::tc_fence_after();
+                const float l = sSum[((ph & 1) * 2 + a) * kM + r];
+                const bool slow = *reinterpret_cast<volatile int *>(&bars->fix[i % kFix]) == i;
+                const float inv = h.vis + r > 0 ? 1.0f / l : 0.0f;
+                const uint32_t tO = tmem + kOCol + a * HD + lanes;
+                const bool store = r < h.rows, none = h.vis + r <= 0;
+#pragma unroll
+                for (int c = 0; c < HD / 32; ++c) {
+                    uint32_t o[32];
+                    tc::tmem_ld32(tO + 32 * c, o);
+                    tc::tmem_ld_wait();
+                    if (slow && store) add_hidden(P, it, h.vis + r, c, o);
+                    if (!store) continue;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t pk[4];
+#pragma unroll
+                        for (int z = 0; z < 4; ++z)
+                            pk[z] = pack_bf16x2(__uint_as_float(o[8 * e + 2 * z]) * inv,
+                                                __uint_as_float(o[8 * e + 2 * z + 1]) * inv);
+                        reinterpret_cast<uint4 *>(dst)[4 * c + e] =
+                            none ? make_uint4(0, 0, 0, 0) : make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                    }
+                }
+                tc::tc_fence_before();
+                tc::mbar_arrive(&bars->o_free[a]);
+            }
+        }
+    } else {
+        tc::regs_dec<64>();
+        if (warp == 12) {
+            // -------------------------------------------------------- MMA issuer
+            // Per key tile: PV of A, S of A's next tile, PV of B, S of B's next tile. The
+            // tensor pipe keeps that order, so P may live in S's columns, and one half's
+            // softmax runs under the other half's products.
+            const uint32_t idesc_s = tc::idesc_bf16_f32(kM, kN, false, false);
+            const uint32_t idesc_o = tc::idesc_bf16_f32(kM, HD, false, true);
+            int t = 0, qn[2] = {0, 0}, pn[2] = {0, 0}, on[2] = {0, 0};
+            bool ok = true;
+            auto issue_s = [&](int a, uint32_t sK, bool last) {
+                if (lane == 0) {
+                    const uint64_t ad = tc::smem_desc_sw128(base + a * C::kTile, 16, 1024);
+                    const uint64_t bd = tc::smem_desc_sw128(sK, 16, 1024);
+#pragma unroll
+                    for (int kk = 0; kk < HD / 16; ++kk) {
+                        const uint64_t step = 1024u * (kk >> 2) + 2u * (kk & 3);
+                        tc::mma_bf16_ss(tmem + kSCol + a * kN, ad + step, bd + step, idesc_s, kk > 0);
+                    }
+                    tc::mma_commit(&bars->s_full[a]);
+                    if (last) tc::mma_commit(&bars->q_empty[a]);
+                }
+                __syncwarp();
+            };
+            auto issue_pv = [&](int a, uint32_t sV, bool first, bool last) {
+                if (lane == 0) {
+                    const uint64_t bv = tc::smem_desc_sw128(sV, kBox, 1024);
+#pragma unroll
+                    for (int kk = 0; kk < kN / 16; ++kk)
+                        tc::mma_bf16_ts(tmem + kOCol + a * HD, tmem + kSCol + a * kN + 8 * kk, bv + 128 * kk, idesc_o,
+                                        !first || kk > 0);
+                    if (last) tc::mma_commit(&bars->o_full[a]);
+                }
+                __syncwarp();
+            };
+            auto stage = [&](int u) { return ring + (u % kStages) * C::kTile; };
+            auto full = [&](int u) { return wait(&bars->kv_full[u % kStages], (u / kStages) & 1); };
+            auto release = [&](int u) {
+                if (lane == 0) tc::mma_commit(&bars->kv_empty[u % kStages]);
+                __syncwarp();
+            };
+            for (int i = 0; ok && i < rounds; ++i) {
+                const Item it = make_item(P, item_id(i));
+                if (!it.work || it.n == 0) continue;
+                ok = full(t);                              // K(0)
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+                    if (ok && it.h[a].n > 0) {
+                        ok = wait(&bars->q_full[a], qn[a]++ & 1);
+                        if (!ok) break;
+                        tc::tc_fence_after();
+                        issue_s(a, stage(t), it.h[a].n == 1);
+                    }
+                if (!ok) break;
+                release(t);
+                for (int j = 0; ok && j < it.n; ++j) {
+                    const int uv = t + 1, uk = t + 2;
+                    ok = full(uv) && wait(&bars->v_ready[uv % kStages], (uv / kStages) & 1);
+                    if (!ok) break;
+                    bool have_k = false;
+#pragma unroll
+                    for (int a = 0; a < 2; ++a) {
+                        const int n = it.h[a].n;
+                        if (j >= n) continue;
+                        ok = wait(&bars->p_full[a], pn[a]++ & 1);
+                        if (ok && j == 0) {
+                            ok = on[a] == 0 || wait(&bars->o_free[a], (on[a] - 1) & 1);
+                            ++on[a];
+                        }
+                        if (!ok) break;
+                        tc::tc_fence_after();
+                        issue_pv(a, stage(uv), j == 0, j + 1 == n);
+                        if (j + 1 < n) {
+                            if (!have_k) {
+                                if (!(ok = full(uk))) break;
+                                have_k = true;
+                            }
+                            issue_s(a, stage(uk), j + 2 == n);
+                        }
+                    }
+                    if (!ok) break;
+                    release(uv);
+                    if (j + 1 < it.n) release(uk);
+                    t += 2;
+                }
+            }
+            if (lane == 0) tc::mma_commit(&bars->drain);
+            __syncwarp();
+            wait(&bars->drain, 0);
+        } else if (warp == 13) {
+            // -------------------------------------------------------- loader
+            int t = 0, qn[2] = {0, 0};
+            bool ok = true;
+            auto slot = [&](int u) { return u < kStages || wait(&bars->kv_empty[u % kStages], (u / kStages - 1) & 1); };
+            auto load_kv = [&](const CUtensorMap *map, int u, int x, int y) {
+                if (lane == 0) {
+                    uint64_t *bar = &bars->kv_full[u % kStages];
+                    tc::mbar_arrive_expect_tx(bar, C::kTile);
+#pragma unroll
+                    for (int c = 0; c < C::kBoxes; ++c)
+                        tc::tma_load_2d(ring + (u % kStages) * C::kTile + c * kBox, map, x + 64 * c, y, bar);
+                }
+                __syncwarp();
+            };
+            for (int i = 0; ok && i < rounds; ++i) {
+                const Item it = make_item(P, item_id(i));
+                if (!it.work || it.n == 0) continue;
+                for (int j = 0; j < it.n; ++j) {
+                    if (!(ok = slot(t))) break;
+                    load_kv(&tmap_k, t, it.hk * HD, it.k0 + j * kN);
+                    ++t;
+                    if (j == 0) {
+#pragma unroll
+                        for (int a = 0; a < 2; ++a) {
+                            if (it.h[a].n == 0) continue;
+                            if (!(ok = qn[a] == 0 || wait(&bars->q_empty[a], (qn[a] - 1) & 1))) break;
+                            ++qn[a];
+                            if (lane == 0) {
+                                tc::mbar_arrive_expect_tx(&bars->q_full[a], C::kTile);
+#pragma unroll
+                                for (int c = 0; c < C::kBoxes; ++c)
+                                    tc::tma_load_2d(base + a * C::kTile + c * kBox, &tmap_q,
+                                                    it.h[a].head * HD + 64 * c, it.h[a].q0, &bars->q_full[a]);
+                            }
+                            __syncwarp();
+                        }
+                        if (!ok) break;
+                    }
+                    if (!(ok = slot(t))) break;
+                    load_kv(&tmap_v, t, it.hk * HD, it.k0 + j * kN);
+                    ++t;
+                }
+            }
+            // no copy may be in flight when the CTA retires
+            for (int u = max(0, t - kStages); u < t; ++u) wait(&bars->kv_full[u % kStages], (u / kStages) & 1);
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+                if (qn[a] > 0) wait(&bars->q_full[a], (qn[a] - 1) & 1);
+        } else {
+            // -------------------------------------------------------- hidden values
+            // A weight of 0 does not hide a NaN or an infinity from a product. In the tiles
+            // that the mask cuts, these two warps zero such values (and every row behind the
+            // last key anybody sees, another sequence's) before the product; the epilogue
+            // gives the zeroed ones back to the rows that see them.
+            int t = 0;
+            bool ok = true;
+            const int w = warp - 14;
+            for (int i = 0; ok && i < rounds; ++i) {
+                const Item it = make_item(P, item_id(i));
+                if (!it.work || it.n == 0) continue;
+                const int first = it.first(), last = it.last();
+                for (int j = 0; j < it.n; ++j, t += 2) {
+                    const int u = t + 1;
+                    if (!(ok = wait(&bars->kv_full[u % kStages], (u / kStages) & 1))) break;
+                    if ((j + 1) * kN > first) {
+                        uint4 *tile = reinterpret_cast<uint4 *>(sbase + 2 * C::kTile + (u % kStages) * C::kTile);
+                        const int cut = last - j * kN;      // rows of the tile that somebody sees
+                        bool found = false;
+#pragma unroll 4
+                        for (int e = lane; e < C::kBoxes * 64 * 8; e += 32) {
+                            // box e / 512, row w * 64 + e / 8 % 64, any 16-byte chunk of it
+                            const int row = w * 64 + (e >> 3 & 63);
+                            uint4 *q = tile + (e >> 9) * (kBox / 16) + row * 8 + (e & 7);
+                            uint4 x = *q;
+                            if (row >= cut) {
+                                *q = make_uint4(0, 0, 0, 0);
+                                continue;
+                            }
+                            uint32_t a[4] = {x.x, x.y, x.z, x.w};
+                            bool hit = false;
+#pragma unroll
+                            for (int z = 0; z < 4; ++z) {
+                                if ((a[z] & 0x7f80u) == 0x7f80u) a[z] &= 0xffff0000u, hit = true;
+                                if ((a[z] & 0x7f800000u) == 0x7f800000u) a[z] &= 0x0000ffffu, hit = true;
+                            }
+                            if (hit) {
+                                *q = make_uint4(a[0], a[1], a[2], a[3]);
+                                found = true;
+                            }
+                        }
+                        if (__any_sync(0xffffffffu, found) && lane == 0)
+                            *reinterpret_cast<volatile int *>(&bars->fix[i % kFix]) = i;
+                        tc::fence_proxy_async_smem();
+                    }
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&bars->v_ready[u % kStages]);
+                }
+            }
+        }
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    if (warp == 12) tc::tmem_dealloc(tmem, kTmemCols);
 }
 
 }  // namespace
@@ -102,17 +546,33 @@ prompt_kernel(const uint16_t *__restrict__ q, int64_t q_ld, const uint16_t *__re
 cudaError_t launch_prompt_attn(const void *q, int64_t q_ld, const void *k, int64_t k_ld, const void *v, int64_t v_ld,
                                int64_t Tq, int64_t Tk, const PromptTile *tiles, int64_t n_tiles, int *err, int H,
                                int Hk, int hd, float scale, void *out, cudaStream_t st) {
-    (void)Tq, (void)Tk, (void)err;
-    const unsigned grid = static_cast<unsigned>(n_tiles * H);
-    auto go = [&](auto kernel) {
-        kernel<<<grid, 128, 0, st>>>(static_cast<const uint16_t *>(q), q_ld, static_cast<const uint16_t *>(k), k_ld,
-                                     static_cast<const uint16_t *>(v), v_ld, tiles, n_tiles, H, Hk, scale * kLog2e,
-                                     static_cast<uint16_t *>(out));
+    if (Tk == 0) return cudaMemsetAsync(out, 0, static_cast<size_t>(Tq) * H * hd * 2, st);
+    CUtensorMap mq, mk, mv;
+    if (!make_bf16_map_pitched(&mq, q, Tq, static_cast<uint64_t>(H) * hd, q_ld, kM) ||
+        !make_bf16_map_pitched(&mk, k, Tk, static_cast<uint64_t>(Hk) * hd, k_ld, kN) ||
+        !make_bf16_map_pitched(&mv, v, Tk, static_cast<uint64_t>(Hk) * hd, v_ld, kN))
+        return cudaErrorInvalidValue;
+    Params p;
+    p.tiles = tiles;
+    p.n_items = static_cast<int>(n_tiles * H);
+    p.H = H;
+    p.Hk = Hk;
+    p.hd = hd;
+    p.pair = (H / Hk) % 2 == 0;
+    p.scale_log2 = scale * kLog2e;
+    p.v = static_cast<const uint16_t *>(v);
+    p.v_ld = v_ld;
+    p.out = static_cast<uint16_t *>(out);
+    p.err = err;
+    const int grid = std::min(p.n_items, device_sm_count());
+    auto go = [&](auto kernel, uint32_t smem) -> cudaError_t {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (e != cudaSuccess) return e;
+        kernel<<<grid, kThreads, smem, st>>>(mq, mk, mv, p);
+        count_launch();
+        return cudaGetLastError();
     };
-    if (hd == 64) go(prompt_kernel<64>);
-    else go(prompt_kernel<128>);
-    count_launch();
-    return cudaGetLastError();
+    return hd == 64 ? go(prompt_tc_kernel<64>, Cfg<64>::kSmem) : go(prompt_tc_kernel<128>, Cfg<128>::kSmem);
 }
 
 }  // namespace mom

@@ -605,18 +605,23 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return fn;
 }
 
-// 2-D bf16 map over a row-major [rows, cols] matrix, box = 64 columns x box_rows, 128-B swizzle.
-bool make_bf16_map(CUtensorMap *map, const void *ptr, uint64_t rows, uint64_t cols, uint32_t box_rows) {
+// 2-D bf16 map over a [rows, cols] matrix of row pitch `pitch` elements, box = 64 columns x
+// box_rows, 128-B swizzle.
+bool make_bf16_map_pitched(CUtensorMap *map, const void *ptr, uint64_t rows, uint64_t cols, uint64_t pitch,
+                           uint32_t box_rows) {
     auto fn = encode_fn();
     if (!fn) return false;
     cuuint64_t dims[2] = {cols, rows};
-    cuuint64_t strides[1] = {cols * 2};
+    cuuint64_t strides[1] = {pitch * 2};
     cuuint32_t box[2] = {64, box_rows};
     cuuint32_t estr[2] = {1, 1};
     CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(ptr), dims, strides, box, estr,
                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS;
+}
+bool make_bf16_map(CUtensorMap *map, const void *ptr, uint64_t rows, uint64_t cols, uint32_t box_rows) {
+    return make_bf16_map_pitched(map, ptr, rows, cols, cols, box_rows);
 }
 
 // head_dim 64 with sets of up to two blocks; head_dim 128 with one block per row

@@ -162,8 +162,9 @@ def test_prompt_attention_refuses():
             attention.prompt_attention(*args)
     with pytest.raises(RuntimeError):
         attention.prompt_attention(q.clone().requires_grad_(True), k, k, plan)
-    with pytest.raises(RuntimeError):
-        attention.prompt_attention(q, k, k, plan, scale=float("nan"))
+    for scale in (float("nan"), 0.0, -0.1):
+        with pytest.raises(RuntimeError):
+            attention.prompt_attention(q, k, k, plan, scale=scale)
     for ql, kl in [([3, -1], None), ([3], [1, 2]), ([1], [-2]), ([1 << 31], None)]:
         with pytest.raises(RuntimeError):
             attention.PromptPlan(ql, kl, device=DEV)
@@ -306,7 +307,7 @@ def test_decode_attention_refuses():
     for args in bad:
         with pytest.raises(RuntimeError):
             attention.decode_attention(*args)
-    for kw in ({"max_len": -1}, {"max_len": 10 ** 6}, {"scale": float("inf")}):
+    for kw in ({"max_len": -1}, {"max_len": 10 ** 6}, {"scale": float("inf")}, {"scale": 0.0}, {"scale": -1.0}):
         with pytest.raises(RuntimeError):
             attention.decode_attention(q, kp, vp, table, sl, **kw)
 
