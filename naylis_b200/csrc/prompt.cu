@@ -42,14 +42,22 @@ constexpr int kM = 128;                        // query rows of a half (TMEM lan
 constexpr int kN = 128;                        // keys of a tile
 constexpr int kThreads = 512;
 constexpr uint32_t kBox = 128 * 128;           // one TMA box: 128 rows x 64 bf16 columns
-constexpr uint32_t kTmemCols = 512;            // S of half A, S of half B, O of A, O of B
-constexpr uint32_t kSCol = 0, kOCol = 256;     // P (bf16 pairs) takes the first 64 columns of its S
+// Tensor memory: S of half A, S of half B, O of A, O of B and, at head_dim 64, P of A, P of
+// B (bf16 pairs, 64 columns each). At head_dim 128 the columns are full: P takes the first
+// 64 of its S.
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kSCol = 0, kOCol = 256, kPCol = 384;
 constexpr int kFix = 8;
 constexpr float kRescale = 8.0f;               // log2 growth of a row maximum that O is rescaled for
 
 template <int HD>
 struct Cfg {
     static constexpr int kBoxes = HD / 64;
+    static constexpr bool kOwnP = HD == 64;                   // P has columns of its own
+    // One pair of exponentials in 8 on the FMA pipe (tc::ex2_poly2) where the softmax waits for
+    // products: 16384 rows of 16 heads 944 us without, 919 with 1 in 8, 1060 with 2. At head_dim
+    // 64 the halves' softmaxes run side by side and none is best: 711, 787, 735 us.
+    static constexpr bool kPoly = HD == 128;
     static constexpr uint32_t kTile = kN * HD * 2;            // a K, V or Q tile
     static constexpr int kStages = HD == 64 ? 8 : 4;          // K and V tiles in turn
     static constexpr uint32_t kRing = kStages * kTile;
@@ -59,8 +67,8 @@ struct Cfg {
 };
 
 struct Bars {
-    uint64_t q_full[2], q_empty[2], kv_full[8], kv_empty[8], v_ready[8], s_full[2], p_full[2], o_full[2], o_free[2],
-        l_full[2], drain;
+    uint64_t q_full[2], q_empty[2], kv_full[8], kv_empty[8], v_ready[8], s_full[2], s_read[2], p_full[2],
+        pv_done[2], o_full[2], o_free[2], l_full[2], drain[2];
     uint32_t tmem_base;
     int abort;
     int fix[kFix];      // item whose values needed the slow path, in slot item % kFix
@@ -83,7 +91,6 @@ struct Half {
 struct Item {
     Half h[2];
     int k0, hk, n;
-    bool work;
     __device__ __forceinline__ int last() const {      // keys any row sees
         return max(h[0].rows > 0 ? h[0].vis + h[0].rows - 1 : 0, h[1].rows > 0 ? h[1].vis + h[1].rows - 1 : 0);
     }
@@ -92,38 +99,58 @@ struct Item {
     }
 };
 
-// Item of this CTA in round i: the costliest items come first in the list and the
-// CTAs take them in turn, every other round backwards, so their sums stay close.
-__device__ __forceinline__ int item_id(int i) {
-    const int g = static_cast<int>(gridDim.x), c = static_cast<int>(blockIdx.x);
-    return i * g + ((i & 1) ? g - 1 - c : c);
-}
+// The items of a CTA one after another, the next one's tile fetched ahead.
+struct Items {
+    const Params &p;
+    int rounds, i = -1, rem = 0, rem_next = 0;
+    bool have = false, have_next = false;
+    PromptTile next;
 
-__device__ __forceinline__ Item make_item(const Params &p, int id) {
-    Item it;
-    it.work = id < p.n_items;
-    if (!it.work) return it;
-    const PromptTile t = p.tiles[id / p.H];
-    const int rem = id % p.H;
-    it.k0 = t.k0;
-    if (p.pair) {
-        const int per = p.H / 2, sub = 1 - rem / per, hp = rem % per;
-        const int rows = min(max(t.rows - sub * kM, 0), kM);
-#pragma unroll
-        for (int a = 0; a < 2; ++a) it.h[a] = Half{t.q0 + sub * kM, rows, t.vis + sub * kM, 2 * hp + a, 0};
-    } else {
-#pragma unroll
-        for (int a = 0; a < 2; ++a)
-            it.h[a] = Half{t.q0 + a * kM, min(max(t.rows - a * kM, 0), kM), t.vis + a * kM, rem, 0};
+    __device__ __forceinline__ explicit Items(const Params &params) : p(params) {
+        rounds = (p.n_items + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+        fetch(0);
     }
+    __device__ __forceinline__ void fetch(int round) {
+        // the costliest items come first in the list and the CTAs take them in turn,
+        // every other round backwards, so that their sums stay close
+        const int g = static_cast<int>(gridDim.x), c = static_cast<int>(blockIdx.x);
+        const int id = round * g + ((round & 1) ? g - 1 - c : c);
+        have_next = round < rounds && id < p.n_items;
+        if (have_next) {
+            next = p.tiles[id / p.H];
+            rem_next = id % p.H;
+        }
+    }
+    // false: no more. An item without rows has it.h[0].rows == 0 and it.n == 0.
+    __device__ __forceinline__ bool get(Item &it) {
+        while (true) {
+            if (++i >= rounds) return false;
+            const PromptTile t = next;
+            const int rem = rem_next;
+            const bool have = have_next;
+            fetch(i + 1);
+            if (!have) continue;
+            it.k0 = t.k0;
+            if (p.pair) {
+                const int per = p.H / 2, sub = 1 - rem / per, hp = rem % per;
+                const int rows = min(max(t.rows - sub * kM, 0), kM);
+                if (rows == 0) continue;
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
-        it.h[a].n = it.h[a].rows > 0 ? max(0, (it.h[a].vis + it.h[a].rows - 1 + kN - 1) / kN) : 0;
-    it.hk = it.h[0].head / (p.H / p.Hk);
-    it.n = max(it.h[0].n, it.h[1].n);
-    it.work = it.h[0].rows > 0;
-    return it;
-}
+                for (int a = 0; a < 2; ++a) it.h[a] = Half{t.q0 + sub * kM, rows, t.vis + sub * kM, 2 * hp + a, 0};
+            } else {
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+                    it.h[a] = Half{t.q0 + a * kM, min(max(t.rows - a * kM, 0), kM), t.vis + a * kM, rem, 0};
+            }
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+                it.h[a].n = it.h[a].rows > 0 ? max(0, (it.h[a].vis + it.h[a].rows - 1 + kN - 1) / kN) : 0;
+            it.hk = it.h[0].head / (p.H / p.Hk);
+            it.n = max(it.h[0].n, it.h[1].n);
+            return true;
+        }
+    }
+};
 
 // The non-finite values that were taken out of an item's cut tiles, back into 32
 // columns of a row that sees `seen` keys: each makes its sum NaN or infinite.
@@ -160,13 +187,15 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
     Bars *bars = reinterpret_cast<Bars *>(sbase + 2 * C::kTile + C::kRing + C::kSum);
     volatile int *abort_flag = &bars->abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rounds = (P.n_items + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
 
     if (threadIdx.x == 0) {
         for (int a = 0; a < 2; ++a) {
+            tc::mbar_init(&bars->drain[a], 1);
             tc::mbar_init(&bars->q_full[a], 1);
             tc::mbar_init(&bars->q_empty[a], 1);
             tc::mbar_init(&bars->s_full[a], 1);
+            tc::mbar_init(&bars->s_read[a], kM);
+            tc::mbar_init(&bars->pv_done[a], 1);
             tc::mbar_init(&bars->p_full[a], kM);
             tc::mbar_init(&bars->o_full[a], 1);
             tc::mbar_init(&bars->o_free[a], kM);
@@ -174,10 +203,9 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
         }
         for (int s = 0; s < kStages; ++s) {
             tc::mbar_init(&bars->kv_full[s], 1);
-            tc::mbar_init(&bars->kv_empty[s], 1);
-            tc::mbar_init(&bars->v_ready[s], 2);
+            tc::mbar_init(&bars->kv_empty[s], 2);
+            tc::mbar_init(&bars->v_ready[s], 1);
         }
-        tc::mbar_init(&bars->drain, 1);
         bars->abort = 0;
         for (int i = 0; i < kFix; ++i) bars->fix[i] = -1;
     }
@@ -185,7 +213,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
         tc::tmem_alloc(&bars->tmem_base, kTmemCols);
         tc::tmem_relinquish();
     }
-    if (warp == 13 && lane == 0) {
+    if (warp == 14 && lane == 0) {
         tc::prefetch_tensormap(&tmap_q);
         tc::prefetch_tensormap(&tmap_k);
         tc::prefetch_tensormap(&tmap_v);
@@ -206,13 +234,22 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
         const uint32_t tS = tmem + kSCol + a * kN + lanes, tO = tmem + kOCol + a * HD + lanes;
         const uint64_t sc2 = tc::f2(P.scale_log2, P.scale_log2);
-        int phase = 0, par = 0;
+        const uint32_t tP = C::kOwnP ? tmem + kPCol + a * 64 + lanes : tS;
+        int phase = 0, par = 0, pv = 0;     // tiles begun, item parity, tiles whose product was waited for
         bool ok = true;
-        for (int i = 0; ok && i < rounds; ++i) {
-            const Item it = make_item(P, item_id(i));
-            if (!it.work) continue;
+        Items items(P);
+        for (Item it; ok && items.get(it);) {
             const Half h = it.h[a];
             float m = -INFINITY, l = 0.0f;
+            // wait for PV of the tile before the present one, once a tile
+            auto pv_done = [&] {
+                if (pv < phase - 1) {
+                    ok = wait(&bars->pv_done[a], (phase - 2) & 1);
+                    pv = phase - 1;
+                    if (ok) tc::tc_fence_after();
+                }
+                return ok;
+            };
             for (int j = 0; j < h.n; ++j) {
                 if (!(ok = wait(&bars->s_full[a], phase & 1))) break;
                 ++phase;
@@ -221,6 +258,10 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
 #pragma unroll
                 for (int c = 0; c < 4; ++c) tc::tmem_ld32(tS + 32 * c, v[c]);
                 tc::tmem_ld_wait();
+                if constexpr (C::kOwnP) {
+                    tc::tc_fence_before();
+                    tc::mbar_arrive(&bars->s_read[a]);
+                }
                 // keys of this tile that the row sees; warp-uniform test whether any row is cut
                 const int seen = h.vis + r - j * kN;
                 if (h.vis + quarter * 32 - j * kN < kN) {
@@ -248,7 +289,9 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                 if (j == 0) {
                     m = mn;
                 } else if (__any_sync(0xffffffffu, mn > m + kRescale)) {
-                    // S(j) was issued behind PV(j-1): O is complete here
+                    // O holds tiles 0 .. j-1 once PV(j-1) is done; with P in S's columns S(j) was
+                    // issued behind it
+                    if (C::kOwnP && !pv_done()) break;
                     const float mo = m == -INFINITY ? mn : m;
                     const float f = mn > m + kRescale ? (mn == INFINITY ? 1.0f : tc::ex2(mo - mn)) : 1.0f;
                     if (mn > m + kRescale) m = mn;
@@ -273,18 +316,20 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                     for (int e = 0; e < 32; ++e) {
                         const uint32_t *s = &v[2 * c + (e >> 4)][2 * (e & 15)];
                         const uint64_t x2 = tc::fma2(tc::f2_bits(s[0], s[1]), sc2, nm2);
-                        const uint64_t p2 = (e & 3) == 3 ? tc::ex2_poly2(x2) : tc::ex2_pair(x2);
+                        const uint64_t p2 = C::kPoly && (e & 7) == 3 ? tc::ex2_poly2(x2) : tc::ex2_pair(x2);
                         l2[e & 1] = tc::add2(l2[e & 1], p2);
                         const float2 p = tc::f2_split(p2);
                         pk[e] = pack_bf16x2(p.x, p.y);
                     }
-                    tc::tmem_st32(tS + 32 * c, pk);
+                    if (C::kOwnP && c == 0 && j > 0 && !pv_done()) break;   // P(j-1) is read
+                    tc::tmem_st32(tP + 32 * c, pk);
                 }
-                const float2 ls = tc::f2_split(tc::add2(l2[0], l2[1]));
-                l += ls.x + ls.y;
+                if (!ok) break;
                 tc::tmem_st_wait();
                 tc::tc_fence_before();
                 tc::mbar_arrive(&bars->p_full[a]);
+                const float2 ls = tc::f2_split(tc::add2(l2[0], l2[1]));
+                l += ls.x + ls.y;
             }
             if (!ok) break;
             if (h.n > 0) {
@@ -301,9 +346,8 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
         int phase[2] = {0, 0};
         bool ok = true;
-        for (int i = 0; ok && i < rounds; ++i) {
-            const Item it = make_item(P, item_id(i));
-            if (!it.work) continue;
+        Items items(P);
+        for (Item it; ok && items.get(it);) {
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
                 const Half h = it.h[a];
@@ -318,7 +362,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                 if (!(ok = wait(&bars->l_full[a], ph & 1) && wait(&bars->o_full[a], ph & 1))) break;
                 tc::tc_fence_after();
                 const float l = sSum[((ph & 1) * 2 + a) * kM + r];
-                const bool slow = *reinterpret_cast<volatile int *>(&bars->fix[i % kFix]) == i;
+                const bool slow = *reinterpret_cast<volatile int *>(&bars->fix[items.i % kFix]) == items.i;
                 const float inv = h.vis + r > 0 ? 1.0f / l : 0.0f;
                 const uint32_t tO = tmem + kOCol + a * HD + lanes;
                 const bool store = r < h.rows, none = h.vis + r <= 0;
@@ -346,95 +390,95 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
         }
     } else {
         tc::regs_dec<64>();
-        if (warp == 12) {
-            // -------------------------------------------------------- MMA issuer
-            // Per key tile: PV of A, S of A's next tile, PV of B, S of B's next tile. The
-            // tensor pipe keeps that order, so P may live in S's columns, and one half's
-            // softmax runs under the other half's products.
+        if (warp < 14) {
+            // -------------------------------------------------------- MMA issuers
+            // Warp 12: half A, 13: half B, each one thread. Where P lives in S's columns: per key
+            // tile PV, then S of the next tile (the tensor pipe keeps a thread's order); one half's
+            // softmax runs under the other half's products. Where P has its own: S of the next
+            // tile as soon as the softmax has read S, so that it never waits for products.
+            const int a = warp - 12;
             const uint32_t idesc_s = tc::idesc_bf16_f32(kM, kN, false, false);
             const uint32_t idesc_o = tc::idesc_bf16_f32(kM, HD, false, true);
-            int t = 0, qn[2] = {0, 0}, pn[2] = {0, 0}, on[2] = {0, 0};
-            bool ok = true;
-            auto issue_s = [&](int a, uint32_t sK, bool last) {
-                if (lane == 0) {
-                    const uint64_t ad = tc::smem_desc_sw128(base + a * C::kTile, 16, 1024);
-                    const uint64_t bd = tc::smem_desc_sw128(sK, 16, 1024);
+            const uint32_t tS = tc::uniform(tmem) + kSCol + a * kN, tO = tc::uniform(tmem) + kOCol + a * HD;
+            const uint32_t tP = C::kOwnP ? tc::uniform(tmem) + kPCol + a * 64 : tS;
+            const uint32_t sQ = tc::uniform(base) + a * C::kTile, sR = tc::uniform(ring);
+            if (tc::elect_one()) {
+                int t = 0, qn = 0, pn = 0, on = 0;
+                bool ok = true;
+                auto wait1 = [&](uint64_t *bar, uint32_t parity) {
+                    return tc::mbar_wait(bar, parity, P.err, 2, abort_flag);
+                };
+                auto full = [&](int u) { return wait1(&bars->kv_full[u % kStages], (u / kStages) & 1); };
+                auto release = [&](int u) { tc::mma_commit(&bars->kv_empty[u % kStages]); };
+                // a tile that this half has no use for: released once it is there, so that no two
+                // of a half's releases fall into one phase of the barrier
+                auto skip = [&](int u) {
+                    const bool there = full(u);
+                    if (there) tc::mbar_arrive(&bars->kv_empty[u % kStages]);
+                    return there;
+                };
+                auto issue_s = [&](int u, bool last) {
+                    const uint64_t ad = tc::smem_desc_sw128(sQ, 16, 1024);
+                    const uint64_t bd = tc::smem_desc_sw128(sR + (u % kStages) * C::kTile, 16, 1024);
 #pragma unroll
                     for (int kk = 0; kk < HD / 16; ++kk) {
                         const uint64_t step = 1024u * (kk >> 2) + 2u * (kk & 3);
-                        tc::mma_bf16_ss(tmem + kSCol + a * kN, ad + step, bd + step, idesc_s, kk > 0);
+                        tc::mma_bf16_ss(tS, ad + step, bd + step, idesc_s, kk > 0);
                     }
                     tc::mma_commit(&bars->s_full[a]);
+                    release(u);
                     if (last) tc::mma_commit(&bars->q_empty[a]);
-                }
-                __syncwarp();
-            };
-            auto issue_pv = [&](int a, uint32_t sV, bool first, bool last) {
-                if (lane == 0) {
-                    const uint64_t bv = tc::smem_desc_sw128(sV, kBox, 1024);
-#pragma unroll
-                    for (int kk = 0; kk < kN / 16; ++kk)
-                        tc::mma_bf16_ts(tmem + kOCol + a * HD, tmem + kSCol + a * kN + 8 * kk, bv + 128 * kk, idesc_o,
-                                        !first || kk > 0);
-                    if (last) tc::mma_commit(&bars->o_full[a]);
-                }
-                __syncwarp();
-            };
-            auto stage = [&](int u) { return ring + (u % kStages) * C::kTile; };
-            auto full = [&](int u) { return wait(&bars->kv_full[u % kStages], (u / kStages) & 1); };
-            auto release = [&](int u) {
-                if (lane == 0) tc::mma_commit(&bars->kv_empty[u % kStages]);
-                __syncwarp();
-            };
-            for (int i = 0; ok && i < rounds; ++i) {
-                const Item it = make_item(P, item_id(i));
-                if (!it.work || it.n == 0) continue;
-                ok = full(t);                              // K(0)
-#pragma unroll
-                for (int a = 0; a < 2; ++a)
-                    if (ok && it.h[a].n > 0) {
-                        ok = wait(&bars->q_full[a], qn[a]++ & 1);
+                };
+                Items items(P);
+                for (Item it; ok && items.get(it);) {
+                    if (it.n == 0) continue;
+                    const int n = it.h[a].n;
+                    if (n > 0) {
+                        ok = full(t) && wait1(&bars->q_full[a], qn++ & 1);
                         if (!ok) break;
                         tc::tc_fence_after();
-                        issue_s(a, stage(t), it.h[a].n == 1);
+                        issue_s(t, n == 1);
+                    } else if (!(ok = skip(t))) {
+                        break;
                     }
-                if (!ok) break;
-                release(t);
-                for (int j = 0; ok && j < it.n; ++j) {
-                    const int uv = t + 1, uk = t + 2;
-                    ok = full(uv) && wait(&bars->v_ready[uv % kStages], (uv / kStages) & 1);
-                    if (!ok) break;
-                    bool have_k = false;
-#pragma unroll
-                    for (int a = 0; a < 2; ++a) {
-                        const int n = it.h[a].n;
-                        if (j >= n) continue;
-                        ok = wait(&bars->p_full[a], pn[a]++ & 1);
-                        if (ok && j == 0) {
-                            ok = on[a] == 0 || wait(&bars->o_free[a], (on[a] - 1) & 1);
-                            ++on[a];
+                    for (int j = 0; j < it.n; ++j, t += 2) {
+                        const int uv = t + 1, uk = t + 2;
+                        if (j >= n) {      // the other half goes on alone
+                            if (!(ok = skip(uv) && (j + 1 >= it.n || skip(uk)))) break;
+                            continue;
                         }
+                        if (C::kOwnP && j + 1 < n) {      // S(j+1) as soon as S(j) is read
+                            if (!(ok = full(uk) && wait1(&bars->s_read[a], pn & 1))) break;
+                            tc::tc_fence_after();
+                            issue_s(uk, j + 2 == n);
+                        }
+                        ok = full(uv) && wait1(&bars->v_ready[uv % kStages], (uv / kStages) & 1) &&
+                             (C::kOwnP || j + 1 >= n || full(uk)) &&
+                             (j > 0 || on == 0 || wait1(&bars->o_free[a], (on - 1) & 1)) &&
+                             wait1(&bars->p_full[a], pn & 1);
                         if (!ok) break;
+                        ++pn;
+                        if (j == 0) ++on;
+                        const uint64_t bv = tc::smem_desc_sw128(sR + (uv % kStages) * C::kTile, kBox, 1024);
                         tc::tc_fence_after();
-                        issue_pv(a, stage(uv), j == 0, j + 1 == n);
+#pragma unroll
+                        for (int kk = 0; kk < kN / 16; ++kk)
+                            tc::mma_bf16_ts(tO, tP + 8 * kk, bv + 128 * kk, idesc_o, j > 0 || kk > 0);
+                        if (C::kOwnP) tc::mma_commit(&bars->pv_done[a]);
+                        release(uv);
+                        if (j + 1 == n) tc::mma_commit(&bars->o_full[a]);
                         if (j + 1 < n) {
-                            if (!have_k) {
-                                if (!(ok = full(uk))) break;
-                                have_k = true;
-                            }
-                            issue_s(a, stage(uk), j + 2 == n);
+                            if (!C::kOwnP) issue_s(uk, j + 2 == n);
+                        } else if (j + 1 < it.n && !(ok = skip(uk))) {
+                            break;
                         }
                     }
-                    if (!ok) break;
-                    release(uv);
-                    if (j + 1 < it.n) release(uk);
-                    t += 2;
                 }
+                tc::mma_commit(&bars->drain[a]);
+                wait1(&bars->drain[a], 0);
             }
-            if (lane == 0) tc::mma_commit(&bars->drain);
             __syncwarp();
-            wait(&bars->drain, 0);
-        } else if (warp == 13) {
+        } else if (warp == 14) {
             // -------------------------------------------------------- loader
             int t = 0, qn[2] = {0, 0};
             bool ok = true;
@@ -449,9 +493,9 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                 }
                 __syncwarp();
             };
-            for (int i = 0; ok && i < rounds; ++i) {
-                const Item it = make_item(P, item_id(i));
-                if (!it.work || it.n == 0) continue;
+            Items items(P);
+            for (Item it; ok && items.get(it);) {
+                if (it.n == 0) continue;
                 for (int j = 0; j < it.n; ++j) {
                     if (!(ok = slot(t))) break;
                     load_kv(&tmap_k, t, it.hk * HD, it.k0 + j * kN);
@@ -486,15 +530,14 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
         } else {
             // -------------------------------------------------------- hidden values
             // A weight of 0 does not hide a NaN or an infinity from a product. In the tiles
-            // that the mask cuts, these two warps zero such values (and every row behind the
+            // that the mask cuts, this warp zeroes such values (and every row behind the
             // last key anybody sees, another sequence's) before the product; the epilogue
             // gives the zeroed ones back to the rows that see them.
             int t = 0;
             bool ok = true;
-            const int w = warp - 14;
-            for (int i = 0; ok && i < rounds; ++i) {
-                const Item it = make_item(P, item_id(i));
-                if (!it.work || it.n == 0) continue;
+            Items items(P);
+            for (Item it; ok && items.get(it);) {
+                if (it.n == 0) continue;
                 const int first = it.first(), last = it.last();
                 for (int j = 0; j < it.n; ++j, t += 2) {
                     const int u = t + 1;
@@ -503,11 +546,11 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                         uint4 *tile = reinterpret_cast<uint4 *>(sbase + 2 * C::kTile + (u % kStages) * C::kTile);
                         const int cut = last - j * kN;      // rows of the tile that somebody sees
                         bool found = false;
-#pragma unroll 4
-                        for (int e = lane; e < C::kBoxes * 64 * 8; e += 32) {
-                            // box e / 512, row w * 64 + e / 8 % 64, any 16-byte chunk of it
-                            const int row = w * 64 + (e >> 3 & 63);
-                            uint4 *q = tile + (e >> 9) * (kBox / 16) + row * 8 + (e & 7);
+#pragma unroll 8
+                        for (int e = lane; e < C::kBoxes * kN * 8; e += 32) {
+                            // 16-byte chunk e: box e / 1024, row e / 8 % 128
+                            const int row = e >> 3 & (kN - 1);
+                            uint4 *q = tile + e;
                             uint4 x = *q;
                             if (row >= cut) {
                                 *q = make_uint4(0, 0, 0, 0);
@@ -526,7 +569,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                             }
                         }
                         if (__any_sync(0xffffffffu, found) && lane == 0)
-                            *reinterpret_cast<volatile int *>(&bars->fix[i % kFix]) = i;
+                            *reinterpret_cast<volatile int *>(&bars->fix[items.i % kFix]) = items.i;
                         tc::fence_proxy_async_smem();
                     }
                     __syncwarp();
