@@ -418,7 +418,7 @@ MOM_API int mom_prompt_plan_check(void *plan, void *stream);
 /* ------------------------------------------------------------------ scoring
  * Log probabilities of given tokens (no counterpart in the reference, which has
  * only the summed training loss): logits (R, V) F32 or BF16 of row pitch ld,
- * y = logits / temperature; targets (R) int64. logprob (R) = log_softmax(y)[t]
+ * y = logits / temperature (1e-6 to 1e6); targets (R) int64. logprob (R) = log_softmax(y)[t]
  * (0 where t == ignore_index, NaN where t is outside [0, V)), entropy (R) of
  * softmax(y), and the top_k (<= 32) greatest logits in order, ties to the lowest
  * index, NaN above all: top_idx (R, top_k) int64 and their top_logprob. All fp32.

@@ -1017,8 +1017,7 @@ int check_logprobs(int dtype, int64_t ld, int64_t R, int64_t V, double temperatu
     MOM_REQUIRE(is_float_dtype(dtype), "logits must be F32 or BF16");
     MOM_REQUIRE(R >= 0 && R < (int64_t(1) << 31) && V > 0 && V < (int64_t(1) << 31), "bad logits geometry");
     MOM_REQUIRE(ld >= V, "row pitch smaller than the vocabulary");
-    MOM_REQUIRE(std::isfinite(temperature) && temperature > 0.0 && std::isfinite(1.0f / (float)temperature),
-                "temperature must be positive");
+    MOM_REQUIRE(temperature >= 1e-6 && temperature <= 1e6, "temperature must be in [1e-6, 1e6] (got %g)", temperature);
     MOM_REQUIRE(top >= 0 && top <= mom::kMaxTopLogprobs && top <= V, "top_k must be in [0, min(%d, vocabulary)]",
                 mom::kMaxTopLogprobs);
     return MOM_OK;

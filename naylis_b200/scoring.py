@@ -94,8 +94,8 @@ def token_logprobs(logits, targets, *, top_k: int = 0, temperature: float = 1.0,
     top_k, temperature = int(top_k), float(temperature)
     if not 0 <= top_k <= min(MAX_TOP, logits.shape[1]):
         raise RuntimeError(f"token_logprobs: top_k {top_k} must be in [0, {min(MAX_TOP, logits.shape[1])}]")
-    if not 0.0 < temperature < float("inf"):
-        raise RuntimeError(f"token_logprobs: temperature {temperature} must be positive and finite")
+    if not 1e-6 <= temperature <= 1e6:
+        raise RuntimeError(f"token_logprobs: temperature {temperature} must be in [1e-6, 1e6]")
     if logits.shape[1] > 1 and logits.stride(1) != 1 or logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]:
         logits = logits.contiguous()
     targets = targets.to(torch.int64).contiguous()
