@@ -9,6 +9,8 @@ import ctypes
 import os
 import threading
 
+import torch
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libnaylis_mom.so")
 
@@ -143,3 +145,17 @@ def check(status: int, func: str) -> None:
 def call(name: str, *args) -> None:
     """Call a status-returning entry point and raise MomError on failure."""
     check(getattr(load(), name)(*args), name)
+
+
+def call_on(index: int, name: str, *args) -> None:
+    """call() on CUDA device `index` with that device's current stream as the last
+    argument: the short way for entry points whose call takes as long as their work
+    (the raw stream handle costs a tenth of a torch.cuda.Stream object)."""
+    lib = _lib or load()
+    if index == torch._C._cuda_getDevice():
+        status = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status != OK:
+        raise MomError(status, name, last_error())

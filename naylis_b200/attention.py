@@ -26,12 +26,12 @@ PAGE_SIZES = (8, 16, 32, 64, 128, 256)
 def _check(name, *ts):
     dev = ts[0].device
     for t in ts:
-        if not t.is_cuda or t.dtype != torch.bfloat16:
+        if t.dtype != torch.bfloat16 or not t.is_cuda:
             raise RuntimeError(f"{name} takes bf16 CUDA tensors, got {t.dtype} on {t.device}")
         if t.device != dev:
             raise RuntimeError(f"{name}: tensors on {dev} and {t.device}")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
-        raise RuntimeError(f"{name} is forward only: run it under torch.no_grad() or detach its inputs")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{name} is forward only: run it under torch.no_grad() or detach its inputs")
 
 
 def _rows(name, t, what):
@@ -40,12 +40,16 @@ def _rows(name, t, what):
     output), else a copy."""
     if t.dim() != 3:
         raise RuntimeError(f"{name}: {what} must be (tokens, heads, head_dim), got {tuple(t.shape)}")
-    hd = t.shape[2]
-    if (t.stride(2) == 1 and (t.stride(1) == hd or t.shape[1] == 1) and t.data_ptr() % 16 == 0
-            and (t.shape[0] <= 1 or (t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] * hd))):
-        return t, t.stride(0) if t.shape[0] > 1 else t.shape[1] * hd
+    T, H, hd = t.shape
+    if t.is_contiguous():
+        if t.data_ptr() % 16 == 0:
+            return t, H * hd
+        return t.clone(), H * hd
+    ld, sh, sd = t.stride()
+    if sd == 1 and (sh == hd or H == 1) and t.data_ptr() % 16 == 0 and (T <= 1 or (ld % 8 == 0 and ld >= H * hd)):
+        return t, ld if T > 1 else H * hd
     t = t.contiguous()
-    return (t if t.data_ptr() % 16 == 0 else t.clone()), t.shape[1] * hd
+    return (t if t.data_ptr() % 16 == 0 else t.clone()), H * hd
 
 
 def _pages(name, k_pages, v_pages):
@@ -70,15 +74,6 @@ def _heads(name, hd, H, Hk):
         raise RuntimeError(f"{name}: head_dim {hd} must be 64 or 128")
     if H <= 0 or Hk <= 0 or H % Hk:
         raise RuntimeError(f"{name}: {H} query heads are not a multiple of {Hk} key heads")
-
-
-def _call(dev, func, *args):
-    """The entry point on the tensors' device and that device's current stream."""
-    if dev.index == torch.cuda.current_device():
-        _lib.call(func, *args, torch.cuda.current_stream(dev).cuda_stream)
-    else:
-        with torch.cuda.device(dev):
-            _lib.call(func, *args, torch.cuda.current_stream(dev).cuda_stream)
 
 
 # ------------------------------------------------------------------ cache write
@@ -119,7 +114,7 @@ def rope_append(qkv, cos, sin, positions, k_pages, v_pages, slots, *, n_heads: i
         sin = sin.clone()
     q = torch.empty(T, H, hd, dtype=torch.bfloat16, device=dev)
     k = torch.empty(T, Hk, hd, dtype=torch.bfloat16, device=dev) if want_k else None
-    _call(dev, "mom_rope_append", qkv.data_ptr(), qkv.stride(0) if T > 1 else qkv.shape[1], cos.data_ptr(),
+    _lib.call_on(dev.index, "mom_rope_append", qkv.data_ptr(), qkv.stride(0) if T > 1 else qkv.shape[1], cos.data_ptr(),
           sin.data_ptr(), cos.shape[0], positions.data_ptr(), pcode, slots.data_ptr(), scode, T, H, Hk, hd, P, page,
           k_pages.data_ptr(), v_pages.data_ptr(), q.data_ptr(), None if k is None else k.data_ptr())
     return q, k
@@ -154,7 +149,7 @@ class PromptPlan:
 
     def check(self):
         """Raise if a kernel that used this plan gave up a wait (synchronises)."""
-        _call(self.device, "mom_prompt_plan_check", self.buffer.data_ptr())
+        _lib.call_on(self.device.index, "mom_prompt_plan_check", self.buffer.data_ptr())
 
 
 def prompt_attention(q, k, v, plan: PromptPlan, *, scale=None):
@@ -178,7 +173,7 @@ def prompt_attention(q, k, v, plan: PromptPlan, *, scale=None):
     if plan.device != q.device:
         raise RuntimeError(f"prompt_attention: the plan is on {plan.device}, q on {q.device}")
     out = torch.empty(Tq, H, hd, dtype=torch.bfloat16, device=q.device)
-    _call(q.device, "mom_prompt_attn", q.data_ptr(), q_ld, k.data_ptr(), k_ld, v.data_ptr(), v_ld, Tq, Tk, H, Hk, hd,
+    _lib.call_on(q.device.index, "mom_prompt_attn", q.data_ptr(), q_ld, k.data_ptr(), k_ld, v.data_ptr(), v_ld, Tq, Tk, H, Hk, hd,
           hd ** -0.5 if scale is None else float(scale), plan.buffer.data_ptr(), plan.buffer.numel(), out.data_ptr())
     return out
 
@@ -220,7 +215,7 @@ def decode_attention(q, k_pages, v_pages, block_table, seq_lens, *, scale=None, 
     out = torch.empty(B, H, hd, dtype=torch.bfloat16, device=dev)
     need = _lib.load().mom_decode_attn_workspace_size(B, H, Hk, hd, max_len)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _call(dev, "mom_decode_attn", q.data_ptr(), q_ld, k_pages.data_ptr(), v_pages.data_ptr(), P, page,
+    _lib.call_on(dev.index, "mom_decode_attn", q.data_ptr(), q_ld, k_pages.data_ptr(), v_pages.data_ptr(), P, page,
           block_table.data_ptr(), table_ld, seq_lens.data_ptr(), max_len, B, H, Hk, hd,
           hd ** -0.5 if scale is None else float(scale), out.data_ptr(), None if ws is None else ws.data_ptr(), need)
     return out

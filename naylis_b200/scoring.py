@@ -28,16 +28,15 @@ class TokenLogprobs(NamedTuple):
 def _forward(logits, targets, top_k, temperature, ignore_index, want_stats):
     R, V = logits.shape
     dev = logits.device
-    ld = logits.stride(0) if R > 1 else V
     logprob = torch.empty(R, dtype=torch.float32, device=dev)
     entropy = torch.empty(R, dtype=torch.float32, device=dev)
     top_lp = torch.empty(R, top_k, dtype=torch.float32, device=dev) if top_k else None
     top_idx = torch.empty(R, top_k, dtype=torch.int64, device=dev) if top_k else None
     stats = torch.empty(R, 4, dtype=torch.float32, device=dev) if want_stats else None
-    _lib.call("mom_logprobs_fwd", logits.data_ptr(), _code(logits), ld, targets.data_ptr(), R, V, ignore_index,
-              temperature, top_k, logprob.data_ptr(), entropy.data_ptr(), None if top_lp is None else top_lp.data_ptr(),
-              None if top_idx is None else top_idx.data_ptr(), None if stats is None else stats.data_ptr(),
-              torch.cuda.current_stream(dev).cuda_stream)
+    _lib.call_on(dev.index, "mom_logprobs_fwd", logits.data_ptr(), _code(logits), logits.stride(0) if R > 1 else V,
+                 targets.data_ptr(), R, V, ignore_index, temperature, top_k, logprob.data_ptr(), entropy.data_ptr(),
+                 top_lp.data_ptr() if top_k else None, top_idx.data_ptr() if top_k else None,
+                 stats.data_ptr() if want_stats else None)
     return logprob, entropy, top_lp, top_idx, stats
 
 
@@ -58,21 +57,20 @@ class _TokenLogprobs(torch.autograd.Function):
         return logprob, entropy
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g_logprob, g_entropy, g_top=None, _g_idx=None):
+        if torch.is_grad_enabled():
+            raise RuntimeError("token_logprobs: its gradient has no gradient (create_graph=True)")
         logits, targets, stats, top_idx = ctx.saved_tensors
         top_k, temperature, ignore_index = ctx.meta
         R, V = logits.shape
-        dev = logits.device
         if g_logprob is None and g_entropy is None and g_top is None:
             return None, None, None, None, None
         g = [None if t is None else t.to(torch.float32).contiguous() for t in (g_logprob, g_entropy, g_top)]
-        dlogits = torch.empty(R, V, dtype=logits.dtype, device=dev)
-        with torch.cuda.device(dev):
-            _lib.call("mom_logprobs_bwd", logits.data_ptr(), _code(logits), logits.stride(0) if R > 1 else V,
-                      targets.data_ptr(), stats.data_ptr(), None if top_idx is None else top_idx.data_ptr(), top_k,
-                      *(None if t is None else t.data_ptr() for t in g), R, V, ignore_index, temperature,
-                      dlogits.data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
+        dlogits = torch.empty(R, V, dtype=logits.dtype, device=logits.device)
+        _lib.call_on(logits.device.index, "mom_logprobs_bwd", logits.data_ptr(), _code(logits),
+                     logits.stride(0) if R > 1 else V, targets.data_ptr(), stats.data_ptr(),
+                     top_idx.data_ptr() if top_k else None, top_k, *(None if t is None else t.data_ptr() for t in g), R,
+                     V, ignore_index, temperature, dlogits.data_ptr())
         return dlogits, None, None, None, None
 
 
@@ -87,32 +85,25 @@ def token_logprobs(logits, targets, *, top_k: int = 0, temperature: float = 1.0,
     Differentiable in logprob, entropy and top_logprob. Returns TokenLogprobs."""
     if not logits.is_cuda or logits.dtype not in (torch.bfloat16, torch.float32):
         raise RuntimeError(f"token_logprobs takes bf16 or fp32 CUDA logits, got {logits.dtype} on {logits.device}")
-    if logits.dim() != 2 or logits.shape[1] == 0 or targets.shape != logits.shape[:1] or \
-            targets.device != logits.device or targets.dtype.is_floating_point:
+    shape = logits.shape
+    if len(shape) != 2 or shape[1] == 0 or targets.shape != shape[:1] or targets.device != logits.device or \
+            targets.dtype.is_floating_point:
         raise RuntimeError(f"token_logprobs: logits (R, V) and integer targets (R,) on one device, got "
-                           f"{tuple(logits.shape)} and {tuple(targets.shape)} {targets.dtype}")
+                           f"{tuple(shape)} and {tuple(targets.shape)} {targets.dtype}")
+    R, V = shape
     top_k, temperature = int(top_k), float(temperature)
-    if not 0 <= top_k <= min(MAX_TOP, logits.shape[1]):
-        raise RuntimeError(f"token_logprobs: top_k {top_k} must be in [0, {min(MAX_TOP, logits.shape[1])}]")
+    if not 0 <= top_k <= min(MAX_TOP, V):
+        raise RuntimeError(f"token_logprobs: top_k {top_k} must be in [0, {min(MAX_TOP, V)}]")
     if not 1e-6 <= temperature <= 1e6:
         raise RuntimeError(f"token_logprobs: temperature {temperature} must be in [1e-6, 1e6]")
-    if logits.shape[1] > 1 and logits.stride(1) != 1 or logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]:
+    if not logits.is_contiguous() and (V > 1 and logits.stride(1) != 1 or R > 1 and logits.stride(0) < V):
         logits = logits.contiguous()
-    targets = targets.to(torch.int64).contiguous()
-    args = (logits, targets, top_k, temperature, int(ignore_index))
-    if logits.device.index != torch.cuda.current_device():
-        with torch.cuda.device(logits.device):
-            return _apply(args)
-    return _apply(args)
-
-
-def _apply(args):
-    if torch.is_grad_enabled() and args[0].requires_grad:
-        out = _TokenLogprobs.apply(*args)
-        logprob, entropy = out[0], out[1]
-        top_lp, top_idx = (out[2], out[3]) if len(out) == 4 else (None, None)
-    else:
-        logprob, entropy, top_lp, top_idx, _ = _forward(*args, False)
+    if targets.dtype != torch.int64 or not targets.is_contiguous():
+        targets = targets.to(torch.int64).contiguous()
+    if logits.requires_grad and torch.is_grad_enabled():
+        out = _TokenLogprobs.apply(logits, targets, top_k, temperature, int(ignore_index))
+        return TokenLogprobs(out[0], out[1], *((out[3], out[2]) if top_k else (None, None)))
+    logprob, entropy, top_lp, top_idx, _ = _forward(logits, targets, top_k, temperature, int(ignore_index), False)
     return TokenLogprobs(logprob, entropy, top_idx, top_lp)
 
 
