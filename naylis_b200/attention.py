@@ -221,4 +221,85 @@ def decode_attention(q, k_pages, v_pages, block_table, seq_lens, *, scale=None, 
     return out
 
 
-__all__ = ["PAGE_SIZES", "PromptPlan", "rope_append", "prompt_attention", "decode_attention"]
+# ------------------------------------------------------------------ cache
+class PagedKVCache:
+    """The pages of every layer and the sequences that own them.
+
+    k, v: (n_layers, num_pages, n_kv_heads, page_size, head_dim) bf16; a sequence's
+    pages are the same in every layer. The book-keeping is on the host: add() a
+    sequence, extend() sequences by their new tokens (which says where those go),
+    free() one when it is done."""
+
+    def __init__(self, n_layers: int, num_pages: int, page_size: int, n_kv_heads: int, head_dim: int, *,
+                 device="cuda"):
+        if page_size not in PAGE_SIZES:
+            raise RuntimeError(f"PagedKVCache: page_size {page_size} must be one of {PAGE_SIZES}")
+        _heads("PagedKVCache", head_dim, n_kv_heads, n_kv_heads)
+        if n_layers <= 0 or num_pages < 0:
+            raise RuntimeError(f"PagedKVCache: {n_layers} layers of {num_pages} pages")
+        shape = (n_layers, num_pages, n_kv_heads, page_size, head_dim)
+        self.k = torch.empty(shape, dtype=torch.bfloat16, device=device)
+        self.v = torch.empty(shape, dtype=torch.bfloat16, device=device)
+        self.page_size, self.num_pages = page_size, num_pages
+        self._free = list(range(num_pages - 1, -1, -1))
+        self._pages, self._len, self._next = {}, {}, 0
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def length(self, seq: int) -> int:
+        return self._len[seq]
+
+    def add(self) -> int:
+        """A new sequence without tokens."""
+        seq, self._next = self._next, self._next + 1
+        self._pages[seq], self._len[seq] = [], 0
+        return seq
+
+    def free(self, seq: int) -> None:
+        """Give a sequence's pages back."""
+        self._free.extend(reversed(self._pages.pop(seq)))
+        del self._len[seq]
+
+    def extend(self, seqs, counts):
+        """Room for counts[i] more tokens of seqs[i] (each named once). Returns
+        (positions, slots) of the new tokens, packed in that order, int64 on the
+        device: rope_append's arguments. Raises, changing nothing, when the pages do
+        not reach."""
+        seqs, counts = list(seqs), [int(c) for c in counts]
+        if len(seqs) != len(counts) or len(set(seqs)) != len(seqs) or any(c < 0 for c in counts):
+            raise RuntimeError("PagedKVCache.extend: one count >= 0 for each sequence, each named once")
+        page = self.page_size
+        need = [-(-(self._len[s] + c) // page) - len(self._pages[s]) for s, c in zip(seqs, counts)]
+        if sum(need) > len(self._free):
+            raise RuntimeError(f"PagedKVCache: {sum(need)} pages needed, {len(self._free)} of {self.num_pages} free")
+        pos, slots = [], []
+        for s, c, n in zip(seqs, counts, need):
+            pages = self._pages[s]
+            pages.extend(self._free.pop() for _ in range(n))
+            at = np.arange(self._len[s], self._len[s] + c, dtype=np.int64)
+            pos.append(at)
+            slots.append(np.asarray(pages, dtype=np.int64)[at // page] * page + at % page if c else at)
+            self._len[s] += c
+        if not pos:
+            both = np.zeros((2, 0), dtype=np.int64)
+        else:
+            both = np.stack([np.concatenate(pos), np.concatenate(slots)])
+        both = torch.from_numpy(both).to(self.k.device)
+        return both[0], both[1]
+
+    def tables(self, seqs):
+        """(block_table (B, n), seq_lens (B)) int32 on the device, and the longest
+        length: decode_attention's arguments."""
+        seqs = list(seqs)
+        most = max((len(self._pages[s]) for s in seqs), default=0)
+        table = np.zeros((len(seqs), most + 1), dtype=np.int32)
+        for i, s in enumerate(seqs):
+            table[i, 0] = self._len[s]
+            table[i, 1:1 + len(self._pages[s])] = self._pages[s]
+        both = torch.from_numpy(table).to(self.k.device)
+        return both[:, 1:], both[:, 0].contiguous(), max((self._len[s] for s in seqs), default=0)
+
+
+__all__ = ["PAGE_SIZES", "PagedKVCache", "PromptPlan", "rope_append", "prompt_attention", "decode_attention"]
