@@ -68,7 +68,7 @@ struct Cfg {
 
 struct Bars {
     uint64_t q_full[2], q_empty[2], kv_full[8], kv_empty[8], v_ready[8], s_full[2], s_read[2], p_full[2],
-        pv_done[2], o_full[2], o_free[2], l_full[2], drain[2];
+        pv_done[2], o_full[2], o_free[2], l_full[2][2], drain[2];
     uint32_t tmem_base;
     int abort;
     int fix[kFix];      // item whose values needed the slow path, in slot item % kFix
@@ -199,7 +199,8 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
             tc::mbar_init(&bars->p_full[a], kM);
             tc::mbar_init(&bars->o_full[a], 1);
             tc::mbar_init(&bars->o_free[a], kM);
-            tc::mbar_init(&bars->l_full[a], kM);
+            tc::mbar_init(&bars->l_full[a][0], kM);
+            tc::mbar_init(&bars->l_full[a][1], kM);
         }
         for (int s = 0; s < kStages; ++s) {
             tc::mbar_init(&bars->kv_full[s], 1);
@@ -321,7 +322,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                         const float2 p = tc::f2_split(p2);
                         pk[e] = pack_bf16x2(p.x, p.y);
                     }
-                    if (C::kOwnP && c == 0 && j > 0 && !pv_done()) break;   // P(j-1) is read
+                    if (C::kOwnP && c == 0 && phase > 1 && !pv_done()) break;   // the last P is read
                     tc::tmem_st32(tP + 32 * c, pk);
                 }
                 if (!ok) break;
@@ -334,7 +335,9 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
             if (!ok) break;
             if (h.n > 0) {
                 sSum[(par * 2 + a) * kM + r] = l;
-                tc::mbar_arrive(&bars->l_full[a]);
+                // one barrier per item parity: a half may finish its next item before the epilogue
+                // comes to this one, but not the one after
+                tc::mbar_arrive(&bars->l_full[a][par]);
                 par ^= 1;
             }
         }
@@ -359,7 +362,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                     continue;
                 }
                 const int ph = phase[a]++;
-                if (!(ok = wait(&bars->l_full[a], ph & 1) && wait(&bars->o_full[a], ph & 1))) break;
+                if (!(ok = wait(&bars->l_full[a][ph & 1], (ph >> 1) & 1) && wait(&bars->o_full[a], ph & 1))) break;
                 tc::tc_fence_after();
                 const float l = sSum[((ph & 1) * 2 + a) * kM + r];
                 const bool slow = *reinterpret_cast<volatile int *>(&bars->fix[items.i % kFix]) == items.i;
@@ -403,7 +406,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
             const uint32_t tP = C::kOwnP ? tc::uniform(tmem) + kPCol + a * 64 : tS;
             const uint32_t sQ = tc::uniform(base) + a * C::kTile, sR = tc::uniform(ring);
             if (tc::elect_one()) {
-                int t = 0, qn = 0, pn = 0, on = 0;
+                int qn = 0, pn = 0, on = 0;      // items begun, tiles, items with a product
                 bool ok = true;
                 auto wait1 = [&](uint64_t *bar, uint32_t parity) {
                     return tc::mbar_wait(bar, parity, P.err, 2, abort_flag);
@@ -429,50 +432,76 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                     release(u);
                     if (last) tc::mma_commit(&bars->q_empty[a]);
                 };
-                Items items(P);
-                for (Item it; ok && items.get(it);) {
-                    if (it.n == 0) continue;
-                    const int n = it.h[a].n;
-                    if (n > 0) {
-                        ok = full(t) && wait1(&bars->q_full[a], qn++ & 1);
-                        if (!ok) break;
-                        tc::tc_fence_after();
-                        issue_s(t, n == 1);
-                    } else if (!(ok = skip(t))) {
-                        break;
+                // the half's key tiles one after another, items and all: tile j of its item, whose
+                // K is the loader's tile t
+                struct Cursor {
+                    Items items;
+                    Item it;
+                    int a, j = 0, t = -2;
+                    bool live = true, in = false;
+                    __device__ __forceinline__ Cursor(const Params &p, int half) : items(p), a(half) {}
+                    __device__ __forceinline__ void next() {
+                        int step = 2;      // loader tiles passed
+                        if (in) {
+                            if (++j < it.h[a].n) {
+                                t += 2;
+                                return;
+                            }
+                            step += 2 * (it.n - j);
+                        }
+                        while ((live = items.get(it))) {
+                            if (it.h[a].n > 0) break;
+                            step += 2 * it.n;
+                        }
+                        in = true;
+                        j = 0;
+                        t += step;
                     }
-                    for (int j = 0; j < it.n; ++j, t += 2) {
-                        const int uv = t + 1, uk = t + 2;
-                        if (j >= n) {      // the other half goes on alone
-                            if (!(ok = skip(uv) && (j + 1 >= it.n || skip(uk)))) break;
-                            continue;
-                        }
-                        if (C::kOwnP && j + 1 < n) {      // S(j+1) as soon as S(j) is read
-                            if (!(ok = full(uk) && wait1(&bars->s_read[a], pn & 1))) break;
-                            tc::tc_fence_after();
-                            issue_s(uk, j + 2 == n);
-                        }
-                        ok = full(uv) && wait1(&bars->v_ready[uv % kStages], (uv / kStages) & 1) &&
-                             (C::kOwnP || j + 1 >= n || full(uk)) &&
-                             (j > 0 || on == 0 || wait1(&bars->o_free[a], (on - 1) & 1)) &&
-                             wait1(&bars->p_full[a], pn & 1);
-                        if (!ok) break;
-                        ++pn;
-                        if (j == 0) ++on;
-                        const uint64_t bv = tc::smem_desc_sw128(sR + (uv % kStages) * C::kTile, kBox, 1024);
+                    __device__ __forceinline__ bool last() const { return j + 1 == it.h[a].n; }
+                };
+                Cursor cs(P, a), cp(P, a);      // scores, products with V
+                auto scores = [&](bool behind) {
+                    ok = full(cs.t) && (cs.j > 0 || wait1(&bars->q_full[a], qn++ & 1)) &&
+                         (!behind || !C::kOwnP || wait1(&bars->s_read[a], (pn - 1) & 1));
+                    if (ok) {
                         tc::tc_fence_after();
+                        issue_s(cs.t, cs.last());
+                    }
+                };
+                int passed = 0;      // loader tiles up to here are used or released
+                auto pass_to = [&](int u) {
+                    while (ok && passed < u) ok = skip(passed++);
+                };
+                cs.next();
+                cp.next();
+                pass_to(cs.t);
+                if (ok && cs.live) scores(false);
+                while (ok && cp.live) {
+                    cs.next();
+                    ++pn;
+                    // S of the next tile ahead of the product where the softmax's columns allow it
+                    // and the ring reaches: its tile may be at most one that the half skips away
+                    const bool lead = C::kOwnP && cs.live && cs.t - cp.t <= 4;
+                    if (lead) scores(true);
+                    const int uv = cp.t + 1;
+                    ok = ok && full(uv) && wait1(&bars->v_ready[uv % kStages], (uv / kStages) & 1) &&
+                         (lead || !cs.live || cs.t != cp.t + 2 || full(cs.t)) &&
+                         (cp.j > 0 || on == 0 || wait1(&bars->o_free[a], (on - 1) & 1)) &&
+                         wait1(&bars->p_full[a], (pn - 1) & 1);
+                    if (!ok) break;
+                    if (cp.j == 0) ++on;
+                    const uint64_t bv = tc::smem_desc_sw128(sR + (uv % kStages) * C::kTile, kBox, 1024);
+                    tc::tc_fence_after();
 #pragma unroll
-                        for (int kk = 0; kk < kN / 16; ++kk)
-                            tc::mma_bf16_ts(tO, tP + 8 * kk, bv + 128 * kk, idesc_o, j > 0 || kk > 0);
-                        if (C::kOwnP) tc::mma_commit(&bars->pv_done[a]);
-                        release(uv);
-                        if (j + 1 == n) tc::mma_commit(&bars->o_full[a]);
-                        if (j + 1 < n) {
-                            if (!C::kOwnP) issue_s(uk, j + 2 == n);
-                        } else if (j + 1 < it.n && !(ok = skip(uk))) {
-                            break;
-                        }
-                    }
+                    for (int kk = 0; kk < kN / 16; ++kk)
+                        tc::mma_bf16_ts(tO, tP + 8 * kk, bv + 128 * kk, idesc_o, cp.j > 0 || kk > 0);
+                    if (C::kOwnP) tc::mma_commit(&bars->pv_done[a]);
+                    release(uv);
+                    if (cp.last()) tc::mma_commit(&bars->o_full[a]);
+                    passed = cp.t + 2;
+                    pass_to(cs.t);
+                    if (ok && !lead && cs.live) scores(true);
+                    cp.next();
                 }
                 tc::mma_commit(&bars->drain[a]);
                 wait1(&bars->drain[a], 0);

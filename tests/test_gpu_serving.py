@@ -147,6 +147,32 @@ def test_prompt_attention_wide_scores(hd):
     _close(out, *_prompt_exact(q, k, v, [n], [n], 1.0))
 
 
+@pytest.mark.parametrize("hd,H,Hk", [(64, 4, 4), (64, 4, 2), (128, 4, 1), (128, 3, 3)])
+@pytest.mark.parametrize("n,seqs,past", [(100, 400, 0), (300, 120, 0), (129, 250, 0), (40, 500, 90), (700, 40, 0)])
+def test_prompt_attention_many_tiles(hd, H, Hk, n, seqs, past):
+    """Several work items for every CTA, down to single key tiles: equal sequences,
+    compared as one batch."""
+    from naylis_b200 import attention
+    m = n + past
+    q = _rand(90, seqs * n, H, hd, scale=2.0)
+    k, v = _rand(91, seqs * m, Hk, hd), _rand(92, seqs * m, Hk, hd)
+    plan = attention.PromptPlan([n] * seqs, [m] * seqs, device=DEV)
+    out = attention.prompt_attention(q, k, v, plan)
+    for _ in range(3):
+        assert torch.equal(out, attention.prompt_attention(q, k, v, plan))
+    plan.check()
+    seen = torch.ones(n, m, dtype=torch.bool, device=DEV).tril(past)
+    for b in range(0, seqs, 50):
+        e = min(seqs, b + 50)
+        qb = q[b * n:e * n].double().view(e - b, n, H, hd).transpose(1, 2)
+        kb, vb = (t[b * m:e * m].double().view(e - b, m, Hk, hd).transpose(1, 2).repeat_interleave(H // Hk, 1)
+                  for t in (k, v))
+        s = (qb @ kb.transpose(2, 3) * hd ** -0.5).masked_fill(~seen, float("-inf"))
+        p = torch.softmax(s, -1)
+        flat = lambda t: t.transpose(1, 2).reshape(-1, H, hd)
+        _close(out[b * n:e * n], flat(p @ vb), flat(p @ vb.abs()))
+
+
 def test_prompt_attention_refuses():
     from naylis_b200 import attention
     plan = attention.PromptPlan([4, 5], device=DEV)
