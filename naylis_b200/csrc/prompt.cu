@@ -62,7 +62,8 @@ struct Cfg {
     static constexpr int kStages = HD == 64 ? 8 : 4;          // K and V tiles in turn
     static constexpr uint32_t kRing = kStages * kTile;
     static constexpr uint32_t kSum = 2 * 2 * kM * 4;          // row sums [item parity][half][row]
-    static constexpr uint32_t kSmem = 2 * kTile + kRing + kSum + 1024 /*barriers*/ + 1024 /*align*/;
+    static constexpr uint32_t kStage = kM * 128;              // 64 output columns of a half
+    static constexpr uint32_t kSmem = 2 * kTile + kRing + kStage + kSum + 1024 /*barriers*/ + 1024 /*align*/;
     static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
@@ -90,7 +91,7 @@ struct Half {
 };
 struct Item {
     Half h[2];
-    int k0, hk, n;
+    int k0, n;
     __device__ __forceinline__ int last() const {      // keys any row sees
         return max(h[0].rows > 0 ? h[0].vis + h[0].rows - 1 : 0, h[1].rows > 0 ? h[1].vis + h[1].rows - 1 : 0);
     }
@@ -99,58 +100,59 @@ struct Item {
     }
 };
 
-// The items of a CTA one after another, the next one's tile fetched ahead.
+// The items of a CTA one after another, the next one's tile fetched ahead. The
+// costliest items come first in the list and the CTAs take them in turn, every other
+// round backwards, so that their sums stay close: item id = round * grid + cta, or
+// + grid - 1 - cta; tile id / H and id % H are carried from step to step.
 struct Items {
     const Params &p;
-    int rounds, i = -1, rem = 0, rem_next = 0;
-    bool have = false, have_next = false;
+    int i = -1;
+    int rounds, tile, rem, rem_next, q0, r0, q1, r1;
+    bool have_next;
     PromptTile next;
 
     __device__ __forceinline__ explicit Items(const Params &params) : p(params) {
-        rounds = (p.n_items + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
-        fetch(0);
-    }
-    __device__ __forceinline__ void fetch(int round) {
-        // the costliest items come first in the list and the CTAs take them in turn,
-        // every other round backwards, so that their sums stay close
         const int g = static_cast<int>(gridDim.x), c = static_cast<int>(blockIdx.x);
-        const int id = round * g + ((round & 1) ? g - 1 - c : c);
-        have_next = round < rounds && id < p.n_items;
-        if (have_next) {
-            next = p.tiles[id / p.H];
-            rem_next = id % p.H;
-        }
+        rounds = (p.n_items + g - 1) / g;
+        const int d0 = 2 * (g - c) - 1, d1 = 2 * c + 1;      // from an even round, from an odd one
+        q0 = d0 / p.H, r0 = d0 % p.H, q1 = d1 / p.H, r1 = d1 % p.H;
+        tile = c / p.H;
+        rem = c % p.H;
+        fetch();
     }
-    // false: no more. An item without rows has it.h[0].rows == 0 and it.n == 0.
-    __device__ __forceinline__ bool get(Item &it) {
+    __device__ __forceinline__ void fetch() {
+        have_next = tile < p.n_items / p.H;
+        rem_next = rem;
+        if (have_next) next = p.tiles[tile];
+    }
+    __device__ __forceinline__ bool get(Item &it) {      // false: no more
         while (true) {
             if (++i >= rounds) return false;
             const PromptTile t = next;
-            const int rem = rem_next;
+            const int now = rem_next;
             const bool have = have_next;
-            fetch(i + 1);
+            tile += (i & 1) ? q1 : q0;
+            rem += (i & 1) ? r1 : r0;
+            if (rem >= p.H) rem -= p.H, ++tile;
+            fetch();
             if (!have) continue;
             it.k0 = t.k0;
-            if (p.pair) {
-                const int per = p.H / 2, sub = 1 - rem / per, hp = rem % per;
-                const int rows = min(max(t.rows - sub * kM, 0), kM);
-                if (rows == 0) continue;
+            const int sub = p.pair && now < p.H / 2 ? 1 : 0;          // pairs: the later rows first
+            const int hp = p.pair && !sub ? now - p.H / 2 : now;
+            const int rows = t.rows - sub * kM;
+            if (rows <= 0) continue;
 #pragma unroll
-                for (int a = 0; a < 2; ++a) it.h[a] = Half{t.q0 + sub * kM, rows, t.vis + sub * kM, 2 * hp + a, 0};
-            } else {
-#pragma unroll
-                for (int a = 0; a < 2; ++a)
-                    it.h[a] = Half{t.q0 + a * kM, min(max(t.rows - a * kM, 0), kM), t.vis + a * kM, rem, 0};
+            for (int a = 0; a < 2; ++a) {
+                const int at = p.pair ? sub * kM : a * kM, left = p.pair ? rows : rows - a * kM;
+                it.h[a] = Half{t.q0 + at, min(max(left, 0), kM), t.vis + at, p.pair ? 2 * hp + a : now, 0};
+                it.h[a].n = left > 0 ? max(0, (it.h[a].vis + it.h[a].rows + kN - 2) >> 7) : 0;
             }
-#pragma unroll
-            for (int a = 0; a < 2; ++a)
-                it.h[a].n = it.h[a].rows > 0 ? max(0, (it.h[a].vis + it.h[a].rows - 1 + kN - 1) / kN) : 0;
-            it.hk = it.h[0].head / (p.H / p.Hk);
             it.n = max(it.h[0].n, it.h[1].n);
             return true;
         }
     }
 };
+static_assert(kN == 128, "key tiles are counted by a shift");
 
 // The non-finite values that were taken out of an item's cut tiles, back into 32
 // columns of a row that sees `seen` keys: each makes its sum NaN or infinite.
@@ -166,7 +168,7 @@ __device__ __forceinline__ void add_hidden(const Params &P, const Item &it, int 
 #pragma unroll
     for (int e = 0; e < 32; ++e) f[e] = 0.0f;
     const int hd = P.hd;
-    add_hidden_at(P.v + static_cast<int64_t>(it.k0) * P.v_ld + it.hk * hd + 32 * c, P.v_ld,
+    add_hidden_at(P.v + static_cast<int64_t>(it.k0) * P.v_ld + it.h[0].head / (P.H / P.Hk) * hd + 32 * c, P.v_ld,
                   max(it.first(), 0) / kN * kN, seen, f);
 #pragma unroll
     for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) + f[e]);
@@ -183,8 +185,8 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
     const uint32_t base = (raw + 1023u) & ~1023u;
     unsigned char *sbase = smem_raw + (base - raw);
     const uint32_t ring = base + 2 * C::kTile;
-    float *sSum = reinterpret_cast<float *>(sbase + 2 * C::kTile + C::kRing);
-    Bars *bars = reinterpret_cast<Bars *>(sbase + 2 * C::kTile + C::kRing + C::kSum);
+    float *sSum = reinterpret_cast<float *>(sbase + 2 * C::kTile + C::kRing + C::kStage);
+    Bars *bars = reinterpret_cast<Bars *>(sbase + 2 * C::kTile + C::kRing + C::kStage + C::kSum);
     volatile int *abort_flag = &bars->abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -267,10 +269,13 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                 const int seen = h.vis + r - j * kN;
                 if (h.vis + quarter * 32 - j * kN < kN) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                    for (int c = 0; c < 4; ++c) {
+                        const int left = min(max(seen - 32 * c, 0), 32);
+                        const uint32_t keep = left == 32 ? 0xffffffffu : (1u << left) - 1u;
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
-                            if (32 * c + e >= seen) v[c][e] = __float_as_uint(-INFINITY);
+                            v[c][e] = keep >> e & 1u ? v[c][e] : __float_as_uint(-INFINITY);
+                    }
                 }
                 float mx[4];
 #pragma unroll
@@ -347,6 +352,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
         tc::regs_dec<80>();
         const int quarter = warp & 3, r = quarter * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+        uint4 *stage = reinterpret_cast<uint4 *>(sbase + 2 * C::kTile + C::kRing) + quarter * 32 * 8;
         int phase[2] = {0, 0};
         bool ok = true;
         Items items(P);
@@ -354,11 +360,11 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
                 const Half h = it.h[a];
-                uint16_t *dst = P.out + (static_cast<int64_t>(h.q0 + r) * P.H + h.head) * HD;
                 if (h.n == 0) {
+                    uint4 *dst = reinterpret_cast<uint4 *>(P.out + (static_cast<int64_t>(h.q0 + r) * P.H + h.head) * HD);
                     if (r < h.rows)
 #pragma unroll
-                        for (int c = 0; c < HD / 8; ++c) reinterpret_cast<uint4 *>(dst)[c] = make_uint4(0, 0, 0, 0);
+                        for (int c = 0; c < HD / 8; ++c) dst[c] = make_uint4(0, 0, 0, 0);
                     continue;
                 }
                 const int ph = phase[a]++;
@@ -368,27 +374,43 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                 const bool slow = *reinterpret_cast<volatile int *>(&bars->fix[items.i % kFix]) == items.i;
                 const float inv = h.vis + r > 0 ? 1.0f / l : 0.0f;
                 const uint32_t tO = tmem + kOCol + a * HD + lanes;
-                const bool store = r < h.rows, none = h.vis + r <= 0;
+                const bool none = h.vis + r <= 0;
+                // 64 columns at a time to the warp's rows in shared memory (16-byte chunks swizzled
+                // by row), from there to global in whole 128-byte runs; O is free once it is read
 #pragma unroll
-                for (int c = 0; c < HD / 32; ++c) {
-                    uint32_t o[32];
-                    tc::tmem_ld32(tO + 32 * c, o);
-                    tc::tmem_ld_wait();
-                    if (slow && store) add_hidden(P, it, h.vis + r, c, o);
-                    if (!store) continue;
+                for (int c = 0; c < HD / 64; ++c) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        uint32_t pk[4];
+                    for (int e = 0; e < 2; ++e) {
+                        uint32_t o[32];
+                        tc::tmem_ld32(tO + 64 * c + 32 * e, o);
+                        tc::tmem_ld_wait();
+                        if (slow && r < h.rows) add_hidden(P, it, h.vis + r, 2 * c + e, o);
 #pragma unroll
-                        for (int z = 0; z < 4; ++z)
-                            pk[z] = pack_bf16x2(__uint_as_float(o[8 * e + 2 * z]) * inv,
-                                                __uint_as_float(o[8 * e + 2 * z + 1]) * inv);
-                        reinterpret_cast<uint4 *>(dst)[4 * c + e] =
-                            none ? make_uint4(0, 0, 0, 0) : make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                        for (int z = 0; z < 4; ++z) {
+                            uint32_t pk[4];
+#pragma unroll
+                            for (int y = 0; y < 4; ++y)
+                                pk[y] = none ? 0u
+                                             : pack_bf16x2(__uint_as_float(o[8 * z + 2 * y]) * inv,
+                                                           __uint_as_float(o[8 * z + 2 * y + 1]) * inv);
+                            stage[lane * 8 + ((4 * e + z) ^ (lane & 7))] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                        }
                     }
+                    if (c + 1 == HD / 64) {
+                        tc::tc_fence_before();
+                        tc::mbar_arrive(&bars->o_free[a]);
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int z = 0; z < 8; ++z) {
+                        const int row = 4 * z + (lane >> 3), chunk = lane & 7;
+                        if (quarter * 32 + row < h.rows)
+                            reinterpret_cast<uint4 *>(P.out + (static_cast<int64_t>(h.q0 + quarter * 32 + row) * P.H +
+                                                               h.head) * HD + 64 * c)[chunk] =
+                                stage[row * 8 + (chunk ^ (row & 7))];
+                    }
+                    __syncwarp();
                 }
-                tc::tc_fence_before();
-                tc::mbar_arrive(&bars->o_free[a]);
             }
         }
     } else {
@@ -432,34 +454,28 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                     release(u);
                     if (last) tc::mma_commit(&bars->q_empty[a]);
                 };
-                // the half's key tiles one after another, items and all: tile j of its item, whose
+                // the half's key tiles one after another, items and all: tile j of the item's n, whose
                 // K is the loader's tile t
+                Items items(P);
                 struct Cursor {
-                    Items items;
-                    Item it;
-                    int a, j = 0, t = -2;
-                    bool live = true, in = false;
-                    __device__ __forceinline__ Cursor(const Params &p, int half) : items(p), a(half) {}
-                    __device__ __forceinline__ void next() {
-                        int step = 2;      // loader tiles passed
-                        if (in) {
-                            if (++j < it.h[a].n) {
-                                t += 2;
-                                return;
-                            }
-                            step += 2 * (it.n - j);
-                        }
-                        while ((live = items.get(it))) {
-                            if (it.h[a].n > 0) break;
-                            step += 2 * it.n;
-                        }
-                        in = true;
-                        j = 0;
-                        t += step;
-                    }
-                    __device__ __forceinline__ bool last() const { return j + 1 == it.h[a].n; }
+                    int j = 0, n = 0, rest = 0, t = -2;      // rest: tiles of the item behind the half's
+                    bool live = true;
+                    __device__ __forceinline__ bool last() const { return j + 1 == n; }
                 };
-                Cursor cs(P, a), cp(P, a);      // scores, products with V
+                Cursor cs, cp;      // scores, products with V
+                auto next = [&](Cursor &c) {
+                    c.t += 2;      // loader tiles passed
+                    if (++c.j < c.n) return;
+                    c.t += 2 * c.rest;
+                    Item it;
+                    while ((c.live = items.get(it))) {
+                        if (it.h[a].n > 0) break;
+                        c.t += 2 * it.n;
+                    }
+                    c.j = 0;
+                    c.n = it.h[a].n;
+                    c.rest = it.n - c.n;
+                };
                 auto scores = [&](bool behind) {
                     ok = full(cs.t) && (cs.j > 0 || wait1(&bars->q_full[a], qn++ & 1)) &&
                          (!behind || !C::kOwnP || wait1(&bars->s_read[a], (pn - 1) & 1));
@@ -472,12 +488,12 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                 auto pass_to = [&](int u) {
                     while (ok && passed < u) ok = skip(passed++);
                 };
-                cs.next();
-                cp.next();
+                next(cs);
+                cp = cs;
                 pass_to(cs.t);
                 if (ok && cs.live) scores(false);
                 while (ok && cp.live) {
-                    cs.next();
+                    next(cs);
                     ++pn;
                     // S of the next tile ahead of the product where the softmax's columns allow it
                     // and the ring reaches: its tile may be at most one that the half skips away
@@ -501,7 +517,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                     passed = cp.t + 2;
                     pass_to(cs.t);
                     if (ok && !lead && cs.live) scores(true);
-                    cp.next();
+                    cp = cs;
                 }
                 tc::mma_commit(&bars->drain[a]);
                 wait1(&bars->drain[a], 0);
@@ -527,7 +543,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                 if (it.n == 0) continue;
                 for (int j = 0; j < it.n; ++j) {
                     if (!(ok = slot(t))) break;
-                    load_kv(&tmap_k, t, it.hk * HD, it.k0 + j * kN);
+                    load_kv(&tmap_k, t, it.h[0].head / (P.H / P.Hk) * HD, it.k0 + j * kN);
                     ++t;
                     if (j == 0) {
 #pragma unroll
@@ -547,7 +563,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                         if (!ok) break;
                     }
                     if (!(ok = slot(t))) break;
-                    load_kv(&tmap_v, t, it.hk * HD, it.k0 + j * kN);
+                    load_kv(&tmap_v, t, it.h[0].head / (P.H / P.Hk) * HD, it.k0 + j * kN);
                     ++t;
                 }
             }
