@@ -53,6 +53,8 @@ constexpr float kRescale = 8.0f;               // log2 growth of a row maximum t
 template <int HD>
 struct Cfg {
     static constexpr int kBoxes = HD / 64;
+    static constexpr int kQBufs = HD == 64 ? 2 : 1;           // items whose Q is held
+    static constexpr uint32_t kQ = 2 * kQBufs * kN * HD * 2;
     static constexpr bool kOwnP = HD == 64;                   // P has columns of its own
     // One pair of exponentials in 8 on the FMA pipe (tc::ex2_poly2) where the softmax waits for
     // products: 16384 rows of 16 heads 944 us without, 919 with 1 in 8, 1060 with 2. At head_dim
@@ -63,15 +65,16 @@ struct Cfg {
     static constexpr uint32_t kRing = kStages * kTile;
     static constexpr uint32_t kSum = 2 * 2 * kM * 4;          // row sums [item parity][half][row]
     static constexpr uint32_t kStage = kM * 128;              // 64 output columns of a half
-    static constexpr uint32_t kSmem = 2 * kTile + kRing + kStage + kSum + 1024 /*barriers*/ + 1024 /*align*/;
+    static constexpr uint32_t kSmem = kQ + kRing + kStage + kSum + 1024 /*barriers*/ + 1024 /*align*/;
     static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
 struct Bars {
-    uint64_t q_full[2], q_empty[2], kv_full[8], kv_empty[8], v_ready[8], s_full[2], s_read[2], p_full[2],
+    uint64_t q_full[2][2], q_empty[2][2], kv_full[8], kv_empty[8], v_ready[8], s_full[2], s_read[2], p_half[2], p_full[2], turn[2],
         pv_done[2], o_full[2], o_free[2], l_full[2][2], drain[2];
     uint32_t tmem_base;
     int abort;
+    float zero;
     int fix[kFix];      // item whose values needed the slow path, in slot item % kFix
 };
 static_assert(sizeof(Bars) <= 1024, "barrier block");
@@ -184,21 +187,25 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
     unsigned char *sbase = smem_raw + (base - raw);
-    const uint32_t ring = base + 2 * C::kTile;
-    float *sSum = reinterpret_cast<float *>(sbase + 2 * C::kTile + C::kRing + C::kStage);
-    Bars *bars = reinterpret_cast<Bars *>(sbase + 2 * C::kTile + C::kRing + C::kStage + C::kSum);
+    const uint32_t ring = base + C::kQ;
+    float *sSum = reinterpret_cast<float *>(sbase + C::kQ + C::kRing + C::kStage);
+    Bars *bars = reinterpret_cast<Bars *>(sbase + C::kQ + C::kRing + C::kStage + C::kSum);
     volatile int *abort_flag = &bars->abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         for (int a = 0; a < 2; ++a) {
             tc::mbar_init(&bars->drain[a], 1);
-            tc::mbar_init(&bars->q_full[a], 1);
-            tc::mbar_init(&bars->q_empty[a], 1);
+            for (int q = 0; q < 2; ++q) {
+                tc::mbar_init(&bars->q_full[a][q], 1);
+                tc::mbar_init(&bars->q_empty[a][q], 1);
+            }
             tc::mbar_init(&bars->s_full[a], 1);
             tc::mbar_init(&bars->s_read[a], kM);
             tc::mbar_init(&bars->pv_done[a], 1);
+            tc::mbar_init(&bars->p_half[a], kM);
             tc::mbar_init(&bars->p_full[a], kM);
+            tc::mbar_init(&bars->turn[a], kM);
             tc::mbar_init(&bars->o_full[a], 1);
             tc::mbar_init(&bars->o_free[a], kM);
             tc::mbar_init(&bars->l_full[a][0], kM);
@@ -210,6 +217,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
             tc::mbar_init(&bars->v_ready[s], 1);
         }
         bars->abort = 0;
+        bars->zero = 0.0f;
         for (int i = 0; i < kFix; ++i) bars->fix[i] = -1;
     }
     if (warp == 12) {
@@ -239,7 +247,8 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
         const uint64_t sc2 = tc::f2(P.scale_log2, P.scale_log2);
         const uint32_t tP = C::kOwnP ? tmem + kPCol + a * 64 + lanes : tS;
         int phase = 0, par = 0, pv = 0;     // tiles begun, item parity, tiles whose product was waited for
-        bool ok = true;
+        int turns = 0;                      // turns of the other half waited for
+        bool ok = true, owed = false;       // owed: the other half's turn has to come before this one's next
         Items items(P);
         for (Item it; ok && items.get(it);) {
             const Half h = it.h[a];
@@ -257,6 +266,25 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                 if (!(ok = wait(&bars->s_full[a], phase & 1))) break;
                 ++phase;
                 tc::tc_fence_after();
+                // cut tiles (warp-uniform: the warp's first row sees less than all): the hidden scores
+                // become -inf where they lie, in a rolled loop, since this code is run once an item
+                // and an unrolled select over the registers below costs more to fetch than to do
+                const int seen = h.vis + r - j * kN;
+                if (h.vis + quarter * 32 - j * kN < kN) {
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        if (h.vis + quarter * 32 - j * kN >= 32 * (c + 1)) continue;
+                        uint32_t x[32];
+                        tc::tmem_ld32(tS + 32 * c, x);
+                        tc::tmem_ld_wait();
+                        const int left = min(max(seen - 32 * c, 0), 32);
+                        const uint32_t keep = left == 32 ? 0xffffffffu : (1u << left) - 1u;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) x[e] = keep >> e & 1u ? x[e] : __float_as_uint(-INFINITY);
+                        tc::tmem_st32(tS + 32 * c, x);
+                    }
+                    tc::tmem_st_wait();
+                }
                 uint32_t v[4][32];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) tc::tmem_ld32(tS + 32 * c, v[c]);
@@ -264,18 +292,6 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                 if constexpr (C::kOwnP) {
                     tc::tc_fence_before();
                     tc::mbar_arrive(&bars->s_read[a]);
-                }
-                // keys of this tile that the row sees; warp-uniform test whether any row is cut
-                const int seen = h.vis + r - j * kN;
-                if (h.vis + quarter * 32 - j * kN < kN) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const int left = min(max(seen - 32 * c, 0), 32);
-                        const uint32_t keep = left == 32 ? 0xffffffffu : (1u << left) - 1u;
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            v[c][e] = keep >> e & 1u ? v[c][e] : __float_as_uint(-INFINITY);
-                    }
                 }
                 float mx[4];
 #pragma unroll
@@ -312,12 +328,24 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                         tc::tmem_st16(tO + 16 * c, o);
                     }
                 }
+                // Turns (P in S's columns): the halves' exponentials one after the other, B's tile j
+                // behind A's, A's next behind B's. In step they share the special-function unit and
+                // then the tensor pipe, each idle while the other is fought over: 16384 rows, 16
+                // heads 1060 us, in turns 900. Each turn is waited for exactly once.
+                const bool shared = !C::kOwnP && j < min(it.h[0].n, it.h[1].n);
+                if (!C::kOwnP && (a == 0 ? owed : shared)) {
+                    if (!(ok = wait(&bars->turn[a ^ 1], turns++ & 1))) break;
+                    owed = false;
+                }
                 const float mref = m == -INFINITY ? 0.0f : m;
-                const uint64_t nm2 = tc::f2(-mref, -mref);
                 uint64_t l2[2] = {tc::f2(0.0f, 0.0f), tc::f2(0.0f, 0.0f)};
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     uint32_t pk[32];
+                    // a value read behind the hand-over of the first half keeps the second half's
+                    // work there
+                    const float ref = C::kOwnP || c == 0 ? mref : mref + *reinterpret_cast<volatile float *>(&bars->zero);
+                    const uint64_t nm2 = tc::f2(-ref, -ref);
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
                         const uint32_t *s = &v[2 * c + (e >> 4)][2 * (e & 15)];
@@ -329,11 +357,20 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                     }
                     if (C::kOwnP && c == 0 && phase > 1 && !pv_done()) break;   // the last P is read
                     tc::tmem_st32(tP + 32 * c, pk);
+                    if (!C::kOwnP && c == 0) {
+                        tc::tmem_st_wait();
+                        tc::tc_fence_before();
+                        tc::mbar_arrive(&bars->p_half[a]);
+                    }
                 }
                 if (!ok) break;
                 tc::tmem_st_wait();
                 tc::tc_fence_before();
                 tc::mbar_arrive(&bars->p_full[a]);
+                if (shared) {
+                    tc::mbar_arrive(&bars->turn[a]);
+                    owed = true;
+                }
                 const float2 ls = tc::f2_split(tc::add2(l2[0], l2[1]));
                 l += ls.x + ls.y;
             }
@@ -352,7 +389,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
         tc::regs_dec<80>();
         const int quarter = warp & 3, r = quarter * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-        uint4 *stage = reinterpret_cast<uint4 *>(sbase + 2 * C::kTile + C::kRing) + quarter * 32 * 8;
+        uint4 *stage = reinterpret_cast<uint4 *>(sbase + C::kQ + C::kRing) + quarter * 32 * 8;
         int phase[2] = {0, 0};
         bool ok = true;
         Items items(P);
@@ -426,7 +463,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
             const uint32_t idesc_o = tc::idesc_bf16_f32(kM, HD, false, true);
             const uint32_t tS = tc::uniform(tmem) + kSCol + a * kN, tO = tc::uniform(tmem) + kOCol + a * HD;
             const uint32_t tP = C::kOwnP ? tc::uniform(tmem) + kPCol + a * 64 : tS;
-            const uint32_t sQ = tc::uniform(base) + a * C::kTile, sR = tc::uniform(ring);
+            const uint32_t sQ = tc::uniform(base) + a * C::kQBufs * C::kTile, sR = tc::uniform(ring);
             if (tc::elect_one()) {
                 int qn = 0, pn = 0, on = 0;      // items begun, tiles, items with a product
                 bool ok = true;
@@ -443,7 +480,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                     return there;
                 };
                 auto issue_s = [&](int u, bool last) {
-                    const uint64_t ad = tc::smem_desc_sw128(sQ, 16, 1024);
+                    const uint64_t ad = tc::smem_desc_sw128(sQ + (qn - 1) % C::kQBufs * C::kTile, 16, 1024);
                     const uint64_t bd = tc::smem_desc_sw128(sR + (u % kStages) * C::kTile, 16, 1024);
 #pragma unroll
                     for (int kk = 0; kk < HD / 16; ++kk) {
@@ -452,7 +489,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                     }
                     tc::mma_commit(&bars->s_full[a]);
                     release(u);
-                    if (last) tc::mma_commit(&bars->q_empty[a]);
+                    if (last) tc::mma_commit(&bars->q_empty[a][(qn - 1) % C::kQBufs]);
                 };
                 // the half's key tiles one after another, items and all: tile j of the item's n, whose
                 // K is the loader's tile t
@@ -476,8 +513,12 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                     c.n = it.h[a].n;
                     c.rest = it.n - c.n;
                 };
+                auto q_ready = [&] {
+                    const int q = qn++;
+                    return wait1(&bars->q_full[a][q % C::kQBufs], (q / C::kQBufs) & 1);
+                };
                 auto scores = [&](bool behind) {
-                    ok = full(cs.t) && (cs.j > 0 || wait1(&bars->q_full[a], qn++ & 1)) &&
+                    ok = full(cs.t) && (cs.j > 0 || q_ready()) &&
                          (!behind || !C::kOwnP || wait1(&bars->s_read[a], (pn - 1) & 1));
                     if (ok) {
                         tc::tc_fence_after();
@@ -503,14 +544,20 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                     ok = ok && full(uv) && wait1(&bars->v_ready[uv % kStages], (uv / kStages) & 1) &&
                          (lead || !cs.live || cs.t != cp.t + 2 || full(cs.t)) &&
                          (cp.j > 0 || on == 0 || wait1(&bars->o_free[a], (on - 1) & 1)) &&
-                         wait1(&bars->p_full[a], (pn - 1) & 1);
+                         wait1(C::kOwnP ? &bars->p_full[a] : &bars->p_half[a], (pn - 1) & 1);
                     if (!ok) break;
                     if (cp.j == 0) ++on;
                     const uint64_t bv = tc::smem_desc_sw128(sR + (uv % kStages) * C::kTile, kBox, 1024);
                     tc::tc_fence_after();
 #pragma unroll
-                    for (int kk = 0; kk < kN / 16; ++kk)
+                    for (int kk = 0; kk < kN / 16; ++kk) {
+                        if (!C::kOwnP && kk == kN / 32) {      // the second half of P
+                            if (!(ok = wait1(&bars->p_full[a], (pn - 1) & 1))) break;
+                            tc::tc_fence_after();
+                        }
                         tc::mma_bf16_ts(tO, tP + 8 * kk, bv + 128 * kk, idesc_o, cp.j > 0 || kk > 0);
+                    }
+                    if (!ok) break;
                     if (C::kOwnP) tc::mma_commit(&bars->pv_done[a]);
                     release(uv);
                     if (cp.last()) tc::mma_commit(&bars->o_full[a]);
@@ -541,37 +588,37 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
             Items items(P);
             for (Item it; ok && items.get(it);) {
                 if (it.n == 0) continue;
-                for (int j = 0; j < it.n; ++j) {
-                    if (!(ok = slot(t))) break;
-                    load_kv(&tmap_k, t, it.h[0].head / (P.H / P.Hk) * HD, it.k0 + j * kN);
-                    ++t;
-                    if (j == 0) {
+                auto load_q = [&](int a) {
+                    if (it.h[a].n == 0) return;
+                    const int q = qn[a]++, buf = q % C::kQBufs;
+                    if (q >= C::kQBufs && !(ok = wait(&bars->q_empty[a][buf], (q / C::kQBufs - 1) & 1))) return;
+                    if (lane == 0) {
+                        tc::mbar_arrive_expect_tx(&bars->q_full[a][buf], C::kTile);
 #pragma unroll
-                        for (int a = 0; a < 2; ++a) {
-                            if (it.h[a].n == 0) continue;
-                            if (!(ok = qn[a] == 0 || wait(&bars->q_empty[a], (qn[a] - 1) & 1))) break;
-                            ++qn[a];
-                            if (lane == 0) {
-                                tc::mbar_arrive_expect_tx(&bars->q_full[a], C::kTile);
-#pragma unroll
-                                for (int c = 0; c < C::kBoxes; ++c)
-                                    tc::tma_load_2d(base + a * C::kTile + c * kBox, &tmap_q,
-                                                    it.h[a].head * HD + 64 * c, it.h[a].q0, &bars->q_full[a]);
-                            }
-                            __syncwarp();
-                        }
-                        if (!ok) break;
+                        for (int c = 0; c < C::kBoxes; ++c)
+                            tc::tma_load_2d(base + (a * C::kQBufs + buf) * C::kTile + c * kBox, &tmap_q,
+                                            it.h[a].head * HD + 64 * c, it.h[a].q0, &bars->q_full[a][buf]);
                     }
+                    __syncwarp();
+                };
+                const int x = it.h[0].head / (P.H / P.Hk) * HD;
+                for (int j = 0; ok && j < it.n; ++j) {
                     if (!(ok = slot(t))) break;
-                    load_kv(&tmap_v, t, it.h[0].head / (P.H / P.Hk) * HD, it.k0 + j * kN);
+                    load_kv(&tmap_k, t, x, it.k0 + j * kN);
                     ++t;
+                    if (j == 0) load_q(0);
+                    if (!ok || !(ok = slot(t))) break;
+                    load_kv(&tmap_v, t, x, it.k0 + j * kN);
+                    ++t;
+                    if (j == 0) load_q(1);      // half A need not wait for B to leave its last item
                 }
             }
             // no copy may be in flight when the CTA retires
             for (int u = max(0, t - kStages); u < t; ++u) wait(&bars->kv_full[u % kStages], (u / kStages) & 1);
 #pragma unroll
             for (int a = 0; a < 2; ++a)
-                if (qn[a] > 0) wait(&bars->q_full[a], (qn[a] - 1) & 1);
+                for (int q = max(0, qn[a] - C::kQBufs); q < qn[a]; ++q)
+                    wait(&bars->q_full[a][q % C::kQBufs], (q / C::kQBufs) & 1);
         } else {
             // -------------------------------------------------------- hidden values
             // A weight of 0 does not hide a NaN or an infinity from a product. In the tiles
@@ -588,7 +635,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                     const int u = t + 1;
                     if (!(ok = wait(&bars->kv_full[u % kStages], (u / kStages) & 1))) break;
                     if ((j + 1) * kN > first) {
-                        uint4 *tile = reinterpret_cast<uint4 *>(sbase + 2 * C::kTile + (u % kStages) * C::kTile);
+                        uint4 *tile = reinterpret_cast<uint4 *>(sbase + C::kQ + (u % kStages) * C::kTile);
                         const int cut = last - j * kN;      // rows of the tile that somebody sees
                         bool found = false;
 #pragma unroll 8
