@@ -402,14 +402,14 @@ MOM_API int mom_decode_attn(const void *q, int64_t q_ld, const void *k_pages, co
  * 0 .. Lk - Lq + r; a row that sees none (Lk < Lq) gets zeros. Values that the
  * mask hides from a row do not reach it, NaN and infinities neither.
  *
- * The plan depends on the lengths alone and serves every layer of a model:
- * mom_prompt_plan fills mom_prompt_plan_size bytes of HOST memory (k_lens may be
- * NULL: k_lens = q_lens), which the caller copies to the device; mom_prompt_attn
- * takes the device copy and its size. mom_prompt_plan_check reads and clears the
+ * The plan depends on the lengths and head counts alone and serves every layer of
+ * a model: mom_prompt_plan fills mom_prompt_plan_size bytes of HOST memory (k_lens
+ * may be NULL: k_lens = q_lens), which the caller copies to the device;
+ * mom_prompt_attn takes the device copy and its size. mom_prompt_plan_check reads and clears the
  * plan's device error word (it synchronises `stream`). */
-MOM_API size_t mom_prompt_plan_size(const int64_t *q_lens, int64_t n);
-MOM_API int mom_prompt_plan(const int64_t *q_lens, const int64_t *k_lens, int64_t n, void *plan_host,
-                            size_t plan_bytes);
+MOM_API size_t mom_prompt_plan_size(const int64_t *q_lens, int64_t n, int64_t H, int64_t Hk);
+MOM_API int mom_prompt_plan(const int64_t *q_lens, const int64_t *k_lens, int64_t n, int64_t H, int64_t Hk,
+                            void *plan_host, size_t plan_bytes);
 MOM_API int mom_prompt_attn(const void *q, int64_t q_ld, const void *k, int64_t k_ld, const void *v, int64_t v_ld,
                             int64_t Tq, int64_t Tk, int64_t H, int64_t Hk, int64_t head_dim, double scale, void *plan,
                             size_t plan_bytes, void *out, void *stream);

@@ -91,8 +91,8 @@ SIGNATURES = {
     "mom_decode_attn_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64]),
     "mom_decode_attn": (_int, [_vp, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64,
                                _c.c_double, _vp, _vp, _sz, _vp]),
-    "mom_prompt_plan_size": (_sz, [_vp, _i64]),
-    "mom_prompt_plan": (_int, [_vp, _vp, _i64, _vp, _sz]),
+    "mom_prompt_plan_size": (_sz, [_vp, _i64, _i64, _i64]),
+    "mom_prompt_plan": (_int, [_vp, _vp, _i64, _i64, _i64, _vp, _sz]),
     "mom_prompt_attn": (_int, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _c.c_double, _vp, _sz,
                                _vp, _vp]),
     "mom_prompt_plan_check": (_int, [_vp, _vp]),

@@ -124,32 +124,41 @@ def rope_append(qkv, cos, sin, positions, k_pages, v_pages, slots, *, n_heads: i
 class PromptPlan:
     """The work list of prompt_attention for one batch of lengths; it holds for
     every layer. q_lens: query tokens of each sequence, in packed order; k_lens:
-    its keys (default: the same), the queries being its last ones."""
+    its keys (default: the same), the queries being its last ones. The list for a
+    pair of head counts is made when it is first asked for."""
 
     def __init__(self, q_lens, k_lens=None, *, device="cuda"):
-        lib = _lib.load()
         self.q_lens = tuple(int(n) for n in q_lens)
         self.k_lens = self.q_lens if k_lens is None else tuple(int(n) for n in k_lens)
         if len(self.k_lens) != len(self.q_lens):
             raise RuntimeError(f"PromptPlan: {len(self.q_lens)} query lengths and {len(self.k_lens)} key lengths")
-        n = len(self.q_lens)
-        lens = (np.asarray(self.q_lens + self.k_lens, dtype=np.int64) if n else np.zeros(2, dtype=np.int64))
-        ql, kl = lens.ctypes.data, lens.ctypes.data + 8 * n
-        size = lib.mom_prompt_plan_size(ql, n)
-        if size == 0:
-            raise RuntimeError(f"PromptPlan: {_lib.last_error()}")
-        host = torch.empty(size, dtype=torch.uint8)
-        _lib.call("mom_prompt_plan", ql, kl, n, host.data_ptr(), size)
+        top = 1 << 30
+        if any(not 0 <= n <= top for n in self.q_lens + self.k_lens) or sum(self.q_lens) > top or \
+                sum(self.k_lens) > top:
+            raise RuntimeError("PromptPlan: lengths, and their sums, must be in [0, 2^30]")
         self.total_q, self.total_k = sum(self.q_lens), sum(self.k_lens)
-        self.buffer = host.to(device)
+        self.device = torch.empty(0, device=device).device
+        self._lists = {}
 
-    @property
-    def device(self):
-        return self.buffer.device
+    def list_for(self, n_heads: int, n_kv_heads: int):
+        """The device buffer of the work list for these head counts."""
+        got = self._lists.get((n_heads, n_kv_heads))
+        if got is None:
+            n = len(self.q_lens)
+            lens = np.asarray(self.q_lens + self.k_lens + (0,), dtype=np.int64)
+            ql, kl = lens.ctypes.data, lens.ctypes.data + 8 * n
+            size = _lib.load().mom_prompt_plan_size(ql, n, n_heads, n_kv_heads)
+            if size == 0:
+                raise RuntimeError(f"PromptPlan: {_lib.last_error()}")
+            host = torch.empty(size, dtype=torch.uint8)
+            _lib.call("mom_prompt_plan", ql, kl, n, n_heads, n_kv_heads, host.data_ptr(), size)
+            got = self._lists[n_heads, n_kv_heads] = host.to(self.device)
+        return got
 
     def check(self):
         """Raise if a kernel that used this plan gave up a wait (synchronises)."""
-        _lib.call_on(self.device.index, "mom_prompt_plan_check", self.buffer.data_ptr())
+        for buffer in self._lists.values():
+            _lib.call_on(self.device.index, "mom_prompt_plan_check", buffer.data_ptr())
 
 
 def prompt_attention(q, k, v, plan: PromptPlan, *, scale=None):
@@ -173,8 +182,9 @@ def prompt_attention(q, k, v, plan: PromptPlan, *, scale=None):
     if plan.device != q.device:
         raise RuntimeError(f"prompt_attention: the plan is on {plan.device}, q on {q.device}")
     out = torch.empty(Tq, H, hd, dtype=torch.bfloat16, device=q.device)
-    _lib.call_on(q.device.index, "mom_prompt_attn", q.data_ptr(), q_ld, k.data_ptr(), k_ld, v.data_ptr(), v_ld, Tq, Tk, H, Hk, hd,
-          hd ** -0.5 if scale is None else float(scale), plan.buffer.data_ptr(), plan.buffer.numel(), out.data_ptr())
+    work = plan.list_for(H, Hk)
+    _lib.call_on(q.device.index, "mom_prompt_attn", q.data_ptr(), q_ld, k.data_ptr(), k_ld, v.data_ptr(), v_ld, Tq, Tk,
+                 H, Hk, hd, hd ** -0.5 if scale is None else float(scale), work.data_ptr(), work.numel(), out.data_ptr())
     return out
 
 

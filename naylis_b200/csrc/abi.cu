@@ -9,6 +9,7 @@
 #include <cstdio>
 #include <cstring>
 #include <atomic>
+#include <exception>
 #include <mutex>
 
 #include <cuda.h>
@@ -957,20 +958,29 @@ int check_prompt_lens(const int64_t *q_lens, const int64_t *k_lens, int64_t n) {
 }
 }  // namespace
 
-size_t mom_prompt_plan_size(const int64_t *q_lens, int64_t n) {
-    if (check_prompt_lens(q_lens, nullptr, n) != MOM_OK) return 0;
-    return mom::kPromptHeader + static_cast<size_t>(mom::prompt_tiles(q_lens, n)) * sizeof(mom::PromptTile);
+size_t mom_prompt_plan_size(const int64_t *q_lens, int64_t n, int64_t H, int64_t Hk) {
+    if (check_attn_geometry(H, Hk, 64) != MOM_OK || check_prompt_lens(q_lens, nullptr, n) != MOM_OK) return 0;
+    const int64_t tiles = mom::prompt_tiles(q_lens, n);
+    if (tiles * H > INT32_MAX) {
+        fail(MOM_ERR_INVALID_ARGUMENT, "too many tiles");
+        return 0;
+    }
+    return mom::prompt_layout(tiles, H).bytes;
 }
 
-int mom_prompt_plan(const int64_t *q_lens, const int64_t *k_lens, int64_t n, void *plan_host, size_t plan_bytes) {
-    int rc = check_prompt_lens(q_lens, k_lens, n);
-    if (rc) return rc;
+int mom_prompt_plan(const int64_t *q_lens, const int64_t *k_lens, int64_t n, int64_t H, int64_t Hk, void *plan_host,
+                    size_t plan_bytes) {
+    int rc = check_attn_geometry(H, Hk, 64);
+    if (rc || (rc = check_prompt_lens(q_lens, k_lens, n))) return rc;
     MOM_REQUIRE(plan_host, "null pointer argument");
-    const size_t need = mom_prompt_plan_size(q_lens, n);
+    const size_t need = mom_prompt_plan_size(q_lens, n, H, Hk);
+    if (need == 0) return MOM_ERR_INVALID_ARGUMENT;
     if (plan_bytes < need) return fail(MOM_ERR_WORKSPACE, "plan of %zu bytes, %zu needed", plan_bytes, need);
-    std::memset(plan_host, 0, mom::kPromptHeader);
-    mom::prompt_plan(q_lens, k_lens, n,
-                     reinterpret_cast<mom::PromptTile *>(static_cast<char *>(plan_host) + mom::kPromptHeader));
+    try {
+        mom::prompt_plan(q_lens, k_lens, n, H, Hk, plan_host);
+    } catch (const std::exception &e) {
+        return fail(MOM_ERR_WORKSPACE, "prompt_plan: %s", e.what());
+    }
     return MOM_OK;
 }
 
@@ -987,15 +997,13 @@ int mom_prompt_attn(const void *q, int64_t q_ld, const void *k, int64_t k_ld, co
     MOM_REQUIRE(q && plan && out && (Tk == 0 || (k && v)), "null pointer argument");
     MOM_REQUIRE(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 16) && aligned(plan, 16),
                 "buffers must be 16-byte aligned");
-    MOM_REQUIRE(plan_bytes > mom::kPromptHeader && (plan_bytes - mom::kPromptHeader) % sizeof(mom::PromptTile) == 0,
-                "plan_bytes is not a plan's size");
-    const int64_t n_tiles = (plan_bytes - mom::kPromptHeader) / sizeof(mom::PromptTile);
-    MOM_REQUIRE(n_tiles * H < (int64_t(1) << 31), "too many tiles");
+    const size_t fixed = mom::prompt_layout(0, H).bytes, per = mom::prompt_layout(1, H).bytes - fixed;
+    MOM_REQUIRE(plan_bytes > fixed && (plan_bytes - fixed) % per == 0, "plan_bytes is not a plan's for these heads");
+    const int64_t n_tiles = static_cast<int64_t>((plan_bytes - fixed) / per);
+    MOM_REQUIRE(n_tiles * H <= INT32_MAX, "too many tiles");
     if ((rc = check_current_device())) return rc;
-    cudaError_t e = mom::launch_prompt_attn(
-        q, q_ld, k, k_ld, v, v_ld, Tq, Tk,
-        reinterpret_cast<const mom::PromptTile *>(static_cast<const char *>(plan) + mom::kPromptHeader), n_tiles,
-        static_cast<int *>(plan), (int)H, (int)Hk, (int)hd, (float)scale, out, static_cast<cudaStream_t>(stream));
+    cudaError_t e = mom::launch_prompt_attn(q, q_ld, k, k_ld, v, v_ld, Tq, Tk, plan, n_tiles, (int)H, (int)Hk, (int)hd,
+                                            (float)scale, out, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? MOM_OK : cuda_fail(e, "prompt_attn");
 }
 

@@ -239,7 +239,7 @@ cudaError_t launch_decode_attn(const void *q, int64_t q_ld, const void *kp, cons
                                int64_t max_len, int64_t B, int H, int Hk, int hd, float scale, void *out, float *part,
                                cudaStream_t st);
 
-// Packed prompts (prompt.cu): the plan's tiles of query rows, costliest first.
+// Packed prompts (prompt.cu): the plan's tiles of query rows.
 constexpr int kPromptRows = 256;
 struct PromptTile {
     int32_t q0;     // first query row (packed)
@@ -247,12 +247,26 @@ struct PromptTile {
     int32_t k0;     // the sequence's first key row (packed)
     int32_t vis;    // keys the first row sees (<= 0: none); row r sees vis + r
 };
-constexpr int kPromptHeader = 16;   // bytes before the tiles in a plan: the error word
+constexpr int kPromptCtas = 148;
+// A plan in memory: the error word (16 bytes), the tiles, first[c] .. first[c + 1]: CTA c's
+// part of the items, and the items {tile, part of it}: H a tile, those without rows left out.
+struct PromptLayout {
+    size_t tiles = 16, first = 0, items = 0, bytes = 0;
+};
+inline PromptLayout prompt_layout(int64_t n_tiles, int64_t H) {
+    PromptLayout L;
+    L.first = L.tiles + static_cast<size_t>(n_tiles) * sizeof(PromptTile);
+    L.items = L.first + (kPromptCtas + 4) * sizeof(int32_t);
+    L.bytes = L.items + static_cast<size_t>(n_tiles * H) * sizeof(int2);
+    return L;
+}
+// Whether a CTA's halves are two heads of a group (else two runs of 128 rows).
+inline bool prompt_pairs(int64_t H, int64_t Hk) { return H / Hk % 2 == 0; }
 int64_t prompt_tiles(const int64_t *q_lens, int64_t n);
-void prompt_plan(const int64_t *q_lens, const int64_t *k_lens, int64_t n, PromptTile *tiles);
+void prompt_plan(const int64_t *q_lens, const int64_t *k_lens, int64_t n, int64_t H, int64_t Hk, void *plan);
 cudaError_t launch_prompt_attn(const void *q, int64_t q_ld, const void *k, int64_t k_ld, const void *v, int64_t v_ld,
-                               int64_t Tq, int64_t Tk, const PromptTile *tiles, int64_t n_tiles, int *err, int H,
-                               int Hk, int hd, float scale, void *out, cudaStream_t st);
+                               int64_t Tq, int64_t Tk, void *plan, int64_t n_tiles, int H, int Hk, int hd, float scale,
+                               void *out, cudaStream_t st);
 
 // Token log probabilities (scoring.cu): logits (R, V) of row pitch ld; stats (R, 4).
 constexpr int kMaxTopLogprobs = 32;

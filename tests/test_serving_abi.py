@@ -16,43 +16,71 @@ def lib():
     return _lib.load()
 
 
-def _plan(lib, ql, kl=None):
+def _plan(lib, ql, kl=None, H=4, Hk=4):
     q = np.asarray(ql, dtype=np.int64)
     k = None if kl is None else np.asarray(kl, dtype=np.int64)
-    size = lib.mom_prompt_plan_size(q.ctypes.data, len(ql))
+    size = lib.mom_prompt_plan_size(q.ctypes.data, len(ql), H, Hk)
     buf = np.full(size, 0xAB, dtype=np.uint8)
-    rc = lib.mom_prompt_plan(q.ctypes.data, None if k is None else k.ctypes.data, len(ql), buf.ctypes.data, size)
+    rc = lib.mom_prompt_plan(q.ctypes.data, None if k is None else k.ctypes.data, len(ql), H, Hk, buf.ctypes.data, size)
     assert rc == OK
-    return buf[:16], buf[16:].view(np.int32).reshape(-1, 4)
+    n = sum(-(-x // 256) for x in ql)
+    words = buf.view(np.int32)
+    assert not words[:4].any()
+    tiles = words[4:4 + 4 * n].reshape(n, 4)
+    first = words[4 + 4 * n:][:149]
+    items = words[4 + 4 * n + 152:].reshape(-1, 2)
+    assert len(items) == n * H
+    return tiles, first, items
 
 
 @pytest.mark.parametrize("ql,kl", [([1], None), ([256, 257, 0, 1, 1000], None), ([5, 300], [400, 10]), ([0, 0], None)])
-def test_plan_covers_every_row_once_and_puts_the_costliest_first(lib, ql, kl):
-    head, tiles = _plan(lib, ql, kl)
-    assert not head.any()
-    seen = np.zeros(sum(ql), dtype=int)
+@pytest.mark.parametrize("H,Hk", [(4, 4), (4, 2), (6, 2)])
+def test_plan_covers_every_row_and_head_once(lib, ql, kl, H, Hk):
+    tiles, first, items = _plan(lib, ql, kl, H, Hk)
+    seen = np.zeros((sum(ql), H), dtype=int)
     q0 = np.concatenate([[0], np.cumsum(ql)])
     k0 = np.concatenate([[0], np.cumsum(kl or ql)])
     for a, rows, k, vis in tiles:
         assert 1 <= rows <= 256
-        seen[a:a + rows] += 1
         i = int(np.searchsorted(q0, a, side="right") - 1)
         assert a + rows <= q0[i + 1] and k == k0[i]
         assert vis == (kl or ql)[i] - ql[i] + (a - q0[i]) + 1
+    assert first[0] == 0 and (np.diff(first) >= 0).all()
+    for t, rem in items[:first[148]]:
+        a, rows = tiles[t][:2]
+        if H // Hk % 2:                      # a head, all rows
+            seen[a:a + rows, rem] += 1
+        else:                                # two heads, rows 0 .. 127 or 128 .. 255
+            sub, pair = (1, rem) if rem < H // 2 else (0, rem - H // 2)
+            assert rows > 128 * sub
+            seen[a + 128 * sub:a + min(rows, 128 * sub + 128), 2 * pair:2 * pair + 2] += 1
     assert (seen == 1).all()
-    last = tiles[:, 3] + tiles[:, 1]
-    assert (np.diff(last) <= 0).all()
+
+
+def test_plan_levels_the_work(lib):
+    """Longest first to the least busy: nobody is above the mean by more than the
+    largest item."""
+    rng = np.random.RandomState(0)
+    ql = [int(x) for x in np.exp(rng.uniform(0, np.log(4000), 40))]
+    tiles, first, items = _plan(lib, ql, None, 8, 8)
+    cost = (tiles[:, 3] + tiles[:, 1] - 1 + 127) // 128 + 1.5
+    per = [cost[items[first[c]:first[c + 1], 0]] for c in range(148)]
+    load = np.array([x.sum() for x in per])
+    assert load.max() <= load.mean() + cost.max()
+    assert all((np.diff(x) <= 0).all() for x in per)
 
 
 def test_plan_refuses(lib):
     one = np.asarray([-1], dtype=np.int64)
-    assert lib.mom_prompt_plan_size(one.ctypes.data, 1) == 0 and b"lengths" in lib.mom_last_error_string()
+    assert lib.mom_prompt_plan_size(one.ctypes.data, 1, 4, 4) == 0 and b"lengths" in lib.mom_last_error_string()
     big = np.asarray([1 << 30, 1 << 30], dtype=np.int64)
-    assert lib.mom_prompt_plan_size(big.ctypes.data, 2) == 0
+    assert lib.mom_prompt_plan_size(big.ctypes.data, 2, 4, 4) == 0
     two = np.asarray([300, 4], dtype=np.int64)
-    buf = np.zeros(64, dtype=np.uint8)
-    assert lib.mom_prompt_plan(two.ctypes.data, None, 2, buf.ctypes.data, 32) == WORKSPACE
-    assert lib.mom_prompt_plan(two.ctypes.data, None, 2, None, 64) == INVALID
+    assert lib.mom_prompt_plan_size(two.ctypes.data, 2, 4, 3) == 0
+    buf = np.zeros(4096, dtype=np.uint8)
+    assert lib.mom_prompt_plan(two.ctypes.data, None, 2, 4, 4, buf.ctypes.data, 32) == WORKSPACE
+    assert lib.mom_prompt_plan(two.ctypes.data, None, 2, 4, 4, None, 4096) == INVALID
+    assert lib.mom_prompt_plan(two.ctypes.data, None, 2, 0, 4, buf.ctypes.data, 4096) == INVALID
 
 
 def _rope(lib, **kw):
@@ -71,7 +99,7 @@ def _decode(lib, **kw):
 
 def _prompt(lib, **kw):
     a = dict(q=P(256), qld=128, k=P(256), kld=128, v=P(256), vld=128, Tq=3, Tk=3, H=2, Hk=2, hd=64, scale=0.1,
-             plan=P(256), bytes=32, out=P(256), stream=None)
+             plan=P(256), bytes=16 + 152 * 4 + 32, out=P(256), stream=None)
     a.update(kw)
     return lib.mom_prompt_attn(*a.values())
 
