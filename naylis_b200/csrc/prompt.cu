@@ -93,7 +93,6 @@ constexpr uint32_t kBox = 128 * 128;           // one TMA box: 128 rows x 64 bf1
 // 64 of its S.
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kSCol = 0, kOCol = 256, kPCol = 384;
-constexpr int kFix = 8;
 constexpr float kRescale = 8.0f;               // log2 growth of a row maximum that O is rescaled for
 
 template <int HD>
@@ -102,10 +101,6 @@ struct Cfg {
     static constexpr int kQBufs = HD == 64 ? 2 : 1;           // items whose Q is held
     static constexpr uint32_t kQ = 2 * kQBufs * kN * HD * 2;
     static constexpr bool kOwnP = HD == 64;                   // P has columns of its own
-    // One pair of exponentials in 8 on the FMA pipe (tc::ex2_poly2) where the softmax waits for
-    // products: 16384 rows of 16 heads 944 us without, 919 with 1 in 8, 1060 with 2. At head_dim
-    // 64 the halves' softmaxes run side by side and none is best: 711, 787, 735 us.
-    static constexpr bool kPoly = HD == 128;
     static constexpr uint32_t kTile = kN * HD * 2;            // a K, V or Q tile
     static constexpr int kStages = HD == 64 ? 8 : 4;          // K and V tiles in turn
     static constexpr uint32_t kRing = kStages * kTile;
@@ -116,12 +111,11 @@ struct Cfg {
 };
 
 struct Bars {
-    uint64_t q_full[2][2], q_empty[2][2], kv_full[8], kv_empty[8], v_ready[8], s_full[2], s_read[2], p_half[2], p_full[2], turn[2],
+    uint64_t q_full[2][2], q_empty[2][2], kv_full[8], kv_empty[8], s_full[2], s_read[2], p_half[2], p_full[2], turn[2],
         pv_done[2], o_full[2], o_free[2], l_full[2][2], drain[2];
     uint32_t tmem_base;
     int abort;
     float zero;
-    int fix[kFix];      // item whose values needed the slow path, in slot item % kFix
 };
 static_assert(sizeof(Bars) <= 1024, "barrier block");
 
@@ -129,10 +123,10 @@ struct Params {
     const PromptTile *tiles;
     const int32_t *first;
     const int2 *items;
-    int H, Hk, hd, pair;      // pair: the halves are two heads of a group, else two runs of rows
+    int H, Hk, pair;      // pair: the halves are two heads of a group, else two runs of rows
     float scale_log2;
-    const uint16_t *v;
-    int64_t v_ld;
+    const uint16_t *q, *k, *v;
+    int64_t q_ld, k_ld, v_ld, Tk;
     uint16_t *out;
     int *err;
 };
@@ -143,12 +137,6 @@ struct Half {
 struct Item {
     Half h[2];
     int k0, n;
-    __device__ __forceinline__ int last() const {      // keys any row sees
-        return max(h[0].rows > 0 ? h[0].vis + h[0].rows - 1 : 0, h[1].rows > 0 ? h[1].vis + h[1].rows - 1 : 0);
-    }
-    __device__ __forceinline__ int first() const {     // keys every row sees
-        return min(h[0].rows > 0 ? h[0].vis : INT_MAX, h[1].rows > 0 ? h[1].vis : INT_MAX);
-    }
 };
 
 // The items of a CTA one after another, the next one's tile and the one after's entry
@@ -189,24 +177,37 @@ struct Items {
 };
 static_assert(kN == 128, "key tiles are counted by a shift");
 
-// The non-finite values that were taken out of an item's cut tiles, back into 32
-// columns of a row that sees `seen` keys: each makes its sum NaN or infinite.
-__device__ __noinline__ void add_hidden_at(const uint16_t *v, int64_t v_ld, int j0, int seen, float *o) {
-    for (int j = j0; j < seen; ++j)
-        for (int e = 0; e < 32; ++e) {
-            const uint16_t x = v[j * v_ld + e];
-            if ((x & 0x7f80) == 0x7f80) o[e] += bf16_bits_to_f32(x);
+// Rows of a half whose sums are not finite although their weights are: if the tiles
+// that the mask cuts hold a non-finite value, it may be a hidden one; then the warp's
+// spoilt rows are computed again, a thread each, over the keys that they see alone.
+// (Values that a row does see make it non-finite again, as they should.)
+template <int HD>
+__device__ __noinline__ void redo_rows(const Params &P, const Half &h, int k0, int r, bool spoilt) {
+    const int lane = threadIdx.x & 31, hk = h.head / (P.H / P.Hk);
+    const uint16_t *v = P.v + static_cast<int64_t>(k0) * P.v_ld + hk * HD, *k = P.k + static_cast<int64_t>(k0) * P.k_ld + hk * HD;
+    bool any = false;
+    for (int j = max(h.vis, 0) / kN * kN; j < min(h.n * kN, static_cast<int>(P.Tk) - k0); ++j)
+        for (int d = lane; d < HD; d += 32) any |= (v[j * P.v_ld + d] & 0x7f80) == 0x7f80;
+    if (!__any_sync(0xffffffffu, any) || !spoilt) return;
+    const int seen = h.vis + r;
+    const uint16_t *q = P.q + static_cast<int64_t>(h.q0 + r) * P.q_ld + h.head * HD;
+    auto score = [&](int j) {
+        float s = 0.0f;
+        for (int d = 0; d < HD; ++d) s = fmaf(bf16_bits_to_f32(q[d]), bf16_bits_to_f32(k[j * P.k_ld + d]), s);
+        return s * P.scale_log2;
+    };
+    float m = -INFINITY, l = 0.0f;
+    for (int j = 0; j < seen; ++j) m = fmaxf(m, score(j));
+    for (int j = 0; j < seen; ++j) l += tc::ex2(score(j) - m);
+    for (int d0 = 0; d0 < HD; d0 += 32) {
+        float o[32] = {};
+        for (int j = 0; j < seen; ++j) {
+            const float p = tc::ex2(score(j) - m);
+            for (int e = 0; e < 32; ++e) o[e] = fmaf(p, bf16_bits_to_f32(v[j * P.v_ld + d0 + e]), o[e]);
         }
-}
-__device__ __forceinline__ void add_hidden(const Params &P, const Item &it, int seen, int c, uint32_t (&o)[32]) {
-    float f[32];
-#pragma unroll
-    for (int e = 0; e < 32; ++e) f[e] = 0.0f;
-    const int hd = P.hd;
-    add_hidden_at(P.v + static_cast<int64_t>(it.k0) * P.v_ld + it.h[0].head / (P.H / P.Hk) * hd + 32 * c, P.v_ld,
-                  max(it.first(), 0) / kN * kN, seen, f);
-#pragma unroll
-    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) + f[e]);
+        uint16_t *dst = P.out + (static_cast<int64_t>(h.q0 + r) * P.H + h.head) * HD + d0;
+        for (int e = 0; e < 32; ++e) dst[e] = f32_to_bf16_bits(o[e] / l);
+    }
 }
 
 template <int HD>
@@ -246,11 +247,9 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
         for (int s = 0; s < kStages; ++s) {
             tc::mbar_init(&bars->kv_full[s], 1);
             tc::mbar_init(&bars->kv_empty[s], 2);
-            tc::mbar_init(&bars->v_ready[s], 1);
         }
         bars->abort = 0;
         bars->zero = 0.0f;
-        for (int i = 0; i < kFix; ++i) bars->fix[i] = -1;
     }
     if (warp == 12) {
         tc::tmem_alloc(&bars->tmem_base, kTmemCols);
@@ -331,14 +330,11 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                     mx[c] = __uint_as_float(v[c][0]);
 #pragma unroll
                     for (int e = 1; e < 31; e += 2)
-                        mx[c] = tc::fmax3_nan(mx[c], __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
+                        mx[c] = tc::fmax3(mx[c], __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
+                    mx[c] = fmaxf(mx[c], __uint_as_float(v[c][31]));
                 }
-                float top = tc::fmax3_nan(mx[0], mx[1], __uint_as_float(v[0][31]));
-                top = tc::fmax3_nan(top, mx[2], __uint_as_float(v[1][31]));
-                top = tc::fmax3_nan(top, mx[3], __uint_as_float(v[2][31]));
-                top = tc::fmax3_nan(top, top, __uint_as_float(v[3][31]));
-                // a score of NaN or +inf makes the row NaN (the polynomial below would lose it)
-                if (!(top < INFINITY)) l = __int_as_float(0x7fc00000);
+                // (a score of NaN or +inf makes its own weight NaN, and with it the row's sum)
+                const float top = fmaxf(tc::fmax3(mx[0], mx[1], mx[2]), mx[3]);
                 const float mn = fmaxf(m, top * P.scale_log2);
                 if (j == 0) {
                     m = mn;
@@ -347,7 +343,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                     // issued behind it
                     if (C::kOwnP && !pv_done()) break;
                     const float mo = m == -INFINITY ? mn : m;
-                    const float f = mn > m + kRescale ? (mn == INFINITY ? 1.0f : tc::ex2(mo - mn)) : 1.0f;
+                    const float f = mn > m + kRescale ? tc::ex2(mo - mn) : 1.0f;
                     if (mn > m + kRescale) m = mn;
                     l *= f;
 #pragma unroll
@@ -382,7 +378,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                     for (int e = 0; e < 32; ++e) {
                         const uint32_t *s = &v[2 * c + (e >> 4)][2 * (e & 15)];
                         const uint64_t x2 = tc::fma2(tc::f2_bits(s[0], s[1]), sc2, nm2);
-                        const uint64_t p2 = C::kPoly && (e & 7) == 3 ? tc::ex2_poly2(x2) : tc::ex2_pair(x2);
+                        const uint64_t p2 = tc::ex2_pair(x2);
                         l2[e & 1] = tc::add2(l2[e & 1], p2);
                         const float2 p = tc::f2_split(p2);
                         pk[e] = pack_bf16x2(p.x, p.y);
@@ -440,7 +436,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                 if (!(ok = wait(&bars->l_full[a][ph & 1], (ph >> 1) & 1) && wait(&bars->o_full[a], ph & 1))) break;
                 tc::tc_fence_after();
                 const float l = sSum[((ph & 1) * 2 + a) * kM + r];
-                const bool slow = *reinterpret_cast<volatile int *>(&bars->fix[items.i % kFix]) == items.i;
+                float big = 0.0f;      // the greatest magnitude of the row's sums, NaN if one is
                 const float inv = h.vis + r > 0 ? 1.0f / l : 0.0f;
                 const uint32_t tO = tmem + kOCol + a * HD + lanes;
                 const bool none = h.vis + r <= 0;
@@ -453,7 +449,9 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                         uint32_t o[32];
                         tc::tmem_ld32(tO + 64 * c + 32 * e, o);
                         tc::tmem_ld_wait();
-                        if (slow && r < h.rows) add_hidden(P, it, h.vis + r, 2 * c + e, o);
+#pragma unroll
+                        for (int z = 0; z < 32; z += 2)
+                            big = tc::fmax3_nan(big, fabsf(__uint_as_float(o[z])), fabsf(__uint_as_float(o[z + 1])));
 #pragma unroll
                         for (int z = 0; z < 4; ++z) {
                             uint32_t pk[4];
@@ -480,6 +478,11 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                     }
                     __syncwarp();
                 }
+                // A weight of 0 does not hide a NaN or an infinity from a product: rows that a value
+                // behind the mask has spoilt are done again, by themselves
+                const bool spoilt = !(big < INFINITY) && l < INFINITY && r < h.rows && !none;
+                if (__any_sync(0xffffffffu, spoilt))
+                    redo_rows<HD>(P, h, it.k0, r, spoilt);
             }
         }
     } else {
@@ -573,7 +576,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                     const bool lead = C::kOwnP && cs.live && cs.t - cp.t <= 4;
                     if (lead) scores(true);
                     const int uv = cp.t + 1;
-                    ok = ok && full(uv) && wait1(&bars->v_ready[uv % kStages], (uv / kStages) & 1) &&
+                    ok = ok && full(uv) &&
                          (lead || !cs.live || cs.t != cp.t + 2 || full(cs.t)) &&
                          (cp.j > 0 || on == 0 || wait1(&bars->o_free[a], (on - 1) & 1)) &&
                          wait1(C::kOwnP ? &bars->p_full[a] : &bars->p_half[a], (pn - 1) & 1);
@@ -651,55 +654,6 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
             for (int a = 0; a < 2; ++a)
                 for (int q = max(0, qn[a] - C::kQBufs); q < qn[a]; ++q)
                     wait(&bars->q_full[a][q % C::kQBufs], (q / C::kQBufs) & 1);
-        } else {
-            // -------------------------------------------------------- hidden values
-            // A weight of 0 does not hide a NaN or an infinity from a product. In the tiles
-            // that the mask cuts, this warp zeroes such values (and every row behind the
-            // last key anybody sees, another sequence's) before the product; the epilogue
-            // gives the zeroed ones back to the rows that see them.
-            int t = 0;
-            bool ok = true;
-            Items items(P);
-            for (Item it; ok && items.get(it);) {
-                if (it.n == 0) continue;
-                const int first = it.first(), last = it.last();
-                for (int j = 0; j < it.n; ++j, t += 2) {
-                    const int u = t + 1;
-                    if (!(ok = wait(&bars->kv_full[u % kStages], (u / kStages) & 1))) break;
-                    if ((j + 1) * kN > first) {
-                        uint4 *tile = reinterpret_cast<uint4 *>(sbase + C::kQ + (u % kStages) * C::kTile);
-                        const int cut = last - j * kN;      // rows of the tile that somebody sees
-                        bool found = false;
-#pragma unroll 8
-                        for (int e = lane; e < C::kBoxes * kN * 8; e += 32) {
-                            // 16-byte chunk e: box e / 1024, row e / 8 % 128
-                            const int row = e >> 3 & (kN - 1);
-                            uint4 *q = tile + e;
-                            uint4 x = *q;
-                            if (row >= cut) {
-                                *q = make_uint4(0, 0, 0, 0);
-                                continue;
-                            }
-                            uint32_t a[4] = {x.x, x.y, x.z, x.w};
-                            bool hit = false;
-#pragma unroll
-                            for (int z = 0; z < 4; ++z) {
-                                if ((a[z] & 0x7f80u) == 0x7f80u) a[z] &= 0xffff0000u, hit = true;
-                                if ((a[z] & 0x7f800000u) == 0x7f800000u) a[z] &= 0x0000ffffu, hit = true;
-                            }
-                            if (hit) {
-                                *q = make_uint4(a[0], a[1], a[2], a[3]);
-                                found = true;
-                            }
-                        }
-                        if (__any_sync(0xffffffffu, found) && lane == 0)
-                            *reinterpret_cast<volatile int *>(&bars->fix[items.i % kFix]) = items.i;
-                        tc::fence_proxy_async_smem();
-                    }
-                    __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(&bars->v_ready[u % kStages]);
-                }
-            }
         }
     }
     tc::tc_fence_before();
@@ -727,11 +681,15 @@ cudaError_t launch_prompt_attn(const void *q, int64_t q_ld, const void *k, int64
     p.items = reinterpret_cast<const int2 *>(base + L.items);
     p.H = H;
     p.Hk = Hk;
-    p.hd = hd;
     p.pair = prompt_pairs(H, Hk);
     p.scale_log2 = scale * kLog2e;
+    p.q = static_cast<const uint16_t *>(q);
+    p.k = static_cast<const uint16_t *>(k);
     p.v = static_cast<const uint16_t *>(v);
+    p.q_ld = q_ld;
+    p.k_ld = k_ld;
     p.v_ld = v_ld;
+    p.Tk = Tk;
     p.out = static_cast<uint16_t *>(out);
     p.err = static_cast<int *>(plan);
     const int grid = static_cast<int>(std::min<int64_t>(n_tiles * H, kPromptCtas));
