@@ -909,7 +909,7 @@ int mom_rope_append(const void *qkv, int64_t qkv_ld, const float *cosv, const fl
 size_t mom_decode_attn_workspace_size(int64_t B, int64_t H, int64_t Hk, int64_t hd, int64_t max_len) {
     if (B <= 0 || H <= 0 || Hk <= 0 || hd <= 0 || max_len <= 0) return 0;
     const mom::DecodeSplit s = mom::decode_split(B, H, Hk, max_len);
-    return s.n_chunks == 1 ? 0 : static_cast<size_t>(B) * H * s.n_chunks * (hd + 4) * sizeof(float);
+    return s.n_chunks == 1 || s.cluster ? 0 : static_cast<size_t>(B) * H * s.n_chunks * (hd + 4) * sizeof(float);
 }
 
 int mom_decode_attn(const void *q, int64_t q_ld, const void *k_pages, const void *v_pages, int64_t num_pages,

@@ -232,6 +232,7 @@ cudaError_t launch_rope_append(const void *qkv, int64_t ld, const float *cosv, c
 struct DecodeSplit {
     int chunk = 0;      // keys of a chunk
     int n_chunks = 1;   // chunks of the longest sequence the call may hold
+    bool cluster = false;   // the chunks join themselves: no parts in memory
 };
 DecodeSplit decode_split(int64_t B, int64_t H, int64_t Hk, int64_t max_len);
 cudaError_t launch_decode_attn(const void *q, int64_t q_ld, const void *kp, const void *vp, int64_t n_pages,

@@ -5,7 +5,7 @@
 //
 // The plan lists tiles of up to kPromptRows query rows and the work of each CTA.
 #include <algorithm>
-#include <climits>
+#include <atomic>
 #include <cstring>
 #include <functional>
 #include <queue>
@@ -693,9 +693,19 @@ cudaError_t launch_prompt_attn(const void *q, int64_t q_ld, const void *k, int64
     p.out = static_cast<uint16_t *>(out);
     p.err = static_cast<int *>(plan);
     const int grid = static_cast<int>(std::min<int64_t>(n_tiles * H, kPromptCtas));
+    static std::atomic<uint64_t> ready{0};      // devices whose kernels have their shared memory set
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+        if ((e = cudaFuncSetAttribute(prompt_tc_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      Cfg<64>::kSmem)) != cudaSuccess ||
+            (e = cudaFuncSetAttribute(prompt_tc_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      Cfg<128>::kSmem)) != cudaSuccess)
+            return e;
+        if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+    }
     auto go = [&](auto kernel, uint32_t smem) -> cudaError_t {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-        if (e != cudaSuccess) return e;
         kernel<<<grid, kThreads, smem, st>>>(mq, mk, mv, p);
         count_launch();
         return cudaGetLastError();

@@ -6,6 +6,7 @@
 // page * page_size + offset. The page size is a power of two (8 .. 256): a
 // key's page and offset are a shift and a mask.
 #include <algorithm>
+#include <atomic>
 
 #include "launch.h"
 #include "tc_common.cuh"
@@ -32,7 +33,10 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
 }
 
 // ------------------------------------------------------------------ rope_append
-// One thread per (token, head, 8 rotation pairs).
+// One thread per (token, head, 8 rotation pairs). Bound by memory: the projection in; q,
+// pages (and k) out. 16384 tokens of 16 + 2 x 4 heads of 128: 38 us, 5.8 TB/s; 64 tokens
+// of 48 heads of 64: 2.0 us. (A warp per token that keeps the tables' values for all its
+// heads: 36.7 and 3.2 us.)
 template <int HD>
 __global__ void __launch_bounds__(256)
 rope_append_kernel(const uint16_t *__restrict__ qkv, int64_t ld, const float *__restrict__ cosv,
@@ -117,6 +121,20 @@ struct Dec {
     static constexpr int kSmem = (kRing > kOut ? kRing : kOut) + (kDecMaxChunk / 8 + 1) * 4;
 };
 
+constexpr int kClusterMost = 8;
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+// The same place in the shared memory of the cluster's CTA `rank`.
+__device__ __forceinline__ float2 ld_cluster(const float2 *p, int rank) {
+    uint32_t at;
+    float2 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];\n" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+    return v;
+}
+
 struct DecodeArgs {
     const uint16_t *q, *kp, *vp;
     const int32_t *table, *seq_lens;
@@ -127,12 +145,16 @@ struct DecodeArgs {
     float *part;        // [b][h][chunk][m, l, HD] when n_chunks > 1
 };
 
-template <int HD>
+// Cluster: the chunks of a list are one cluster, which joins its own parts through its
+// shared memory (no second launch, no workspace). For calls that fit the GPU at once:
+// a CTA whose chunk the sequence does not reach stays for the join.
+template <int HD, bool Cluster>
 __global__ void __launch_bounds__(kDecWarps * 32)
 decode_split_kernel(const __grid_constant__ DecodeArgs P) {
     using C = Dec<HD>;
     extern __shared__ __align__(128) unsigned char dsm[];
     __shared__ float s_m[kDecWarps][kDecHeads], s_l[kDecWarps][kDecHeads];
+    __shared__ float2 s_part[kDecHeads];
     int32_t *s_page = reinterpret_cast<int32_t *>(dsm + C::kSmem - (kDecMaxChunk / 8 + 1) * 4);
     const int b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = P.H / P.Hk, groups = (G + kDecHeads - 1) / kDecHeads;
@@ -162,7 +184,7 @@ decode_split_kernel(const __grid_constant__ DecodeArgs P) {
     }
     const int64_t len = P.seq_lens[b];
     bool lost = len > P.max_len;
-    if (P.n_chunks > 1 && j0 > 0 && (j0 >= len || lost)) return;      // the join does not look
+    if (!Cluster && P.n_chunks > 1 && j0 > 0 && (j0 >= len || lost)) return;      // the join does not look
     const int n = lost ? 0 : static_cast<int>(max(min(len - j0, static_cast<int64_t>(P.chunk)), static_cast<int64_t>(0)));
     // one page outside the cache makes the sequence's result NaN
     const int pages = n > 0 ? ((off + n - 1) >> P.page_shift) + 1 : 0;
@@ -314,7 +336,11 @@ decode_split_kernel(const __grid_constant__ DecodeArgs P) {
         }
         if (lost) L = __int_as_float(0x7fc00000);
         const int64_t row = static_cast<int64_t>(b) * P.H + h0 + g;
-        if (P.n_chunks == 1) {
+        if constexpr (Cluster) {
+            // this CTA's part stays where warp 0's outputs were
+            *reinterpret_cast<float4 *>(s_o + g * HD + d) = o;
+            if (d == 0) s_part[g] = make_float2(M, L);
+        } else if (P.n_chunks == 1) {
             const float inv = L == 0.0f ? 0.0f : 1.0f / L;
             *reinterpret_cast<uint2 *>(P.out + row * HD + d) =
                 make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
@@ -323,6 +349,39 @@ decode_split_kernel(const __grid_constant__ DecodeArgs P) {
             *reinterpret_cast<float4 *>(dst + 4 + d) = o;
             if (d == 0) *reinterpret_cast<float2 *>(dst) = make_float2(M, L);
         }
+    }
+    if constexpr (Cluster) {
+        cluster_sync();
+        // pairs of columns, dealt out over the cluster's threads; parts in chunk order
+        const int ctas = P.n_chunks, me = static_cast<int>(blockIdx.x);
+        for (int e = me * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x); e < nh * (HD / 2);
+             e += ctas * static_cast<int>(blockDim.x)) {
+            const int g = e / (HD / 2), d = e % (HD / 2) * 2;
+            float2 ml[kClusterMost], x[kClusterMost];
+            float M = -INFINITY, L = 0.0f, o0 = 0.0f, o1 = 0.0f;
+#pragma unroll
+            for (int c = 0; c < kClusterMost; ++c) {
+                ml[c] = make_float2(-INFINITY, 0.0f);
+                x[c] = make_float2(0.0f, 0.0f);
+                if (c < ctas) {
+                    ml[c] = ld_cluster(&s_part[g], c);
+                    x[c] = ld_cluster(reinterpret_cast<const float2 *>(s_o + g * HD + d), c);
+                }
+                M = fmaxf(M, ml[c].x);
+            }
+#pragma unroll
+            for (int c = 0; c < kClusterMost; ++c) {
+                // a chunk whose maximum is -inf saw no key, or NaN alone (its sum says so)
+                const float f = ml[c].x == -INFINITY ? 0.0f : tc::ex2(ml[c].x - M);
+                L += ml[c].x == -INFINITY ? ml[c].y : f * ml[c].y;
+                o0 = fmaf(f, x[c].x, o0);
+                o1 = fmaf(f, x[c].y, o1);
+            }
+            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+            *reinterpret_cast<uint32_t *>(P.out + (static_cast<int64_t>(b) * P.H + h0 + g) * HD + d) =
+                pack_bf16x2(o0 * inv, o1 * inv);
+        }
+        cluster_sync();      // nobody leaves while its part is read
     }
 }
 
@@ -441,9 +500,63 @@ DecodeSplit decode_split(int64_t B, int64_t H, int64_t Hk, int64_t max_len) {
     const auto over = [&](int64_t ctas) { return (lists * max_len + ctas - 1) / ctas; };
     int64_t chunk = std::max(over(12 * 148), std::min<int64_t>(512, over(2 * 148)));
     chunk = std::min<int64_t>(std::max<int64_t>((chunk + 63) / 64 * 64, 64), kDecMaxChunk);
+    // few short lists: as one cluster each, of up to 8 chunks of up to 512 keys
+    if (lists * kClusterMost <= 2 * 148 && max_len <= kClusterMost * 512) {
+        chunk = std::max<int64_t>((max_len + kClusterMost - 1) / kClusterMost, 64);
+        chunk = (chunk + 63) / 64 * 64;
+        s.cluster = true;
+    }
     s.chunk = static_cast<int>(chunk);
     s.n_chunks = static_cast<int>(std::max<int64_t>(1, (max_len + s.chunk - 1) / s.chunk));
+    s.cluster = s.cluster && s.n_chunks > 1;
     return s;
+}
+
+template <int HD>
+static cudaError_t launch_decode(const DecodeArgs &p, const DecodeSplit &s, dim3 grid, int64_t rows, cudaStream_t st) {
+    constexpr int smem = Dec<HD>::kSmem;
+    static std::atomic<uint64_t> ready{0};      // devices whose kernels have their shared memory set
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+        if ((e = cudaFuncSetAttribute(decode_split_kernel<HD, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      smem)) != cudaSuccess ||
+            (e = cudaFuncSetAttribute(decode_split_kernel<HD, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      smem)) != cudaSuccess)
+            return e;
+        if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (s.cluster) {
+        cfg.gridDim = grid;
+        cfg.blockDim = dim3(kDecWarps * 32);
+        cfg.dynamicSmemBytes = smem;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = static_cast<unsigned>(s.n_chunks);
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        e = cudaLaunchKernelEx(&cfg, decode_split_kernel<HD, true>, p);
+        count_launch();
+        return e;
+    }
+    decode_split_kernel<HD, false><<<grid, kDecWarps * 32, smem, st>>>(p);
+    count_launch();
+    e = cudaGetLastError();
+    if (e != cudaSuccess || s.n_chunks == 1) return e;
+    // the join's launch overlaps the split's end; its threads wait for the parts
+    const bool few = s.n_chunks <= 2 || (s.n_chunks <= 16 && rows >= 1024);
+    cfg.gridDim = dim3(static_cast<unsigned>(few ? (rows + kJoinWarps - 1) / kJoinWarps : rows));
+    cfg.blockDim = dim3(kJoinWarps * 32);
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    e = few ? cudaLaunchKernelEx(&cfg, decode_join_kernel<HD, 1>, p, rows)
+            : cudaLaunchKernelEx(&cfg, decode_join_kernel<HD, 8>, p, rows);
+    count_launch();
+    return e;
 }
 
 cudaError_t launch_decode_attn(const void *q, int64_t q_ld, const void *kp, const void *vp, int64_t n_pages,
@@ -471,32 +584,7 @@ cudaError_t launch_decode_attn(const void *q, int64_t q_ld, const void *kp, cons
     p.scale_log2 = scale * kLog2e;
     p.out = static_cast<uint16_t *>(out);
     p.part = part;
-    auto go = [&](auto split, auto join, auto join_few, int smem) -> cudaError_t {
-        cudaError_t e = cudaFuncSetAttribute(split, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) return e;
-        split<<<grid, kDecWarps * 32, smem, st>>>(p);
-        count_launch();
-        e = cudaGetLastError();
-        if (e != cudaSuccess || s.n_chunks == 1) return e;
-        // the join's launch overlaps the split's end; its threads wait for the parts
-        cudaLaunchConfig_t cfg = {};
-        const int64_t rows = B * H;
-        const bool few = s.n_chunks <= 2 || (s.n_chunks <= 16 && rows >= 1024);
-        cfg.gridDim = dim3(static_cast<unsigned>(few ? (rows + kJoinWarps - 1) / kJoinWarps : rows));
-        cfg.blockDim = dim3(kJoinWarps * 32);
-        cfg.stream = st;
-        cudaLaunchAttribute attr;
-        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr.val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
-        e = few ? cudaLaunchKernelEx(&cfg, join_few, p, rows) : cudaLaunchKernelEx(&cfg, join, p, rows);
-        count_launch();
-        return e;
-    };
-    return hd == 64 ? go(decode_split_kernel<64>, decode_join_kernel<64, 8>, decode_join_kernel<64, 1>, Dec<64>::kSmem)
-                    : go(decode_split_kernel<128>, decode_join_kernel<128, 8>, decode_join_kernel<128, 1>,
-                         Dec<128>::kSmem);
+    return hd == 64 ? launch_decode<64>(p, s, grid, B * H, st) : launch_decode<128>(p, s, grid, B * H, st);
 }
 
 }  // namespace mom
