@@ -1,7 +1,34 @@
-// Causal attention over packed prompts: sequences of different lengths one after
-// another in q (Tq, H, hd) and k, v (Tk, Hk, hd), query head h on key head
-// h / (H / Hk), the mask aligned at each sequence's end (row r of a sequence of
-// Lq queries and Lk keys sees keys 0 .. Lk - Lq + r).
+// Causal attention over packed prompts on the 5th-generation tensor cores: sequences
+// of different lengths one after another in q (Tq, H, hd) and k, v (Tk, Hk, hd), query
+// head h on key head h / (H / Hk), the mask aligned at each sequence's end (row r of a
+// sequence of Lq queries and Lk keys sees keys 0 .. Lk - Lq + r).
+//
+//   O[r] = sum_j 2^(x_rj - m_r) v_j / sum_j 2^(x_rj - m_r),  x = (scale log2 e) q . k
+//
+// in one pass over the keys: m is the row's running maximum, and O and the sum are
+// rescaled only when it has grown by more than 2^8 (the weights then stay below 2^8,
+// exact enough in bf16, whose relative step does not depend on their size; the sum is
+// fp32). The weights are rounded to bf16 for the second product, as its operand type
+// asks; the output is rounded once.
+//
+// A CTA works on two halves of 128 rows that share their keys: two heads of a group
+// where the group is even (the halves then see the same keys and a tile of 128 rows
+// wastes less on short sequences), else 256 rows of a head. Per half a softmax
+// warpgroup (one row a thread: no exchange between threads) and an issuing thread; one
+// loader (K and V tiles of 128 keys through a ring, TMA), one epilogue warpgroup an
+// item behind. Tensor memory is full at head_dim 128 (two S, two O of 128 columns).
+//
+// What bounds it, 148 SMs, B200: head_dim 128 the chain softmax - product with V -
+// scores of the next tile of a half, under which the other half's is laid (a step of
+// both halves takes about 2900 cycles; their products alone 2048): 8 sequences of 2048,
+// 16 heads on 4, 139 us, 990 TFLOP/s of the causal half's flops, tensor pipe 49 % busy;
+// one of 16384 868 us, 1.27 PFLOP/s (under a lasting load 1005 us: the power limit takes
+// the clock from 1.9 to 1.6 GHz). head_dim 64 has half the products for the same
+// exponentials: bound by the special-function unit (62 %) and what the softmax waits
+// for: 8 of 2048, 16 heads, 116 us, 594 TFLOP/s. Also tried: exponentials partly on the
+// FMA pipe (no gain while the halves take turns; -2 % at head_dim 64), two softmax
+// warps a row (more exchange than it hides: 717 against 711 us at 16384, head_dim 64),
+// items handed out at run time (the waits for them cost more than their balance gave).
 //
 // The plan lists tiles of up to kPromptRows query rows and the work of each CTA.
 #include <algorithm>
