@@ -908,8 +908,8 @@ int mom_rope_append(const void *qkv, int64_t qkv_ld, const float *cosv, const fl
 
 size_t mom_decode_attn_workspace_size(int64_t B, int64_t H, int64_t Hk, int64_t hd, int64_t max_len) {
     if (B <= 0 || H <= 0 || Hk <= 0 || hd <= 0 || max_len <= 0) return 0;
-    const mom::DecodeSplit s = mom::decode_split(B, H, Hk, max_len);
-    return s.n_chunks == 1 || s.cluster ? 0 : static_cast<size_t>(B) * H * s.n_chunks * (hd + 4) * sizeof(float);
+    const mom::DecodeSplit s = mom::decode_split(B, H, Hk, hd, max_len);
+    return s.bytes(H, Hk, hd);
 }
 
 int mom_decode_attn(const void *q, int64_t q_ld, const void *k_pages, const void *v_pages, int64_t num_pages,
@@ -921,6 +921,8 @@ int mom_decode_attn(const void *q, int64_t q_ld, const void *k_pages, const void
     if ((rc = check_cache_geometry(num_pages, page_size))) return rc;
     MOM_REQUIRE(B >= 0 && B <= 65535, "B must be in [0, 65535] (got %lld)", (long long)B);
     MOM_REQUIRE(max_len >= 0 && max_len <= INT32_MAX, "max_len out of range");
+    MOM_REQUIRE(B * H <= (1 << 30) && B * H * (max_len / 16 + 8) <= (int64_t(1) << 40),
+                "too many sequences, heads and keys (2^30, 2^44)");
     MOM_REQUIRE(table_ld >= 0 && max_len <= table_ld * page_size, "max_len exceeds the block table (%lld pages of %lld)",
                 (long long)table_ld, (long long)page_size);
     MOM_REQUIRE(q_ld >= H * hd && q_ld % 8 == 0, "q row pitch must hold all heads and be a multiple of 8");

@@ -6,6 +6,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 namespace mom {
 
 // Kernels launched by this library since it was loaded (all devices/threads).
@@ -223,18 +225,25 @@ int device_sm_count();
 
 // Serving (serve.cu): rotary embedding by explicit positions of a fused projection's
 // heads with the cache write, and one new token's attention over paged K / V
-// (n_pages, Hk, 1 << page_shift, hd) bf16. `part` holds the chunks' partial sums:
-// decode_split says how many chunks a call of these sizes takes.
+// (n_pages, Hk, 1 << page_shift, hd) bf16. `part` holds the partial sums
+// of a call's parts and where lists are cut (DecodeSplit::bytes).
 cudaError_t launch_rope_append(const void *qkv, int64_t ld, const float *cosv, const float *sinv, int64_t n_pos,
                                const void *positions, int pos64, const void *slots, int slot64, int64_t T, int H,
                                int Hk, int hd, int64_t n_pages, int page_shift, void *kp, void *vp, void *q, void *k,
                                cudaStream_t st);
 struct DecodeSplit {
-    int chunk = 0;      // keys of a chunk
-    int n_chunks = 1;   // chunks of the longest sequence the call may hold
-    bool cluster = false;   // the chunks join themselves: no parts in memory
+    bool cluster = false;       // a list (a sequence's key head) is one cluster of chunks that join themselves
+    int chunk = 0, n_chunks = 1;
+    int64_t ctas = 0, lists = 0;        // else: spans of the lists' tiles, one after another, for so many CTAs
+    static int heads(int64_t H, int64_t Hk) { return static_cast<int>(std::min<int64_t>(H / std::max<int64_t>(Hk, 1), 16)); }
+    size_t part_floats(int64_t H, int64_t Hk, int64_t hd) const {
+        return static_cast<size_t>(ctas + lists) * heads(H, Hk) * (hd + 4);
+    }
+    size_t bytes(int64_t H, int64_t Hk, int64_t hd) const {
+        return cluster ? 0 : part_floats(H, Hk, hd) * sizeof(float) + static_cast<size_t>(std::min(ctas, lists)) * 8;
+    }
 };
-DecodeSplit decode_split(int64_t B, int64_t H, int64_t Hk, int64_t max_len);
+DecodeSplit decode_split(int64_t B, int64_t H, int64_t Hk, int64_t hd, int64_t max_len);
 cudaError_t launch_decode_attn(const void *q, int64_t q_ld, const void *kp, const void *vp, int64_t n_pages,
                                int page_shift, const int32_t *table, int64_t table_ld, const int32_t *seq_lens,
                                int64_t max_len, int64_t B, int H, int Hk, int hd, float scale, void *out, float *part,

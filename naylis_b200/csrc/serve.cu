@@ -95,32 +95,39 @@ rope_append_kernel(const uint16_t *__restrict__ qkv, int64_t ld, const float *__
 // ------------------------------------------------------------------ decode attention
 // out[b, h] = sum_j softmax_j(scale q . k_j) v_j over the sequence's seq_lens[b] keys.
 //
-// Bound by reading the cache once. A CTA takes a chunk of one sequence's keys for the
-// (up to 16) query heads that share a key head, so that a key is read once for all of
-// them; its warps take tiles of 16 keys in turn, each through a ring of its own in
-// shared memory (16-byte asynchronous copies, kStages tiles ahead, no barrier between
-// warps), and keep a running maximum, sum and output per head. Scores and outputs are
-// m16n8k16 products with the heads as rows: at one query per sequence the tensor pipe
-// is idle whatever the shape, and one instruction serves 1 to 16 heads alike. The
-// weights enter as two bf16 terms (p = hi + lo), which the idle pipe gives for free:
-// the result is rounded once. Rows behind the sequence's end are zero-filled by the
-// copy, so stale pages never reach a product. 64 sequences of 8192, 32 heads on 8 of 128:
-// 325 us, 6.6 TB/s; 4 of 87000 to 131072, 16 heads on 4: 143 us, 6.2 TB/s; 48 of 64 to
-// 4096, 16 heads of 64: 45 us, 4.3 TB/s (bound by the longest sequences' last chunks).
+// Bound by reading the cache once. A list is a sequence's key head with the (up to 16)
+// query heads that share it, so that a key is read once for all of them. The lists' tiles
+// of 16 keys, one list after another, are cut into one span for each CTA that fits the GPU;
+// only the device knows the lengths, so each CTA finds its span from their running sum. A
+// CTA's warps take its tiles in turn, each through a ring of its own in shared memory
+// (16-byte asynchronous copies, kStages tiles ahead whatever list they are of, no barrier
+// between warps), and keep a running maximum, sum and output per head until the list ends.
+// Scores and outputs are m16n8k16 products with the heads as rows: at one query per
+// sequence the tensor pipe is idle whatever the shape, and one instruction serves 1 to 16
+// heads alike. The weights enter as two bf16 terms (p = hi + lo), which the idle pipe gives
+// for free: the result is rounded once. Rows behind the sequence's end are zero-filled by
+// the copy, so stale pages never reach a product. With the join: 64 sequences of 8192, 32
+// heads on 8 of 128: 316 us, 6.8 TB/s (326 with a CTA for each chunk of a list); 4 of 87000 to
+// 131072, 16 heads on 4: 135 us, 6.6 TB/s (143); 128 of 1024, 32 on 8: 91 us, 5.9 TB/s (99);
+// 48 of 64 to 4096, 16 heads of 64: 43 us, 4.5 TB/s (46): the spans begin to read after 3.5 us
+// and end after 30 to 40, an SM's first CTA before its fourth (further, shorter spans for
+// the SMs that are done first: 47 to 52; spans after the CTA's place: 46).
 constexpr int kDecWarps = 4;
 constexpr int kDecTile = 16;                      // keys of a warp's step
 constexpr int kDecHeads = 16;                     // query heads of a CTA
-constexpr int kDecMaxChunk = 4096;                // keys of a CTA
+constexpr int kDecLeast = 8;                      // tiles of a CTA's span, at least
+// tiles that a list's start and end cost (48 sequences of 64 to 4096: 43 us with 6, 47 with 3, 44 with 10)
+constexpr int kDecListCost = 6;
 
 template <int HD>
 struct Dec {
     static constexpr int kStages = 3;
+    static constexpr int kCtas = HD == 64 ? 4 : 2;    // resident on an SM
     static constexpr int kRowBytes = HD * 2;
     static constexpr int kTileBytes = kDecTile * kRowBytes;
     static constexpr int kRing = kDecWarps * kStages * 2 * kTileBytes;
-    // the ring, later the warps' outputs [warp][16][HD] fp32
-    static constexpr int kOut = kDecWarps * kDecHeads * HD * 4;
-    static constexpr int kSmem = (kRing > kOut ? kRing : kOut) + (kDecMaxChunk / 8 + 1) * 4;
+    // the warps' outputs, four heads at a time: [warp][4][HD] fp32
+    static constexpr int kSmem = kRing + kDecWarps * 4 * HD * 4;
 };
 
 constexpr int kClusterMost = 8;
@@ -140,42 +147,195 @@ __device__ __forceinline__ float2 ld_cluster(const float2 *p, int rank) {
 struct DecodeArgs {
     const uint16_t *q, *kp, *vp;
     const int32_t *table, *seq_lens;
-    int64_t q_ld, table_ld, n_pages, max_len;
-    int H, Hk, page_shift, chunk, n_chunks;
+    int64_t q_ld, table_ld, n_pages, max_len, B;
+    int H, Hk, page_shift, n_chunks, chunk;     // n_chunks, chunk (keys): a cluster's
     float scale_log2;
     uint16_t *out;
-    float *part;        // [b][h][chunk][m, l, HD] when n_chunks > 1
+    float *part;        // [part][head of the CTA][m, l, -, -, HD]
+    int2 *cut;          // where lists are cut, by the smaller of the two: [list] its first CTA and its number of
+                        // CTAs, or [CTA] the list that begins in its span and ends behind it, and its number
+    bool by_list;
 };
+
+// A sequence's keys as the kernels take them, and its tiles: one without keys for a
+// sequence without (its output is zero) and for one that is too long (NaN).
+struct DecLen {
+    int n, tiles;
+    bool lost;
+    __device__ __forceinline__ DecLen(int32_t len, int64_t max_len) {
+        lost = len > max_len;
+        n = lost || len < 0 ? 0 : len;
+        tiles = max(static_cast<int>((static_cast<unsigned>(n) + kDecTile - 1) / kDecTile), 1);
+    }
+};
+
+// The work of all lists (a sequence's key head), one after another, cut into equal spans
+// for the grid's CTAs. It is counted in tiles, and a list's start and end as kDecListCost
+// of them ahead of its own. Where span blockIdx.x begins:
+struct DecSpan {
+    int64_t base, span;          // units before the list that it begins in, and units of a span
+    int b, y, i, n;              // sequence, list of it, tile of that, the sequence's length
+    int end;                     // the span's end, in units from base
+};
+__device__ __forceinline__ bool decode_span(const DecodeArgs &P, int lists, DecSpan &got) {
+    __shared__ int64_t s_sum[kDecWarps];
+    __shared__ DecSpan s_got;
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+    const int per = static_cast<int>((P.B + kDecWarps * 32 - 1) / (kDecWarps * 32));      // sequences of a thread
+    const int64_t b0 = static_cast<int64_t>(t) * per, b1 = min(b0 + per, P.B);
+    int64_t mine = 0;
+    for (int64_t b = b0; b < b1; ++b) mine += DecLen(P.seq_lens[b], P.max_len).tiles + kDecListCost;
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+    }
+    if (lane == 31) s_sum[warp] = upto;
+    __syncthreads();
+    int64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < kDecWarps; ++w) {
+        if (w < warp) upto += s_sum[w];
+        total += s_sum[w];
+    }
+    total *= lists;
+    const int64_t span = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(kDecLeast));
+    const int64_t from = blockIdx.x * span;
+    if (from >= total) return false;
+    int64_t base = (upto - mine) * lists;
+    if (from >= base && from < upto * lists) {
+        for (int64_t b = b0; b < b1; ++b) {
+            const int32_t len = P.seq_lens[b];
+            const int units = DecLen(len, P.max_len).tiles + kDecListCost;
+            const int64_t next = base + static_cast<int64_t>(units) * lists;
+            if (from < next) {
+                const int y = static_cast<int>((from - base) / units);
+                base += static_cast<int64_t>(y) * units;
+                s_got = {base, span, static_cast<int>(b), y, max(static_cast<int>(from - base) - kDecListCost, 0), len,
+                         static_cast<int>(min(from + span, total) - base)};
+                break;
+            }
+            base = next;
+        }
+    }
+    __syncthreads();
+    got = s_got;
+    return true;
+}
 
 // Cluster: the chunks of a list are one cluster, which joins its own parts through its
 // shared memory (no second launch, no workspace). For calls that fit the GPU at once:
 // a CTA whose chunk the sequence does not reach stays for the join.
 template <int HD, bool Cluster>
-__global__ void __launch_bounds__(kDecWarps * 32)
+__global__ void __launch_bounds__(kDecWarps * 32, Dec<HD>::kCtas)
 decode_split_kernel(const __grid_constant__ DecodeArgs P) {
     using C = Dec<HD>;
     extern __shared__ __align__(128) unsigned char dsm[];
     __shared__ float s_m[kDecWarps][kDecHeads], s_l[kDecWarps][kDecHeads];
     __shared__ float2 s_part[kDecHeads];
-    int32_t *s_page = reinterpret_cast<int32_t *>(dsm + C::kSmem - (kDecMaxChunk / 8 + 1) * 4);
-    const int b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int G = P.H / P.Hk, groups = (G + kDecHeads - 1) / kDecHeads;
-    const int hk = blockIdx.y / groups, g0 = blockIdx.y % groups * kDecHeads, nh = min(kDecHeads, G - g0);
-    const int h0 = hk * G + g0;
-    const int64_t j0 = static_cast<int64_t>(blockIdx.x) * P.chunk;
+    float *s_o = reinterpret_cast<float *>(dsm + C::kRing);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int G = P.H / P.Hk, groups = (G + kDecHeads - 1) / kDecHeads, lists = P.Hk * groups;
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-    // length, pages and queries are on their way together: the pages up to max_len are
-    // read before the length is known
-    const int page_mask = (1 << P.page_shift) - 1, off = static_cast<int>(j0) & page_mask;
-    const int most = static_cast<int>(min(P.max_len - j0, static_cast<int64_t>(P.chunk)));
-    const int pages_most = most > 0 ? ((off + most - 1) >> P.page_shift) + 1 : 0;
-    const int32_t *row = P.table + b * P.table_ld + (j0 >> P.page_shift);
-    const int32_t page0 = static_cast<int>(threadIdx.x) < pages_most ? row[threadIdx.x] : 0;
+    DecSpan at;
+    if constexpr (Cluster) {
+        const int first = static_cast<int>(blockIdx.x) * P.chunk / kDecTile;
+        at = {0, 0, static_cast<int>(blockIdx.z), static_cast<int>(blockIdx.y), first, P.seq_lens[blockIdx.z],
+              first + P.chunk / kDecTile + kDecListCost};
+    } else if (!decode_span(P, lists, at)) {
+        if (threadIdx.x == 0 && !P.by_list) P.cut[blockIdx.x] = make_int2(0, 0);
+        return;
+    }
+    DecLen len(at.n, P.max_len);
+    // the tiles of a list that are before the span's end
+    const int end = at.end;
+    const auto tiles_to = [&](int base, int tiles) { return max(min(tiles, end - base - kDecListCost), 0); };
+
+    // The copies' side of this warp: it takes every fourth tile of the span, whatever list
+    // it is of. The page numbers of a tile are read while the copies of the one before it
+    // are issued. A tile starts at a multiple of 16 keys: it lies in one page, or in two of
+    // 8. A page outside the cache copies nothing and makes the sequence's result NaN.
+    const uint32_t ring = smem_u32(dsm) + warp * C::kStages * 2 * C::kTileBytes;
+    constexpr int kLanes = HD / 8;                // lanes of a row
+    constexpr int kRowsPer = 32 / kLanes;         // rows of one copy instruction
+    const int chunk_col = lane % kLanes, row0 = lane / kLanes;
+    const int page_mask = (1 << P.page_shift) - 1;
+    int fbase = 0, fb = at.b, fy = at.y, fhk = fy / groups, fi = at.i, fn = len.n, fall = len.tiles;
+    int fend = tiles_to(fbase, fall);
+    int32_t flen = !Cluster && fb + 1 < P.B ? P.seq_lens[fb + 1] : 0;      // the next sequence's
+    struct Tile {
+        int32_t page[2];
+        int rows, in_page, hk;      // rows: of the sequence; < 0: no tile
+    };
+    bool more = true, bad[C::kStages] = {};
+    auto look = [&](int step) {
+        Tile tile = {{0, 0}, -1, 0, 0};
+        if (!more) return tile;
+        fi += step;
+        while (fi >= fend) {
+            fi -= fend;
+            fbase += fall + kDecListCost;
+            if (Cluster || fbase + kDecListCost >= end) {
+                more = false;
+                return tile;
+            }
+            if (++fy == lists) {
+                fy = 0;
+                ++fb;
+                const DecLen next(flen, P.max_len);
+                fn = next.n, fall = next.tiles;
+                flen = fb + 1 < P.B ? P.seq_lens[fb + 1] : 0;
+            }
+            fhk = fy / groups;
+            fend = tiles_to(fbase, fall);
+        }
+        tile.rows = min(fn - fi * kDecTile, kDecTile);
+        tile.in_page = (fi * kDecTile) & page_mask;
+        tile.hk = fhk;
+        if (tile.rows > 0) {
+            const int32_t *row = P.table + fb * P.table_ld;
+            const int64_t j = static_cast<int64_t>(fi) * kDecTile;
+            tile.page[0] = row[j >> P.page_shift];
+            tile.page[1] = tile.rows > 8 ? row[(j + 8) >> P.page_shift] : tile.page[0];
+        }
+        return tile;
+    };
+    auto fetch = [&](int stage, const Tile &tile) {
+        if (tile.rows >= 0) {
+            const uint32_t sk = ring + stage * 2 * C::kTileBytes, sv = sk + C::kTileBytes;
+            const bool out = tile.rows > 0 && (tile.page[0] < 0 || tile.page[0] >= P.n_pages || tile.page[1] < 0 ||
+                                               tile.page[1] >= P.n_pages);
+#pragma unroll
+            for (int e = 0; e < C::kStages; ++e)
+                if (e == stage) bad[e] = out;
+#pragma unroll
+            for (int u = 0; u < kDecTile / kRowsPer; ++u) {
+                const int r = row0 + u * kRowsPer;
+                const bool in = !out && r < tile.rows;
+                const int64_t from = (((static_cast<int64_t>(tile.page[r >> 3]) * P.Hk + tile.hk) << P.page_shift) +
+                                      ((tile.in_page + r) & page_mask)) * HD + chunk_col * 8;
+                const uint32_t dst = swz(r, chunk_col, C::kRowBytes);
+                cp_async16(sk + dst, in ? P.kp + from : P.q, in ? 16 : 0);      // zeros behind the end
+                cp_async16(sv + dst, in ? P.vp + from : P.q, in ? 16 : 0);
+            }
+        }
+        cp_async_commit();
+    };
+    int head = 0;
+    static_assert(C::kStages == 3);
+    const Tile tile0 = look(warp), tile1 = look(kDecWarps);      // both tables' reads under way together
+    fetch(0, tile0);
+    fetch(1, tile1);
+    Tile tile = look(kDecWarps);
+
+    // The products' side, list by list.
+    int b = at.b, y = at.y, i0 = at.i, taken = 0;
     // queries: row lane / 4 (+ 8), dimensions 16 kk + 2 (lane % 4) (+ 8)
     uint32_t qa[HD / 16][4];
-    {
-        const int r = lane >> 2, d = 2 * (lane & 3);
-        const uint16_t *q0 = P.q + b * P.q_ld + static_cast<int64_t>(h0 + r) * HD + d;
+    auto queries = [&](int qb, int qy) {
+        const int r = lane >> 2, d = 2 * (lane & 3), g0 = qy % groups * kDecHeads, nh = min(kDecHeads, G - g0);
+        const uint16_t *q0 = P.q + qb * P.q_ld + static_cast<int64_t>(qy / groups * G + g0 + r) * HD + d;
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk)
 #pragma unroll
@@ -183,54 +343,25 @@ decode_split_kernel(const __grid_constant__ DecodeArgs P) {
                 qa[kk][e] = r + 8 * (e & 1) < nh
                                 ? *reinterpret_cast<const uint32_t *>(q0 + 8 * (e & 1) * HD + 16 * kk + 8 * (e >> 1))
                                 : 0u;
-    }
-    const int64_t len = P.seq_lens[b];
-    bool lost = len > P.max_len;
-    if (!Cluster && P.n_chunks > 1 && j0 > 0 && (j0 >= len || lost)) return;      // the join does not look
-    const int n = lost ? 0 : static_cast<int>(max(min(len - j0, static_cast<int64_t>(P.chunk)), static_cast<int64_t>(0)));
-    // one page outside the cache makes the sequence's result NaN
-    const int pages = n > 0 ? ((off + n - 1) >> P.page_shift) + 1 : 0;
-    for (int i = threadIdx.x; i < pages; i += blockDim.x) {
-        const int32_t p = i == static_cast<int>(threadIdx.x) ? page0 : row[i];
-        if (p < 0 || p >= P.n_pages) lost = true;
-        s_page[i] = p;
-    }
-    lost = __syncthreads_or(lost);
-
-    float acc[HD / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    };
+    queries(b, y);
+    int2 cut = make_int2(0, 0);
+    for (int base = 0; Cluster || base + kDecListCost < end;) {
+        const int g0 = y % groups * kDecHeads, nh = min(kDecHeads, G - g0), h0 = y / groups * G + g0;
+        const int tiles = tiles_to(base, len.tiles) - i0;
+        bool lost = len.lost;
+        float acc[HD / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < HD / 8; ++i)
+        for (int i = 0; i < HD / 8; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][e] = 0.0f;
-    const int tiles = lost ? 0 : (n + kDecTile - 1) / kDecTile;
-    if (warp < tiles) {
-        const uint32_t ring = smem_u32(dsm) + warp * C::kStages * 2 * C::kTileBytes;
-        constexpr int kLanes = HD / 8;                // lanes of a row
-        constexpr int kRowsPer = 32 / kLanes;         // rows of one copy instruction
-        const int chunk_col = lane % kLanes, row0 = lane / kLanes;
-        auto fetch = [&](int i, int stage) {
-            if (i < tiles) {
-                const uint32_t sk = ring + stage * 2 * C::kTileBytes, sv = sk + C::kTileBytes;
-#pragma unroll
-                for (int u = 0; u < kDecTile / kRowsPer; ++u) {
-                    const int row = row0 + u * kRowsPer, j = i * kDecTile + row;
-                    const bool in = j < n;
-                    const int jc = off + (in ? j : 0);
-                    const int64_t at = (((static_cast<int64_t>(s_page[jc >> P.page_shift]) * P.Hk + hk) << P.page_shift) +
-                                        (jc & page_mask)) * HD + chunk_col * 8;
-                    const uint32_t dst = swz(row, chunk_col, C::kRowBytes);
-                    cp_async16(sk + dst, P.kp + at, in ? 16 : 0);
-                    cp_async16(sv + dst, P.vp + at, in ? 16 : 0);
-                }
-            }
-            cp_async_commit();
-        };
-        int head = 0;
-#pragma unroll
-        for (int s = 0; s < C::kStages - 1; ++s) fetch(warp + s * kDecWarps, s);
-        for (int i = warp; i < tiles; i += kDecWarps) {
+            for (int e = 0; e < 4; ++e) acc[i][e] = 0.0f;
+        for (int i = (warp - taken) & (kDecWarps - 1); i < tiles; i += kDecWarps) {
             cp_async_wait<C::kStages - 2>();
             __syncwarp();
+#pragma unroll
+            for (int e = 0; e < C::kStages; ++e)
+                if (e == head) lost |= bad[e];
+            const int n = len.n - (i0 + i) * kDecTile;
             const uint32_t sk = ring + head * 2 * C::kTileBytes, sv = sk + C::kTileBytes;
             float s[2][4] = {};
 #pragma unroll
@@ -242,12 +373,12 @@ decode_split_kernel(const __grid_constant__ DecodeArgs P) {
             }
             float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const bool in = i * kDecTile + 8 * t + 2 * (lane & 3) + (e & 1) < n;
-                    s[t][e] = in ? s[t][e] * P.scale_log2 : -INFINITY;
-                    mx[e >> 1] = fmaxf(mx[e >> 1], s[t][e]);
+                    const bool in = 8 * u + 2 * (lane & 3) + (e & 1) < n;
+                    s[u][e] = in ? s[u][e] * P.scale_log2 : -INFINITY;
+                    mx[e >> 1] = fmaxf(mx[e >> 1], s[u][e]);
                 }
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
@@ -270,15 +401,15 @@ decode_split_kernel(const __grid_constant__ DecodeArgs P) {
             }
             uint32_t hi[4], lo[4];
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     const float ref = m[r] == -INFINITY ? 0.0f : m[r];
-                    const float p0 = tc::ex2(s[t][2 * r] - ref), p1 = tc::ex2(s[t][2 * r + 1] - ref);
+                    const float p0 = tc::ex2(s[u][2 * r] - ref), p1 = tc::ex2(s[u][2 * r + 1] - ref);
                     l[r] += p0 + p1;
                     const uint32_t h = pack_bf16x2(p0, p1);
-                    hi[2 * t + r] = h;
-                    lo[2 * t + r] = pack_bf16x2(p0 - __uint_as_float(h << 16), p1 - __uint_as_float(h & 0xffff0000u));
+                    hi[2 * u + r] = h;
+                    lo[2 * u + r] = pack_bf16x2(p0 - __uint_as_float(h << 16), p1 - __uint_as_float(h & 0xffff0000u));
                 }
 #pragma unroll
             for (int d = 0; d < HD / 16; ++d) {
@@ -290,72 +421,103 @@ decode_split_kernel(const __grid_constant__ DecodeArgs P) {
                 mma_bf16_16816(acc[2 * d + 1], lo, vb[2], vb[3]);
             }
             __syncwarp();      // the stage that the next copy overwrites has been read
-            const int ahead = i + (C::kStages - 1) * kDecWarps;
-            fetch(ahead, head == 0 ? C::kStages - 1 : head - 1);
+            fetch(head == 0 ? C::kStages - 1 : head - 1, tile);
+            tile = look(kDecWarps);
             head = head + 1 == C::kStages ? 0 : head + 1;
         }
-        cp_async_wait<0>();
-    }
 
-    // join the warps: their maxima and sums, then the outputs through the ring's memory
+        // the next list, and its queries on their way
+        const int next = base + len.tiles + kDecListCost;
+        int32_t blen = 0;
+        int ny = y + 1, nb = b;
+        if (ny == lists) ny = 0, ++nb;
+        if (!Cluster && next + kDecListCost < end) {
+            queries(nb, ny);
+            if (nb != b) blen = P.seq_lens[nb];
+        }
+
+        // join the warps: their maxima and sums, then the outputs of four heads at a time
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-        if ((lane & 3) == 0) {
-            s_m[warp][(lane >> 2) + 8 * r] = m[r];
-            s_l[warp][(lane >> 2) + 8 * r] = l[r];
+        for (int r = 0; r < 2; ++r) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+            if ((lane & 3) == 0) {
+                s_m[warp][(lane >> 2) + 8 * r] = m[r];
+                s_l[warp][(lane >> 2) + 8 * r] = l[r];
+            }
+        }
+        lost = __syncthreads_or(lost);
+        const int64_t list = static_cast<int64_t>(b) * lists + y;
+        const bool whole = i0 == 0 && tiles == len.tiles;
+#pragma unroll
+        for (int p = 0; p < kDecHeads / 4; ++p) {
+            if (4 * p >= nh) break;
+            const int r = p >> 1, g = (lane >> 2) + 8 * r;
+            if (g >> 2 == p && g < nh) {
+                float M = s_m[0][g];
+#pragma unroll
+                for (int w = 1; w < kDecWarps; ++w) M = fmaxf(M, s_m[w][g]);
+                const float f = m[r] == -INFINITY ? 0.0f : tc::ex2(m[r] - M);
+#pragma unroll
+                for (int d = 0; d < HD / 8; ++d)
+                    *reinterpret_cast<float2 *>(s_o + (warp * 4 + (g & 3)) * HD + 8 * d + 2 * (lane & 3)) =
+                        make_float2(acc[d][2 * r] * f, acc[d][2 * r + 1] * f);
+            }
+            __syncthreads();
+            const int left = min(nh - 4 * p, 4) * (HD / 4);
+            for (int e = threadIdx.x; e < left; e += blockDim.x) {
+                const int g = 4 * p + e / (HD / 4), d = e % (HD / 4) * 4;
+                float M = s_m[0][g], L = 0.0f;
+#pragma unroll
+                for (int w = 1; w < kDecWarps; ++w) M = fmaxf(M, s_m[w][g]);
+                float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int w = 0; w < kDecWarps; ++w) {
+                    // a warp whose maximum is -inf saw nothing, or NaN alone
+                    L += s_m[w][g] == -INFINITY ? s_l[w][g] : s_l[w][g] * tc::ex2(s_m[w][g] - M);
+                    const float4 x = *reinterpret_cast<const float4 *>(s_o + (w * 4 + (g & 3)) * HD + d);
+                    o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+                }
+                if (lost) L = __int_as_float(0x7fc00000);
+                if constexpr (Cluster) {
+                    // this CTA's part stays where the ring was
+                    *reinterpret_cast<float4 *>(reinterpret_cast<float *>(dsm) + g * HD + d) = o;
+                    if (d == 0) s_part[g] = make_float2(M, L);
+                } else if (whole) {
+                    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+                    *reinterpret_cast<uint2 *>(P.out + (static_cast<int64_t>(b) * P.H + h0 + g) * HD + d) =
+                        make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+                } else {
+                    // a CTA and a list that follow one another in the order of tiles: no two
+                    // parts have the same sum
+                    float *dst = P.part + ((blockIdx.x + list) * min(G, kDecHeads) + g) * (HD + 4);
+                    *reinterpret_cast<float4 *>(dst + 4 + d) = o;
+                    if (d == 0) *reinterpret_cast<float2 *>(dst) = make_float2(M, L);
+                }
+            }
+            __syncthreads();
+        }
+        if constexpr (Cluster) break;
+        if (i0 == 0 && threadIdx.x == 0) {
+            const int n = static_cast<int>((at.base + next - 1) / at.span) - static_cast<int>(blockIdx.x) + 1;
+            if (P.by_list) P.cut[list] = make_int2(blockIdx.x, n);
+            else if (n > 1) cut = make_int2(static_cast<int>(list), n);
+        }
+        taken += tiles;
+        base = next;
+        i0 = 0;
+        y = ny;
+        if (nb != b) {
+            b = nb;
+            len = DecLen(blen, P.max_len);
         }
     }
-    __syncthreads();
-    float *s_o = reinterpret_cast<float *>(dsm);
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        const int g = (lane >> 2) + 8 * r;
-        if (g >= nh) continue;
-        float M = s_m[0][g];
-#pragma unroll
-        for (int w = 1; w < kDecWarps; ++w) M = fmaxf(M, s_m[w][g]);
-        const float f = m[r] == -INFINITY ? 0.0f : tc::ex2(m[r] - M);
-#pragma unroll
-        for (int d = 0; d < HD / 8; ++d)
-            *reinterpret_cast<float2 *>(s_o + (warp * kDecHeads + g) * HD + 8 * d + 2 * (lane & 3)) =
-                make_float2(acc[d][2 * r] * f, acc[d][2 * r + 1] * f);
-    }
-    __syncthreads();
-    for (int e = threadIdx.x; e < nh * (HD / 4); e += blockDim.x) {
-        const int g = e / (HD / 4), d = e % (HD / 4) * 4;
-        float M = s_m[0][g], L = 0.0f;
-#pragma unroll
-        for (int w = 1; w < kDecWarps; ++w) M = fmaxf(M, s_m[w][g]);
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int w = 0; w < kDecWarps; ++w) {
-            // a warp whose maximum is -inf saw nothing, or NaN alone
-            L += s_m[w][g] == -INFINITY ? s_l[w][g] : s_l[w][g] * tc::ex2(s_m[w][g] - M);
-            const float4 x = *reinterpret_cast<const float4 *>(s_o + (w * kDecHeads + g) * HD + d);
-            o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
-        }
-        if (lost) L = __int_as_float(0x7fc00000);
-        const int64_t row = static_cast<int64_t>(b) * P.H + h0 + g;
-        if constexpr (Cluster) {
-            // this CTA's part stays where warp 0's outputs were
-            *reinterpret_cast<float4 *>(s_o + g * HD + d) = o;
-            if (d == 0) s_part[g] = make_float2(M, L);
-        } else if (P.n_chunks == 1) {
-            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-            *reinterpret_cast<uint2 *>(P.out + row * HD + d) =
-                make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
-        } else {
-            float *dst = P.part + (row * P.n_chunks + blockIdx.x) * (HD + 4);
-            *reinterpret_cast<float4 *>(dst + 4 + d) = o;
-            if (d == 0) *reinterpret_cast<float2 *>(dst) = make_float2(M, L);
-        }
-    }
+    if (!Cluster && threadIdx.x == 0 && !P.by_list) P.cut[blockIdx.x] = cut;
     if constexpr (Cluster) {
         cluster_sync();
         // pairs of columns, dealt out over the cluster's threads; parts in chunk order
         const int ctas = P.n_chunks, me = static_cast<int>(blockIdx.x);
+        const int g0 = y % groups * kDecHeads, nh = min(kDecHeads, G - g0), h0 = y / groups * G + g0;
         for (int e = me * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x); e < nh * (HD / 2);
              e += ctas * static_cast<int>(blockDim.x)) {
             const int g = e / (HD / 2), d = e % (HD / 2) * 2;
@@ -367,7 +529,7 @@ decode_split_kernel(const __grid_constant__ DecodeArgs P) {
                 x[c] = make_float2(0.0f, 0.0f);
                 if (c < ctas) {
                     ml[c] = ld_cluster(&s_part[g], c);
-                    x[c] = ld_cluster(reinterpret_cast<const float2 *>(s_o + g * HD + d), c);
+                    x[c] = ld_cluster(reinterpret_cast<const float2 *>(reinterpret_cast<float *>(dsm) + g * HD + d), c);
                 }
                 M = fmaxf(M, ml[c].x);
             }
@@ -387,87 +549,71 @@ decode_split_kernel(const __grid_constant__ DecodeArgs P) {
     }
 }
 
-// Joins the parts of the chunks that a sequence has, per (sequence, head): a CTA of
-// eight warps, each taking every eighth chunk, or (W = 1, few chunks) a warp.
-constexpr int kJoinWarps = 8;
-template <int HD, int W>
-__global__ void __launch_bounds__(kJoinWarps * 32)
-decode_join_kernel(const __grid_constant__ DecodeArgs P, int64_t rows) {
-    constexpr int kD = HD / 32;
-    __shared__ float s_m[kJoinWarps], s_l[kJoinWarps], s_o[kJoinWarps][HD];
-    const int64_t r = W == 1 ? blockIdx.x * static_cast<int64_t>(kJoinWarps) + (threadIdx.x >> 5) : blockIdx.x;
-    const int warp = W == 1 ? 0 : threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (r >= rows) return;
-    const int64_t len = P.seq_lens[r / P.H];
-    const int chunks = len > P.max_len ? 1 : static_cast<int>(max((len + P.chunk - 1) / P.chunk, static_cast<int64_t>(1)));
-    const float *src = P.part + r * P.n_chunks * (HD + 4);
+// Joins the parts of the lists that are cut: a CTA for each of these, each head and (Wide)
+// each 32 columns. Lanes threads, four columns each, take a part, the others further
+// parts; their sums are joined at the end. Wide is for lists of many parts: 1 sequence of
+// 32768, 32 heads on 2 (148 parts): the call takes 18 us, 34 with the narrow form; 18 parts:
+// 135 and 138 us.
+struct DecSum {
+    float M, L;
+    float4 o;
+    __device__ __forceinline__ void add(float m, float l, float4 x) {
+        // what has a maximum of -inf saw no key, or NaN alone (its sum says so)
+        const float top = fmaxf(M, m), f = M == -INFINITY ? 0.0f : tc::ex2(M - top), g = m == -INFINITY ? 0.0f : tc::ex2(m - top);
+        L = (M == -INFINITY ? L : f * L) + (m == -INFINITY ? l : g * l);
+        o.x = fmaf(g, x.x, f * o.x), o.y = fmaf(g, x.y, f * o.y);
+        o.z = fmaf(g, x.z, f * o.z), o.w = fmaf(g, x.w, f * o.w);
+        M = top;
+    }
+};
+template <int HD, bool Wide>
+__global__ void __launch_bounds__(Wide ? 512 : 128)
+decode_join_kernel(const __grid_constant__ DecodeArgs P) {
+    constexpr int kThreads = Wide ? 512 : 128, kLanes = Wide ? 8 : HD / 4, kGroups = kThreads / kLanes, kRound = 4;
+    __shared__ DecSum s_sum[kThreads / 32][kLanes];
+    const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes, warp = threadIdx.x / 32;
+    const int d = (static_cast<int>(blockIdx.z) * kLanes + lane) * 4;
+    const int G = P.H / P.Hk, per = min(G, kDecHeads), groups = (G + kDecHeads - 1) / kDecHeads, lists = P.Hk * groups;
     asm volatile("griddepcontrol.wait;\n" ::: "memory");      // the parts are written
-    // this warp's parts against its own maximum, all loads of a round under way at once
-    float M = -INFINITY, L = 0.0f, o[kD] = {};
-    constexpr int kRound = 8;
-    for (int c0 = warp; c0 < chunks; c0 += kRound * W) {
+    const int2 cut = P.cut[blockIdx.x];
+    const int list = P.by_list ? blockIdx.x : cut.x, cta = P.by_list ? cut.x : blockIdx.x;
+    const int y = list % lists, h = y / groups * G + y % groups * kDecHeads + static_cast<int>(blockIdx.y);
+    if (cut.y <= 1 || h >= (y / groups + 1) * G) return;
+    const int64_t step = static_cast<int64_t>(per) * (HD + 4);
+    const float *src = P.part + (static_cast<int64_t>(cta) + list) * step + blockIdx.y * (HD + 4);
+    DecSum sum = {-INFINITY, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+    for (int c0 = group; c0 < cut.y; c0 += kRound * kGroups) {
         float2 ml[kRound];
-        float x[kRound][kD];
+        float4 x[kRound];
 #pragma unroll
         for (int u = 0; u < kRound; ++u) {
-            const int c = c0 + u * W;
+            const int c = c0 + u * kGroups;
             ml[u] = make_float2(-INFINITY, 0.0f);
-#pragma unroll
-            for (int d = 0; d < kD; ++d) x[u][d] = 0.0f;
-            if (c < chunks) {
-                const float *p = src + c * (HD + 4);
-                ml[u] = *reinterpret_cast<const float2 *>(p);
-#pragma unroll
-                for (int d = 0; d < kD; d += 2)
-                    *reinterpret_cast<float2 *>(&x[u][d]) = *reinterpret_cast<const float2 *>(p + 4 + lane * kD + d);
+            x[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (c < cut.y) {
+                ml[u] = *reinterpret_cast<const float2 *>(src + c * step);
+                x[u] = *reinterpret_cast<const float4 *>(src + c * step + 4 + d);
             }
         }
-        float top = M;
 #pragma unroll
-        for (int u = 0; u < kRound; ++u) top = fmaxf(top, ml[u].x);
-        const float f = M == -INFINITY ? 0.0f : tc::ex2(M - top);
-        L *= M == -INFINITY ? 1.0f : f;
-        M = top;
-#pragma unroll
-        for (int d = 0; d < kD; ++d) o[d] *= f;
-#pragma unroll
-        for (int u = 0; u < kRound; ++u) {
-            // a chunk whose maximum is -inf saw no key, or NaN alone (its sum says so)
-            const float g = ml[u].x == -INFINITY ? 0.0f : tc::ex2(ml[u].x - M);
-            L += ml[u].x == -INFINITY ? ml[u].y : g * ml[u].y;
-#pragma unroll
-            for (int d = 0; d < kD; ++d) o[d] = fmaf(g, x[u][d], o[d]);
-        }
-    }
-    if constexpr (W == 1) {
-        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-#pragma unroll
-        for (int d = 0; d < kD; d += 2)
-            *reinterpret_cast<uint32_t *>(P.out + r * HD + lane * kD + d) = pack_bf16x2(o[d] * inv, o[d + 1] * inv);
-        return;
-    }
-    if (lane == 0) {
-        s_m[warp] = M;
-        s_l[warp] = L;
+        for (int u = 0; u < kRound; ++u) sum.add(ml[u].x, ml[u].y, x[u]);
     }
 #pragma unroll
-    for (int d = 0; d < kD; ++d) s_o[warp][lane * kD + d] = o[d];
+    for (int o = kLanes; o < 32; o <<= 1) {
+        const auto other = [&](float v) { return __shfl_xor_sync(0xffffffffu, v, o); };
+        const float m = other(sum.M), l = other(sum.L);
+        sum.add(m, l, make_float4(other(sum.o.x), other(sum.o.y), other(sum.o.z), other(sum.o.w)));
+    }
+    if (threadIdx.x % 32 < kLanes) s_sum[warp][lane] = sum;
     __syncthreads();
-    if (threadIdx.x >= HD / 2) return;
-    const int d = 2 * threadIdx.x;
-    float top = -INFINITY, x = 0.0f, y = 0.0f;
-    L = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, s_m[w]);
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) {
-        const float g = s_m[w] == -INFINITY ? 0.0f : tc::ex2(s_m[w] - top);
-        L += s_m[w] == -INFINITY ? s_l[w] : g * s_l[w];
-        x = fmaf(g, s_o[w][d], x);
-        y = fmaf(g, s_o[w][d + 1], y);
+    if (group > 0) return;
+    for (int w = 1; w < kThreads / 32; ++w) {
+        const DecSum &x = s_sum[w][lane];
+        sum.add(x.M, x.L, x.o);
     }
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    *reinterpret_cast<uint32_t *>(P.out + r * HD + d) = pack_bf16x2(x * inv, y * inv);
+    const float inv = sum.L == 0.0f ? 0.0f : 1.0f / sum.L;
+    *reinterpret_cast<uint2 *>(P.out + (static_cast<int64_t>(list / lists) * P.H + h) * HD + d) =
+        make_uint2(pack_bf16x2(sum.o.x * inv, sum.o.y * inv), pack_bf16x2(sum.o.z * inv, sum.o.w * inv));
 }
 
 }  // namespace
@@ -490,32 +636,28 @@ cudaError_t launch_rope_append(const void *qkv, int64_t ld, const float *cosv, c
     return cudaGetLastError();
 }
 
-// Keys of a chunk. The host knows only the longest length a sequence may have: about
-// 12 CTAs an SM by that bound keep ragged batches level (48 sequences of 64 to 4096:
-// 45 us, 57 with 6 an SM, 41 with 24; 4 of 131072: 142, 151, 156), but a CTA of under 512 keys pays more for its start and its
-// part than it saves (8 sequences of 2048, 16 heads: 15 us with 512, 17 with 256),
-// except where there would not be two CTAs an SM (1 sequence of 32768, 2 key heads:
-// 13.7 us with 256, 18 with 512).
-DecodeSplit decode_split(int64_t B, int64_t H, int64_t Hk, int64_t max_len) {
+DecodeSplit decode_split(int64_t B, int64_t H, int64_t Hk, int64_t hd, int64_t max_len) {
     DecodeSplit s;
     const int64_t G = H / std::max<int64_t>(Hk, 1), lists = B * Hk * ((G + kDecHeads - 1) / kDecHeads);
-    const auto over = [&](int64_t ctas) { return (lists * max_len + ctas - 1) / ctas; };
-    int64_t chunk = std::max(over(12 * 148), std::min<int64_t>(512, over(2 * 148)));
-    chunk = std::min<int64_t>(std::max<int64_t>((chunk + 63) / 64 * 64, 64), kDecMaxChunk);
-    // few short lists: as one cluster each, of up to 8 chunks of up to 512 keys
-    if (lists * kClusterMost <= 2 * 148 && max_len <= kClusterMost * 512) {
-        chunk = std::max<int64_t>((max_len + kClusterMost - 1) / kClusterMost, 64);
-        chunk = (chunk + 63) / 64 * 64;
+    const int64_t resident = static_cast<int64_t>(device_sm_count()) * (hd == 64 ? Dec<64>::kCtas : Dec<128>::kCtas);
+    // few short lists: as one cluster each, of up to 8 chunks of up to 512 keys (8 sequences of
+    // 2048, 16 heads of 64: 16 us, 21 in spans with a join)
+    const int64_t most = std::min<int64_t>(kClusterMost, resident / std::max<int64_t>(lists, 1));
+    if (most > 0 && max_len <= most * 512) {
+        const int64_t chunk = std::max<int64_t>((max_len + most - 1) / most, 64);
+        s.chunk = static_cast<int>((chunk + 63) / 64 * 64);
+        s.n_chunks = static_cast<int>(std::max<int64_t>(1, (max_len + s.chunk - 1) / s.chunk));
         s.cluster = true;
+        return s;
     }
-    s.chunk = static_cast<int>(chunk);
-    s.n_chunks = static_cast<int>(std::max<int64_t>(1, (max_len + s.chunk - 1) / s.chunk));
-    s.cluster = s.cluster && s.n_chunks > 1;
+    s.ctas = resident;
+    s.ctas = std::min(s.ctas, lists * std::max<int64_t>((max_len + kDecTile * kDecLeast - 1) / (kDecTile * kDecLeast), 1));
+    s.lists = lists;
     return s;
 }
 
 template <int HD>
-static cudaError_t launch_decode(const DecodeArgs &p, const DecodeSplit &s, dim3 grid, int64_t rows, cudaStream_t st) {
+static cudaError_t launch_decode(const DecodeArgs &p, const DecodeSplit &s, dim3 grid, cudaStream_t st) {
     constexpr int smem = Dec<HD>::kSmem;
     static std::atomic<uint64_t> ready{0};      // devices whose kernels have their shared memory set
     int dev = 0;
@@ -548,15 +690,15 @@ static cudaError_t launch_decode(const DecodeArgs &p, const DecodeSplit &s, dim3
     decode_split_kernel<HD, false><<<grid, kDecWarps * 32, smem, st>>>(p);
     count_launch();
     e = cudaGetLastError();
-    if (e != cudaSuccess || s.n_chunks == 1) return e;
+    if (e != cudaSuccess) return e;
     // the join's launch overlaps the split's end; its threads wait for the parts
-    const bool few = s.n_chunks <= 2 || (s.n_chunks <= 16 && rows >= 1024);
-    cfg.gridDim = dim3(static_cast<unsigned>(few ? (rows + kJoinWarps - 1) / kJoinWarps : rows));
-    cfg.blockDim = dim3(kJoinWarps * 32);
+    const bool wide = s.ctas > 8 * s.lists;
+    cfg.blockDim = dim3(wide ? 512 : 128);
+    cfg.gridDim = dim3(static_cast<unsigned>(std::min(s.ctas, s.lists)), std::min(p.H / p.Hk, kDecHeads), wide ? HD / 32 : 1);
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
-    e = few ? cudaLaunchKernelEx(&cfg, decode_join_kernel<HD, 1>, p, rows)
-            : cudaLaunchKernelEx(&cfg, decode_join_kernel<HD, 8>, p, rows);
+    e = wide ? cudaLaunchKernelEx(&cfg, decode_join_kernel<HD, true>, p)
+             : cudaLaunchKernelEx(&cfg, decode_join_kernel<HD, false>, p);
     count_launch();
     return e;
 }
@@ -565,10 +707,11 @@ cudaError_t launch_decode_attn(const void *q, int64_t q_ld, const void *kp, cons
                                int page_shift, const int32_t *table, int64_t table_ld, const int32_t *seq_lens,
                                int64_t max_len, int64_t B, int H, int Hk, int hd, float scale, void *out, float *part,
                                cudaStream_t st) {
-    const DecodeSplit s = decode_split(B, H, Hk, max_len);
+    const DecodeSplit s = decode_split(B, H, Hk, hd, max_len);
     const int G = H / Hk;
-    const dim3 grid(s.n_chunks, Hk * ((G + kDecHeads - 1) / kDecHeads), static_cast<unsigned>(B));
-    DecodeArgs p;
+    const unsigned lists = Hk * ((G + kDecHeads - 1) / kDecHeads);
+    const dim3 grid = s.cluster ? dim3(s.n_chunks, lists, static_cast<unsigned>(B)) : dim3(static_cast<unsigned>(s.ctas));
+    DecodeArgs p = {};
     p.q = static_cast<const uint16_t *>(q);
     p.kp = static_cast<const uint16_t *>(kp);
     p.vp = static_cast<const uint16_t *>(vp);
@@ -581,12 +724,16 @@ cudaError_t launch_decode_attn(const void *q, int64_t q_ld, const void *kp, cons
     p.H = H;
     p.Hk = Hk;
     p.page_shift = page_shift;
+    p.B = B;
     p.chunk = s.chunk;
     p.n_chunks = s.n_chunks;
     p.scale_log2 = scale * kLog2e;
     p.out = static_cast<uint16_t *>(out);
     p.part = part;
-    return hd == 64 ? launch_decode<64>(p, s, grid, B * H, st) : launch_decode<128>(p, s, grid, B * H, st);
+    // the parts, then the CTAs' cut lists
+    p.by_list = s.lists <= s.ctas;
+    p.cut = s.cluster ? nullptr : reinterpret_cast<int2 *>(part + s.part_floats(H, Hk, hd));
+    return hd == 64 ? launch_decode<64>(p, s, grid, st) : launch_decode<128>(p, s, grid, st);
 }
 
 }  // namespace mom

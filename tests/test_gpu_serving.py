@@ -248,6 +248,34 @@ def test_decode_attention(hd, H, Hk, page):
                want[0][b:b + 1], want[1][b:b + 1])
 
 
+@pytest.mark.parametrize("B,hd,H,Hk", [(300, 64, 4, 4), (140, 128, 40, 2), (40, 64, 16, 16), (3, 128, 16, 1)])
+def test_decode_attention_spans_of_many_lists(B, hd, H, Hk):
+    """More sequences than a CTA has threads and lists that share a CTA, one list over
+    many CTAs, more than 16 heads to a key head; lengths of none, one and tiles' ends."""
+    from naylis_b200 import attention
+    g = torch.Generator().manual_seed(B)
+    lens = [[0, 1, 16, 17, -3, 96][i % 6] if i % 2 else int(torch.randint(0, 300, (1,), generator=g)) for i in range(B)]
+    lens[B // 2] = 9000
+    page = 16
+    kp, vp, table, sl, ks, vs = _cache(11, [max(n, 0) for n in lens], Hk, page, hd, fill=float("nan"))
+    sl = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    q = _rand(12, B, H, hd, scale=2.0)
+    want = _decode_exact(q, ks, vs, hd ** -0.5)
+    out = attention.decode_attention(q, kp, vp, table, sl)
+    _close(out, *want)
+    assert torch.equal(out, attention.decode_attention(q, kp, vp, table, sl))
+    # a page outside the cache and a length over max_len spoil their own sequences alone
+    table[B // 2, 300] = kp.shape[0]
+    table[0, 0] = -1
+    sl[0], sl[B - 1] = 5, 9001
+    got = attention.decode_attention(q, kp, vp, table, sl, max_len=9000)
+    spoilt = torch.zeros(B, dtype=torch.bool, device=DEV)
+    spoilt[[0, B // 2, B - 1]] = True
+    assert got[spoilt].isnan().all()
+    if not spoilt.all():
+        _close(got[~spoilt], want[0][~spoilt], want[1][~spoilt])
+
+
 def test_decode_attention_strides_stream_and_scores():
     """q as a slice of a fused projection, a table with a wider pitch, scores hundreds
     of units apart, on another stream."""

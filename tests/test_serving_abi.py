@@ -145,3 +145,10 @@ def test_bad_arguments_fail_before_device_work(lib):
     assert _lp(lib, R=0, x=None) == OK
     for kw in (dict(stats=None), dict(dx=None), dict(ti=None), dict(dx=P(257)), dict(T=-1.0)):
         assert _lpb(lib, **kw) == INVALID, kw
+
+
+def test_decode_refuses_more_keys_than_it_counts(lib):
+    many = dict(B=65535, H=64, Hk=64, ld=4096, tld=1 << 20, max_len=1 << 24)
+    assert _decode(lib, **many) == INVALID
+    assert lib.mom_decode_attn_workspace_size(65535, 64, 64, 64, 1 << 20) > 0
+    assert lib.mom_decode_attn_workspace_size(2, 2, 2, 64, 0) == 0      # few short lists need none
