@@ -194,9 +194,10 @@ def decode_attention(q, k_pages, v_pages, block_table, seq_lens, *, scale=None, 
     bf16; k_pages, v_pages (num_pages, Hk, page_size, hd); block_table (B, n)
     int32, each sequence's pages in order; seq_lens (B) int32 on the device, each
     sequence's keys (the new token's among them). max_len, known to the host,
-    bounds seq_lens (default n * page_size): the work is split over it. A sequence
-    of length <= 0 gets zeros; one longer than max_len, or with a page outside the
-    cache, NaN. Returns (B, H, hd) bf16."""
+    bounds seq_lens (default n * page_size); the keys are shared out by the lengths
+    themselves, so it need not be near. A sequence of length <= 0 gets zeros; one
+    longer than max_len, or with a page outside the cache, NaN. Returns (B, H, hd)
+    bf16."""
     _check("decode_attention", q, k_pages, v_pages)
     _pages("decode_attention", k_pages, v_pages)
     q, q_ld = _rows("decode_attention", q, "q")
