@@ -331,14 +331,20 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                 if (h.vis + quarter * 32 - j * kN < kN) {
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
-                        if (h.vis + quarter * 32 - j * kN >= 32 * (c + 1)) continue;
+                        const int first = h.vis + quarter * 32 - j * kN - 32 * c;      // what the warp's first row sees
+                        if (first >= 32) continue;
                         uint32_t x[32];
-                        tc::tmem_ld32(tS + 32 * c, x);
-                        tc::tmem_ld_wait();
-                        const int left = min(max(seen - 32 * c, 0), 32);
-                        const uint32_t keep = left == 32 ? 0xffffffffu : (1u << left) - 1u;
+                        if (first > -31) {
+                            tc::tmem_ld32(tS + 32 * c, x);
+                            tc::tmem_ld_wait();
+                            const int left = min(max(seen - 32 * c, 0), 32);
+                            const uint32_t keep = left == 32 ? 0xffffffffu : (1u << left) - 1u;
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) x[e] = keep >> e & 1u ? x[e] : __float_as_uint(-INFINITY);
+                            for (int e = 0; e < 32; ++e) x[e] = keep >> e & 1u ? x[e] : __float_as_uint(-INFINITY);
+                        } else {      // hidden from all of them
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(-INFINITY);
+                        }
                         tc::tmem_st32(tS + 32 * c, x);
                     }
                     tc::tmem_st_wait();
