@@ -129,6 +129,9 @@ struct Cfg {
     static constexpr uint32_t kQ = 2 * kQBufs * kN * HD * 2;
     static constexpr bool kOwnP = HD == 64;                   // P has columns of its own
     static constexpr uint32_t kTile = kN * HD * 2;            // a K, V or Q tile
+    // registers of a thread of the softmax (8 warps), the epilogue (4) and the others (4)
+    static constexpr int kSoftRegs = 184, kEpiRegs = 80, kRestRegs = 64;
+    static_assert(32 * (8 * kSoftRegs + 4 * kEpiRegs + 4 * kRestRegs) <= 512 * 128, "registers at launch");
     static constexpr int kStages = HD == 64 ? 8 : 4;          // K and V tiles in turn
     static constexpr uint32_t kRing = kStages * kTile;
     static constexpr uint32_t kSum = 2 * 2 * kM * 4;          // row sums [item parity][half][row]
@@ -203,6 +206,11 @@ struct Items {
     }
 };
 static_assert(kN == 128, "key tiles are counted by a shift");
+
+// Whether a NaN or an infinity is in a pair of bf16.
+__device__ __forceinline__ bool not_finite(uint32_t pair) {
+    return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u;
+}
 
 // Rows of a half whose sums are not finite although their weights are: if the tiles
 // that the mask cuts hold a non-finite value, it may be a hidden one; then the warp's
@@ -298,7 +306,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
     if (warp < 8) {
         // ------------------------------------------------------------ softmax
         // Warps 0-3: half A, 4-7: half B; a thread holds one row of scores.
-        tc::regs_inc<184>();
+        tc::regs_inc<C::kSoftRegs>();
         const int a = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
         const uint32_t tS = tmem + kSCol + a * kN + lanes, tO = tmem + kOCol + a * HD + lanes;
@@ -447,12 +455,12 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
     } else if (warp < 12) {
         // ------------------------------------------------------------ epilogue
         // One item behind the softmax: O / l to global, each thread one row.
-        tc::regs_dec<80>();
+        tc::regs_dec<C::kEpiRegs>();
         const int quarter = warp & 3, r = quarter * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
         uint4 *stage = reinterpret_cast<uint4 *>(sbase + C::kQ + C::kRing) + quarter * 32 * 8;
         int phase[2] = {0, 0};
-        bool ok = true;
+        bool ok = true, again = false;
         Items items(P);
         for (Item it; ok && items.get(it);) {
 #pragma unroll
@@ -511,15 +519,35 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                     }
                     __syncwarp();
                 }
-                // A weight of 0 does not hide a NaN or an infinity from a product: rows that a value
-                // behind the mask has spoilt are done again, by themselves
-                const bool spoilt = !(big < INFINITY) && l < INFINITY && r < h.rows && !none;
-                if (__any_sync(0xffffffffu, spoilt))
-                    redo_rows<HD>(P, h, it.k0, r, spoilt);
+                again |= !(big < INFINITY) && l < INFINITY && r < h.rows && !none;
+            }
+        }
+        // A weight of 0 does not hide a NaN or an infinity from a product: rows that a value
+        // behind the mask may have spoilt are done again, by themselves. Behind the loop, since a call in it,
+        // though never made, takes registers from what it does (8 sequences of 2048, 16 heads on 4 of
+        // 128: 128 us, 136 with it; 64 of 256, 16 of 64: 36 and 40).
+        if (ok && __any_sync(0xffffffffu, again)) {
+            Items past(P);
+            for (Item it; past.get(it);) {
+#pragma unroll 1
+                for (int a = 0; a < 2; ++a) {
+                    const Half h = it.h[a];
+                    bool spoilt = false;
+                    if (h.n > 0 && r < h.rows && h.vis + r > 0) {
+                        const uint4 *row = reinterpret_cast<const uint4 *>(P.out + (static_cast<int64_t>(h.q0 + r) * P.H +
+                                                                                    h.head) * HD);
+#pragma unroll 1
+                        for (int c = 0; c < HD / 8; ++c) {
+                            const uint4 x = row[c];
+                            spoilt |= not_finite(x.x) || not_finite(x.y) || not_finite(x.z) || not_finite(x.w);
+                        }
+                    }
+                    if (__any_sync(0xffffffffu, spoilt)) redo_rows<HD>(P, h, it.k0, r, spoilt);
+                }
             }
         }
     } else {
-        tc::regs_dec<64>();
+        tc::regs_dec<C::kRestRegs>();
         if (warp < 14) {
             // -------------------------------------------------------- MMA issuers
             // Warp 12: half A, 13: half B, each one thread. Where P lives in S's columns: per key
