@@ -486,22 +486,22 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
 #pragma unroll
                 for (int c = 0; c < HD / 64; ++c) {
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        uint32_t o[32];
-                        tc::tmem_ld32(tO + 64 * c + 32 * e, o);
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t o[16];
+                        tc::tmem_ld16(tO + 64 * c + 16 * e, o);
                         tc::tmem_ld_wait();
 #pragma unroll
-                        for (int z = 0; z < 32; z += 2)
+                        for (int z = 0; z < 16; z += 2)
                             big = tc::fmax3_nan(big, fabsf(__uint_as_float(o[z])), fabsf(__uint_as_float(o[z + 1])));
 #pragma unroll
-                        for (int z = 0; z < 4; ++z) {
+                        for (int z = 0; z < 2; ++z) {
                             uint32_t pk[4];
 #pragma unroll
                             for (int y = 0; y < 4; ++y)
                                 pk[y] = none ? 0u
                                              : pack_bf16x2(__uint_as_float(o[8 * z + 2 * y]) * inv,
                                                            __uint_as_float(o[8 * z + 2 * y + 1]) * inv);
-                            stage[lane * 8 + ((4 * e + z) ^ (lane & 7))] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                            stage[lane * 8 + ((2 * e + z) ^ (lane & 7))] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
                         }
                     }
                     if (c + 1 == HD / 64) {
