@@ -907,7 +907,8 @@ int mom_rope_append(const void *qkv, int64_t qkv_ld, const float *cosv, const fl
 }
 
 size_t mom_decode_attn_workspace_size(int64_t B, int64_t H, int64_t Hk, int64_t hd, int64_t max_len) {
-    if (B <= 0 || H <= 0 || Hk <= 0 || hd <= 0 || max_len <= 0) return 0;
+    // of the split that the launch takes, at max_len 0 too: many lists without keys are spans that write their cuts
+    if (B <= 0 || H <= 0 || Hk <= 0 || hd <= 0 || max_len < 0) return 0;
     const mom::DecodeSplit s = mom::decode_split(B, H, Hk, hd, max_len);
     return s.bytes(H, Hk, hd);
 }

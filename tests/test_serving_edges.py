@@ -1,0 +1,37 @@
+"""CPU tests of the serving entry points' edges: sizes that the host has to get right
+before a kernel may run."""
+import ctypes
+
+import pytest
+
+P = ctypes.c_void_p
+OK, INVALID, UNSUPPORTED, WORKSPACE = 0, 1, 2, 4
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from naylis_b200 import _lib, build
+    build.build()
+    return _lib.load()
+
+
+def _decode(lib, **kw):
+    a = dict(q=P(256), ld=1024, kp=P(256), vp=P(256), pages=4, page=16, table=P(256), tld=4, lens=P(256), max_len=64,
+             B=64, H=16, Hk=16, hd=64, scale=0.1, out=P(256), ws=P(256), wsb=1 << 30, stream=None)
+    a.update(kw)
+    return lib.mom_decode_attn(*a.values())
+
+
+@pytest.mark.parametrize("B,H,Hk,hd", [(64, 16, 16, 64), (38, 16, 16, 64), (10, 32, 32, 128), (297, 40, 1, 128)])
+def test_decode_without_keys_has_its_workspace(lib, B, H, Hk, hd):
+    """More lists (sequences x key heads) than CTAs fit the GPU are cut into spans,
+    whose cuts are written to the workspace, though no list has a key: a call without
+    one is refused."""
+    need = lib.mom_decode_attn_workspace_size(B, H, Hk, hd, 0)
+    assert need > 0
+    none = dict(B=B, H=H, Hk=Hk, hd=hd, ld=H * hd, max_len=0, tld=0, table=None)
+    assert _decode(lib, **none, ws=None, wsb=0) == WORKSPACE
+    assert _decode(lib, **none, wsb=need - 1) == WORKSPACE
+    # few lists: one cluster each, as ever
+    assert lib.mom_decode_attn_workspace_size(2, H, Hk, hd, 0) == 0
+    assert lib.mom_decode_attn_workspace_size(B, H, Hk, hd, -1) == 0
