@@ -385,7 +385,7 @@ MOM_API int mom_rope_append(const void *qkv, int64_t qkv_ld, const float *cos, c
  * order; seq_lens (B) I32 on the device, the keys of each sequence (the new
  * token's own among them). out (B, H, hd) = softmax(scale q.k) v, scale > 0. max_len: an
  * upper bound of seq_lens known to the host (at most table_ld * page_size, and
- * B H (max_len / 16 + 8) at most 2^40); the work is shared out by the lengths, and a
+ * B H (max_len / 16 + 8) at most 2^38); the work is shared out by the lengths, and a
  * workspace of mom_decode_attn_workspace_size bytes joins the parts. A sequence of length <= 0 gets zeros; one longer than max_len,
  * or with a page outside [0, num_pages) among its keys, gets NaN. What the pages
  * hold behind a sequence's end is not read into the result, NaN neither. */

@@ -922,8 +922,9 @@ int mom_decode_attn(const void *q, int64_t q_ld, const void *k_pages, const void
     if ((rc = check_cache_geometry(num_pages, page_size))) return rc;
     MOM_REQUIRE(B >= 0 && B <= 65535, "B must be in [0, 65535] (got %lld)", (long long)B);
     MOM_REQUIRE(max_len >= 0 && max_len <= INT32_MAX, "max_len out of range");
-    MOM_REQUIRE(B * H <= (1 << 30) && B * H * (max_len / 16 + 8) <= (int64_t(1) << 40),
-                "too many sequences, heads and keys (2^30, 2^44)");
+    // a span, 1/296 of the tiles at most, is counted in 32 bits, and so is a list that ends behind it
+    MOM_REQUIRE(B * H <= (1 << 30) && B * H * (max_len / 16 + 8) <= (int64_t(1) << 38),
+                "too many sequences, heads and keys (2^30, 2^42)");
     MOM_REQUIRE(table_ld >= 0 && max_len <= table_ld * page_size, "max_len exceeds the block table (%lld pages of %lld)",
                 (long long)table_ld, (long long)page_size);
     MOM_REQUIRE(q_ld >= H * hd && q_ld % 8 == 0, "q row pitch must hold all heads and be a multiple of 8");

@@ -35,3 +35,16 @@ def test_decode_without_keys_has_its_workspace(lib, B, H, Hk, hd):
     # few lists: one cluster each, as ever
     assert lib.mom_decode_attn_workspace_size(2, H, Hk, hd, 0) == 0
     assert lib.mom_decode_attn_workspace_size(B, H, Hk, hd, -1) == 0
+
+
+def test_decode_counts_a_span_in_32_bits(lib):
+    """A list's tiles are counted in 32 bits from the start of the one that a span
+    begins in, up to the end of the one that it ends in: what does not fit is refused.
+    296 CTAs is the least that spans are cut for (head_dim 128)."""
+    lists, fits = 1 << 16, (1 << 26) - 256
+    long = dict(B=1 << 10, H=64, Hk=64, hd=128, ld=64 * 128, tld=1 << 23, ws=None, wsb=0)
+    assert _decode(lib, **long, max_len=fits) == WORKSPACE
+    assert _decode(lib, **long, max_len=1 << 26) == INVALID
+    assert _decode(lib, **long, max_len=1 << 27) == INVALID
+    units = fits // 16 + 6
+    assert units + lists * units // 296 + units < 1 << 31
