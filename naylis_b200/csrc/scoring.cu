@@ -25,6 +25,11 @@ namespace mom {
 namespace {
 
 constexpr float kNaN = __builtin_nanf("");
+// Logits are summed as at least kFloor, which is below every reference that counts: the
+// weight of a masked one is then 0, not 0 x inf. Rows whose maximum lies beyond kFar
+// (nothing but masks of the type's lowest value, say) are summed by themselves.
+constexpr float kFloor = -0x1.92p+99f;      // the bf16 nearest -1e30
+constexpr float kFar = 1e29f;
 
 template <int DT>
 __device__ __forceinline__ float logit(const void *row, int64_t j) {
@@ -87,19 +92,19 @@ __device__ __forceinline__ void unpack(const uint4 &v, float (&x)[16 / sizeof(ty
     }
 }
 
-// The same with values below -1e30 (a masked logit's -inf, a NaN) raised to it.
+// The same with values below kFloor (a masked logit's, -inf or the type's lowest, a NaN) raised to it.
 template <int DT>
 __device__ __forceinline__ void unpack_floor(const uint4 &v, float (&x)[16 / sizeof(typename Elem<DT>::T)]) {
     if constexpr (DT == MOM_BF16) {
         uint32_t a[4] = {v.x, v.y, v.z, v.w};
-        const uint32_t floor2 = 0xf149f149u;      // the bf16 nearest -1e30, twice
+        const uint32_t floor2 = 0xf149f149u;      // kFloor, the bf16 nearest -1e30, twice
 #pragma unroll
         for (int i = 0; i < 4; ++i) asm("max.bf16x2 %0, %0, %1;\n" : "+r"(a[i]) : "r"(floor2));
         unpack<DT>(make_uint4(a[0], a[1], a[2], a[3]), x);
     } else {
         unpack<DT>(v, x);
 #pragma unroll
-        for (float &y : x) y = fmaxf(y, -1e30f);
+        for (float &y : x) y = fmaxf(y, kFloor);
     }
 }
 
@@ -123,8 +128,7 @@ __device__ __forceinline__ float vec_max(const uint4 &v) {
 // sums e^(y-c) and e^(y-c) (y-c) against a reference c of its own, the maximum of its
 // first kHold vectors, moved only when a later one passes it by more than kSlack (so
 // the sums neither overflow nor lose digits); the row's threads rebase to the greatest
-// reference at the end. A masked logit (-inf) counts as -1e30: its term is 0, not
-// 0 x inf.
+// reference at the end. A masked logit counts as kFloor, and a reference is no lower.
 //
 // Alternatives: the k-th greatest of the groups' maxima bounds the k-th greatest
 // logit from below, so few elements reach it; the threads that hold them list them
@@ -183,14 +187,14 @@ logprobs_fwd_kernel(const void *__restrict__ logits, int64_t ld, const int64_t *
         const uint64_t cc2 = tc::f2(c2, c2);
         auto rebase = [&](float to) {
             if (ref > -INFINITY) {
-                const float delta = (ref - to) * c2, f = tc::ex2(delta);
+                const float delta = fmaxf((ref - to) * c2, -256.0f), f = tc::ex2(delta);      // f is 0 there
                 w2 = tc::mul2(tc::fma2(tc::f2(delta, delta), s2, w2), tc::f2(f, f));
                 s2 = tc::mul2(s2, tc::f2(f, f));
             }
             ref = to;
             ref2 = tc::f2(to, to);
         };
-        auto add = [&](float xa, float xb) {      // xa, xb finite: at least -1e30
+        auto add = [&](float xa, float xb) {      // xa, xb finite: at least kFloor
             // the difference first: it is exact near the reference, whatever that is. (x c2 - ref c2 in one step
             // leaves the rounding of ref c2 in every term, and so in ln Z: 4e-5 at logits of 1000.)
             const uint64_t z = tc::mul2(tc::sub2(tc::f2(xa, xb), ref2), cc2);
@@ -200,8 +204,8 @@ logprobs_fwd_kernel(const void *__restrict__ logits, int64_t ld, const int64_t *
         };
         if (x_extra > -INFINITY) {
             ref = -INFINITY;
-            rebase(x_extra);
-            add(x_extra, -1e30f);
+            rebase(fmaxf(x_extra, kFloor));
+            add(fmaxf(x_extra, kFloor), kFloor);
         }
         const float slack = kSlack / c2;
         // the batches' maxima, those of batch b, b + 4, ... in one: where the alternatives are looked for
@@ -225,7 +229,7 @@ logprobs_fwd_kernel(const void *__restrict__ logits, int64_t ld, const int64_t *
 #pragma unroll
             for (int q = 0; q < 4; ++q)
                 if ((batch & 3) == q) bmax[q] = tc::fmax3_nan(bmax[q], bmax[q], vm[0]);
-            if (vm[0] > ref + slack) rebase(vm[0]);
+            if (vm[0] > ref + slack) rebase(fmaxf(vm[0], kFloor));
             auto sum = [&](const uint4 &q) {
                 float x[kVE];
                 unpack_floor<DT>(q, x);
@@ -254,10 +258,31 @@ logprobs_fwd_kernel(const void *__restrict__ logits, int64_t ld, const int64_t *
             __syncthreads();
             M_order = __reduce_max_sync(0xffffffffu, lane < (TPR / 32) ? S.top[lane] : 0u);
         }
-        const float M = value_of(M_order);
+        float M = value_of(M_order);
         if (ref > -INFINITY && M < INFINITY) rebase(M);
         const float2 ss = tc::f2_split(s2), ww = tc::f2_split(w2);
         float s = ss.x + ss.y, w = ww.x + ww.y;
+        if (fabsf(M) > kFar && fabsf(M) < INFINITY) {
+            // a row of masks alone, or a logit whose distance from the floor is not finite: once more,
+            // element by element, against the row's maximum
+            M_order = __reduce_max_sync(0xffffffffu, mine);
+            if constexpr (TPR > 32) {
+                __syncthreads();      // S.top is read
+                if (lane == 0) S.top[warp] = M_order;
+                __syncthreads();
+                M_order = __reduce_max_sync(0xffffffffu, lane < (TPR / 32) ? S.top[lane] : 0u);
+            }
+            M = value_of(M_order);
+            s = w = 0.0f;
+#pragma unroll 1
+            for (int j = t; j < V; j += TPR) {
+                const float z = (logit<DT>(row.row, j) - M) * c2, e = tc::ex2(z);
+                if (e > 0.0f) {      // not 0 x inf
+                    s += e;
+                    w = fmaf(e, z, w);
+                }
+            }
+        }
         if (!(M < INFINITY)) s = kNaN;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {

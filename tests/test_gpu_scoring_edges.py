@@ -132,3 +132,28 @@ def _patterns(base, fill):
 @pytest.mark.parametrize("T", [1.0, 0.7])
 def test_finite_masks(dtype, V, fill, T):
     _check(_patterns(_base(V + 2, 10, V, dtype), fill), 20, T)
+
+
+@pytest.mark.parametrize("dtype,V", LENGTHS)
+@pytest.mark.parametrize("fill", [-1e30, -3e38, "lowest", -5e29, 1e30, "greatest"])
+@pytest.mark.parametrize("T", [1.0, 0.7, 1e-6, 1e6])
+def test_masks_of_the_lowest_value(dtype, V, fill, T):
+    """Down to the type's lowest value, and up to its greatest."""
+    ends = {"lowest": torch.finfo(dtype).min, "greatest": torch.finfo(dtype).max}
+    _check(_patterns(_base(V + 3, 10, V, dtype), ends.get(fill, fill)), 20, T)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_short_rows_of_masks(dtype):
+    """Rows of one to nine elements, none of whose threads has a whole vector."""
+    low = torch.finfo(dtype).min
+    for V in range(1, 10):
+        x = _base(V, 12, V, dtype)
+        x[:6] = low
+        x[1, V // 2] = float("-inf") if V > 1 else low
+        x[2, 0] = 2.0
+        x[3, -1] = -1e30
+        x[4, V // 2] = torch.finfo(dtype).max
+        x[7, 0] = low
+        x[8, -1] = low
+        _check(x, min(V, 3), 1.0)
