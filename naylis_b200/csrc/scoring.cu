@@ -449,10 +449,11 @@ logprobs_bwd_kernel(const void *__restrict__ logits, int64_t ld, const int64_t *
         for (int k = 0; k < top; ++k) G += g_top[r * top + k];
     // p (G + h (ln p + H)) with ln p = y - ln Z and p = e^y / Z
     const float inv_z = 1.0f / st.y, base = G + h * (st.w - st.z), c2 = inv_t * kLog2e, hy = h * inv_t;
+    const float far = -256.0f / c2;      // p is 0 from there on
     auto grad = [&](float x) {
-        const float dx = fmaxf(x - st.x, -1e30f);
+        const float dx = fmaxf(x - st.x, far);
         const float p = tc::ex2(dx * c2) * inv_z;
-        // a masked logit: 0 whatever the rest (p = 0 here, and dx is finite)
+        // a masked logit: 0 whatever the rest (p = 0 here, and hy dx is at most 178 h)
         return -p * fmaf(hy, dx, base) * inv_t;
     };
     if (alike) {

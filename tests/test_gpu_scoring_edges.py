@@ -157,3 +157,22 @@ def test_short_rows_of_masks(dtype):
         x[7, 0] = low
         x[8, -1] = low
         _check(x, min(V, 3), 1.0)
+
+
+@pytest.mark.parametrize("dtype,V", LENGTHS)
+@pytest.mark.parametrize("T,weight", [(1e-6, 1e4), (1e-3, 1e9), (1.0, 1e10)])
+def test_gradient_of_masked_logits_is_zero(dtype, V, T, weight):
+    """However much the entropy's gradient weighs: 0 where the probability is, and
+    finite elsewhere (two equal logits share the row: p = 1/2, H = ln 2, no gradient)."""
+    from naylis_b200 import scoring
+    for fill in (float("-inf"), torch.finfo(dtype).min, -1e30):
+        x = torch.full((2, V), fill, dtype=dtype, device=DEV)
+        x[:, 5], x[:, V - 1] = 1.5, 1.5
+        x.requires_grad_(True)
+        r = scoring.token_logprobs(x, torch.tensor([5, 7], device=DEV), temperature=T)
+        d, = torch.autograd.grad(r.entropy, x, torch.full((2,), weight, device=DEV))
+        gone = torch.ones(V, dtype=torch.bool, device=DEV)
+        gone[[5, V - 1]] = False
+        assert bool((d[:, gone] == 0).all())
+        # ln p + H is 0 within 32 u of ln 2: e_z and the roundings of its terms
+        assert bool((d.double().abs() <= weight / T * (V / 32 + 64 + 32) * U).all())
