@@ -426,7 +426,8 @@ MOM_API int mom_prompt_plan_check(void *plan, void *stream);
  * -inf, gets NaN. stats (R, 4) fp32 for the backward, or NULL.
  * mom_logprobs_bwd: dlogits (R, V) in the logits' dtype, contiguous, from the
  * gradients of logprob (R), entropy (R) and top_logprob (R, top_k), each of which
- * may be NULL (none); ignored rows have no gradient from their logprob. */
+ * may be NULL (none); ignored rows have no gradient from their logprob, and a row
+ * whose target is outside [0, V) has NaN from it. */
 MOM_API int mom_logprobs_fwd(const void *logits, int dtype, int64_t ld, const int64_t *targets, int64_t R, int64_t V,
                              int64_t ignore_index, double temperature, int64_t top_k, float *logprob, float *entropy,
                              float *top_logprob, int64_t *top_idx, float *stats, void *stream);

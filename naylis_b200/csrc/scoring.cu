@@ -442,7 +442,7 @@ logprobs_bwd_kernel(const void *__restrict__ logits, int64_t ld, const int64_t *
     const float4 st = stats[r];
     const int64_t tok = targets[r];
     float g = g_lp && tok != ignore ? g_lp[r] : 0.0f;
-    if (tok != ignore && (tok < 0 || tok >= V)) g = kNaN;
+    if (g_lp && tok != ignore && (tok < 0 || tok >= V)) g = kNaN;      // its logprob is; the rest is not its concern
     const float h = g_ent ? g_ent[r] : 0.0f;
     float G = g;
     if (g_top)

@@ -176,3 +176,25 @@ def test_gradient_of_masked_logits_is_zero(dtype, V, T, weight):
         assert bool((d[:, gone] == 0).all())
         # ln p + H is 0 within 32 u of ln 2: e_z and the roundings of its terms
         assert bool((d.double().abs() <= weight / T * (V / 32 + 64 + 32) * U).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_target_outside_spoils_its_logprob_alone(dtype):
+    """The entropy's and the alternatives' gradients do not depend on the target."""
+    from naylis_b200 import scoring
+    V, top = 300, 4
+    x = _base(3, 4, V, dtype).requires_grad_(True)
+    outside = torch.tensor([V, -1, 3, 1 << 40], device=DEV)
+    inside = torch.tensor([0, 1, 3, 7], device=DEV)
+    bad = torch.tensor([True, True, False, True], device=DEV)
+    g, a = torch.randn(4, device=DEV), torch.randn(4, top, device=DEV)
+
+    def gradient(t, which):
+        r = scoring.token_logprobs(x, t, top_k=top)
+        return torch.autograd.grad([r[i] for i in which], x, [g if i < 2 else a for i in which])[0]
+
+    for which in ((1,), (3,), (1, 3)):
+        assert torch.equal(gradient(outside, which), gradient(inside, which))
+    for which in ((0,), (0, 1)):
+        d = gradient(outside, which)
+        assert bool(torch.isnan(d[bad]).all()) and torch.equal(d[~bad], gradient(inside, which)[~bad])
