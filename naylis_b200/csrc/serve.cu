@@ -484,7 +484,7 @@ decode_split_kernel(const __grid_constant__ DecodeArgs P) {
                     *reinterpret_cast<float4 *>(reinterpret_cast<float *>(dsm) + g * HD + d) = o;
                     if (d == 0) s_part[g] = make_float2(M, L);
                 } else if (whole) {
-                    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+                    const float inv = len.n == 0 && !lost ? 0.0f : 1.0f / L;
                     *reinterpret_cast<uint2 *>(P.out + (static_cast<int64_t>(b) * P.H + h0 + g) * HD + d) =
                         make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
                 } else {
@@ -541,7 +541,7 @@ decode_split_kernel(const __grid_constant__ DecodeArgs P) {
                 o0 = fmaf(f, x[c].x, o0);
                 o1 = fmaf(f, x[c].y, o1);
             }
-            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+            const float inv = len.n == 0 && !len.lost ? 0.0f : 1.0f / L;
             *reinterpret_cast<uint32_t *>(P.out + (static_cast<int64_t>(b) * P.H + h0 + g) * HD + d) =
                 pack_bf16x2(o0 * inv, o1 * inv);
         }
@@ -611,7 +611,7 @@ decode_join_kernel(const __grid_constant__ DecodeArgs P) {
         const DecSum &x = s_sum[w][lane];
         sum.add(x.M, x.L, x.o);
     }
-    const float inv = sum.L == 0.0f ? 0.0f : 1.0f / sum.L;
+    const float inv = 1.0f / sum.L;      // a list that is cut has keys
     *reinterpret_cast<uint2 *>(P.out + (static_cast<int64_t>(list / lists) * P.H + h) * HD + d) =
         make_uint2(pack_bf16x2(sum.o.x * inv, sum.o.y * inv), pack_bf16x2(sum.o.z * inv, sum.o.w * inv));
 }

@@ -30,3 +30,46 @@ def test_decode_without_keys(B, H, Hk, hd, pages):
     lens[0], lens[B - 1] = 1, 1 << 30
     out = attention.decode_attention(q, kp, vp, table, lens, max_len=0)
     assert bool(torch.isnan(out[[0, B - 1]]).all()) and bool((out[1:B - 1] == 0).all())
+
+
+
+def _paged(seed, lens, Hk, page, hd):
+    need = [-(-n // page) for n in lens]
+    kp, vp = _rand(seed, sum(need) + 1, Hk, page, hd), _rand(seed + 1, sum(need) + 1, Hk, page, hd)
+    ids = torch.randperm(sum(need), generator=torch.Generator().manual_seed(seed)).tolist()
+    table = torch.full((len(lens), max(need)), -1, dtype=torch.int32)
+    for b, n in enumerate(need):
+        table[b, :n] = torch.tensor([ids.pop() for _ in range(n)], dtype=torch.int32)
+    return kp, vp, table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV)
+
+
+def _place(table, b, j, page):
+    return int(table[b, j // page]), j % page
+
+
+# lists that fit as clusters, and more than that: spans, one of them over many CTAs
+BATCHES = [([1, 40, 700, 2], 64, 4, 2), ([1, 40, 700, 2], 128, 2, 2), ([5000] + [33] * 199, 64, 4, 4),
+           ([5000] + [33] * 199, 128, 20, 2)]
+
+
+@pytest.mark.parametrize("lens,hd,H,Hk", BATCHES)
+def test_decode_scores_of_minus_infinity(lens, hd, H, Hk):
+    """A sequence whose scores are all -inf has no softmax: NaN, as torch's; one key with a
+    finite score takes all the weight."""
+    from naylis_b200 import attention
+    page = 16
+    kp, vp, table, sl = _paged(4, lens, Hk, page, hd)
+    q = _rand(6, len(lens), H, hd)
+    q[..., 0] = 1.0
+    kp[..., 0] = float("-inf")
+    alone = [0, 17]      # of sequences 0 and 1
+    for b, j in enumerate(alone):
+        if j < lens[b]:
+            at, off = _place(table, b, j, page)
+            kp[at, :, off, 0] = 0.5
+    out = attention.decode_attention(q, kp, vp, table, sl)
+    for b, j in enumerate(alone):
+        at, off = _place(table, b, j, page)
+        want = vp[at, :, off].repeat_interleave(H // Hk, 0)
+        assert torch.equal(out[b], want)
+    assert bool(torch.isnan(out[2:]).all())
