@@ -104,8 +104,8 @@ rope_append_kernel(const uint16_t *__restrict__ qkv, int64_t ld, const float *__
 // between warps), and keep a running maximum, sum and output per head until the list ends.
 // Scores and outputs are m16n8k16 products with the heads as rows: at one query per
 // sequence the tensor pipe is idle whatever the shape, and one instruction serves 1 to 16
-// heads alike. The weights enter as two bf16 terms (p = hi + lo), which the idle pipe gives
-// for free: the result is rounded once. Rows behind the sequence's end are zero-filled by
+// heads alike. The weights enter as two bf16 terms (p = hi + lo, to 2^-16 of p), which the
+// idle pipe gives for free: the result is rounded once. Rows behind the sequence's end are zero-filled by
 // the copy, so stale pages never reach a product. With the join: 64 sequences of 8192, 32
 // heads on 8 of 128: 316 us, 6.8 TB/s (326 with a CTA for each chunk of a list); 4 of 87000 to
 // 131072, 16 heads on 4: 135 us, 6.6 TB/s (143); 128 of 1024, 32 on 8: 91 us, 5.9 TB/s (99);
@@ -407,9 +407,12 @@ decode_split_kernel(const __grid_constant__ DecodeArgs P) {
                     const float ref = m[r] == -INFINITY ? 0.0f : m[r];
                     const float p0 = tc::ex2(s[u][2 * r] - ref), p1 = tc::ex2(s[u][2 * r + 1] - ref);
                     l[r] += p0 + p1;
-                    const uint32_t h = pack_bf16x2(p0, p1);
-                    hi[2 * u + r] = h;
-                    lo[2 * u + r] = pack_bf16x2(p0 - __uint_as_float(h << 16), p1 - __uint_as_float(h & 0xffff0000u));
+                    // hi is cut, not rounded, and lo above 0: an infinite value has the same sign in both
+                    // products. (2^-126 is below a weight's last bit wherever the value is finite.)
+                    const float c0 = __uint_as_float(__float_as_uint(p0) & 0xffff0000u);
+                    const float c1 = __uint_as_float(__float_as_uint(p1) & 0xffff0000u);
+                    hi[2 * u + r] = __byte_perm(__float_as_uint(p0), __float_as_uint(p1), 0x7632);
+                    lo[2 * u + r] = pack_bf16x2(fmaxf(p0 - c0, 0x1p-126f), fmaxf(p1 - c1, 0x1p-126f));
                 }
 #pragma unroll
             for (int d = 0; d < HD / 16; ++d) {

@@ -73,3 +73,45 @@ def test_decode_scores_of_minus_infinity(lens, hd, H, Hk):
         want = vp[at, :, off].repeat_interleave(H // Hk, 0)
         assert torch.equal(out[b], want)
     assert bool(torch.isnan(out[2:]).all())
+
+
+@pytest.mark.parametrize("lens,hd,H,Hk", BATCHES)
+def test_decode_infinite_values(lens, hd, H, Hk):
+    """An infinite value that a sequence sees makes its column infinite, of its sign; two
+    of different signs NaN; the other columns, heads and sequences keep their results."""
+    from naylis_b200 import attention
+    page, inf = 16, float("inf")
+    kp, vp, table, sl = _paged(8, lens, Hk, page, hd)
+    q = _rand(10, len(lens), H, hd)
+    clean = attention.decode_attention(q, kp, vp, table, sl)
+    a, ao = _place(table, 1, 5, page)
+    vp[a, 0, ao, 3], vp[a, Hk - 1, ao, 7] = inf, -inf
+    a, ao = _place(table, 1, 21, page)
+    vp[a, 0, ao, 3], vp[a, 0, ao, 4] = -inf, inf
+    G = H // Hk
+    want = clean.clone()
+    want[1, :G, 3] = float("nan")
+    want[1, :G, 4] = inf
+    want[1, H - G:, 7] = -inf
+    out = attention.decode_attention(q, kp, vp, table, sl)
+    special = ~torch.isfinite(want)
+    assert torch.equal(out[special].nan_to_num(nan=5.0), want[special].nan_to_num(nan=5.0))
+    assert torch.equal(out[~special], clean[~special])
+
+
+@pytest.mark.parametrize("lens,hd,H,Hk", BATCHES)
+def test_decode_is_rounded_once(lens, hd, H, Hk):
+    """The weights' two terms hold them to 2^-16: of the output's half ulp (2^-8 of it),
+    2^-12 of sum p |v| is left for them, the exponential and the sums."""
+    from naylis_b200 import attention
+    page = 16
+    kp, vp, table, sl = _paged(12, lens, Hk, page, hd)
+    q = _rand(14, len(lens), H, hd, scale=2.0)
+    out = attention.decode_attention(q, kp, vp, table, sl).double()
+    for b in (0, 1, 2, 3, len(lens) - 1):
+        ids = table[b, :-(-lens[b] // page)].long()
+        k, v = (t[ids].transpose(1, 2).reshape(-1, Hk, hd)[:lens[b]].double().repeat_interleave(H // Hk, 1)
+                for t in (kp, vp))
+        p = torch.softmax(torch.einsum("hd,jhd->hj", q[b].double(), k) * hd ** -0.5, -1)
+        want, A = torch.einsum("hj,jhd->hd", p, v), torch.einsum("hj,jhd->hd", p, v.abs())
+        assert bool(((out[b] - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -12 * A).all())
