@@ -143,8 +143,8 @@ class Session:
 
     def add(self, prompts):
         """Prefill prompts (lists of token ids) as new sequences; returns the logits
-        (len(prompts), vocab) bf16 of each one's next token. The cache has to reach:
-        nothing is added otherwise."""
+        (len(prompts), vocab) bf16 of each one's next token. Where it raises (the cache
+        does not reach, the pass fails) nothing is added."""
         prompts = self._check_prompts(prompts)
         if not prompts:
             raise RuntimeError("generate: no prompts")
@@ -152,14 +152,14 @@ class Session:
         new = [self.cache.add() for _ in prompts]
         try:
             positions, slots = self.cache.extend(new, lens)
-        except RuntimeError:
+            with self._mode():
+                h, sums = self._prefill(prompts, positions, slots)
+                last = torch.tensor(lens, device=self.device).cumsum(0) - 1
+                logits = trunk.linear_f32grad(h[last], self.model.lm_head.weight)
+        except BaseException:
             for s in new:
                 self.cache.free(s)
             raise
-        with self._mode():
-            h, sums = self._prefill(prompts, positions, slots)
-            last = torch.tensor(lens, device=self.device).cumsum(0) - 1
-            logits = trunk.linear_f32grad(h[last], self.model.lm_head.weight)
         self.sums = sums if self.sums is None else [torch.cat(p) for p in zip(self.sums, sums)]
         self.seqs += new
         return logits

@@ -1,0 +1,84 @@
+"""CPU tests of a Session's book-keeping (naylis_b200/generate.py): the trunk's pass is a
+stand-in, its failures are raised on the host."""
+import types
+
+import pytest
+import torch
+
+from naylis_b200 import attention, generate
+
+D, V, LAYERS = 4, 11, 2
+
+
+class Fails(Exception):
+    pass
+
+
+@pytest.fixture
+def session(monkeypatch):
+    """A Session on the CPU whose pass files nothing, adds each token's id to every layer's
+    router sum and returns hidden states of 1. `session.fail` makes it raise behind the
+    first layer."""
+    monkeypatch.setattr(generate, "_check_model", lambda model: None)
+    monkeypatch.setattr(generate.trunk, "bank_kv", lambda *a: None)
+    monkeypatch.setattr(generate.trunk, "linear_f32grad", lambda x, w: (x @ w.t()).bfloat16())
+    mom = types.SimpleNamespace(k_proj=types.SimpleNamespace(weight=None), v_proj=types.SimpleNamespace(weight=None),
+                                mem_slots=0, router_down=types.SimpleNamespace(weight=None),
+                                router_up=types.SimpleNamespace(weight=None), top_blocks=1)
+    layers = [types.SimpleNamespace(mom=mom) for _ in range(LAYERS)]
+    model = types.SimpleNamespace(
+        config=types.SimpleNamespace(num_hidden_layers=LAYERS, num_attention_heads=2, head_dim=64, vocab_size=V),
+        model=types.SimpleNamespace(embed_tokens=types.SimpleNamespace(weight=torch.ones(V, D)), layers=layers,
+                                    M_blocks=None),
+        lm_head=types.SimpleNamespace(weight=torch.ones(V, D)))
+
+    class Ops:
+        def __init__(self, *a):
+            pass
+
+        def zero_carry(self, x, mode):
+            return None
+
+        def route(self, x, *a):
+            return None, torch.zeros(1, x.shape[1], 1), torch.ones(1, x.shape[1], 1), x.sum(1)
+
+    monkeypatch.setattr(generate, "CudaShardOps", Ops)
+    monkeypatch.setattr(generate.mk, "mom_route_log_gates",
+                        lambda mean, *a: (None, torch.zeros(len(mean), 1, 1), None, torch.zeros(len(mean), 1, 1)))
+    s = generate.Session(model, num_pages=4, page_size=8)
+    s.fail = False
+
+    def run(ids, positions, slots, longest, attend, route, want_k):
+        assert len(ids) == len(positions) == len(slots)
+        y32 = ids.float()[:, None].expand(-1, D)
+        for i in range(LAYERS):
+            route(i, mom, y32)
+            if s.fail:
+                raise Fails
+        return torch.ones(len(ids), D)
+
+    monkeypatch.setattr(s, "_pass", run)
+    return s
+
+
+def _state(s):
+    return (list(s.seqs), [s.cache.length(q) for q in s.seqs], s.cache.free_pages,
+            None if s.sums is None else [t.tolist() for t in s.sums])
+
+
+def test_a_prefill_that_fails_adds_nothing(session):
+    s = session
+    for prompts, error in (([[1, 2, 3]], Fails), ([[1] * 9, [2] * 33], RuntimeError)):
+        s.fail = error is Fails
+        before = _state(s)
+        with pytest.raises(error):
+            s.add(prompts)
+        assert _state(s) == before
+    s.fail = False
+    s.add([[1, 2, 3], [4] * 9])
+    assert _state(s) == (s.seqs, [3, 9], 1, [[[6.0] * D, [36.0] * D]] * LAYERS)
+    s.fail = True
+    before = _state(s)
+    with pytest.raises(Fails):
+        s.add([[5]])
+    assert _state(s) == before
