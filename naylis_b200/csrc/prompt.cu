@@ -138,6 +138,7 @@ struct Cfg {
     static constexpr uint32_t kStage = kM * 128;              // 64 output columns of a half
     static constexpr uint32_t kSmem = kQ + kRing + kStage + kSum + 1024 /*barriers*/ + 1024 /*align*/;
     static_assert(kSmem <= 227 * 1024, "shared memory");
+    static_assert(16 * 4 * HD * 4 <= kQ, "redo_rows' columns");
 };
 
 struct Bars {
@@ -212,36 +213,200 @@ __device__ __forceinline__ bool not_finite(uint32_t pair) {
     return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u;
 }
 
-// Rows of a half whose sums are not finite although their weights are: if the tiles
-// that the mask cuts hold a non-finite value, it may be a hidden one; then the warp's
-// spoilt rows are computed again, a thread each, over the keys that they see alone.
-// (Values that a row does see make it non-finite again, as they should.)
+// What hidden values that are not finite did to the CTA's rows, undone: a warp takes 16
+// rows of a half. A column is spoilt for a row if the tiles that the mask cuts hold such
+// a value there behind the row's last key. Values that the row does see decide the column
+// where they are not finite; else the rows' sums are taken again without the others
+// (m16n8k16 products, operands read as they lie). A row without a softmax (a score of NaN
+// or +inf, or none above -inf) is NaN in every column and stays so. A call of 4096 tokens, 16
+// heads on 4 of 128, takes 65 us; with values that are NaN throughout 123 (they decide
+// everything: 1.2 ms for 860 us at 16384), with the last token's NaN 3.8 ms (16 at
+// 16384), with +inf throughout 3.7 ms. (A thread a row, whatever it saw: 475 ms for NaN.)
 template <int HD>
-__device__ __noinline__ void redo_rows(const Params &P, const Half &h, int k0, int r, bool spoilt) {
-    const int lane = threadIdx.x & 31, hk = h.head / (P.H / P.Hk);
-    const uint16_t *v = P.v + static_cast<int64_t>(k0) * P.v_ld + hk * HD, *k = P.k + static_cast<int64_t>(k0) * P.k_ld + hk * HD;
-    bool any = false;
-    for (int j = max(h.vis, 0) / kN * kN; j < min(h.n * kN, static_cast<int>(P.Tk) - k0); ++j)
-        for (int d = lane; d < HD; d += 32) any |= (v[j * P.v_ld + d] & 0x7f80) == 0x7f80;
-    if (!__any_sync(0xffffffffu, any) || !spoilt) return;
-    const int seen = h.vis + r;
-    const uint16_t *q = P.q + static_cast<int64_t>(h.q0 + r) * P.q_ld + h.head * HD;
-    auto score = [&](int j) {
-        float s = 0.0f;
-        for (int d = 0; d < HD; ++d) s = fmaf(bf16_bits_to_f32(q[d]), bf16_bits_to_f32(k[j * P.k_ld + d]), s);
-        return s * P.scale_log2;
-    };
-    float m = -INFINITY, l = 0.0f;
-    for (int j = 0; j < seen; ++j) m = fmaxf(m, score(j));
-    for (int j = 0; j < seen; ++j) l += tc::ex2(score(j) - m);
-    for (int d0 = 0; d0 < HD; d0 += 32) {
-        float o[32] = {};
-        for (int j = 0; j < seen; ++j) {
-            const float p = tc::ex2(score(j) - m);
-            for (int e = 0; e < 32; ++e) o[e] = fmaf(p, bf16_bits_to_f32(v[j * P.v_ld + d0 + e]), o[e]);
+__device__ __noinline__ void redo_rows(const Params P) {
+    constexpr int kC = HD / 32;      // columns of a lane
+    constexpr unsigned kAll = 0xffffffffu;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r0 = warp % 8 * 16;
+    // of each column: the last value that is not finite in the cut tiles, the first NaN, +inf and -inf
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    int *last = reinterpret_cast<int *>(smem_raw) + warp * 4 * HD, *first = last + HD;
+    Items items(P);
+    for (Item it; items.get(it);) {
+        const Half h = it.h[warp / 8];
+        const int rows = min(h.rows - r0, 16);
+        if (h.n == 0 || rows <= 0) continue;
+        uint16_t *out = P.out + (static_cast<int64_t>(h.q0 + r0) * P.H + h.head) * HD;
+        const int64_t out_ld = static_cast<int64_t>(P.H) * HD;
+        bool spoilt = false;
+#pragma unroll 4
+        for (int i = lane; i < rows * (HD / 8); i += 32) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(out + i / (HD / 8) * out_ld + i % (HD / 8) * 8);
+            spoilt |= not_finite(x.x) || not_finite(x.y) || not_finite(x.z) || not_finite(x.w);
         }
-        uint16_t *dst = P.out + (static_cast<int64_t>(h.q0 + r) * P.H + h.head) * HD + d0;
-        for (int e = 0; e < 32; ++e) dst[e] = f32_to_bf16_bits(o[e] / l);
+        if (!__any_sync(kAll, spoilt)) continue;
+        const int vis = h.vis + r0, hk = h.head / (P.H / P.Hk);      // row i sees vis + i keys
+        const uint16_t *v = P.v + static_cast<int64_t>(it.k0) * P.v_ld + hk * HD;
+        const uint16_t *k = P.k + static_cast<int64_t>(it.k0) * P.k_ld + hk * HD;
+        const int cut = max(h.vis, 0) / kN * kN, end = min(h.n * kN, static_cast<int>(P.Tk) - it.k0);
+        auto bad = [](uint32_t x) { return (x & 0x7f80u) == 0x7f80u; };
+        auto values = [&](int j, uint32_t (&x)[kC / 2]) {      // this lane's columns
+            const uint16_t *row = v + j * P.v_ld + lane * kC;
+            if constexpr (kC == 4) {
+                const uint2 y = *reinterpret_cast<const uint2 *>(row);
+                x[0] = y.x, x[1] = y.y;
+            } else {
+                x[0] = *reinterpret_cast<const uint32_t *>(row);
+            }
+        };
+        int at[kC], most = -1;
+#pragma unroll
+        for (int c = 0; c < kC; ++c) at[c] = -1;
+#pragma unroll 4
+        for (int j = cut; j < end; ++j) {
+            uint32_t x[kC / 2];
+            values(j, x);
+#pragma unroll
+            for (int c = 0; c < kC; ++c)
+                if (bad(x[c / 2] >> (16 * (c & 1)))) at[c] = j;
+        }
+#pragma unroll
+        for (int c = 0; c < kC; ++c) most = max(most, at[c]);
+        if (!__any_sync(kAll, most >= vis)) continue;      // the first row sees the fewest
+        __syncwarp();
+        int begin[3][kC];
+#pragma unroll
+        for (int c = 0; c < kC; ++c) begin[0][c] = begin[1][c] = begin[2][c] = INT32_MAX;
+        for (int j0 = 0; j0 < end; j0 += 8) {
+            bool open = false;      // a column that is spoilt for some row, without a NaN so far
+#pragma unroll
+            for (int c = 0; c < kC; ++c) open |= at[c] >= vis && begin[0][c] == INT32_MAX;
+            if (!__any_sync(kAll, open)) break;
+            uint32_t x[8][kC / 2];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) values(min(j0 + e, end - 1), x[e]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int c = 0; c < kC; ++c) {
+                    const uint32_t y = x[e][c / 2] >> (16 * (c & 1)) & 0xffffu;
+                    const int j = min(j0 + e, end - 1);
+                    if ((y & 0x7fffu) > 0x7f80u) begin[0][c] = min(begin[0][c], j);
+                    if (y == 0x7f80u) begin[1][c] = min(begin[1][c], j);
+                    if (y == 0xff80u) begin[2][c] = min(begin[2][c], j);
+                }
+        }
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+            last[lane * kC + c] = at[c];
+#pragma unroll
+            for (int i = 0; i < 3; ++i) first[lane * kC + c + i * HD] = begin[i][c];
+        }
+        __syncwarp();
+        // what the values seen make of a column: 0 finite, else the result
+        auto decided = [&](int seen, int c) -> uint16_t {
+            const bool nan = first[c] < seen, up = first[c + HD] < seen, down = first[c + 2 * HD] < seen;
+            return nan || (up && down) ? 0x7fff : up ? 0x7f80 : down ? 0xff80 : 0;
+        };
+        uint32_t sums = 0;      // rows whose sums are needed
+        for (int i = 0; i < rows; ++i) {
+            const int seen = vis + i;
+            bool lost = true, need = false, set = false;
+            for (int c = lane; c < HD; c += 32) {
+                const uint16_t to = decided(seen, c);
+                const bool fix = seen > 0 && last[c] >= seen && to != 0x7fff;
+                need |= fix && to == 0;
+                set |= fix;
+                lost &= (out[i * out_ld + c] & 0x7fff) > 0x7f80;
+            }
+            if (!__any_sync(kAll, set)) continue;
+            if (__any_sync(kAll, need) || __all_sync(kAll, lost)) {
+                sums |= 1u << i;
+                continue;
+            }
+            for (int c = lane; c < HD; c += 32) {
+                const uint16_t to = decided(seen, c);
+                if (last[c] >= seen && to != 0x7fff) out[i * out_ld + c] = to;
+            }
+        }
+        if (sums == 0) continue;
+        const int r = lane >> 2, d = 2 * (lane & 3), far = vis + rows;      // far: keys that some row sees, and one
+        const uint16_t *q0 = P.q + static_cast<int64_t>(h.q0 + r0 + min(r, rows - 1)) * P.q_ld + h.head * HD + d;
+        const uint16_t *q1 = P.q + static_cast<int64_t>(h.q0 + r0 + min(r + 8, rows - 1)) * P.q_ld + h.head * HD + d;
+        auto pair = [](const uint16_t *p) { return *reinterpret_cast<const uint32_t *>(p); };
+#pragma unroll 1
+        for (int c0 = 0; c0 < HD; c0 += 64) {
+            float acc[8][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll 1
+            for (int j0 = 0; j0 < far - 1; j0 += 16) {
+                float s[2][4] = {};
+#pragma unroll 2
+                for (int kk = 0; kk < HD / 16; ++kk) {
+                    const uint32_t a[4] = {pair(q0 + 16 * kk), pair(q1 + 16 * kk), pair(q0 + 16 * kk + 8),
+                                           pair(q1 + 16 * kk + 8)};
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const uint16_t *kr = k + min(j0 + 8 * u + r, far - 2) * P.k_ld + 16 * kk + d;
+                        mma_bf16_16816(s[u], a, pair(kr), pair(kr + 8));
+                    }
+                }
+                float top[2] = {m[0], m[1]};
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const bool in = j0 + 8 * u + d + (e & 1) < vis + r + 8 * (e >> 1);
+                        s[u][e] = in ? s[u][e] * P.scale_log2 : -INFINITY;
+                        top[e >> 1] = fmaxf(top[e >> 1], s[u][e]);
+                    }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    top[i] = fmaxf(top[i], __shfl_xor_sync(kAll, top[i], 1));
+                    top[i] = fmaxf(top[i], __shfl_xor_sync(kAll, top[i], 2));
+                    const float f = top[i] > m[i] ? tc::ex2(m[i] - top[i]) : 1.0f;
+                    m[i] = top[i];
+                    l[i] *= f;
+#pragma unroll
+                    for (int t = 0; t < 8; ++t) acc[t][2 * i] *= f, acc[t][2 * i + 1] *= f;
+                }
+                uint32_t p[4];
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float ref = m[i] == -INFINITY ? 0.0f : m[i];
+                        const float x = tc::ex2(s[u][2 * i] - ref), y = tc::ex2(s[u][2 * i + 1] - ref);
+                        l[i] += x + y;
+                        p[2 * u + i] = pack_bf16x2(x, y);
+                    }
+                auto value = [&](int j, int c) {
+                    const uint32_t x = v[min(j, far - 2) * P.v_ld + c];
+                    return bad(x) ? 0u : x;
+                };
+#pragma unroll
+                for (int t = 0; t < 8; ++t) {
+                    const int c = c0 + 8 * t + r;
+                    mma_bf16_16816(acc[t], p, value(j0 + d, c) | value(j0 + d + 1, c) << 16,
+                                   value(j0 + d + 8, c) | value(j0 + d + 9, c) << 16);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                l[i] += __shfl_xor_sync(kAll, l[i], 1);
+                l[i] += __shfl_xor_sync(kAll, l[i], 2);
+                const int row = r + 8 * i, seen = vis + row;
+                if (row >= rows || !(sums >> row & 1u) || !(l[i] > 0.0f && l[i] < INFINITY)) continue;
+#pragma unroll
+                for (int t = 0; t < 8; ++t)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int c = c0 + 8 * t + d + e;
+                        const uint16_t to = decided(seen, c);
+                        if (last[c] >= seen && to != 0x7fff)
+                            out[row * out_ld + c] = to ? to : f32_to_bf16_bits(acc[t][2 * i + e] / l[i]);
+                    }
+            }
+            __syncwarp();
+        }
     }
 }
 
@@ -252,6 +417,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
     using C = Cfg<HD>;
     constexpr int kStages = C::kStages;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
+    __shared__ int s_again;      // set: a row that a hidden value may have spoilt
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
     unsigned char *sbase = smem_raw + (base - raw);
@@ -283,7 +449,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
             tc::mbar_init(&bars->kv_full[s], 1);
             tc::mbar_init(&bars->kv_empty[s], 2);
         }
-        bars->abort = 0;
+        bars->abort = s_again = 0;
         bars->zero = 0.0f;
     }
     if (warp == 12) {
@@ -522,30 +688,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                 again |= !(big < INFINITY) && l < INFINITY && r < h.rows && !none;
             }
         }
-        // A weight of 0 does not hide a NaN or an infinity from a product: rows that a value
-        // behind the mask may have spoilt are done again, by themselves. Behind the loop, since a call in it,
-        // though never made, takes registers from what it does (8 sequences of 2048, 16 heads on 4 of
-        // 128: 128 us, 136 with it; 64 of 256, 16 of 64: 36 and 40).
-        if (ok && __any_sync(0xffffffffu, again)) {
-            Items past(P);
-            for (Item it; past.get(it);) {
-#pragma unroll 1
-                for (int a = 0; a < 2; ++a) {
-                    const Half h = it.h[a];
-                    bool spoilt = false;
-                    if (h.n > 0 && r < h.rows && h.vis + r > 0) {
-                        const uint4 *row = reinterpret_cast<const uint4 *>(P.out + (static_cast<int64_t>(h.q0 + r) * P.H +
-                                                                                    h.head) * HD);
-#pragma unroll 1
-                        for (int c = 0; c < HD / 8; ++c) {
-                            const uint4 x = row[c];
-                            spoilt |= not_finite(x.x) || not_finite(x.y) || not_finite(x.z) || not_finite(x.w);
-                        }
-                    }
-                    if (__any_sync(0xffffffffu, spoilt)) redo_rows<HD>(P, h, it.k0, r, spoilt);
-                }
-            }
-        }
+        if (ok && again) s_again = 1;
     } else {
         tc::regs_dec<C::kRestRegs>();
         if (warp < 14) {
@@ -721,6 +864,15 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
     __syncthreads();
     tc::tc_fence_after();
     if (warp == 12) tc::tmem_dealloc(tmem, kTmemCols);
+    // A weight of 0 does not hide a NaN or an infinity from a product: rows that a value
+    // behind the mask may have spoilt are looked at again, by all warps with the registers of
+    // the launch, in the tiles' memory. Here the call, though never made, costs the other code 1 us (128 us for 8
+    // sequences of 2048, 16 heads on 4 of 128), in the epilogue's loop 8.
+    if (s_again) {
+        if (warp < 8) tc::regs_dec<128>();
+        else tc::regs_inc<128>();
+        redo_rows<HD>(P);
+    }
 }
 
 }  // namespace

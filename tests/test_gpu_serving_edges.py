@@ -115,3 +115,98 @@ def test_decode_is_rounded_once(lens, hd, H, Hk):
         p = torch.softmax(torch.einsum("hd,jhd->hj", q[b].double(), k) * hd ** -0.5, -1)
         want, A = torch.einsum("hj,jhd->hd", p, v), torch.einsum("hj,jhd->hd", p, v.abs())
         assert bool(((out[b] - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -12 * A).all())
+
+
+def _prompt_want(q, k, v, lens, scale):
+    """Per row and column: what the values that a row sees make of it (NaN, or infinities
+    of one sign, there decide; else the sum), in 64 bits, with sum p |v|."""
+    H, G = q.shape[1], q.shape[1] // k.shape[1]
+    outs, sizes, o = [], [], 0
+    for n in lens:
+        qs, ks, vs = (t[o:o + n].double().transpose(0, 1) for t in (q, k.repeat_interleave(G, 1), v.repeat_interleave(G, 1)))
+        see = torch.ones(n, n, dtype=torch.bool, device=DEV).tril()
+        p = torch.softmax((qs @ ks.transpose(1, 2) * scale).masked_fill(~see, float("-inf")), -1)
+        plain = torch.where(torch.isfinite(vs), vs, 0.0)
+        out, size = p @ plain, p @ plain.abs()
+        seen = lambda hit: torch.cummax(hit.int(), 1)[0].bool()
+        nan, up, down = seen(torch.isnan(vs)), seen(vs == float("inf")), seen(vs == float("-inf"))
+        out[up] = float("inf")
+        out[down] = float("-inf")
+        out[nan | (up & down)] = float("nan")
+        out[torch.isnan(p.sum(-1))] = float("nan")
+        outs.append(out.transpose(0, 1))
+        sizes.append(size.transpose(0, 1))
+        o += n
+    return torch.cat(outs), torch.cat(sizes)
+
+
+def _prompt_check(q, k, v, lens):
+    from naylis_b200 import attention
+    scale = 0.25 * q.shape[2] ** -0.5
+    plan = attention.PromptPlan(lens, device=DEV)
+    out = attention.prompt_attention(q, k, v, plan, scale=scale).double()
+    plan.check()
+    want, size = _prompt_want(q, k, v, lens, scale)
+    special = ~torch.isfinite(want)
+    assert torch.equal(torch.isnan(out), torch.isnan(want))
+    assert torch.equal(out[special].nan_to_num(nan=5.0), want[special].nan_to_num(nan=5.0))
+    tol = 2.0 ** -7 + 2.0 ** -12      # weights and output rounded to bf16, the exponential
+    assert bool(((out - want).abs()[~special] <= tol * size[~special] + 2.0 ** -40).all())
+
+
+@pytest.mark.parametrize("hd,H,Hk", [(64, 4, 4), (64, 4, 2), (128, 4, 2), (128, 3, 1)])
+def test_prompt_values_that_are_not_finite(hd, H, Hk):
+    """Each row and column by itself: hidden values leave no trace, seen ones decide, and a
+    row without a softmax is NaN whatever its values are."""
+    lens, inf, nan = [300, 140, 257], float("inf"), float("nan")
+    q, k, v = (_rand(20 + i, sum(lens), h, hd) for i, h in enumerate((H, Hk, Hk)))
+    last = Hk - 1
+    v[200, 0, 3], v[210, 0, 3] = nan, inf
+    v[90, 0, 4], v[220, 0, 4] = -inf, inf
+    v[299, last, 5], v[150, last, 5] = inf, inf
+    v[130, last, 6] = -inf
+    v[299, 0], v[300, 0] = nan, inf              # the first sequence's last row, the second's first
+    k[500, 0, 1] = nan
+    v[520, 0, 7], v[440 + 256, 0, 7] = inf, nan
+    _prompt_check(q, k, v, lens)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("fill", ["nan", "inf", "one", "both"])
+def test_prompt_values_of_a_diverged_model(hd, fill):
+    """Values that are NaN, infinite of one sign or of both throughout, or for one token."""
+    lens, H, Hk = [513, 200], 4, 2
+    q, k, v = (_rand(30 + i, sum(lens), h, hd) for i, h in enumerate((H, Hk, Hk)))
+    if fill == "one":
+        v[500] = float("nan")
+    elif fill == "both":
+        v[:] = torch.where(v > 0, float("inf"), float("-inf")).to(v.dtype)
+    else:
+        v[:] = float(fill)
+    _prompt_check(q, k, v, lens)
+
+
+@pytest.mark.parametrize("hd,H,Hk", [(64, 16, 16), (128, 16, 4)])
+def test_prompt_of_nan_values_takes_no_longer(hd, H, Hk):
+    """A diverged model's values leave nothing to compute again: the call stays within 4
+    times an ordinary one's (the rows are looked at once more: for 4096 rows of 16 heads
+    some 100 us behind the 100 to 150 of the call)."""
+    from naylis_b200 import attention
+    n = 4096
+    q, k, v = (_rand(40 + i, n, h, hd) for i, h in enumerate((H, Hk, Hk)))
+    plan = attention.PromptPlan([n], device=DEV)
+
+    def least(values):
+        best = math.inf
+        for _ in range(5):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(4):
+                attention.prompt_attention(q, k, values, plan)
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    plain = least(v)
+    assert least(torch.full_like(v, float("nan"))) <= 4 * plain
