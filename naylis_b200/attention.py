@@ -238,8 +238,8 @@ class PagedKVCache:
 
     k, v: (n_layers, num_pages, n_kv_heads, page_size, head_dim) bf16; a sequence's
     pages are the same in every layer. The book-keeping is on the host: add() a
-    sequence, extend() sequences by their new tokens (which says where those go),
-    free() one when it is done."""
+    sequence, extend() sequences by their new tokens (which says where those go) or
+    retract() those, free() one when it is done."""
 
     def __init__(self, n_layers: int, num_pages: int, page_size: int, n_kv_heads: int, head_dim: int, *,
                  device="cuda"):
@@ -299,6 +299,19 @@ class PagedKVCache:
             both = np.stack([np.concatenate(pos), np.concatenate(slots)])
         both = torch.from_numpy(both).to(self.k.device)
         return both[0], both[1]
+
+    def retract(self, seqs, counts):
+        """Take the last counts[i] tokens of seqs[i] (each named once) back: what undoes an
+        extend() whose pass failed. Raises, changing nothing, when one has fewer."""
+        seqs, counts = list(seqs), [int(c) for c in counts]
+        if len(seqs) != len(counts) or len(set(seqs)) != len(seqs) or any(
+                not 0 <= c <= self._len[s] for s, c in zip(seqs, counts)):
+            raise RuntimeError("PagedKVCache.retract: one count in [0, length] for each sequence, each named once")
+        for s, c in zip(reversed(seqs), reversed(counts)):
+            self._len[s] -= c
+            pages, keep = self._pages[s], -(-self._len[s] // self.page_size)
+            self._free.extend(reversed(pages[keep:]))
+            del pages[keep:]
 
     def tables(self, seqs):
         """(block_table (B, n), seq_lens (B)) int32 on the device, and the longest

@@ -166,24 +166,37 @@ class Session:
 
     def step(self, tokens):
         """Append tokens (len(self.seqs),) int64 on the device, one to each running
-        sequence; returns the next logits (len(self.seqs), vocab) bf16."""
-        positions, slots = self.cache.extend(self.seqs, [1] * len(self.seqs))
+        sequence; returns the next logits (len(self.seqs), vocab) bf16. Where it raises
+        no sequence has grown."""
+        one = [1] * len(self.seqs)
+        positions, slots = self.cache.extend(self.seqs, one)
+        try:
+            logits, sums = self._step(tokens, positions, slots)
+        except BaseException:
+            self.cache.retract(self.seqs, one)
+            raise
+        self.sums = sums
+        return logits
+
+    def _step(self, tokens, positions, slots):
+        """step()'s pass -> (logits, the router's prefix sums behind it)."""
         table, lens, longest = self.cache.tables(self.seqs)
         count = lens.to(torch.float32)[:, None]
+        sums = []
 
         def attend(i, q, k, v):
             return attention.decode_attention(q, self.cache.k[i], self.cache.v[i], table, lens, max_len=longest)
 
         def route(i, m, y32):
-            self.sums[i] += y32
-            mean = self.sums[i] / count          # the scan's division; a sequence of one row is its own mean
+            sums.append(self.sums[i] + y32)
+            mean = sums[i] / count          # the scan's division; a sequence of one row is its own mean
             _, idx, _, lg = mk.mom_route_log_gates(mean[:, None], m.router_down.weight, m.router_up.weight,
                                                    m.top_blocks)
             return idx.transpose(0, 1), lg.transpose(0, 1)
 
         with self._mode():
             h = self._pass(tokens, positions, slots, longest, attend, route, False)
-            return trunk.linear_f32grad(h, self.model.lm_head.weight)
+            return trunk.linear_f32grad(h, self.model.lm_head.weight), sums
 
     def drop(self, rows):
         """End the sequences at these rows of .seqs and give their pages back."""

@@ -82,3 +82,37 @@ def test_a_prefill_that_fails_adds_nothing(session):
     with pytest.raises(Fails):
         s.add([[5]])
     assert _state(s) == before
+
+
+def test_a_step_that_fails_leaves_the_sequences(session):
+    """Lengths, pages and the router's sums stay, also where the token would have begun a
+    page; the same step then goes through."""
+    s = session
+    s.add([[1, 2, 3], [4] * 8])
+    tokens = torch.tensor([7, 9])
+    before = _state(s)
+    s.fail = True
+    for _ in range(3):
+        with pytest.raises(Fails):
+            s.step(tokens)
+        assert _state(s) == before
+    s.fail = False
+    logits = s.step(tokens)
+    assert logits.shape == (2, V)
+    assert _state(s) == (s.seqs, [4, 9], 1, [[[13.0] * D, [41.0] * D]] * LAYERS)
+
+
+def test_retract():
+    c = attention.PagedKVCache(1, 4, 8, 1, 64, device="cpu")
+    a, b = c.add(), c.add()
+    c.extend([a, b], [8, 3])
+    first = c.extend([a, b], [9, 1])
+    c.retract([a, b], [9, 1])
+    assert (c.length(a), c.length(b), c.free_pages) == (8, 3, 2)
+    assert [t.tolist() for t in c.extend([a, b], [9, 1])] == [t.tolist() for t in first]
+    for seqs, counts in (([a, b], [1, 5]), ([a], [-1]), ([a, a], [1, 1]), ([a], [])):
+        with pytest.raises(RuntimeError):
+            c.retract(seqs, counts)
+    assert (c.length(a), c.length(b), c.free_pages) == (17, 4, 0)
+    c.retract([a, b], [17, 4])
+    assert c.free_pages == 4
