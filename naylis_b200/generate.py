@@ -19,6 +19,7 @@ Its bank's k and v are projected once.
 from __future__ import annotations
 
 import dataclasses
+import operator
 from typing import List, Optional
 
 import torch
@@ -199,14 +200,18 @@ class Session:
             return trunk.linear_f32grad(h, self.model.lm_head.weight), sums
 
     def drop(self, rows):
-        """End the sequences at these rows of .seqs and give their pages back."""
-        rows = set(rows)
+        """End the sequences at these rows of .seqs (0 .. len(.seqs) - 1) and give their pages
+        back. Returns the rows that stay."""
+        rows = {operator.index(i) for i in rows}
+        if any(not 0 <= i < len(self.seqs) for i in rows):
+            raise RuntimeError(f"Session.drop: rows {sorted(rows)} of {len(self.seqs)} sequences")
         for i in rows:
             self.cache.free(self.seqs[i])
         keep = [i for i in range(len(self.seqs)) if i not in rows]
         self.seqs = [self.seqs[i] for i in keep]
         at = torch.tensor(keep, dtype=torch.int64, device=self.device)
-        self.sums = [s[at] for s in self.sums]
+        if self.sums is not None:
+            self.sums = [s[at] for s in self.sums]
         return at
 
 

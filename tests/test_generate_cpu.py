@@ -116,3 +116,20 @@ def test_retract():
     assert (c.length(a), c.length(b), c.free_pages) == (17, 4, 0)
     c.retract([a, b], [17, 4])
     assert c.free_pages == 4
+
+
+def test_drop_takes_rows_that_there_are(session):
+    s = session
+    assert s.drop([]).tolist() == []
+    s.add([[1], [2] * 9, [3]])
+    before = _state(s)
+    for rows in ([-1], [3], [0, 5], [1, -3]):
+        with pytest.raises(RuntimeError):
+            s.drop(rows)
+        assert _state(s) == before
+    with pytest.raises(TypeError):
+        s.drop([1.5])
+    assert _state(s) == before
+    last = s.seqs[2]
+    assert s.drop([0, 1, 1]).tolist() == [2]
+    assert _state(s) == ([last], [1], 3, [[[3.0] * D]] * LAYERS)
