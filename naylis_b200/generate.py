@@ -109,7 +109,9 @@ class Session:
         return trunk.add_rmsnorm(x, pending, net.norm.weight, net.norm.eps)[1]
 
     def _prefill(self, prompts, positions, slots):
-        """Packed prompts through the trunk -> (hidden states, per layer prefix sums)."""
+        """Packed prompts through the trunk -> (hidden states, per layer prefix sums, the
+        plan: its check() tells, once the caller's work is on its way, whether a wait of the
+        attention gave up)."""
         lens = [len(p) for p in prompts]
         plan = attention.PromptPlan(lens, device=self.device)
         ids = torch.tensor([t for p in prompts for t in p], dtype=torch.int64, device=self.device)
@@ -132,7 +134,7 @@ class Session:
             return torch.cat(idx, 1), torch.cat(gates, 1).clamp_min(1e-9).log()
 
         h = self._pass(ids, positions, slots, max(lens), attend, route, True)
-        return h, sums
+        return h, sums, plan
 
     def _check_prompts(self, prompts):
         out = [[int(t) for t in p] for p in prompts]
@@ -154,9 +156,10 @@ class Session:
         try:
             positions, slots = self.cache.extend(new, lens)
             with self._mode():
-                h, sums = self._prefill(prompts, positions, slots)
+                h, sums, plan = self._prefill(prompts, positions, slots)
                 last = torch.tensor(lens, device=self.device).cumsum(0) - 1
                 logits = trunk.linear_f32grad(h[last], self.model.lm_head.weight)
+            plan.check()
         except BaseException:
             for s in new:
                 self.cache.free(s)
@@ -292,10 +295,11 @@ def score(model: NaylisForCausalLM, sequences, *, top_logprobs: int = 0, tempera
     positions = torch.cat([torch.arange(n) for n in lens]).to(session.device)
     slots = torch.full_like(positions, -1)
     with session._mode():
-        h, _ = session._prefill(sequences, positions, slots)
+        h, _, plan = session._prefill(sequences, positions, slots)
         logits = trunk.linear_f32grad(h, model.lm_head.weight)
         targets = torch.tensor([t for s in sequences for t in s[1:] + [-100]], device=session.device)
         r = scoring.token_logprobs(logits, targets, top_k=top_logprobs, temperature=temperature)
+    plan.check()
     out, o = [], 0
     for n in lens:
         out.append(scoring.TokenLogprobs(*(None if t is None else t[o:o + n - 1] for t in r)))

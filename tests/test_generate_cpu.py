@@ -133,3 +133,33 @@ def test_drop_takes_rows_that_there_are(session):
     last = s.seqs[2]
     assert s.drop([0, 1, 1]).tolist() == [2]
     assert _state(s) == ([last], [1], 3, [[[3.0] * D]] * LAYERS)
+
+
+class _Plan:
+    """A PromptPlan that a wait of the attention gave up on, `times` times."""
+    times = 0
+
+    def __init__(self, lens, device):
+        pass
+
+    def check(self):
+        if _Plan.times > 0:
+            _Plan.times -= 1
+            raise attention._lib.MomError(6, "mom_prompt_plan_check", "a bounded device-side wait gave up")
+
+
+def test_a_wait_that_gave_up_is_an_error(session, monkeypatch):
+    monkeypatch.setattr(generate.attention, "PromptPlan", _Plan)
+    s, _Plan.times = session, 1
+    before = _state(s)
+    with pytest.raises(attention._lib.MomError):
+        s.add([[1, 2]])
+    assert _state(s) == before and _Plan.times == 0
+    assert s.add([[1, 2]]).shape == (1, V)
+
+    monkeypatch.setattr(generate, "Session", lambda *a: session)
+    monkeypatch.setattr(generate.scoring, "token_logprobs", lambda x, t, **kw: (t.float(), t.float(), None, None))
+    _Plan.times = 1
+    with pytest.raises(attention._lib.MomError):
+        generate.score(None, [[1, 2, 3]])
+    assert generate.score(None, [[1, 2, 3], [4, 5]])[1].logprob.tolist() == [5.0]
