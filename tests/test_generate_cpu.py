@@ -161,5 +161,5 @@ def test_a_wait_that_gave_up_is_an_error(session, monkeypatch):
     monkeypatch.setattr(generate.scoring, "token_logprobs", lambda x, t, **kw: (t.float(), t.float(), None, None))
     _Plan.times = 1
     with pytest.raises(attention._lib.MomError):
-        generate.score(None, [[1, 2, 3]])
-    assert generate.score(None, [[1, 2, 3], [4, 5]])[1].logprob.tolist() == [5.0]
+        generate.score(session.model, [[1, 2, 3]])
+    assert generate.score(session.model, [[1, 2, 3], [4, 5]])[1].logprob.tolist() == [5.0]
