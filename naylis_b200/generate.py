@@ -169,9 +169,16 @@ class Session:
         return logits
 
     def step(self, tokens):
-        """Append tokens (len(self.seqs),) int64 on the device, one to each running
+        """Append tokens (len(self.seqs),) int32 or int64 on the device, one to each running
         sequence; returns the next logits (len(self.seqs), vocab) bf16. Where it raises
-        no sequence has grown."""
+        (a token outside the vocabulary, no page left, a pass that fails) no sequence has
+        grown."""
+        V = self.model.config.vocab_size
+        if not isinstance(tokens, torch.Tensor) or tokens.shape != (len(self.seqs),) or tokens.dtype not in (
+                torch.int32, torch.int64) or tokens.device != self.device:
+            raise RuntimeError(f"Session.step: tokens must be ({len(self.seqs)},) int32 or int64 on {self.device}")
+        if bool(((tokens < 0) | (tokens >= V)).any()):      # the embedding would fault on them
+            raise RuntimeError(f"Session.step: a token is outside [0, {V})")
         one = [1] * len(self.seqs)
         positions, slots = self.cache.extend(self.seqs, one)
         try:

@@ -163,3 +163,18 @@ def test_a_wait_that_gave_up_is_an_error(session, monkeypatch):
     with pytest.raises(attention._lib.MomError):
         generate.score(session.model, [[1, 2, 3]])
     assert generate.score(session.model, [[1, 2, 3], [4, 5]])[1].logprob.tolist() == [5.0]
+
+
+def test_step_refuses_what_the_embedding_would_fault_on(session):
+    s = session
+    s.add([[1, 2], [3]])
+    before = _state(s)
+    for tokens in (torch.tensor([1, V]), torch.tensor([-1, 1]), torch.tensor([1 << 40, 1]), torch.tensor([1]),
+                   torch.tensor([1, 2, 3]), torch.tensor([[1, 2]]), torch.tensor([1.0, 2.0]),
+                   torch.tensor([True, False]), [1, 2]):
+        with pytest.raises(RuntimeError):
+            s.step(tokens)
+        assert _state(s) == before
+    s.step(torch.tensor([0, V - 1]))
+    s.step(torch.tensor([0, V - 1], dtype=torch.int32))
+    assert [s.cache.length(q) for q in s.seqs] == [4, 3]
