@@ -179,6 +179,8 @@ class Session:
             raise RuntimeError(f"Session.step: tokens must be ({len(self.seqs)},) int32 or int64 on {self.device}")
         if bool(((tokens < 0) | (tokens >= V)).any()):      # the embedding would fault on them
             raise RuntimeError(f"Session.step: a token is outside [0, {V})")
+        if not self.seqs:
+            return torch.empty(0, V, dtype=torch.bfloat16, device=self.device)
         one = [1] * len(self.seqs)
         positions, slots = self.cache.extend(self.seqs, one)
         try:

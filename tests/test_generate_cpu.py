@@ -178,3 +178,15 @@ def test_step_refuses_what_the_embedding_would_fault_on(session):
     s.step(torch.tensor([0, V - 1]))
     s.step(torch.tensor([0, V - 1], dtype=torch.int32))
     assert [s.cache.length(q) for q in s.seqs] == [4, 3]
+
+
+def test_step_without_sequences(session):
+    """Before the first and behind the last: no rows, no pass."""
+    s, none = session, torch.zeros(0, dtype=torch.int64)
+    s.fail = True
+    assert s.step(none).shape == (0, V) and s.step(none).dtype == torch.bfloat16
+    s.fail = False
+    s.add([[1, 2]])
+    s.drop([0])
+    s.fail = True
+    assert s.step(none).shape == (0, V) and s.cache.free_pages == 4
