@@ -43,10 +43,10 @@ class Generation:
 
 
 def _check_model(model):
-    cfg = model.config
-    p = model.model.embed_tokens.weight
-    if not isinstance(model, NaylisForCausalLM) or not p.is_cuda or p.dtype != torch.float32:
+    p = model.model.embed_tokens.weight if isinstance(model, NaylisForCausalLM) else None
+    if p is None or not p.is_cuda or p.dtype != torch.float32:
         raise RuntimeError("generate: a NaylisForCausalLM with fp32 parameters on a CUDA device is needed")
+    cfg = model.config
     if cfg.hidden_size not in (128, 256, 512, 1024, 2048) or cfg.head_dim not in (64, 128):
         raise RuntimeError(f"generate: the serving kernels take hidden_size 128 to 2048 and head_dim 64 or 128, got "
                            f"{cfg.hidden_size} and {cfg.head_dim}")

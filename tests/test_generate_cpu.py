@@ -190,3 +190,14 @@ def test_step_without_sequences(session):
     s.drop([0])
     s.fail = True
     assert s.step(none).shape == (0, V) and s.cache.free_pages == 4
+
+
+def test_models_that_cannot_answer_are_refused():
+    from naylis_b200.decoder import NaylisConfig, NaylisForCausalLM
+    cfg = NaylisConfig(vocab_size=16, hidden_size=128, intermediate_size=128, num_hidden_layers=1,
+                       num_attention_heads=2, mem_size=128, mom_block_size=128, mom_top_blocks=1, mom_router_rank=8)
+    for model in (None, torch.nn.Linear(2, 2), NaylisForCausalLM(cfg)):      # the last is on the CPU
+        for call in (lambda: generate.Session(model, 1), lambda: generate.generate(model, [[1]], 1),
+                     lambda: generate.score(model, [[1, 2]])):
+            with pytest.raises(RuntimeError, match="NaylisForCausalLM"):
+                call()
