@@ -383,7 +383,7 @@ MOM_API int mom_rope_append(const void *qkv, int64_t qkv_ld, const float *cos, c
 /* Attention of one new token per sequence over its cached keys: q (B, H, hd) of
  * row pitch q_ld; block_table (B, table_ld) I32, the pages of each sequence in
  * order; seq_lens (B) I32 on the device, the keys of each sequence (the new
- * token's own among them). out (B, H, hd) = softmax(scale q.k) v, scale > 0. max_len: an
+ * token's own among them). out (B, H, hd) = softmax(scale q.k) v, scale > 0 (in fp32). max_len: an
  * upper bound of seq_lens known to the host (at most table_ld * page_size, and
  * B H (max_len / 16 + 8) at most 2^38); the work is shared out by the lengths, and a
  * workspace of mom_decode_attn_workspace_size bytes joins the parts. A sequence of length <= 0 gets zeros; one longer than max_len,
@@ -397,7 +397,7 @@ MOM_API int mom_decode_attn(const void *q, int64_t q_ld, const void *k_pages, co
 
 /* Causal attention over packed prompts: n sequences one after another in q
  * (Tq, H, hd) and k, v (Tk, Hk, hd), rows of pitch q_ld, k_ld, v_ld; out
- * (Tq, H, hd) contiguous; scale > 0. A sequence may have more keys than queries (its prefix
+ * (Tq, H, hd) contiguous; scale > 0 (in fp32). A sequence may have more keys than queries (its prefix
  * is cached): the mask is aligned at the end, row r of Lq sees keys
  * 0 .. Lk - Lq + r; a row that sees none (Lk < Lq) gets zeros. Values that the
  * mask hides from a row do not reach it, NaN and infinities neither.

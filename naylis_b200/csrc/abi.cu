@@ -873,6 +873,12 @@ int check_attn_geometry(int64_t H, int64_t Hk, int64_t hd) {
     if (hd != 64 && hd != 128) return fail(MOM_ERR_UNSUPPORTED, "head_dim %lld: 64 or 128", (long long)hd);
     return MOM_OK;
 }
+// The kernels work with scale log2 e in fp32: 0 there times a masked score's -inf would be NaN.
+int check_scale(double scale) {
+    const float s = static_cast<float>(scale) * mom::kLog2e;
+    MOM_REQUIRE(std::isfinite(s) && s > 0.0f, "scale must be positive and fit fp32 (got %g)", scale);
+    return MOM_OK;
+}
 int check_cache_geometry(int64_t num_pages, int64_t page_size) {
     MOM_REQUIRE(num_pages >= 0, "num_pages must be >= 0");
     MOM_REQUIRE(page_size >= 8 && page_size <= 256 && (page_size & (page_size - 1)) == 0,
@@ -928,7 +934,7 @@ int mom_decode_attn(const void *q, int64_t q_ld, const void *k_pages, const void
     MOM_REQUIRE(table_ld >= 0 && max_len <= table_ld * page_size, "max_len exceeds the block table (%lld pages of %lld)",
                 (long long)table_ld, (long long)page_size);
     MOM_REQUIRE(q_ld >= H * hd && q_ld % 8 == 0, "q row pitch must hold all heads and be a multiple of 8");
-    MOM_REQUIRE(std::isfinite(scale) && scale > 0.0, "scale must be positive");
+    if ((rc = check_scale(scale))) return rc;
     if (B == 0) return MOM_OK;
     MOM_REQUIRE(q && seq_lens && out, "null pointer argument");
     MOM_REQUIRE(max_len == 0 || (block_table && (num_pages == 0 || (k_pages && v_pages))), "null pointer argument");
@@ -996,7 +1002,7 @@ int mom_prompt_attn(const void *q, int64_t q_ld, const void *k, int64_t k_ld, co
     MOM_REQUIRE(Tq >= 0 && Tk >= 0 && Tq <= (1 << 30) && Tk <= (1 << 30), "packed rows out of range (2^30)");
     MOM_REQUIRE(q_ld >= H * hd && q_ld % 8 == 0 && k_ld >= Hk * hd && k_ld % 8 == 0 && v_ld >= Hk * hd && v_ld % 8 == 0,
                 "row pitches must hold all heads and be multiples of 8");
-    MOM_REQUIRE(std::isfinite(scale) && scale > 0.0, "scale must be positive");
+    if ((rc = check_scale(scale))) return rc;
     if (Tq == 0) return MOM_OK;
     MOM_REQUIRE(q && plan && out && (Tk == 0 || (k && v)), "null pointer argument");
     MOM_REQUIRE(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 16) && aligned(plan, 16),

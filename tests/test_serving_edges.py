@@ -48,3 +48,20 @@ def test_decode_counts_a_span_in_32_bits(lib):
     assert _decode(lib, **long, max_len=1 << 27) == INVALID
     units = fits // 16 + 6
     assert units + lists * units // 296 + units < 1 << 31
+
+
+def _prompt(lib, **kw):
+    a = dict(q=P(256), qld=128, k=P(256), kld=128, v=P(256), vld=128, Tq=3, Tk=3, H=2, Hk=2, hd=64, scale=0.1,
+             plan=P(256), bytes=16 + 152 * 4 + 16 + 16, out=P(256), stream=None)
+    a.update(kw)
+    return lib.mom_prompt_attn(*a.values())
+
+
+def test_a_scale_is_positive_and_finite_in_fp32(lib):
+    """The kernels take it, times log2 e, in fp32."""
+    for scale in (1e-46, 1e-300, 1e39, 1e300, 3e38, 0.0, -1.0, float("inf"), float("nan")):
+        assert _prompt(lib, scale=scale) == INVALID, scale
+        assert _decode(lib, scale=scale) == INVALID, scale
+        assert b"scale" in lib.mom_last_error_string()
+    for scale in (1e-44, 1e-30, 2e38):      # on to the next check
+        assert _decode(lib, scale=scale, max_len=4096, tld=256, ws=None, wsb=0) == WORKSPACE
