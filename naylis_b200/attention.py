@@ -138,11 +138,16 @@ class PromptPlan:
             raise RuntimeError("PromptPlan: lengths, and their sums, must be in [0, 2^30]")
         self.total_q, self.total_k = sum(self.q_lens), sum(self.k_lens)
         self.device = torch.empty(0, device=device).device
-        self._lists = {}
+        self._lists, self._stream = {}, {}      # by head counts: the buffers, the streams that they were made on
 
     def list_for(self, n_heads: int, n_kv_heads: int):
-        """The device buffer of the work list for these head counts."""
+        """The device buffer of the work list for these head counts. The first call copies it
+        from the host, which a graph capture refuses: ask, or run a call, before one."""
         got = self._lists.get((n_heads, n_kv_heads))
+        stream = torch._C._cuda_getCurrentRawStream(self.device.index) if self.device.type == "cuda" else 0
+        if got is not None and stream != self._stream[n_heads, n_kv_heads]:
+            # a list lives until the work of every stream that it was asked for on is done
+            got.record_stream(torch.cuda.current_stream(self.device))
         if got is None:
             n = len(self.q_lens)
             lens = np.asarray(self.q_lens + self.k_lens + (0,), dtype=np.int64)
@@ -153,10 +158,12 @@ class PromptPlan:
             host = torch.empty(size, dtype=torch.uint8)
             _lib.call("mom_prompt_plan", ql, kl, n, n_heads, n_kv_heads, host.data_ptr(), size)
             got = self._lists[n_heads, n_kv_heads] = host.to(self.device)
+            self._stream[n_heads, n_kv_heads] = stream
         return got
 
     def check(self):
-        """Raise if a kernel that used this plan gave up a wait (synchronises)."""
+        """Raise if a kernel that used this plan gave up a wait: of the work before it on the
+        current stream, which it synchronises."""
         for buffer in self._lists.values():
             _lib.call_on(self.device.index, "mom_prompt_plan_check", buffer.data_ptr())
 

@@ -210,3 +210,21 @@ def test_prompt_of_nan_values_takes_no_longer(hd, H, Hk):
 
     plain = least(v)
     assert least(torch.full_like(v, float("nan"))) <= 4 * plain
+
+
+def test_a_plan_outlives_its_use_on_another_stream():
+    """A plan's list, made on one stream and read on another, is not given to a new tensor
+    while the other stream's work is pending. (Nothing reads the list here.)"""
+    from naylis_b200 import attention
+    plan = attention.PromptPlan([300, 20], device=DEV)
+    buffer = plan.list_for(4, 2)
+    at, size = buffer.data_ptr(), buffer.numel()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)      # about 0.1 s
+        assert plan.list_for(4, 2) is buffer
+    del plan, buffer
+    others = [torch.empty(size, dtype=torch.uint8, device=DEV) for _ in range(4)]
+    pending = not side.query()
+    assert all(t.data_ptr() != at for t in others) and pending
+    side.synchronize()
