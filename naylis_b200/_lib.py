@@ -10,6 +10,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libnaylis_mom.so")
@@ -145,6 +146,12 @@ def check(status: int, func: str) -> None:
 def call(name: str, *args) -> None:
     """Call a status-returning entry point and raise MomError on failure."""
     check(getattr(load(), name)(*args), name)
+
+
+def no_tangent(name: str, *tensors) -> None:
+    """Raise if a tensor carries a forward-mode tangent, which the kernels would drop."""
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{name} has no forward-mode derivative: detach its inputs")
 
 
 def call_on(index: int, name: str, *args) -> None:

@@ -30,8 +30,13 @@ def _check(name, *ts):
             raise RuntimeError(f"{name} takes bf16 CUDA tensors, got {t.dtype} on {t.device}")
         if t.device != dev:
             raise RuntimeError(f"{name}: tensors on {dev} and {t.device}")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError(f"{name} is forward only: run it under torch.no_grad() or detach its inputs")
+    _forward_only(name, *ts)
+
+
+def _forward_only(name, *ts):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+        raise RuntimeError(f"{name} is forward only: run it under torch.no_grad() or detach its inputs")
+    _lib.no_tangent(name, *ts)
 
 
 def _rows(name, t, what):
@@ -102,6 +107,7 @@ def rope_append(qkv, cos, sin, positions, k_pages, v_pages, slots, *, n_heads: i
     for t in (cos, sin):
         if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != hd or t.shape != cos.shape or t.device != dev:
             raise RuntimeError(f"rope_append: cos and sin must be (n_pos, {hd}) fp32 on {dev}")
+    _forward_only("rope_append", cos, sin)
     T = qkv.shape[0]
     positions, pcode = _index("rope_append", positions, T, dev, "positions")
     slots, scode = _index("rope_append", slots, T, dev, "slots")

@@ -228,3 +228,36 @@ def test_a_plan_outlives_its_use_on_another_stream():
     pending = not side.query()
     assert all(t.data_ptr() != at for t in others) and pending
     side.synchronize()
+
+
+def test_derivatives_are_refused_not_dropped():
+    """Forward-mode tangents, and tables that require grad, as any input that does."""
+    from torch.autograd import forward_ad
+
+    from naylis_b200 import attention, scoring
+    hd, H, Hk, T = 64, 2, 1, 3
+    qkv = _rand(1, T, (H + 2 * Hk) * hd)
+    kp, vp = _rand(2, 1, Hk, 16, hd), _rand(3, 1, Hk, 16, hd)
+    cos, sin = torch.ones(T, hd, device=DEV), torch.zeros(T, hd, device=DEV)
+    at = torch.arange(T, device=DEV)
+    q, k = _rand(4, T, H, hd), _rand(5, T, Hk, hd)
+    plan = attention.PromptPlan([T], device=DEV)
+    table, lens = torch.zeros(T, 1, dtype=torch.int32, device=DEV), torch.ones(T, dtype=torch.int32, device=DEV)
+    logits, target = torch.randn(T, 50, device=DEV), at
+    calls = [(lambda x: attention.rope_append(x, cos, sin, at, kp, vp, at, n_heads=H), qkv),
+             (lambda x: attention.rope_append(qkv, x, sin, at, kp, vp, at, n_heads=H), cos),
+             (lambda x: attention.rope_append(qkv, cos, x, at, kp, vp, at, n_heads=H), sin),
+             (lambda x: attention.prompt_attention(x, k, k, plan), q),
+             (lambda x: attention.decode_attention(x, kp, vp, table, lens), q)]
+    for call, x in calls:
+        call(x)
+        with pytest.raises(RuntimeError, match="forward only"):
+            call(x.clone().requires_grad_(True))
+        with torch.no_grad():
+            call(x.clone().requires_grad_(True))
+    calls.append((lambda x: scoring.token_logprobs(x, target), logits))
+    with forward_ad.dual_level():
+        for call, x in calls:
+            call(x)
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(forward_ad.make_dual(x, torch.ones_like(x)))

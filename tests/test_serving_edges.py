@@ -65,3 +65,16 @@ def test_a_scale_is_positive_and_finite_in_fp32(lib):
         assert b"scale" in lib.mom_last_error_string()
     for scale in (1e-44, 1e-30, 2e38):      # on to the next check
         assert _decode(lib, scale=scale, max_len=4096, tld=256, ws=None, wsb=0) == WORKSPACE
+
+
+def test_tangents_are_noticed():
+    import torch
+    from torch.autograd import forward_ad
+
+    from naylis_b200 import _lib
+    x = torch.ones(3)
+    _lib.no_tangent("op", x)
+    with forward_ad.dual_level():
+        _lib.no_tangent("op", x)
+        with pytest.raises(RuntimeError, match="op has no forward-mode"):
+            _lib.no_tangent("op", x, forward_ad.make_dual(x, x))
