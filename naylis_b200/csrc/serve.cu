@@ -569,8 +569,10 @@ struct DecSum {
         M = top;
     }
 };
+// (48 registers a thread: at the 40 that were chosen without a word the narrow form at
+// head_dim 64 spilled; 48 sequences of 64 to 4096 44.8 -> 43.9 us.)
 template <int HD, bool Wide>
-__global__ void __launch_bounds__(Wide ? 512 : 128)
+__global__ void __launch_bounds__(Wide ? 512 : 128, Wide ? 2 : 10)
 decode_join_kernel(const __grid_constant__ DecodeArgs P) {
     constexpr int kThreads = Wide ? 512 : 128, kLanes = Wide ? 8 : HD / 4, kGroups = kThreads / kLanes, kRound = 4;
     __shared__ DecSum s_sum[kThreads / 32][kLanes];
