@@ -253,6 +253,8 @@ def generate(model: NaylisForCausalLM, prompts, max_new_tokens: int, *, temperat
     prompts = [list(p) for p in prompts]
     if max_new_tokens < 0 or not (temperature == 0.0 or 1e-6 <= temperature <= 1e6):
         raise RuntimeError(f"generate: max_new_tokens {max_new_tokens}, temperature {temperature}")
+    if page_size not in attention.PAGE_SIZES:
+        raise RuntimeError(f"generate: page_size {page_size} must be one of {attention.PAGE_SIZES}")
     out = [Generation() for _ in prompts]
     if not prompts or max_new_tokens == 0:
         return out

@@ -201,3 +201,9 @@ def test_models_that_cannot_answer_are_refused():
                      lambda: generate.score(model, [[1, 2]])):
             with pytest.raises(RuntimeError, match="NaylisForCausalLM"):
                 call()
+
+
+def test_page_sizes_are_checked_before_they_are_used():
+    for size in (0, -8, 12, 512):
+        with pytest.raises(RuntimeError, match="page_size"):
+            generate.generate(None, [[1, 2]], 3, page_size=size)
