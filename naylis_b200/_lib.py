@@ -149,8 +149,9 @@ def call(name: str, *args) -> None:
 
 
 def no_tangent(name: str, *tensors) -> None:
-    """Raise if a tensor carries a forward-mode tangent, which the kernels would drop."""
-    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+    """Raise if a tensor carries a forward-mode tangent, which the kernels would drop (there
+    are none while forward_ad._current_level is -1)."""
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise RuntimeError(f"{name} has no forward-mode derivative: detach its inputs")
 
 

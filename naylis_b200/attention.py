@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -30,13 +31,15 @@ def _check(name, *ts):
             raise RuntimeError(f"{name} takes bf16 CUDA tensors, got {t.dtype} on {t.device}")
         if t.device != dev:
             raise RuntimeError(f"{name}: tensors on {dev} and {t.device}")
-    _forward_only(name, *ts)
+        if t.requires_grad:
+            _no_grad(name)
+    if forward_ad._current_level >= 0:
+        _lib.no_tangent(name, *ts)
 
 
-def _forward_only(name, *ts):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+def _no_grad(name):
+    if torch.is_grad_enabled():
         raise RuntimeError(f"{name} is forward only: run it under torch.no_grad() or detach its inputs")
-    _lib.no_tangent(name, *ts)
 
 
 def _rows(name, t, what):
@@ -107,7 +110,10 @@ def rope_append(qkv, cos, sin, positions, k_pages, v_pages, slots, *, n_heads: i
     for t in (cos, sin):
         if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != hd or t.shape != cos.shape or t.device != dev:
             raise RuntimeError(f"rope_append: cos and sin must be (n_pos, {hd}) fp32 on {dev}")
-    _forward_only("rope_append", cos, sin)
+        if t.requires_grad:
+            _no_grad("rope_append")
+    if forward_ad._current_level >= 0:
+        _lib.no_tangent("rope_append", cos, sin)
     T = qkv.shape[0]
     positions, pcode = _index("rope_append", positions, T, dev, "positions")
     slots, scode = _index("rope_append", slots, T, dev, "slots")
@@ -144,16 +150,13 @@ class PromptPlan:
             raise RuntimeError("PromptPlan: lengths, and their sums, must be in [0, 2^30]")
         self.total_q, self.total_k = sum(self.q_lens), sum(self.k_lens)
         self.device = torch.empty(0, device=device).device
-        self._lists, self._stream = {}, {}      # by head counts: the buffers, the streams that they were made on
+        self._lists = {}      # by head counts: the buffer, the stream that it was made on
 
     def list_for(self, n_heads: int, n_kv_heads: int):
         """The device buffer of the work list for these head counts. The first call copies it
         from the host, which a graph capture refuses: ask, or run a call, before one."""
-        got = self._lists.get((n_heads, n_kv_heads))
+        got, own = self._lists.get((n_heads, n_kv_heads), (None, 0))
         stream = torch._C._cuda_getCurrentRawStream(self.device.index) if self.device.type == "cuda" else 0
-        if got is not None and stream != self._stream[n_heads, n_kv_heads]:
-            # a list lives until the work of every stream that it was asked for on is done
-            got.record_stream(torch.cuda.current_stream(self.device))
         if got is None:
             n = len(self.q_lens)
             lens = np.asarray(self.q_lens + self.k_lens + (0,), dtype=np.int64)
@@ -163,14 +166,15 @@ class PromptPlan:
                 raise RuntimeError(f"PromptPlan: {_lib.last_error()}")
             host = torch.empty(size, dtype=torch.uint8)
             _lib.call("mom_prompt_plan", ql, kl, n, n_heads, n_kv_heads, host.data_ptr(), size)
-            got = self._lists[n_heads, n_kv_heads] = host.to(self.device)
-            self._stream[n_heads, n_kv_heads] = stream
+            got, own = self._lists[n_heads, n_kv_heads] = host.to(self.device), stream
+        if stream != own:      # the list lives until the work of every stream that asks for it is done
+            got.record_stream(torch.cuda.current_stream(self.device))
         return got
 
     def check(self):
         """Raise if a kernel that used this plan gave up a wait: of the work before it on the
         current stream, which it synchronises."""
-        for buffer in self._lists.values():
+        for buffer, _ in self._lists.values():
             _lib.call_on(self.device.index, "mom_prompt_plan_check", buffer.data_ptr())
 
 

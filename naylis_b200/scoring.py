@@ -10,6 +10,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -85,7 +86,8 @@ def token_logprobs(logits, targets, *, top_k: int = 0, temperature: float = 1.0,
     Differentiable in logprob, entropy and top_logprob. Returns TokenLogprobs."""
     if not logits.is_cuda or logits.dtype not in (torch.bfloat16, torch.float32):
         raise RuntimeError(f"token_logprobs takes bf16 or fp32 CUDA logits, got {logits.dtype} on {logits.device}")
-    _lib.no_tangent("token_logprobs", logits)
+    if forward_ad._current_level >= 0:
+        _lib.no_tangent("token_logprobs", logits)
     shape = logits.shape
     if len(shape) != 2 or shape[1] == 0 or targets.shape != shape[:1] or targets.device != logits.device or \
             targets.dtype.is_floating_point:
