@@ -25,7 +25,7 @@
 // one of 16384 862 us, 1.28 PFLOP/s (under a lasting load 990 us: the power limit takes
 // the clock from 1.9 to 1.6 GHz). head_dim 64 has half the products for the same
 // exponentials: bound by the special-function unit (64 %) and what the softmax waits
-// for: 8 of 2048, 16 heads, 107 us, 642 TFLOP/s. Also tried: exponentials partly on the
+// for: 8 of 2048, 16 heads, 108 us, 635 TFLOP/s. Also tried: exponentials partly on the
 // FMA pipe (no gain while the halves take turns; -2 % at head_dim 64), two softmax
 // warps a row (more exchange than it hides: 717 against 711 us at 16384, head_dim 64),
 // items handed out at run time (the waits for them cost more than their balance gave).
@@ -219,11 +219,11 @@ __device__ __forceinline__ bool not_finite(uint32_t pair) {
 // where they are not finite; else the rows' sums are taken again without the others
 // (m16n8k16 products, operands read as they lie). A row without a softmax (a score of NaN
 // or +inf, or none above -inf) is NaN in every column and stays so. A call of 4096 tokens, 16
-// heads on 4 of 128, takes 65 us; with values that are NaN throughout 123 (they decide
-// everything: 1.2 ms for 860 us at 16384), with the last token's NaN 3.8 ms (16 at
+// heads on 4 of 128, takes 63 us; with values that are NaN throughout 121 (they decide
+// everything: 1.1 ms for 860 us at 16384), with the last token's NaN 3.8 ms (16 at
 // 16384), with +inf throughout 3.7 ms. (A thread a row, whatever it saw: 475 ms for NaN.)
 template <int HD>
-__device__ __noinline__ void redo_rows(const Params P) {
+__device__ __forceinline__ void redo_rows(const Params &P) {
     constexpr int kC = HD / 32;      // columns of a lane
     constexpr unsigned kAll = 0xffffffffu;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r0 = warp % 8 * 16;
@@ -408,6 +408,13 @@ __device__ __noinline__ void redo_rows(const Params P) {
             __syncwarp();
         }
     }
+}
+
+// The same as a call. Inlined, though never run, it costs the other code 0.5 us at
+// head_dim 128 and up to 4 at 64 (64 sequences of 256: 36 -> 40 us), called 2 and 1.
+template <int HD>
+__device__ __noinline__ void call_redo_rows(const Params P) {
+    redo_rows<HD>(P);
 }
 
 template <int HD>
@@ -866,12 +873,13 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
     if (warp == 12) tc::tmem_dealloc(tmem, kTmemCols);
     // A weight of 0 does not hide a NaN or an infinity from a product: rows that a value
     // behind the mask may have spoilt are looked at again, by all warps with the registers of
-    // the launch, in the tiles' memory. Here the call, though never made, costs the other code 1 us (128 us for 8
-    // sequences of 2048, 16 heads on 4 of 128), in the epilogue's loop 8.
+    // the launch, in the tiles' memory. (In the epilogue's loop the call would take registers from
+    // it: 8 sequences of 2048, 16 heads on 4 of 128: 128 us, 136 with it.)
     if (s_again) {
         if (warp < 8) tc::regs_dec<128>();
         else tc::regs_inc<128>();
-        redo_rows<HD>(P);
+        if constexpr (HD == 128) redo_rows<HD>(P);
+        else call_redo_rows<HD>(P);
     }
 }
 
