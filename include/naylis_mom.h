@@ -386,8 +386,9 @@ MOM_API int mom_rope_append(const void *qkv, int64_t qkv_ld, const float *cos, c
  * token's own among them). out (B, H, hd) = softmax(scale q.k) v, scale > 0 (in fp32). max_len: an
  * upper bound of seq_lens known to the host (at most table_ld * page_size, and
  * B H (max_len / 16 + 8) at most 2^38); the work is shared out by the lengths, and a
- * workspace of mom_decode_attn_workspace_size bytes joins the parts. A sequence of length <= 0 gets zeros; one longer than max_len,
- * or with a page outside [0, num_pages) among its keys, gets NaN. What the pages
+ * workspace of mom_decode_attn_workspace_size bytes joins the parts. A sequence of
+ * length <= 0 gets zeros; one longer than max_len, or with a page outside
+ * [0, num_pages) among its keys, or whose scores are all -inf, gets NaN. What the pages
  * hold behind a sequence's end is not read into the result, NaN neither. */
 MOM_API size_t mom_decode_attn_workspace_size(int64_t B, int64_t H, int64_t Hk, int64_t head_dim, int64_t max_len);
 MOM_API int mom_decode_attn(const void *q, int64_t q_ld, const void *k_pages, const void *v_pages, int64_t num_pages,

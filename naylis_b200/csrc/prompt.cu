@@ -21,10 +21,10 @@
 // What bounds it, 148 SMs, B200: head_dim 128 the chain softmax - product with V -
 // scores of the next tile of a half, under which the other half's is laid (a step of
 // both halves takes about 2900 cycles; their products alone 2048): 8 sequences of 2048,
-// 16 heads on 4, 130 us, 1.06 PFLOP/s of the causal half's flops, tensor pipe 51 % busy;
+// 16 heads on 4, 130 us, 1.06 PFLOP/s of the causal half's flops, tensor pipe 56 % busy;
 // one of 16384 862 us, 1.28 PFLOP/s (under a lasting load 990 us: the power limit takes
 // the clock from 1.9 to 1.6 GHz). head_dim 64 has half the products for the same
-// exponentials: bound by the special-function unit (64 %) and what the softmax waits
+// exponentials: bound by the special-function unit (63 %) and what the softmax waits
 // for: 8 of 2048, 16 heads, 108 us, 635 TFLOP/s. Also tried: exponentials partly on the
 // FMA pipe (no gain while the halves take turns; -2 % at head_dim 64), two softmax
 // warps a row (more exchange than it hides: 717 against 711 us at 16384, head_dim 64),

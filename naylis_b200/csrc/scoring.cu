@@ -7,14 +7,14 @@
 // p_j = e^(y_j-m) / Z and G = g + sum a_k:
 //   dx_j = (1/T) (g 1(j=t) + sum_k a_k 1(j=i_k) - p_j (G + h (ln p_j + H)))
 // stats keeps (m, Z, ln Z, H) of each row in fp32 for the backward (m: the reference
-// that the sums are taken against, the maximum up to kSlack). A masked logit (-inf) has
-// probability 0 and gradient 0; a row that holds a NaN or +inf, or nothing but -inf, has
-// NaN everywhere, as its softmax has.
+// that the sums are taken against, the maximum up to kSlack). A masked logit (-inf, or the
+// type's lowest value next to ordinary ones) has probability 0 and gradient 0; a row that
+// holds a NaN or +inf, or nothing but -inf, has NaN everywhere, as its softmax has.
 //
 // Bound by reading the logits (and, backward, writing their gradient). 16376 rows of
-// 32000 in bf16, B200: forward 191 us, 5.5 TB/s (the special-function unit, one
-// exponential an element, is 66 % busy), with 8 alternatives 246 us; backward 302 us,
-// 7.0 TB/s. In fp32, 4096 rows of 32003: forward 92 us, 5.7 TB/s.
+// 32000 in bf16, B200: forward 190 us, 5.5 TB/s (the special-function unit, one
+// exponential an element, is 66 % busy), with 8 alternatives 247 us; backward 303 us,
+// 6.9 TB/s. In fp32, 4096 rows of 32003: forward 89 us, 5.9 TB/s.
 #include <algorithm>
 
 #include "launch.h"

@@ -109,7 +109,7 @@ rope_append_kernel(const uint16_t *__restrict__ qkv, int64_t ld, const float *__
 // the copy, so stale pages never reach a product. With the join: 64 sequences of 8192, 32
 // heads on 8 of 128: 316 us, 6.8 TB/s (326 with a CTA for each chunk of a list); 4 of 87000 to
 // 131072, 16 heads on 4: 135 us, 6.6 TB/s (143); 128 of 1024, 32 on 8: 91 us, 5.9 TB/s (99);
-// 48 of 64 to 4096, 16 heads of 64: 43 us, 4.5 TB/s (46): the spans begin to read after 3.5 us
+// 48 of 64 to 4096, 16 heads of 64: 44 us, 4.5 TB/s (46): the spans begin to read after 3.5 us
 // and end after 30 to 40, an SM's first CTA before its fourth (further, shorter spans for
 // the SMs that are done first: 47 to 52; spans after the CTA's place: 46).
 constexpr int kDecWarps = 4;

@@ -57,7 +57,10 @@ def _check_model(model):
 class Session:
     """Sequences of one model in a paged cache. add() prefills prompts, step()
     appends one token to each running sequence; both return the next token's logits
-    (rows in the order of .seqs). drop() ends sequences."""
+    (rows in the order of .seqs). drop() ends sequences. The weights must not change
+    while a session lives: the cached keys and values, and the bank's, projected once
+    here, are the old ones'. An error raised by add() or step() leaves the session as
+    it was."""
 
     def __init__(self, model: NaylisForCausalLM, num_pages: int, page_size: int = 16):
         _check_model(model)

@@ -80,8 +80,9 @@ def token_logprobs(logits, targets, *, top_k: int = 0, temperature: float = 1.0,
     (R, V) bf16 or fp32 (rows may be strided), with each row's entropy and, for
     top_k > 0 (at most 32), its top_k greatest logits in order: ties to the lowest
     index, NaN above all. A row whose target is ignore_index has logprob 0 (and no
-    gradient from it); a target outside [0, V) gives NaN. A logit of -inf has
-    probability 0; a row with a NaN or +inf, or of nothing but -inf, gives NaN.
+    gradient from it); a target outside [0, V) gives a logprob of NaN. A logit of -inf
+    has probability 0, a finite mask what its softmax gives; a row with a NaN or +inf,
+    or of nothing but -inf, gives NaN.
     Sums are fp32 whatever the logits' dtype; the gradient has the logits' dtype.
     Differentiable in logprob, entropy and top_logprob. Returns TokenLogprobs."""
     if not logits.is_cuda or logits.dtype not in (torch.bfloat16, torch.float32):
