@@ -1033,7 +1033,8 @@ int mom_prompt_plan_check(void *plan, void *stream) {
 namespace {
 int check_logprobs(int dtype, int64_t ld, int64_t R, int64_t V, double temperature, int64_t top) {
     MOM_REQUIRE(is_float_dtype(dtype), "logits must be F32 or BF16");
-    MOM_REQUIRE(R >= 0 && R < (int64_t(1) << 31) && V > 0 && V < (int64_t(1) << 31), "bad logits geometry");
+    // elements of a row are counted in 32 bits, a CTA's span (8192 at most) past its end
+    MOM_REQUIRE(R >= 0 && R < (int64_t(1) << 31) && V > 0 && V <= INT32_MAX - 65536, "bad logits geometry");
     MOM_REQUIRE(ld >= V, "row pitch smaller than the vocabulary");
     MOM_REQUIRE(temperature >= 1e-6 && temperature <= 1e6, "temperature must be in [1e-6, 1e6] (got %g)", temperature);
     MOM_REQUIRE(top >= 0 && top <= mom::kMaxTopLogprobs && top <= V, "top_k must be in [0, min(%d, vocabulary)]",

@@ -78,3 +78,20 @@ def test_tangents_are_noticed():
         _lib.no_tangent("op", x)
         with pytest.raises(RuntimeError, match="op has no forward-mode"):
             _lib.no_tangent("op", x, forward_ad.make_dual(x, x))
+
+
+def _logprobs(lib, R, V, back=False):
+    if back:
+        return lib.mom_logprobs_bwd(P(256), 1, V, P(256), None, P(256), 0, P(256), P(256), P(256), R, V, -100, 1.0, P(256),
+                                    None)
+    return lib.mom_logprobs_fwd(P(256), 1, V, None, R, V, -100, 1.0, 0, P(256), P(256), None, None, None, None)
+
+
+def test_logits_rows_are_counted_in_32_bits(lib):
+    """The threads' steps past a row's end fit too. (A null pointer stops the calls that
+    pass.)"""
+    for back in (False, True):
+        for V in ((1 << 31) - 1, (1 << 31) - 512, 1 << 31):
+            assert _logprobs(lib, 1, V, back) == INVALID and b"geometry" in lib.mom_last_error_string(), V
+        assert _logprobs(lib, 1, (1 << 31) - (1 << 17), back) == INVALID
+        assert b"null" in lib.mom_last_error_string()
