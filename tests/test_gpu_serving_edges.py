@@ -171,6 +171,44 @@ def test_prompt_values_that_are_not_finite(hd, H, Hk):
     _prompt_check(q, k, v, lens)
 
 
+@pytest.mark.parametrize("hd,H,Hk", [(64, 4, 4), (128, 4, 2), (128, 3, 3)])
+@pytest.mark.parametrize("q_lens,k_lens", [([64, 200, 5], [10, 455, 3]), ([300, 130], [172, 258]), ([1, 33, 129], [300, 400, 129])])
+def test_prompt_hidden_values_behind_a_prefix(hd, H, Hk, q_lens, k_lens):
+    """More keys than queries, and fewer (rows without one stay 0): values of the last key
+    of each sequence, and of one in its middle, are NaN or infinite."""
+    from naylis_b200 import attention
+    q, k, v = (_rand(60 + i, n, h, hd) for i, (n, h) in enumerate(
+        ((sum(q_lens), H), (sum(k_lens), Hk), (sum(k_lens), Hk))))
+    end = 0
+    for m in k_lens:
+        v[end + m // 2, 0, 1], v[end + m // 2, Hk - 1, 2] = float("inf"), float("nan")
+        end += m
+        v[end - 1, :, 3], v[end - 1, 0, 4] = float("nan"), float("-inf")
+    scale = 0.25 * hd ** -0.5
+    plan = attention.PromptPlan(q_lens, k_lens, device=DEV)
+    out = attention.prompt_attention(q, k, v, plan, scale=scale).double()
+    plan.check()
+    a = b = 0
+    for n, m in zip(q_lens, k_lens):
+        for r in range(n):
+            seen, got = m - n + r + 1, out[a + r]
+            if seen <= 0:
+                assert bool((got == 0).all())
+                continue
+            ks, vs = (t[b:b + seen].double().repeat_interleave(H // Hk, 1) for t in (k, v))
+            p = torch.softmax(torch.einsum("hd,jhd->hj", q[a + r].double(), ks) * scale, -1)
+            plain = torch.where(torch.isfinite(vs), vs, 0.0)
+            want, size = torch.einsum("hj,jhd->hd", p, plain), torch.einsum("hj,jhd->hd", p, plain.abs())
+            want[(vs == float("inf")).any(0)] = float("inf")
+            want[(vs == float("-inf")).any(0)] = float("-inf")
+            want[torch.isnan(vs).any(0)] = float("nan")
+            special = ~torch.isfinite(want)
+            assert torch.equal(got[special].nan_to_num(nan=5.0), want[special].nan_to_num(nan=5.0))
+            tol = 2.0 ** -7 + 2.0 ** -12
+            assert bool(((got - want).abs()[~special] <= tol * size[~special] + 2.0 ** -40).all())
+        a, b = a + n, b + m
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("fill", ["nan", "inf", "one", "both"])
 def test_prompt_values_of_a_diverged_model(hd, fill):
