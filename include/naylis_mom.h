@@ -396,6 +396,38 @@ MOM_API int mom_decode_attn(const void *q, int64_t q_ld, const void *k_pages, co
                             int64_t max_len, int64_t B, int64_t H, int64_t Hk, int64_t head_dim, double scale,
                             void *out, void *workspace, size_t workspace_bytes, void *stream);
 
+/* The same over a cache in 4 bits. A row (a token's key or value of one head) is cut into
+ * groups of 64 values; a group keeps zero = its least value, scale = bf16((greatest -
+ * least) / 15) and of each value x the number n = round((x - zero) / scale), 0 to 15 (0
+ * where scale is 0): it stands for zero + n scale. A group with a value that is not
+ * finite, or a range beyond fp32, stands for NaN. k_pages, v_pages (num_pages, Hk,
+ * page_size, hd / 2) bytes, the even dimension's number in a byte's low half; scales
+ * (num_pages, Hk, page_size, hd / 64, 4) bf16, the key's scale and zero and the value's.
+ * num_pages * Hk * page_size at most 2^31. Pages and scales 16-byte aligned.
+ *
+ * mom_rope_append_int4: mom_rope_append into such a cache; the numbers are those of the
+ * rotated key rounded to bf16. When k (v) is not NULL it gets what the filed keys
+ * (values) stand for, rounded to bf16, (T, Hk, hd) side by side: what later steps will see. */
+MOM_API int mom_rope_append_int4(const void *qkv, int64_t qkv_ld, const float *cos, const float *sin, int64_t n_pos,
+                                 const void *positions, int pos_dtype, const void *slots, int slot_dtype, int64_t T,
+                                 int64_t H, int64_t Hk, int64_t head_dim, int64_t num_pages, int64_t page_size,
+                                 void *k_pages, void *v_pages, void *scales, void *q, void *k, void *v, void *stream);
+
+/* mom_decode_attn_int4: attention of up to n_new (1 to 64) new tokens of each sequence,
+ * the last ones of its seq_lens keys: q (B, n_new, H, hd), token pitch q_ld; out
+ * (B, n_new, H, hd) contiguous. new_lens (B) I32 on the device, or NULL (n_new of each):
+ * new token j sees the keys 0 .. seq_len - new_len + j; one that sees none, and one at or
+ * behind new_len, gets zeros. A new_len outside [0, n_new] makes the sequence NaN. What a
+ * token does not see does not reach it, NaN neither. Else as mom_decode_attn, with B n_new
+ * H at most 2^30 and B n_new H (max_len / 32 + 8) at most 2^37. */
+MOM_API size_t mom_decode_attn_int4_workspace_size(int64_t B, int64_t n_new, int64_t H, int64_t Hk, int64_t head_dim,
+                                                   int64_t max_len);
+MOM_API int mom_decode_attn_int4(const void *q, int64_t q_ld, const void *k_pages, const void *v_pages,
+                                 const void *scales, int64_t num_pages, int64_t page_size, const int32_t *block_table,
+                                 int64_t table_ld, const int32_t *seq_lens, const int32_t *new_lens, int64_t max_len,
+                                 int64_t B, int64_t n_new, int64_t H, int64_t Hk, int64_t head_dim, double scale,
+                                 void *out, void *workspace, size_t workspace_bytes, void *stream);
+
 /* Causal attention over packed prompts: n sequences one after another in q
  * (Tq, H, hd) and k, v (Tk, Hk, hd), rows of pitch q_ld, k_ld, v_ld; out
  * (Tq, H, hd) contiguous; scale > 0 (in fp32). A sequence may have more keys than queries (its prefix

@@ -9,8 +9,15 @@ token at a time. Per layer:
     prefill   q, k = rope_append(qkv, ...);  o = prompt_attention(q, k, v, plan)
     decode    q, _ = rope_append(qkv, ...);  o = decode_attention(q, pages, table, lens)
 
-All tensors are bf16 CUDA tensors with head_dim 64 or 128; a group of query heads
-may share a key head. Everything else raises. Forward only: an input that requires
+The cache may be held in 4 bits instead (csrc/serve_int4.cu: 9/32 of the memory and of
+a step's bytes), and a step over it may bring several new tokens of a sequence, as a
+check of drafted tokens does:
+
+    prefill   q, k, v = rope_append_int4(qkv, ..., want_kv=True);  o = prompt_attention(q, k, v, plan)
+    decode    q, _, _ = rope_append_int4(qkv, ...);  o = decode_attention_int4(q, *cache, table, lens)
+
+All tensors are bf16 CUDA tensors (pages in 4 bits: uint8) with head_dim 64 or 128; a
+group of query heads may share a key head. Everything else raises. Forward only: an input that requires
 grad raises while grad mode is on (training attends through torch's attention).
 """
 from __future__ import annotations
@@ -84,6 +91,33 @@ def _heads(name, hd, H, Hk):
         raise RuntimeError(f"{name}: {H} query heads are not a multiple of {Hk} key heads")
 
 
+def _projection(name, qkv, cos, sin, positions, slots, H, Hk, hd):
+    """The checked arguments of an append, each as the kernels take it."""
+    _heads(name, hd, H, Hk)
+    if qkv.dim() != 2 or qkv.shape[1] != (H + 2 * Hk) * hd:
+        raise RuntimeError(f"{name}: qkv must be (T, {(H + 2 * Hk) * hd}) for {H} + 2 x {Hk} heads of {hd}, got "
+                           f"{tuple(qkv.shape)}")
+    dev = qkv.device
+    for t in (cos, sin):
+        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != hd or t.shape != cos.shape or t.device != dev:
+            raise RuntimeError(f"{name}: cos and sin must be (n_pos, {hd}) fp32 on {dev}")
+        if t.requires_grad:
+            _no_grad(name)
+    if forward_ad._current_level >= 0:
+        _lib.no_tangent(name, cos, sin)
+    T = qkv.shape[0]
+    positions, pcode = _index(name, positions, T, dev, "positions")
+    slots, scode = _index(name, slots, T, dev, "slots")
+    if qkv.stride(1) != 1 or qkv.data_ptr() % 16 or (T > 1 and (qkv.stride(0) % 8 or qkv.stride(0) < qkv.shape[1])):
+        qkv = qkv.clone(memory_format=torch.contiguous_format)
+    cos, sin = cos.contiguous(), sin.contiguous()
+    if cos.data_ptr() % 16:
+        cos = cos.clone()
+    if sin.data_ptr() % 16:
+        sin = sin.clone()
+    return qkv, cos, sin, positions, pcode, slots, scode
+
+
 # ------------------------------------------------------------------ cache write
 def rope_append(qkv, cos, sin, positions, k_pages, v_pages, slots, *, n_heads: int, want_k: bool = False):
     """Rotate the heads of a fused projection by their tokens' positions and file
@@ -102,28 +136,8 @@ def rope_append(qkv, cos, sin, positions, k_pages, v_pages, slots, *, n_heads: i
     _pages("rope_append", k_pages, v_pages)
     P, Hk, page, hd = k_pages.shape
     H = int(n_heads)
-    _heads("rope_append", hd, H, Hk)
-    if qkv.dim() != 2 or qkv.shape[1] != (H + 2 * Hk) * hd:
-        raise RuntimeError(f"rope_append: qkv must be (T, {(H + 2 * Hk) * hd}) for {H} + 2 x {Hk} heads of {hd}, got "
-                           f"{tuple(qkv.shape)}")
-    dev = qkv.device
-    for t in (cos, sin):
-        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != hd or t.shape != cos.shape or t.device != dev:
-            raise RuntimeError(f"rope_append: cos and sin must be (n_pos, {hd}) fp32 on {dev}")
-        if t.requires_grad:
-            _no_grad("rope_append")
-    if forward_ad._current_level >= 0:
-        _lib.no_tangent("rope_append", cos, sin)
-    T = qkv.shape[0]
-    positions, pcode = _index("rope_append", positions, T, dev, "positions")
-    slots, scode = _index("rope_append", slots, T, dev, "slots")
-    if qkv.stride(1) != 1 or qkv.data_ptr() % 16 or (T > 1 and (qkv.stride(0) % 8 or qkv.stride(0) < qkv.shape[1])):
-        qkv = qkv.clone(memory_format=torch.contiguous_format)
-    cos, sin = cos.contiguous(), sin.contiguous()
-    if cos.data_ptr() % 16:
-        cos = cos.clone()
-    if sin.data_ptr() % 16:
-        sin = sin.clone()
+    qkv, cos, sin, positions, pcode, slots, scode = _projection("rope_append", qkv, cos, sin, positions, slots, H, Hk, hd)
+    T, dev = qkv.shape[0], qkv.device
     q = torch.empty(T, H, hd, dtype=torch.bfloat16, device=dev)
     k = torch.empty(T, Hk, hd, dtype=torch.bfloat16, device=dev) if want_k else None
     _lib.call_on(dev.index, "mom_rope_append", qkv.data_ptr(), qkv.stride(0) if T > 1 else qkv.shape[1], cos.data_ptr(),
@@ -206,6 +220,27 @@ def prompt_attention(q, k, v, plan: PromptPlan, *, scale=None):
 
 
 # ------------------------------------------------------------------ decode
+def _block_table(name, block_table, seq_lens, B, page, max_len, dev):
+    """Checked: (block_table, its pitch, seq_lens, max_len) as the kernels take them."""
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or \
+            block_table.device != dev:
+        raise RuntimeError(f"{name}: block_table must be ({B}, pages) int32 on {dev}")
+    if seq_lens.dtype != torch.int32 or seq_lens.shape != (B,) or seq_lens.device != dev:
+        raise RuntimeError(f"{name}: seq_lens must be ({B},) int32 on {dev}")
+    if block_table.shape[1] > 1 and block_table.stride(1) != 1:
+        block_table = block_table.contiguous()
+    seq_lens = seq_lens.contiguous()
+    table_ld = block_table.stride(0) if B > 1 else block_table.shape[1]
+    if table_ld < block_table.shape[1]:
+        block_table = block_table.contiguous()
+        table_ld = block_table.shape[1]
+    cap = block_table.shape[1] * page
+    max_len = cap if max_len is None else int(max_len)
+    if not 0 <= max_len <= cap:
+        raise RuntimeError(f"{name}: max_len {max_len} must be in [0, {cap}], what the block table holds")
+    return block_table, table_ld, seq_lens, max_len
+
+
 def decode_attention(q, k_pages, v_pages, block_table, seq_lens, *, scale=None, max_len=None):
     """Attention of one new token per sequence over its cached keys: q (B, H, hd)
     bf16; k_pages, v_pages (num_pages, Hk, page_size, hd); block_table (B, n)
@@ -224,28 +259,105 @@ def decode_attention(q, k_pages, v_pages, block_table, seq_lens, *, scale=None, 
         raise RuntimeError(f"decode_attention: q has head_dim {hd}, the cache {hd_k}")
     _heads("decode_attention", hd, H, Hk)
     dev = q.device
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or \
-            block_table.device != dev:
-        raise RuntimeError(f"decode_attention: block_table must be ({B}, pages) int32 on {dev}")
-    if seq_lens.dtype != torch.int32 or seq_lens.shape != (B,) or seq_lens.device != dev:
-        raise RuntimeError(f"decode_attention: seq_lens must be ({B},) int32 on {dev}")
-    if block_table.shape[1] > 1 and block_table.stride(1) != 1:
-        block_table = block_table.contiguous()
-    seq_lens = seq_lens.contiguous()
-    table_ld = block_table.stride(0) if B > 1 else block_table.shape[1]
-    if table_ld < block_table.shape[1]:
-        block_table = block_table.contiguous()
-        table_ld = block_table.shape[1]
-    cap = block_table.shape[1] * page
-    max_len = cap if max_len is None else int(max_len)
-    if not 0 <= max_len <= cap:
-        raise RuntimeError(f"decode_attention: max_len {max_len} must be in [0, {cap}], what the block table holds")
+    block_table, table_ld, seq_lens, max_len = _block_table("decode_attention", block_table, seq_lens, B, page, max_len, dev)
     out = torch.empty(B, H, hd, dtype=torch.bfloat16, device=dev)
     need = _lib.load().mom_decode_attn_workspace_size(B, H, Hk, hd, max_len)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     _lib.call_on(dev.index, "mom_decode_attn", q.data_ptr(), q_ld, k_pages.data_ptr(), v_pages.data_ptr(), P, page,
           block_table.data_ptr(), table_ld, seq_lens.data_ptr(), max_len, B, H, Hk, hd,
           hd ** -0.5 if scale is None else float(scale), out.data_ptr(), None if ws is None else ws.data_ptr(), need)
+    return out
+
+
+# ------------------------------------------------------------------ a cache in 4 bits
+GROUP = 64          # values that share a scale and a zero
+MAX_NEW = 64        # new tokens of a sequence in a step
+
+
+def _pages_int4(name, k_pages, v_pages, scales):
+    for t in (k_pages, v_pages):
+        if t.dtype != torch.uint8 or not t.is_cuda or t.dim() != 4 or t.shape != k_pages.shape or \
+                t.device != k_pages.device or not t.is_contiguous():
+            raise RuntimeError(f"{name}: k_pages and v_pages must both be contiguous (num_pages, n_kv_heads, page_size, "
+                               f"head_dim / 2) uint8 CUDA tensors, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    P, Hk, page, half = k_pages.shape
+    if page not in PAGE_SIZES:
+        raise RuntimeError(f"{name}: page_size {page} must be one of {PAGE_SIZES}")
+    if half not in (32, 64):
+        raise RuntimeError(f"{name}: head_dim {2 * half} must be 64 or 128")
+    if scales.shape != (P, Hk, page, 2 * half // GROUP, 4) or not scales.is_contiguous():
+        raise RuntimeError(f"{name}: scales must be contiguous {(P, Hk, page, 2 * half // GROUP, 4)} for these pages, got "
+                           f"{tuple(scales.shape)}")
+    return P, Hk, page, 2 * half
+
+
+def rope_append_int4(qkv, cos, sin, positions, k_pages, v_pages, scales, slots, *, n_heads: int, want_kv: bool = False):
+    """rope_append into a cache in 4 bits: k_pages, v_pages (num_pages, n_kv_heads,
+    page_size, hd / 2) uint8, scales (num_pages, n_kv_heads, page_size, hd / 64, 4)
+    bf16, written in place.
+
+    Each 64 values of a key (rotated, rounded to bf16) or a value keep zero = the
+    least of them and scale = bf16((greatest - least) / 15), in fp32, and of each x the
+    number n = round((x - zero) / scale), 0 to 15 (0 where scale is 0): it stands for
+    zero + n scale. A group with a value that is not finite, or a range beyond fp32,
+    stands for NaN. Two numbers share a byte, the even dimension's in the low half;
+    the last axis of scales is the key's scale and zero, then the value's.
+
+    Returns (q (T, n_heads, hd) rotated, k, v): with want_kv what the filed keys and
+    values stand for, rounded to bf16, (T, n_kv_heads, hd), so that a prefill attends
+    to what later steps will see; else None."""
+    name = "rope_append_int4"
+    P, Hk, page, hd = _pages_int4(name, k_pages, v_pages, scales)
+    _check(name, qkv, scales)
+    if k_pages.device != qkv.device:
+        raise RuntimeError(f"{name}: tensors on {qkv.device} and {k_pages.device}")
+    H = int(n_heads)
+    qkv, cos, sin, positions, pcode, slots, scode = _projection(name, qkv, cos, sin, positions, slots, H, Hk, hd)
+    T, dev = qkv.shape[0], qkv.device
+    q = torch.empty(T, H, hd, dtype=torch.bfloat16, device=dev)
+    k, v = torch.empty(2, T, Hk, hd, dtype=torch.bfloat16, device=dev) if want_kv else (None, None)
+    _lib.call_on(dev.index, "mom_rope_append_int4", qkv.data_ptr(), qkv.stride(0) if T > 1 else qkv.shape[1],
+                 cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(), pcode, slots.data_ptr(), scode, T, H,
+                 Hk, hd, P, page, k_pages.data_ptr(), v_pages.data_ptr(), scales.data_ptr(), q.data_ptr(),
+                 None if k is None else k.data_ptr(), None if v is None else v.data_ptr())
+    return q, k, v
+
+
+def decode_attention_int4(q, k_pages, v_pages, scales, block_table, seq_lens, *, new_lens=None, scale=None, max_len=None):
+    """Attention of the newest tokens of each sequence over a cache in 4 bits: q
+    (B, n, H, hd) bf16, the last n of each sequence's seq_lens keys (n at most 64), or
+    with new_lens (B) int32 on the device the last new_lens of them, whose queries
+    come first. New token j sees the keys 0 .. seq_len - new_len + j; one that sees none,
+    and rows behind new_len, get zeros. pages and scales as rope_append_int4 files
+    them; block_table, seq_lens, scale and max_len as decode_attention takes them. A
+    sequence longer than max_len, with a page outside the cache or with a new_len
+    outside [0, n]: NaN. What a token does not see does not reach it. Returns
+    (B, n, H, hd) bf16."""
+    name = "decode_attention_int4"
+    P, Hk, page, hd = _pages_int4(name, k_pages, v_pages, scales)
+    _check(name, q, scales)
+    if q.dim() != 4 or q.shape[3] != hd:
+        raise RuntimeError(f"{name}: q must be (sequences, new tokens, heads, {hd}), got {tuple(q.shape)}")
+    if k_pages.device != q.device:
+        raise RuntimeError(f"{name}: tensors on {q.device} and {k_pages.device}")
+    B, n, H, _ = q.shape
+    _heads(name, hd, H, Hk)
+    if not 1 <= n <= MAX_NEW:
+        raise RuntimeError(f"{name}: {n} new tokens must be in [1, {MAX_NEW}]")
+    q, q_ld = _rows(name, q.reshape(B * n, H, hd), "q")
+    dev = q.device
+    if new_lens is not None:
+        if new_lens.dtype != torch.int32 or new_lens.shape != (B,) or new_lens.device != dev:
+            raise RuntimeError(f"{name}: new_lens must be ({B},) int32 on {dev}")
+        new_lens = new_lens.contiguous()
+    block_table, table_ld, seq_lens, max_len = _block_table(name, block_table, seq_lens, B, page, max_len, dev)
+    out = torch.empty(B, n, H, hd, dtype=torch.bfloat16, device=dev)
+    need = _lib.load().mom_decode_attn_int4_workspace_size(B, n, H, Hk, hd, max_len)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _lib.call_on(dev.index, "mom_decode_attn_int4", q.data_ptr(), q_ld, k_pages.data_ptr(), v_pages.data_ptr(),
+                 scales.data_ptr(), P, page, block_table.data_ptr(), table_ld, seq_lens.data_ptr(),
+                 None if new_lens is None else new_lens.data_ptr(), max_len, B, n, H, Hk, hd,
+                 hd ** -0.5 if scale is None else float(scale), out.data_ptr(), None if ws is None else ws.data_ptr(), need)
     return out
 
 
@@ -343,4 +455,5 @@ class PagedKVCache:
         return both[:, 1:], both[:, 0].contiguous(), max((self._len[s] for s in seqs), default=0)
 
 
-__all__ = ["PAGE_SIZES", "PagedKVCache", "PromptPlan", "rope_append", "prompt_attention", "decode_attention"]
+__all__ = ["GROUP", "MAX_NEW", "PAGE_SIZES", "PagedKVCache", "PromptPlan", "rope_append", "rope_append_int4",
+           "prompt_attention", "decode_attention", "decode_attention_int4"]

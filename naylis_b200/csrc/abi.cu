@@ -953,6 +953,82 @@ int mom_decode_attn(const void *q, int64_t q_ld, const void *k_pages, const void
 }
 
 namespace {
+int check_int4_cache(int64_t num_pages, int64_t Hk, int64_t page_size) {
+    int rc = check_cache_geometry(num_pages, page_size);
+    if (rc) return rc;
+    // the kernels count the cache's rows in 32 bits
+    MOM_REQUIRE(num_pages <= (int64_t(1) << 31) / (Hk * page_size), "the cache has more than 2^31 rows");
+    return MOM_OK;
+}
+}  // namespace
+
+int mom_rope_append_int4(const void *qkv, int64_t qkv_ld, const float *cosv, const float *sinv, int64_t n_pos,
+                         const void *positions, int pos_dtype, const void *slots, int slot_dtype, int64_t T, int64_t H,
+                         int64_t Hk, int64_t hd, int64_t num_pages, int64_t page_size, void *k_pages, void *v_pages,
+                         void *scales, void *q, void *k, void *v, void *stream) {
+    int rc = check_attn_geometry(H, Hk, hd);
+    if (rc) return rc;
+    if ((rc = check_int4_cache(num_pages, Hk, page_size))) return rc;
+    MOM_REQUIRE(is_idx_dtype(pos_dtype) && is_idx_dtype(slot_dtype), "positions and slots must be I32 or I64");
+    MOM_REQUIRE(T >= 0 && n_pos >= 0 && T < (int64_t(1) << 31), "bad token or position count");
+    MOM_REQUIRE(qkv_ld >= (H + 2 * Hk) * hd && qkv_ld % 8 == 0, "qkv row pitch must hold all heads and be a multiple of 8");
+    if (T == 0) return MOM_OK;
+    MOM_REQUIRE(qkv && cosv && sinv && positions && slots && q, "null pointer argument");
+    MOM_REQUIRE(num_pages == 0 || (k_pages && v_pages && scales), "null pointer argument");
+    MOM_REQUIRE(aligned(qkv, 16) && aligned(cosv, 16) && aligned(sinv, 16) && aligned(k_pages, 16) &&
+                    aligned(v_pages, 16) && aligned(scales, 16) && aligned(q, 16) && aligned(k, 16) && aligned(v, 16),
+                "buffers must be 16-byte aligned");
+    if ((rc = check_current_device())) return rc;
+    cudaError_t e = mom::launch_rope_append_int4(qkv, qkv_ld, cosv, sinv, n_pos, positions, pos_dtype == MOM_I64, slots,
+                                                 slot_dtype == MOM_I64, T, (int)H, (int)Hk, (int)hd, num_pages,
+                                                 page_shift_of(page_size), k_pages, v_pages, scales, q, k, v,
+                                                 static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? MOM_OK : cuda_fail(e, "rope_append_int4");
+}
+
+size_t mom_decode_attn_int4_workspace_size(int64_t B, int64_t n_new, int64_t H, int64_t Hk, int64_t hd,
+                                           int64_t max_len) {
+    if (B <= 0 || n_new <= 0 || H <= 0 || Hk <= 0 || H < Hk || hd <= 0 || max_len < 0) return 0;
+    return mom::decode_int4_bytes(B, n_new * (H / Hk), Hk, hd, max_len);
+}
+
+int mom_decode_attn_int4(const void *q, int64_t q_ld, const void *k_pages, const void *v_pages, const void *scales,
+                         int64_t num_pages, int64_t page_size, const int32_t *block_table, int64_t table_ld,
+                         const int32_t *seq_lens, const int32_t *new_lens, int64_t max_len, int64_t B, int64_t n_new,
+                         int64_t H, int64_t Hk, int64_t hd, double scale, void *out, void *workspace,
+                         size_t workspace_bytes, void *stream) {
+    int rc = check_attn_geometry(H, Hk, hd);
+    if (rc) return rc;
+    if ((rc = check_int4_cache(num_pages, Hk, page_size))) return rc;
+    MOM_REQUIRE(B >= 0 && B <= 65535, "B must be in [0, 65535] (got %lld)", (long long)B);
+    MOM_REQUIRE(n_new >= 1 && n_new <= 64, "n_new must be in [1, 64] (got %lld)", (long long)n_new);
+    MOM_REQUIRE(max_len >= 0 && max_len <= INT32_MAX, "max_len out of range");
+    // a span, 1/444 of the tiles at most, is counted in 32 bits, and so is a list that ends behind it
+    MOM_REQUIRE(B * n_new * H <= (1 << 30) && B * n_new * H * (max_len / 32 + 8) <= (int64_t(1) << 37),
+                "too many sequences, new tokens, heads and keys (2^30, 2^42)");
+    MOM_REQUIRE(table_ld >= 0 && max_len <= table_ld * page_size, "max_len exceeds the block table (%lld pages of %lld)",
+                (long long)table_ld, (long long)page_size);
+    MOM_REQUIRE(q_ld >= H * hd && q_ld % 8 == 0, "q row pitch must hold all heads and be a multiple of 8");
+    if ((rc = check_scale(scale))) return rc;
+    if (B == 0) return MOM_OK;
+    MOM_REQUIRE(q && seq_lens && out, "null pointer argument");
+    MOM_REQUIRE(max_len == 0 || (block_table && (num_pages == 0 || (k_pages && v_pages && scales))),
+                "null pointer argument");
+    MOM_REQUIRE(aligned(q, 16) && aligned(k_pages, 16) && aligned(v_pages, 16) && aligned(scales, 16) &&
+                    aligned(out, 16) && aligned(workspace, 16),
+                "buffers must be 16-byte aligned");
+    const size_t need = mom_decode_attn_int4_workspace_size(B, n_new, H, Hk, hd, max_len);
+    if (need > 0 && (!workspace || workspace_bytes < need))
+        return fail(MOM_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    if ((rc = check_current_device())) return rc;
+    cudaError_t e = mom::launch_decode_attn_int4(q, q_ld, k_pages, v_pages, scales, num_pages, page_shift_of(page_size),
+                                                 block_table, table_ld, seq_lens, new_lens, max_len, B, (int)n_new,
+                                                 (int)H, (int)Hk, (int)hd, (float)scale, out,
+                                                 static_cast<float *>(workspace), static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? MOM_OK : cuda_fail(e, "decode_attn_int4");
+}
+
+namespace {
 int check_prompt_lens(const int64_t *q_lens, const int64_t *k_lens, int64_t n) {
     MOM_REQUIRE(n >= 0 && n < (int64_t(1) << 31) && (n == 0 || q_lens), "bad sequence count or null lengths");
     int64_t tq = 0, tk = 0;

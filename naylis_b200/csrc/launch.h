@@ -249,6 +249,20 @@ cudaError_t launch_decode_attn(const void *q, int64_t q_ld, const void *kp, cons
                                int64_t max_len, int64_t B, int H, int Hk, int hd, float scale, void *out, float *part,
                                cudaStream_t st);
 
+// The same over a cache in 4 bits (serve_int4.cu): pages (n_pages, Hk, 1 << page_shift, hd / 2)
+// bytes, scales (n_pages, Hk, 1 << page_shift, hd / 64, 4) bf16; up to n_new new tokens of
+// each sequence, `rows` = n_new x heads of a group rows of a key head.
+cudaError_t launch_rope_append_int4(const void *qkv, int64_t ld, const float *cosv, const float *sinv, int64_t n_pos,
+                                    const void *positions, int pos64, const void *slots, int slot64, int64_t T, int H,
+                                    int Hk, int hd, int64_t n_pages, int page_shift, void *kp, void *vp, void *scales,
+                                    void *q, void *k, void *v, cudaStream_t st);
+size_t decode_int4_bytes(int64_t B, int64_t rows, int64_t Hk, int64_t hd, int64_t max_len);
+cudaError_t launch_decode_attn_int4(const void *q, int64_t q_ld, const void *kp, const void *vp, const void *scales,
+                                    int64_t n_pages, int page_shift, const int32_t *table, int64_t table_ld,
+                                    const int32_t *seq_lens, const int32_t *new_lens, int64_t max_len, int64_t B,
+                                    int n_new, int H, int Hk, int hd, float scale, void *out, float *part,
+                                    cudaStream_t st);
+
 // Packed prompts (prompt.cu): the plan's tiles of query rows.
 constexpr int kPromptRows = 256;
 struct PromptTile {

@@ -8,29 +8,11 @@
 #include <algorithm>
 #include <atomic>
 
-#include "launch.h"
-#include "tc_common.cuh"
+#include "decode.cuh"
 
 namespace mom {
 
 namespace {
-
-__device__ __forceinline__ int64_t load_index(const void *p, int i64, int64_t i) {
-    return i64 ? static_cast<const int64_t *>(p)[i] : static_cast<int64_t>(static_cast<const int32_t *>(p)[i]);
-}
-
-__device__ __forceinline__ void unpack8(const uint4 &v, float (&f)[8]) {
-    const uint32_t a[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        f[2 * i] = __uint_as_float(a[i] << 16);
-        f[2 * i + 1] = __uint_as_float(a[i] & 0xFFFF0000u);
-    }
-}
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-    return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
-                      pack_bf16x2(f[6], f[7]));
-}
 
 // ------------------------------------------------------------------ rope_append
 // One thread per (token, head, 8 rotation pairs). Bound by memory: the projection in; q,
@@ -112,9 +94,7 @@ rope_append_kernel(const uint16_t *__restrict__ qkv, int64_t ld, const float *__
 // 48 of 64 to 4096, 16 heads of 64: 44 us, 4.5 TB/s (46): the spans begin to read after 3.5 us
 // and end after 30 to 40, an SM's first CTA before its fourth (further, shorter spans for
 // the SMs that are done first: 47 to 52; spans after the CTA's place: 46).
-constexpr int kDecWarps = 4;
 constexpr int kDecTile = 16;                      // keys of a warp's step
-constexpr int kDecHeads = 16;                     // query heads of a CTA
 constexpr int kDecLeast = 8;                      // tiles of a CTA's span, at least
 // tiles that a list's start and end cost (48 sequences of 64 to 4096: 43 us with 6, 47 with 3, 44 with 10)
 constexpr int kDecListCost = 6;
@@ -129,100 +109,7 @@ struct Dec {
     // the warps' outputs, four heads at a time: [warp][4][HD] fp32
     static constexpr int kSmem = kRing + kDecWarps * 4 * HD * 4;
 };
-
-constexpr int kClusterMost = 8;
-
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-}
-// The same place in the shared memory of the cluster's CTA `rank`.
-__device__ __forceinline__ float2 ld_cluster(const float2 *p, int rank) {
-    uint32_t at;
-    float2 v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];\n" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
-    return v;
-}
-
-struct DecodeArgs {
-    const uint16_t *q, *kp, *vp;
-    const int32_t *table, *seq_lens;
-    int64_t q_ld, table_ld, n_pages, max_len, B;
-    int H, Hk, page_shift, n_chunks, chunk;     // n_chunks, chunk (keys): a cluster's
-    float scale_log2;
-    uint16_t *out;
-    float *part;        // [part][head of the CTA][m, l, -, -, HD]
-    int2 *cut;          // where lists are cut, by the smaller of the two: [list] its first CTA and its number of
-                        // CTAs, or [CTA] the list that begins in its span and ends behind it, and its number
-    bool by_list;
-};
-
-// A sequence's keys as the kernels take them, and its tiles: one without keys for a
-// sequence without (its output is zero) and for one that is too long (NaN).
-struct DecLen {
-    int n, tiles;
-    bool lost;
-    __device__ __forceinline__ DecLen(int32_t len, int64_t max_len) {
-        lost = len > max_len;
-        n = lost || len < 0 ? 0 : len;
-        tiles = max(static_cast<int>((static_cast<unsigned>(n) + kDecTile - 1) / kDecTile), 1);
-    }
-};
-
-// The work of all lists (a sequence's key head), one after another, cut into equal spans
-// for the grid's CTAs. It is counted in tiles, and a list's start and end as kDecListCost
-// of them ahead of its own. Where span blockIdx.x begins:
-struct DecSpan {
-    int64_t base, span;          // units before the list that it begins in, and units of a span
-    int b, y, i, n;              // sequence, list of it, tile of that, the sequence's length
-    int end;                     // the span's end, in units from base
-};
-__device__ __forceinline__ bool decode_span(const DecodeArgs &P, int lists, DecSpan &got) {
-    __shared__ int64_t s_sum[kDecWarps];
-    __shared__ DecSpan s_got;
-    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-    const int per = static_cast<int>((P.B + kDecWarps * 32 - 1) / (kDecWarps * 32));      // sequences of a thread
-    const int64_t b0 = static_cast<int64_t>(t) * per, b1 = min(b0 + per, P.B);
-    int64_t mine = 0;
-    for (int64_t b = b0; b < b1; ++b) mine += DecLen(P.seq_lens[b], P.max_len).tiles + kDecListCost;
-    int64_t upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += v;
-    }
-    if (lane == 31) s_sum[warp] = upto;
-    __syncthreads();
-    int64_t total = 0;
-#pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) {
-        if (w < warp) upto += s_sum[w];
-        total += s_sum[w];
-    }
-    total *= lists;
-    const int64_t span = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(kDecLeast));
-    const int64_t from = blockIdx.x * span;
-    if (from >= total) return false;
-    int64_t base = (upto - mine) * lists;
-    if (from >= base && from < upto * lists) {
-        for (int64_t b = b0; b < b1; ++b) {
-            const int32_t len = P.seq_lens[b];
-            const int units = DecLen(len, P.max_len).tiles + kDecListCost;
-            const int64_t next = base + static_cast<int64_t>(units) * lists;
-            if (from < next) {
-                const int y = static_cast<int>((from - base) / units);
-                base += static_cast<int64_t>(y) * units;
-                s_got = {base, span, static_cast<int>(b), y, max(static_cast<int>(from - base) - kDecListCost, 0), len,
-                         static_cast<int>(min(from + span, total) - base)};
-                break;
-            }
-            base = next;
-        }
-    }
-    __syncthreads();
-    got = s_got;
-    return true;
-}
+using Len = DecLen<kDecTile>;
 
 // Cluster: the chunks of a list are one cluster, which joins its own parts through its
 // shared memory (no second launch, no workspace). For calls that fit the GPU at once:
@@ -243,11 +130,11 @@ decode_split_kernel(const __grid_constant__ DecodeArgs P) {
         const int first = static_cast<int>(blockIdx.x) * P.chunk / kDecTile;
         at = {0, 0, static_cast<int>(blockIdx.z), static_cast<int>(blockIdx.y), first, P.seq_lens[blockIdx.z],
               first + P.chunk / kDecTile + kDecListCost};
-    } else if (!decode_span(P, lists, at)) {
+    } else if (!decode_span<kDecTile, kDecListCost, kDecLeast>(P, lists, at)) {
         if (threadIdx.x == 0 && !P.by_list) P.cut[blockIdx.x] = make_int2(0, 0);
         return;
     }
-    DecLen len(at.n, P.max_len);
+    Len len(at.n, P.max_len);
     // the tiles of a list that are before the span's end
     const int end = at.end;
     const auto tiles_to = [&](int base, int tiles) { return max(min(tiles, end - base - kDecListCost), 0); };
@@ -283,7 +170,7 @@ decode_split_kernel(const __grid_constant__ DecodeArgs P) {
             if (++fy == lists) {
                 fy = 0;
                 ++fb;
-                const DecLen next(flen, P.max_len);
+                const Len next(flen, P.max_len);
                 fn = next.n, fall = next.tiles;
                 flen = fb + 1 < P.B ? P.seq_lens[fb + 1] : 0;
             }
@@ -512,7 +399,7 @@ decode_split_kernel(const __grid_constant__ DecodeArgs P) {
         y = ny;
         if (nb != b) {
             b = nb;
-            len = DecLen(blen, P.max_len);
+            len = Len(blen, P.max_len);
         }
     }
     if (!Cluster && threadIdx.x == 0 && !P.by_list) P.cut[blockIdx.x] = cut;
@@ -550,75 +437,6 @@ decode_split_kernel(const __grid_constant__ DecodeArgs P) {
         }
         cluster_sync();      // nobody leaves while its part is read
     }
-}
-
-// Joins the parts of the lists that are cut: a CTA for each of these, each head and (Wide)
-// each 32 columns. Lanes threads, four columns each, take a part, the others further
-// parts; their sums are joined at the end. Wide is for lists of many parts: 1 sequence of
-// 32768, 32 heads on 2 (148 parts): the call takes 18 us, 34 with the narrow form; 18 parts:
-// 135 and 138 us.
-struct DecSum {
-    float M, L;
-    float4 o;
-    __device__ __forceinline__ void add(float m, float l, float4 x) {
-        // what has a maximum of -inf saw no key, or NaN alone (its sum says so)
-        const float top = fmaxf(M, m), f = M == -INFINITY ? 0.0f : tc::ex2(M - top), g = m == -INFINITY ? 0.0f : tc::ex2(m - top);
-        L = (M == -INFINITY ? L : f * L) + (m == -INFINITY ? l : g * l);
-        o.x = fmaf(g, x.x, f * o.x), o.y = fmaf(g, x.y, f * o.y);
-        o.z = fmaf(g, x.z, f * o.z), o.w = fmaf(g, x.w, f * o.w);
-        M = top;
-    }
-};
-// (48 registers a thread: at the 40 that were chosen without a word the narrow form at
-// head_dim 64 spilled; 48 sequences of 64 to 4096 44.8 -> 43.9 us.)
-template <int HD, bool Wide>
-__global__ void __launch_bounds__(Wide ? 512 : 128, Wide ? 2 : 10)
-decode_join_kernel(const __grid_constant__ DecodeArgs P) {
-    constexpr int kThreads = Wide ? 512 : 128, kLanes = Wide ? 8 : HD / 4, kGroups = kThreads / kLanes, kRound = 4;
-    __shared__ DecSum s_sum[kThreads / 32][kLanes];
-    const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes, warp = threadIdx.x / 32;
-    const int d = (static_cast<int>(blockIdx.z) * kLanes + lane) * 4;
-    const int G = P.H / P.Hk, per = min(G, kDecHeads), groups = (G + kDecHeads - 1) / kDecHeads, lists = P.Hk * groups;
-    asm volatile("griddepcontrol.wait;\n" ::: "memory");      // the parts are written
-    const int2 cut = P.cut[blockIdx.x];
-    const int list = P.by_list ? blockIdx.x : cut.x, cta = P.by_list ? cut.x : blockIdx.x;
-    const int y = list % lists, h = y / groups * G + y % groups * kDecHeads + static_cast<int>(blockIdx.y);
-    if (cut.y <= 1 || h >= (y / groups + 1) * G) return;
-    const int64_t step = static_cast<int64_t>(per) * (HD + 4);
-    const float *src = P.part + (static_cast<int64_t>(cta) + list) * step + blockIdx.y * (HD + 4);
-    DecSum sum = {-INFINITY, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
-    for (int c0 = group; c0 < cut.y; c0 += kRound * kGroups) {
-        float2 ml[kRound];
-        float4 x[kRound];
-#pragma unroll
-        for (int u = 0; u < kRound; ++u) {
-            const int c = c0 + u * kGroups;
-            ml[u] = make_float2(-INFINITY, 0.0f);
-            x[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (c < cut.y) {
-                ml[u] = *reinterpret_cast<const float2 *>(src + c * step);
-                x[u] = *reinterpret_cast<const float4 *>(src + c * step + 4 + d);
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < kRound; ++u) sum.add(ml[u].x, ml[u].y, x[u]);
-    }
-#pragma unroll
-    for (int o = kLanes; o < 32; o <<= 1) {
-        const auto other = [&](float v) { return __shfl_xor_sync(0xffffffffu, v, o); };
-        const float m = other(sum.M), l = other(sum.L);
-        sum.add(m, l, make_float4(other(sum.o.x), other(sum.o.y), other(sum.o.z), other(sum.o.w)));
-    }
-    if (threadIdx.x % 32 < kLanes) s_sum[warp][lane] = sum;
-    __syncthreads();
-    if (group > 0) return;
-    for (int w = 1; w < kThreads / 32; ++w) {
-        const DecSum &x = s_sum[w][lane];
-        sum.add(x.M, x.L, x.o);
-    }
-    const float inv = 1.0f / sum.L;      // a list that is cut has keys
-    *reinterpret_cast<uint2 *>(P.out + (static_cast<int64_t>(list / lists) * P.H + h) * HD + d) =
-        make_uint2(pack_bf16x2(sum.o.x * inv, sum.o.y * inv), pack_bf16x2(sum.o.z * inv, sum.o.w * inv));
 }
 
 }  // namespace
@@ -702,8 +520,8 @@ static cudaError_t launch_decode(const DecodeArgs &p, const DecodeSplit &s, dim3
     cfg.gridDim = dim3(static_cast<unsigned>(std::min(s.ctas, s.lists)), std::min(p.H / p.Hk, kDecHeads), wide ? HD / 32 : 1);
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
-    e = wide ? cudaLaunchKernelEx(&cfg, decode_join_kernel<HD, true>, p)
-             : cudaLaunchKernelEx(&cfg, decode_join_kernel<HD, false>, p);
+    e = wide ? cudaLaunchKernelEx(&cfg, decode_join_kernel<HD, true, false>, p)
+             : cudaLaunchKernelEx(&cfg, decode_join_kernel<HD, false, false>, p);
     count_launch();
     return e;
 }
@@ -728,6 +546,9 @@ cudaError_t launch_decode_attn(const void *q, int64_t q_ld, const void *kp, cons
     p.max_len = max_len;
     p.H = H;
     p.Hk = Hk;
+    p.rows = G;
+    p.per = std::min(G, kDecHeads);
+    p.n_new = 1;
     p.page_shift = page_shift;
     p.B = B;
     p.chunk = s.chunk;

@@ -1,0 +1,869 @@
+// A paged key-value cache in 4 bits: the rotary embedding that files into it, and the
+// attention of one or several new tokens of each sequence over it.
+//
+// A row (a token's key or value of one head) is cut into groups of 64 values. A group
+// keeps zero = its least value and scale = bf16((greatest - least) / 15), and of each
+// value x the number n = round((x - zero) / scale), 0 .. 15; it stands for zero + n scale.
+// Pages (num_pages, Hk, page_size, hd / 2) bytes, the even dimension in a byte's low half;
+// scales (num_pages, Hk, page_size, hd / 64, 4) bf16: the key's scale and zero, the
+// value's. A row of hd 64 is 36 bytes, of hd 128 72: 9/32 of bf16.
+#include <algorithm>
+#include <atomic>
+
+#include "decode.cuh"
+
+namespace mom {
+
+namespace {
+
+// ------------------------------------------------------------------ rope_append
+// One thread per (token, head, 8 rotation pairs), as in the bf16 cache's; the threads of a
+// group find its range with shuffles among themselves.
+template <int HD>
+__global__ void __launch_bounds__(256)
+rope_append_int4_kernel(const uint16_t *__restrict__ qkv, int64_t ld, const float *__restrict__ cosv,
+                        const float *__restrict__ sinv, int64_t n_pos, const void *__restrict__ positions, int pos64,
+                        const void *__restrict__ slots, int slot64, int64_t T, int H, int Hk, int64_t n_slots,
+                        int page_shift, uint8_t *__restrict__ kp, uint8_t *__restrict__ vp,
+                        uint16_t *__restrict__ scales, uint16_t *__restrict__ q, uint16_t *__restrict__ k,
+                        uint16_t *__restrict__ v) {
+    constexpr int kHalf = HD / 2, kThreads = kHalf / 8, kGroups = HD / 64;
+    const int heads = H + 2 * Hk;
+    const int64_t total = T * heads * kThreads;
+    const int lane = threadIdx.x & 31;
+    // the lanes of a head: they pass through the loop together (total and the strides are multiples of them)
+    const uint32_t mates = ((1u << kThreads) - 1) << (lane & ~(kThreads - 1));
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
+         i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+        const int p = static_cast<int>(i % kThreads) * 8;
+        const int h = static_cast<int>(i / kThreads % heads);
+        const int64_t t = i / kThreads / heads;
+        const uint16_t *src = qkv + t * ld + static_cast<int64_t>(h) * HD;
+        uint4 lo = *reinterpret_cast<const uint4 *>(src + p), hi = *reinterpret_cast<const uint4 *>(src + p + kHalf);
+        float x[2][8];
+        unpack8(lo, x[0]);
+        unpack8(hi, x[1]);
+        if (h < H + Hk) {
+            const int64_t pos = load_index(positions, pos64, t);
+            float y1[8], y2[8];
+            if (pos >= 0 && pos < n_pos) {
+                const float *cs = cosv + pos * HD + p, *sn = sinv + pos * HD + p;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    y1[j] = __fadd_rn(__fmul_rn(x[0][j], cs[j]), __fmul_rn(-x[1][j], sn[j]));
+                    y2[j] = __fadd_rn(__fmul_rn(x[1][j], cs[j + kHalf]), __fmul_rn(x[0][j], sn[j + kHalf]));
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y1[j] = y2[j] = __int_as_float(0x7fc00000);
+            }
+            lo = pack8(y1);
+            hi = pack8(y2);
+            if (h < H) {
+                uint16_t *dst = q + (t * H + h) * HD + p;
+                *reinterpret_cast<uint4 *>(dst) = lo;
+                *reinterpret_cast<uint4 *>(dst + kHalf) = hi;
+                continue;
+            }
+            unpack8(lo, x[0]);      // the cache holds the bf16 key's numbers
+            unpack8(hi, x[1]);
+        }
+        // the range of each group: at hd 64 one of all, at hd 128 one of each half of the row
+        float least[2], most[2];
+        bool odd[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            least[s] = most[s] = x[s][0];
+            odd[s] = false;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                least[s] = fminf(least[s], x[s][j]);
+                most[s] = fmaxf(most[s], x[s][j]);
+                odd[s] |= !(fabsf(x[s][j]) < INFINITY);
+            }
+        }
+        if (kGroups == 1) {
+            least[0] = fminf(least[0], least[1]);
+            most[0] = fmaxf(most[0], most[1]);
+            odd[0] |= odd[1];
+        }
+        float step[2];
+#pragma unroll
+        for (int s = 0; s < kGroups; ++s) {
+#pragma unroll
+            for (int o = 1; o < kThreads; o <<= 1) {
+                least[s] = fminf(least[s], __shfl_xor_sync(mates, least[s], o));
+                most[s] = fmaxf(most[s], __shfl_xor_sync(mates, most[s], o));
+            }
+            const float range = __fsub_rn(most[s], least[s]);
+            step[s] = round_bf16(__fmul_rn(range, 1.0f / 15.0f));
+            // a value that is not finite, or a range beyond fp32: the group stands for NaN
+            if (__any_sync(mates, odd[s]) || !(range < INFINITY)) step[s] = least[s] = __int_as_float(0x7fc00000);
+        }
+        if (kGroups == 1) {
+            least[1] = least[0];
+            step[1] = step[0];
+        }
+        uint32_t word[2];
+        float y[2][8];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            word[s] = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float n = 0.0f;
+                if (step[s] > 0.0f) n = fminf(rintf(__fdiv_rn(__fsub_rn(x[s][j], least[s]), step[s])), 15.0f);
+                word[s] |= static_cast<uint32_t>(n) << (4 * j);
+                y[s][j] = __fadd_rn(__fmul_rn(n, step[s]), least[s]);
+            }
+        }
+        const bool value = h >= H + Hk;
+        const int hk = h - H - (value ? Hk : 0);
+        const int64_t slot = load_index(slots, slot64, t);
+        if (slot >= 0 && slot < n_slots) {
+            const int64_t row = (((slot >> page_shift) * Hk + hk) << page_shift) + (slot & ((1 << page_shift) - 1));
+            uint8_t *dst = (value ? vp : kp) + row * (HD / 2) + p / 2;
+            *reinterpret_cast<uint32_t *>(dst) = word[0];
+            *reinterpret_cast<uint32_t *>(dst + kHalf / 2) = word[1];
+            if (p < 8 * kGroups)      // the head's first thread, or its first two: a group each
+                *reinterpret_cast<uint32_t *>(scales + (row * kGroups + p / 8) * 4 + (value ? 2 : 0)) =
+                    pack_bf16x2(p == 0 ? step[0] : step[1], p == 0 ? least[0] : least[1]);
+        }
+        if (uint16_t *to = value ? v : k) {
+            uint16_t *dst = to + (t * Hk + hk) * HD + p;
+            *reinterpret_cast<uint4 *>(dst) = pack8(y[0]);
+            *reinterpret_cast<uint4 *>(dst + kHalf) = pack8(y[1]);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ decode attention
+// out[b, j, h] = sum_t softmax_t(scale q . k_t) v_t over the keys t that new token j sees.
+//
+// With n_t the numbers, s_t, z_t a group's scale and zero and Q the sum of q over it:
+//   q . k_t = sum over groups of s_t (q . n_t) + z_t Q
+//   out     = sum_t (p_t s_t) n_t + sum_t p_t z_t
+// so that neither product needs the values themselves. The numbers enter the m16n8k16
+// products as fp16 straight from memory's bits: a number in bits 0 .. 3 of a half is the
+// subnormal n 2^-24, in bits 4 .. 7 n 2^-20, both exact, for one AND each (and a shift for
+// every second pair); the powers of two go into the queries and out of the results.
+//
+// Scores: rows (heads, new tokens) by keys, as in the bf16 cache's kernel. Outputs the
+// other way round, dimensions by rows: the weights then enter as the second operand in the
+// registers that the scores came in, and 8 rows cost half of what 16 do.
+// The queries of a row are scaled by a power of two to 2^9 .. 2^10 at most, so that fp16
+// holds all their bits. The weights p_t s_t are fp16, scaled to 2^13 at most by a power of
+// two above every scale so far: 11 bits, a quarter of the output's own rounding; weights
+// below 2^-24 of the largest lose bits. Everything else is fp32.
+//
+// A warp takes tiles of 32 keys through its ring as the bf16 kernel does.
+constexpr int kTile = 32;
+constexpr int kLeast = 4;           // tiles of a CTA's span, at least
+constexpr int kListCost = 4;        // tiles that a list's start and end cost
+
+template <int HD, int ROWS>
+struct Dec4 {
+    static constexpr int kStages = 3;
+    static constexpr int kCtas = HD == 64 ? (ROWS == 8 ? 5 : 4) : 3;      // resident on an SM
+    static constexpr int kGroups = HD / 64, kRowBytes = HD / 2, kScaleBytes = 8 * kGroups;
+    static constexpr int kSide = kTile * kRowBytes;
+    static constexpr int kStage = 2 * kSide + kTile * kScaleBytes;
+    static constexpr int kRing = kDecWarps * kStages * kStage;
+    static constexpr int kSmem = kRing + kDecWarps * 8 * HD * 4;          // the warps' outputs, 8 rows at a time
+};
+
+struct Decode4Args : DecodeArgs {
+    const uint8_t *k4, *v4;
+    const uint16_t *scales;
+};
+
+// D(16x8 fp32) += A(16x16 fp16, row) * B(16x8 fp16, col)
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+        "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+    uint32_t v;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(v) : "f"(hi), "f"(lo));
+    return v;
+}
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }      // -126 .. 127
+__device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+__device__ __forceinline__ void lds64(uint32_t (&r)[2], uint32_t at) {
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];\n" : "=r"(r[0]), "=r"(r[1]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t at) {
+    uint32_t r;
+    asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(r) : "r"(at) : "memory");
+    return r;
+}
+__device__ __forceinline__ void lds128(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
+}
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void *src, int src_bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(dst), "l"(src), "r"(src_bytes));
+}
+constexpr uint32_t kEven = 0x000F000Fu, kOdd = 0x00F000F0u;      // numbers 0 and 4, 1 and 5 of a word's eight
+
+// Column 2 c + e of score tile j is key 8 j + 4 e + c: a thread's two columns are then rows
+// of the values that four threads read from four neighbouring rows, without bank conflicts.
+// Keys lie in the ring in the columns' order.
+__device__ __forceinline__ int column_of(int key) { return (key & ~7) | (key & 3) << 1 | (key >> 2 & 1); }
+
+template <int HD, int ROWS, bool Cluster>
+__global__ void __launch_bounds__(kDecWarps * 32, Dec4<HD, ROWS>::kCtas)
+decode_int4_kernel(const __grid_constant__ Decode4Args P) {
+    using C = Dec4<HD, ROWS>;
+    constexpr int NG = C::kGroups, NR = ROWS / 8;
+    extern __shared__ __align__(128) unsigned char dsm[];
+    __shared__ float s_m[kDecWarps][ROWS], s_l[kDecWarps][ROWS], s_z[kDecWarps][NG][ROWS];
+    __shared__ float2 s_part[ROWS];
+    float *s_o = reinterpret_cast<float *>(dsm + C::kRing);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c4 = lane & 3, r8 = lane >> 2;
+    const int G = P.H / P.Hk, groups = (P.rows + P.per - 1) / P.per, lists = P.Hk * groups;
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    DecSpan at;
+    if constexpr (Cluster) {
+        const int first = static_cast<int>(blockIdx.x) * P.chunk / kTile;
+        at = {0, 0, static_cast<int>(blockIdx.z), static_cast<int>(blockIdx.y), first, P.seq_lens[blockIdx.z],
+              first + P.chunk / kTile + kListCost};
+    } else if (!decode_span<kTile, kListCost, kLeast>(P, lists, at)) {
+        if (threadIdx.x == 0 && !P.by_list) P.cut[blockIdx.x] = make_int2(0, 0);
+        return;
+    }
+    using Len = DecLen<kTile>;
+    Len len(at.n, P.max_len);
+    // the tiles of a list that are before the span's end
+    const int end = at.end;
+    const auto tiles_to = [&](int base, int tiles) { return max(min(tiles, end - base - kListCost), 0); };
+
+    // The copies' side of this warp: it takes every fourth tile of the span, whatever list
+    // it is of. A lane looks its own key's page up while the tile before is copied. A page
+    // outside the cache copies nothing and makes the sequence's result NaN.
+    const uint32_t ring = smem_u32(dsm) + warp * C::kStages * C::kStage;
+    const int page_mask = (1 << P.page_shift) - 1;
+    int fbase = 0, fb = at.b, fy = at.y, fhk = fy / groups, fi = at.i, fn = len.n, fall = len.tiles;
+    int fend = tiles_to(fbase, fall);
+    int32_t flen = !Cluster && fb + 1 < P.B ? P.seq_lens[fb + 1] : 0;      // the next sequence's
+    struct Tile {
+        int32_t page;
+        int rows, in_page, hk;      // rows: of the sequence; < 0: no tile
+    };
+    bool more = true, bad[C::kStages] = {};
+    auto look = [&](int step) {
+        Tile tile = {0, -1, 0, 0};
+        if (!more) return tile;
+        fi += step;
+        while (fi >= fend) {
+            fi -= fend;
+            fbase += fall + kListCost;
+            if (Cluster || fbase + kListCost >= end) {
+                more = false;
+                return tile;
+            }
+            if (++fy == lists) {
+                fy = 0;
+                ++fb;
+                const Len next(flen, P.max_len);
+                fn = next.n, fall = next.tiles;
+                flen = fb + 1 < P.B ? P.seq_lens[fb + 1] : 0;
+            }
+            fhk = fy / groups;
+            fend = tiles_to(fbase, fall);
+        }
+        const int64_t j = static_cast<int64_t>(fi) * kTile + lane;
+        tile.rows = min(fn - fi * kTile, kTile);
+        tile.in_page = static_cast<int>(j) & page_mask;
+        tile.hk = fhk;
+        if (lane < tile.rows) tile.page = P.table[fb * P.table_ld + (j >> P.page_shift)];
+        return tile;
+    };
+    auto fetch = [&](int stage, const Tile &tile) {
+        if (tile.rows >= 0) {
+            const uint32_t sk = ring + stage * C::kStage, sv = sk + C::kSide, ss = sv + C::kSide;
+            const bool out = lane < tile.rows && (tile.page < 0 || tile.page >= P.n_pages);
+            const bool any = __any_sync(0xffffffffu, out);
+#pragma unroll
+            for (int e = 0; e < C::kStages; ++e)
+                if (e == stage) bad[e] = any;
+            // rows of the cache are counted in 32 bits (the caller's check), bytes in 64
+            constexpr uint32_t kNone = 0xffffffffu;
+            const uint32_t mine = lane < tile.rows && !out
+                                      ? ((static_cast<uint32_t>(tile.page) * P.Hk + tile.hk) << P.page_shift) + tile.in_page
+                                      : kNone;
+            const uint16_t *sc = mine != kNone ? P.scales + static_cast<uint64_t>(mine) * (4 * NG) : P.scales;
+            const int bytes = mine != kNone ? C::kScaleBytes : 0;
+            const uint32_t sdst = ss + column_of(lane) * C::kScaleBytes;
+            if constexpr (NG == 1) cp_async8(sdst, sc, bytes);
+            else cp_async16(sdst, sc, bytes);
+            constexpr int kChunks = C::kRowBytes / 16, kPer = 32 / kChunks;      // of a row; rows of an instruction
+            const int chunk = lane % kChunks;
+#pragma unroll
+            for (int u = 0; u < kChunks; ++u) {
+                const int r = u * kPer + lane / kChunks, col = column_of(r);
+                const uint32_t row = __shfl_sync(0xffffffffu, mine, r);
+                const bool in = row != kNone;
+                const uint64_t from = in ? static_cast<uint64_t>(row) * C::kRowBytes + chunk * 16 : 0;
+                // at hd 128 a row's two groups change places in every second pair of rows: no bank conflicts
+                const int flip = NG == 1 ? chunk * 16 : (chunk & 1) * 16, kg = chunk >> 1;
+                const uint32_t kdst = sk + col * C::kRowBytes + flip + (NG == 1 ? 0 : 32 * (kg ^ (col >> 1 & 1)));
+                const uint32_t vdst = sv + r * C::kRowBytes + flip + (NG == 1 ? 0 : 32 * (kg ^ (r >> 1 & 1)));
+                cp_async16(kdst, P.k4 + from, in ? 16 : 0);      // zeros behind the end
+                cp_async16(vdst, P.v4 + from, in ? 16 : 0);
+            }
+        }
+        cp_async_commit();
+    };
+    int head = 0;
+    static_assert(C::kStages == 3);
+    const Tile tile0 = look(warp), tile1 = look(kDecWarps);      // both tables' reads under way together
+    fetch(0, tile0);
+    fetch(1, tile1);
+    Tile tile = look(kDecWarps);
+
+    // The products' side, list by list. Queries: rows r8 (+ 8); of each group the 16
+    // dimensions from 16 c4 on, as the numbers of a thread's two words pair up. even: those
+    // that meet numbers in the low places, 16 times the others.
+    uint32_t qa[NG][4][2 * NR];
+    float crow[NR], qsum[NG][NR];      // scores from products; the queries' sums in the products' units
+    auto queries = [&](int qb, int qy) {
+        const int row0 = qy % groups * P.per, nr = min(P.per, P.rows - row0), hk = qy / groups;
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            const int mine = r8 + 8 * r, row = row0 + mine;
+            uint4 raw[NG][2];
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    raw[g][w] = make_uint4(0, 0, 0, 0);
+                    if (mine < nr)
+                        raw[g][w] = *reinterpret_cast<const uint4 *>(
+                            P.q + (static_cast<int64_t>(qb) * P.n_new + row / G) * P.q_ld +
+                            static_cast<int64_t>(hk * G + row % G) * HD + 64 * g + 16 * c4 + 8 * w);
+                }
+            uint32_t top = 0;      // the greatest magnitude's bits
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const uint32_t x[4] = {raw[g][w].x, raw[g][w].y, raw[g][w].z, raw[g][w].w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top = max(top, max(x[e] & 0x7fffu, x[e] >> 16 & 0x7fffu));
+                }
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // 2^up takes the greatest to 2^9 .. 2^10 (a row of tiny values not as far up: its scores are equal anyway)
+            const int up = min(136 - static_cast<int>(top >> 7), 100);
+            const float f = pow2(up);
+            // positive and finite: beyond these bounds one key has all the weight, or all have the same
+            crow[r] = fminf(fmaxf(P.scale_log2 * pow2(min(20 - up, 127)), 1e-37f), 3e38f);
+            if (top >= 0x7f80u) crow[r] = __int_as_float(0x7fc00000);            // a query that is not finite
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    float x[8];
+                    unpack8(raw[g][w], x);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        x[e] *= f;
+                        sum += x[e];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        qa[g][2 * w + e][r] = pack_f16x2(16.0f * x[2 * e], 16.0f * x[2 * e + 4]);
+                        qa[g][2 * w + e][NR + r] = pack_f16x2(x[2 * e + 1], x[2 * e + 5]);
+                    }
+                }
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                qsum[g][r] = sum * 0x1p-20f;
+            }
+        }
+    };
+    int b = at.b, y = at.y, i0 = at.i, taken = 0;
+    queries(b, y);
+    DecNew fresh(P, b, at.n);
+    int2 cut = make_int2(0, 0);
+    for (int base = 0; Cluster || base + kListCost < end;) {
+        const int row0 = y % groups * P.per, nr = min(P.per, P.rows - row0);
+        const int tiles = tiles_to(base, len.tiles) - i0;
+        bool lost = len.lost || fresh.lost;
+        // keys that this thread's rows see (of rows that are no new token's: whatever there is), and that all see
+        int sees[NR];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            const int j = (row0 + r8 + 8 * r) / G;
+            sees[r] = j < fresh.count ? fresh.first + j : INT32_MAX;
+        }
+        const int all_see = row0 / G < fresh.count ? fresh.first + row0 / G : INT32_MAX;
+        float acc[NG][4][NR][4], m[NR], l[NR], z[NG][NR];
+        int top[NG];        // 2^(top - 127) is above every scale so far
+#pragma unroll
+        for (int r = 0; r < NR; ++r) m[r] = -INFINITY, l[r] = 0.0f;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            top[g] = 15;
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                z[g][r] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[g][i][r][e] = 0.0f;
+            }
+        }
+        for (int i = (warp - taken) & (kDecWarps - 1); i < tiles; i += kDecWarps) {
+            cp_async_wait<C::kStages - 2>();
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < C::kStages; ++e)
+                if (e == head) lost |= bad[e];
+            const int key0 = (i0 + i) * kTile;
+            const uint32_t sk = ring + head * C::kStage, sv = sk + C::kSide, ss = sv + C::kSide;
+            // scales and zeros of this thread's columns: [key's, value's] of column 2 c4, of 2 c4 + 1
+            uint32_t sc[NG][4][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if constexpr (NG == 1) {
+                    lds128(sc[0][j], ss + (8 * j + 2 * c4) * 8);
+                } else {
+                    uint32_t x[2][4];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) lds128(x[e], ss + (8 * j + 2 * c4 + e) * 16);
+#pragma unroll
+                    for (int g = 0; g < NG; ++g)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sc[g][j][e] = x[e >> 1][2 * g + (e & 1)];
+                }
+            float t[4][2 * NR];
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t w[2];
+                    lds64(w, sk + (8 * j + r8) * C::kRowBytes + 8 * c4 + (NG == 1 ? 0 : 32 * (g ^ (r8 >> 1 & 1))));
+                    float d[4] = {};
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) {
+                        const uint32_t x = s & 1 ? w[s >> 1] >> 8 : w[s >> 1];
+                        if constexpr (NR == 1) mma_f16(d, qa[g][s][0], 0u, qa[g][s][1], 0u, x & kEven, x & kOdd);
+                        else mma_f16(d, qa[g][s][0], qa[g][s][1], qa[g][s][2], qa[g][s][3], x & kEven, x & kOdd);
+                    }
+#pragma unroll
+                    for (int r = 0; r < NR; ++r)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float zero = bf_hi(sc[g][j][2 * e]) * qsum[g][r];
+                            t[j][2 * r + e] = fmaf(bf_lo(sc[g][j][2 * e]), d[2 * r + e],
+                                                   g == 0 ? zero : t[j][2 * r + e] + zero);
+                        }
+                }
+            const bool masked = key0 + kTile > all_see;
+            if (masked) {
+#pragma unroll
+                for (int r = 0; r < NR; ++r)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            if (key0 + 8 * j + 4 * e + c4 >= sees[r]) t[j][2 * r + e] = -INFINITY;
+            }
+            float mx[NR];
+            bool grown = false;
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                mx[r] = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mx[r] = fmaxf(mx[r], fmaxf(t[j][2 * r], t[j][2 * r + 1]));
+                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+                mx[r] = mx[r] == -INFINITY ? m[r] : fmaxf(mx[r] * crow[r], m[r]);
+                grown |= mx[r] > m[r];
+            }
+            if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                    const float f = mx[r] > m[r] ? tc::ex2(m[r] - mx[r]) : 1.0f;
+                    m[r] = mx[r];
+                    l[r] *= f;
+                    const float f0 = __shfl_sync(0xffffffffu, f, 8 * c4), f1 = __shfl_sync(0xffffffffu, f, 8 * c4 + 4);
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        z[g][r] *= f;
+#pragma unroll
+                        for (int i2 = 0; i2 < 4; ++i2)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[g][i2][r][e] *= e & 1 ? f1 : f0;
+                    }
+                }
+            }
+            // the values' scales: a finite one above the power of two so far raises it
+            float unit[NG];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                uint32_t s = lds32(ss + lane * C::kScaleBytes + 8 * g + 4) & 0xffffu;
+                s = __reduce_max_sync(0xffffffffu, s < 0x7f80u ? s : 0u);
+                if (static_cast<int>(s >> 7) >= top[g]) {
+                    const int to = static_cast<int>(s >> 7) + 1;
+                    const float f = to - top[g] <= 126 ? pow2(top[g] - to) : 0.0f;
+                    top[g] = to;
+#pragma unroll
+                    for (int i2 = 0; i2 < 4; ++i2)
+#pragma unroll
+                        for (int r = 0; r < NR; ++r)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[g][i2][r][e] *= f;
+                }
+                unit[g] = pow2(140 - top[g]);
+            }
+            uint32_t pw[NG][4][NR];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                    const float ref = m[r] == -INFINITY ? 0.0f : m[r];
+                    float p[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        p[e] = tc::ex2(fmaf(t[j][2 * r + e], crow[r], -ref));
+                        l[r] += p[e];
+                    }
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        float w[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            w[e] = p[e] * (bf_lo(sc[g][j][2 * e + 1]) * unit[g]);
+                            float zero = bf_hi(sc[g][j][2 * e + 1]);
+                            // what a row does not see does not reach it: NaN scales neither
+                            if (masked && key0 + 8 * j + 4 * e + c4 >= sees[r]) w[e] = 0.0f, zero = 0.0f;
+                            z[g][r] = fmaf(p[e], zero, z[g][r]);
+                        }
+                        pw[g][j][r] = pack_f16x2(w[0], w[1]);
+                    }
+                }
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    uint32_t w[2][2];      // numbers 0 .. 3 and 4 .. 7 of both tokens, of score tiles 2 s and 2 s + 1
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const uint32_t src = sv + (16 * s + 8 * u + c4) * C::kRowBytes + 4 * r8 +
+                                             (NG == 1 ? 0 : 32 * (g ^ (c4 >> 1)));
+                        const uint32_t x0 = lds32(src), x1 = lds32(src + 4 * C::kRowBytes);
+                        w[u][0] = __byte_perm(x0, x1, 0x5410);
+                        w[u][1] = __byte_perm(x0, x1, 0x7632);
+                    }
+#pragma unroll
+                    for (int i2 = 0; i2 < 4; ++i2) {
+                        const uint32_t x = i2 & 1 ? w[0][i2 >> 1] >> 8 : w[0][i2 >> 1];
+                        const uint32_t x2 = i2 & 1 ? w[1][i2 >> 1] >> 8 : w[1][i2 >> 1];
+#pragma unroll
+                        for (int r = 0; r < NR; ++r)
+                            mma_f16(acc[g][i2][r], x & kEven, x & kOdd, x2 & kEven, x2 & kOdd, pw[g][2 * s][r],
+                                    pw[g][2 * s + 1][r]);
+                    }
+                }
+            __syncwarp();      // the stage that the next copy overwrites has been read
+            fetch(head == 0 ? C::kStages - 1 : head - 1, tile);
+            tile = look(kDecWarps);
+            head = head + 1 == C::kStages ? 0 : head + 1;
+        }
+
+        // the next list, and its queries on their way
+        const int next = base + len.tiles + kListCost;
+        int32_t blen = 0;
+        int ny = y + 1, nb = b;
+        if (ny == lists) ny = 0, ++nb;
+        const DecNew now = fresh;
+        if (!Cluster && next + kListCost < end) {
+            queries(nb, ny);
+            if (nb != b) blen = P.seq_lens[nb];
+        }
+
+        // join the warps: their maxima and sums, then the outputs of eight rows at a time
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+            if (c4 == 0) {
+                s_m[warp][r8 + 8 * r] = m[r];
+                s_l[warp][r8 + 8 * r] = l[r];
+            }
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                z[g][r] += __shfl_xor_sync(0xffffffffu, z[g][r], 1);
+                z[g][r] += __shfl_xor_sync(0xffffffffu, z[g][r], 2);
+                if (c4 == 0) s_z[warp][g][r8 + 8 * r] = z[g][r];
+            }
+        }
+        lost = __syncthreads_or(lost);
+        const int64_t list = static_cast<int64_t>(b) * lists + y;
+        const bool whole = i0 == 0 && tiles == len.tiles;
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            if (8 * r >= nr) break;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int row = 8 * r + 2 * c4 + e;
+                float M = s_m[0][row];
+#pragma unroll
+                for (int w = 1; w < kDecWarps; ++w) M = fmaxf(M, s_m[w][row]);
+                const float f = s_m[warp][row] == -INFINITY ? 0.0f : tc::ex2(s_m[warp][row] - M);
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    // the numbers' 2^-24 or 2^-20 and the weights' unit taken out
+                    const float u = pow2(min(top[g] - 127, 127)) * f;
+                    float *dst = s_o + (warp * 8 + 2 * c4 + e) * HD + 64 * g + 8 * r8;
+#pragma unroll
+                    for (int i2 = 0; i2 < 4; i2 += 2)
+                        *reinterpret_cast<float4 *>(dst + 2 * i2) =
+                            make_float4(acc[g][i2][r][e] * 2048.0f * u, acc[g][i2][r][2 + e] * 128.0f * u,
+                                        acc[g][i2 + 1][r][e] * 2048.0f * u, acc[g][i2 + 1][r][2 + e] * 128.0f * u);
+                }
+            }
+            __syncthreads();
+            const int left = min(nr - 8 * r, 8) * (HD / 4);
+            for (int e = threadIdx.x; e < left; e += blockDim.x) {
+                const int in8 = e / (HD / 4), row = 8 * r + in8, d = e % (HD / 4) * 4;
+                float M = s_m[0][row], L = 0.0f;
+#pragma unroll
+                for (int w = 1; w < kDecWarps; ++w) M = fmaxf(M, s_m[w][row]);
+                float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int w = 0; w < kDecWarps; ++w) {
+                    // a warp whose maximum is -inf saw nothing, or NaN alone
+                    const float f = s_m[w][row] == -INFINITY ? 1.0f : tc::ex2(s_m[w][row] - M);
+                    L += s_l[w][row] * f;
+                    const float4 x = *reinterpret_cast<const float4 *>(s_o + (w * 8 + in8) * HD + d);
+                    const float zero = s_z[w][d / 64][row] * f;
+                    o.x += x.x + zero, o.y += x.y + zero, o.z += x.z + zero, o.w += x.w + zero;
+                }
+                if (lost) L = __int_as_float(0x7fc00000);
+                if constexpr (Cluster) {
+                    // this CTA's part stays where the ring was
+                    *reinterpret_cast<float4 *>(reinterpret_cast<float *>(dsm) + row * HD + d) = o;
+                    if (d == 0) s_part[row] = make_float2(M, L);
+                } else if (whole) {
+                    const int j = (row0 + row) / G, h = y / groups * G + (row0 + row) % G;
+                    const float inv = 1.0f / L;
+                    uint2 got = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+                    if (now.sees(j) <= 0) got = make_uint2(0, 0);
+                    *reinterpret_cast<uint2 *>(P.out + ((static_cast<int64_t>(b) * P.n_new + j) * P.H + h) * HD + d) = got;
+                } else {
+                    // a CTA and a list that follow one another in the order of tiles: no two
+                    // parts have the same sum
+                    float *dst = P.part + ((blockIdx.x + list) * P.per + row) * (HD + 4);
+                    *reinterpret_cast<float4 *>(dst + 4 + d) = o;
+                    if (d == 0) *reinterpret_cast<float2 *>(dst) = make_float2(M, L);
+                }
+            }
+            __syncthreads();
+        }
+        if constexpr (Cluster) break;
+        if (i0 == 0 && threadIdx.x == 0) {
+            const int n = static_cast<int>((at.base + next - 1) / at.span) - static_cast<int>(blockIdx.x) + 1;
+            if (P.by_list) P.cut[list] = make_int2(blockIdx.x, n);
+            else if (n > 1) cut = make_int2(static_cast<int>(list), n);
+        }
+        taken += tiles;
+        base = next;
+        i0 = 0;
+        y = ny;
+        if (nb != b) {
+            b = nb;
+            len = Len(blen, P.max_len);
+            if (base + kListCost < end) fresh = DecNew(P, b, blen);
+        }
+    }
+    if (!Cluster && threadIdx.x == 0 && !P.by_list) P.cut[blockIdx.x] = cut;
+    if constexpr (Cluster) {
+        cluster_sync();
+        // pairs of columns, dealt out over the cluster's threads; parts in chunk order
+        const int ctas = P.n_chunks, me = static_cast<int>(blockIdx.x);
+        const int row0 = y % groups * P.per, nr = min(P.per, P.rows - row0);
+        for (int e = me * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x); e < nr * (HD / 2);
+             e += ctas * static_cast<int>(blockDim.x)) {
+            const int row = e / (HD / 2), d = e % (HD / 2) * 2;
+            float2 ml[kClusterMost], x[kClusterMost];
+            float M = -INFINITY, L = 0.0f, o0 = 0.0f, o1 = 0.0f;
+#pragma unroll
+            for (int c = 0; c < kClusterMost; ++c) {
+                ml[c] = make_float2(-INFINITY, 0.0f);
+                x[c] = make_float2(0.0f, 0.0f);
+                if (c < ctas) {
+                    ml[c] = ld_cluster(&s_part[row], c);
+                    x[c] = ld_cluster(reinterpret_cast<const float2 *>(reinterpret_cast<float *>(dsm) + row * HD + d), c);
+                }
+                M = fmaxf(M, ml[c].x);
+            }
+#pragma unroll
+            for (int c = 0; c < kClusterMost; ++c) {
+                // a chunk whose maximum is -inf saw no key, or NaN alone (its sum says so)
+                const float f = ml[c].x == -INFINITY ? 0.0f : tc::ex2(ml[c].x - M);
+                L += ml[c].x == -INFINITY ? ml[c].y : f * ml[c].y;
+                o0 = fmaf(f, x[c].x, o0);
+                o1 = fmaf(f, x[c].y, o1);
+            }
+            const int j = (row0 + row) / G, h = y / groups * G + (row0 + row) % G;
+            const float inv = 1.0f / L;
+            *reinterpret_cast<uint32_t *>(P.out + ((static_cast<int64_t>(b) * P.n_new + j) * P.H + h) * HD + d) =
+                fresh.sees(j) <= 0 ? 0u : pack_bf16x2(o0 * inv, o1 * inv);
+        }
+        cluster_sync();      // nobody leaves while its part is read
+    }
+}
+
+}  // namespace
+
+cudaError_t launch_rope_append_int4(const void *qkv, int64_t ld, const float *cosv, const float *sinv, int64_t n_pos,
+                                    const void *positions, int pos64, const void *slots, int slot64, int64_t T, int H,
+                                    int Hk, int hd, int64_t n_pages, int page_shift, void *kp, void *vp, void *scales,
+                                    void *q, void *k, void *v, cudaStream_t st) {
+    const int64_t work = T * (H + 2 * Hk) * (hd / 16);
+    const int grid = static_cast<int>(std::min<int64_t>((work + 255) / 256, 148 * 16));
+    auto go = [&](auto kernel) {
+        kernel<<<grid, 256, 0, st>>>(static_cast<const uint16_t *>(qkv), ld, cosv, sinv, n_pos, positions, pos64,
+                                     slots, slot64, T, H, Hk, n_pages << page_shift, page_shift,
+                                     static_cast<uint8_t *>(kp), static_cast<uint8_t *>(vp),
+                                     static_cast<uint16_t *>(scales), static_cast<uint16_t *>(q),
+                                     static_cast<uint16_t *>(k), static_cast<uint16_t *>(v));
+    };
+    if (hd == 64) go(rope_append_int4_kernel<64>);
+    else go(rope_append_int4_kernel<128>);
+    count_launch();
+    return cudaGetLastError();
+}
+
+// Rows of a key head that one list takes: all up to 16, else shared out evenly.
+static int list_rows(int64_t rows) {
+    const int64_t groups = (rows + kDecHeads - 1) / kDecHeads;
+    return static_cast<int>((rows + groups - 1) / groups);
+}
+
+DecodeSplit decode_int4_split(int64_t B, int64_t rows, int64_t Hk, int64_t hd, int64_t max_len) {
+    DecodeSplit s;
+    const int per = list_rows(rows);
+    const int64_t lists = B * Hk * ((rows + per - 1) / per);
+    const int ctas = hd == 64 ? (per <= 8 ? Dec4<64, 8>::kCtas : Dec4<64, 16>::kCtas)
+                              : (per <= 8 ? Dec4<128, 8>::kCtas : Dec4<128, 16>::kCtas);
+    const int64_t resident = static_cast<int64_t>(device_sm_count()) * ctas;
+    // few short lists: as one cluster each, of up to 8 chunks of up to 1024 keys
+    const int64_t most = std::min<int64_t>(kClusterMost, resident / std::max<int64_t>(lists, 1));
+    if (most > 0 && max_len <= most * 1024) {
+        const int64_t chunk = std::max<int64_t>((max_len + most - 1) / most, 128);
+        s.chunk = static_cast<int>((chunk + 63) / 64 * 64);
+        s.n_chunks = static_cast<int>(std::max<int64_t>(1, (max_len + s.chunk - 1) / s.chunk));
+        s.cluster = true;
+        return s;
+    }
+    s.ctas = std::min(resident, lists * std::max<int64_t>((max_len + kTile * kLeast - 1) / (kTile * kLeast), 1));
+    s.lists = lists;
+    return s;
+}
+
+size_t decode_int4_bytes(int64_t B, int64_t rows, int64_t Hk, int64_t hd, int64_t max_len) {
+    return decode_int4_split(B, rows, Hk, hd, max_len).bytes(list_rows(rows), 1, hd);
+}
+
+template <int HD, int ROWS>
+static cudaError_t launch_decode(const Decode4Args &p, const DecodeSplit &s, dim3 grid, cudaStream_t st) {
+    constexpr int smem = Dec4<HD, ROWS>::kSmem;
+    static std::atomic<uint64_t> ready{0};      // devices whose kernels have their shared memory set
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+        if ((e = cudaFuncSetAttribute(decode_int4_kernel<HD, ROWS, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      smem)) != cudaSuccess ||
+            (e = cudaFuncSetAttribute(decode_int4_kernel<HD, ROWS, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      smem)) != cudaSuccess)
+            return e;
+        if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (s.cluster) {
+        cfg.gridDim = grid;
+        cfg.blockDim = dim3(kDecWarps * 32);
+        cfg.dynamicSmemBytes = smem;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = static_cast<unsigned>(s.n_chunks);
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        e = cudaLaunchKernelEx(&cfg, decode_int4_kernel<HD, ROWS, true>, p);
+        count_launch();
+        return e;
+    }
+    decode_int4_kernel<HD, ROWS, false><<<grid, kDecWarps * 32, smem, st>>>(p);
+    count_launch();
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    // the join's launch overlaps the split's end; its threads wait for the parts
+    const bool wide = s.ctas > 8 * s.lists;
+    cfg.blockDim = dim3(wide ? 512 : 128);
+    cfg.gridDim = dim3(static_cast<unsigned>(std::min(s.ctas, s.lists)), p.per, wide ? HD / 32 : 1);
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    const DecodeArgs &join = p;
+    e = wide ? cudaLaunchKernelEx(&cfg, decode_join_kernel<HD, true, true>, join)
+             : cudaLaunchKernelEx(&cfg, decode_join_kernel<HD, false, true>, join);
+    count_launch();
+    return e;
+}
+
+cudaError_t launch_decode_attn_int4(const void *q, int64_t q_ld, const void *kp, const void *vp, const void *scales,
+                                    int64_t n_pages, int page_shift, const int32_t *table, int64_t table_ld,
+                                    const int32_t *seq_lens, const int32_t *new_lens, int64_t max_len, int64_t B,
+                                    int n_new, int H, int Hk, int hd, float scale, void *out, float *part,
+                                    cudaStream_t st) {
+    const int G = H / Hk, rows = G * n_new, per = list_rows(rows);
+    const DecodeSplit s = decode_int4_split(B, rows, Hk, hd, max_len);
+    const unsigned lists = Hk * ((rows + per - 1) / per);
+    const dim3 grid = s.cluster ? dim3(s.n_chunks, lists, static_cast<unsigned>(B)) : dim3(static_cast<unsigned>(s.ctas));
+    Decode4Args p = {};
+    p.q = static_cast<const uint16_t *>(q);
+    p.k4 = static_cast<const uint8_t *>(kp);
+    p.v4 = static_cast<const uint8_t *>(vp);
+    p.scales = static_cast<const uint16_t *>(scales);
+    p.table = table;
+    p.seq_lens = seq_lens;
+    p.new_lens = new_lens;
+    p.q_ld = q_ld;
+    p.table_ld = table_ld;
+    p.n_pages = n_pages;
+    p.max_len = max_len;
+    p.H = H;
+    p.Hk = Hk;
+    p.n_new = n_new;
+    p.rows = rows;
+    p.per = per;
+    p.page_shift = page_shift;
+    p.B = B;
+    p.chunk = s.chunk;
+    p.n_chunks = s.n_chunks;
+    p.scale_log2 = scale * kLog2e;
+    p.out = static_cast<uint16_t *>(out);
+    p.part = part;
+    // the parts, then the CTAs' cut lists
+    p.by_list = s.lists <= s.ctas;
+    p.cut = s.cluster ? nullptr : reinterpret_cast<int2 *>(part + s.part_floats(per, 1, hd));
+    if (hd == 64) return per <= 8 ? launch_decode<64, 8>(p, s, grid, st) : launch_decode<64, 16>(p, s, grid, st);
+    return per <= 8 ? launch_decode<128, 8>(p, s, grid, st) : launch_decode<128, 16>(p, s, grid, st);
+}
+
+}  // namespace mom
