@@ -469,6 +469,26 @@ MOM_API int mom_logprobs_bwd(const void *logits, int dtype, int64_t ld, const in
                              const float *g_top, int64_t R, int64_t V, int64_t ignore_index, double temperature,
                              void *dlogits, void *stream);
 
+/* Drafted tokens against the target's distribution (speculative sampling): logits
+ * (B, K + 1, V) F32 or BF16, pitches ld_seq and ld_row, the target's behind each
+ * sequence's last token and behind each of its drafts (B, K) int64; K 0 to 32. p =
+ * softmax(logits / temperature), q the same of draft_logits (B, K, V) in the logits' dtype, or
+ * without them (NULL) all of it on the draft itself. uniforms (B, K + 1) in [0, 1).
+ * Draft j stays while u_j q_j(d_j) < p_j(d_j); at the first that falls the next token is
+ * drawn from max(p_j - q_j, 0) (from p_j where that is 0 everywhere), behind all drafts
+ * from p: the least index whose running sum exceeds u_K times the whole. temperature 0:
+ * greedy, a draft stays while it is its row's greatest logit (ties to the lowest index, NaN
+ * above all), draft_logits and uniforms may be NULL. draft_lens (B) I32 on the device, or
+ * NULL: the drafts of each sequence, 0 to K. tokens (B, K + 1) int64: the drafts that
+ * stay, the next token, then -1; accepted (B) int64: how many stay. The next token is -1,
+ * and nothing behind it is looked at, where a row that decides has no distribution (a NaN
+ * or, sampling, +inf or nothing but -inf); with a draft_len outside [0, K] accepted is 0 and
+ * all tokens are -1. A draft outside [0, V) falls. Choices are made in 64 bits. */
+MOM_API int mom_verify_drafts(const void *logits, int dtype, int64_t ld_seq, int64_t ld_row, const void *draft_logits,
+                              int64_t draft_ld_seq, int64_t draft_ld_row, const int64_t *drafts, const float *uniforms,
+                              const int32_t *draft_lens, int64_t B, int64_t K, int64_t V, double temperature,
+                              int64_t *tokens, int64_t *accepted, void *stream);
+
 /* Reads (and clears) the device error word of a plan: MOM_OK, or
  * MOM_ERR_DEVICE_INDEX when mom_bucket saw an index outside [0, nb).
  * Synchronises `stream`. */

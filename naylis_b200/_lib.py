@@ -104,6 +104,8 @@ SIGNATURES = {
     "mom_prompt_plan_check": (_int, [_vp, _vp]),
     "mom_logprobs_fwd": (_int, [_vp, _int, _i64, _vp, _i64, _i64, _i64, _c.c_double, _i64, _fp, _fp, _fp, _vp, _fp,
                                 _vp]),
+    "mom_verify_drafts": (_int, [_vp, _int, _i64, _i64, _vp, _i64, _i64, _vp, _fp, _vp, _i64, _i64, _i64, _c.c_double,
+                                 _vp, _vp, _vp]),
     "mom_logprobs_bwd": (_int, [_vp, _int, _i64, _vp, _fp, _vp, _i64, _fp, _fp, _fp, _i64, _i64, _i64, _c.c_double,
                                 _vp, _vp]),
 }

@@ -1152,6 +1152,30 @@ int mom_logprobs_bwd(const void *logits, int dtype, int64_t ld, const int64_t *t
     return e == cudaSuccess ? MOM_OK : cuda_fail(e, "logprobs_bwd");
 }
 
+int mom_verify_drafts(const void *logits, int dtype, int64_t ld_seq, int64_t ld_row, const void *draft_logits,
+                      int64_t draft_ld_seq, int64_t draft_ld_row, const int64_t *drafts, const float *uniforms,
+                      const int32_t *draft_lens, int64_t B, int64_t K, int64_t V, double temperature, int64_t *tokens,
+                      int64_t *accepted, void *stream) {
+    MOM_REQUIRE(is_float_dtype(dtype), "logits must be F32 or BF16");
+    MOM_REQUIRE(B >= 0 && B <= 65535, "B must be in [0, 65535] (got %lld)", (long long)B);
+    MOM_REQUIRE(K >= 0 && K <= mom::kMaxDrafts, "drafts of a sequence must be in [0, %d] (got %lld)", mom::kMaxDrafts,
+                (long long)K);
+    MOM_REQUIRE(V > 0 && V <= INT32_MAX - 65536, "bad vocabulary");
+    MOM_REQUIRE(temperature == 0.0 || (temperature >= 1e-6 && temperature <= 1e6),
+                "temperature must be 0 or in [1e-6, 1e6] (got %g)", temperature);
+    MOM_REQUIRE(ld_row >= 0 && ld_seq >= 0 && draft_ld_row >= 0 && draft_ld_seq >= 0, "pitches must be >= 0");
+    if (B == 0) return MOM_OK;
+    MOM_REQUIRE(logits && tokens && accepted && (K == 0 || drafts), "null pointer argument");
+    MOM_REQUIRE(temperature == 0.0 || uniforms, "sampling takes uniforms");
+    MOM_REQUIRE(aligned(logits, dt_size(dtype)) && aligned(draft_logits, dt_size(dtype)), "logits misaligned");
+    int rc = check_current_device();
+    if (rc) return rc;
+    cudaError_t e = mom::launch_verify_drafts(logits, dtype, ld_seq, ld_row, draft_logits, draft_ld_seq, draft_ld_row,
+                                              drafts, uniforms, draft_lens, B, (int)K, (int)V, temperature, tokens,
+                                              accepted, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? MOM_OK : cuda_fail(e, "verify_drafts");
+}
+
 // ------------------------------------------------- read backward, no allocation
 // mom_read_bwd_noalloc runs mom_read_bwd with its workspace (the per-row delta,
 // H x B*S fp32) in a fixed device array of this library instead of caller

@@ -302,4 +302,12 @@ cudaError_t launch_logprobs_bwd(const void *logits, int dt, int64_t ld, const in
                                 const float *g_top, int64_t R, int V, int64_t ignore, float inv_t, void *dlogits,
                                 cudaStream_t st);
 
+// Drafted tokens (verify.cu): logits (B, K + 1, V) and draft (B, K, V, or null) of pitches ld_seq,
+// ld_row; temperature 0: greedy, without uniforms.
+constexpr int kMaxDrafts = 32;
+cudaError_t launch_verify_drafts(const void *logits, int dt, int64_t ld_seq, int64_t ld_row, const void *draft,
+                                 int64_t draft_ld_seq, int64_t draft_ld_row, const int64_t *drafts,
+                                 const float *uniforms, const int32_t *draft_lens, int64_t B, int K, int V,
+                                 double temperature, int64_t *tokens, int64_t *accepted, cudaStream_t st);
+
 }  // namespace mom

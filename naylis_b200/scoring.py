@@ -1,6 +1,7 @@
 """Scoring tokens: the log probabilities of given tokens under a row of logits,
 the distribution's entropy and its top alternatives, with the gradient that a
-policy update or a distillation needs (csrc/scoring.cu, through the C ABI).
+policy update or a distillation needs (csrc/scoring.cu, through the C ABI); and
+which drafted tokens a target's distribution keeps (csrc/verify.cu).
 
 The training loss (trunk.cross_entropy_sum) gives one sum; an answer's tokens are
 scored one by one, and a policy-gradient step weighs each token's gradient.
@@ -15,6 +16,7 @@ from torch.autograd import forward_ad
 from . import _lib
 
 MAX_TOP = 32
+MAX_DRAFTS = 32
 
 
 class TokenLogprobs(NamedTuple):
@@ -111,4 +113,76 @@ def token_logprobs(logits, targets, *, top_k: int = 0, temperature: float = 1.0,
     return TokenLogprobs(logprob, entropy, top_idx, top_lp)
 
 
-__all__ = ["MAX_TOP", "TokenLogprobs", "token_logprobs"]
+class Verified(NamedTuple):
+    """tokens (B, K + 1) int64: the drafts that stay, the token that follows them, then -1;
+    accepted (B) int64: how many stay."""
+    tokens: torch.Tensor
+    accepted: torch.Tensor
+
+
+def _logits3(t, B, rows, V, like):
+    if t.dim() != 3 or t.shape != (B, rows, V) or t.dtype != like.dtype or t.device != like.device:
+        raise RuntimeError(f"verify_drafts: draft_logits must be {(B, rows, V)} {like.dtype} on {like.device}, got "
+                           f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    return t if V == 1 or t.stride(2) == 1 else t.contiguous()
+
+
+def verify_drafts(logits, drafts, uniforms=None, *, draft_logits=None, temperature: float = 1.0, draft_lens=None):
+    """Which drafted tokens the target keeps, and the token that follows them, by
+    speculative sampling: tokens come out distributed as the target's own samples.
+
+    logits (B, K + 1, V) bf16 or fp32: the target's behind each sequence's last token and
+    behind each of its drafts (B, K) int64, K at most 32. p = softmax(logits /
+    temperature); q the same of draft_logits (B, K, V), the distributions that the drafts
+    were drawn from, or without them all of it on the draft itself (drafts that were
+    looked up). uniforms (B, K + 1) fp32 in [0, 1): draft j stays while
+    u_j q_j(d_j) < p_j(d_j); at the first that falls the next token is drawn from
+    max(p_j - q_j, 0) (from p_j where nothing of it is left), behind all drafts from p:
+    the least index whose running sum exceeds u_K times the whole. Choices are made in 64
+    bits. temperature 0: greedy, without uniforms; a draft stays while it is its row's
+    greatest logit (the lowest index of equals, NaN above all).
+
+    draft_lens (B) int32 on the device: sequences with fewer than K drafts. A row that
+    decides and is no distribution (a NaN; sampling, +inf or nothing but -inf) ends its
+    sequence with a token of -1; a draft_len outside [0, K] gives no tokens but -1. A
+    draft outside [0, V) falls. Not differentiable. Returns Verified."""
+    if not logits.is_cuda or logits.dtype not in (torch.bfloat16, torch.float32):
+        raise RuntimeError(f"verify_drafts takes bf16 or fp32 CUDA logits, got {logits.dtype} on {logits.device}")
+    dev = logits.device
+    if logits.dim() != 3 or drafts.dim() != 2 or logits.shape[0] != drafts.shape[0] or \
+            logits.shape[1] != drafts.shape[1] + 1 or logits.shape[2] == 0 or drafts.dtype != torch.int64 or \
+            drafts.device != dev:
+        raise RuntimeError(f"verify_drafts: logits (B, K + 1, V) and int64 drafts (B, K) on one device, got "
+                           f"{tuple(logits.shape)} and {tuple(drafts.shape)} {drafts.dtype}")
+    B, K = drafts.shape
+    V = logits.shape[2]
+    temperature = float(temperature)
+    if K > MAX_DRAFTS:
+        raise RuntimeError(f"verify_drafts: {K} drafts must be at most {MAX_DRAFTS}")
+    if not (temperature == 0.0 or 1e-6 <= temperature <= 1e6):
+        raise RuntimeError(f"verify_drafts: temperature {temperature} must be 0 or in [1e-6, 1e6]")
+    if uniforms is not None:
+        if uniforms.dtype != torch.float32 or uniforms.shape != (B, K + 1) or uniforms.device != dev:
+            raise RuntimeError(f"verify_drafts: uniforms must be {(B, K + 1)} fp32 on {dev}")
+        uniforms = uniforms.contiguous()
+    elif temperature != 0.0:
+        raise RuntimeError("verify_drafts: sampling takes uniforms")
+    if draft_lens is not None:
+        if draft_lens.dtype != torch.int32 or draft_lens.shape != (B,) or draft_lens.device != dev:
+            raise RuntimeError(f"verify_drafts: draft_lens must be ({B},) int32 on {dev}")
+        draft_lens = draft_lens.contiguous()
+    logits = _logits3(logits, B, K + 1, V, logits)
+    drafts = drafts.contiguous()
+    if draft_logits is not None:
+        draft_logits = _logits3(draft_logits, B, K, V, logits)
+    tokens = torch.empty(B, K + 1, dtype=torch.int64, device=dev)
+    accepted = torch.empty(B, dtype=torch.int64, device=dev)
+    _lib.call_on(dev.index, "mom_verify_drafts", logits.data_ptr(), _code(logits), logits.stride(0), logits.stride(1),
+                 None if draft_logits is None else draft_logits.data_ptr(),
+                 *((0, 0) if draft_logits is None else draft_logits.stride()[:2]), drafts.data_ptr(),
+                 None if uniforms is None else uniforms.data_ptr(), None if draft_lens is None else draft_lens.data_ptr(),
+                 B, K, V, temperature, tokens.data_ptr(), accepted.data_ptr())
+    return Verified(tokens, accepted)
+
+
+__all__ = ["MAX_DRAFTS", "MAX_TOP", "TokenLogprobs", "Verified", "token_logprobs", "verify_drafts"]
