@@ -9,6 +9,7 @@
 // value's. A row of hd 64 is 36 bytes, of hd 128 72: 9/32 of bf16.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "decode.cuh"
 
@@ -169,7 +170,8 @@ struct Dec4 {
     static constexpr int kSide = kTile * kRowBytes;
     static constexpr int kStage = 2 * kSide + kTile * kScaleBytes;
     static constexpr int kRing = kDecWarps * kStages * kStage;
-    static constexpr int kSmem = kRing + kDecWarps * 8 * HD * 4;          // the warps' outputs, 8 rows at a time
+    // the warps' tiles' scales and zeros in fp32; at a list's end their outputs, 8 rows at a time
+    static constexpr int kSmem = kRing + std::max(kDecWarps * kTile * 16 * kGroups, kDecWarps * 8 * HD * 4);
 };
 
 struct Decode4Args : DecodeArgs {
@@ -194,20 +196,6 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }      // -126 .. 127
 __device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
-__device__ __forceinline__ void lds64(uint32_t (&r)[2], uint32_t at) {
-    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];\n" : "=r"(r[0]), "=r"(r[1]) : "r"(at) : "memory");
-}
-__device__ __forceinline__ uint32_t lds32(uint32_t at) {
-    uint32_t r;
-    asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(r) : "r"(at) : "memory");
-    return r;
-}
-__device__ __forceinline__ void lds128(uint32_t (&r)[4], uint32_t at) {
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(at)
-                 : "memory");
-}
 __device__ __forceinline__ void cp_async8(uint32_t dst, const void *src, int src_bytes) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(dst), "l"(src), "r"(src_bytes));
 }
@@ -228,6 +216,7 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
     __shared__ float2 s_part[ROWS];
     float *s_o = reinterpret_cast<float *>(dsm + C::kRing);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c4 = lane & 3, r8 = lane >> 2;
+    float4 *s_x = reinterpret_cast<float4 *>(dsm + C::kRing) + warp * kTile * NG;      // [group][pair of columns][key's, value's]
     const int G = P.H / P.Hk, groups = (P.rows + P.per - 1) / P.per, lists = P.Hk * groups;
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     DecSpan at;
@@ -253,11 +242,13 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
     int fbase = 0, fb = at.b, fy = at.y, fhk = fy / groups, fi = at.i, fn = len.n, fall = len.tiles;
     int fend = tiles_to(fbase, fall);
     int32_t flen = !Cluster && fb + 1 < P.B ? P.seq_lens[fb + 1] : 0;      // the next sequence's
+    const int32_t *frow = P.table + fb * P.table_ld;
     struct Tile {
         int32_t page;
         int rows, in_page, hk;      // rows: of the sequence; < 0: no tile
     };
-    bool more = true, bad[C::kStages] = {};
+    bool more = true;
+    uint32_t bad = 0;      // a bit for each stage
     auto look = [&](int step) {
         Tile tile = {0, -1, 0, 0};
         if (!more) return tile;
@@ -275,49 +266,46 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                 const Len next(flen, P.max_len);
                 fn = next.n, fall = next.tiles;
                 flen = fb + 1 < P.B ? P.seq_lens[fb + 1] : 0;
+                frow = P.table + fb * P.table_ld;
             }
             fhk = fy / groups;
             fend = tiles_to(fbase, fall);
         }
-        const int64_t j = static_cast<int64_t>(fi) * kTile + lane;
+        const int j = fi * kTile + lane;      // below 2^31 where it is a key
         tile.rows = min(fn - fi * kTile, kTile);
-        tile.in_page = static_cast<int>(j) & page_mask;
+        tile.in_page = j & page_mask;
         tile.hk = fhk;
-        if (lane < tile.rows) tile.page = P.table[fb * P.table_ld + (j >> P.page_shift)];
+        if (lane < tile.rows) tile.page = frow[j >> P.page_shift];
         return tile;
     };
+    // A lane's copies: chunk of 16 bytes `chunk` of rows u kPer + lane / kChunks. At hd 128 a row's
+    // two groups change places in every second pair of rows: no bank conflicts.
+    constexpr int kChunks = C::kRowBytes / 16, kPer = 32 / kChunks;
+    const int chunk = lane % kChunks, crow0 = lane / kChunks, ccol0 = column_of(crow0);
+    const auto in_row = [&](int row) {
+        return row * C::kRowBytes + (NG == 1 ? chunk * 16 : (chunk & 1) * 16 + 32 * ((chunk >> 1) ^ (row >> 1 & 1)));
+    };
+    const uint32_t kdst = ring + in_row(ccol0), vdst = ring + C::kSide + in_row(crow0);
+    const uint32_t sdst = ring + 2 * C::kSide + column_of(lane) * C::kScaleBytes;
+    const uint8_t *const ksrc = P.k4 + chunk * 16, *const vsrc = P.v4 + chunk * 16;
     auto fetch = [&](int stage, const Tile &tile) {
         if (tile.rows >= 0) {
-            const uint32_t sk = ring + stage * C::kStage, sv = sk + C::kSide, ss = sv + C::kSide;
-            const bool out = lane < tile.rows && (tile.page < 0 || tile.page >= P.n_pages);
-            const bool any = __any_sync(0xffffffffu, out);
-#pragma unroll
-            for (int e = 0; e < C::kStages; ++e)
-                if (e == stage) bad[e] = any;
-            // rows of the cache are counted in 32 bits (the caller's check), bytes in 64
-            constexpr uint32_t kNone = 0xffffffffu;
-            const uint32_t mine = lane < tile.rows && !out
-                                      ? ((static_cast<uint32_t>(tile.page) * P.Hk + tile.hk) << P.page_shift) + tile.in_page
-                                      : kNone;
-            const uint16_t *sc = mine != kNone ? P.scales + static_cast<uint64_t>(mine) * (4 * NG) : P.scales;
-            const int bytes = mine != kNone ? C::kScaleBytes : 0;
-            const uint32_t sdst = ss + column_of(lane) * C::kScaleBytes;
-            if constexpr (NG == 1) cp_async8(sdst, sc, bytes);
-            else cp_async16(sdst, sc, bytes);
-            constexpr int kChunks = C::kRowBytes / 16, kPer = 32 / kChunks;      // of a row; rows of an instruction
-            const int chunk = lane % kChunks;
+            const bool in = lane < tile.rows && tile.page >= 0 && tile.page < P.n_pages;
+            const uint32_t have = __ballot_sync(0xffffffffu, in);
+            const bool lacks = static_cast<int>(__popc(have)) < tile.rows;
+            bad = (bad & ~(1u << stage)) | static_cast<uint32_t>(lacks) << stage;
+            // rows of the cache are counted in 32 bits (the caller's check), bytes in 64; zeros behind the end
+            const uint32_t mine = in ? ((static_cast<uint32_t>(tile.page) * P.Hk + tile.hk) << P.page_shift) + tile.in_page : 0u;
+            const uint32_t at = stage * C::kStage;
+            const uint16_t *sc = P.scales + static_cast<uint64_t>(mine) * (4 * NG);
+            if constexpr (NG == 1) cp_async8(sdst + at, sc, in ? 8 : 0);
+            else cp_async16(sdst + at, sc, in ? 16 : 0);
 #pragma unroll
             for (int u = 0; u < kChunks; ++u) {
-                const int r = u * kPer + lane / kChunks, col = column_of(r);
-                const uint32_t row = __shfl_sync(0xffffffffu, mine, r);
-                const bool in = row != kNone;
-                const uint64_t from = in ? static_cast<uint64_t>(row) * C::kRowBytes + chunk * 16 : 0;
-                // at hd 128 a row's two groups change places in every second pair of rows: no bank conflicts
-                const int flip = NG == 1 ? chunk * 16 : (chunk & 1) * 16, kg = chunk >> 1;
-                const uint32_t kdst = sk + col * C::kRowBytes + flip + (NG == 1 ? 0 : 32 * (kg ^ (col >> 1 & 1)));
-                const uint32_t vdst = sv + r * C::kRowBytes + flip + (NG == 1 ? 0 : 32 * (kg ^ (r >> 1 & 1)));
-                cp_async16(kdst, P.k4 + from, in ? 16 : 0);      // zeros behind the end
-                cp_async16(vdst, P.v4 + from, in ? 16 : 0);
+                const uint64_t from = static_cast<uint64_t>(__shfl_sync(0xffffffffu, mine, u * kPer + crow0)) * C::kRowBytes;
+                const int bytes = have >> (u * kPer + crow0) & 1 ? 16 : 0;
+                cp_async16(kdst + at + u * kPer * C::kRowBytes, ksrc + from, bytes);
+                cp_async16(vdst + at + u * kPer * C::kRowBytes, vsrc + from, bytes);
             }
         }
         cp_async_commit();
@@ -407,16 +395,18 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
             sees[r] = j < fresh.count ? fresh.first + j : INT32_MAX;
         }
         const int all_see = row0 / G < fresh.count ? fresh.first + row0 / G : INT32_MAX;
-        float acc[NG][4][NR][4], m[NR], l[NR], z[NG][NR];
+        float acc[NG][4][NR][4], m[NR];
+        uint64_t l2[NR], z2[NG][NR];      // of a thread's even and odd columns
         int top[NG];        // 2^(top - 127) is above every scale so far
+        const uint64_t none2 = tc::f2(0.0f, 0.0f);
 #pragma unroll
-        for (int r = 0; r < NR; ++r) m[r] = -INFINITY, l[r] = 0.0f;
+        for (int r = 0; r < NR; ++r) m[r] = -INFINITY, l2[r] = none2;
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             top[g] = 15;
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
-                z[g][r] = 0.0f;
+                z2[g][r] = none2;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -426,33 +416,44 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
         for (int i = (warp - taken) & (kDecWarps - 1); i < tiles; i += kDecWarps) {
             cp_async_wait<C::kStages - 2>();
             __syncwarp();
-#pragma unroll
-            for (int e = 0; e < C::kStages; ++e)
-                if (e == head) lost |= bad[e];
+            lost |= bad >> head & 1;
             const int key0 = (i0 + i) * kTile;
-            const uint32_t sk = ring + head * C::kStage, sv = sk + C::kSide, ss = sv + C::kSide;
-            // scales and zeros of this thread's columns: [key's, value's] of column 2 c4, of 2 c4 + 1
-            uint32_t sc[NG][4][4];
+            const unsigned char *sk = dsm + (warp * C::kStages + head) * C::kStage, *sv = sk + C::kSide, *ss = sv + C::kSide;
+            // Scales and zeros in fp32, once for the warp: an even lane those of the keys of columns
+            // lane, lane + 1, an odd one those of its columns' values (lane - 1, lane), whose scales
+            // take the weights' unit along. A finite one above the power of two so far raises that.
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if constexpr (NG == 1) {
-                    lds128(sc[0][j], ss + (8 * j + 2 * c4) * 8);
-                } else {
-                    uint32_t x[2][4];
+            for (int g = 0; g < NG; ++g) {
+                const uint32_t *two = reinterpret_cast<const uint32_t *>(ss + (lane & ~1) * C::kScaleBytes) + 2 * g + (lane & 1);
+                const uint32_t a = two[0], c = two[2 * NG];
+                float sa = bf_lo(a), sb = bf_lo(c);
+                const float most = lane & 1 ? fmaxf(sa, sb) : 0.0f;
+                if (__any_sync(0xffffffffu, most >= pow2(top[g] - 127))) {
+                    const int to = (__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(most, 0.0f))) >> 23) + 1;
+                    const float f = to - top[g] <= 126 ? pow2(top[g] - to) : 0.0f;
+                    top[g] = to;
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) lds128(x[e], ss + (8 * j + 2 * c4 + e) * 16);
+                    for (int i2 = 0; i2 < 4; ++i2)
 #pragma unroll
-                    for (int g = 0; g < NG; ++g)
+                        for (int r = 0; r < NR; ++r)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) sc[g][j][e] = x[e >> 1][2 * g + (e & 1)];
+                            for (int e = 0; e < 4; ++e) acc[g][i2][r][e] *= f;
                 }
+                if (lane & 1) {
+                    const float unit = pow2(140 - top[g]);
+                    sa *= unit, sb *= unit;
+                }
+                s_x[g * kTile + lane] = make_float4(sa, sb, bf_hi(a), bf_hi(c));
+            }
+            __syncwarp();
             float t[4][2 * NR];
 #pragma unroll
             for (int g = 0; g < NG; ++g)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    uint32_t w[2];
-                    lds64(w, sk + (8 * j + r8) * C::kRowBytes + 8 * c4 + (NG == 1 ? 0 : 32 * (g ^ (r8 >> 1 & 1))));
+                    const uint2 w2 = *reinterpret_cast<const uint2 *>(sk + (8 * j + r8) * C::kRowBytes + 8 * c4 +
+                                                                      (NG == 1 ? 0 : 32 * (g ^ (r8 >> 1 & 1))));
+                    const uint32_t w[2] = {w2.x, w2.y};
                     float d[4] = {};
 #pragma unroll
                     for (int s = 0; s < 4; ++s) {
@@ -460,14 +461,15 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                         if constexpr (NR == 1) mma_f16(d, qa[g][s][0], 0u, qa[g][s][1], 0u, x & kEven, x & kOdd);
                         else mma_f16(d, qa[g][s][0], qa[g][s][1], qa[g][s][2], qa[g][s][3], x & kEven, x & kOdd);
                     }
+                    const ulonglong2 sz = *reinterpret_cast<const ulonglong2 *>(&s_x[g * kTile + 8 * j + 2 * c4]);
 #pragma unroll
-                    for (int r = 0; r < NR; ++r)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float zero = bf_hi(sc[g][j][2 * e]) * qsum[g][r];
-                            t[j][2 * r + e] = fmaf(bf_lo(sc[g][j][2 * e]), d[2 * r + e],
-                                                   g == 0 ? zero : t[j][2 * r + e] + zero);
-                        }
+                    for (int r = 0; r < NR; ++r) {
+                        const uint64_t q2 = tc::f2(qsum[g][r], qsum[g][r]);
+                        const uint64_t zero = g == 0 ? tc::mul2(sz.y, q2) : tc::fma2(sz.y, q2, tc::f2(t[j][2 * r], t[j][2 * r + 1]));
+                        const float2 got = tc::f2_split(tc::fma2(sz.x, tc::f2(d[2 * r], d[2 * r + 1]), zero));
+                        t[j][2 * r] = got.x;
+                        t[j][2 * r + 1] = got.y;
+                    }
                 }
             const bool masked = key0 + kTile > all_see;
             if (masked) {
@@ -483,24 +485,25 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
             bool grown = false;
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
-                mx[r] = -INFINITY;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) mx[r] = fmaxf(mx[r], fmaxf(t[j][2 * r], t[j][2 * r + 1]));
+                mx[r] = fmaxf(tc::fmax3(tc::fmax3(t[0][2 * r], t[0][2 * r + 1], t[1][2 * r]), t[1][2 * r + 1], t[2][2 * r]),
+                              tc::fmax3(t[2][2 * r + 1], t[3][2 * r], t[3][2 * r + 1]));
                 mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
                 mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-                mx[r] = mx[r] == -INFINITY ? m[r] : fmaxf(mx[r] * crow[r], m[r]);
+                // (the greatest of nothing, or of NaN alone, leaves the maximum as it was)
+                mx[r] = fmaxf(mx[r] * crow[r], m[r]);
                 grown |= mx[r] > m[r];
             }
             if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
                 for (int r = 0; r < NR; ++r) {
                     const float f = mx[r] > m[r] ? tc::ex2(m[r] - mx[r]) : 1.0f;
+                    const uint64_t ff = tc::f2(f, f);
                     m[r] = mx[r];
-                    l[r] *= f;
+                    l2[r] = tc::mul2(l2[r], ff);
                     const float f0 = __shfl_sync(0xffffffffu, f, 8 * c4), f1 = __shfl_sync(0xffffffffu, f, 8 * c4 + 4);
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
-                        z[g][r] *= f;
+                        z2[g][r] = tc::mul2(z2[g][r], ff);
 #pragma unroll
                         for (int i2 = 0; i2 < 4; ++i2)
 #pragma unroll
@@ -508,51 +511,35 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                     }
                 }
             }
-            // the values' scales: a finite one above the power of two so far raises it
-            float unit[NG];
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                uint32_t s = lds32(ss + lane * C::kScaleBytes + 8 * g + 4) & 0xffffu;
-                s = __reduce_max_sync(0xffffffffu, s < 0x7f80u ? s : 0u);
-                if (static_cast<int>(s >> 7) >= top[g]) {
-                    const int to = static_cast<int>(s >> 7) + 1;
-                    const float f = to - top[g] <= 126 ? pow2(top[g] - to) : 0.0f;
-                    top[g] = to;
-#pragma unroll
-                    for (int i2 = 0; i2 < 4; ++i2)
-#pragma unroll
-                        for (int r = 0; r < NR; ++r)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) acc[g][i2][r][e] *= f;
-                }
-                unit[g] = pow2(140 - top[g]);
-            }
             uint32_t pw[NG][4][NR];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
+            auto weigh = [&](auto some_hidden) {
 #pragma unroll
                 for (int r = 0; r < NR; ++r) {
-                    const float ref = m[r] == -INFINITY ? 0.0f : m[r];
-                    float p[2];
+                    const float ref = m[r] == -INFINITY ? 0.0f : -m[r];
+                    const uint64_t ref2 = tc::f2(ref, ref), c2 = tc::f2(crow[r], crow[r]);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        p[e] = tc::ex2(fmaf(t[j][2 * r + e], crow[r], -ref));
-                        l[r] += p[e];
-                    }
+                    for (int j = 0; j < 4; ++j) {
+                        const uint64_t p2 = tc::ex2_pair(tc::fma2(tc::f2(t[j][2 * r], t[j][2 * r + 1]), c2, ref2));
+                        l2[r] = tc::add2(l2[r], p2);
 #pragma unroll
-                    for (int g = 0; g < NG; ++g) {
-                        float w[2];
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            w[e] = p[e] * (bf_lo(sc[g][j][2 * e + 1]) * unit[g]);
-                            float zero = bf_hi(sc[g][j][2 * e + 1]);
-                            // what a row does not see does not reach it: NaN scales neither
-                            if (masked && key0 + 8 * j + 4 * e + c4 >= sees[r]) w[e] = 0.0f, zero = 0.0f;
-                            z[g][r] = fmaf(p[e], zero, z[g][r]);
+                        for (int g = 0; g < NG; ++g) {
+                            ulonglong2 sz = *reinterpret_cast<const ulonglong2 *>(&s_x[g * kTile + 8 * j + 2 * c4 + 1]);
+                            if constexpr (some_hidden.value) {
+                                // what a row does not see does not reach it: NaN scales neither
+                                const bool h0 = key0 + 8 * j + c4 >= sees[r], h1 = key0 + 8 * j + 4 + c4 >= sees[r];
+                                const float2 a = tc::f2_split(sz.x), c = tc::f2_split(sz.y);
+                                sz.x = tc::f2(h0 ? 0.0f : a.x, h1 ? 0.0f : a.y);
+                                sz.y = tc::f2(h0 ? 0.0f : c.x, h1 ? 0.0f : c.y);
+                            }
+                            z2[g][r] = tc::fma2(p2, sz.y, z2[g][r]);
+                            const float2 w = tc::f2_split(tc::mul2(p2, sz.x));
+                            pw[g][j][r] = pack_f16x2(w.x, w.y);
                         }
-                        pw[g][j][r] = pack_f16x2(w[0], w[1]);
                     }
                 }
+            };
+            if (masked) weigh(std::true_type{});
+            else weigh(std::false_type{});
 #pragma unroll
             for (int g = 0; g < NG; ++g)
 #pragma unroll
@@ -560,9 +547,10 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                     uint32_t w[2][2];      // numbers 0 .. 3 and 4 .. 7 of both tokens, of score tiles 2 s and 2 s + 1
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        const uint32_t src = sv + (16 * s + 8 * u + c4) * C::kRowBytes + 4 * r8 +
-                                             (NG == 1 ? 0 : 32 * (g ^ (c4 >> 1)));
-                        const uint32_t x0 = lds32(src), x1 = lds32(src + 4 * C::kRowBytes);
+                        const unsigned char *src = sv + (16 * s + 8 * u + c4) * C::kRowBytes + 4 * r8 +
+                                                   (NG == 1 ? 0 : 32 * (g ^ (c4 >> 1)));
+                        const uint32_t x0 = *reinterpret_cast<const uint32_t *>(src);
+                        const uint32_t x1 = *reinterpret_cast<const uint32_t *>(src + 4 * C::kRowBytes);
                         w[u][0] = __byte_perm(x0, x1, 0x5410);
                         w[u][1] = __byte_perm(x0, x1, 0x7632);
                     }
@@ -594,19 +582,23 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
         }
 
         // join the warps: their maxima and sums, then the outputs of eight rows at a time
+        const auto whole_row = [](uint64_t v2) {
+            const float2 v = tc::f2_split(v2);
+            float sum = v.x + v.y;
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            return sum + __shfl_xor_sync(0xffffffffu, sum, 2);
+        };
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+            const float l = whole_row(l2[r]);
             if (c4 == 0) {
                 s_m[warp][r8 + 8 * r] = m[r];
-                s_l[warp][r8 + 8 * r] = l[r];
+                s_l[warp][r8 + 8 * r] = l;
             }
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                z[g][r] += __shfl_xor_sync(0xffffffffu, z[g][r], 1);
-                z[g][r] += __shfl_xor_sync(0xffffffffu, z[g][r], 2);
-                if (c4 == 0) s_z[warp][g][r8 + 8 * r] = z[g][r];
+                const float z = whole_row(z2[g][r]);
+                if (c4 == 0) s_z[warp][g][r8 + 8 * r] = z;
             }
         }
         lost = __syncthreads_or(lost);
@@ -837,9 +829,10 @@ cudaError_t launch_decode_attn_int4(const void *q, int64_t q_ld, const void *kp,
     const dim3 grid = s.cluster ? dim3(s.n_chunks, lists, static_cast<unsigned>(B)) : dim3(static_cast<unsigned>(s.ctas));
     Decode4Args p = {};
     p.q = static_cast<const uint16_t *>(q);
-    p.k4 = static_cast<const uint8_t *>(kp);
-    p.v4 = static_cast<const uint8_t *>(vp);
-    p.scales = static_cast<const uint16_t *>(scales);
+    // a cache without pages: addresses that nothing is copied from
+    p.k4 = static_cast<const uint8_t *>(kp ? kp : q);
+    p.v4 = static_cast<const uint8_t *>(vp ? vp : q);
+    p.scales = static_cast<const uint16_t *>(scales ? scales : q);
     p.table = table;
     p.seq_lens = seq_lens;
     p.new_lens = new_lens;
