@@ -149,29 +149,31 @@ rope_append_int4_kernel(const uint16_t *__restrict__ qkv, int64_t ld, const floa
 // subnormal n 2^-24, in bits 4 .. 7 n 2^-20, both exact, for one AND each (and a shift for
 // every second pair); the powers of two go into the queries and out of the results.
 //
-// Scores: rows (heads, new tokens) by keys, as in the bf16 cache's kernel. Outputs the
-// other way round, dimensions by rows: the weights then enter as the second operand in the
-// registers that the scores came in, and 8 rows cost half of what 16 do.
-// The queries of a row are scaled by a power of two to 2^9 .. 2^10 at most, so that fp16
-// holds all their bits. The weights p_t s_t are fp16, scaled to 2^13 at most by a power of
-// two above every scale so far: 11 bits, a quarter of the output's own rounding; weights
-// below 2^-24 of the largest lose bits. Everything else is fp32.
+// Both products have the numbers as their first operand: scores are keys by rows (heads, new
+// tokens), outputs dimensions by rows, so that 8 rows cost half of what 16 do; the weights
+// turn from the one layout to the other by movmatrix. The queries of a row are scaled by
+// a power of two to 2^9 .. 2^10 at most, so that fp16 holds all their bits. The weights
+// p_t s_t are fp16, scaled by a power of two above every scale so far: 11 bits, a quarter
+// of the output's own rounding; those below 2^-36 of the largest lose bits. p is taken
+// against a reference within 2^3 of the greatest so far, which moves when that is
+// passed: there is no search for the maximum in a tile that does not. Everything else is fp32.
 //
-// A warp takes tiles of 32 keys through its ring as the bf16 kernel does.
-constexpr int kTile = 32;
+// A warp takes tiles of 64 keys (hd 128: 32) through its ring as the bf16 kernel does.
+constexpr float kSlack = 3.0f;      // log2
 constexpr int kLeast = 4;           // tiles of a CTA's span, at least
-constexpr int kListCost = 4;        // tiles that a list's start and end cost
+constexpr int kListCost = 3;        // tiles that a list's start and end cost
 
 template <int HD, int ROWS>
 struct Dec4 {
     static constexpr int kStages = 3;
-    static constexpr int kCtas = HD == 64 ? (ROWS == 8 ? 5 : 4) : 3;      // resident on an SM
+    static constexpr int kCtas = 3;                   // resident on an SM
+    static constexpr int kTile = 4096 / HD;           // keys of a warp's step
     static constexpr int kGroups = HD / 64, kRowBytes = HD / 2, kScaleBytes = 8 * kGroups;
     static constexpr int kSide = kTile * kRowBytes;
     static constexpr int kStage = 2 * kSide + kTile * kScaleBytes;
     static constexpr int kRing = kDecWarps * kStages * kStage;
-    // the warps' tiles' scales and zeros in fp32; at a list's end their outputs, 8 rows at a time
-    static constexpr int kSmem = kRing + std::max(kDecWarps * kTile * 16 * kGroups, kDecWarps * 8 * HD * 4);
+    // the warps' tiles' scales and zeros in fp32, twice each; at a list's end their outputs, 8 rows at a time
+    static constexpr int kSmem = kRing + std::max(kDecWarps * kTile * 32 * kGroups, kDecWarps * 8 * HD * 4);
 };
 
 struct Decode4Args : DecodeArgs {
@@ -201,22 +203,28 @@ __device__ __forceinline__ void cp_async8(uint32_t dst, const void *src, int src
 }
 constexpr uint32_t kEven = 0x000F000Fu, kOdd = 0x00F000F0u;      // numbers 0 and 4, 1 and 5 of a word's eight
 
-// Column 2 c + e of score tile j is key 8 j + 4 e + c: a thread's two columns are then rows
-// of the values that four threads read from four neighbouring rows, without bank conflicts.
-// Keys lie in the ring in the columns' order.
-__device__ __forceinline__ int column_of(int key) { return (key & ~7) | (key & 3) << 1 | (key >> 2 & 1); }
+// The transpose of an 8 x 8 matrix of halves, a row's two neighbours in a thread.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
+    return r;
+}
+// Where a key's value lies in the ring: keys 2 c and 2 c + 1 of eight, which a thread pairs, in
+// rows c and c + 4, so that four threads read four neighbouring rows.
+__device__ __forceinline__ int value_row(int key) { return (key & ~7) | (key & 1) << 2 | (key >> 1 & 3); }
 
 template <int HD, int ROWS, bool Cluster>
 __global__ void __launch_bounds__(kDecWarps * 32, Dec4<HD, ROWS>::kCtas)
 decode_int4_kernel(const __grid_constant__ Decode4Args P) {
     using C = Dec4<HD, ROWS>;
-    constexpr int NG = C::kGroups, NR = ROWS / 8;
+    constexpr int NG = C::kGroups, NR = ROWS / 8, kTile = C::kTile, kKeys = kTile / 32, NM = kTile / 16;
     extern __shared__ __align__(128) unsigned char dsm[];
-    __shared__ float s_m[kDecWarps][ROWS], s_l[kDecWarps][ROWS], s_z[kDecWarps][NG][ROWS];
+    __shared__ __align__(16) float s_m[kDecWarps][ROWS], s_l[kDecWarps][ROWS], s_z[kDecWarps][NG][ROWS];
     __shared__ float2 s_part[ROWS];
     float *s_o = reinterpret_cast<float *>(dsm + C::kRing);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c4 = lane & 3, r8 = lane >> 2;
-    float4 *s_x = reinterpret_cast<float4 *>(dsm + C::kRing) + warp * kTile * NG;      // [group][pair of columns][key's, value's]
+    // [group][key's, value's][key]: scale, scale, zero, zero
+    ulonglong2 *s_x = reinterpret_cast<ulonglong2 *>(dsm + C::kRing) + warp * 2 * kTile * NG;
     const int G = P.H / P.Hk, groups = (P.rows + P.per - 1) / P.per, lists = P.Hk * groups;
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     DecSpan at;
@@ -235,7 +243,7 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
     const auto tiles_to = [&](int base, int tiles) { return max(min(tiles, end - base - kListCost), 0); };
 
     // The copies' side of this warp: it takes every fourth tile of the span, whatever list
-    // it is of. A lane looks its own key's page up while the tile before is copied. A page
+    // it is of. A lane looks its own keys' pages up while the tile before is copied. A page
     // outside the cache copies nothing and makes the sequence's result NaN.
     const uint32_t ring = smem_u32(dsm) + warp * C::kStages * C::kStage;
     const int page_mask = (1 << P.page_shift) - 1;
@@ -244,13 +252,14 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
     int32_t flen = !Cluster && fb + 1 < P.B ? P.seq_lens[fb + 1] : 0;      // the next sequence's
     const int32_t *frow = P.table + fb * P.table_ld;
     struct Tile {
-        int32_t page;
-        int rows, in_page, hk;      // rows: of the sequence; < 0: no tile
+        int32_t page[kKeys];
+        int rows, first, hk;      // rows: of the sequence; < 0: no tile
     };
     bool more = true;
     uint32_t bad = 0;      // a bit for each stage
     auto look = [&](int step) {
-        Tile tile = {0, -1, 0, 0};
+        Tile tile = {};
+        tile.rows = -1;
         if (!more) return tile;
         fi += step;
         while (fi >= fend) {
@@ -271,39 +280,49 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
             fhk = fy / groups;
             fend = tiles_to(fbase, fall);
         }
-        const int j = fi * kTile + lane;      // below 2^31 where it is a key
-        tile.rows = min(fn - fi * kTile, kTile);
-        tile.in_page = j & page_mask;
+        tile.first = fi * kTile;
+        tile.rows = min(fn - tile.first, kTile);
         tile.hk = fhk;
-        if (lane < tile.rows) tile.page = frow[j >> P.page_shift];
+#pragma unroll
+        for (int k = 0; k < kKeys; ++k)
+            if (lane + 32 * k < tile.rows) tile.page[k] = frow[(tile.first + lane + 32 * k) >> P.page_shift];
         return tile;
     };
-    // A lane's copies: chunk of 16 bytes `chunk` of rows u kPer + lane / kChunks. At hd 128 a row's
-    // two groups change places in every second pair of rows: no bank conflicts.
+    // A lane's copies: chunk of 16 bytes `chunk` of rows u kPer + crow0. At hd 128 a row's two
+    // groups change places in every second pair of rows: no bank conflicts.
     constexpr int kChunks = C::kRowBytes / 16, kPer = 32 / kChunks;
-    const int chunk = lane % kChunks, crow0 = lane / kChunks, ccol0 = column_of(crow0);
+    const int chunk = lane % kChunks, crow0 = lane / kChunks;
     const auto in_row = [&](int row) {
         return row * C::kRowBytes + (NG == 1 ? chunk * 16 : (chunk & 1) * 16 + 32 * ((chunk >> 1) ^ (row >> 1 & 1)));
     };
-    const uint32_t kdst = ring + in_row(ccol0), vdst = ring + C::kSide + in_row(crow0);
-    const uint32_t sdst = ring + 2 * C::kSide + column_of(lane) * C::kScaleBytes;
+    const uint32_t kdst = ring + in_row(crow0), vdst = ring + C::kSide + in_row(value_row(crow0));
+    const uint32_t sdst = ring + 2 * C::kSide + lane * C::kScaleBytes;
     const uint8_t *const ksrc = P.k4 + chunk * 16, *const vsrc = P.v4 + chunk * 16;
     auto fetch = [&](int stage, const Tile &tile) {
         if (tile.rows >= 0) {
-            const bool in = lane < tile.rows && tile.page >= 0 && tile.page < P.n_pages;
-            const uint32_t have = __ballot_sync(0xffffffffu, in);
-            const bool lacks = static_cast<int>(__popc(have)) < tile.rows;
-            bad = (bad & ~(1u << stage)) | static_cast<uint32_t>(lacks) << stage;
-            // rows of the cache are counted in 32 bits (the caller's check), bytes in 64; zeros behind the end
-            const uint32_t mine = in ? ((static_cast<uint32_t>(tile.page) * P.Hk + tile.hk) << P.page_shift) + tile.in_page : 0u;
             const uint32_t at = stage * C::kStage;
-            const uint16_t *sc = P.scales + static_cast<uint64_t>(mine) * (4 * NG);
-            if constexpr (NG == 1) cp_async8(sdst + at, sc, in ? 8 : 0);
-            else cp_async16(sdst + at, sc, in ? 16 : 0);
+            uint32_t mine[kKeys], have[kKeys];
+            int there = 0;
 #pragma unroll
-            for (int u = 0; u < kChunks; ++u) {
-                const uint64_t from = static_cast<uint64_t>(__shfl_sync(0xffffffffu, mine, u * kPer + crow0)) * C::kRowBytes;
-                const int bytes = have >> (u * kPer + crow0) & 1 ? 16 : 0;
+            for (int k = 0; k < kKeys; ++k) {
+                const int key = lane + 32 * k;
+                const bool in = key < tile.rows && tile.page[k] >= 0 && tile.page[k] < P.n_pages;
+                have[k] = __ballot_sync(0xffffffffu, in);
+                there += __popc(have[k]);
+                // rows of the cache are counted in 32 bits (the caller's check), bytes in 64; zeros behind the end
+                mine[k] = in ? ((static_cast<uint32_t>(tile.page[k]) * P.Hk + tile.hk) << P.page_shift) +
+                                   ((tile.first + key) & page_mask)
+                             : 0u;
+                const uint16_t *sc = P.scales + static_cast<uint64_t>(mine[k]) * (4 * NG);
+                if constexpr (NG == 1) cp_async8(sdst + at + 32 * k * C::kScaleBytes, sc, in ? 8 : 0);
+                else cp_async16(sdst + at + 32 * k * C::kScaleBytes, sc, in ? 16 : 0);
+            }
+            bad = (bad & ~(1u << stage)) | static_cast<uint32_t>(there < tile.rows) << stage;
+#pragma unroll
+            for (int u = 0; u < kTile / kPer; ++u) {
+                const int k = u * kPer / 32, r = u * kPer % 32 + crow0;
+                const uint64_t from = static_cast<uint64_t>(__shfl_sync(0xffffffffu, mine[k], r)) * C::kRowBytes;
+                const int bytes = have[k] >> r & 1 ? 16 : 0;
                 cp_async16(kdst + at + u * kPer * C::kRowBytes, ksrc + from, bytes);
                 cp_async16(vdst + at + u * kPer * C::kRowBytes, vsrc + from, bytes);
             }
@@ -317,12 +336,16 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
     fetch(1, tile1);
     Tile tile = look(kDecWarps);
 
-    // The products' side, list by list. Queries: rows r8 (+ 8); of each group the 16
-    // dimensions from 16 c4 on, as the numbers of a thread's two words pair up. even: those
-    // that meet numbers in the low places, 16 times the others.
-    uint32_t qa[NG][4][2 * NR];
-    float crow[NR], qsum[NG][NR];      // scores from products; the queries' sums in the products' units
-    auto queries = [&](int qb, int qy) {
+    // The products' side, list by list. Queries: of row r8 (+ 8) and each group the 16
+    // dimensions from 16 c4 on, as the numbers of a thread's two words pair up; those that meet
+    // numbers in the low places are 16 times the others. A thread's scores are of rows 2 c4,
+    // 2 c4 + 1 (+ 8): for these, from products to scores, and the queries' sums in the products' units.
+    uint32_t qb[NG][4][NR][2];
+    uint64_t crow[NR], qsum[NG][NR];
+    const auto two_rows = [&](float v) {      // of the rows r8 that threads hold, this thread's two
+        return tc::f2(__shfl_sync(0xffffffffu, v, 8 * c4), __shfl_sync(0xffffffffu, v, 8 * c4 + 4));
+    };
+    auto queries = [&](int seq, int qy) {
         const int row0 = qy % groups * P.per, nr = min(P.per, P.rows - row0), hk = qy / groups;
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
@@ -335,7 +358,7 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                     raw[g][w] = make_uint4(0, 0, 0, 0);
                     if (mine < nr)
                         raw[g][w] = *reinterpret_cast<const uint4 *>(
-                            P.q + (static_cast<int64_t>(qb) * P.n_new + row / G) * P.q_ld +
+                            P.q + (static_cast<int64_t>(seq) * P.n_new + row / G) * P.q_ld +
                             static_cast<int64_t>(hk * G + row % G) * HD + 64 * g + 16 * c4 + 8 * w);
                 }
             uint32_t top = 0;      // the greatest magnitude's bits
@@ -353,8 +376,9 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
             const int up = min(136 - static_cast<int>(top >> 7), 100);
             const float f = pow2(up);
             // positive and finite: beyond these bounds one key has all the weight, or all have the same
-            crow[r] = fminf(fmaxf(P.scale_log2 * pow2(min(20 - up, 127)), 1e-37f), 3e38f);
-            if (top >= 0x7f80u) crow[r] = __int_as_float(0x7fc00000);            // a query that is not finite
+            float c = fminf(fmaxf(P.scale_log2 * pow2(min(20 - up, 127)), 1e-37f), 3e38f);
+            if (top >= 0x7f80u) c = __int_as_float(0x7fc00000);            // a query that is not finite
+            crow[r] = two_rows(c);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 float sum = 0.0f;
@@ -369,13 +393,13 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                     }
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        qa[g][2 * w + e][r] = pack_f16x2(16.0f * x[2 * e], 16.0f * x[2 * e + 4]);
-                        qa[g][2 * w + e][NR + r] = pack_f16x2(x[2 * e + 1], x[2 * e + 5]);
+                        qb[g][2 * w + e][r][0] = pack_f16x2(16.0f * x[2 * e], 16.0f * x[2 * e + 4]);
+                        qb[g][2 * w + e][r][1] = pack_f16x2(x[2 * e + 1], x[2 * e + 5]);
                     }
                 }
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                qsum[g][r] = sum * 0x1p-20f;
+                qsum[g][r] = two_rows(sum * 0x1p-20f);
             }
         }
     };
@@ -388,19 +412,21 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
         const int tiles = tiles_to(base, len.tiles) - i0;
         bool lost = len.lost || fresh.lost;
         // keys that this thread's rows see (of rows that are no new token's: whatever there is), and that all see
-        int sees[NR];
+        int sees[NR][2];
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-            const int j = (row0 + r8 + 8 * r) / G;
-            sees[r] = j < fresh.count ? fresh.first + j : INT32_MAX;
-        }
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int j = (row0 + 8 * r + 2 * c4 + e) / G;
+                sees[r][e] = j < fresh.count ? fresh.first + j : INT32_MAX;
+            }
         const int all_see = row0 / G < fresh.count ? fresh.first + row0 / G : INT32_MAX;
-        float acc[NG][4][NR][4], m[NR];
-        uint64_t l2[NR], z2[NG][NR];      // of a thread's even and odd columns
+        float acc[NG][4][NR][4], m[NR][2];
+        uint64_t l2[NR], z2[NG][NR];
         int top[NG];        // 2^(top - 127) is above every scale so far
         const uint64_t none2 = tc::f2(0.0f, 0.0f);
 #pragma unroll
-        for (int r = 0; r < NR; ++r) m[r] = -INFINITY, l2[r] = none2;
+        for (int r = 0; r < NR; ++r) m[r][0] = m[r][1] = -INFINITY, l2[r] = none2;
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             top[g] = 15;
@@ -419,17 +445,19 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
             lost |= bad >> head & 1;
             const int key0 = (i0 + i) * kTile;
             const unsigned char *sk = dsm + (warp * C::kStages + head) * C::kStage, *sv = sk + C::kSide, *ss = sv + C::kSide;
-            // Scales and zeros in fp32, once for the warp: an even lane those of the keys of columns
-            // lane, lane + 1, an odd one those of its columns' values (lane - 1, lane), whose scales
-            // take the weights' unit along. A finite one above the power of two so far raises that.
+            // Scales and zeros in fp32, once for the warp, each lane its keys'; the values' scales take
+            // the weights' unit along. A finite one above the power of two so far raises that.
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                const uint32_t *two = reinterpret_cast<const uint32_t *>(ss + (lane & ~1) * C::kScaleBytes) + 2 * g + (lane & 1);
-                const uint32_t a = two[0], c = two[2 * NG];
-                float sa = bf_lo(a), sb = bf_lo(c);
-                const float most = lane & 1 ? fmaxf(sa, sb) : 0.0f;
+                uint2 raw[kKeys];
+                float most = 0.0f;
+#pragma unroll
+                for (int k = 0; k < kKeys; ++k) {
+                    raw[k] = *reinterpret_cast<const uint2 *>(ss + (lane + 32 * k) * C::kScaleBytes + 8 * g);
+                    most = fmaxf(most, bf_lo(raw[k].y));
+                }
                 if (__any_sync(0xffffffffu, most >= pow2(top[g] - 127))) {
-                    const int to = (__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(most, 0.0f))) >> 23) + 1;
+                    const int to = static_cast<int>(__reduce_max_sync(0xffffffffu, __float_as_uint(most)) >> 23) + 1;
                     const float f = to - top[g] <= 126 ? pow2(top[g] - to) : 0.0f;
                     top[g] = to;
 #pragma unroll
@@ -439,103 +467,131 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
 #pragma unroll
                             for (int e = 0; e < 4; ++e) acc[g][i2][r][e] *= f;
                 }
-                if (lane & 1) {
-                    const float unit = pow2(140 - top[g]);
-                    sa *= unit, sb *= unit;
+                const float unit = pow2(139 - top[g]);
+#pragma unroll
+                for (int k = 0; k < kKeys; ++k) {
+                    const float ks = bf_lo(raw[k].x), kz = bf_hi(raw[k].x), vs = bf_lo(raw[k].y) * unit, vz = bf_hi(raw[k].y);
+                    s_x[(2 * g) * kTile + lane + 32 * k] = make_ulonglong2(tc::f2(ks, ks), tc::f2(kz, kz));
+                    s_x[(2 * g + 1) * kTile + lane + 32 * k] = make_ulonglong2(tc::f2(vs, vs), tc::f2(vz, vz));
                 }
-                s_x[g * kTile + lane] = make_float4(sa, sb, bf_hi(a), bf_hi(c));
             }
             __syncwarp();
-            float t[4][2 * NR];
+            // scores of keys 16 mt + 8 h + r8, both rows of a pair in one register pair
+            uint64_t t[NM][2][NR];
 #pragma unroll
             for (int g = 0; g < NG; ++g)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint2 w2 = *reinterpret_cast<const uint2 *>(sk + (8 * j + r8) * C::kRowBytes + 8 * c4 +
-                                                                      (NG == 1 ? 0 : 32 * (g ^ (r8 >> 1 & 1))));
-                    const uint32_t w[2] = {w2.x, w2.y};
-                    float d[4] = {};
+                for (int mt = 0; mt < NM; ++mt) {
+                    uint32_t w[2][2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int row = 16 * mt + 8 * h + r8;
+                        const uint2 x = *reinterpret_cast<const uint2 *>(sk + row * C::kRowBytes + 8 * c4 +
+                                                                         (NG == 1 ? 0 : 32 * (g ^ (r8 >> 1 & 1))));
+                        w[h][0] = x.x, w[h][1] = x.y;
+                    }
+                    float d[NR][4] = {};
 #pragma unroll
                     for (int s = 0; s < 4; ++s) {
-                        const uint32_t x = s & 1 ? w[s >> 1] >> 8 : w[s >> 1];
-                        if constexpr (NR == 1) mma_f16(d, qa[g][s][0], 0u, qa[g][s][1], 0u, x & kEven, x & kOdd);
-                        else mma_f16(d, qa[g][s][0], qa[g][s][1], qa[g][s][2], qa[g][s][3], x & kEven, x & kOdd);
-                    }
-                    const ulonglong2 sz = *reinterpret_cast<const ulonglong2 *>(&s_x[g * kTile + 8 * j + 2 * c4]);
+                        const uint32_t x = s & 1 ? w[0][s >> 1] >> 8 : w[0][s >> 1];
+                        const uint32_t x2 = s & 1 ? w[1][s >> 1] >> 8 : w[1][s >> 1];
 #pragma unroll
-                    for (int r = 0; r < NR; ++r) {
-                        const uint64_t q2 = tc::f2(qsum[g][r], qsum[g][r]);
-                        const uint64_t zero = g == 0 ? tc::mul2(sz.y, q2) : tc::fma2(sz.y, q2, tc::f2(t[j][2 * r], t[j][2 * r + 1]));
-                        const float2 got = tc::f2_split(tc::fma2(sz.x, tc::f2(d[2 * r], d[2 * r + 1]), zero));
-                        t[j][2 * r] = got.x;
-                        t[j][2 * r + 1] = got.y;
+                        for (int r = 0; r < NR; ++r)
+                            mma_f16(d[r], x & kEven, x2 & kEven, x & kOdd, x2 & kOdd, qb[g][s][r][0], qb[g][s][r][1]);
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const ulonglong2 sz = s_x[(2 * g) * kTile + 16 * mt + 8 * h + r8];
+#pragma unroll
+                        for (int r = 0; r < NR; ++r) {
+                            const uint64_t zero = g == 0 ? tc::mul2(sz.y, qsum[g][r]) : tc::fma2(sz.y, qsum[g][r], t[mt][h][r]);
+                            t[mt][h][r] = tc::fma2(sz.x, tc::f2(d[r][2 * h], d[r][2 * h + 1]), zero);
+                        }
                     }
                 }
             const bool masked = key0 + kTile > all_see;
             if (masked) {
 #pragma unroll
-                for (int r = 0; r < NR; ++r)
+                for (int mt = 0; mt < NM; ++mt)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
+                    for (int h = 0; h < 2; ++h) {
+                        const int key = key0 + 16 * mt + 8 * h + r8;
 #pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            if (key0 + 8 * j + 4 * e + c4 >= sees[r]) t[j][2 * r + e] = -INFINITY;
+                        for (int r = 0; r < NR; ++r) {
+                            const float2 x = tc::f2_split(t[mt][h][r]);
+                            t[mt][h][r] = tc::f2(key < sees[r][0] ? x.x : -INFINITY, key < sees[r][1] ? x.y : -INFINITY);
+                        }
+                    }
             }
-            float mx[NR];
+            // the greatest score that this thread has of each row (NaN left out); the references move if one is far above
+            float mx[NR][2];
             bool grown = false;
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
-                mx[r] = fmaxf(tc::fmax3(tc::fmax3(t[0][2 * r], t[0][2 * r + 1], t[1][2 * r]), t[1][2 * r + 1], t[2][2 * r]),
-                              tc::fmax3(t[2][2 * r + 1], t[3][2 * r], t[3][2 * r + 1]));
-                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-                // (the greatest of nothing, or of NaN alone, leaves the maximum as it was)
-                mx[r] = fmaxf(mx[r] * crow[r], m[r]);
-                grown |= mx[r] > m[r];
+                float2 x = tc::f2_split(t[0][0][r]);
+                mx[r][0] = x.x, mx[r][1] = x.y;
+#pragma unroll
+                for (int k = 1; k < 2 * NM; k += 2) {
+                    x = tc::f2_split(t[k >> 1][k & 1][r]);
+                    const float2 x2 = k + 1 < 2 * NM ? tc::f2_split(t[(k + 1) >> 1][(k + 1) & 1][r]) : x;
+                    mx[r][0] = tc::fmax3(mx[r][0], x.x, x2.x);
+                    mx[r][1] = tc::fmax3(mx[r][1], x.y, x2.y);
+                }
+                const float2 c = tc::f2_split(crow[r]);
+                mx[r][0] *= c.x, mx[r][1] *= c.y;
+                grown |= mx[r][0] > m[r][0] + kSlack || mx[r][1] > m[r][1] + kSlack;
             }
             if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
                 for (int r = 0; r < NR; ++r) {
-                    const float f = mx[r] > m[r] ? tc::ex2(m[r] - mx[r]) : 1.0f;
-                    const uint64_t ff = tc::f2(f, f);
-                    m[r] = mx[r];
-                    l2[r] = tc::mul2(l2[r], ff);
-                    const float f0 = __shfl_sync(0xffffffffu, f, 8 * c4), f1 = __shfl_sync(0xffffffffu, f, 8 * c4 + 4);
+                    float f[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float x = fmaxf(mx[r][e], m[r][e]);      // not NaN
+#pragma unroll
+                        for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+                        f[e] = x > m[r][e] ? tc::ex2(m[r][e] - x) : 1.0f;
+                        m[r][e] = x;
+                    }
+                    const uint64_t f2 = tc::f2(f[0], f[1]);
+                    l2[r] = tc::mul2(l2[r], f2);
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
-                        z2[g][r] = tc::mul2(z2[g][r], ff);
+                        z2[g][r] = tc::mul2(z2[g][r], f2);
 #pragma unroll
                         for (int i2 = 0; i2 < 4; ++i2)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) acc[g][i2][r][e] *= e & 1 ? f1 : f0;
+                            for (int e = 0; e < 4; ++e) acc[g][i2][r][e] *= f[e & 1];
                     }
                 }
             }
-            uint32_t pw[NG][4][NR];
+            uint32_t pw[NG][NM][2][NR];
             auto weigh = [&](auto some_hidden) {
 #pragma unroll
                 for (int r = 0; r < NR; ++r) {
-                    const float ref = m[r] == -INFINITY ? 0.0f : -m[r];
-                    const uint64_t ref2 = tc::f2(ref, ref), c2 = tc::f2(crow[r], crow[r]);
+                    const uint64_t ref = tc::f2(m[r][0] == -INFINITY ? 0.0f : -m[r][0], m[r][1] == -INFINITY ? 0.0f : -m[r][1]);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint64_t p2 = tc::ex2_pair(tc::fma2(tc::f2(t[j][2 * r], t[j][2 * r + 1]), c2, ref2));
-                        l2[r] = tc::add2(l2[r], p2);
+                    for (int mt = 0; mt < NM; ++mt)
 #pragma unroll
-                        for (int g = 0; g < NG; ++g) {
-                            ulonglong2 sz = *reinterpret_cast<const ulonglong2 *>(&s_x[g * kTile + 8 * j + 2 * c4 + 1]);
-                            if constexpr (some_hidden.value) {
-                                // what a row does not see does not reach it: NaN scales neither
-                                const bool h0 = key0 + 8 * j + c4 >= sees[r], h1 = key0 + 8 * j + 4 + c4 >= sees[r];
-                                const float2 a = tc::f2_split(sz.x), c = tc::f2_split(sz.y);
-                                sz.x = tc::f2(h0 ? 0.0f : a.x, h1 ? 0.0f : a.y);
-                                sz.y = tc::f2(h0 ? 0.0f : c.x, h1 ? 0.0f : c.y);
+                        for (int h = 0; h < 2; ++h) {
+                            const uint64_t p2 = tc::ex2_pair(tc::fma2(t[mt][h][r], crow[r], ref));
+                            l2[r] = tc::add2(l2[r], p2);
+                            const int key = 16 * mt + 8 * h + r8;
+#pragma unroll
+                            for (int g = 0; g < NG; ++g) {
+                                ulonglong2 sz = s_x[(2 * g + 1) * kTile + key];
+                                if constexpr (some_hidden.value) {
+                                    // what a row does not see does not reach it: NaN scales neither
+                                    const bool s0 = key0 + key < sees[r][0], s1 = key0 + key < sees[r][1];
+                                    const float a = tc::f2_split(sz.x).x, c = tc::f2_split(sz.y).x;
+                                    sz.x = tc::f2(s0 ? a : 0.0f, s1 ? a : 0.0f);
+                                    sz.y = tc::f2(s0 ? c : 0.0f, s1 ? c : 0.0f);
+                                }
+                                z2[g][r] = tc::fma2(p2, sz.y, z2[g][r]);
+                                const float2 w = tc::f2_split(tc::mul2(p2, sz.x));
+                                pw[g][mt][h][r] = transpose8(pack_f16x2(w.x, w.y));
                             }
-                            z2[g][r] = tc::fma2(p2, sz.y, z2[g][r]);
-                            const float2 w = tc::f2_split(tc::mul2(p2, sz.x));
-                            pw[g][j][r] = pack_f16x2(w.x, w.y);
                         }
-                    }
                 }
             };
             if (masked) weigh(std::true_type{});
@@ -543,16 +599,16 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
 #pragma unroll
             for (int g = 0; g < NG; ++g)
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    uint32_t w[2][2];      // numbers 0 .. 3 and 4 .. 7 of both tokens, of score tiles 2 s and 2 s + 1
+                for (int mt = 0; mt < NM; ++mt) {
+                    uint32_t w[2][2];      // numbers 0 .. 3 and 4 .. 7 of keys 2 c4 and 2 c4 + 1 (+ 8)
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const unsigned char *src = sv + (16 * s + 8 * u + c4) * C::kRowBytes + 4 * r8 +
+                    for (int h = 0; h < 2; ++h) {
+                        const unsigned char *src = sv + (16 * mt + 8 * h + c4) * C::kRowBytes + 4 * r8 +
                                                    (NG == 1 ? 0 : 32 * (g ^ (c4 >> 1)));
                         const uint32_t x0 = *reinterpret_cast<const uint32_t *>(src);
                         const uint32_t x1 = *reinterpret_cast<const uint32_t *>(src + 4 * C::kRowBytes);
-                        w[u][0] = __byte_perm(x0, x1, 0x5410);
-                        w[u][1] = __byte_perm(x0, x1, 0x7632);
+                        w[h][0] = __byte_perm(x0, x1, 0x5410);
+                        w[h][1] = __byte_perm(x0, x1, 0x7632);
                     }
 #pragma unroll
                     for (int i2 = 0; i2 < 4; ++i2) {
@@ -560,8 +616,7 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                         const uint32_t x2 = i2 & 1 ? w[1][i2 >> 1] >> 8 : w[1][i2 >> 1];
 #pragma unroll
                         for (int r = 0; r < NR; ++r)
-                            mma_f16(acc[g][i2][r], x & kEven, x & kOdd, x2 & kEven, x2 & kOdd, pw[g][2 * s][r],
-                                    pw[g][2 * s + 1][r]);
+                            mma_f16(acc[g][i2][r], x & kEven, x & kOdd, x2 & kEven, x2 & kOdd, pw[g][mt][0][r], pw[g][mt][1][r]);
                     }
                 }
             __syncwarp();      // the stage that the next copy overwrites has been read
@@ -582,23 +637,26 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
         }
 
         // join the warps: their maxima and sums, then the outputs of eight rows at a time
-        const auto whole_row = [](uint64_t v2) {
-            const float2 v = tc::f2_split(v2);
-            float sum = v.x + v.y;
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            return sum + __shfl_xor_sync(0xffffffffu, sum, 2);
+        const auto whole_rows = [](uint64_t v2) {
+            float2 v = tc::f2_split(v2);
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+                v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+            }
+            return v;
         };
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-            const float l = whole_row(l2[r]);
-            if (c4 == 0) {
-                s_m[warp][r8 + 8 * r] = m[r];
-                s_l[warp][r8 + 8 * r] = l;
+            const float2 l = whole_rows(l2[r]);
+            if (r8 == 0) {
+                *reinterpret_cast<float2 *>(&s_m[warp][8 * r + 2 * c4]) = make_float2(m[r][0], m[r][1]);
+                *reinterpret_cast<float2 *>(&s_l[warp][8 * r + 2 * c4]) = l;
             }
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                const float z = whole_row(z2[g][r]);
-                if (c4 == 0) s_z[warp][g][r8 + 8 * r] = z;
+                const float2 z = whole_rows(z2[g][r]);
+                if (r8 == 0) *reinterpret_cast<float2 *>(&s_z[warp][g][8 * r + 2 * c4]) = z;
             }
         }
         lost = __syncthreads_or(lost);
@@ -622,8 +680,8 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
 #pragma unroll
                     for (int i2 = 0; i2 < 4; i2 += 2)
                         *reinterpret_cast<float4 *>(dst + 2 * i2) =
-                            make_float4(acc[g][i2][r][e] * 2048.0f * u, acc[g][i2][r][2 + e] * 128.0f * u,
-                                        acc[g][i2 + 1][r][e] * 2048.0f * u, acc[g][i2 + 1][r][2 + e] * 128.0f * u);
+                            make_float4(acc[g][i2][r][e] * 4096.0f * u, acc[g][i2][r][2 + e] * 256.0f * u,
+                                        acc[g][i2 + 1][r][e] * 4096.0f * u, acc[g][i2 + 1][r][2 + e] * 256.0f * u);
                 }
             }
             __syncthreads();
@@ -747,7 +805,7 @@ static int list_rows(int64_t rows) {
 
 DecodeSplit decode_int4_split(int64_t B, int64_t rows, int64_t Hk, int64_t hd, int64_t max_len) {
     DecodeSplit s;
-    const int per = list_rows(rows);
+    const int per = list_rows(rows), tile = hd == 64 ? Dec4<64, 8>::kTile : Dec4<128, 8>::kTile;
     const int64_t lists = B * Hk * ((rows + per - 1) / per);
     const int ctas = hd == 64 ? (per <= 8 ? Dec4<64, 8>::kCtas : Dec4<64, 16>::kCtas)
                               : (per <= 8 ? Dec4<128, 8>::kCtas : Dec4<128, 16>::kCtas);
@@ -755,13 +813,13 @@ DecodeSplit decode_int4_split(int64_t B, int64_t rows, int64_t Hk, int64_t hd, i
     // few short lists: as one cluster each, of up to 8 chunks of up to 1024 keys
     const int64_t most = std::min<int64_t>(kClusterMost, resident / std::max<int64_t>(lists, 1));
     if (most > 0 && max_len <= most * 1024) {
-        const int64_t chunk = std::max<int64_t>((max_len + most - 1) / most, 128);
+        const int64_t chunk = std::max<int64_t>((max_len + most - 1) / most, 4 * tile);
         s.chunk = static_cast<int>((chunk + 63) / 64 * 64);
         s.n_chunks = static_cast<int>(std::max<int64_t>(1, (max_len + s.chunk - 1) / s.chunk));
         s.cluster = true;
         return s;
     }
-    s.ctas = std::min(resident, lists * std::max<int64_t>((max_len + kTile * kLeast - 1) / (kTile * kLeast), 1));
+    s.ctas = std::min(resident, lists * std::max<int64_t>((max_len + tile * kLeast - 1) / (tile * kLeast), 1));
     s.lists = lists;
     return s;
 }
