@@ -146,34 +146,57 @@ rope_append_int4_kernel(const uint16_t *__restrict__ qkv, int64_t ld, const floa
 //   out     = sum_t (p_t s_t) n_t + sum_t p_t z_t
 // so that neither product needs the values themselves. The numbers enter the m16n8k16
 // products as fp16 straight from memory's bits: a number in bits 0 .. 3 of a half is the
-// subnormal n 2^-24, in bits 4 .. 7 n 2^-20, both exact, for one AND each (and a shift for
-// every second pair); the powers of two go into the queries and out of the results.
+// subnormal n 2^-24, in bits 4 .. 7 n 2^-20, a byte n + 16 n' times 2^-24, all exact, for
+// one AND or byte permutation each; where a byte stands for its two numbers, the upper
+// one's product is taken off again (fp32 sums, 16 times the size of what is left).
 //
 // Both products have the numbers as their first operand: scores are keys by rows (heads, new
 // tokens), outputs dimensions by rows, so that 8 rows cost half of what 16 do; the weights
-// turn from the one layout to the other by movmatrix. The queries of a row are scaled by
-// a power of two to 2^9 .. 2^10 at most, so that fp16 holds all their bits. The weights
-// p_t s_t are fp16, scaled by a power of two above every scale so far: 11 bits, a quarter
-// of the output's own rounding; those below 2^-36 of the largest lose bits. p is taken
-// against a reference within 2^3 of the greatest so far, which moves when that is
-// passed: there is no search for the maximum in a tile that does not. Everything else is fp32.
+// turn from the one layout to the other by movmatrix. One row alone (a head of keys for
+// each of queries, one new token) has a form of its own: the columns that other rows would
+// have take the parts of a byte and of a word apart, and the softmax is shared out over all
+// lanes. The queries of a row are scaled by a power of two to 2^9 .. 2^10 at most, so that fp16
+// holds all their bits. The weights p_t s_t are fp16, scaled by a power of two above every
+// scale so far: 11 bits, a quarter of the output's own rounding; those below 2^-36 of the
+// largest lose bits. p is taken against a reference within 2^3 of the greatest so far, which
+// moves when that is passed: no search for the maximum in a tile that does not. Everything
+// else is fp32.
 //
-// A warp takes tiles of 64 keys (hd 128: 32) through its ring as the bf16 kernel does.
+// A warp takes tiles of 64 keys (hd 128: 32) through a ring of its own, as the bf16 kernel
+// does, by bulk copies: a lane for each page's keys, values or scales (16-byte copies of
+// each row took 105 instructions a tile). What a page holds behind the sequence's end
+// comes along and is hidden like all that a row does not see.
 constexpr float kSlack = 3.0f;      // log2
 constexpr int kLeast = 4;           // tiles of a CTA's span, at least
 constexpr int kListCost = 3;        // tiles that a list's start and end cost
+constexpr int kMostRows = 24;       // of a list
 
+#ifndef S1
+#define S1 2
+#define C1 4
+#define S8 3
+#define C8 3
+#define S16 2
+#define C16 2
+#endif
 template <int HD, int ROWS>
 struct Dec4 {
-    static constexpr int kStages = 3;
-    static constexpr int kCtas = 3;                   // resident on an SM
+    static constexpr int kStages = ROWS == 1 ? S1 : ROWS == 8 ? S8 : S16;
+    static constexpr int kCtas = ROWS == 1 ? C1 : ROWS == 8 ? C8 : C16;                   // resident on an SM
     static constexpr int kTile = 4096 / HD;           // keys of a warp's step
     static constexpr int kGroups = HD / 64, kRowBytes = HD / 2, kScaleBytes = 8 * kGroups;
     static constexpr int kSide = kTile * kRowBytes;
     static constexpr int kStage = 2 * kSide + kTile * kScaleBytes;
     static constexpr int kRing = kDecWarps * kStages * kStage;
-    // the warps' tiles' scales and zeros in fp32, twice each; at a list's end their outputs, 8 rows at a time
-    static constexpr int kSmem = kRing + std::max(kDecWarps * kTile * 32 * kGroups, kDecWarps * 8 * HD * 4);
+    static constexpr int kPass = ROWS == 1 ? 1 : 8;   // rows that are joined at a time
+    // a warp's words between its lanes: the weights of a tile, in the low and in the high half
+    // (ROWS 1), or its scales and zeros in fp32, twice each
+    static constexpr int kStride = kTile / 4 + 4;
+    static constexpr int kWords = ROWS == 1 ? 8 * kStride * kGroups : kTile * 8 * kGroups;
+    // that, and at a list's end the warps' outputs
+    static constexpr int kSmem = kRing + std::max(kDecWarps * kWords * 4, kDecWarps * kPass * HD * 4);
+    // a grid of kCtas an SM is resident at once: an SM's shared memory, 1 KB and the static part a CTA
+    static_assert(kCtas * (kSmem + 1024 + kDecWarps * (kStages + 2 * (ROWS + 7)) * 8 + kDecWarps * kGroups * (ROWS + 7) * 4) <= 228 * 1024);
 };
 
 struct Decode4Args : DecodeArgs {
@@ -190,6 +213,15 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The same without anything to add to.
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+        "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
     uint32_t v;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(v) : "f"(hi), "f"(lo));
@@ -198,35 +230,53 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }      // -126 .. 127
 __device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
-__device__ __forceinline__ void cp_async8(uint32_t dst, const void *src, int src_bytes) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(dst), "l"(src), "r"(src_bytes));
-}
-constexpr uint32_t kEven = 0x000F000Fu, kOdd = 0x00F000F0u;      // numbers 0 and 4, 1 and 5 of a word's eight
-
 // The transpose of an 8 x 8 matrix of halves, a row's two neighbours in a thread.
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
     uint32_t r;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
     return r;
 }
-// Where a key's value lies in the ring: keys 2 c and 2 c + 1 of eight, which a thread pairs, in
-// rows c and c + 4, so that four threads read four neighbouring rows.
-__device__ __forceinline__ int value_row(int key) { return (key & ~7) | (key & 1) << 2 | (key >> 1 & 3); }
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+// Waits for a barrier's phase, for about a second at most.
+__device__ __forceinline__ bool wait_phase(uint64_t *bar, uint32_t parity) {
+    if (tc::mbar_try_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+    while (!tc::mbar_try_wait_suspend(bar, parity, tc::kWaitSuspendNs))
+        if (clock64() - t0 > tc::kWaitLimitCycles) return false;
+    return true;
+}
+constexpr uint32_t kEven = 0x000F000Fu, kOdd = 0x00F000F0u;      // numbers 0 and 4, 1 and 5 of a word's eight
+// Byte 0 (1) of both halves of a word, as halves.
+__device__ __forceinline__ uint32_t bytes_of(uint32_t w, int which) { return __byte_perm(w, 0, which ? 0x4341 : 0x4240); }
+// The key of eight in row p of a score block. Rows p of four threads, and after the transpose
+// rows 2 c (or 2 c + 1) of four, are then rows of the ring that differ mod 4: no bank conflicts.
+__device__ __forceinline__ int key_of(int p) { return (p >> 1 & 1) | ((p ^ p >> 2) & 1) << 1 | (p & 4); }
 
 template <int HD, int ROWS, bool Cluster>
 __global__ void __launch_bounds__(kDecWarps * 32, Dec4<HD, ROWS>::kCtas)
 decode_int4_kernel(const __grid_constant__ Decode4Args P) {
     using C = Dec4<HD, ROWS>;
-    constexpr int NG = C::kGroups, NR = ROWS / 8, kTile = C::kTile, kKeys = kTile / 32, NM = kTile / 16;
+    constexpr int NG = C::kGroups, NR = (ROWS + 7) / 8, kTile = C::kTile, kKeys = kTile / 32, NM = kTile / 16;
     extern __shared__ __align__(128) unsigned char dsm[];
-    __shared__ __align__(16) float s_m[kDecWarps][ROWS], s_l[kDecWarps][ROWS], s_z[kDecWarps][NG][ROWS];
-    __shared__ float2 s_part[ROWS];
+    __shared__ uint64_t s_full[kDecWarps][C::kStages];
+    __shared__ __align__(16) float s_m[kDecWarps][8 * NR], s_l[kDecWarps][8 * NR], s_z[kDecWarps][NG][8 * NR];
+    __shared__ float2 s_part[8 * NR];
     float *s_o = reinterpret_cast<float *>(dsm + C::kRing);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c4 = lane & 3, r8 = lane >> 2;
-    // [group][key's, value's][key]: scale, scale, zero, zero
-    ulonglong2 *s_x = reinterpret_cast<ulonglong2 *>(dsm + C::kRing) + warp * 2 * kTile * NG;
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) >> 5, 0);
+    const int lane = threadIdx.x & 31, c4 = lane & 3, r8 = lane >> 2;
+    uint32_t *s_w = reinterpret_cast<uint32_t *>(dsm + C::kRing) + warp * C::kWords;
     const int G = P.H / P.Hk, groups = (P.rows + P.per - 1) / P.per, lists = P.Hk * groups;
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    if (lane == 0) {
+#pragma unroll
+        for (int e = 0; e < C::kStages; ++e) tc::mbar_init(&s_full[warp][e], 1);
+        tc::fence_proxy_async_smem();
+    }
+    __syncwarp();
     DecSpan at;
     if constexpr (Cluster) {
         const int first = static_cast<int>(blockIdx.x) * P.chunk / kTile;
@@ -243,23 +293,27 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
     const auto tiles_to = [&](int base, int tiles) { return max(min(tiles, end - base - kListCost), 0); };
 
     // The copies' side of this warp: it takes every fourth tile of the span, whatever list
-    // it is of. A lane looks its own keys' pages up while the tile before is copied. A page
-    // outside the cache copies nothing and makes the sequence's result NaN.
-    const uint32_t ring = smem_u32(dsm) + warp * C::kStages * C::kStage;
-    const int page_mask = (1 << P.page_shift) - 1;
+    // it is of. Lane 4 i + kind looks the tile's page i up while the tile before is copied,
+    // and copies its keys, values or scales (kind 0, 1, 2). A page outside the cache is not
+    // copied and makes the sequence's result NaN.
+    const int page_mask = (1 << P.page_shift) - 1, page_rows = min(1 << P.page_shift, kTile);
+    const int kind = lane & 3, piece = lane >> 2;
+    const uint32_t row_bytes = kind < 2 ? C::kRowBytes : C::kScaleBytes;
+    const uint8_t *const src = kind == 0 ? P.k4 : kind == 1 ? P.v4 : reinterpret_cast<const uint8_t *>(P.scales);
+    const uint32_t dst = smem_u32(dsm) + warp * C::kStages * C::kStage + kind * C::kSide + piece * page_rows * row_bytes;
+    const int piece_first = kind < 3 ? piece * page_rows : kTile;      // its first key; none is that far
     int fbase = 0, fb = at.b, fy = at.y, fhk = fy / groups, fi = at.i, fn = len.n, fall = len.tiles;
     int fend = tiles_to(fbase, fall);
     int32_t flen = !Cluster && fb + 1 < P.B ? P.seq_lens[fb + 1] : 0;      // the next sequence's
     const int32_t *frow = P.table + fb * P.table_ld;
     struct Tile {
-        int32_t page[kKeys];
+        int32_t page;
         int rows, first, hk;      // rows: of the sequence; < 0: no tile
     };
     bool more = true;
     uint32_t bad = 0;      // a bit for each stage
     auto look = [&](int step) {
-        Tile tile = {};
-        tile.rows = -1;
+        Tile tile = {0, -1, 0, 0};
         if (!more) return tile;
         fi += step;
         while (fi >= fend) {
@@ -281,75 +335,50 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
             fend = tiles_to(fbase, fall);
         }
         tile.first = fi * kTile;
-        tile.rows = min(fn - tile.first, kTile);
+        tile.rows = fn - tile.first;
         tile.hk = fhk;
-#pragma unroll
-        for (int k = 0; k < kKeys; ++k)
-            if (lane + 32 * k < tile.rows) tile.page[k] = frow[(tile.first + lane + 32 * k) >> P.page_shift];
+        if (piece_first < min(tile.rows, kTile)) tile.page = frow[(tile.first >> P.page_shift) + piece];
         return tile;
     };
-    // A lane's copies: chunk of 16 bytes `chunk` of rows u kPer + crow0. At hd 128 a row's two
-    // groups change places in every second pair of rows: no bank conflicts.
-    constexpr int kChunks = C::kRowBytes / 16, kPer = 32 / kChunks;
-    const int chunk = lane % kChunks, crow0 = lane / kChunks;
-    const auto in_row = [&](int row) {
-        return row * C::kRowBytes + (NG == 1 ? chunk * 16 : (chunk & 1) * 16 + 32 * ((chunk >> 1) ^ (row >> 1 & 1)));
-    };
-    const uint32_t kdst = ring + in_row(crow0), vdst = ring + C::kSide + in_row(value_row(crow0));
-    const uint32_t sdst = ring + 2 * C::kSide + lane * C::kScaleBytes;
-    const uint8_t *const ksrc = P.k4 + chunk * 16, *const vsrc = P.v4 + chunk * 16;
     auto fetch = [&](int stage, const Tile &tile) {
         if (tile.rows >= 0) {
-            const uint32_t at = stage * C::kStage;
-            uint32_t mine[kKeys], have[kKeys];
-            int there = 0;
-#pragma unroll
-            for (int k = 0; k < kKeys; ++k) {
-                const int key = lane + 32 * k;
-                const bool in = key < tile.rows && tile.page[k] >= 0 && tile.page[k] < P.n_pages;
-                have[k] = __ballot_sync(0xffffffffu, in);
-                there += __popc(have[k]);
-                // rows of the cache are counted in 32 bits (the caller's check), bytes in 64; zeros behind the end
-                mine[k] = in ? ((static_cast<uint32_t>(tile.page[k]) * P.Hk + tile.hk) << P.page_shift) +
-                                   ((tile.first + key) & page_mask)
-                             : 0u;
-                const uint16_t *sc = P.scales + static_cast<uint64_t>(mine[k]) * (4 * NG);
-                if constexpr (NG == 1) cp_async8(sdst + at + 32 * k * C::kScaleBytes, sc, in ? 8 : 0);
-                else cp_async16(sdst + at + 32 * k * C::kScaleBytes, sc, in ? 16 : 0);
-            }
-            bad = (bad & ~(1u << stage)) | static_cast<uint32_t>(there < tile.rows) << stage;
-#pragma unroll
-            for (int u = 0; u < kTile / kPer; ++u) {
-                const int k = u * kPer / 32, r = u * kPer % 32 + crow0;
-                const uint64_t from = static_cast<uint64_t>(__shfl_sync(0xffffffffu, mine[k], r)) * C::kRowBytes;
-                const int bytes = have[k] >> r & 1 ? 16 : 0;
-                cp_async16(kdst + at + u * kPer * C::kRowBytes, ksrc + from, bytes);
-                cp_async16(vdst + at + u * kPer * C::kRowBytes, vsrc + from, bytes);
-            }
+            const bool mine = piece_first < min(tile.rows, kTile);
+            const bool in = mine && static_cast<uint32_t>(tile.page) < static_cast<uint32_t>(P.n_pages);
+            bad = (bad & ~(1u << stage)) | static_cast<uint32_t>(mine && !in) << stage;
+            const uint32_t pieces = __popc(__ballot_sync(0xffffffffu, in && kind == 0));
+            uint64_t *bar = &s_full[warp][stage];
+            if (lane == 0) tc::mbar_arrive_expect_tx(bar, pieces * page_rows * (2 * C::kRowBytes + C::kScaleBytes));
+            __syncwarp();
+            // rows of the cache are counted in 32 bits (the caller's check), bytes in 64
+            const uint32_t row = ((static_cast<uint32_t>(tile.page) * P.Hk + tile.hk) << P.page_shift) + (tile.first & page_mask);
+            if (in) bulk_load(dst + stage * C::kStage, src + static_cast<uint64_t>(row) * row_bytes, page_rows * row_bytes, bar);
         }
-        cp_async_commit();
     };
     int head = 0;
-    static_assert(C::kStages == 3);
-    const Tile tile0 = look(warp), tile1 = look(kDecWarps);      // both tables' reads under way together
-    fetch(0, tile0);
-    fetch(1, tile1);
+    uint32_t parity = 0;
+    bool waits = true;      // none has run out
+    Tile ahead[C::kStages];      // the tables' reads under way together
+#pragma unroll
+    for (int e = 0; e < C::kStages; ++e) ahead[e] = look(e == 0 ? warp : kDecWarps);
+#pragma unroll
+    for (int e = 0; e < C::kStages; ++e) fetch(e, ahead[e]);
     Tile tile = look(kDecWarps);
 
-    // The products' side, list by list. Queries: of row r8 (+ 8) and each group the 16
-    // dimensions from 16 c4 on, as the numbers of a thread's two words pair up; those that meet
-    // numbers in the low places are 16 times the others. A thread's scores are of rows 2 c4,
-    // 2 c4 + 1 (+ 8): for these, from products to scores, and the queries' sums in the products' units.
+    // The products' side, list by list. Queries: of row r8 (+ 8, ...) and each group the 16
+    // dimensions from 16 c4 on, as the numbers of a thread's two words pair up. A thread's
+    // scores are of rows 2 c4, 2 c4 + 1 (+ 8, ...): for these, from products to scores, and
+    // the queries' sums in the products' units. (ROWS 1: of the row.)
     uint32_t qb[NG][4][NR][2];
     uint64_t crow[NR], qsum[NG][NR];
     const auto two_rows = [&](float v) {      // of the rows r8 that threads hold, this thread's two
+        if constexpr (ROWS == 1) return tc::f2(v, v);
         return tc::f2(__shfl_sync(0xffffffffu, v, 8 * c4), __shfl_sync(0xffffffffu, v, 8 * c4 + 4));
     };
     auto queries = [&](int seq, int qy) {
         const int row0 = qy % groups * P.per, nr = min(P.per, P.rows - row0), hk = qy / groups;
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-            const int mine = r8 + 8 * r, row = row0 + mine;
+            const int mine = ROWS == 1 ? 0 : r8 + 8 * r, row = row0 + mine;
             uint4 raw[NG][2];
 #pragma unroll
             for (int g = 0; g < NG; ++g)
@@ -393,8 +422,13 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                     }
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        qb[g][2 * w + e][r][0] = pack_f16x2(16.0f * x[2 * e], 16.0f * x[2 * e + 4]);
-                        qb[g][2 * w + e][r][1] = pack_f16x2(x[2 * e + 1], x[2 * e + 5]);
+                        // against numbers in the low places (or bytes), 16 times, and in the high ones
+                        const uint32_t low = pack_f16x2(16.0f * x[2 * e], 16.0f * x[2 * e + 4]);
+                        const uint32_t high = pack_f16x2(x[2 * e + 1], x[2 * e + 5]);
+                        // ROWS 1: an even column has the bytes' and the upper numbers' products, an odd one what
+                        // the bytes' have of the upper numbers
+                        qb[g][2 * w + e][r][0] = ROWS == 1 && (r8 & 1) ? 0u : low;
+                        qb[g][2 * w + e][r][1] = ROWS == 1 && (r8 & 1) ? low : high;
                     }
                 }
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
@@ -417,212 +451,327 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
         for (int r = 0; r < NR; ++r)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int j = (row0 + 8 * r + 2 * c4 + e) / G;
+                const int j = (row0 + (ROWS == 1 ? 0 : 8 * r + 2 * c4 + e)) / G;
                 sees[r][e] = j < fresh.count ? fresh.first + j : INT32_MAX;
             }
         const int all_see = row0 / G < fresh.count ? fresh.first + row0 / G : INT32_MAX;
-        float acc[NG][4][NR][4], m[NR][2];
-        uint64_t l2[NR], z2[NG][NR];
-        int top[NG];        // 2^(top - 127) is above every scale so far
+        // ROWS 1: acc[g][i][0], i < 2: of bytes i and i + 2, sums l2 and z2 of a lane's keys in their low halves
+        float acc[NG][ROWS == 1 ? 2 : 4][NR][4], m[NR][2];
+        uint64_t l2[NR], z2[NG][NR], ref[NR];      // ref: what is added to a score for its weight, -m or 0
+        float far[NR][2];       // a score above moves the references
+        int top[NG];            // 2^(top - 127) is above every scale so far
+        float above[NG], unit[NG];      // that, and the weights' unit
         const uint64_t none2 = tc::f2(0.0f, 0.0f);
 #pragma unroll
-        for (int r = 0; r < NR; ++r) m[r][0] = m[r][1] = -INFINITY, l2[r] = none2;
+        for (int r = 0; r < NR; ++r) m[r][0] = m[r][1] = far[r][0] = far[r][1] = -INFINITY, l2[r] = ref[r] = none2;
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             top[g] = 15;
+            above[g] = pow2(15 - 127);
+            unit[g] = pow2(139 - 15);
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
                 z2[g][r] = none2;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < (ROWS == 1 ? 2 : 4); ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[g][i][r][e] = 0.0f;
             }
         }
+        // every output so far times f (of the row in a column)
+        auto rescale = [&](int g, int r, float f0, float f1) {
+#pragma unroll
+            for (int i = 0; i < (ROWS == 1 ? 2 : 4); ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[g][i][r][e] *= e & 1 ? f1 : f0;
+        };
+        // the values' scales of this lane's keys, `most` their greatest: a finite one above the power of two so far raises it
+        auto raise = [&](int g, float most) {
+            if (__any_sync(0xffffffffu, most >= above[g])) {
+                const int to = static_cast<int>(__reduce_max_sync(0xffffffffu, __float_as_uint(most)) >> 23) + 1;
+                const float f = to - top[g] <= 126 ? pow2(top[g] - to) : 0.0f;
+                top[g] = to;
+                above[g] = to <= 254 ? pow2(to - 127) : INFINITY;
+                unit[g] = pow2(139 - to);
+#pragma unroll
+                for (int r = 0; r < NR; ++r) rescale(g, r, f, f);
+            }
+        };
         for (int i = (warp - taken) & (kDecWarps - 1); i < tiles; i += kDecWarps) {
-            cp_async_wait<C::kStages - 2>();
-            __syncwarp();
-            lost |= bad >> head & 1;
-            const int key0 = (i0 + i) * kTile;
+            if (waits && !wait_phase(&s_full[warp][head], parity)) waits = false;
+            lost |= (bad >> head & 1) || !waits;
+            const int key0 = (i0 + i) * kTile, there = len.n - key0;      // there: keys of the sequence from here on
             const unsigned char *sk = dsm + (warp * C::kStages + head) * C::kStage, *sv = sk + C::kSide, *ss = sv + C::kSide;
-            // Scales and zeros in fp32, once for the warp, each lane its keys'; the values' scales take
-            // the weights' unit along. A finite one above the power of two so far raises that.
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                uint2 raw[kKeys];
-                float most = 0.0f;
-#pragma unroll
-                for (int k = 0; k < kKeys; ++k) {
-                    raw[k] = *reinterpret_cast<const uint2 *>(ss + (lane + 32 * k) * C::kScaleBytes + 8 * g);
-                    most = fmaxf(most, bf_lo(raw[k].y));
-                }
-                if (__any_sync(0xffffffffu, most >= pow2(top[g] - 127))) {
-                    const int to = static_cast<int>(__reduce_max_sync(0xffffffffu, __float_as_uint(most)) >> 23) + 1;
-                    const float f = to - top[g] <= 126 ? pow2(top[g] - to) : 0.0f;
-                    top[g] = to;
-#pragma unroll
-                    for (int i2 = 0; i2 < 4; ++i2)
-#pragma unroll
-                        for (int r = 0; r < NR; ++r)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) acc[g][i2][r][e] *= f;
-                }
-                const float unit = pow2(139 - top[g]);
-#pragma unroll
-                for (int k = 0; k < kKeys; ++k) {
-                    const float ks = bf_lo(raw[k].x), kz = bf_hi(raw[k].x), vs = bf_lo(raw[k].y) * unit, vz = bf_hi(raw[k].y);
-                    s_x[(2 * g) * kTile + lane + 32 * k] = make_ulonglong2(tc::f2(ks, ks), tc::f2(kz, kz));
-                    s_x[(2 * g + 1) * kTile + lane + 32 * k] = make_ulonglong2(tc::f2(vs, vs), tc::f2(vz, vz));
-                }
-            }
-            __syncwarp();
-            // scores of keys 16 mt + 8 h + r8, both rows of a pair in one register pair
-            uint64_t t[NM][2][NR];
-#pragma unroll
-            for (int g = 0; g < NG; ++g)
-#pragma unroll
-                for (int mt = 0; mt < NM; ++mt) {
-                    uint32_t w[2][2];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int row = 16 * mt + 8 * h + r8;
-                        const uint2 x = *reinterpret_cast<const uint2 *>(sk + row * C::kRowBytes + 8 * c4 +
-                                                                         (NG == 1 ? 0 : 32 * (g ^ (r8 >> 1 & 1))));
-                        w[h][0] = x.x, w[h][1] = x.y;
-                    }
-                    float d[NR][4] = {};
-#pragma unroll
-                    for (int s = 0; s < 4; ++s) {
-                        const uint32_t x = s & 1 ? w[0][s >> 1] >> 8 : w[0][s >> 1];
-                        const uint32_t x2 = s & 1 ? w[1][s >> 1] >> 8 : w[1][s >> 1];
-#pragma unroll
-                        for (int r = 0; r < NR; ++r)
-                            mma_f16(d[r], x & kEven, x2 & kEven, x & kOdd, x2 & kOdd, qb[g][s][r][0], qb[g][s][r][1]);
-                    }
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const ulonglong2 sz = s_x[(2 * g) * kTile + 16 * mt + 8 * h + r8];
-#pragma unroll
-                        for (int r = 0; r < NR; ++r) {
-                            const uint64_t zero = g == 0 ? tc::mul2(sz.y, qsum[g][r]) : tc::fma2(sz.y, qsum[g][r], t[mt][h][r]);
-                            t[mt][h][r] = tc::fma2(sz.x, tc::f2(d[r][2 * h], d[r][2 * h + 1]), zero);
-                        }
-                    }
-                }
             const bool masked = key0 + kTile > all_see;
-            if (masked) {
+            if constexpr (ROWS == 1) {
+                // scores: this lane's are of keys 8 c4 + r8 (+ 32), one of each four blocks
+                float t[kKeys];
+                uint2 raw[NG][kKeys];
 #pragma unroll
-                for (int mt = 0; mt < NM; ++mt)
+                for (int k = 0; k < kKeys; ++k) t[k] = 0.0f;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int key = key0 + 16 * mt + 8 * h + r8;
+                for (int g = 0; g < NG; ++g) {
+                    float most = 0.0f;
 #pragma unroll
-                        for (int r = 0; r < NR; ++r) {
-                            const float2 x = tc::f2_split(t[mt][h][r]);
-                            t[mt][h][r] = tc::f2(key < sees[r][0] ? x.x : -INFINITY, key < sees[r][1] ? x.y : -INFINITY);
+                    for (int k = 0; k < kKeys; ++k) {
+                        const int key = 32 * k + 8 * c4 + r8;
+                        raw[g][k] = *reinterpret_cast<const uint2 *>(ss + key * C::kScaleBytes + 8 * g);
+                        if (key < there) most = fmaxf(most, bf_lo(raw[g][k].y));
+                    }
+                    raise(g, most);
+                    float d[NM][4];
+#pragma unroll
+                    for (int mt = 0; mt < NM; ++mt) {
+                        uint32_t w[2][2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint2 x = *reinterpret_cast<const uint2 *>(sk + (16 * mt + 8 * h + r8) * C::kRowBytes + 32 * g + 8 * c4);
+                            w[h][0] = x.x, w[h][1] = x.y;
+                        }
+#pragma unroll
+                        for (int s = 0; s < 4; ++s) {
+                            const uint32_t x = bytes_of(w[0][s >> 1], s & 1), x2 = bytes_of(w[1][s >> 1], s & 1);
+                            if (s == 0) mma_f16_first(d[mt], x, x2, x & kOdd, x2 & kOdd, qb[g][s][0][0], qb[g][s][0][1]);
+                            else mma_f16(d[mt], x, x2, x & kOdd, x2 & kOdd, qb[g][s][0][0], qb[g][s][0][1]);
                         }
                     }
-            }
-            // the greatest score that this thread has of each row (NaN left out); the references move if one is far above
-            float mx[NR][2];
-            bool grown = false;
+                    const float q = tc::f2_split(qsum[g][0]).x;
 #pragma unroll
-            for (int r = 0; r < NR; ++r) {
-                float2 x = tc::f2_split(t[0][0][r]);
-                mx[r][0] = x.x, mx[r][1] = x.y;
+                    for (int k = 0; k < kKeys; ++k) {
+                        float x[4];
 #pragma unroll
-                for (int k = 1; k < 2 * NM; k += 2) {
-                    x = tc::f2_split(t[k >> 1][k & 1][r]);
-                    const float2 x2 = k + 1 < 2 * NM ? tc::f2_split(t[(k + 1) >> 1][(k + 1) & 1][r]) : x;
-                    mx[r][0] = tc::fmax3(mx[r][0], x.x, x2.x);
-                    mx[r][1] = tc::fmax3(mx[r][1], x.y, x2.y);
-                }
-                const float2 c = tc::f2_split(crow[r]);
-                mx[r][0] *= c.x, mx[r][1] *= c.y;
-                grown |= mx[r][0] > m[r][0] + kSlack || mx[r][1] > m[r][1] + kSlack;
-            }
-            if (__any_sync(0xffffffffu, grown)) {
-#pragma unroll
-                for (int r = 0; r < NR; ++r) {
-                    float f[2];
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float x = fmaxf(mx[r][e], m[r][e]);      // not NaN
-#pragma unroll
-                        for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-                        f[e] = x > m[r][e] ? tc::ex2(m[r][e] - x) : 1.0f;
-                        m[r][e] = x;
+                        for (int e = 0; e < 4; ++e) x[e] = d[2 * k + (e >> 1)][2 * (e & 1)] - d[2 * k + (e >> 1)][2 * (e & 1) + 1];
+                        const float dot = c4 & 2 ? (c4 & 1 ? x[3] : x[2]) : (c4 & 1 ? x[1] : x[0]);
+                        t[k] = fmaf(bf_lo(raw[g][k].x), dot, fmaf(bf_hi(raw[g][k].x), q, t[k]));
                     }
-                    const uint64_t f2 = tc::f2(f[0], f[1]);
-                    l2[r] = tc::mul2(l2[r], f2);
+                }
+                float mx = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < kKeys; ++k) {
+                    if (masked && key0 + 32 * k + 8 * c4 + r8 >= sees[0][0]) t[k] = -INFINITY;
+                    mx = fmaxf(mx, t[k]);
+                }
+                const float c = tc::f2_split(crow[0]).x;
+                if (__any_sync(0xffffffffu, mx * c > far[0][0])) {
+                    float x = fmaxf(mx * c, m[0][0]);      // not NaN
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+                    const float f = x > m[0][0] ? tc::ex2(m[0][0] - x) : 1.0f;
+                    const uint64_t f2 = tc::f2(f, f);
+                    m[0][0] = x;
+                    far[0][0] = x + kSlack;
+                    ref[0] = tc::f2(x == -INFINITY ? 0.0f : -x, 0.0f);
+                    l2[0] = tc::mul2(l2[0], f2);
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
-                        z2[g][r] = tc::mul2(z2[g][r], f2);
-#pragma unroll
-                        for (int i2 = 0; i2 < 4; ++i2)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) acc[g][i2][r][e] *= f[e & 1];
+                        z2[g][0] = tc::mul2(z2[g][0], f2);
+                        rescale(g, 0, f, f);
                     }
                 }
-            }
-            uint32_t pw[NG][NM][2][NR];
-            auto weigh = [&](auto some_hidden) {
+                // weights to the lanes that multiply them: key t at (t mod 4, t / 4), once in the low half and once in the high one
 #pragma unroll
-                for (int r = 0; r < NR; ++r) {
-                    const uint64_t ref = tc::f2(m[r][0] == -INFINITY ? 0.0f : -m[r][0], m[r][1] == -INFINITY ? 0.0f : -m[r][1]);
+                for (int k = 0; k < kKeys; ++k) {
+                    const int key = 32 * k + 8 * c4 + r8;
+                    const bool hidden = masked && key0 + key >= sees[0][0];
+                    const float p = tc::ex2(fmaf(t[k], c, tc::f2_split(ref[0]).x));
+                    l2[0] = tc::f2(tc::f2_split(l2[0]).x + p, 0.0f);
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        // what the row does not see does not reach it: NaN scales neither
+                        const float w = hidden ? 0.0f : p * (bf_lo(raw[g][k].y) * unit[g]), zero = hidden ? 0.0f : bf_hi(raw[g][k].y);
+                        z2[g][0] = tc::f2(fmaf(p, zero, tc::f2_split(z2[g][0]).x), 0.0f);
+                        const uint32_t half = pack_f16x2(w, 0.0f);
+                        uint32_t *to = s_w + 8 * C::kStride * g + (key & 3) * C::kStride + (key >> 2);
+                        to[0] = half;
+                        to[4 * C::kStride] = half << 16;
+                    }
+                }
+                __syncwarp();
+                // outputs: words r8 of keys 4 j + c4; an even column has their low halves' products, an odd one the high ones'
+#pragma unroll
+                for (int g = 0; g < NG; ++g)
+#pragma unroll
+                    for (int j = 0; j < kTile / 4; j += 4) {
+                        const uint4 w = *reinterpret_cast<const uint4 *>(s_w + 8 * C::kStride * g + (4 * (r8 & 1) + c4) * C::kStride + j);
+                        const uint32_t pw[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                        for (int u = 0; u < 4; u += 2) {
+                            const unsigned char *at = sv + (4 * (j + u) + c4) * C::kRowBytes + 32 * g + 4 * r8;
+                            const uint32_t x0 = *reinterpret_cast<const uint32_t *>(at);
+                            const uint32_t x1 = *reinterpret_cast<const uint32_t *>(at + 4 * C::kRowBytes);
+#pragma unroll
+                            for (int s = 0; s < 2; ++s) {
+                                const uint32_t x = bytes_of(x0, s), x2 = bytes_of(x1, s);
+                                mma_f16(acc[g][s][0], x, x & kOdd, x2, x2 & kOdd, pw[u], pw[u + 1]);
+                            }
+                        }
+                    }
+            } else {
+                // [group][key's, value's][key]: scale, scale, zero, zero in fp32, once for the warp, each
+                // lane its keys'; the values' scales take the weights' unit along
+                ulonglong2 *s_x = reinterpret_cast<ulonglong2 *>(s_w);
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    uint2 raw[kKeys];
+                    float most = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < kKeys; ++k) {
+                        raw[k] = *reinterpret_cast<const uint2 *>(ss + (lane + 32 * k) * C::kScaleBytes + 8 * g);
+                        if (lane + 32 * k < there) most = fmaxf(most, bf_lo(raw[k].y));
+                    }
+                    raise(g, most);
+#pragma unroll
+                    for (int k = 0; k < kKeys; ++k) {
+                        const float ks = bf_lo(raw[k].x), kz = bf_hi(raw[k].x), vs = bf_lo(raw[k].y) * unit[g], vz = bf_hi(raw[k].y);
+                        s_x[(2 * g) * kTile + lane + 32 * k] = make_ulonglong2(tc::f2(ks, ks), tc::f2(kz, kz));
+                        s_x[(2 * g + 1) * kTile + lane + 32 * k] = make_ulonglong2(tc::f2(vs, vs), tc::f2(vz, vz));
+                    }
+                }
+                __syncwarp();
+                // scores of keys 16 mt + 8 h + key_of(r8), both rows of a pair in one register pair
+                const int mine = key_of(r8);
+                uint64_t t[NM][2][NR];
+#pragma unroll
+                for (int g = 0; g < NG; ++g)
+#pragma unroll
+                    for (int mt = 0; mt < NM; ++mt) {
+                        uint32_t w[2][2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint2 x = *reinterpret_cast<const uint2 *>(sk + (16 * mt + 8 * h + mine) * C::kRowBytes + 32 * g + 8 * c4);
+                            w[h][0] = x.x, w[h][1] = x.y;
+                        }
+                        float d[NR][4];
+#pragma unroll
+                        for (int s = 0; s < 4; ++s) {
+                            const uint32_t x = s & 1 ? w[0][s >> 1] >> 8 : w[0][s >> 1];
+                            const uint32_t x2 = s & 1 ? w[1][s >> 1] >> 8 : w[1][s >> 1];
+#pragma unroll
+                            for (int r = 0; r < NR; ++r) {
+                                if (s == 0) mma_f16_first(d[r], x & kEven, x2 & kEven, x & kOdd, x2 & kOdd, qb[g][s][r][0], qb[g][s][r][1]);
+                                else mma_f16(d[r], x & kEven, x2 & kEven, x & kOdd, x2 & kOdd, qb[g][s][r][0], qb[g][s][r][1]);
+                            }
+                        }
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const ulonglong2 sz = s_x[(2 * g) * kTile + 16 * mt + 8 * h + mine];
+#pragma unroll
+                            for (int r = 0; r < NR; ++r) {
+                                const uint64_t zero = g == 0 ? tc::mul2(sz.y, qsum[g][r]) : tc::fma2(sz.y, qsum[g][r], t[mt][h][r]);
+                                t[mt][h][r] = tc::fma2(sz.x, tc::f2(d[r][2 * h], d[r][2 * h + 1]), zero);
+                            }
+                        }
+                    }
+                if (masked) {
 #pragma unroll
                     for (int mt = 0; mt < NM; ++mt)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const uint64_t p2 = tc::ex2_pair(tc::fma2(t[mt][h][r], crow[r], ref));
-                            l2[r] = tc::add2(l2[r], p2);
-                            const int key = 16 * mt + 8 * h + r8;
+                            const int key = key0 + 16 * mt + 8 * h + mine;
 #pragma unroll
-                            for (int g = 0; g < NG; ++g) {
-                                ulonglong2 sz = s_x[(2 * g + 1) * kTile + key];
-                                if constexpr (some_hidden.value) {
-                                    // what a row does not see does not reach it: NaN scales neither
-                                    const bool s0 = key0 + key < sees[r][0], s1 = key0 + key < sees[r][1];
-                                    const float a = tc::f2_split(sz.x).x, c = tc::f2_split(sz.y).x;
-                                    sz.x = tc::f2(s0 ? a : 0.0f, s1 ? a : 0.0f);
-                                    sz.y = tc::f2(s0 ? c : 0.0f, s1 ? c : 0.0f);
-                                }
-                                z2[g][r] = tc::fma2(p2, sz.y, z2[g][r]);
-                                const float2 w = tc::f2_split(tc::mul2(p2, sz.x));
-                                pw[g][mt][h][r] = transpose8(pack_f16x2(w.x, w.y));
+                            for (int r = 0; r < NR; ++r) {
+                                const float2 x = tc::f2_split(t[mt][h][r]);
+                                t[mt][h][r] = tc::f2(key < sees[r][0] ? x.x : -INFINITY, key < sees[r][1] ? x.y : -INFINITY);
                             }
                         }
                 }
-            };
-            if (masked) weigh(std::true_type{});
-            else weigh(std::false_type{});
+                // the greatest score that this thread has of each row (NaN left out); the references move if one is far above
+                float mx[NR][2];
+                bool grown = false;
 #pragma unroll
-            for (int g = 0; g < NG; ++g)
+                for (int r = 0; r < NR; ++r) {
+                    float2 x = tc::f2_split(t[0][0][r]);
+                    mx[r][0] = x.x, mx[r][1] = x.y;
 #pragma unroll
-                for (int mt = 0; mt < NM; ++mt) {
-                    uint32_t w[2][2];      // numbers 0 .. 3 and 4 .. 7 of keys 2 c4 and 2 c4 + 1 (+ 8)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const unsigned char *src = sv + (16 * mt + 8 * h + c4) * C::kRowBytes + 4 * r8 +
-                                                   (NG == 1 ? 0 : 32 * (g ^ (c4 >> 1)));
-                        const uint32_t x0 = *reinterpret_cast<const uint32_t *>(src);
-                        const uint32_t x1 = *reinterpret_cast<const uint32_t *>(src + 4 * C::kRowBytes);
-                        w[h][0] = __byte_perm(x0, x1, 0x5410);
-                        w[h][1] = __byte_perm(x0, x1, 0x7632);
+                    for (int k = 1; k < 2 * NM; k += 2) {
+                        x = tc::f2_split(t[k >> 1][k & 1][r]);
+                        const float2 x2 = k + 1 < 2 * NM ? tc::f2_split(t[(k + 1) >> 1][(k + 1) & 1][r]) : x;
+                        mx[r][0] = tc::fmax3(mx[r][0], x.x, x2.x);
+                        mx[r][1] = tc::fmax3(mx[r][1], x.y, x2.y);
                     }
+                    const float2 c = tc::f2_split(crow[r]);
+                    mx[r][0] *= c.x, mx[r][1] *= c.y;
+                    grown |= mx[r][0] > far[r][0] || mx[r][1] > far[r][1];
+                }
+                if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
-                    for (int i2 = 0; i2 < 4; ++i2) {
-                        const uint32_t x = i2 & 1 ? w[0][i2 >> 1] >> 8 : w[0][i2 >> 1];
-                        const uint32_t x2 = i2 & 1 ? w[1][i2 >> 1] >> 8 : w[1][i2 >> 1];
+                    for (int r = 0; r < NR; ++r) {
+                        float f[2];
 #pragma unroll
-                        for (int r = 0; r < NR; ++r)
-                            mma_f16(acc[g][i2][r], x & kEven, x & kOdd, x2 & kEven, x2 & kOdd, pw[g][mt][0][r], pw[g][mt][1][r]);
+                        for (int e = 0; e < 2; ++e) {
+                            float x = fmaxf(mx[r][e], m[r][e]);      // not NaN
+#pragma unroll
+                            for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+                            f[e] = x > m[r][e] ? tc::ex2(m[r][e] - x) : 1.0f;
+                            m[r][e] = x;
+                            far[r][e] = x + kSlack;
+                        }
+                        ref[r] = tc::f2(m[r][0] == -INFINITY ? 0.0f : -m[r][0], m[r][1] == -INFINITY ? 0.0f : -m[r][1]);
+                        const uint64_t f2 = tc::f2(f[0], f[1]);
+                        l2[r] = tc::mul2(l2[r], f2);
+#pragma unroll
+                        for (int g = 0; g < NG; ++g) {
+                            z2[g][r] = tc::mul2(z2[g][r], f2);
+                            rescale(g, r, f[0], f[1]);
+                        }
                     }
                 }
-            __syncwarp();      // the stage that the next copy overwrites has been read
-            fetch(head == 0 ? C::kStages - 1 : head - 1, tile);
+                uint32_t pw[NG][NM][2][NR];
+                auto weigh = [&](auto some_hidden) {
+#pragma unroll
+                    for (int r = 0; r < NR; ++r)
+#pragma unroll
+                        for (int mt = 0; mt < NM; ++mt)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const uint64_t p2 = tc::ex2_pair(tc::fma2(t[mt][h][r], crow[r], ref[r]));
+                                l2[r] = tc::add2(l2[r], p2);
+                                const int key = 16 * mt + 8 * h + mine;
+#pragma unroll
+                                for (int g = 0; g < NG; ++g) {
+                                    ulonglong2 sz = s_x[(2 * g + 1) * kTile + key];
+                                    if constexpr (some_hidden.value) {
+                                        // what a row does not see does not reach it: NaN scales neither
+                                        const bool s0 = key0 + key < sees[r][0], s1 = key0 + key < sees[r][1];
+                                        const float a = tc::f2_split(sz.x).x, c = tc::f2_split(sz.y).x;
+                                        sz.x = tc::f2(s0 ? a : 0.0f, s1 ? a : 0.0f);
+                                        sz.y = tc::f2(s0 ? c : 0.0f, s1 ? c : 0.0f);
+                                    }
+                                    z2[g][r] = tc::fma2(p2, sz.y, z2[g][r]);
+                                    const float2 w = tc::f2_split(tc::mul2(p2, sz.x));
+                                    pw[g][mt][h][r] = transpose8(pack_f16x2(w.x, w.y));
+                                }
+                            }
+                };
+                if (masked) weigh(std::true_type{});
+                else weigh(std::false_type{});
+                const int even_row = key_of(2 * c4), odd_row = key_of(2 * c4 + 1);
+#pragma unroll
+                for (int g = 0; g < NG; ++g)
+#pragma unroll
+                    for (int mt = 0; mt < NM; ++mt) {
+                        uint32_t w[2][2];      // bytes 0, 1 and 2, 3 of the keys in rows 2 c4 and 2 c4 + 1 (+ 8)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const unsigned char *at = sv + (16 * mt + 8 * h) * C::kRowBytes + 32 * g + 4 * r8;
+                            const uint32_t x0 = *reinterpret_cast<const uint32_t *>(at + even_row * C::kRowBytes);
+                            const uint32_t x1 = *reinterpret_cast<const uint32_t *>(at + odd_row * C::kRowBytes);
+                            w[h][0] = __byte_perm(x0, x1, 0x5410);
+                            w[h][1] = __byte_perm(x0, x1, 0x7632);
+                        }
+#pragma unroll
+                        for (int i2 = 0; i2 < 4; ++i2) {
+                            const uint32_t x = bytes_of(w[0][i2 >> 1], i2 & 1), x2 = bytes_of(w[1][i2 >> 1], i2 & 1);
+#pragma unroll
+                            for (int r = 0; r < NR; ++r)
+                                mma_f16(acc[g][i2][r], x, x & kOdd, x2, x2 & kOdd, pw[g][mt][0][r], pw[g][mt][1][r]);
+                        }
+                    }
+            }
+            __syncwarp();      // the stage, and the words between the lanes, have been read
+            fetch(head, tile);
             tile = look(kDecWarps);
-            head = head + 1 == C::kStages ? 0 : head + 1;
+            if (++head == C::kStages) head = 0, parity ^= 1;
         }
 
         // the next list, and its queries on their way
@@ -636,11 +785,11 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
             if (nb != b) blen = P.seq_lens[nb];
         }
 
-        // join the warps: their maxima and sums, then the outputs of eight rows at a time
+        // join the warps: their references and sums, then the outputs of some rows at a time
         const auto whole_rows = [](uint64_t v2) {
             float2 v = tc::f2_split(v2);
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) {
+            for (int o = ROWS == 1 ? 1 : 4; o < 32; o <<= 1) {
                 v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
                 v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
             }
@@ -665,39 +814,57 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
             if (8 * r >= nr) break;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int row = 8 * r + 2 * c4 + e;
+            const auto reference = [&](int row) {
                 float M = s_m[0][row];
 #pragma unroll
                 for (int w = 1; w < kDecWarps; ++w) M = fmaxf(M, s_m[w][row]);
-                const float f = s_m[warp][row] == -INFINITY ? 0.0f : tc::ex2(s_m[warp][row] - M);
+                return M;
+            };
+            // the bytes' units and the weights' taken out: even dimensions are what the bytes' sums have beyond the odd ones'
+            if constexpr (ROWS == 1) {
+                const float f = s_m[warp][0] == -INFINITY ? 0.0f : tc::ex2(s_m[warp][0] - reference(0));
+                if (c4 == 0) {
 #pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    // the numbers' 2^-24 or 2^-20 and the weights' unit taken out
-                    const float u = pow2(min(top[g] - 127, 127)) * f;
-                    float *dst = s_o + (warp * 8 + 2 * c4 + e) * HD + 64 * g + 8 * r8;
+                    for (int g = 0; g < NG; ++g) {
+                        const float u = pow2(min(top[g] - 127, 127)) * f;
+                        float4 *dst = reinterpret_cast<float4 *>(s_o + warp * HD + 64 * g + 8 * r8);
 #pragma unroll
-                    for (int i2 = 0; i2 < 4; i2 += 2)
-                        *reinterpret_cast<float4 *>(dst + 2 * i2) =
-                            make_float4(acc[g][i2][r][e] * 4096.0f * u, acc[g][i2][r][2 + e] * 256.0f * u,
-                                        acc[g][i2 + 1][r][e] * 4096.0f * u, acc[g][i2 + 1][r][2 + e] * 256.0f * u);
+                        for (int h = 0; h < 2; ++h)
+                            dst[h] = make_float4((acc[g][0][0][h] - acc[g][0][0][2 + h]) * 4096.0f * u, acc[g][0][0][2 + h] * 256.0f * u,
+                                                 (acc[g][1][0][h] - acc[g][1][0][2 + h]) * 4096.0f * u, acc[g][1][0][2 + h] * 256.0f * u);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int row = 8 * r + 2 * c4 + e;
+                    const float f = s_m[warp][row] == -INFINITY ? 0.0f : tc::ex2(s_m[warp][row] - reference(row));
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        const float u = pow2(min(top[g] - 127, 127)) * f;
+                        float *dst = s_o + (warp * 8 + 2 * c4 + e) * HD + 64 * g + 8 * r8;
+#pragma unroll
+                        for (int i2 = 0; i2 < 4; i2 += 2)
+                            *reinterpret_cast<float4 *>(dst + 2 * i2) =
+                                make_float4((acc[g][i2][r][e] - acc[g][i2][r][2 + e]) * 4096.0f * u, acc[g][i2][r][2 + e] * 256.0f * u,
+                                            (acc[g][i2 + 1][r][e] - acc[g][i2 + 1][r][2 + e]) * 4096.0f * u,
+                                            acc[g][i2 + 1][r][2 + e] * 256.0f * u);
+                    }
                 }
             }
             __syncthreads();
             const int left = min(nr - 8 * r, 8) * (HD / 4);
             for (int e = threadIdx.x; e < left; e += blockDim.x) {
                 const int in8 = e / (HD / 4), row = 8 * r + in8, d = e % (HD / 4) * 4;
-                float M = s_m[0][row], L = 0.0f;
-#pragma unroll
-                for (int w = 1; w < kDecWarps; ++w) M = fmaxf(M, s_m[w][row]);
+                const float M = reference(row);
+                float L = 0.0f;
                 float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                 for (int w = 0; w < kDecWarps; ++w) {
-                    // a warp whose maximum is -inf saw nothing, or NaN alone
+                    // a warp without a reference saw nothing, or NaN alone
                     const float f = s_m[w][row] == -INFINITY ? 1.0f : tc::ex2(s_m[w][row] - M);
                     L += s_l[w][row] * f;
-                    const float4 x = *reinterpret_cast<const float4 *>(s_o + (w * 8 + in8) * HD + d);
+                    const float4 x = *reinterpret_cast<const float4 *>(s_o + (w * C::kPass + in8) * HD + d);
                     const float zero = s_z[w][d / 64][row] * f;
                     o.x += x.x + zero, o.y += x.y + zero, o.z += x.z + zero, o.w += x.w + zero;
                 }
@@ -797,18 +964,25 @@ cudaError_t launch_rope_append_int4(const void *qkv, int64_t ld, const float *co
     return cudaGetLastError();
 }
 
-// Rows of a key head that one list takes: all up to 16, else shared out evenly.
+// Rows of a key head that one list takes: all up to kMostRows (one pass over the keys), else shared out evenly.
 static int list_rows(int64_t rows) {
-    const int64_t groups = (rows + kDecHeads - 1) / kDecHeads;
+    const int64_t groups = (rows + kMostRows - 1) / kMostRows;
     return static_cast<int>((rows + groups - 1) / groups);
 }
 
-DecodeSplit decode_int4_split(int64_t B, int64_t rows, int64_t Hk, int64_t hd, int64_t max_len) {
+// f with the kernel's head_dim and rows: those that a list of `per` rows takes.
+template <typename F>
+static auto with_form(int64_t hd, int per, F f) {
+    if (hd == 64)
+        return per == 1 ? f(Dec4<64, 1>{}) : per <= 8 ? f(Dec4<64, 8>{}) : per <= 16 ? f(Dec4<64, 16>{}) : f(Dec4<64, 24>{});
+    return per == 1 ? f(Dec4<128, 1>{}) : per <= 8 ? f(Dec4<128, 8>{}) : per <= 16 ? f(Dec4<128, 16>{}) : f(Dec4<128, 24>{});
+}
+
+static DecodeSplit decode_int4_split(int64_t B, int64_t rows, int64_t Hk, int64_t hd, int64_t max_len) {
     DecodeSplit s;
-    const int per = list_rows(rows), tile = hd == 64 ? Dec4<64, 8>::kTile : Dec4<128, 8>::kTile;
-    const int64_t lists = B * Hk * ((rows + per - 1) / per);
-    const int ctas = hd == 64 ? (per <= 8 ? Dec4<64, 8>::kCtas : Dec4<64, 16>::kCtas)
-                              : (per <= 8 ? Dec4<128, 8>::kCtas : Dec4<128, 16>::kCtas);
+    const int per = list_rows(rows);
+    const int64_t lists = B * Hk * ((rows + per - 1) / per), tile = 4096 / hd;
+    const int ctas = with_form(hd, per, [](auto form) { return decltype(form)::kCtas; });
     const int64_t resident = static_cast<int64_t>(device_sm_count()) * ctas;
     // few short lists: as one cluster each, of up to 8 chunks of up to 1024 keys
     const int64_t most = std::min<int64_t>(kClusterMost, resident / std::max<int64_t>(lists, 1));
@@ -824,12 +998,18 @@ DecodeSplit decode_int4_split(int64_t B, int64_t rows, int64_t Hk, int64_t hd, i
     return s;
 }
 
+// A call's parts; where the lists are cut comes behind them.
+static size_t part_floats(const DecodeSplit &s, int per, int64_t hd) {
+    return static_cast<size_t>(s.ctas + s.lists) * per * (hd + 4);
+}
+
 size_t decode_int4_bytes(int64_t B, int64_t rows, int64_t Hk, int64_t hd, int64_t max_len) {
-    return decode_int4_split(B, rows, Hk, hd, max_len).bytes(list_rows(rows), 1, hd);
+    const DecodeSplit s = decode_int4_split(B, rows, Hk, hd, max_len);
+    return s.cluster ? 0 : part_floats(s, list_rows(rows), hd) * sizeof(float) + static_cast<size_t>(std::min(s.ctas, s.lists)) * 8;
 }
 
 template <int HD, int ROWS>
-static cudaError_t launch_decode(const Decode4Args &p, const DecodeSplit &s, dim3 grid, cudaStream_t st) {
+static cudaError_t launch_decode(Dec4<HD, ROWS>, const Decode4Args &p, const DecodeSplit &s, dim3 grid, cudaStream_t st) {
     constexpr int smem = Dec4<HD, ROWS>::kSmem;
     static std::atomic<uint64_t> ready{0};      // devices whose kernels have their shared memory set
     int dev = 0;
@@ -912,9 +1092,8 @@ cudaError_t launch_decode_attn_int4(const void *q, int64_t q_ld, const void *kp,
     p.part = part;
     // the parts, then the CTAs' cut lists
     p.by_list = s.lists <= s.ctas;
-    p.cut = s.cluster ? nullptr : reinterpret_cast<int2 *>(part + s.part_floats(per, 1, hd));
-    if (hd == 64) return per <= 8 ? launch_decode<64, 8>(p, s, grid, st) : launch_decode<64, 16>(p, s, grid, st);
-    return per <= 8 ? launch_decode<128, 8>(p, s, grid, st) : launch_decode<128, 16>(p, s, grid, st);
+    p.cut = s.cluster ? nullptr : reinterpret_cast<int2 *>(part + part_floats(s, per, hd));
+    return with_form(hd, per, [&](auto form) { return launch_decode(form, p, s, grid, st); });
 }
 
 }  // namespace mom
