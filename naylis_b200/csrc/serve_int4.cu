@@ -152,10 +152,12 @@ rope_append_int4_kernel(const uint16_t *__restrict__ qkv, int64_t ld, const floa
 //
 // Both products have the numbers as their first operand: scores are keys by rows (heads, new
 // tokens), outputs dimensions by rows, so that 8 rows cost half of what 16 do; the weights
-// turn from the one layout to the other by movmatrix. One row alone (a head of keys for
-// each of queries, one new token) has a form of its own: the columns that other rows would
-// have take the parts of a byte and of a word apart, and the softmax is shared out over all
-// lanes. The queries of a row are scaled by a power of two to 2^9 .. 2^10 at most, so that fp16
+// turn from the one layout to the other by movmatrix. Up to 4 rows have two columns each,
+// which take the parts of a byte and of a word apart: neither masks nor pairs of keys to
+// make. One row alone (a head of keys for each of queries, one new token) has its softmax
+// shared out over all lanes. More than 8 rows are lists of their own, which read the keys
+// again (from L2: 24 sequences of 1024 to 8191, 20 rows on each of 4 heads of 128: 52 us; up to 16
+// or 24 rows a list, whose sums leave room for 2 CTAs an SM: 56 and 59). The queries of a row are scaled by a power of two to 2^9 .. 2^10 at most, so that fp16
 // holds all their bits. The weights p_t s_t are fp16, scaled by a power of two above every
 // scale so far: 11 bits, a quarter of the output's own rounding; those below 2^-36 of the
 // largest lose bits. p is taken against a reference within 2^3 of the greatest so far, which
@@ -169,34 +171,25 @@ rope_append_int4_kernel(const uint16_t *__restrict__ qkv, int64_t ld, const floa
 constexpr float kSlack = 3.0f;      // log2
 constexpr int kLeast = 4;           // tiles of a CTA's span, at least
 constexpr int kListCost = 3;        // tiles that a list's start and end cost
-constexpr int kMostRows = 24;       // of a list
+constexpr int kMostRows = 8;        // of a list
 
-#ifndef S1
-#define S1 2
-#define C1 4
-#define S8 3
-#define C8 3
-#define S16 2
-#define C16 2
-#endif
 template <int HD, int ROWS>
 struct Dec4 {
-    static constexpr int kStages = ROWS == 1 ? S1 : ROWS == 8 ? S8 : S16;
-    static constexpr int kCtas = ROWS == 1 ? C1 : ROWS == 8 ? C8 : C16;                   // resident on an SM
+    static constexpr int kStages = ROWS == 1 ? 2 : 3;
+    static constexpr int kCtas = ROWS == 1 ? 4 : 3;   // resident on an SM
     static constexpr int kTile = 4096 / HD;           // keys of a warp's step
     static constexpr int kGroups = HD / 64, kRowBytes = HD / 2, kScaleBytes = 8 * kGroups;
     static constexpr int kSide = kTile * kRowBytes;
     static constexpr int kStage = 2 * kSide + kTile * kScaleBytes;
     static constexpr int kRing = kDecWarps * kStages * kStage;
-    static constexpr int kPass = ROWS == 1 ? 1 : 8;   // rows that are joined at a time
     // a warp's words between its lanes: the weights of a tile, in the low and in the high half
-    // (ROWS 1), or its scales and zeros in fp32, twice each
+    // (1 row), or its scales and zeros in fp32, twice each (8)
     static constexpr int kStride = kTile / 4 + 4;
-    static constexpr int kWords = ROWS == 1 ? 8 * kStride * kGroups : kTile * 8 * kGroups;
+    static constexpr int kWords = ROWS == 1 ? 8 * kStride * kGroups : ROWS == 8 ? kTile * 8 * kGroups : 0;
     // that, and at a list's end the warps' outputs
-    static constexpr int kSmem = kRing + std::max(kDecWarps * kWords * 4, kDecWarps * kPass * HD * 4);
+    static constexpr int kSmem = kRing + std::max(kDecWarps * kWords * 4, kDecWarps * ROWS * HD * 4);
     // a grid of kCtas an SM is resident at once: an SM's shared memory, 1 KB and the static part a CTA
-    static_assert(kCtas * (kSmem + 1024 + kDecWarps * (kStages + 2 * (ROWS + 7)) * 8 + kDecWarps * kGroups * (ROWS + 7) * 4) <= 228 * 1024);
+    static_assert(kCtas * (kSmem + 1024 + kDecWarps * (kStages * 8 + (2 + kGroups) * 8 * 4) + 512) <= 228 * 1024);
 };
 
 struct Decode4Args : DecodeArgs {
@@ -260,11 +253,12 @@ template <int HD, int ROWS, bool Cluster>
 __global__ void __launch_bounds__(kDecWarps * 32, Dec4<HD, ROWS>::kCtas)
 decode_int4_kernel(const __grid_constant__ Decode4Args P) {
     using C = Dec4<HD, ROWS>;
-    constexpr int NG = C::kGroups, NR = (ROWS + 7) / 8, kTile = C::kTile, kKeys = kTile / 32, NM = kTile / 16;
+    constexpr int NG = C::kGroups, kTile = C::kTile, kKeys = kTile / 32, NB = kTile / 8;      // NB: score blocks, of 8 keys
+    constexpr int NA = ROWS == 8 ? 4 : 2;       // output tiles of a group: pairs of numbers of a word, or its bytes 0, 2 and 1, 3
     extern __shared__ __align__(128) unsigned char dsm[];
     __shared__ uint64_t s_full[kDecWarps][C::kStages];
-    __shared__ __align__(16) float s_m[kDecWarps][8 * NR], s_l[kDecWarps][8 * NR], s_z[kDecWarps][NG][8 * NR];
-    __shared__ float2 s_part[8 * NR];
+    __shared__ __align__(16) float s_m[kDecWarps][8], s_l[kDecWarps][8], s_z[kDecWarps][NG][8];
+    __shared__ float2 s_part[8];
     float *s_o = reinterpret_cast<float *>(dsm + C::kRing);
     const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) >> 5, 0);
     const int lane = threadIdx.x & 31, c4 = lane & 3, r8 = lane >> 2;
@@ -364,77 +358,75 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
     for (int e = 0; e < C::kStages; ++e) fetch(e, ahead[e]);
     Tile tile = look(kDecWarps);
 
-    // The products' side, list by list. Queries: of row r8 (+ 8, ...) and each group the 16
-    // dimensions from 16 c4 on, as the numbers of a thread's two words pair up. A thread's
-    // scores are of rows 2 c4, 2 c4 + 1 (+ 8, ...): for these, from products to scores, and
-    // the queries' sums in the products' units. (ROWS 1: of the row.)
-    uint32_t qb[NG][4][NR][2];
-    uint64_t crow[NR], qsum[NG][NR];
-    const auto two_rows = [&](float v) {      // of the rows r8 that threads hold, this thread's two
-        if constexpr (ROWS == 1) return tc::f2(v, v);
-        return tc::f2(__shfl_sync(0xffffffffu, v, 8 * c4), __shfl_sync(0xffffffffu, v, 8 * c4 + 4));
+    // The products' side, list by list. Queries: of row r8 and each group the 16 dimensions
+    // from 16 c4 on, as the numbers of a thread's two words pair up; up to 4 rows, columns 2 r
+    // and 2 r + 1 are row r's. A thread's scores are of rows 2 c4 and 2 c4 + 1, of row c4 (4 rows), of
+    // the row: for these, from products to scores, and the queries' sums in the products' units.
+    uint32_t qb[NG][4][2];
+    uint64_t crow, qsum[NG];
+    const auto of_rows = [&](float v) {      // of the rows that threads r8 hold, this thread's
+        if constexpr (ROWS == 1) return tc::f2(v, 0.0f);
+        const float v0 = __shfl_sync(0xffffffffu, v, 8 * c4);
+        return tc::f2(v0, ROWS == 4 ? 0.0f : __shfl_sync(0xffffffffu, v, 8 * c4 + 4));
     };
     auto queries = [&](int seq, int qy) {
         const int row0 = qy % groups * P.per, nr = min(P.per, P.rows - row0), hk = qy / groups;
+        const int mine = ROWS == 1 ? 0 : ROWS == 4 ? r8 >> 1 : r8, row = row0 + mine;
+        const bool odd = ROWS < 8 && (r8 & 1);
+        uint4 raw[NG][2];
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-            const int mine = ROWS == 1 ? 0 : r8 + 8 * r, row = row0 + mine;
-            uint4 raw[NG][2];
+        for (int g = 0; g < NG; ++g)
 #pragma unroll
-            for (int g = 0; g < NG; ++g)
-#pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    raw[g][w] = make_uint4(0, 0, 0, 0);
-                    if (mine < nr)
-                        raw[g][w] = *reinterpret_cast<const uint4 *>(
-                            P.q + (static_cast<int64_t>(seq) * P.n_new + row / G) * P.q_ld +
-                            static_cast<int64_t>(hk * G + row % G) * HD + 64 * g + 16 * c4 + 8 * w);
-                }
-            uint32_t top = 0;      // the greatest magnitude's bits
-#pragma unroll
-            for (int g = 0; g < NG; ++g)
-#pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    const uint32_t x[4] = {raw[g][w].x, raw[g][w].y, raw[g][w].z, raw[g][w].w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) top = max(top, max(x[e] & 0x7fffu, x[e] >> 16 & 0x7fffu));
-                }
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // 2^up takes the greatest to 2^9 .. 2^10 (a row of tiny values not as far up: its scores are equal anyway)
-            const int up = min(136 - static_cast<int>(top >> 7), 100);
-            const float f = pow2(up);
-            // positive and finite: beyond these bounds one key has all the weight, or all have the same
-            float c = fminf(fmaxf(P.scale_log2 * pow2(min(20 - up, 127)), 1e-37f), 3e38f);
-            if (top >= 0x7f80u) c = __int_as_float(0x7fc00000);            // a query that is not finite
-            crow[r] = two_rows(c);
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                float sum = 0.0f;
-#pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    float x[8];
-                    unpack8(raw[g][w], x);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        x[e] *= f;
-                        sum += x[e];
-                    }
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        // against numbers in the low places (or bytes), 16 times, and in the high ones
-                        const uint32_t low = pack_f16x2(16.0f * x[2 * e], 16.0f * x[2 * e + 4]);
-                        const uint32_t high = pack_f16x2(x[2 * e + 1], x[2 * e + 5]);
-                        // ROWS 1: an even column has the bytes' and the upper numbers' products, an odd one what
-                        // the bytes' have of the upper numbers
-                        qb[g][2 * w + e][r][0] = ROWS == 1 && (r8 & 1) ? 0u : low;
-                        qb[g][2 * w + e][r][1] = ROWS == 1 && (r8 & 1) ? low : high;
-                    }
-                }
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                qsum[g][r] = two_rows(sum * 0x1p-20f);
+            for (int w = 0; w < 2; ++w) {
+                raw[g][w] = make_uint4(0, 0, 0, 0);
+                if (mine < nr)
+                    raw[g][w] = *reinterpret_cast<const uint4 *>(
+                        P.q + (static_cast<int64_t>(seq) * P.n_new + row / G) * P.q_ld +
+                        static_cast<int64_t>(hk * G + row % G) * HD + 64 * g + 16 * c4 + 8 * w);
             }
+        uint32_t top = 0;      // the greatest magnitude's bits
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                const uint32_t x[4] = {raw[g][w].x, raw[g][w].y, raw[g][w].z, raw[g][w].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top = max(top, max(x[e] & 0x7fffu, x[e] >> 16 & 0x7fffu));
+            }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // 2^up takes the greatest to 2^9 .. 2^10 (a row of tiny values not as far up: its scores are equal anyway)
+        const int up = min(136 - static_cast<int>(top >> 7), 100);
+        const float f = pow2(up);
+        // positive and finite: beyond these bounds one key has all the weight, or all have the same
+        float c = fminf(fmaxf(P.scale_log2 * pow2(min(20 - up, 127)), 1e-37f), 3e38f);
+        if (top >= 0x7f80u) c = __int_as_float(0x7fc00000);            // a query that is not finite
+        crow = of_rows(c);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                float x[8];
+                unpack8(raw[g][w], x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[e] *= f;
+                    sum += x[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    // against numbers in the low places (or bytes), 16 times, and in the high ones. Up to 4 rows, an even
+                    // column has the bytes' and the upper numbers' products, an odd one what the bytes' have of the upper
+                    const uint32_t low = pack_f16x2(16.0f * x[2 * e], 16.0f * x[2 * e + 4]);
+                    const uint32_t high = pack_f16x2(x[2 * e + 1], x[2 * e + 5]);
+                    qb[g][2 * w + e][0] = odd ? 0u : low;
+                    qb[g][2 * w + e][1] = odd ? low : high;
+                }
+            }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            qsum[g] = of_rows(sum * 0x1p-20f);
         }
     };
     int b = at.b, y = at.y, i0 = at.i, taken = 0;
@@ -446,46 +438,39 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
         const int tiles = tiles_to(base, len.tiles) - i0;
         bool lost = len.lost || fresh.lost;
         // keys that this thread's rows see (of rows that are no new token's: whatever there is), and that all see
-        int sees[NR][2];
+        int sees[2];
 #pragma unroll
-        for (int r = 0; r < NR; ++r)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int j = (row0 + (ROWS == 1 ? 0 : 8 * r + 2 * c4 + e)) / G;
-                sees[r][e] = j < fresh.count ? fresh.first + j : INT32_MAX;
-            }
+        for (int e = 0; e < 2; ++e) {
+            const int j = (row0 + (ROWS == 1 ? 0 : ROWS == 4 ? c4 : 2 * c4 + e)) / G;
+            sees[e] = j < fresh.count ? fresh.first + j : INT32_MAX;
+        }
         const int all_see = row0 / G < fresh.count ? fresh.first + row0 / G : INT32_MAX;
-        // ROWS 1: acc[g][i][0], i < 2: of bytes i and i + 2, sums l2 and z2 of a lane's keys in their low halves
-        float acc[NG][ROWS == 1 ? 2 : 4][NR][4], m[NR][2];
-        uint64_t l2[NR], z2[NG][NR], ref[NR];      // ref: what is added to a score for its weight, -m or 0
-        float far[NR][2];       // a score above moves the references
-        int top[NG];            // 2^(top - 127) is above every scale so far
-        float above[NG], unit[NG];      // that, and the weights' unit
+        // sums of this thread's keys, references and limits: of its row, or of its two
         const uint64_t none2 = tc::f2(0.0f, 0.0f);
-#pragma unroll
-        for (int r = 0; r < NR; ++r) m[r][0] = m[r][1] = far[r][0] = far[r][1] = -INFINITY, l2[r] = ref[r] = none2;
+        float acc[NG][NA][4], m[2] = {-INFINITY, -INFINITY};
+        float far[2] = {-INFINITY, -INFINITY};      // a score above moves the references
+        uint64_t l2 = none2, z2[NG], ref = none2;   // ref: what is added to a score for its weight, -m or 0
+        int top[NG];                    // 2^(top - 127) is above every scale so far
+        float above[NG], unit[NG];      // that, and the weights' unit
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             top[g] = 15;
             above[g] = pow2(15 - 127);
             unit[g] = pow2(139 - 15);
+            z2[g] = none2;
 #pragma unroll
-            for (int r = 0; r < NR; ++r) {
-                z2[g][r] = none2;
+            for (int i = 0; i < NA; ++i)
 #pragma unroll
-                for (int i = 0; i < (ROWS == 1 ? 2 : 4); ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[g][i][r][e] = 0.0f;
-            }
+                for (int e = 0; e < 4; ++e) acc[g][i][e] = 0.0f;
         }
-        // every output so far times f (of the row in a column)
-        auto rescale = [&](int g, int r, float f0, float f1) {
+        // every output so far times f (of the row that a column is of)
+        auto rescale = [&](int g, float f0, float f1) {
 #pragma unroll
-            for (int i = 0; i < (ROWS == 1 ? 2 : 4); ++i)
+            for (int i = 0; i < NA; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[g][i][r][e] *= e & 1 ? f1 : f0;
+                for (int e = 0; e < 4; ++e) acc[g][i][e] *= e & 1 ? f1 : f0;
         };
-        // the values' scales of this lane's keys, `most` their greatest: a finite one above the power of two so far raises it
+        // `most`, the greatest of the values' scales of this lane's keys: a finite one above the power of two so far raises it
         auto raise = [&](int g, float most) {
             if (__any_sync(0xffffffffu, most >= above[g])) {
                 const int to = static_cast<int>(__reduce_max_sync(0xffffffffu, __float_as_uint(most)) >> 23) + 1;
@@ -493,16 +478,51 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                 top[g] = to;
                 above[g] = to <= 254 ? pow2(to - 127) : INFINITY;
                 unit[g] = pow2(139 - to);
-#pragma unroll
-                for (int r = 0; r < NR; ++r) rescale(g, r, f, f);
+                rescale(g, f, f);
             }
         };
+        // the references to the greatest scores, over the lanes that share a row
+        auto move = [&](float x0, float x1) {
+            float f[2], x[2] = {fmaxf(x0, m[0]), fmaxf(x1, m[1])};      // not NaN
+#pragma unroll
+            for (int e = 0; e < (ROWS == 8 ? 2 : 1); ++e) {
+#pragma unroll
+                for (int o = ROWS == 1 ? 1 : 4; o < 32; o <<= 1) x[e] = fmaxf(x[e], __shfl_xor_sync(0xffffffffu, x[e], o));
+                f[e] = x[e] > m[e] ? tc::ex2(m[e] - x[e]) : 1.0f;
+                m[e] = x[e];
+                far[e] = x[e] + kSlack;
+            }
+            if (ROWS < 8) f[1] = f[0];
+            ref = tc::f2(m[0] == -INFINITY ? 0.0f : -m[0], m[1] == -INFINITY ? 0.0f : -m[1]);
+            const uint64_t f2 = tc::f2(f[0], f[1]);
+            l2 = tc::mul2(l2, f2);
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                z2[g] = tc::mul2(z2[g], f2);
+                rescale(g, f[0], f[1]);
+            }
+        };
+        const auto low = [](uint64_t v) { return tc::f2_split(v).x; };
         for (int i = (warp - taken) & (kDecWarps - 1); i < tiles; i += kDecWarps) {
             if (waits && !wait_phase(&s_full[warp][head], parity)) waits = false;
             lost |= (bad >> head & 1) || !waits;
             const int key0 = (i0 + i) * kTile, there = len.n - key0;      // there: keys of the sequence from here on
             const unsigned char *sk = dsm + (warp * C::kStages + head) * C::kStage, *sv = sk + C::kSide, *ss = sv + C::kSide;
             const bool masked = key0 + kTile > all_see;
+            // the two words that a thread multiplies of a key's group
+            const auto key_words = [&](int key, int g) {
+                return *reinterpret_cast<const uint2 *>(sk + key * C::kRowBytes + 32 * g + 8 * c4);
+            };
+            // up to 4 rows: the products with keys in rows r8 of blocks 2 mt and 2 mt + 1, in even columns with the bytes and
+            // the upper numbers, in odd ones what the bytes have of the upper numbers
+            const auto byte_products = [&](float (&d)[4], uint2 k0, uint2 k1, int g) {
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    const uint32_t x = bytes_of(s & 2 ? k0.y : k0.x, s & 1), x2 = bytes_of(s & 2 ? k1.y : k1.x, s & 1);
+                    if (s == 0) mma_f16_first(d, x, x2, x & kOdd, x2 & kOdd, qb[g][s][0], qb[g][s][1]);
+                    else mma_f16(d, x, x2, x & kOdd, x2 & kOdd, qb[g][s][0], qb[g][s][1]);
+                }
+            };
             if constexpr (ROWS == 1) {
                 // scores: this lane's are of keys 8 c4 + r8 (+ 32), one of each four blocks
                 float t[kKeys];
@@ -519,67 +539,38 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                         if (key < there) most = fmaxf(most, bf_lo(raw[g][k].y));
                     }
                     raise(g, most);
-                    float d[NM][4];
+                    float d[NB / 2][4];
 #pragma unroll
-                    for (int mt = 0; mt < NM; ++mt) {
-                        uint32_t w[2][2];
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const uint2 x = *reinterpret_cast<const uint2 *>(sk + (16 * mt + 8 * h + r8) * C::kRowBytes + 32 * g + 8 * c4);
-                            w[h][0] = x.x, w[h][1] = x.y;
-                        }
-#pragma unroll
-                        for (int s = 0; s < 4; ++s) {
-                            const uint32_t x = bytes_of(w[0][s >> 1], s & 1), x2 = bytes_of(w[1][s >> 1], s & 1);
-                            if (s == 0) mma_f16_first(d[mt], x, x2, x & kOdd, x2 & kOdd, qb[g][s][0][0], qb[g][s][0][1]);
-                            else mma_f16(d[mt], x, x2, x & kOdd, x2 & kOdd, qb[g][s][0][0], qb[g][s][0][1]);
-                        }
-                    }
-                    const float q = tc::f2_split(qsum[g][0]).x;
+                    for (int mt = 0; mt < NB / 2; ++mt)
+                        byte_products(d[mt], key_words(16 * mt + r8, g), key_words(16 * mt + 8 + r8, g), g);
 #pragma unroll
                     for (int k = 0; k < kKeys; ++k) {
                         float x[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) x[e] = d[2 * k + (e >> 1)][2 * (e & 1)] - d[2 * k + (e >> 1)][2 * (e & 1) + 1];
                         const float dot = c4 & 2 ? (c4 & 1 ? x[3] : x[2]) : (c4 & 1 ? x[1] : x[0]);
-                        t[k] = fmaf(bf_lo(raw[g][k].x), dot, fmaf(bf_hi(raw[g][k].x), q, t[k]));
+                        t[k] = fmaf(bf_lo(raw[g][k].x), dot, fmaf(bf_hi(raw[g][k].x), low(qsum[g]), t[k]));
                     }
                 }
                 float mx = -INFINITY;
 #pragma unroll
                 for (int k = 0; k < kKeys; ++k) {
-                    if (masked && key0 + 32 * k + 8 * c4 + r8 >= sees[0][0]) t[k] = -INFINITY;
+                    if (masked && key0 + 32 * k + 8 * c4 + r8 >= sees[0]) t[k] = -INFINITY;
                     mx = fmaxf(mx, t[k]);
                 }
-                const float c = tc::f2_split(crow[0]).x;
-                if (__any_sync(0xffffffffu, mx * c > far[0][0])) {
-                    float x = fmaxf(mx * c, m[0][0]);      // not NaN
-#pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-                    const float f = x > m[0][0] ? tc::ex2(m[0][0] - x) : 1.0f;
-                    const uint64_t f2 = tc::f2(f, f);
-                    m[0][0] = x;
-                    far[0][0] = x + kSlack;
-                    ref[0] = tc::f2(x == -INFINITY ? 0.0f : -x, 0.0f);
-                    l2[0] = tc::mul2(l2[0], f2);
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) {
-                        z2[g][0] = tc::mul2(z2[g][0], f2);
-                        rescale(g, 0, f, f);
-                    }
-                }
+                if (__any_sync(0xffffffffu, mx * low(crow) > far[0])) move(mx * low(crow), -INFINITY);
                 // weights to the lanes that multiply them: key t at (t mod 4, t / 4), once in the low half and once in the high one
 #pragma unroll
                 for (int k = 0; k < kKeys; ++k) {
                     const int key = 32 * k + 8 * c4 + r8;
-                    const bool hidden = masked && key0 + key >= sees[0][0];
-                    const float p = tc::ex2(fmaf(t[k], c, tc::f2_split(ref[0]).x));
-                    l2[0] = tc::f2(tc::f2_split(l2[0]).x + p, 0.0f);
+                    const bool hidden = masked && key0 + key >= sees[0];
+                    const float p = tc::ex2(fmaf(t[k], low(crow), low(ref)));
+                    l2 = tc::f2(low(l2) + p, 0.0f);
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
                         // what the row does not see does not reach it: NaN scales neither
                         const float w = hidden ? 0.0f : p * (bf_lo(raw[g][k].y) * unit[g]), zero = hidden ? 0.0f : bf_hi(raw[g][k].y);
-                        z2[g][0] = tc::f2(fmaf(p, zero, tc::f2_split(z2[g][0]).x), 0.0f);
+                        z2[g] = tc::f2(fmaf(p, zero, low(z2[g])), 0.0f);
                         const uint32_t half = pack_f16x2(w, 0.0f);
                         uint32_t *to = s_w + 8 * C::kStride * g + (key & 3) * C::kStride + (key >> 2);
                         to[0] = half;
@@ -602,10 +593,68 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
 #pragma unroll
                             for (int s = 0; s < 2; ++s) {
                                 const uint32_t x = bytes_of(x0, s), x2 = bytes_of(x1, s);
-                                mma_f16(acc[g][s][0], x, x & kOdd, x2, x2 & kOdd, pw[u], pw[u + 1]);
+                                mma_f16(acc[g][s], x, x & kOdd, x2, x2 & kOdd, pw[u], pw[u + 1]);
                             }
                         }
                     }
+            } else if constexpr (ROWS == 4) {
+                // scores of row c4: keys key_of(r8) of each block
+                const int mine = key_of(r8);
+                float t[NB];
+                uint2 raw[NG][NB];
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    float most = 0.0f;
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) {
+                        raw[g][n] = *reinterpret_cast<const uint2 *>(ss + (8 * n + mine) * C::kScaleBytes + 8 * g);
+                        if (8 * n + mine < there) most = fmaxf(most, bf_lo(raw[g][n].y));
+                    }
+                    raise(g, most);
+#pragma unroll
+                    for (int mt = 0; mt < NB / 2; ++mt) {
+                        float d[4];
+                        byte_products(d, key_words(16 * mt + mine, g), key_words(16 * mt + 8 + mine, g), g);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int n = 2 * mt + h;
+                            const float zero = bf_hi(raw[g][n].x) * low(qsum[g]);
+                            t[n] = fmaf(bf_lo(raw[g][n].x), d[2 * h] - d[2 * h + 1], g == 0 ? zero : t[n] + zero);
+                        }
+                    }
+                }
+                float mx = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    if (masked && key0 + 8 * n + mine >= sees[0]) t[n] = -INFINITY;
+                    mx = fmaxf(mx, t[n]);
+                }
+                if (__any_sync(0xffffffffu, mx * low(crow) > far[0])) move(mx * low(crow), -INFINITY);
+                // weights: transposed, a thread has those of keys in rows 2 c4 and 2 c4 + 1 of row r8 / 2: in an even column
+                // for the words' low halves, in an odd one for the high ones
+                const uint32_t first = r8 & 1 ? 0x1044u : 0x4410u, second = r8 & 1 ? 0x3244u : 0x4432u;
+                const unsigned char *v0 = sv + key_of(2 * c4) * C::kRowBytes + 4 * r8, *v1 = sv + key_of(2 * c4 + 1) * C::kRowBytes + 4 * r8;
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    const bool hidden = masked && key0 + 8 * n + mine >= sees[0];
+                    const float p = tc::ex2(fmaf(t[n], low(crow), low(ref)));
+                    l2 = tc::f2(low(l2) + p, 0.0f);
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        // what a row does not see does not reach it: NaN scales neither
+                        const float w = hidden ? 0.0f : p * (bf_lo(raw[g][n].y) * unit[g]), zero = hidden ? 0.0f : bf_hi(raw[g][n].y);
+                        z2[g] = tc::f2(fmaf(p, zero, low(z2[g])), 0.0f);
+                        const uint32_t both = transpose8(pack_f16x2(w, w));
+                        const uint32_t b0 = __byte_perm(both, 0, first), b1 = __byte_perm(both, 0, second);
+                        const uint32_t x0 = *reinterpret_cast<const uint32_t *>(v0 + 8 * n * C::kRowBytes + 32 * g);
+                        const uint32_t x1 = *reinterpret_cast<const uint32_t *>(v1 + 8 * n * C::kRowBytes + 32 * g);
+#pragma unroll
+                        for (int s = 0; s < 2; ++s) {
+                            const uint32_t x = bytes_of(x0, s), x2 = bytes_of(x1, s);
+                            mma_f16(acc[g][s], x, x & kOdd, x2, x2 & kOdd, b0, b1);
+                        }
+                    }
+                }
             } else {
                 // [group][key's, value's][key]: scale, scale, zero, zero in fp32, once for the warp, each
                 // lane its keys'; the values' scales take the weights' unit along
@@ -628,143 +677,90 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                     }
                 }
                 __syncwarp();
-                // scores of keys 16 mt + 8 h + key_of(r8), both rows of a pair in one register pair
+                // scores of keys key_of(r8) of each block, both rows of a pair in one register pair
                 const int mine = key_of(r8);
-                uint64_t t[NM][2][NR];
+                uint64_t t[NB];
 #pragma unroll
                 for (int g = 0; g < NG; ++g)
 #pragma unroll
-                    for (int mt = 0; mt < NM; ++mt) {
-                        uint32_t w[2][2];
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const uint2 x = *reinterpret_cast<const uint2 *>(sk + (16 * mt + 8 * h + mine) * C::kRowBytes + 32 * g + 8 * c4);
-                            w[h][0] = x.x, w[h][1] = x.y;
-                        }
-                        float d[NR][4];
+                    for (int mt = 0; mt < NB / 2; ++mt) {
+                        const uint2 k0 = key_words(16 * mt + mine, g), k1 = key_words(16 * mt + 8 + mine, g);
+                        float d[4];
 #pragma unroll
                         for (int s = 0; s < 4; ++s) {
-                            const uint32_t x = s & 1 ? w[0][s >> 1] >> 8 : w[0][s >> 1];
-                            const uint32_t x2 = s & 1 ? w[1][s >> 1] >> 8 : w[1][s >> 1];
-#pragma unroll
-                            for (int r = 0; r < NR; ++r) {
-                                if (s == 0) mma_f16_first(d[r], x & kEven, x2 & kEven, x & kOdd, x2 & kOdd, qb[g][s][r][0], qb[g][s][r][1]);
-                                else mma_f16(d[r], x & kEven, x2 & kEven, x & kOdd, x2 & kOdd, qb[g][s][r][0], qb[g][s][r][1]);
-                            }
+                            const uint32_t x = (s & 2 ? k0.y : k0.x) >> 8 * (s & 1), x2 = (s & 2 ? k1.y : k1.x) >> 8 * (s & 1);
+                            if (s == 0) mma_f16_first(d, x & kEven, x2 & kEven, x & kOdd, x2 & kOdd, qb[g][s][0], qb[g][s][1]);
+                            else mma_f16(d, x & kEven, x2 & kEven, x & kOdd, x2 & kOdd, qb[g][s][0], qb[g][s][1]);
                         }
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const ulonglong2 sz = s_x[(2 * g) * kTile + 16 * mt + 8 * h + mine];
-#pragma unroll
-                            for (int r = 0; r < NR; ++r) {
-                                const uint64_t zero = g == 0 ? tc::mul2(sz.y, qsum[g][r]) : tc::fma2(sz.y, qsum[g][r], t[mt][h][r]);
-                                t[mt][h][r] = tc::fma2(sz.x, tc::f2(d[r][2 * h], d[r][2 * h + 1]), zero);
-                            }
+                            const int n = 2 * mt + h;
+                            const ulonglong2 sz = s_x[(2 * g) * kTile + 8 * n + mine];
+                            const uint64_t zero = g == 0 ? tc::mul2(sz.y, qsum[g]) : tc::fma2(sz.y, qsum[g], t[n]);
+                            t[n] = tc::fma2(sz.x, tc::f2(d[2 * h], d[2 * h + 1]), zero);
                         }
                     }
                 if (masked) {
 #pragma unroll
-                    for (int mt = 0; mt < NM; ++mt)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int key = key0 + 16 * mt + 8 * h + mine;
-#pragma unroll
-                            for (int r = 0; r < NR; ++r) {
-                                const float2 x = tc::f2_split(t[mt][h][r]);
-                                t[mt][h][r] = tc::f2(key < sees[r][0] ? x.x : -INFINITY, key < sees[r][1] ? x.y : -INFINITY);
-                            }
-                        }
+                    for (int n = 0; n < NB; ++n) {
+                        const float2 x = tc::f2_split(t[n]);
+                        const int key = key0 + 8 * n + mine;
+                        t[n] = tc::f2(key < sees[0] ? x.x : -INFINITY, key < sees[1] ? x.y : -INFINITY);
+                    }
                 }
                 // the greatest score that this thread has of each row (NaN left out); the references move if one is far above
-                float mx[NR][2];
-                bool grown = false;
+                float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int r = 0; r < NR; ++r) {
-                    float2 x = tc::f2_split(t[0][0][r]);
-                    mx[r][0] = x.x, mx[r][1] = x.y;
-#pragma unroll
-                    for (int k = 1; k < 2 * NM; k += 2) {
-                        x = tc::f2_split(t[k >> 1][k & 1][r]);
-                        const float2 x2 = k + 1 < 2 * NM ? tc::f2_split(t[(k + 1) >> 1][(k + 1) & 1][r]) : x;
-                        mx[r][0] = tc::fmax3(mx[r][0], x.x, x2.x);
-                        mx[r][1] = tc::fmax3(mx[r][1], x.y, x2.y);
-                    }
-                    const float2 c = tc::f2_split(crow[r]);
-                    mx[r][0] *= c.x, mx[r][1] *= c.y;
-                    grown |= mx[r][0] > far[r][0] || mx[r][1] > far[r][1];
+                for (int n = 0; n < NB; n += 2) {
+                    const float2 x = tc::f2_split(t[n]), x2 = tc::f2_split(t[n + 1]);
+                    mx[0] = tc::fmax3(mx[0], x.x, x2.x);
+                    mx[1] = tc::fmax3(mx[1], x.y, x2.y);
                 }
-                if (__any_sync(0xffffffffu, grown)) {
-#pragma unroll
-                    for (int r = 0; r < NR; ++r) {
-                        float f[2];
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            float x = fmaxf(mx[r][e], m[r][e]);      // not NaN
-#pragma unroll
-                            for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-                            f[e] = x > m[r][e] ? tc::ex2(m[r][e] - x) : 1.0f;
-                            m[r][e] = x;
-                            far[r][e] = x + kSlack;
-                        }
-                        ref[r] = tc::f2(m[r][0] == -INFINITY ? 0.0f : -m[r][0], m[r][1] == -INFINITY ? 0.0f : -m[r][1]);
-                        const uint64_t f2 = tc::f2(f[0], f[1]);
-                        l2[r] = tc::mul2(l2[r], f2);
-#pragma unroll
-                        for (int g = 0; g < NG; ++g) {
-                            z2[g][r] = tc::mul2(z2[g][r], f2);
-                            rescale(g, r, f[0], f[1]);
-                        }
-                    }
-                }
-                uint32_t pw[NG][NM][2][NR];
+                const float2 c = tc::f2_split(crow);
+                mx[0] *= c.x, mx[1] *= c.y;
+                if (__any_sync(0xffffffffu, mx[0] > far[0] || mx[1] > far[1])) move(mx[0], mx[1]);
+                uint32_t pw[NG][NB];
                 auto weigh = [&](auto some_hidden) {
 #pragma unroll
-                    for (int r = 0; r < NR; ++r)
+                    for (int n = 0; n < NB; ++n) {
+                        const uint64_t p2 = tc::ex2_pair(tc::fma2(t[n], crow, ref));
+                        l2 = tc::add2(l2, p2);
 #pragma unroll
-                        for (int mt = 0; mt < NM; ++mt)
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const uint64_t p2 = tc::ex2_pair(tc::fma2(t[mt][h][r], crow[r], ref[r]));
-                                l2[r] = tc::add2(l2[r], p2);
-                                const int key = 16 * mt + 8 * h + mine;
-#pragma unroll
-                                for (int g = 0; g < NG; ++g) {
-                                    ulonglong2 sz = s_x[(2 * g + 1) * kTile + key];
-                                    if constexpr (some_hidden.value) {
-                                        // what a row does not see does not reach it: NaN scales neither
-                                        const bool s0 = key0 + key < sees[r][0], s1 = key0 + key < sees[r][1];
-                                        const float a = tc::f2_split(sz.x).x, c = tc::f2_split(sz.y).x;
-                                        sz.x = tc::f2(s0 ? a : 0.0f, s1 ? a : 0.0f);
-                                        sz.y = tc::f2(s0 ? c : 0.0f, s1 ? c : 0.0f);
-                                    }
-                                    z2[g][r] = tc::fma2(p2, sz.y, z2[g][r]);
-                                    const float2 w = tc::f2_split(tc::mul2(p2, sz.x));
-                                    pw[g][mt][h][r] = transpose8(pack_f16x2(w.x, w.y));
-                                }
+                        for (int g = 0; g < NG; ++g) {
+                            ulonglong2 sz = s_x[(2 * g + 1) * kTile + 8 * n + mine];
+                            if constexpr (some_hidden.value) {
+                                // what a row does not see does not reach it: NaN scales neither
+                                const bool s0 = key0 + 8 * n + mine < sees[0], s1 = key0 + 8 * n + mine < sees[1];
+                                const float vs = low(sz.x), vz = low(sz.y);
+                                sz.x = tc::f2(s0 ? vs : 0.0f, s1 ? vs : 0.0f);
+                                sz.y = tc::f2(s0 ? vz : 0.0f, s1 ? vz : 0.0f);
                             }
+                            z2[g] = tc::fma2(p2, sz.y, z2[g]);
+                            const float2 w = tc::f2_split(tc::mul2(p2, sz.x));
+                            pw[g][n] = transpose8(pack_f16x2(w.x, w.y));
+                        }
+                    }
                 };
                 if (masked) weigh(std::true_type{});
                 else weigh(std::false_type{});
-                const int even_row = key_of(2 * c4), odd_row = key_of(2 * c4 + 1);
+                const unsigned char *v0 = sv + key_of(2 * c4) * C::kRowBytes + 4 * r8, *v1 = sv + key_of(2 * c4 + 1) * C::kRowBytes + 4 * r8;
 #pragma unroll
                 for (int g = 0; g < NG; ++g)
 #pragma unroll
-                    for (int mt = 0; mt < NM; ++mt) {
-                        uint32_t w[2][2];      // bytes 0, 1 and 2, 3 of the keys in rows 2 c4 and 2 c4 + 1 (+ 8)
+                    for (int mt = 0; mt < NB / 2; ++mt) {
+                        uint32_t w[2][2];      // bytes 0, 1 and 2, 3 of the keys in rows 2 c4 and 2 c4 + 1 of both blocks
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const unsigned char *at = sv + (16 * mt + 8 * h) * C::kRowBytes + 32 * g + 4 * r8;
-                            const uint32_t x0 = *reinterpret_cast<const uint32_t *>(at + even_row * C::kRowBytes);
-                            const uint32_t x1 = *reinterpret_cast<const uint32_t *>(at + odd_row * C::kRowBytes);
+                            const int at = (16 * mt + 8 * h) * C::kRowBytes + 32 * g;
+                            const uint32_t x0 = *reinterpret_cast<const uint32_t *>(v0 + at);
+                            const uint32_t x1 = *reinterpret_cast<const uint32_t *>(v1 + at);
                             w[h][0] = __byte_perm(x0, x1, 0x5410);
                             w[h][1] = __byte_perm(x0, x1, 0x7632);
                         }
 #pragma unroll
                         for (int i2 = 0; i2 < 4; ++i2) {
                             const uint32_t x = bytes_of(w[0][i2 >> 1], i2 & 1), x2 = bytes_of(w[1][i2 >> 1], i2 & 1);
-#pragma unroll
-                            for (int r = 0; r < NR; ++r)
-                                mma_f16(acc[g][i2][r], x, x & kOdd, x2, x2 & kOdd, pw[g][mt][0][r], pw[g][mt][1][r]);
+                            mma_f16(acc[g][i2], x, x & kOdd, x2, x2 & kOdd, pw[g][2 * mt], pw[g][2 * mt + 1]);
                         }
                     }
             }
@@ -785,110 +781,108 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
             if (nb != b) blen = P.seq_lens[nb];
         }
 
-        // join the warps: their references and sums, then the outputs of some rows at a time
+        // join the warps: their references and sums, then the outputs
         const auto whole_rows = [](uint64_t v2) {
             float2 v = tc::f2_split(v2);
 #pragma unroll
             for (int o = ROWS == 1 ? 1 : 4; o < 32; o <<= 1) {
                 v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-                v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+                if (ROWS == 8) v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
             }
             return v;
         };
+        const auto put = [&](float *to, float2 v) {
+            if constexpr (ROWS == 8) *reinterpret_cast<float2 *>(to + 2 * c4) = v;
+            else to[c4] = v.x;
+        };
+        const float2 l = whole_rows(l2);
+        if (r8 == 0) {
+            put(s_m[warp], make_float2(m[0], m[1]));
+            put(s_l[warp], l);
+        }
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-            const float2 l = whole_rows(l2[r]);
-            if (r8 == 0) {
-                *reinterpret_cast<float2 *>(&s_m[warp][8 * r + 2 * c4]) = make_float2(m[r][0], m[r][1]);
-                *reinterpret_cast<float2 *>(&s_l[warp][8 * r + 2 * c4]) = l;
-            }
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                const float2 z = whole_rows(z2[g][r]);
-                if (r8 == 0) *reinterpret_cast<float2 *>(&s_z[warp][g][8 * r + 2 * c4]) = z;
-            }
+        for (int g = 0; g < NG; ++g) {
+            const float2 z = whole_rows(z2[g]);
+            if (r8 == 0) put(s_z[warp][g], z);
         }
         lost = __syncthreads_or(lost);
         const int64_t list = static_cast<int64_t>(b) * lists + y;
         const bool whole = i0 == 0 && tiles == len.tiles;
+        const auto reference = [&](int row) {
+            float M = s_m[0][row];
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-            if (8 * r >= nr) break;
-            const auto reference = [&](int row) {
-                float M = s_m[0][row];
+            for (int w = 1; w < kDecWarps; ++w) M = fmaxf(M, s_m[w][row]);
+            return M;
+        };
+        // the bytes' units and the weights' taken out; an even dimension's sum is what the bytes' has beyond the odd one's
+        const auto part_of = [&](int row, int g) {
+            const float f = s_m[warp][row] == -INFINITY ? 0.0f : tc::ex2(s_m[warp][row] - reference(row));
+            return pow2(min(top[g] - 127, 127)) * f;
+        };
+        const auto pair_of = [](const float (&x)[4], int e, float u) {
+            return make_float2((x[e] - x[2 + e]) * 4096.0f * u, x[2 + e] * 256.0f * u);
+        };
 #pragma unroll
-                for (int w = 1; w < kDecWarps; ++w) M = fmaxf(M, s_m[w][row]);
-                return M;
-            };
-            // the bytes' units and the weights' taken out: even dimensions are what the bytes' sums have beyond the odd ones'
-            if constexpr (ROWS == 1) {
-                const float f = s_m[warp][0] == -INFINITY ? 0.0f : tc::ex2(s_m[warp][0] - reference(0));
-                if (c4 == 0) {
+        for (int g = 0; g < NG; ++g) {
+            if constexpr (ROWS < 8) {
+                const int row = ROWS == 1 ? 0 : c4;
+                if (ROWS == 4 || c4 == 0) {
+                    const float u = part_of(row, g);
+                    float4 *to = reinterpret_cast<float4 *>(s_o + (warp * ROWS + row) * HD + 64 * g + 8 * r8);
 #pragma unroll
-                    for (int g = 0; g < NG; ++g) {
-                        const float u = pow2(min(top[g] - 127, 127)) * f;
-                        float4 *dst = reinterpret_cast<float4 *>(s_o + warp * HD + 64 * g + 8 * r8);
-#pragma unroll
-                        for (int h = 0; h < 2; ++h)
-                            dst[h] = make_float4((acc[g][0][0][h] - acc[g][0][0][2 + h]) * 4096.0f * u, acc[g][0][0][2 + h] * 256.0f * u,
-                                                 (acc[g][1][0][h] - acc[g][1][0][2 + h]) * 4096.0f * u, acc[g][1][0][2 + h] * 256.0f * u);
+                    for (int e = 0; e < 2; ++e) {
+                        const float2 x = pair_of(acc[g][0], e, u), x2 = pair_of(acc[g][1], e, u);
+                        to[e] = make_float4(x.x, x.y, x2.x, x2.y);
                     }
                 }
             } else {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int row = 8 * r + 2 * c4 + e;
-                    const float f = s_m[warp][row] == -INFINITY ? 0.0f : tc::ex2(s_m[warp][row] - reference(row));
+                    const float u = part_of(2 * c4 + e, g);
+                    float4 *to = reinterpret_cast<float4 *>(s_o + (warp * ROWS + 2 * c4 + e) * HD + 64 * g + 8 * r8);
 #pragma unroll
-                    for (int g = 0; g < NG; ++g) {
-                        const float u = pow2(min(top[g] - 127, 127)) * f;
-                        float *dst = s_o + (warp * 8 + 2 * c4 + e) * HD + 64 * g + 8 * r8;
-#pragma unroll
-                        for (int i2 = 0; i2 < 4; i2 += 2)
-                            *reinterpret_cast<float4 *>(dst + 2 * i2) =
-                                make_float4((acc[g][i2][r][e] - acc[g][i2][r][2 + e]) * 4096.0f * u, acc[g][i2][r][2 + e] * 256.0f * u,
-                                            (acc[g][i2 + 1][r][e] - acc[g][i2 + 1][r][2 + e]) * 4096.0f * u,
-                                            acc[g][i2 + 1][r][2 + e] * 256.0f * u);
+                    for (int h = 0; h < 2; ++h) {
+                        const float2 x = pair_of(acc[g][2 * h], e, u), x2 = pair_of(acc[g][2 * h + 1], e, u);
+                        to[h] = make_float4(x.x, x.y, x2.x, x2.y);
                     }
                 }
             }
-            __syncthreads();
-            const int left = min(nr - 8 * r, 8) * (HD / 4);
-            for (int e = threadIdx.x; e < left; e += blockDim.x) {
-                const int in8 = e / (HD / 4), row = 8 * r + in8, d = e % (HD / 4) * 4;
-                const float M = reference(row);
-                float L = 0.0f;
-                float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-                for (int w = 0; w < kDecWarps; ++w) {
-                    // a warp without a reference saw nothing, or NaN alone
-                    const float f = s_m[w][row] == -INFINITY ? 1.0f : tc::ex2(s_m[w][row] - M);
-                    L += s_l[w][row] * f;
-                    const float4 x = *reinterpret_cast<const float4 *>(s_o + (w * C::kPass + in8) * HD + d);
-                    const float zero = s_z[w][d / 64][row] * f;
-                    o.x += x.x + zero, o.y += x.y + zero, o.z += x.z + zero, o.w += x.w + zero;
-                }
-                if (lost) L = __int_as_float(0x7fc00000);
-                if constexpr (Cluster) {
-                    // this CTA's part stays where the ring was
-                    *reinterpret_cast<float4 *>(reinterpret_cast<float *>(dsm) + row * HD + d) = o;
-                    if (d == 0) s_part[row] = make_float2(M, L);
-                } else if (whole) {
-                    const int j = (row0 + row) / G, h = y / groups * G + (row0 + row) % G;
-                    const float inv = 1.0f / L;
-                    uint2 got = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
-                    if (now.sees(j) <= 0) got = make_uint2(0, 0);
-                    *reinterpret_cast<uint2 *>(P.out + ((static_cast<int64_t>(b) * P.n_new + j) * P.H + h) * HD + d) = got;
-                } else {
-                    // a CTA and a list that follow one another in the order of tiles: no two
-                    // parts have the same sum
-                    float *dst = P.part + ((blockIdx.x + list) * P.per + row) * (HD + 4);
-                    *reinterpret_cast<float4 *>(dst + 4 + d) = o;
-                    if (d == 0) *reinterpret_cast<float2 *>(dst) = make_float2(M, L);
-                }
-            }
-            __syncthreads();
         }
+        __syncthreads();
+        for (int e = threadIdx.x; e < nr * (HD / 4); e += blockDim.x) {
+            const int row = e / (HD / 4), d = e % (HD / 4) * 4;
+            const float M = reference(row);
+            float L = 0.0f;
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < kDecWarps; ++w) {
+                // a warp without a reference saw nothing, or NaN alone
+                const float f = s_m[w][row] == -INFINITY ? 1.0f : tc::ex2(s_m[w][row] - M);
+                L += s_l[w][row] * f;
+                const float4 x = *reinterpret_cast<const float4 *>(s_o + (w * ROWS + row) * HD + d);
+                const float zero = s_z[w][d / 64][row] * f;
+                o.x += x.x + zero, o.y += x.y + zero, o.z += x.z + zero, o.w += x.w + zero;
+            }
+            if (lost) L = __int_as_float(0x7fc00000);
+            if constexpr (Cluster) {
+                // this CTA's part stays where the ring was
+                *reinterpret_cast<float4 *>(reinterpret_cast<float *>(dsm) + row * HD + d) = o;
+                if (d == 0) s_part[row] = make_float2(M, L);
+            } else if (whole) {
+                const int j = (row0 + row) / G, h = y / groups * G + (row0 + row) % G;
+                const float inv = 1.0f / L;
+                uint2 got = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+                if (now.sees(j) <= 0) got = make_uint2(0, 0);
+                *reinterpret_cast<uint2 *>(P.out + ((static_cast<int64_t>(b) * P.n_new + j) * P.H + h) * HD + d) = got;
+            } else {
+                // a CTA and a list that follow one another in the order of tiles: no two
+                // parts have the same sum
+                float *dst = P.part + ((blockIdx.x + list) * P.per + row) * (HD + 4);
+                *reinterpret_cast<float4 *>(dst + 4 + d) = o;
+                if (d == 0) *reinterpret_cast<float2 *>(dst) = make_float2(M, L);
+            }
+        }
+        __syncthreads();
         if constexpr (Cluster) break;
         if (i0 == 0 && threadIdx.x == 0) {
             const int n = static_cast<int>((at.base + next - 1) / at.span) - static_cast<int>(blockIdx.x) + 1;
@@ -973,9 +967,8 @@ static int list_rows(int64_t rows) {
 // f with the kernel's head_dim and rows: those that a list of `per` rows takes.
 template <typename F>
 static auto with_form(int64_t hd, int per, F f) {
-    if (hd == 64)
-        return per == 1 ? f(Dec4<64, 1>{}) : per <= 8 ? f(Dec4<64, 8>{}) : per <= 16 ? f(Dec4<64, 16>{}) : f(Dec4<64, 24>{});
-    return per == 1 ? f(Dec4<128, 1>{}) : per <= 8 ? f(Dec4<128, 8>{}) : per <= 16 ? f(Dec4<128, 16>{}) : f(Dec4<128, 24>{});
+    if (hd == 64) return per == 1 ? f(Dec4<64, 1>{}) : per <= 4 ? f(Dec4<64, 4>{}) : f(Dec4<64, 8>{});
+    return per == 1 ? f(Dec4<128, 1>{}) : per <= 4 ? f(Dec4<128, 4>{}) : f(Dec4<128, 8>{});
 }
 
 static DecodeSplit decode_int4_split(int64_t B, int64_t rows, int64_t Hk, int64_t hd, int64_t max_len) {
