@@ -170,7 +170,7 @@ rope_append_int4_kernel(const uint16_t *__restrict__ qkv, int64_t ld, const floa
 // comes along and is hidden like all that a row does not see.
 constexpr float kSlack = 3.0f;      // log2
 constexpr int kLeast = 4;           // tiles of a CTA's span, at least
-constexpr int kListCost = 3;        // tiles that a list's start and end cost
+constexpr int kListCost = 6;        // tiles that a list's start and end cost
 constexpr int kMostRows = 8;        // of a list
 
 template <int HD, int ROWS>
@@ -234,6 +234,12 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
                  "l"(src), "r"(bytes), "r"(smem_u32(bar))
                  : "memory");
 }
+// One lane of the warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(one));
+    return one != 0;
+}
 // Waits for a barrier's phase, for about a second at most.
 __device__ __forceinline__ bool wait_phase(uint64_t *bar, uint32_t parity) {
     if (tc::mbar_try_wait(bar, parity)) return true;
@@ -287,15 +293,12 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
     const auto tiles_to = [&](int base, int tiles) { return max(min(tiles, end - base - kListCost), 0); };
 
     // The copies' side of this warp: it takes every fourth tile of the span, whatever list
-    // it is of. Lane 4 i + kind looks the tile's page i up while the tile before is copied,
-    // and copies its keys, values or scales (kind 0, 1, 2). A page outside the cache is not
-    // copied and makes the sequence's result NaN.
+    // it is of. Lane i looks the tile's page i up while the tile before is copied; one lane then
+    // copies each page's keys, values and scales. A page outside the cache is not copied and
+    // makes the sequence's result NaN.
     const int page_mask = (1 << P.page_shift) - 1, page_rows = min(1 << P.page_shift, kTile);
-    const int kind = lane & 3, piece = lane >> 2;
-    const uint32_t row_bytes = kind < 2 ? C::kRowBytes : C::kScaleBytes;
-    const uint8_t *const src = kind == 0 ? P.k4 : kind == 1 ? P.v4 : reinterpret_cast<const uint8_t *>(P.scales);
-    const uint32_t dst = smem_u32(dsm) + warp * C::kStages * C::kStage + kind * C::kSide + piece * page_rows * row_bytes;
-    const int piece_first = kind < 3 ? piece * page_rows : kTile;      // its first key; none is that far
+    const uint32_t ring = smem_u32(dsm) + warp * C::kStages * C::kStage;
+    const int piece_first = lane * page_rows;      // the first key of the page that this lane looks up
     int fbase = 0, fb = at.b, fy = at.y, fhk = fy / groups, fi = at.i, fn = len.n, fall = len.tiles;
     int fend = tiles_to(fbase, fall);
     int32_t flen = !Cluster && fb + 1 < P.B ? P.seq_lens[fb + 1] : 0;      // the next sequence's
@@ -331,7 +334,7 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
         tile.first = fi * kTile;
         tile.rows = fn - tile.first;
         tile.hk = fhk;
-        if (piece_first < min(tile.rows, kTile)) tile.page = frow[(tile.first >> P.page_shift) + piece];
+        if (piece_first < min(tile.rows, kTile)) tile.page = frow[(tile.first >> P.page_shift) + lane];
         return tile;
     };
     auto fetch = [&](int stage, const Tile &tile) {
@@ -339,13 +342,23 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
             const bool mine = piece_first < min(tile.rows, kTile);
             const bool in = mine && static_cast<uint32_t>(tile.page) < static_cast<uint32_t>(P.n_pages);
             bad = (bad & ~(1u << stage)) | static_cast<uint32_t>(mine && !in) << stage;
-            const uint32_t pieces = __popc(__ballot_sync(0xffffffffu, in && kind == 0));
+            uint32_t have = __ballot_sync(0xffffffffu, in);
             uint64_t *bar = &s_full[warp][stage];
-            if (lane == 0) tc::mbar_arrive_expect_tx(bar, pieces * page_rows * (2 * C::kRowBytes + C::kScaleBytes));
-            __syncwarp();
+            const bool one = elect_one();
+            if (one) tc::mbar_arrive_expect_tx(bar, __popc(have) * page_rows * (2 * C::kRowBytes + C::kScaleBytes));
             // rows of the cache are counted in 32 bits (the caller's check), bytes in 64
             const uint32_t row = ((static_cast<uint32_t>(tile.page) * P.Hk + tile.hk) << P.page_shift) + (tile.first & page_mask);
-            if (in) bulk_load(dst + stage * C::kStage, src + static_cast<uint64_t>(row) * row_bytes, page_rows * row_bytes, bar);
+            for (; have; have &= have - 1) {
+                const int piece = __ffs(have) - 1;
+                const uint64_t from = __shfl_sync(0xffffffffu, row, piece);
+                const uint32_t to = ring + stage * C::kStage + piece * page_rows * C::kRowBytes;
+                if (one) {
+                    bulk_load(to, P.k4 + from * C::kRowBytes, page_rows * C::kRowBytes, bar);
+                    bulk_load(to + C::kSide, P.v4 + from * C::kRowBytes, page_rows * C::kRowBytes, bar);
+                    bulk_load(ring + stage * C::kStage + 2 * C::kSide + piece * page_rows * C::kScaleBytes,
+                              reinterpret_cast<const uint8_t *>(P.scales) + from * C::kScaleBytes, page_rows * C::kScaleBytes, bar);
+                }
+            }
         }
     };
     int head = 0;
@@ -553,24 +566,29 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                     }
                 }
                 float mx = -INFINITY;
+                if (masked) {
+                    // what the row does not see does not reach it: a value that stands for NaN neither
 #pragma unroll
-                for (int k = 0; k < kKeys; ++k) {
-                    if (masked && key0 + 32 * k + 8 * c4 + r8 >= sees[0]) t[k] = -INFINITY;
-                    mx = fmaxf(mx, t[k]);
+                    for (int k = 0; k < kKeys; ++k)
+                        if (key0 + 32 * k + 8 * c4 + r8 >= sees[0]) {
+                            t[k] = -INFINITY;
+#pragma unroll
+                            for (int g = 0; g < NG; ++g) raw[g][k].y = 0u;
+                        }
                 }
+#pragma unroll
+                for (int k = 0; k < kKeys; ++k) mx = fmaxf(mx, t[k]);
                 if (__any_sync(0xffffffffu, mx * low(crow) > far[0])) move(mx * low(crow), -INFINITY);
                 // weights to the lanes that multiply them: key t at (t mod 4, t / 4), once in the low half and once in the high one
 #pragma unroll
                 for (int k = 0; k < kKeys; ++k) {
                     const int key = 32 * k + 8 * c4 + r8;
-                    const bool hidden = masked && key0 + key >= sees[0];
                     const float p = tc::ex2(fmaf(t[k], low(crow), low(ref)));
                     l2 = tc::f2(low(l2) + p, 0.0f);
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
-                        // what the row does not see does not reach it: NaN scales neither
-                        const float w = hidden ? 0.0f : p * (bf_lo(raw[g][k].y) * unit[g]), zero = hidden ? 0.0f : bf_hi(raw[g][k].y);
-                        z2[g] = tc::f2(fmaf(p, zero, low(z2[g])), 0.0f);
+                        const float w = p * (bf_lo(raw[g][k].y) * unit[g]);
+                        z2[g] = tc::f2(fmaf(p, bf_hi(raw[g][k].y), low(z2[g])), 0.0f);
                         const uint32_t half = pack_f16x2(w, 0.0f);
                         uint32_t *to = s_w + 8 * C::kStride * g + (key & 3) * C::kStride + (key >> 2);
                         to[0] = half;
@@ -624,11 +642,18 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                     }
                 }
                 float mx = -INFINITY;
+                if (masked) {
+                    // what a row does not see does not reach it: a value that stands for NaN neither
 #pragma unroll
-                for (int n = 0; n < NB; ++n) {
-                    if (masked && key0 + 8 * n + mine >= sees[0]) t[n] = -INFINITY;
-                    mx = fmaxf(mx, t[n]);
+                    for (int n = 0; n < NB; ++n)
+                        if (key0 + 8 * n + mine >= sees[0]) {
+                            t[n] = -INFINITY;
+#pragma unroll
+                            for (int g = 0; g < NG; ++g) raw[g][n].y = 0u;
+                        }
                 }
+#pragma unroll
+                for (int n = 0; n < NB; n += 2) mx = tc::fmax3(mx, t[n], t[n + 1]);
                 if (__any_sync(0xffffffffu, mx * low(crow) > far[0])) move(mx * low(crow), -INFINITY);
                 // weights: transposed, a thread has those of keys in rows 2 c4 and 2 c4 + 1 of row r8 / 2: in an even column
                 // for the words' low halves, in an odd one for the high ones
@@ -636,14 +661,12 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                 const unsigned char *v0 = sv + key_of(2 * c4) * C::kRowBytes + 4 * r8, *v1 = sv + key_of(2 * c4 + 1) * C::kRowBytes + 4 * r8;
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {
-                    const bool hidden = masked && key0 + 8 * n + mine >= sees[0];
                     const float p = tc::ex2(fmaf(t[n], low(crow), low(ref)));
                     l2 = tc::f2(low(l2) + p, 0.0f);
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
-                        // what a row does not see does not reach it: NaN scales neither
-                        const float w = hidden ? 0.0f : p * (bf_lo(raw[g][n].y) * unit[g]), zero = hidden ? 0.0f : bf_hi(raw[g][n].y);
-                        z2[g] = tc::f2(fmaf(p, zero, low(z2[g])), 0.0f);
+                        const float w = p * (bf_lo(raw[g][n].y) * unit[g]);
+                        z2[g] = tc::f2(fmaf(p, bf_hi(raw[g][n].y), low(z2[g])), 0.0f);
                         const uint32_t both = transpose8(pack_f16x2(w, w));
                         const uint32_t b0 = __byte_perm(both, 0, first), b1 = __byte_perm(both, 0, second);
                         const uint32_t x0 = *reinterpret_cast<const uint32_t *>(v0 + 8 * n * C::kRowBytes + 32 * g);
