@@ -14,8 +14,11 @@
 // comparison of two numbers: the rows' sums for it are 32-bit, and where u q and p are within
 // 2^-13 of one another, far above those sums' error, it is done again in 64 bits.
 //
-// One cluster takes a sequence, each of its warps a stretch of every row.
+// One cluster takes a sequence. Its warps share the rows out for the 32-bit sums, each some
+// contiguous part of one row at a time; in 64 bits each has a stretch of the vocabulary, whose
+// exponentials it keeps in shared memory where they fit (the search then reads them).
 #include <algorithm>
+#include <atomic>
 #include <cfloat>
 
 #include "logits.cuh"
@@ -24,9 +27,13 @@ namespace mom {
 
 namespace {
 
-constexpr int kWarps = 16, kThreads = kWarps * 32;
+constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr int kMostCtas = 8;
-constexpr int kHold = 4;            // vectors of a lane in flight
+constexpr int kHold = 4;            // vectors of a lane in flight, twice
+constexpr int kBatch = 8;           // elements of a lane in flight, of each row
+constexpr int kRounds = 9;          // parts of rows that a warp takes, at most: all rows, one CTA
+constexpr int kTableBits = 7, kTable = 1 << kTableBits;
+constexpr int kMostKeep = 8300;     // doubles that a CTA keeps, for three CTAs an SM
 
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
@@ -55,26 +62,42 @@ struct VerifyArgs {
     const float *uniforms;
     const int32_t *draft_lens;          // null: all K
     int V, K, ctas;
+    int keep;                           // elements of a CTA's stretch of a row that are kept, 0: none
     float c2;                           // log2(e) / T
-    double inv_t;
+    double scale;                       // kTable log2(e) / T
     int64_t *tokens, *accepted;
 };
 
 enum Verdict { kFalls, kStays, kUnsure, kBroken };
 
+// e^(d s / kTable ln 2) for d <= 0 in 64 bits, by table and polynomial (Tang, 1989): d s is
+// rounded to n, 2^(n mod kTable / kTable) comes from the table and the rest, within 1/2 of a
+// kTable-th, from a polynomial of degree 4: 1e-15 of the result, and |d s| 2^-53 / kTable more.
+__device__ __forceinline__ double exp_of(double d, double s, const double *table) {
+    constexpr double kMagic = 6755399441055744.0;      // 1.5 2^52: the sum's low bits are the rounded number
+    constexpr double kL = 0.69314718055994530942 / kTable;
+    const double t = fma(d, s, kMagic), f = fma(d, s, kMagic - t);
+    const int n = __double2loint(t);
+    double p = fma(f, kL * kL * kL * kL / 24, kL * kL * kL / 6);
+    p = fma(p, f, kL * kL / 2);
+    p = fma(p, f, kL) * f;
+    const double v = table[n & (kTable - 1)];
+    const double two = __hiloint2double(__double2hiint(v) + (n >> kTableBits << 20), __double2loint(v));
+    return d * s > -1000.0 * kTable ? fma(two, p, two) : 0.0;      // (NaN: 0; a row with one is not summed)
+}
+
 // Greedy: a row's greatest logit, ties to the lowest index. Own: the drafts have logits.
 template <int DT, bool Greedy, bool Own>
-__global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_constant__ VerifyArgs P) {
+__global__ void __launch_bounds__(kThreads, 3) verify_kernel(const __grid_constant__ VerifyArgs P) {
     using T = typename Elem<DT>::T;
     constexpr int kVE = RowSpan<DT>::kVE;
-    constexpr int kRows = 2 * kMaxDrafts + 1;
-    // of a row: the warps' greatest logit and sum (Greedy: rank key), then this CTA's
-    __shared__ uint64_t s_warp[kWarps][Greedy ? kMaxDrafts + 1 : kRows], s_cta[Greedy ? kMaxDrafts + 1 : kRows];
-    __shared__ float s_max[kRows];              // of the whole row
-    __shared__ float s_sum[kRows];
+    constexpr int kRows = Greedy || !Own ? kMaxDrafts + 1 : 2 * kMaxDrafts + 1;
+    extern __shared__ double s_keep[];          // a stretch's terms: of the target's row, then of the draft's
+    __shared__ uint64_t s_unit[kRounds][kWarps];      // the greatest logit and the sum (Greedy: rank key) of a part of a row
+    __shared__ uint64_t s_row[kRows];           // of whole rows
     __shared__ int s_verdict[kMaxDrafts];
     __shared__ double s_part[2][kWarps];        // the warps' sums in 64 bits, for the target and the draft
-    __shared__ double s_whole[2], s_left[kWarps], s_find[2];
+    __shared__ double s_whole[2], s_left[kWarps], s_find[2], s_table[kTable];
     __shared__ int s_owner;
     const int b = static_cast<int>(blockIdx.y), me = static_cast<int>(blockIdx.x), ctas = P.ctas;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -92,73 +115,17 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
         base = P.draft;
         return b * P.draft_ld_seq + (r - n - 1) * P.draft_ld_row;
     };
+    if constexpr (!Greedy)
+        if (threadIdx.x < kTable) s_table[threadIdx.x] = exp2(static_cast<double>(threadIdx.x) / kTable);
 
-    // ---- every row's greatest logit and sum, a stretch of it to each warp
-    for (int r = 0; r < rows; ++r) {
-        const void *base;
-        const int64_t off = place(r, base);
-        const RowSpan<DT> row(base, off, P.V);
-        const int v0 = static_cast<int>(static_cast<int64_t>(row.nvec) * w / W);
-        const int v1 = static_cast<int>(static_cast<int64_t>(row.nvec) * (w + 1) / W);
-        const int ex = w == 0 ? row.extra(lane) : -1;
-        const float x_extra = ex >= 0 ? logit<DT>(row.row, ex) : -INFINITY;
-        if constexpr (Greedy) {
-            uint64_t best = ex >= 0 ? rank_key(order_of(x_extra), ex) : 0;
-            for (int v = v0 + lane; v < v1; v += kHold * 32) {
-                uint4 d[kHold];
-#pragma unroll
-                for (int i = 0; i < kHold; ++i)
-                    if (v + 32 * i < v1) d[i] = __ldg(row.vec + v + 32 * i);
-#pragma unroll
-                for (int i = 0; i < kHold; ++i) {
-                    if (v + 32 * i >= v1 || order_of(vec_max<DT>(d[i])) < static_cast<uint32_t>(best >> 32)) continue;
-                    float x[kVE];
-                    unpack<DT>(d[i], x);
-#pragma unroll
-                    for (int e = 0; e < kVE; ++e)
-                        best = max(best, rank_key(order_of(x[e]), row.index(v + 32 * i, e)));
-                }
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-            if (lane == 0) s_warp[warp][r] = best;
-        } else {
-            float m = x_extra, ref = fmaxf(m, -FLT_MAX), s = ex >= 0 && x_extra > -INFINITY ? 1.0f : 0.0f;
-            for (int v = v0 + lane; v < v1; v += kHold * 32) {
-                uint4 d[kHold];
-                constexpr uint32_t none = DT == MOM_BF16 ? 0xff80ff80u : 0xff800000u;      // -inf adds nothing
-#pragma unroll
-                for (int i = 0; i < kHold; ++i) {
-                    d[i] = make_uint4(none, none, none, none);
-                    if (v + 32 * i < v1) d[i] = __ldg(row.vec + v + 32 * i);
-                }
-                float top = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < kHold; ++i) top = tc::fmax3_nan(top, top, vec_max<DT>(d[i]));
-                m = tc::fmax3_nan(m, m, top);
-                if (top > ref) {
-                    s *= tc::ex2((ref - top) * P.c2);
-                    ref = top;
-                }
-#pragma unroll
-                for (int i = 0; i < kHold; ++i) {
-                    float x[kVE], add = 0.0f;
-                    unpack<DT>(d[i], x);
-#pragma unroll
-                    for (int e = 0; e < kVE; ++e) add += tc::ex2((x[e] - ref) * P.c2);
-                    s += add;
-                }
-            }
-            float to = m;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) to = tc::fmax3_nan(to, to, __shfl_xor_sync(0xffffffffu, to, o));
-            s *= tc::ex2((ref - fmaxf(to, -FLT_MAX)) * P.c2);
-            s = mom::warp_sum(s);
-            if (lane == 0) s_warp[warp][r] = static_cast<uint64_t>(__float_as_uint(to)) << 32 | __float_as_uint(s);
-        }
+    // ---- every row's greatest logit and sum: parts of rows, as many as give each warp about the same
+    int parts = 1;
+    for (int rounds = 1; rounds <= 4; ++rounds) {
+        parts = max(rounds * W / rows, 1);
+        if (rows * parts * 8 >= rounds * W * 7) break;
     }
-    __syncthreads();
-    auto join = [&](uint64_t a, uint64_t c) {      // of two stretches
+    parts = min(parts, max(P.V / (64 * kVE), 1));
+    const auto join = [&](uint64_t a, uint64_t c) {      // of two parts
         if constexpr (Greedy) return max(a, c);
         const float ma = __uint_as_float(static_cast<uint32_t>(a >> 32)), mc = __uint_as_float(static_cast<uint32_t>(c >> 32));
         const float m = tc::fmax3_nan(ma, ma, mc), ref = fmaxf(m, -FLT_MAX);
@@ -166,22 +133,93 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
                         __uint_as_float(static_cast<uint32_t>(c)) * tc::ex2((fmaxf(mc, -FLT_MAX) - ref) * P.c2);
         return static_cast<uint64_t>(__float_as_uint(m)) << 32 | __float_as_uint(s);
     };
-    for (int r = threadIdx.x; r < rows; r += kThreads) {
-        uint64_t got = s_warp[0][r];
-        for (int i = 1; i < kWarps; ++i) got = join(got, s_warp[i][r]);
-        s_cta[r] = got;
+    const auto join_lanes = [&](uint64_t v) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v = join(v, __shfl_xor_sync(0xffffffffu, v, o));
+        return v;
+    };
+    constexpr uint64_t kNothing = Greedy ? 0 : static_cast<uint64_t>(0xff800000u) << 32;
+    for (int unit = w, round = 0; unit < rows * parts; unit += W, ++round) {
+        const int r = unit / parts, part = unit - r * parts;
+        const void *base;
+        const int64_t off = place(r, base);
+        const RowSpan<DT> row(base, off, P.V);
+        const int v1 = static_cast<int>(static_cast<int64_t>(row.nvec) * (part + 1) / parts);
+        int v = static_cast<int>(static_cast<int64_t>(row.nvec) * part / parts) + lane;
+        const int ex = part == 0 ? row.extra(lane) : -1;
+        const float x_extra = ex >= 0 ? logit<DT>(row.row, ex) : -INFINITY;
+        constexpr uint32_t none = DT == MOM_BF16 ? 0xff80ff80u : 0xff800000u;      // -inf adds nothing
+        const auto load = [&](uint4 (&d)[kHold], int at) {
+#pragma unroll
+            for (int i = 0; i < kHold; ++i) {
+                d[i] = make_uint4(none, none, none, none);
+                if (at + 32 * i < v1) d[i] = __ldg(row.vec + at + 32 * i);
+            }
+        };
+        uint64_t best = Greedy && ex >= 0 ? rank_key(order_of(x_extra), ex) : 0;
+        float m = x_extra, ref = fmaxf(m, -FLT_MAX);
+        uint64_t s2 = tc::f2(ex >= 0 && x_extra > -INFINITY ? 1.0f : 0.0f, 0.0f);
+        const uint64_t cc2 = tc::f2(P.c2, P.c2);
+        uint4 d[kHold];
+        load(d, v);
+        for (; v - lane < v1; v += kHold * 32) {
+            uint4 next[kHold];
+            load(next, v + kHold * 32);
+            if constexpr (Greedy) {
+#pragma unroll
+                for (int i = 0; i < kHold; ++i) {
+                    if (v + 32 * i >= v1 || order_of(vec_max<DT>(d[i])) < static_cast<uint32_t>(best >> 32)) continue;
+                    float x[kVE];
+                    unpack<DT>(d[i], x);
+#pragma unroll
+                    for (int e = 0; e < kVE; ++e) best = max(best, rank_key(order_of(x[e]), row.index(v + 32 * i, e)));
+                }
+            } else {
+                float top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < kHold; ++i) top = tc::fmax3_nan(top, top, vec_max<DT>(d[i]));
+                m = tc::fmax3_nan(m, m, top);
+                if (top > ref) {
+                    const float f = tc::ex2((ref - top) * P.c2);
+                    s2 = tc::mul2(s2, tc::f2(f, f));
+                    ref = top;
+                }
+                const uint64_t ref2 = tc::f2(ref, ref);
+#pragma unroll
+                for (int i = 0; i < kHold; ++i) {
+                    float x[kVE];
+                    unpack<DT>(d[i], x);
+#pragma unroll
+                    for (int e = 0; e < kVE; e += 2)
+                        s2 = tc::add2(s2, tc::ex2_pair(tc::mul2(tc::sub2(tc::f2(x[e], x[e + 1]), ref2), cc2)));
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kHold; ++i) d[i] = next[i];
+        }
+        if constexpr (!Greedy) {
+            float to = m;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) to = tc::fmax3_nan(to, to, __shfl_xor_sync(0xffffffffu, to, o));
+            const float2 s = tc::f2_split(s2);
+            const float all = mom::warp_sum((s.x + s.y) * tc::ex2((ref - fmaxf(to, -FLT_MAX)) * P.c2));
+            best = static_cast<uint64_t>(__float_as_uint(to)) << 32 | __float_as_uint(all);
+        } else {
+            best = join_lanes(best);
+        }
+        if (lane == 0) s_unit[round][warp] = best;
     }
     cluster_sync();
-    for (int r = threadIdx.x; r < rows; r += kThreads) {
-        uint64_t got = ld_cluster(&s_cta[r], 0);
-        for (int c = 1; c < ctas; ++c) got = join(got, ld_cluster(&s_cta[r], c));
-        if constexpr (Greedy) {
-            // the token, -1 for a row with a NaN
-            s_warp[0][r] = static_cast<uint32_t>(got >> 32) == 0xffffffffu ? ~0ull : static_cast<uint64_t>(rank_index(got));
-        } else {
-            s_max[r] = __uint_as_float(static_cast<uint32_t>(got >> 32));
-            s_sum[r] = __uint_as_float(static_cast<uint32_t>(got));
+    for (int r = warp; r < rows; r += kWarps) {
+        uint64_t got = kNothing;
+        for (int part = lane; part < parts; part += 32) {
+            const int unit = r * parts + part, of = unit % W;
+            got = join(got, ld_cluster(&s_unit[unit / W][of % kWarps], of / kWarps));
         }
+        got = join_lanes(got);
+        // Greedy: the token, -1 for a row with a NaN
+        if (Greedy) got = static_cast<uint32_t>(got >> 32) == 0xffffffffu ? ~0ull : static_cast<uint64_t>(rank_index(got));
+        if (lane == 0) s_row[r] = got;
     }
     __syncthreads();
 
@@ -194,201 +232,243 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
     if constexpr (Greedy) {
         if (me == 0) {
             int stay = 0;
-            while (stay < n && s_warp[0][stay] != ~0ull && drafts[stay] == static_cast<int64_t>(s_warp[0][stay])) ++stay;
+            while (stay < n && s_row[stay] != ~0ull && drafts[stay] == static_cast<int64_t>(s_row[stay])) ++stay;
             finish(stay);
-            if (threadIdx.x == 0) tokens[stay] = refused ? -1 : static_cast<int64_t>(s_warp[0][stay]);
+            if (threadIdx.x == 0) tokens[stay] = refused ? -1 : static_cast<int64_t>(s_row[stay]);
         }
         cluster_sync();      // nobody leaves while its part is read
         return;
-    }
-
-    // ---- 64 bits from here on: the terms of a row, the sums over the cluster
-    const int e0 = static_cast<int>(static_cast<int64_t>(P.V) * w / W), e1 = static_cast<int>(static_cast<int64_t>(P.V) * (w + 1) / W);
-    auto row_of = [&](int r) {
-        const void *base;
-        const int64_t off = place(r, base);
-        return static_cast<const T *>(base) + off;
-    };
-    auto term = [&](const T *row, float top, int i) {      // e^((x - top) / T)
-        return exp((static_cast<double>(Elem<DT>::load(row, i)) - static_cast<double>(top)) * P.inv_t);
-    };
-    // The sums of the target's row r (without its element `skip`) and, Own and r < n, of the draft's;
-    // the stretches' in s_part.
-    auto whole = [&](int r, int skip, bool both, double &zp, double &zq) {
-        const T *p = row_of(r), *q = both ? row_of(n + 1 + r) : nullptr;
-        const float mp = s_max[r], mq = both ? s_max[n + 1 + r] : 0.0f;
-        double a = 0.0, c = 0.0;
-#pragma unroll 4
-        for (int i = e0 + lane; i < e1; i += 32) {
-            if (i != skip) a += term(p, mp, i);
-            if (both) c += term(q, mq, i);
+    } else {
+        // ---- 64 bits from here on: the terms of a row, the sums over the cluster
+        const auto greatest = [&](int r) { return __uint_as_float(static_cast<uint32_t>(s_row[r] >> 32)); };
+        const auto sum_of = [&](int r) { return __uint_as_float(static_cast<uint32_t>(s_row[r])); };
+        const int c0 = static_cast<int>(static_cast<int64_t>(P.V) * me / ctas);      // this CTA's first element
+        const int e0 = static_cast<int>(static_cast<int64_t>(P.V) * w / W), e1 = static_cast<int>(static_cast<int64_t>(P.V) * (w + 1) / W);
+        auto row_of = [&](int r) {
+            const void *base;
+            const int64_t off = place(r, base);
+            return static_cast<const T *>(base) + off;
+        };
+        auto term = [&](float x, float top) {      // e^((x - top) / T)
+            return exp_of(static_cast<double>(x) - static_cast<double>(top), P.scale, s_table);
+        };
+        // The sums of the target's row r (without its element `skip`) and, both, of the draft's; the
+        // stretches' in s_part, the terms kept.
+        auto whole = [&](int r, int skip, bool both, double &zp, double &zq) {
+            const T *p = row_of(r), *q = both ? row_of(n + 1 + r) : p;
+            const float mp = greatest(r), mq = both ? greatest(n + 1 + r) : 0.0f;
+            double a = 0.0, c = 0.0;
+            for (int i = e0 + lane; i - lane < e1; i += 32 * kBatch) {
+                float x[kBatch], y[kBatch];
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k)
+                    if (i + 32 * k < e1) x[k] = Elem<DT>::load(p, i + 32 * k);
+                if (both) {
+#pragma unroll
+                    for (int k = 0; k < kBatch; ++k)
+                        if (i + 32 * k < e1) y[k] = Elem<DT>::load(q, i + 32 * k);
+                }
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) {
+                    const int at = i + 32 * k;
+                    if (at >= e1) break;
+                    const double e = at == skip ? 0.0 : term(x[k], mp);
+                    a += e;
+                    if (P.keep) s_keep[at - c0] = e;
+                    if (both) {
+                        const double f = term(y[k], mq);
+                        c += f;
+                        if (P.keep) s_keep[P.keep + at - c0] = f;
+                    }
+                }
+            }
+            a = warp_sum(a);
+            if (both) c = warp_sum(c);
+            if (lane == 0) s_part[0][warp] = a, s_part[1][warp] = c;
+            __syncthreads();
+            if (threadIdx.x < 2) {
+                double s = 0.0;
+#pragma unroll
+                for (int i = 0; i < kWarps; ++i) s += s_part[threadIdx.x][i];
+                s_whole[threadIdx.x] = s;
+            }
+            cluster_sync();
+            zp = zq = 0.0;
+#pragma unroll
+            for (int c2 = 0; c2 < kMostCtas; ++c2)
+                if (c2 < ctas) {
+                    zp += ld_cluster(&s_whole[0], c2);
+                    if (both) zq += ld_cluster(&s_whole[1], c2);
+                }
+        };
+        auto broken = [&](int r) { return !(greatest(r) < INFINITY) || greatest(r) == -INFINITY; };
+        auto chance = [&](int r, int64_t d, double z) {      // of token d in row r
+            return d >= 0 && d < P.V ? term(Elem<DT>::load(row_of(r), static_cast<int>(d)), greatest(r)) / z : 0.0;
+        };
+        const float *u = P.uniforms + static_cast<int64_t>(b) * (P.K + 1);
+        for (int j = threadIdx.x; j < n; j += kThreads) {
+            int v = kBroken;
+            const int64_t d = drafts[j];
+            if (!broken(j) && !(Own && broken(n + 1 + j))) {
+                const double p = chance(j, d, sum_of(j));
+                const double q = u[j] * (Own ? chance(n + 1 + j, d, sum_of(n + 1 + j)) : 1.0);
+                v = d >= 0 && d < P.V && q < p ? kStays : kFalls;
+                if (fabs(q - p) <= 0x1p-13 * fmax(fabs(q), p) && p > 0.0) v = kUnsure;
+            }
+            s_verdict[j] = v;
         }
-        a = warp_sum(a);
-        if (both) c = warp_sum(c);
-        if (lane == 0) s_part[0][warp] = a, s_part[1][warp] = c;
         __syncthreads();
-        if (threadIdx.x < 2) {
-            double s = 0.0;
-            for (int i = 0; i < kWarps; ++i) s += s_part[threadIdx.x][i];
-            s_whole[threadIdx.x] = s;
+        // all of the cluster's threads come to the same verdicts
+        int stay = 0, verdict = kStays;
+        double zp = 0.0, zq = 0.0;
+        for (; stay < n; ++stay) {
+            verdict = s_verdict[stay];
+            if (verdict == kUnsure) {
+                whole(stay, -1, Own, zp, zq);
+                const int64_t d = drafts[stay];
+                const double q = u[stay] * (Own ? chance(n + 1 + stay, d, zq) : 1.0);
+                verdict = q < chance(stay, d, zp) ? kStays : kFalls;
+                cluster_sync();      // the sums are read
+            }
+            if (verdict != kStays) break;
         }
-        cluster_sync();
-        zp = zq = 0.0;
-        for (int c2 = 0; c2 < ctas; ++c2) {
-            zp += ld_cluster(&s_whole[0], c2);
-            if (both) zq += ld_cluster(&s_whole[1], c2);
+        if (refused || broken(stay) || verdict == kBroken) {
+            if (me == 0) {
+                finish(stay);
+                if (threadIdx.x == 0) tokens[stay] = -1;
+            }
+            cluster_sync();
+            return;
         }
-    };
-    auto broken = [&](int r) { return !(s_max[r] < INFINITY) || s_max[r] == -INFINITY; };
-    auto chance = [&](int r, int64_t d, double z) {      // of token d in row r
-        return d >= 0 && d < P.V ? term(row_of(r), s_max[r], static_cast<int>(d)) / z : 0.0;
-    };
-    const float *u = P.uniforms + static_cast<int64_t>(b) * (P.K + 1);
-    for (int j = threadIdx.x; j < n; j += kThreads) {
-        int v = kBroken;
-        const int64_t d = drafts[j];
-        if (!broken(j) && !(Own && broken(n + 1 + j))) {
-            const double p = chance(j, d, s_sum[j]);
-            const double q = u[j] * (Own ? chance(n + 1 + j, d, s_sum[n + 1 + j]) : 1.0);
-            v = d >= 0 && d < P.V && q < p ? kStays : kFalls;
-            if (fabs(q - p) <= 0x1p-13 * fmax(fabs(q), p) && p > 0.0) v = kUnsure;
-        }
-        s_verdict[j] = v;
-    }
-    __syncthreads();
-    // all of the cluster's threads come to the same verdicts
-    int stay = 0, verdict = kStays;
-    double zp = 0.0, zq = 0.0;
-    for (; stay < n; ++stay) {
-        verdict = s_verdict[stay];
-        if (verdict == kUnsure) {
-            whole(stay, -1, Own, zp, zq);
-            const int64_t d = drafts[stay];
-            const double q = u[stay] * (Own ? chance(n + 1 + stay, d, zq) : 1.0);
-            verdict = q < chance(stay, d, zp) ? kStays : kFalls;
-            cluster_sync();      // the sums are read
-        }
-        if (verdict != kStays) break;
-    }
-    if (refused || broken(stay) || verdict == kBroken) {
-        if (me == 0) {
-            finish(stay);
-            if (threadIdx.x == 0) tokens[stay] = -1;
-        }
-        cluster_sync();
-        return;
-    }
-    const bool fell = stay < n;
-    const int64_t d = fell ? drafts[stay] : -1;
-    const T *p = row_of(stay), *q = Own && fell ? row_of(n + 1 + stay) : nullptr;
-    const float mp = s_max[stay], mq = q ? s_max[n + 1 + stay] : 0.0f;
-    int skip = !Own && fell && d >= 0 && d < P.V ? static_cast<int>(d) : -1;
-    bool both = q != nullptr;
-    whole(stay, skip, both, zp, zq);
-    double fp = 1.0, fq = 0.0;
-    if (both) fp = 1.0 / zp, fq = 1.0 / zq;
-    auto left = [&](int i) {      // what the token is drawn from
-        double v = i == skip ? 0.0 : term(p, mp, i) * fp;
-        if (both) v = fmax(v - term(q, mq, i) * fq, 0.0);
-        return v;
-    };
-    if (both) {
-        double a = 0.0;
+        const bool fell = stay < n;
+        const int64_t d = fell ? drafts[stay] : -1;
+        const T *p = row_of(stay), *q = Own && fell ? row_of(n + 1 + stay) : nullptr;
+        const float mp = greatest(stay), mq = q ? greatest(n + 1 + stay) : 0.0f;
+        int skip = !Own && fell && d >= 0 && d < P.V ? static_cast<int>(d) : -1;
+        bool both = q != nullptr;
+        whole(stay, skip, both, zp, zq);
+        double fp = 1.0, fq = 0.0;
+        if (both) fp = 1.0 / zp, fq = 1.0 / zq;
+        auto left = [&](int i) {      // what the token is drawn from
+            double v = P.keep ? s_keep[i - c0] : i == skip ? 0.0 : term(Elem<DT>::load(p, i), mp);
+            if (both) v = fmax(v * fp - (P.keep ? s_keep[P.keep + i - c0] : term(Elem<DT>::load(q, i), mq)) * fq, 0.0);
+            return v;
+        };
+        if (both) {
+            double a = 0.0;
 #pragma unroll 4
-        for (int i = e0 + lane; i < e1; i += 32) a += left(i);
-        a = warp_sum(a);
-        if (lane == 0) s_left[warp] = a;
-    } else if (lane == 0) {
-        s_left[warp] = s_part[0][warp];
-    }
-    cluster_sync();
-    // where the running sum passes u times the whole: among the cluster's stretches
-    auto find = [&]() {
-        if (warp == 0) {
-            // each lane takes neighbouring stretches
-            constexpr int kPer = kMostCtas * kWarps / 32;
-            const int per = (W + 31) / 32;
-            double x[kPer], mine = 0.0;
+            for (int i = e0 + lane; i < e1; i += 32) a += left(i);
+            a = warp_sum(a);
+            if (lane == 0) s_left[warp] = a;
+        } else if (lane == 0) {
+            s_left[warp] = s_part[0][warp];
+        }
+        cluster_sync();
+        // where the running sum passes u times the whole: among the cluster's stretches
+        auto find = [&]() {
+            if (warp == 0) {
+                // each lane takes neighbouring stretches
+                constexpr int kPer = kMostCtas * kWarps / 32;
+                const int per = (W + 31) / 32;
+                double x[kPer], mine = 0.0;
 #pragma unroll
-            for (int k = 0; k < kPer; ++k) {
-                const int i = lane * per + k;
-                x[k] = k < per && i < W ? ld_cluster(&s_left[i % kWarps], i / kWarps) : 0.0;
-            }
-#pragma unroll
-            for (int k = 0; k < kPer; ++k) mine += x[k];
-            double upto = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double y = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += y;
-            }
-            const double goal = u[P.K] * __shfl_sync(0xffffffffu, upto, 31);
-            const uint32_t some = __ballot_sync(0xffffffffu, mine > 0.0);
-            const uint32_t past = __ballot_sync(0xffffffffu, mine > 0.0 && upto > goal);
-            if (lane == 0) s_owner = -1;
-            __syncwarp();
-            // u at or above 1, or its last bit: the last stretch with anything
-            if (some && lane == (past ? __ffs(past) - 1 : 31 - __clz(some))) {
-                double run = upto - mine;
                 for (int k = 0; k < kPer; ++k) {
-                    if (x[k] > 0.0) {
-                        s_owner = lane * per + k;
-                        s_find[0] = goal;
-                        s_find[1] = run;
-                        if (run + x[k] > goal) break;
-                    }
-                    run += x[k];
+                    const int i = lane * per + k;
+                    x[k] = k < per && i < W ? ld_cluster(&s_left[i % kWarps], i / kWarps) : 0.0;
                 }
-            }
-        }
-        __syncthreads();
-    };
-    find();
-    if (s_owner < 0) {
-        // nothing is left (the draft's distribution is the target's): from the target's own
-        skip = -1, both = false, fp = 1.0;
-        cluster_sync();      // the sums are read
-        double z0, z1;
-        whole(stay, -1, false, z0, z1);
-        if (lane == 0) s_left[warp] = s_part[0][warp];
-        cluster_sync();
-        find();
-    }
-    const int owner = s_owner;
-    if (owner / kWarps == me) {
-        finish(stay);
-        if (owner % kWarps == warp) {
-            // the owner's lanes take neighbouring elements each
-            const int per = (e1 - e0 + 31) / 32, i0 = min(e0 + lane * per, e1), i1 = min(i0 + per, e1);
-            double mine = 0.0;
-            for (int i = i0; i < i1; ++i) mine += left(i);
-            double upto = mine;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double x = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += x;
-            }
-            const double goal = s_find[0];
-            upto += s_find[1];
-            const uint32_t some = __ballot_sync(0xffffffffu, mine > 0.0);
-            uint32_t past = __ballot_sync(0xffffffffu, mine > 0.0 && upto > goal);
-            if (!past) past = 1u << (31 - __clz(some));
-            if (lane == __ffs(past) - 1) {
-                double run = upto - mine;
-                int at = -1;
-                for (int i = i0; i < i1; ++i) {
-                    const double x = left(i);
-                    run += x;
-                    if (x > 0.0) {
-                        at = i;
-                        if (run > goal) break;
+                for (int k = 0; k < kPer; ++k) mine += x[k];
+                double upto = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const double y = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += y;
+                }
+                const double goal = u[P.K] * __shfl_sync(0xffffffffu, upto, 31);
+                const uint32_t some = __ballot_sync(0xffffffffu, mine > 0.0);
+                const uint32_t past = __ballot_sync(0xffffffffu, mine > 0.0 && upto > goal);
+                if (lane == 0) s_owner = -1;
+                __syncwarp();
+                // u at or above 1, or its last bit: the last stretch with anything
+                if (some && lane == (past ? __ffs(past) - 1 : 31 - __clz(some))) {
+                    double run = upto - mine;
+                    for (int k = 0; k < kPer; ++k) {
+                        if (x[k] > 0.0) {
+                            s_owner = lane * per + k;
+                            s_find[0] = goal;
+                            s_find[1] = run;
+                            if (run + x[k] > goal) break;
+                        }
+                        run += x[k];
                     }
                 }
-                tokens[stay] = at;
+            }
+            __syncthreads();
+        };
+        find();
+        if (s_owner < 0) {
+            // nothing is left (the draft's distribution is the target's): from the target's own
+            skip = -1, both = false;
+            cluster_sync();      // the sums are read
+            double z0, z1;
+            whole(stay, -1, false, z0, z1);
+            if (lane == 0) s_left[warp] = s_part[0][warp];
+            cluster_sync();
+            find();
+        }
+        const int owner = s_owner;
+        if (owner / kWarps == me) {
+            finish(stay);
+            if (owner % kWarps == warp) {
+                // the owner's lanes take neighbouring elements each
+                const int per = (e1 - e0 + 31) / 32, i0 = min(e0 + lane * per, e1), i1 = min(i0 + per, e1);
+                double mine = 0.0;
+#pragma unroll 4
+                for (int i = i0; i < i1; ++i) mine += left(i);
+                double upto = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const double x = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += x;
+                }
+                const double goal = s_find[0];
+                upto += s_find[1];
+                const uint32_t some = __ballot_sync(0xffffffffu, mine > 0.0);
+                uint32_t past = __ballot_sync(0xffffffffu, mine > 0.0 && upto > goal);
+                if (!past) past = 1u << (31 - __clz(some));
+                if (lane == __ffs(past) - 1) {
+                    double run = upto - mine;
+                    int at = -1;
+                    for (int i = i0; i < i1; ++i) {
+                        const double x = left(i);
+                        run += x;
+                        if (x > 0.0) {
+                            at = i;
+                            if (run > goal) break;
+                        }
+                    }
+                    tokens[stay] = at;
+                }
             }
         }
+        cluster_sync();      // nobody leaves while its sums are read
     }
-    cluster_sync();      // nobody leaves while its sums are read
+}
+
+template <int DT, bool Greedy, bool Own>
+cudaError_t launch(cudaLaunchConfig_t &cfg, const VerifyArgs &p) {
+    static std::atomic<uint64_t> ready{0};      // devices whose kernel has its shared memory set
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+        e = cudaFuncSetAttribute(verify_kernel<DT, Greedy, Own>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostKeep * 8);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+    }
+    e = cudaLaunchKernelEx(&cfg, verify_kernel<DT, Greedy, Own>, p);
+    count_launch();
+    return e;
 }
 
 }  // namespace
@@ -410,13 +490,16 @@ cudaError_t launch_verify_drafts(const void *logits, int dt, int64_t ld_seq, int
     p.V = V;
     p.K = K;
     const bool greedy = temperature == 0.0;
-    p.inv_t = greedy ? 1.0 : 1.0 / temperature;
-    p.c2 = static_cast<float>(p.inv_t * 1.4426950408889634);
+    const double per = greedy ? 1.0 : 1.4426950408889634 / temperature;
+    p.c2 = static_cast<float>(per);
+    p.scale = kTable * per;
     p.tokens = tokens;
     p.accepted = accepted;
     // as many CTAs a sequence as fit the GPU with those of all sequences
     p.ctas = kMostCtas;
-    while (p.ctas > 1 && B * p.ctas > 2 * device_sm_count()) p.ctas /= 2;
+    while (p.ctas > 1 && B * p.ctas > 3 * device_sm_count()) p.ctas /= 2;
+    const int keep = (V + p.ctas - 1) / p.ctas + 1;
+    if (!greedy && static_cast<int64_t>(keep) * (draft ? 2 : 1) <= kMostKeep) p.keep = keep;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -424,19 +507,15 @@ cudaError_t launch_verify_drafts(const void *logits, int dt, int64_t ld_seq, int
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.gridDim = dim3(static_cast<unsigned>(p.ctas), static_cast<unsigned>(B));
     cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = static_cast<size_t>(p.keep) * (draft ? 2 : 1) * sizeof(double);
     cfg.stream = st;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    auto go = [&](auto kernel) { return cudaLaunchKernelEx(&cfg, kernel, p); };
-    cudaError_t e;
     if (dt == MOM_BF16)
-        e = greedy ? go(verify_kernel<MOM_BF16, true, false>)
-                   : draft ? go(verify_kernel<MOM_BF16, false, true>) : go(verify_kernel<MOM_BF16, false, false>);
-    else
-        e = greedy ? go(verify_kernel<MOM_F32, true, false>)
-                   : draft ? go(verify_kernel<MOM_F32, false, true>) : go(verify_kernel<MOM_F32, false, false>);
-    count_launch();
-    return e;
+        return greedy ? launch<MOM_BF16, true, false>(cfg, p)
+                      : draft ? launch<MOM_BF16, false, true>(cfg, p) : launch<MOM_BF16, false, false>(cfg, p);
+    return greedy ? launch<MOM_F32, true, false>(cfg, p)
+                  : draft ? launch<MOM_F32, false, true>(cfg, p) : launch<MOM_F32, false, false>(cfg, p);
 }
 
 }  // namespace mom
