@@ -83,7 +83,7 @@ __device__ __forceinline__ double exp_of(double d, double s, const double *table
     p = fma(p, f, kL) * f;
     const double v = table[n & (kTable - 1)];
     const double two = __hiloint2double(__double2hiint(v) + (n >> kTableBits << 20), __double2loint(v));
-    return d * s > -1000.0 * kTable ? fma(two, p, two) : 0.0;      // (NaN: 0; a row with one is not summed)
+    return d * s > -1020.0 * kTable ? fma(two, p, two) : 0.0;      // (NaN: 0; a row with one is not summed)
 }
 
 // Greedy: a row's greatest logit, ties to the lowest index. Own: the drafts have logits.
@@ -115,6 +115,27 @@ __global__ void __launch_bounds__(kThreads, 3) verify_kernel(const __grid_consta
         base = P.draft;
         return b * P.draft_ld_seq + (r - n - 1) * P.draft_ld_row;
     };
+    // what a draft's test needs, on its way while the rows are summed
+    float given_u = 0.0f, last_u = 0.0f, draft_p = -INFINITY, draft_q = -INFINITY;
+    int64_t draft = -1;
+    if constexpr (!Greedy) {
+        const float *u = P.uniforms + static_cast<int64_t>(b) * (P.K + 1);
+        last_u = u[P.K];
+        const int j = static_cast<int>(threadIdx.x);
+        if (j < n) {
+            given_u = u[j];
+            draft = drafts[j];
+            if (draft >= 0 && draft < P.V) {
+                const void *base;
+                int64_t off = place(j, base);
+                draft_p = logit<DT>(base, off + draft);
+                if (Own) {
+                    off = place(n + 1 + j, base);
+                    draft_q = logit<DT>(base, off + draft);
+                }
+            }
+        }
+    }
     if constexpr (!Greedy)
         if (threadIdx.x < kTable) s_table[threadIdx.x] = exp2(static_cast<double>(threadIdx.x) / kTable);
 
@@ -258,29 +279,31 @@ __global__ void __launch_bounds__(kThreads, 3) verify_kernel(const __grid_consta
             const T *p = row_of(r), *q = both ? row_of(n + 1 + r) : p;
             const float mp = greatest(r), mq = both ? greatest(n + 1 + r) : 0.0f;
             double a = 0.0, c = 0.0;
-            for (int i = e0 + lane; i - lane < e1; i += 32 * kBatch) {
-                float x[kBatch], y[kBatch];
-#pragma unroll
-                for (int k = 0; k < kBatch; ++k)
-                    if (i + 32 * k < e1) x[k] = Elem<DT>::load(p, i + 32 * k);
-                if (both) {
-#pragma unroll
-                    for (int k = 0; k < kBatch; ++k)
-                        if (i + 32 * k < e1) y[k] = Elem<DT>::load(q, i + 32 * k);
-                }
+            // the terms of a batch side by side: each is a chain of a dozen operations
+            const auto batch = [&](const T *row, float top, int without, int i, double &sum, int keep_at) {
+                float x[kBatch];
+                double e[kBatch];
 #pragma unroll
                 for (int k = 0; k < kBatch; ++k) {
                     const int at = i + 32 * k;
-                    if (at >= e1) break;
-                    const double e = at == skip ? 0.0 : term(x[k], mp);
-                    a += e;
-                    if (P.keep) s_keep[at - c0] = e;
-                    if (both) {
-                        const double f = term(y[k], mq);
-                        c += f;
-                        if (P.keep) s_keep[P.keep + at - c0] = f;
-                    }
+                    x[k] = at < e1 && at != without ? Elem<DT>::load(row, at) : -INFINITY;
                 }
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) e[k] = term(x[k], top);
+                if (P.keep) {
+#pragma unroll
+                    for (int k = 0; k < kBatch; ++k)
+                        if (i + 32 * k < e1) s_keep[keep_at + i + 32 * k - c0] = e[k];
+                }
+#pragma unroll
+                for (int o = kBatch / 2; o > 0; o >>= 1)
+#pragma unroll
+                    for (int k = 0; k < o; ++k) e[k] += e[k + o];
+                sum += e[0];
+            };
+            for (int i = e0 + lane; i - lane < e1; i += 32 * kBatch) {
+                batch(p, mp, skip, i, a, 0);
+                if (both) batch(q, mq, -1, i, c, P.keep);
             }
             a = warp_sum(a);
             if (both) c = warp_sum(c);
@@ -302,18 +325,22 @@ __global__ void __launch_bounds__(kThreads, 3) verify_kernel(const __grid_consta
                 }
         };
         auto broken = [&](int r) { return !(greatest(r) < INFINITY) || greatest(r) == -INFINITY; };
-        auto chance = [&](int r, int64_t d, double z) {      // of token d in row r
-            return d >= 0 && d < P.V ? term(Elem<DT>::load(row_of(r), static_cast<int>(d)), greatest(r)) / z : 0.0;
+        // a draft's test: u q < p, and (32 bits) whether the two are too near one another
+        auto test = [&](float u, float xp, float xq, int r, double zp, double zq, bool &near) {
+            const double p = term(xp, greatest(r)), q = u * (Own ? term(xq, greatest(n + 1 + r)) : 1.0);      // times z
+            const double l = q * zp, m = Own ? p * zq : p;
+            near = fabs(l - m) <= 0x1p-13 * fmax(fabs(l), m) && m > 0.0;
+            return l < m ? kStays : kFalls;
         };
-        const float *u = P.uniforms + static_cast<int64_t>(b) * (P.K + 1);
-        for (int j = threadIdx.x; j < n; j += kThreads) {
+        if (static_cast<int>(threadIdx.x) < n) {
+            const int j = static_cast<int>(threadIdx.x);
             int v = kBroken;
-            const int64_t d = drafts[j];
             if (!broken(j) && !(Own && broken(n + 1 + j))) {
-                const double p = chance(j, d, sum_of(j));
-                const double q = u[j] * (Own ? chance(n + 1 + j, d, sum_of(n + 1 + j)) : 1.0);
-                v = d >= 0 && d < P.V && q < p ? kStays : kFalls;
-                if (fabs(q - p) <= 0x1p-13 * fmax(fabs(q), p) && p > 0.0) v = kUnsure;
+                v = kFalls;      // outside the vocabulary
+                bool near = false;
+                if (draft >= 0 && draft < P.V)
+                    v = test(given_u, draft_p, draft_q, j, sum_of(j), Own ? sum_of(n + 1 + j) : 1.0f, near);
+                if (near) v = kUnsure;
             }
             s_verdict[j] = v;
         }
@@ -325,9 +352,11 @@ __global__ void __launch_bounds__(kThreads, 3) verify_kernel(const __grid_consta
             verdict = s_verdict[stay];
             if (verdict == kUnsure) {
                 whole(stay, -1, Own, zp, zq);
-                const int64_t d = drafts[stay];
-                const double q = u[stay] * (Own ? chance(n + 1 + stay, d, zq) : 1.0);
-                verdict = q < chance(stay, d, zp) ? kStays : kFalls;
+                const int64_t d = drafts[stay];      // in the vocabulary
+                const float u = P.uniforms[static_cast<int64_t>(b) * (P.K + 1) + stay];
+                bool near;
+                verdict = test(u, Elem<DT>::load(row_of(stay), d), Own ? Elem<DT>::load(row_of(n + 1 + stay), d) : 0.0f, stay, zp,
+                               zq, near);
                 cluster_sync();      // the sums are read
             }
             if (verdict != kStays) break;
@@ -341,10 +370,10 @@ __global__ void __launch_bounds__(kThreads, 3) verify_kernel(const __grid_consta
             return;
         }
         const bool fell = stay < n;
-        const int64_t d = fell ? drafts[stay] : -1;
+        const int64_t d = fell && !Own ? drafts[stay] : -1;
         const T *p = row_of(stay), *q = Own && fell ? row_of(n + 1 + stay) : nullptr;
         const float mp = greatest(stay), mq = q ? greatest(n + 1 + stay) : 0.0f;
-        int skip = !Own && fell && d >= 0 && d < P.V ? static_cast<int>(d) : -1;
+        int skip = d >= 0 && d < P.V ? static_cast<int>(d) : -1;
         bool both = q != nullptr;
         whole(stay, skip, both, zp, zq);
         double fp = 1.0, fq = 0.0;
@@ -356,10 +385,15 @@ __global__ void __launch_bounds__(kThreads, 3) verify_kernel(const __grid_consta
         };
         if (both) {
             double a = 0.0;
-#pragma unroll 4
-            for (int i = e0 + lane; i < e1; i += 32) a += left(i);
+#pragma unroll 8
+            for (int i = e0 + lane; i < e1; i += 32) {
+                const double x = left(i);
+                a += x;
+                if (P.keep) s_keep[i - c0] = x;
+            }
             a = warp_sum(a);
             if (lane == 0) s_left[warp] = a;
+            if (P.keep) both = false, fp = 1.0;      // s_keep has it from here on
         } else if (lane == 0) {
             s_left[warp] = s_part[0][warp];
         }
@@ -384,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 3) verify_kernel(const __grid_consta
                     const double y = __shfl_up_sync(0xffffffffu, upto, o);
                     if (lane >= o) upto += y;
                 }
-                const double goal = u[P.K] * __shfl_sync(0xffffffffu, upto, 31);
+                const double goal = last_u * __shfl_sync(0xffffffffu, upto, 31);
                 const uint32_t some = __ballot_sync(0xffffffffu, mine > 0.0);
                 const uint32_t past = __ballot_sync(0xffffffffu, mine > 0.0 && upto > goal);
                 if (lane == 0) s_owner = -1;
@@ -408,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 3) verify_kernel(const __grid_consta
         find();
         if (s_owner < 0) {
             // nothing is left (the draft's distribution is the target's): from the target's own
-            skip = -1, both = false;
+            skip = -1, both = false, fp = 1.0;
             cluster_sync();      // the sums are read
             double z0, z1;
             whole(stay, -1, false, z0, z1);
@@ -436,19 +470,26 @@ __global__ void __launch_bounds__(kThreads, 3) verify_kernel(const __grid_consta
                 const uint32_t some = __ballot_sync(0xffffffffu, mine > 0.0);
                 uint32_t past = __ballot_sync(0xffffffffu, mine > 0.0 && upto > goal);
                 if (!past) past = 1u << (31 - __clz(some));
-                if (lane == __ffs(past) - 1) {
-                    double run = upto - mine;
-                    int at = -1;
-                    for (int i = i0; i < i1; ++i) {
-                        const double x = left(i);
-                        run += x;
-                        if (x > 0.0) {
-                            at = i;
-                            if (run > goal) break;
-                        }
+                // that lane's elements, one to each lane in turn
+                const int of = __ffs(past) - 1;
+                double run = __shfl_sync(0xffffffffu, upto - mine, of);
+                const int f0 = __shfl_sync(0xffffffffu, i0, of), f1 = __shfl_sync(0xffffffffu, i1, of);
+                int at = -1;
+                for (int i = f0; i < f1; i += 32) {
+                    const double x = i + lane < f1 ? left(i + lane) : 0.0;
+                    double sum = x;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const double y = __shfl_up_sync(0xffffffffu, sum, o);
+                        if (lane >= o) sum += y;
                     }
-                    tokens[stay] = at;
+                    const uint32_t any = __ballot_sync(0xffffffffu, x > 0.0);
+                    const uint32_t over = __ballot_sync(0xffffffffu, x > 0.0 && run + sum > goal);
+                    if (any) at = i + (over ? __ffs(over) - 1 : 31 - __clz(any));
+                    if (over) break;
+                    run += __shfl_sync(0xffffffffu, sum, 31);
                 }
+                if (lane == 0) tokens[stay] = at;
             }
         }
         cluster_sync();      // nobody leaves while its sums are read
@@ -497,7 +538,7 @@ cudaError_t launch_verify_drafts(const void *logits, int dt, int64_t ld_seq, int
     p.accepted = accepted;
     // as many CTAs a sequence as fit the GPU with those of all sequences
     p.ctas = kMostCtas;
-    while (p.ctas > 1 && B * p.ctas > 3 * device_sm_count()) p.ctas /= 2;
+    while (p.ctas > 1 && B * p.ctas > (greedy ? 4 : 3) * device_sm_count()) p.ctas /= 2;
     const int keep = (V + p.ctas - 1) / p.ctas + 1;
     if (!greedy && static_cast<int64_t>(keep) * (draft ? 2 : 1) <= kMostKeep) p.keep = keep;
     cudaLaunchConfig_t cfg = {};
