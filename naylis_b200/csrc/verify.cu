@@ -28,7 +28,7 @@ namespace mom {
 namespace {
 
 constexpr int kWarps = 8, kThreads = kWarps * 32;
-constexpr int kMostCtas = 8;
+constexpr int kMostCtas = 16;      // of a cluster: 16 where there are few sequences, else 8 at most
 constexpr int kHold = 4;            // vectors of a lane in flight, twice
 constexpr int kBatch = 8;           // elements of a lane in flight, of each row
 constexpr int kRounds = 9;          // parts of rows that a warp takes, at most: all rows, one CTA
@@ -86,9 +86,17 @@ __device__ __forceinline__ double exp_of(double d, double s, const double *table
     return d * s > -1020.0 * kTable ? fma(two, p, two) : 0.0;      // (NaN: 0; a row with one is not summed)
 }
 
+__device__ __forceinline__ double sum_of_batch(double (&e)[kBatch]) {
+#pragma unroll
+    for (int o = kBatch / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < o; ++k) e[k] += e[k + o];
+    return e[0];
+}
+
 // Greedy: a row's greatest logit, ties to the lowest index. Own: the drafts have logits.
 template <int DT, bool Greedy, bool Own>
-__global__ void __launch_bounds__(kThreads, 3) verify_kernel(const __grid_constant__ VerifyArgs P) {
+__global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const __grid_constant__ VerifyArgs P) {
     using T = typename Elem<DT>::T;
     constexpr int kVE = RowSpan<DT>::kVE;
     constexpr int kRows = Greedy || !Own ? kMaxDrafts + 1 : 2 * kMaxDrafts + 1;
@@ -178,6 +186,9 @@ __global__ void __launch_bounds__(kThreads, 3) verify_kernel(const __grid_consta
             }
         };
         uint64_t best = Greedy && ex >= 0 ? rank_key(order_of(x_extra), ex) : 0;
+        // Greedy: the first of the greatest vectors, NaN left out; which element it is comes behind the loop
+        float great = -INFINITY;
+        int at = v < v1 ? v : -1;
         float m = x_extra, ref = fmaxf(m, -FLT_MAX);
         uint64_t s2 = tc::f2(ex >= 0 && x_extra > -INFINITY ? 1.0f : 0.0f, 0.0f);
         const uint64_t cc2 = tc::f2(P.c2, P.c2);
@@ -189,11 +200,9 @@ __global__ void __launch_bounds__(kThreads, 3) verify_kernel(const __grid_consta
             if constexpr (Greedy) {
 #pragma unroll
                 for (int i = 0; i < kHold; ++i) {
-                    if (v + 32 * i >= v1 || order_of(vec_max<DT>(d[i])) < static_cast<uint32_t>(best >> 32)) continue;
-                    float x[kVE];
-                    unpack<DT>(d[i], x);
-#pragma unroll
-                    for (int e = 0; e < kVE; ++e) best = max(best, rank_key(order_of(x[e]), row.index(v + 32 * i, e)));
+                    const float x = vec_max<DT>(d[i]);
+                    m = tc::fmax3_nan(m, m, x);
+                    if (x > great) great = x, at = v + 32 * i;
                 }
             } else {
                 float top = -INFINITY;
@@ -226,6 +235,16 @@ __global__ void __launch_bounds__(kThreads, 3) verify_kernel(const __grid_consta
             const float all = mom::warp_sum((s.x + s.y) * tc::ex2((ref - fmaxf(to, -FLT_MAX)) * P.c2));
             best = static_cast<uint64_t>(__float_as_uint(to)) << 32 | __float_as_uint(all);
         } else {
+            if (at >= 0) {
+                float x[kVE];
+                unpack<DT>(__ldg(row.vec + at), x);
+                int e = 0;
+#pragma unroll
+                for (int i = kVE - 1; i >= 0; --i)
+                    if (x[i] == great) e = i;
+                best = max(best, rank_key(order_of(great), row.index(at, e)));
+            }
+            if (m != m) best = rank_key(order_of(m), 0);      // a NaN
             best = join_lanes(best);
         }
         if (lane == 0) s_unit[round][warp] = best;
@@ -279,31 +298,31 @@ __global__ void __launch_bounds__(kThreads, 3) verify_kernel(const __grid_consta
             const T *p = row_of(r), *q = both ? row_of(n + 1 + r) : p;
             const float mp = greatest(r), mq = both ? greatest(n + 1 + r) : 0.0f;
             double a = 0.0, c = 0.0;
-            // the terms of a batch side by side: each is a chain of a dozen operations
-            const auto batch = [&](const T *row, float top, int without, int i, double &sum, int keep_at) {
-                float x[kBatch];
-                double e[kBatch];
+            // a batch of both rows on its way together, and its terms side by side: each is a chain of a dozen operations
+            const auto fetch = [&](float (&x)[kBatch], const T *row, int i, int without) {
 #pragma unroll
                 for (int k = 0; k < kBatch; ++k) {
                     const int at = i + 32 * k;
                     x[k] = at < e1 && at != without ? Elem<DT>::load(row, at) : -INFINITY;
                 }
+            };
+            const auto batch = [&](const float (&x)[kBatch], float top, int i, double *keep) {
+                double e[kBatch];
 #pragma unroll
                 for (int k = 0; k < kBatch; ++k) e[k] = term(x[k], top);
                 if (P.keep) {
 #pragma unroll
                     for (int k = 0; k < kBatch; ++k)
-                        if (i + 32 * k < e1) s_keep[keep_at + i + 32 * k - c0] = e[k];
+                        if (i + 32 * k < e1) keep[i + 32 * k - c0] = e[k];
                 }
-#pragma unroll
-                for (int o = kBatch / 2; o > 0; o >>= 1)
-#pragma unroll
-                    for (int k = 0; k < o; ++k) e[k] += e[k + o];
-                sum += e[0];
+                return sum_of_batch(e);
             };
             for (int i = e0 + lane; i - lane < e1; i += 32 * kBatch) {
-                batch(p, mp, skip, i, a, 0);
-                if (both) batch(q, mq, -1, i, c, P.keep);
+                float x[kBatch], y[kBatch];
+                fetch(x, p, i, skip);
+                if (both) fetch(y, q, i, -1);
+                a += batch(x, mp, i, s_keep);
+                if (both) c += batch(y, mq, i, s_keep + P.keep);
             }
             a = warp_sum(a);
             if (both) c = warp_sum(c);
@@ -385,11 +404,16 @@ __global__ void __launch_bounds__(kThreads, 3) verify_kernel(const __grid_consta
         };
         if (both) {
             double a = 0.0;
-#pragma unroll 8
-            for (int i = e0 + lane; i < e1; i += 32) {
-                const double x = left(i);
-                a += x;
-                if (P.keep) s_keep[i - c0] = x;
+            for (int i = e0 + lane; i - lane < e1; i += 32 * kBatch) {
+                double e[kBatch];
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) e[k] = i + 32 * k < e1 ? left(i + 32 * k) : 0.0;
+                if (P.keep) {
+#pragma unroll
+                    for (int k = 0; k < kBatch; ++k)
+                        if (i + 32 * k < e1) s_keep[i + 32 * k - c0] = e[k];
+                }
+                a += sum_of_batch(e);
             }
             a = warp_sum(a);
             if (lane == 0) s_left[warp] = a;
@@ -454,11 +478,15 @@ __global__ void __launch_bounds__(kThreads, 3) verify_kernel(const __grid_consta
         if (owner / kWarps == me) {
             finish(stay);
             if (owner % kWarps == warp) {
-                // the owner's lanes take neighbouring elements each
-                const int per = (e1 - e0 + 31) / 32, i0 = min(e0 + lane * per, e1), i1 = min(i0 + per, e1);
+                // the owner's lanes take neighbouring elements each, an odd number of them: no bank conflicts
+                const int per = (e1 - e0 + 31) / 32 | 1, i0 = min(e0 + lane * per, e1), i1 = min(i0 + per, e1);
                 double mine = 0.0;
-#pragma unroll 4
-                for (int i = i0; i < i1; ++i) mine += left(i);
+                for (int i = i0; i < i1; i += kBatch) {
+                    double e[kBatch];
+#pragma unroll
+                    for (int k = 0; k < kBatch; ++k) e[k] = i + k < i1 ? left(i + k) : 0.0;
+                    mine += sum_of_batch(e);
+                }
                 double upto = mine;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -504,6 +532,8 @@ cudaError_t launch(cudaLaunchConfig_t &cfg, const VerifyArgs &p) {
     if (e != cudaSuccess) return e;
     if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
         e = cudaFuncSetAttribute(verify_kernel<DT, Greedy, Own>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostKeep * 8);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(verify_kernel<DT, Greedy, Own>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
         if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
     }
@@ -537,7 +567,7 @@ cudaError_t launch_verify_drafts(const void *logits, int dt, int64_t ld_seq, int
     p.tokens = tokens;
     p.accepted = accepted;
     // as many CTAs a sequence as fit the GPU with those of all sequences
-    p.ctas = kMostCtas;
+    p.ctas = B <= 8 ? kMostCtas : 8;
     while (p.ctas > 1 && B * p.ctas > (greedy ? 4 : 3) * device_sm_count()) p.ctas /= 2;
     const int keep = (V + p.ctas - 1) / p.ctas + 1;
     if (!greedy && static_cast<int64_t>(keep) * (draft ? 2 : 1) <= kMostKeep) p.keep = keep;
