@@ -86,6 +86,12 @@ __device__ __forceinline__ double exp_of(double d, double s, const double *table
     return d * s > -1020.0 * kTable ? fma(two, p, two) : 0.0;      // (NaN: 0; a row with one is not summed)
 }
 
+// x in 64 bits by integer operations (the conversion has a twelfth of their rate). Zeros and
+// subnormals become 2^-127 and a little more, infinities 2^128: below and above whatever matters here.
+__device__ __forceinline__ double wide(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return __hiloint2double(static_cast<int>((b & 0x80000000u) | ((b & 0x7fffffffu) >> 3) + 0x38000000u), static_cast<int>(b << 29));
+}
 __device__ __forceinline__ double sum_of_batch(double (&e)[kBatch]) {
 #pragma unroll
     for (int o = kBatch / 2; o > 0; o >>= 1)
@@ -290,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const 
             return static_cast<const T *>(base) + off;
         };
         auto term = [&](float x, float top) {      // e^((x - top) / T)
-            return exp_of(static_cast<double>(x) - static_cast<double>(top), P.scale, s_table);
+            return exp_of(wide(x) - wide(top), P.scale, s_table);
         };
         // The sums of the target's row r (without its element `skip`) and, both, of the draft's; the
         // stretches' in s_part, the terms kept.
@@ -335,13 +341,11 @@ __global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const 
                 s_whole[threadIdx.x] = s;
             }
             cluster_sync();
-            zp = zq = 0.0;
-#pragma unroll
-            for (int c2 = 0; c2 < kMostCtas; ++c2)
-                if (c2 < ctas) {
-                    zp += ld_cluster(&s_whole[0], c2);
-                    if (both) zq += ld_cluster(&s_whole[1], c2);
-                }
+            // all CTAs' sums by the lanes at once, then the same sum in each
+            const double x = lane < ctas ? ld_cluster(&s_whole[0], lane) : 0.0;
+            const double y = both && lane < ctas ? ld_cluster(&s_whole[1], lane) : 0.0;
+            zp = warp_sum(x);
+            zq = both ? warp_sum(y) : 0.0;
         };
         auto broken = [&](int r) { return !(greatest(r) < INFINITY) || greatest(r) == -INFINITY; };
         // a draft's test: u q < p, and (32 bits) whether the two are too near one another
@@ -397,27 +401,33 @@ __global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const 
         whole(stay, skip, both, zp, zq);
         double fp = 1.0, fq = 0.0;
         if (both) fp = 1.0 / zp, fq = 1.0 / zq;
-        auto left = [&](int i) {      // what the token is drawn from
-            double v = P.keep ? s_keep[i - c0] : i == skip ? 0.0 : term(Elem<DT>::load(p, i), mp);
-            if (both) v = fmax(v * fp - (P.keep ? s_keep[P.keep + i - c0] : term(Elem<DT>::load(q, i), mq)) * fq, 0.0);
-            return v;
+        auto left = [&](int i) {      // what the token is drawn from, where it is not kept
+            double v = i == skip ? 0.0 : term(Elem<DT>::load(p, i), mp);
+            if (both) v = v * fp - term(Elem<DT>::load(q, i), mq) * fq;
+            return v > 0.0 ? v : 0.0;
         };
         if (both) {
             double a = 0.0;
             for (int i = e0 + lane; i - lane < e1; i += 32 * kBatch) {
                 double e[kBatch];
-#pragma unroll
-                for (int k = 0; k < kBatch; ++k) e[k] = i + 32 * k < e1 ? left(i + 32 * k) : 0.0;
                 if (P.keep) {
+#pragma unroll
+                    for (int k = 0; k < kBatch; ++k) {
+                        const int at = i + 32 * k - c0;
+                        e[k] = i + 32 * k < e1 ? s_keep[at] * fp - s_keep[P.keep + at] * fq : 0.0;
+                        e[k] = e[k] > 0.0 ? e[k] : 0.0;
+                    }
 #pragma unroll
                     for (int k = 0; k < kBatch; ++k)
                         if (i + 32 * k < e1) s_keep[i + 32 * k - c0] = e[k];
+                } else {
+#pragma unroll
+                    for (int k = 0; k < kBatch; ++k) e[k] = i + 32 * k < e1 ? left(i + 32 * k) : 0.0;
                 }
                 a += sum_of_batch(e);
             }
             a = warp_sum(a);
             if (lane == 0) s_left[warp] = a;
-            if (P.keep) both = false, fp = 1.0;      // s_keep has it from here on
         } else if (lane == 0) {
             s_left[warp] = s_part[0][warp];
         }
@@ -483,8 +493,13 @@ __global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const 
                 double mine = 0.0;
                 for (int i = i0; i < i1; i += kBatch) {
                     double e[kBatch];
+                    if (P.keep) {
 #pragma unroll
-                    for (int k = 0; k < kBatch; ++k) e[k] = i + k < i1 ? left(i + k) : 0.0;
+                        for (int k = 0; k < kBatch; ++k) e[k] = i + k < i1 ? s_keep[i + k - c0] : 0.0;
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < kBatch; ++k) e[k] = i + k < i1 ? left(i + k) : 0.0;
+                    }
                     mine += sum_of_batch(e);
                 }
                 double upto = mine;
@@ -504,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const 
                 const int f0 = __shfl_sync(0xffffffffu, i0, of), f1 = __shfl_sync(0xffffffffu, i1, of);
                 int at = -1;
                 for (int i = f0; i < f1; i += 32) {
-                    const double x = i + lane < f1 ? left(i + lane) : 0.0;
+                    const double x = i + lane >= f1 ? 0.0 : P.keep ? s_keep[i + lane - c0] : left(i + lane);
                     double sum = x;
 #pragma unroll
                     for (int o = 1; o < 32; o <<= 1) {
