@@ -315,7 +315,8 @@ def rope_append_int4(qkv, cos, sin, positions, k_pages, v_pages, scales, slots, 
     qkv, cos, sin, positions, pcode, slots, scode = _projection(name, qkv, cos, sin, positions, slots, H, Hk, hd)
     T, dev = qkv.shape[0], qkv.device
     q = torch.empty(T, H, hd, dtype=torch.bfloat16, device=dev)
-    k, v = torch.empty(2, T, Hk, hd, dtype=torch.bfloat16, device=dev) if want_kv else (None, None)
+    k = torch.empty(T, Hk, hd, dtype=torch.bfloat16, device=dev) if want_kv else None
+    v = torch.empty_like(k) if want_kv else None
     _lib.call_on(dev.index, "mom_rope_append_int4", qkv.data_ptr(), qkv.stride(0) if T > 1 else qkv.shape[1],
                  cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(), pcode, slots.data_ptr(), scode, T, H,
                  Hk, hd, P, page, k_pages.data_ptr(), v_pages.data_ptr(), scales.data_ptr(), q.data_ptr(),
@@ -365,21 +366,30 @@ def decode_attention_int4(q, k_pages, v_pages, scales, block_table, seq_lens, *,
 class PagedKVCache:
     """The pages of every layer and the sequences that own them.
 
-    k, v: (n_layers, num_pages, n_kv_heads, page_size, head_dim) bf16; a sequence's
-    pages are the same in every layer. The book-keeping is on the host: add() a
+    k, v: (n_layers, num_pages, n_kv_heads, page_size, head_dim) bf16, or with bits 4
+    (..., head_dim / 2) uint8 and scales (..., head_dim / 64, 4) bf16 (rope_append_int4's);
+    layer(i) is one layer's, as the calls take them. A sequence's pages are the same in
+    every layer. The book-keeping is on the host: add() a
     sequence, extend() sequences by their new tokens (which says where those go) or
     retract() those, free() one when it is done."""
 
     def __init__(self, n_layers: int, num_pages: int, page_size: int, n_kv_heads: int, head_dim: int, *,
-                 device="cuda"):
+                 bits: int = 16, device="cuda"):
         if page_size not in PAGE_SIZES:
             raise RuntimeError(f"PagedKVCache: page_size {page_size} must be one of {PAGE_SIZES}")
         _heads("PagedKVCache", head_dim, n_kv_heads, n_kv_heads)
         if n_layers <= 0 or num_pages < 0:
             raise RuntimeError(f"PagedKVCache: {n_layers} layers of {num_pages} pages")
-        shape = (n_layers, num_pages, n_kv_heads, page_size, head_dim)
-        self.k = torch.empty(shape, dtype=torch.bfloat16, device=device)
-        self.v = torch.empty(shape, dtype=torch.bfloat16, device=device)
+        if bits not in (4, 16):
+            raise RuntimeError(f"PagedKVCache: {bits} bits must be 4 or 16")
+        rows = (n_layers, num_pages, n_kv_heads, page_size)
+        shape, dtype = (rows + (head_dim // 2,), torch.uint8) if bits == 4 else (rows + (head_dim,), torch.bfloat16)
+        self.k = torch.empty(shape, dtype=dtype, device=device)
+        self.v = torch.empty(shape, dtype=dtype, device=device)
+        self.scales = None
+        if bits == 4:
+            self.scales = torch.empty(rows + (head_dim // GROUP, 4), dtype=torch.bfloat16, device=device)
+        self.bits = bits
         self.page_size, self.num_pages = page_size, num_pages
         self._free = list(range(num_pages - 1, -1, -1))
         self._pages, self._len, self._next = {}, {}, 0
@@ -387,6 +397,10 @@ class PagedKVCache:
     @property
     def free_pages(self) -> int:
         return len(self._free)
+
+    def layer(self, i: int):
+        """Layer i's pages: (k, v), and its scales with bits 4."""
+        return (self.k[i], self.v[i]) if self.bits == 16 else (self.k[i], self.v[i], self.scales[i])
 
     def length(self, seq: int) -> int:
         return self._len[seq]

@@ -11,6 +11,11 @@ only runs the training trunk's kernels on packed rows (csrc/trunk.cu) with
     decode_attention   one new token of each sequence over its pages
     token_logprobs     the log probability, entropy and alternatives of each token
 
+With kv_bits=4 the cache is held in 4 bits (rope_append_int4, decode_attention_int4): 9/32
+of the memory and of what a step reads. A pass may append several tokens to each
+sequence (Session.extend), and the last ones can be taken back (Session.retract): a
+smaller model's drafts are checked together and verify_drafts says which stay.
+
 The MoM router needs of the past only its running sum: a layer keeps, per sequence,
 the fp32 prefix sum of its router input, carried in token order (the sum that the
 training router's fp32 scan carries, so that a token is routed as in one pass).
@@ -55,21 +60,28 @@ def _check_model(model):
 
 
 class Session:
-    """Sequences of one model in a paged cache. add() prefills prompts, step()
-    appends one token to each running sequence; both return the next token's logits
-    (rows in the order of .seqs). drop() ends sequences. The weights must not change
-    while a session lives: the cached keys and values, and the bank's, projected once
-    here, are the old ones'. An error raised by add() or step() leaves the session as
-    it was."""
+    """Sequences of one model in a paged cache, of bf16 or (kv_bits 4) of 4-bit numbers.
+    add() prefills prompts, step() appends one token to each running sequence, extend()
+    several; they return the next tokens' logits (rows in the order of .seqs). retract()
+    takes the last tokens back, up to `undo` of a sequence; drop() ends sequences. The
+    weights must not change while a session lives: the cached keys and values, and the
+    bank's, projected once here, are the old ones'. An error raised by add(), step() or
+    extend() leaves the session as it was."""
 
-    def __init__(self, model: NaylisForCausalLM, num_pages: int, page_size: int = 16):
+    def __init__(self, model: NaylisForCausalLM, num_pages: int, page_size: int = 16, kv_bits: int = 16,
+                 undo: int = 0):
         _check_model(model)
+        if undo < 0:
+            raise RuntimeError(f"Session: undo {undo} must be >= 0")
         self.model, cfg = model, model.config
         self.device = model.model.embed_tokens.weight.device
         self.cache = attention.PagedKVCache(cfg.num_hidden_layers, num_pages, page_size, cfg.num_attention_heads,
-                                            cfg.head_dim, device=self.device)
+                                            cfg.head_dim, bits=kv_bits, device=self.device)
         self.seqs: List[int] = []
         self.sums = None                 # per layer: (sequences, hidden) fp32 prefix sums of the router's input
+        self.undo = undo
+        self._past = None                # per layer: (sequences, undo, hidden) these sums before the last tokens
+        self._known: List[int] = []      # and how many of them, from the last one back, each sequence has
         self._cos = self._sin = None
         with self._mode():
             self.bank = [trunk.bank_kv(model.model.M_blocks, l.mom.k_proj.weight, l.mom.v_proj.weight, l.mom.mem_slots)
@@ -96,9 +108,14 @@ class Session:
             a, m = layer.self_attn, layer.mom
             x, y = trunk.add_rmsnorm(x, pending, layer.input_layernorm.weight, layer.input_layernorm.eps)
             qkv = trunk.linear_f32grad(y, a.q_proj.weight, a.k_proj.weight, a.v_proj.weight)
-            q, k = attention.rope_append(qkv, cos, sin, positions, self.cache.k[i], self.cache.v[i], slots, n_heads=H,
-                                         want_k=want_k)
-            o = attend(i, q, k, qkv.view(-1, 3 * H, cfg.head_dim)[:, 2 * H:])
+            if self.cache.bits == 4:
+                q, k, v = attention.rope_append_int4(qkv, cos, sin, positions, *self.cache.layer(i), slots, n_heads=H,
+                                                     want_kv=want_k)
+            else:
+                q, k = attention.rope_append(qkv, cos, sin, positions, *self.cache.layer(i), slots, n_heads=H,
+                                             want_k=want_k)
+                v = qkv.view(-1, 3 * H, cfg.head_dim)[:, 2 * H:]
+            o = attend(i, q, k, v)
             o = trunk.linear_f32grad(o.view(-1, d), a.o_proj.weight)
             x, y, y32 = trunk.add_rmsnorm(x, o, layer.mom_norm.weight, layer.mom_norm.eps, want_f32=True)
             idx, log_gates = route(i, m, y32)
@@ -167,6 +184,10 @@ class Session:
             for s in new:
                 self.cache.free(s)
             raise
+        if self.undo:
+            past = [s.new_zeros(len(new), self.undo, s.shape[1]) for s in sums]
+            self._past = past if self._past is None else [torch.cat(p) for p in zip(self._past, past)]
+            self._known += [0] * len(new)
         self.sums = sums if self.sums is None else [torch.cat(p) for p in zip(self.sums, sums)]
         self.seqs += new
         return logits
@@ -188,11 +209,121 @@ class Session:
         positions, slots = self.cache.extend(self.seqs, one)
         try:
             logits, sums = self._step(tokens, positions, slots)
+            past = None
+            if self.undo:
+                past = [torch.cat((p[:, 1:], s[:, None]), 1) for p, s in zip(self._past, self.sums)]
         except BaseException:
             self.cache.retract(self.seqs, one)
             raise
         self.sums = sums
+        if self.undo:
+            self._past, self._known = past, [min(n + 1, self.undo) for n in self._known]
         return logits
+
+    def extend(self, tokens, counts=None):
+        """Append tokens[i, :counts[i]] (default: all of a row) to each running sequence;
+        tokens (len(self.seqs), n) int32 or int64 on the device, counts on the host.
+        Returns the logits behind each token, (len(self.seqs), n, vocab) bf16, zeros behind
+        a sequence's count: what verify_drafts takes. Where it raises no sequence has
+        grown."""
+        V, B = self.model.config.vocab_size, len(self.seqs)
+        if not isinstance(tokens, torch.Tensor) or tokens.dim() != 2 or tokens.shape[0] != B or tokens.dtype not in (
+                torch.int32, torch.int64) or tokens.device != self.device:
+            raise RuntimeError(f"Session.extend: tokens must be ({B}, n) int32 or int64 on {self.device}")
+        n = tokens.shape[1]
+        counts = [n] * B if counts is None else [operator.index(c) for c in counts]
+        if len(counts) != B or any(not 0 <= c <= n for c in counts) or n > attention.MAX_NEW:
+            raise RuntimeError(f"Session.extend: a count in [0, {n}] for each of {B} sequences, at most "
+                               f"{attention.MAX_NEW} tokens each")
+        # the places of the tokens in a (B, n) grid, and the packed ones
+        at = torch.tensor([i * n + j for i, c in enumerate(counts) for j in range(c)], dtype=torch.int64,
+                          device=self.device)
+        ids = tokens.reshape(-1)[at]
+        if bool(((ids < 0) | (ids >= V)).any()):      # the embedding would fault on them
+            raise RuntimeError(f"Session.extend: a token is outside [0, {V})")
+        logits = torch.zeros(B, n, V, dtype=torch.bfloat16, device=self.device)
+        if not len(at):
+            return logits
+        positions, slots = self.cache.extend(self.seqs, counts)
+        try:
+            got, trail = self._extend(ids, at, n, counts, positions, slots)
+            logits.view(-1, V)[at] = got
+            end = torch.tensor(counts, dtype=torch.int64, device=self.device)
+            sums, past = self._cut(trail, end)
+        except BaseException:
+            self.cache.retract(self.seqs, counts)
+            raise
+        self.sums = sums
+        if self.undo:
+            self._past, self._known = past, [min(k + c, self.undo) for k, c in zip(self._known, counts)]
+        return logits
+
+    def _extend(self, ids, at, n, counts, positions, slots):
+        """extend()'s pass -> (logits of the packed tokens, per layer the router's prefix sums before
+        each token of the grid and behind the last, (B, n + 1, hidden))."""
+        B, even = len(counts), min(counts) == n
+        table, lens, longest = self.cache.tables(self.seqs)
+        new = torch.tensor(counts, dtype=torch.int32, device=self.device)
+        owner, place = at // n, at % n
+        sees = lens[owner] - new[owner] + place.to(torch.int32) + 1      # each token's keys
+        trail = []
+
+        def grid(x):
+            if even:
+                return x.view(B, n, *x.shape[1:])
+            return x.new_zeros(B * n, *x.shape[1:]).index_copy_(0, at, x).view(B, n, *x.shape[1:])
+
+        def attend(i, q, k, v):
+            if self.cache.bits == 4:
+                o = attention.decode_attention_int4(grid(q), *self.cache.layer(i), table, lens, new_lens=new,
+                                                    max_len=longest)
+                return o.view(B * n, *q.shape[1:])[at]
+            # a token is a sequence of its own, of the keys that it sees
+            return attention.decode_attention(q, *self.cache.layer(i), table[owner], sees, max_len=longest)
+
+        def route(i, m, y32):
+            y, steps = grid(y32), [self.sums[i]]
+            for j in range(n):                     # token by token: the sums that steps of one would carry
+                steps.append(steps[-1] + y[:, j])
+            trail.append(torch.stack(steps, 1))
+            mean = trail[-1][owner, place + 1] / sees.to(torch.float32)[:, None]
+            _, idx, _, lg = mk.mom_route_log_gates(mean[:, None], m.router_down.weight, m.router_up.weight,
+                                                   m.top_blocks)
+            return idx.transpose(0, 1), lg.transpose(0, 1)
+
+        with self._mode():
+            h = self._pass(ids, positions, slots, longest, attend, route, False)
+            return trunk.linear_f32grad(h, self.model.lm_head.weight), trail
+
+    def _cut(self, trail, end):
+        """Per layer the sums of a trail (sequences, n, hidden) at `end` of each sequence, and (undo) the
+        sums before it."""
+        row = torch.arange(len(end), device=self.device)
+        sums = [t[row, end] for t in trail]
+        if not self.undo:
+            return sums, None
+        u, back = self.undo, torch.arange(self.undo, device=self.device)
+        past = [torch.cat((p, t), 1)[row[:, None], end[:, None] + back] for p, t in zip(self._past, trail)]
+        return sums, past
+
+    def retract(self, counts):
+        """Take the last counts[i] tokens of each running sequence back, as if they had not been
+        appended: at most `undo`, and no more than steps have brought since it was added. Raises,
+        changing nothing, when a sequence has fewer."""
+        counts = [operator.index(c) for c in counts]
+        if len(counts) != len(self.seqs) or any(not 0 <= c <= k for c, k in zip(counts, self._known or [0] * len(counts))):
+            raise RuntimeError(f"Session.retract: for each of {len(self.seqs)} sequences a count of tokens that can be "
+                               f"taken back, at most {self._known or 0}")
+        if not any(counts):
+            return
+        back = self.undo - torch.tensor(counts, dtype=torch.int64, device=self.device)
+        row, order = torch.arange(len(counts), device=self.device), torch.arange(self.undo, device=self.device)
+        trail = [torch.cat((p, s[:, None]), 1) for p, s in zip(self._past, self.sums)]
+        sums = [t[row, back] for t in trail]
+        past = [t[row[:, None], (order + back[:, None] - self.undo).clamp_min(0)] for t in trail]
+        self.cache.retract(self.seqs, counts)
+        self.sums, self._past = sums, past
+        self._known = [k - c for k, c in zip(self._known, counts)]
 
     def _step(self, tokens, positions, slots):
         """step()'s pass -> (logits, the router's prefix sums behind it)."""
@@ -201,7 +332,9 @@ class Session:
         sums = []
 
         def attend(i, q, k, v):
-            return attention.decode_attention(q, self.cache.k[i], self.cache.v[i], table, lens, max_len=longest)
+            if self.cache.bits == 4:
+                return attention.decode_attention_int4(q[:, None], *self.cache.layer(i), table, lens, max_len=longest)[:, 0]
+            return attention.decode_attention(q, *self.cache.layer(i), table, lens, max_len=longest)
 
         def route(i, m, y32):
             sums.append(self.sums[i] + y32)
@@ -227,6 +360,9 @@ class Session:
         at = torch.tensor(keep, dtype=torch.int64, device=self.device)
         if self.sums is not None:
             self.sums = [s[at] for s in self.sums]
+        if self._past is not None:
+            self._past = [p[at] for p in self._past]
+            self._known = [self._known[i] for i in keep]
         return at
 
 
@@ -245,61 +381,132 @@ class _NoGrad:
         self.no_grad.__exit__(*exc)
 
 
+def _choose(logits, temperature, generator):
+    """The next tokens of rows of logits, greedily or sampled."""
+    if temperature == 0.0:
+        return logits.argmax(-1)
+    return torch.multinomial(torch.softmax(logits.float() / temperature, -1), 1, generator=generator)[:, 0]
+
+
+def _record(answer, tokens, scores, top_logprobs, eos_token):
+    """File an answer's next tokens, up to its end; whether it has come. scores: lists of token_logprobs'."""
+    for j, token in enumerate(tokens):
+        answer.tokens.append(token)
+        answer.logprobs.append(scores[0][j])
+        answer.entropies.append(scores[1][j])
+        if top_logprobs:
+            answer.top_ids.append(scores[2][j])
+            answer.top_logprobs.append(scores[3][j])
+        if eos_token is not None and token == eos_token:
+            return True
+    return False
+
+
 def generate(model: NaylisForCausalLM, prompts, max_new_tokens: int, *, temperature: float = 0.0,
              top_logprobs: int = 0, eos_token: Optional[int] = None, generator: Optional[torch.Generator] = None,
-             page_size: int = 16, num_pages: Optional[int] = None) -> List[Generation]:
+             page_size: int = 16, num_pages: Optional[int] = None, kv_bits: int = 16,
+             draft_model: Optional[NaylisForCausalLM] = None, draft_tokens: int = 4) -> List[Generation]:
     """Continue each prompt (a list of token ids) by up to max_new_tokens, greedily
     (temperature 0, ties to the lowest id) or by sampling from
     softmax(logits / temperature), until eos_token. Scores are of the distribution
     sampled from (of softmax(logits) when greedy). num_pages sizes the cache (default:
-    what the prompts and answers can take)."""
+    what the prompts and answers can take); kv_bits 4 holds it in 4 bits.
+
+    With draft_model, a smaller model of the same vocabulary, that one drafts up to
+    draft_tokens tokens at a time, which the model checks in one pass (verify_drafts): the
+    answers are the model's own choices, greedily, and distributed as its own samples."""
     prompts = [list(p) for p in prompts]
     if max_new_tokens < 0 or not (temperature == 0.0 or 1e-6 <= temperature <= 1e6):
         raise RuntimeError(f"generate: max_new_tokens {max_new_tokens}, temperature {temperature}")
     if page_size not in attention.PAGE_SIZES:
         raise RuntimeError(f"generate: page_size {page_size} must be one of {attention.PAGE_SIZES}")
+    if draft_model is not None:
+        most = min(attention.MAX_NEW - 1, scoring.MAX_DRAFTS)
+        if not 1 <= draft_tokens <= most:
+            raise RuntimeError(f"generate: draft_tokens {draft_tokens} must be in [1, {most}]")
+        _check_model(draft_model)
+        if draft_model.config.vocab_size != model.config.vocab_size:
+            raise RuntimeError(f"generate: the draft model has {draft_model.config.vocab_size} tokens, the model "
+                               f"{model.config.vocab_size}")
+        if draft_model.model.embed_tokens.weight.device != model.model.embed_tokens.weight.device:
+            raise RuntimeError("generate: the draft model is on another device")
     out = [Generation() for _ in prompts]
     if not prompts or max_new_tokens == 0:
         return out
+    K = draft_tokens if draft_model is not None else 0
     if num_pages is None:
         num_pages = sum(-(-(len(p) + max_new_tokens) // page_size) for p in prompts)
-    session = Session(model, num_pages, page_size)
+    session = Session(model, num_pages, page_size, kv_bits=kv_bits, undo=K)
+    helper = None
+    if draft_model is not None:
+        pages = sum(-(-(len(p) + max_new_tokens + K) // page_size) for p in prompts)
+        helper = Session(draft_model, pages, page_size, kv_bits=kv_bits, undo=K)
+        helper.add(prompts)
     logits = session.add(prompts)
     running = list(range(len(prompts)))
-    for n in range(max_new_tokens):
-        with torch.no_grad():
-            if temperature == 0.0:
-                tokens = logits.argmax(-1)
-            else:
-                tokens = torch.multinomial(torch.softmax(logits.float() / temperature, -1), 1,
-                                           generator=generator)[:, 0]
-            score = scoring.token_logprobs(logits, tokens, top_k=top_logprobs, temperature=temperature or 1.0)
-        host = [t if t is None else t.tolist() for t in (tokens, *score)]
-        done = []
-        for i, r in enumerate(running):
-            g = out[r]
-            g.tokens.append(host[0][i])
-            g.logprobs.append(host[1][i])
-            g.entropies.append(host[2][i])
-            if top_logprobs:
-                g.top_ids.append(host[3][i])
-                g.top_logprobs.append(host[4][i])
-            if eos_token is not None and host[0][i] == eos_token:
-                done.append(i)
-        if n + 1 == max_new_tokens or len(done) == len(running):
-            break
+    with torch.no_grad():
+        tokens = _choose(logits, temperature, generator)
+        score = scoring.token_logprobs(logits, tokens, top_k=top_logprobs, temperature=temperature or 1.0)
+    host = [[[x] for x in t.tolist()] for t in (tokens, *(t for t in score if t is not None))]
+    while True:
+        done = [i for i, r in enumerate(running) if _record(out[r], host[0][i], [t[i] for t in host[1:]], top_logprobs,
+                                                             eos_token) or len(out[r].tokens) == max_new_tokens]
+        if len(done) == len(running):
+            return out
         if done:
             tokens = tokens[session.drop(done)]
+            if helper is not None:
+                helper.drop(done)
             running = [r for i, r in enumerate(running) if i not in done]
-        logits = session.step(tokens)
-    return out
+        if helper is None:
+            logits = session.step(tokens)
+            with torch.no_grad():
+                tokens = _choose(logits, temperature, generator)
+                score = scoring.token_logprobs(logits, tokens, top_k=top_logprobs, temperature=temperature or 1.0)
+            host = [[[x] for x in t.tolist()] for t in (tokens, *(t for t in score if t is not None))]
+        else:
+            lens = [min(K, max_new_tokens - len(out[r].tokens) - 1) for r in running]
+            tokens, host = _checked(session, helper, tokens, lens, K, temperature, generator, top_logprobs)
 
 
-def score(model: NaylisForCausalLM, sequences, *, top_logprobs: int = 0, temperature: float = 1.0):
+def _checked(session, helper, tokens, lens, K, temperature, generator, top_logprobs):
+    """A round of drafts: the helper's up to K tokens behind `tokens`, lens of each sequence, checked by
+    the session's model -> (the last token of each sequence, lists of the new tokens and their scores)."""
+    steps, drafted = [tokens], []
+    for _ in range(K):
+        drafted.append(helper.step(steps[-1]))
+        with torch.no_grad():
+            steps.append(_choose(drafted[-1], temperature, generator))
+    helper.step(steps[-1])                        # its keys, should all drafts stay
+    logits = session.extend(torch.stack(steps, 1), [n + 1 for n in lens])
+    B, V = len(lens), logits.shape[2]
+    with torch.no_grad():
+        u = None
+        if temperature != 0.0:
+            u = torch.rand(B, K + 1, generator=generator, device=session.device)
+        drafts = torch.stack(steps[1:], 1)
+        kept = scoring.verify_drafts(logits, drafts, u, draft_logits=torch.stack(drafted, 1) if u is not None else None,
+                                     temperature=temperature,
+                                     draft_lens=torch.tensor(lens, dtype=torch.int32, device=session.device))
+        score = scoring.token_logprobs(logits.view(B * (K + 1), V), kept.tokens.view(-1), top_k=top_logprobs,
+                                       temperature=temperature or 1.0, ignore_index=-1)
+        last = kept.tokens.gather(1, kept.accepted[:, None])[:, 0]
+    stay, ends = kept.accepted.tolist(), last.tolist()
+    if min(ends) < 0:
+        raise RuntimeError("generate: the logits are not finite")
+    session.retract([n - a for n, a in zip(lens, stay)])
+    helper.retract([K - a for a in stay])
+    host = [kept.tokens.tolist()] + [t.view(B, K + 1, *t.shape[1:]).tolist() for t in score if t is not None]
+    return last, [[row[:a + 1] for row, a in zip(rows, stay)] for rows in host]
+
+
+def score(model: NaylisForCausalLM, sequences, *, top_logprobs: int = 0, temperature: float = 1.0,
+          kv_bits: int = 16):
     """Log probabilities of given sequences (lists of two or more token ids) under the
     model: per sequence a scoring.TokenLogprobs of its tokens 1 .. n - 1, each given
-    those before it. One packed pass; no cache."""
-    session = Session(model, 0)
+    those before it. One packed pass; no cache (kv_bits 4: its keys and values are rounded
+    as one in 4 bits would)."""
+    session = Session(model, 0, 16, kv_bits)
     sequences = session._check_prompts(sequences)
     if any(len(s) < 2 for s in sequences):
         raise RuntimeError("score: a sequence is two or more tokens")
