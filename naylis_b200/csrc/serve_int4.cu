@@ -193,9 +193,13 @@ rope_append_int4_kernel(const uint16_t *__restrict__ qkv, int64_t ld, const floa
 //   out     = sum_t (p_t s_t) n_t + sum_t p_t z_t
 // so that neither product needs the values themselves. The numbers enter the m16n8k16
 // products as fp16 straight from memory's bits: a number in bits 0 .. 3 of a half is the
-// subnormal n 2^-24, in bits 4 .. 7 n 2^-20, a byte n + 16 n' times 2^-24, all exact, for
-// one AND or byte permutation each; where a byte stands for its two numbers, the upper
-// one's product is taken off again (fp32 sums, 16 times the size of what is left).
+// subnormal n 2^-24, in bits 4 .. 7 n 2^-20, both exact, for one AND each (and a shift for
+// every second pair). Up to 4 rows' scores take a byte n + 16 n' at once and the upper
+// number's part off again: fp32 sums over one row of the cache, 16 times what is left. An
+// output's sum is long and what is left of it small, so there each number enters by itself,
+// and the products' accumulators (which round towards zero) are added up in fp32 after
+// each tile (8 rows: after four, in shared memory): 4 sequences of 131072, error against 64
+// bits 1.7e-3, a bf16 result's own 1.6e-3; with bytes and one accumulator it was 3.3e-3.
 //
 // Both products have the numbers as their first operand: scores are keys by rows (heads, new
 // tokens), outputs dimensions by rows, so that 8 rows cost half of what 16 do; the weights
@@ -222,7 +226,7 @@ constexpr int kMostRows = 8;        // of a list
 
 template <int HD, int ROWS>
 struct Dec4 {
-    static constexpr int kStages = ROWS == 1 ? 2 : 3;
+    static constexpr int kStages = 2;
     static constexpr int kCtas = ROWS == 1 ? 4 : 3;   // resident on an SM
     static constexpr int kTile = 4096 / HD;           // keys of a warp's step
     static constexpr int kGroups = HD / 64, kRowBytes = HD / 2, kScaleBytes = 8 * kGroups;
@@ -233,8 +237,9 @@ struct Dec4 {
     // (1 row), or its scales and zeros in fp32, twice each (8)
     static constexpr int kStride = kTile / 4 + 4;
     static constexpr int kWords = ROWS == 1 ? 8 * kStride * kGroups : ROWS == 8 ? kTile * 8 * kGroups : 0;
-    // that, and at a list's end the warps' outputs
-    static constexpr int kSmem = kRing + std::max(kDecWarps * kWords * 4, kDecWarps * ROWS * HD * 4);
+    static constexpr int kSums = kRing + (ROWS == 8 ? kDecWarps * kWords * 4 : 0);
+    // that, and the warps' outputs: at a list's end, with 8 rows also on the way
+    static constexpr int kSmem = std::max(kRing + kDecWarps * kWords * 4, kSums + kDecWarps * ROWS * HD * 4);
     // a grid of kCtas an SM is resident at once: an SM's shared memory, 1 KB and the static part a CTA
     static_assert(kCtas * (kSmem + 1024 + kDecWarps * (kStages * 8 + (2 + kGroups) * 8 * 4) + 512) <= 228 * 1024);
 };
@@ -312,7 +317,7 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
     __shared__ uint64_t s_full[kDecWarps][C::kStages];
     __shared__ __align__(16) float s_m[kDecWarps][8], s_l[kDecWarps][8], s_z[kDecWarps][NG][8];
     __shared__ float2 s_part[8];
-    float *s_o = reinterpret_cast<float *>(dsm + C::kRing);
+    float *s_o = reinterpret_cast<float *>(dsm + C::kSums);
     const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) >> 5, 0);
     const int lane = threadIdx.x & 31, c4 = lane & 3, r8 = lane >> 2;
     uint32_t *s_w = reinterpret_cast<uint32_t *>(dsm + C::kRing) + warp * C::kWords;
@@ -523,12 +528,22 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[g][i][e] = 0.0f;
         }
+        // 8 rows: the sums of tiles that are through, as this thread has them in acc
+        float4 *const kept = reinterpret_cast<float4 *>(s_o + warp * ROWS * HD) + lane;
+        bool some_kept = false;
         // every output so far times f (of the row that a column is of)
         auto rescale = [&](int g, float f0, float f1) {
 #pragma unroll
             for (int i = 0; i < NA; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[g][i][e] *= e & 1 ? f1 : f0;
+            if (ROWS == 8 && some_kept) {
+#pragma unroll
+                for (int i = 0; i < NA; ++i) {
+                    float4 &x = kept[(g * NA + i) * 32];
+                    x = make_float4(x.x * f0, x.y * f1, x.z * f0, x.w * f1);
+                }
+            }
         };
         // `most`, the greatest of the values' scales of this lane's keys: a finite one above the power of two so far raises it
         auto raise = [&](int g, float most) {
@@ -582,6 +597,21 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                     if (s == 0) mma_f16_first(d, x, x2, x & kOdd, x2 & kOdd, qb[g][s][0], qb[g][s][1]);
                     else mma_f16(d, x, x2, x & kOdd, x2 & kOdd, qb[g][s][0], qb[g][s][1]);
                 }
+            };
+            // and with values: words x and x2 of two keys, whose weights are b0 and b1; numbers 0, 4 and 1, 5, then 2, 6 and 3, 7
+            const auto value_products = [&](float (&d)[2][4], uint32_t x, uint32_t x2, uint32_t b0, uint32_t b1, bool first) {
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const uint32_t y = x >> 8 * s, y2 = x2 >> 8 * s;
+                    if (first) mma_f16_first(d[s], y & kEven, y & kOdd, y2 & kEven, y2 & kOdd, b0, b1);
+                    else mma_f16(d[s], y & kEven, y & kOdd, y2 & kEven, y2 & kOdd, b0, b1);
+                }
+            };
+            const auto add = [&](int g, const float (&d)[2][4]) {
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[g][s][e] += d[s][e];
             };
             if constexpr (ROWS == 1) {
                 // scores: this lane's are of keys 8 c4 + r8 (+ 32), one of each four blocks
@@ -645,7 +675,8 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                 __syncwarp();
                 // outputs: words r8 of keys 4 j + c4; an even column has their low halves' products, an odd one the high ones'
 #pragma unroll
-                for (int g = 0; g < NG; ++g)
+                for (int g = 0; g < NG; ++g) {
+                    float d[2][4];
 #pragma unroll
                     for (int j = 0; j < kTile / 4; j += 4) {
                         const uint4 w = *reinterpret_cast<const uint4 *>(s_w + 8 * C::kStride * g + (4 * (r8 & 1) + c4) * C::kStride + j);
@@ -653,15 +684,12 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
 #pragma unroll
                         for (int u = 0; u < 4; u += 2) {
                             const unsigned char *at = sv + (4 * (j + u) + c4) * C::kRowBytes + 32 * g + 4 * r8;
-                            const uint32_t x0 = *reinterpret_cast<const uint32_t *>(at);
-                            const uint32_t x1 = *reinterpret_cast<const uint32_t *>(at + 4 * C::kRowBytes);
-#pragma unroll
-                            for (int s = 0; s < 2; ++s) {
-                                const uint32_t x = bytes_of(x0, s), x2 = bytes_of(x1, s);
-                                mma_f16(acc[g][s], x, x & kOdd, x2, x2 & kOdd, pw[u], pw[u + 1]);
-                            }
+                            value_products(d, *reinterpret_cast<const uint32_t *>(at),
+                                           *reinterpret_cast<const uint32_t *>(at + 4 * C::kRowBytes), pw[u], pw[u + 1], j + u == 0);
                         }
                     }
+                    add(g, d);
+                }
             } else if constexpr (ROWS == 4) {
                 // scores of row c4: keys key_of(r8) of each block
                 const int mine = key_of(r8);
@@ -671,10 +699,14 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                 for (int g = 0; g < NG; ++g) {
                     float most = 0.0f;
 #pragma unroll
-                    for (int n = 0; n < NB; ++n) {
-                        raw[g][n] = *reinterpret_cast<const uint2 *>(ss + (8 * n + mine) * C::kScaleBytes + 8 * g);
-                        if (8 * n + mine < there) most = fmaxf(most, bf_lo(raw[g][n].y));
+                    for (int n = 0; n < NB; ++n) raw[g][n] = *reinterpret_cast<const uint2 *>(ss + (8 * n + mine) * C::kScaleBytes + 8 * g);
+                    if (there < kTile) {
+#pragma unroll
+                        for (int n = 0; n < NB; ++n)
+                            if (8 * n + mine >= there) raw[g][n].y = 0u;
                     }
+#pragma unroll
+                    for (int n = 0; n < NB; n += 2) most = tc::fmax3(most, bf_lo(raw[g][n].y), bf_lo(raw[g][n + 1].y));
                     raise(g, most);
 #pragma unroll
                     for (int mt = 0; mt < NB / 2; ++mt) {
@@ -706,6 +738,7 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                 // for the words' low halves, in an odd one for the high ones
                 const uint32_t first = r8 & 1 ? 0x1044u : 0x4410u, second = r8 & 1 ? 0x3244u : 0x4432u;
                 const unsigned char *v0 = sv + key_of(2 * c4) * C::kRowBytes + 4 * r8, *v1 = sv + key_of(2 * c4 + 1) * C::kRowBytes + 4 * r8;
+                float d[NG][2][4];
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {
                     const float p = tc::ex2(fmaf(t[n], low(crow), low(ref)));
@@ -715,16 +748,13 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                         const float w = p * (bf_lo(raw[g][n].y) * unit[g]);
                         z2[g] = tc::f2(fmaf(p, bf_hi(raw[g][n].y), low(z2[g])), 0.0f);
                         const uint32_t both = transpose8(pack_f16x2(w, w));
-                        const uint32_t b0 = __byte_perm(both, 0, first), b1 = __byte_perm(both, 0, second);
-                        const uint32_t x0 = *reinterpret_cast<const uint32_t *>(v0 + 8 * n * C::kRowBytes + 32 * g);
-                        const uint32_t x1 = *reinterpret_cast<const uint32_t *>(v1 + 8 * n * C::kRowBytes + 32 * g);
-#pragma unroll
-                        for (int s = 0; s < 2; ++s) {
-                            const uint32_t x = bytes_of(x0, s), x2 = bytes_of(x1, s);
-                            mma_f16(acc[g][s], x, x & kOdd, x2, x2 & kOdd, b0, b1);
-                        }
+                        const int at = 8 * n * C::kRowBytes + 32 * g;
+                        value_products(d[g], *reinterpret_cast<const uint32_t *>(v0 + at), *reinterpret_cast<const uint32_t *>(v1 + at),
+                                       __byte_perm(both, 0, first), __byte_perm(both, 0, second), n == 0);
                     }
                 }
+#pragma unroll
+                for (int g = 0; g < NG; ++g) add(g, d[g]);
             } else {
                 // [group][key's, value's][key]: scale, scale, zero, zero in fp32, once for the warp, each
                 // lane its keys'; the values' scales take the weights' unit along
@@ -818,7 +848,7 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                 for (int g = 0; g < NG; ++g)
 #pragma unroll
                     for (int mt = 0; mt < NB / 2; ++mt) {
-                        uint32_t w[2][2];      // bytes 0, 1 and 2, 3 of the keys in rows 2 c4 and 2 c4 + 1 of both blocks
+                        uint32_t w[2][2];      // numbers 0 .. 3 and 4 .. 7 of the keys in rows 2 c4 and 2 c4 + 1 of both blocks
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             const int at = (16 * mt + 8 * h) * C::kRowBytes + 32 * g;
@@ -829,10 +859,23 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                         }
 #pragma unroll
                         for (int i2 = 0; i2 < 4; ++i2) {
-                            const uint32_t x = bytes_of(w[0][i2 >> 1], i2 & 1), x2 = bytes_of(w[1][i2 >> 1], i2 & 1);
-                            mma_f16(acc[g][i2], x, x & kOdd, x2, x2 & kOdd, pw[g][2 * mt], pw[g][2 * mt + 1]);
+                            const uint32_t x = w[0][i2 >> 1] >> 8 * (i2 & 1), x2 = w[1][i2 >> 1] >> 8 * (i2 & 1);
+                            mma_f16(acc[g][i2], x & kEven, x & kOdd, x2 & kEven, x2 & kOdd, pw[g][2 * mt], pw[g][2 * mt + 1]);
                         }
                     }
+                if ((i & (4 * kDecWarps - 1)) < kDecWarps) {      // every fourth of this warp's tiles
+#pragma unroll
+                    for (int g = 0; g < NG; ++g)
+#pragma unroll
+                        for (int i2 = 0; i2 < NA; ++i2) {
+                            float4 &x = kept[(g * NA + i2) * 32];
+                            const float4 old = some_kept ? x : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            x = make_float4(old.x + acc[g][i2][0], old.y + acc[g][i2][1], old.z + acc[g][i2][2], old.w + acc[g][i2][3]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[g][i2][e] = 0.0f;
+                        }
+                    some_kept = true;
+                }
             }
             __syncwarp();      // the stage, and the words between the lanes, have been read
             fetch(head, tile);
@@ -884,13 +927,23 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
             for (int w = 1; w < kDecWarps; ++w) M = fmaxf(M, s_m[w][row]);
             return M;
         };
-        // the bytes' units and the weights' taken out; an even dimension's sum is what the bytes' has beyond the odd one's
+        if (ROWS == 8 && some_kept) {
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+                for (int i2 = 0; i2 < NA; ++i2) {
+                    const float4 x = kept[(g * NA + i2) * 32];
+                    acc[g][i2][0] += x.x, acc[g][i2][1] += x.y, acc[g][i2][2] += x.z, acc[g][i2][3] += x.w;
+                }
+            __syncwarp();      // the warp's sums are read; their place takes its outputs
+        }
+        // the numbers' 2^-24 and 2^-20 and the weights' unit taken out
         const auto part_of = [&](int row, int g) {
             const float f = s_m[warp][row] == -INFINITY ? 0.0f : tc::ex2(s_m[warp][row] - reference(row));
             return pow2(min(top[g] - 127, 127)) * f;
         };
         const auto pair_of = [](const float (&x)[4], int e, float u) {
-            return make_float2((x[e] - x[2 + e]) * 4096.0f * u, x[2 + e] * 256.0f * u);
+            return make_float2(x[e] * 4096.0f * u, x[2 + e] * 256.0f * u);
         };
 #pragma unroll
         for (int g = 0; g < NG; ++g) {

@@ -158,6 +158,25 @@ def test_a_long_sequence(hd):
     _close(_run(q, cache, table, sl), *_exact(q, cache, table, lens, [2, 2], hd ** -0.5))
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("H,n", [(2, 1), (8, 1), (2, 7)])
+def test_a_long_mean(hd, H, n):
+    """All keys alike (a query of 0): the mean of 131072 values, near 0 with numbers around the
+    middle of their groups. Weights are the values' scales, exact in fp16; a warp's sums, of up
+    to all keys of a list, may be off by 2^-20 of what they sum (fp32, rounded towards zero
+    within a few tiles): 15 scales, so 2^-16 of the greatest scale, twice for the two sums."""
+    lens = [131072]
+    q, (k, v, s), table, sl = _case(hd, H, 2, 64, lens, n, seed=12)
+    g = torch.Generator().manual_seed(5)
+    num = torch.randn(2, *v.shape, generator=g).mul(3.2).add(7.5).round().clamp(0, 15).to(torch.uint8).to(DEV)
+    cache = (k, num[0] | num[1] << 4, s)
+    s[..., 3] = (-7.5 * s[..., 2].float()).to(torch.bfloat16)
+    got = _run(q * 0, cache, table, sl)
+    out, A = _exact(q * 0, cache, table, lens, [n], 1.0)
+    worst = float(((got.double() - out).abs() - 2.0 ** -8 * out.abs()).max())
+    assert worst <= 2.0 ** -15 * float(s[..., 2].max()), worst
+
+
 @pytest.mark.parametrize("lens", [[300, 40], [30000, 257]], ids=str)
 @pytest.mark.parametrize("hd", [64, 128])
 def test_scales_of_very_different_size(hd, lens):
