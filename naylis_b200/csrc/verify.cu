@@ -298,55 +298,6 @@ __global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const 
         auto term = [&](float x, float top) {      // e^((x - top) / T)
             return exp_of(wide(x) - wide(top), P.scale, s_table);
         };
-        // The sums of the target's row r (without its element `skip`) and, both, of the draft's; the
-        // stretches' in s_part, the terms kept.
-        auto whole = [&](int r, int skip, bool both, double &zp, double &zq) {
-            const T *p = row_of(r), *q = both ? row_of(n + 1 + r) : p;
-            const float mp = greatest(r), mq = both ? greatest(n + 1 + r) : 0.0f;
-            double a = 0.0, c = 0.0;
-            // a batch of both rows on its way together, and its terms side by side: each is a chain of a dozen operations
-            const auto fetch = [&](float (&x)[kBatch], const T *row, int i, int without) {
-#pragma unroll
-                for (int k = 0; k < kBatch; ++k) {
-                    const int at = i + 32 * k;
-                    x[k] = at < e1 && at != without ? Elem<DT>::load(row, at) : -INFINITY;
-                }
-            };
-            const auto batch = [&](const float (&x)[kBatch], float top, int i, double *keep) {
-                double e[kBatch];
-#pragma unroll
-                for (int k = 0; k < kBatch; ++k) e[k] = term(x[k], top);
-                if (P.keep) {
-#pragma unroll
-                    for (int k = 0; k < kBatch; ++k)
-                        if (i + 32 * k < e1) keep[i + 32 * k - c0] = e[k];
-                }
-                return sum_of_batch(e);
-            };
-            for (int i = e0 + lane; i - lane < e1; i += 32 * kBatch) {
-                float x[kBatch], y[kBatch];
-                fetch(x, p, i, skip);
-                if (both) fetch(y, q, i, -1);
-                a += batch(x, mp, i, s_keep);
-                if (both) c += batch(y, mq, i, s_keep + P.keep);
-            }
-            a = warp_sum(a);
-            if (both) c = warp_sum(c);
-            if (lane == 0) s_part[0][warp] = a, s_part[1][warp] = c;
-            __syncthreads();
-            if (threadIdx.x < 2) {
-                double s = 0.0;
-#pragma unroll
-                for (int i = 0; i < kWarps; ++i) s += s_part[threadIdx.x][i];
-                s_whole[threadIdx.x] = s;
-            }
-            cluster_sync();
-            // all CTAs' sums by the lanes at once, then the same sum in each
-            const double x = lane < ctas ? ld_cluster(&s_whole[0], lane) : 0.0;
-            const double y = both && lane < ctas ? ld_cluster(&s_whole[1], lane) : 0.0;
-            zp = warp_sum(x);
-            zq = both ? warp_sum(y) : 0.0;
-        };
         auto broken = [&](int r) { return !(greatest(r) < INFINITY) || greatest(r) == -INFINITY; };
         // a draft's test: u q < p, and (32 bits) whether the two are too near one another
         auto test = [&](float u, float xp, float xq, int r, double zp, double zq, bool &near) {
@@ -368,70 +319,6 @@ __global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const 
             s_verdict[j] = v;
         }
         __syncthreads();
-        // all of the cluster's threads come to the same verdicts
-        int stay = 0, verdict = kStays;
-        double zp = 0.0, zq = 0.0;
-        for (; stay < n; ++stay) {
-            verdict = s_verdict[stay];
-            if (verdict == kUnsure) {
-                whole(stay, -1, Own, zp, zq);
-                const int64_t d = drafts[stay];      // in the vocabulary
-                const float u = P.uniforms[static_cast<int64_t>(b) * (P.K + 1) + stay];
-                bool near;
-                verdict = test(u, Elem<DT>::load(row_of(stay), d), Own ? Elem<DT>::load(row_of(n + 1 + stay), d) : 0.0f, stay, zp,
-                               zq, near);
-                cluster_sync();      // the sums are read
-            }
-            if (verdict != kStays) break;
-        }
-        if (refused || broken(stay) || verdict == kBroken) {
-            if (me == 0) {
-                finish(stay);
-                if (threadIdx.x == 0) tokens[stay] = -1;
-            }
-            cluster_sync();
-            return;
-        }
-        const bool fell = stay < n;
-        const int64_t d = fell && !Own ? drafts[stay] : -1;
-        const T *p = row_of(stay), *q = Own && fell ? row_of(n + 1 + stay) : nullptr;
-        const float mp = greatest(stay), mq = q ? greatest(n + 1 + stay) : 0.0f;
-        int skip = d >= 0 && d < P.V ? static_cast<int>(d) : -1;
-        bool both = q != nullptr;
-        whole(stay, skip, both, zp, zq);
-        double fp = 1.0, fq = 0.0;
-        if (both) fp = 1.0 / zp, fq = 1.0 / zq;
-        auto left = [&](int i) {      // what the token is drawn from, where it is not kept
-            double v = i == skip ? 0.0 : term(Elem<DT>::load(p, i), mp);
-            if (both) v = v * fp - term(Elem<DT>::load(q, i), mq) * fq;
-            return v > 0.0 ? v : 0.0;
-        };
-        if (both) {
-            double a = 0.0;
-            for (int i = e0 + lane; i - lane < e1; i += 32 * kBatch) {
-                double e[kBatch];
-                if (P.keep) {
-#pragma unroll
-                    for (int k = 0; k < kBatch; ++k) {
-                        const int at = i + 32 * k - c0;
-                        e[k] = i + 32 * k < e1 ? s_keep[at] * fp - s_keep[P.keep + at] * fq : 0.0;
-                        e[k] = e[k] > 0.0 ? e[k] : 0.0;
-                    }
-#pragma unroll
-                    for (int k = 0; k < kBatch; ++k)
-                        if (i + 32 * k < e1) s_keep[i + 32 * k - c0] = e[k];
-                } else {
-#pragma unroll
-                    for (int k = 0; k < kBatch; ++k) e[k] = i + 32 * k < e1 ? left(i + 32 * k) : 0.0;
-                }
-                a += sum_of_batch(e);
-            }
-            a = warp_sum(a);
-            if (lane == 0) s_left[warp] = a;
-        } else if (lane == 0) {
-            s_left[warp] = s_part[0][warp];
-        }
-        cluster_sync();
         // where the running sum passes u times the whole: among the cluster's stretches
         auto find = [&]() {
             if (warp == 0) {
@@ -473,19 +360,118 @@ __global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const 
             }
             __syncthreads();
         };
-        find();
-        if (s_owner < 0) {
-            // nothing is left (the draft's distribution is the target's): from the target's own
-            skip = -1, both = false, fp = 1.0;
-            cluster_sync();      // the sums are read
-            double z0, z1;
-            whole(stay, -1, false, z0, z1);
-            if (lane == 0) s_left[warp] = s_part[0][warp];
+        // All of the cluster's threads come to the same verdicts. The row that decides is summed in 64 bits, for
+        // a verdict on its draft first where that is unsure, then for the token.
+        int stay = 0, skip;
+        bool both, own_alone = false;
+        double fp, fq;
+        const T *p, *q;
+        float mp, mq;
+        auto left = [&](int i) {      // what the token is drawn from, where it is not kept
+            double v = i == skip ? 0.0 : term(Elem<DT>::load(p, i), mp);
+            if (both) v = v * fp - term(Elem<DT>::load(q, i), mq) * fq;
+            return v > 0.0 ? v : 0.0;
+        };
+        while (true) {
+            while (stay < n && s_verdict[stay] == kStays) ++stay;
+            const int verdict = stay < n ? s_verdict[stay] : kFalls;
+            if (refused || broken(stay) || verdict == kBroken) {
+                if (me == 0) {
+                    finish(stay);
+                    if (threadIdx.x == 0) tokens[stay] = -1;
+                }
+                cluster_sync();
+                return;
+            }
+            const int64_t d = stay < n ? drafts[stay] : -1;
+            both = Own && stay < n && !own_alone;
+            skip = !Own && verdict == kFalls && !own_alone && d >= 0 && d < P.V ? static_cast<int>(d) : -1;
+            p = row_of(stay), q = both ? row_of(n + 1 + stay) : p;
+            mp = greatest(stay), mq = both ? greatest(n + 1 + stay) : 0.0f;
+            double a = 0.0, c = 0.0;
+            // a batch of both rows on its way together, and its terms side by side: each is a chain of a dozen operations
+            for (int i = e0 + lane; i - lane < e1; i += 32 * kBatch) {
+                float x[2][kBatch];
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) {
+                    const int at = i + 32 * k;
+                    x[0][k] = at < e1 && at != skip ? Elem<DT>::load(p, at) : -INFINITY;
+                    x[1][k] = both && at < e1 ? Elem<DT>::load(q, at) : -INFINITY;
+                }
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    if (r == 1 && !both) break;
+                    double e[kBatch];
+#pragma unroll
+                    for (int k = 0; k < kBatch; ++k) e[k] = term(x[r][k], r == 0 ? mp : mq);
+                    if (P.keep) {
+#pragma unroll
+                        for (int k = 0; k < kBatch; ++k)
+                            if (i + 32 * k < e1) s_keep[r * P.keep + i + 32 * k - c0] = e[k];
+                    }
+                    (r == 0 ? a : c) += sum_of_batch(e);
+                }
+            }
+            a = warp_sum(a);
+            if (both) c = warp_sum(c);
+            if (lane == 0) s_part[0][warp] = a, s_part[1][warp] = c;
+            if (both || verdict == kUnsure) {
+                __syncthreads();
+                if (threadIdx.x < 2) {
+                    double s = 0.0;
+#pragma unroll
+                    for (int i = 0; i < kWarps; ++i) s += s_part[threadIdx.x][i];
+                    s_whole[threadIdx.x] = s;
+                }
+                cluster_sync();
+                // all CTAs' sums by the lanes at once, then the same sum in each
+                const double zp = warp_sum(lane < ctas ? ld_cluster(&s_whole[0], lane) : 0.0);
+                const double zq = both ? warp_sum(lane < ctas ? ld_cluster(&s_whole[1], lane) : 0.0) : 0.0;
+                if (verdict == kUnsure) {
+                    const float u = P.uniforms[static_cast<int64_t>(b) * (P.K + 1) + stay];
+                    bool near;
+                    const int now = test(u, Elem<DT>::load(p, d), Own ? Elem<DT>::load(q, d) : 0.0f, stay, zp, zq, near);
+                    cluster_sync();      // the sums are read, and the verdict
+                    if (threadIdx.x == 0) s_verdict[stay] = now;
+                    __syncthreads();
+                    continue;
+                }
+                fp = 1.0 / zp, fq = 1.0 / zq;
+            }
+            if (both) {
+                a = 0.0;
+                for (int i = e0 + lane; i - lane < e1; i += 32 * kBatch) {
+                    double e[kBatch];
+                    if (P.keep) {
+#pragma unroll
+                        for (int k = 0; k < kBatch; ++k) {
+                            const int at = i + 32 * k - c0;
+                            e[k] = i + 32 * k < e1 ? s_keep[at] * fp - s_keep[P.keep + at] * fq : 0.0;
+                            e[k] = e[k] > 0.0 ? e[k] : 0.0;
+                        }
+#pragma unroll
+                        for (int k = 0; k < kBatch; ++k)
+                            if (i + 32 * k < e1) s_keep[i + 32 * k - c0] = e[k];
+                    } else {
+#pragma unroll 1
+                        for (int k = 0; k < kBatch; ++k) a += i + 32 * k < e1 ? left(i + 32 * k) : 0.0;
+#pragma unroll
+                        for (int k = 0; k < kBatch; ++k) e[k] = 0.0;
+                    }
+                    a += sum_of_batch(e);
+                }
+                a = warp_sum(a);
+            }
+            if (lane == 0) s_left[warp] = a;
             cluster_sync();
             find();
+            // nothing is left (the draft's distribution is the target's): from the target's own
+            if (s_owner >= 0 || own_alone) break;
+            own_alone = true;
+            cluster_sync();      // the sums are read
         }
         const int owner = s_owner;
-        if (owner / kWarps == me) {
+        if (owner >= 0 && owner / kWarps == me) {
             finish(stay);
             if (owner % kWarps == warp) {
                 // the owner's lanes take neighbouring elements each, an odd number of them: no bank conflicts
@@ -497,8 +483,10 @@ __global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const 
 #pragma unroll
                         for (int k = 0; k < kBatch; ++k) e[k] = i + k < i1 ? s_keep[i + k - c0] : 0.0;
                     } else {
+#pragma unroll 1
+                        for (int k = 0; k < kBatch; ++k) mine += i + k < i1 ? left(i + k) : 0.0;
 #pragma unroll
-                        for (int k = 0; k < kBatch; ++k) e[k] = i + k < i1 ? left(i + k) : 0.0;
+                        for (int k = 0; k < kBatch; ++k) e[k] = 0.0;
                     }
                     mine += sum_of_batch(e);
                 }
