@@ -94,21 +94,22 @@ def _heads(name, hd, H, Hk):
 def _projection(name, qkv, cos, sin, positions, slots, H, Hk, hd):
     """The checked arguments of an append, each as the kernels take it."""
     _heads(name, hd, H, Hk)
-    if qkv.dim() != 2 or qkv.shape[1] != (H + 2 * Hk) * hd:
-        raise RuntimeError(f"{name}: qkv must be (T, {(H + 2 * Hk) * hd}) for {H} + 2 x {Hk} heads of {hd}, got "
-                           f"{tuple(qkv.shape)}")
-    dev = qkv.device
-    for t in (cos, sin):
-        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != hd or t.shape != cos.shape or t.device != dev:
-            raise RuntimeError(f"{name}: cos and sin must be (n_pos, {hd}) fp32 on {dev}")
-        if t.requires_grad:
-            _no_grad(name)
+    width = (H + 2 * Hk) * hd
+    if qkv.dim() != 2 or qkv.shape[1] != width:
+        raise RuntimeError(f"{name}: qkv must be (T, {width}) for {H} + 2 x {Hk} heads of {hd}, got {tuple(qkv.shape)}")
+    dev, shape = qkv.device, cos.shape
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or len(shape) != 2 or shape[1] != hd or \
+            sin.shape != shape or cos.device != dev or sin.device != dev:
+        raise RuntimeError(f"{name}: cos and sin must be (n_pos, {hd}) fp32 on {dev}")
+    if cos.requires_grad or sin.requires_grad:
+        _no_grad(name)
     if forward_ad._current_level >= 0:
         _lib.no_tangent(name, cos, sin)
     T = qkv.shape[0]
     positions, pcode = _index(name, positions, T, dev, "positions")
     slots, scode = _index(name, slots, T, dev, "slots")
-    if qkv.stride(1) != 1 or qkv.data_ptr() % 16 or (T > 1 and (qkv.stride(0) % 8 or qkv.stride(0) < qkv.shape[1])):
+    ld, step = qkv.stride()
+    if step != 1 or qkv.data_ptr() % 16 or (T > 1 and (ld % 8 or ld < width)):
         qkv = qkv.clone(memory_format=torch.contiguous_format)
     cos, sin = cos.contiguous(), sin.contiguous()
     if cos.data_ptr() % 16:
@@ -275,12 +276,14 @@ MAX_NEW = 64        # new tokens of a sequence in a step
 
 
 def _pages_int4(name, k_pages, v_pages, scales):
-    for t in (k_pages, v_pages):
-        if t.dtype != torch.uint8 or not t.is_cuda or t.dim() != 4 or t.shape != k_pages.shape or \
-                t.device != k_pages.device or not t.is_contiguous():
-            raise RuntimeError(f"{name}: k_pages and v_pages must both be contiguous (num_pages, n_kv_heads, page_size, "
-                               f"head_dim / 2) uint8 CUDA tensors, got {tuple(t.shape)} {t.dtype} on {t.device}")
-    P, Hk, page, half = k_pages.shape
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape or k_pages.dtype != torch.uint8 or v_pages.dtype != torch.uint8 or \
+            not k_pages.is_cuda or v_pages.device != k_pages.device or not k_pages.is_contiguous() or \
+            not v_pages.is_contiguous():
+        raise RuntimeError(f"{name}: k_pages and v_pages must both be contiguous (num_pages, n_kv_heads, page_size, "
+                           f"head_dim / 2) uint8 CUDA tensors, got {tuple(shape)} {k_pages.dtype} on {k_pages.device} and "
+                           f"{tuple(v_pages.shape)} {v_pages.dtype} on {v_pages.device}")
+    P, Hk, page, half = shape
     if page not in PAGE_SIZES:
         raise RuntimeError(f"{name}: page_size {page} must be one of {PAGE_SIZES}")
     if half not in (32, 64):
