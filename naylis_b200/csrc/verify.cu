@@ -17,6 +17,9 @@
 // One cluster takes a sequence. Its warps share the rows out for the 32-bit sums, each some
 // contiguous part of one row at a time; in 64 bits each has a stretch of the vocabulary, whose
 // exponentials it keeps in shared memory where they fit (the search then reads them).
+// Rows of 32000, bf16: 1 sequence of 4 drafts 12 us, 48 of 4 23 us, 40 of 7 in fp32 17 us (drafts
+// without logits), bound by the chain of phases (sums, decision, the row's terms, search), a barrier
+// behind each; 256 of 7 greedily 25 us, 5.2 TB/s, by memory.
 #include <algorithm>
 #include <atomic>
 #include <cfloat>
