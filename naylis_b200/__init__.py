@@ -7,9 +7,11 @@ Public surface:
   naylis_b200.data_parallel   explicit bucketed NCCL gradient all-reduce
   naylis_b200.attention       serving attention: packed prompts, one token over a
                             paged key-value cache, the rotary embedding with the
-                            cache write, the cache itself
-  naylis_b200.scoring         token log probabilities, entropy, alternatives
-  naylis_b200.generate        answering with the decoder (generate, Session, score)
+                            cache write, the cache itself, in bf16 or in 4 bits
+  naylis_b200.scoring         token log probabilities, entropy, alternatives; which
+                              drafted tokens stay
+  naylis_b200.generate        answering with the decoder (generate, Session, score),
+                              also with a smaller model's drafts
   naylis_b200.build           in-tree nvcc build of libnaylis_mom.so
 """
 from . import mom_kernels  # noqa: F401
