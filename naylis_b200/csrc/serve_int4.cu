@@ -584,6 +584,12 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
             }
         };
         const auto low = [](uint64_t v) { return tc::f2_split(v).x; };
+        // a weight's exponent. The product is rounded by itself, as the reference was: the difference of a huge score to
+        // its own rounding is no exponent. (In packed pairs the product and the sum became one operation again.)
+        const auto weight_of = [&](float t, int row) {
+            const float2 c = tc::f2_split(crow), r = tc::f2_split(ref);
+            return __fadd_rn(__fmul_rn(t, row ? c.y : c.x), row ? r.y : r.x);
+        };
         for (int i = (warp - taken) & (kDecWarps - 1); i < tiles; i += kDecWarps) {
             if (waits && !wait_phase(&s_full[warp][head], parity)) waits = false;
             lost |= (bad >> head & 1) || !waits;
@@ -666,7 +672,7 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
 #pragma unroll
                 for (int k = 0; k < kKeys; ++k) {
                     const int key = 32 * k + 8 * c4 + r8;
-                    const float p = tc::ex2(fmaf(t[k], low(crow), low(ref)));
+                    const float p = tc::ex2(weight_of(t[k], 0));
                     l2 = tc::f2(low(l2) + p, 0.0f);
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
@@ -747,7 +753,7 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                 float d[NG][2][4];
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {
-                    const float p = tc::ex2(fmaf(t[n], low(crow), low(ref)));
+                    const float p = tc::ex2(weight_of(t[n], 0));
                     l2 = tc::f2(low(l2) + p, 0.0f);
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
@@ -829,7 +835,7 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                 auto weigh = [&](auto some_hidden) {
 #pragma unroll
                     for (int n = 0; n < NB; ++n) {
-                        const uint64_t p2 = tc::ex2_pair(tc::fma2(t[n], crow, ref));
+                        const uint64_t p2 = tc::ex2_pair(tc::f2(weight_of(tc::f2_split(t[n]).x, 0), weight_of(tc::f2_split(t[n]).y, 1)));
                         l2 = tc::add2(l2, p2);
 #pragma unroll
                         for (int g = 0; g < NG; ++g) {
