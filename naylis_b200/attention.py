@@ -223,19 +223,20 @@ def prompt_attention(q, k, v, plan: PromptPlan, *, scale=None):
 # ------------------------------------------------------------------ decode
 def _block_table(name, block_table, seq_lens, B, page, max_len, dev):
     """Checked: (block_table, its pitch, seq_lens, max_len) as the kernels take them."""
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or \
-            block_table.device != dev:
+    shape = block_table.shape
+    if block_table.dtype != torch.int32 or len(shape) != 2 or shape[0] != B or block_table.device != dev:
         raise RuntimeError(f"{name}: block_table must be ({B}, pages) int32 on {dev}")
     if seq_lens.dtype != torch.int32 or seq_lens.shape != (B,) or seq_lens.device != dev:
         raise RuntimeError(f"{name}: seq_lens must be ({B},) int32 on {dev}")
-    if block_table.shape[1] > 1 and block_table.stride(1) != 1:
-        block_table = block_table.contiguous()
+    pages = table_ld = shape[1]
+    if B > 1 or pages > 1:
+        ld, step = block_table.stride()
+        if (pages > 1 and step != 1) or (B > 1 and ld < pages):
+            block_table = block_table.contiguous()
+        elif B > 1:
+            table_ld = ld
     seq_lens = seq_lens.contiguous()
-    table_ld = block_table.stride(0) if B > 1 else block_table.shape[1]
-    if table_ld < block_table.shape[1]:
-        block_table = block_table.contiguous()
-        table_ld = block_table.shape[1]
-    cap = block_table.shape[1] * page
+    cap = pages * page
     max_len = cap if max_len is None else int(max_len)
     if not 0 <= max_len <= cap:
         raise RuntimeError(f"{name}: max_len {max_len} must be in [0, {cap}], what the block table holds")
@@ -340,16 +341,18 @@ def decode_attention_int4(q, k_pages, v_pages, scales, block_table, seq_lens, *,
     name = "decode_attention_int4"
     P, Hk, page, hd = _pages_int4(name, k_pages, v_pages, scales)
     _check(name, q, scales)
-    if q.dim() != 4 or q.shape[3] != hd:
-        raise RuntimeError(f"{name}: q must be (sequences, new tokens, heads, {hd}), got {tuple(q.shape)}")
-    if k_pages.device != q.device:
-        raise RuntimeError(f"{name}: tensors on {q.device} and {k_pages.device}")
-    B, n, H, _ = q.shape
+    shape, dev = q.shape, q.device
+    if len(shape) != 4 or shape[3] != hd:
+        raise RuntimeError(f"{name}: q must be (sequences, new tokens, heads, {hd}), got {tuple(shape)}")
+    if k_pages.device != dev:
+        raise RuntimeError(f"{name}: tensors on {dev} and {k_pages.device}")
+    B, n, H, _ = shape
     _heads(name, hd, H, Hk)
     if not 1 <= n <= MAX_NEW:
         raise RuntimeError(f"{name}: {n} new tokens must be in [1, {MAX_NEW}]")
-    q, q_ld = _rows(name, q.reshape(B * n, H, hd), "q")
-    dev = q.device
+    q_ld = H * hd
+    if not q.is_contiguous() or q.data_ptr() % 16:
+        q, q_ld = _rows(name, q.reshape(B * n, H, hd), "q")
     if new_lens is not None:
         if new_lens.dtype != torch.int32 or new_lens.shape != (B,) or new_lens.device != dev:
             raise RuntimeError(f"{name}: new_lens must be ({B},) int32 on {dev}")

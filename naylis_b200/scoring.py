@@ -120,13 +120,6 @@ class Verified(NamedTuple):
     accepted: torch.Tensor
 
 
-def _logits3(t, B, rows, V, like):
-    if t.dim() != 3 or t.shape != (B, rows, V) or t.dtype != like.dtype or t.device != like.device:
-        raise RuntimeError(f"verify_drafts: draft_logits must be {(B, rows, V)} {like.dtype} on {like.device}, got "
-                           f"{tuple(t.shape)} {t.dtype} on {t.device}")
-    return t if V == 1 or t.stride(2) == 1 else t.contiguous()
-
-
 def verify_drafts(logits, drafts, uniforms=None, *, draft_logits=None, temperature: float = 1.0, draft_lens=None):
     """Which drafted tokens the target keeps, and the token that follows them, by
     speculative sampling: tokens come out distributed as the target's own samples.
@@ -149,13 +142,13 @@ def verify_drafts(logits, drafts, uniforms=None, *, draft_logits=None, temperatu
     if not logits.is_cuda or logits.dtype not in (torch.bfloat16, torch.float32):
         raise RuntimeError(f"verify_drafts takes bf16 or fp32 CUDA logits, got {logits.dtype} on {logits.device}")
     dev = logits.device
-    if logits.dim() != 3 or drafts.dim() != 2 or logits.shape[0] != drafts.shape[0] or \
-            logits.shape[1] != drafts.shape[1] + 1 or logits.shape[2] == 0 or drafts.dtype != torch.int64 or \
-            drafts.device != dev:
+    shape, rows = logits.shape, drafts.shape
+    if len(shape) != 3 or len(rows) != 2 or shape[0] != rows[0] or shape[1] != rows[1] + 1 or shape[2] == 0 or \
+            drafts.dtype != torch.int64 or drafts.device != dev:
         raise RuntimeError(f"verify_drafts: logits (B, K + 1, V) and int64 drafts (B, K) on one device, got "
-                           f"{tuple(logits.shape)} and {tuple(drafts.shape)} {drafts.dtype}")
-    B, K = drafts.shape
-    V = logits.shape[2]
+                           f"{tuple(shape)} and {tuple(rows)} {drafts.dtype}")
+    B, K = rows
+    V = shape[2]
     temperature = float(temperature)
     if K > MAX_DRAFTS:
         raise RuntimeError(f"verify_drafts: {K} drafts must be at most {MAX_DRAFTS}")
@@ -171,15 +164,24 @@ def verify_drafts(logits, drafts, uniforms=None, *, draft_logits=None, temperatu
         if draft_lens.dtype != torch.int32 or draft_lens.shape != (B,) or draft_lens.device != dev:
             raise RuntimeError(f"verify_drafts: draft_lens must be ({B},) int32 on {dev}")
         draft_lens = draft_lens.contiguous()
-    logits = _logits3(logits, B, K + 1, V, logits)
+    ld_seq, ld_row, step = logits.stride()
+    if step != 1 and V > 1:
+        logits = logits.contiguous()
+        ld_seq, ld_row = (K + 1) * V, V
     drafts = drafts.contiguous()
+    draft_ld_seq = draft_ld_row = 0
     if draft_logits is not None:
-        draft_logits = _logits3(draft_logits, B, K, V, logits)
+        if draft_logits.shape != (B, K, V) or draft_logits.dtype != logits.dtype or draft_logits.device != dev:
+            raise RuntimeError(f"verify_drafts: draft_logits must be {(B, K, V)} {logits.dtype} on {dev}, got "
+                               f"{tuple(draft_logits.shape)} {draft_logits.dtype} on {draft_logits.device}")
+        draft_ld_seq, draft_ld_row, step = draft_logits.stride()
+        if step != 1 and V > 1:
+            draft_logits = draft_logits.contiguous()
+            draft_ld_seq, draft_ld_row = K * V, V
     tokens = torch.empty(B, K + 1, dtype=torch.int64, device=dev)
     accepted = torch.empty(B, dtype=torch.int64, device=dev)
-    _lib.call_on(dev.index, "mom_verify_drafts", logits.data_ptr(), _code(logits), logits.stride(0), logits.stride(1),
-                 None if draft_logits is None else draft_logits.data_ptr(),
-                 *((0, 0) if draft_logits is None else draft_logits.stride()[:2]), drafts.data_ptr(),
+    _lib.call_on(dev.index, "mom_verify_drafts", logits.data_ptr(), _code(logits), ld_seq, ld_row,
+                 None if draft_logits is None else draft_logits.data_ptr(), draft_ld_seq, draft_ld_row, drafts.data_ptr(),
                  None if uniforms is None else uniforms.data_ptr(), None if draft_lens is None else draft_lens.data_ptr(),
                  B, K, V, temperature, tokens.data_ptr(), accepted.data_ptr())
     return Verified(tokens, accepted)
