@@ -489,6 +489,18 @@ MOM_API int mom_verify_drafts(const void *logits, int dtype, int64_t ld_seq, int
                               const int32_t *draft_lens, int64_t B, int64_t K, int64_t V, double temperature,
                               int64_t *tokens, int64_t *accepted, void *stream);
 
+/* The entry points of single steps, whose work takes no longer than a foreign-function
+ * interface's conversion of their arguments: entry's arguments in order, n of them, 8 bytes
+ * each (pointers and integers as int64, floating-point ones as double), returns its status. */
+typedef enum {
+    MOM_CALL_ROPE_APPEND = 0,
+    MOM_CALL_DECODE_ATTN = 1,
+    MOM_CALL_ROPE_APPEND_INT4 = 2,
+    MOM_CALL_DECODE_ATTN_INT4 = 3,
+    MOM_CALL_VERIFY_DRAFTS = 4
+} mom_call;
+MOM_API int mom_call_packed(int entry, const void *args, int n);
+
 /* Reads (and clears) the device error word of a plan: MOM_OK, or
  * MOM_ERR_DEVICE_INDEX when mom_bucket saw an index outside [0, nb).
  * Synchronises `stream`. */

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -106,8 +107,18 @@ SIGNATURES = {
                                 _vp]),
     "mom_verify_drafts": (_int, [_vp, _int, _i64, _i64, _vp, _i64, _i64, _vp, _fp, _vp, _i64, _i64, _i64, _c.c_double,
                                  _vp, _vp, _vp]),
+    "mom_call_packed": (_int, [_int, _vp, _int]),
     "mom_logprobs_bwd": (_int, [_vp, _int, _i64, _vp, _fp, _vp, _i64, _fp, _fp, _fp, _i64, _i64, _i64, _c.c_double,
                                 _vp, _vp]),
+}
+
+# Entry points that call_on() gives their arguments packed, 8 bytes each: name -> (mom_call, packer, count).
+# ctypes converts 20 arguments one by one in as long as such a call's kernel takes (4 us; packed 1.3).
+_PACKED = {
+    name: (i, struct.Struct("".join("d" if t is _c.c_double else "q" for t in SIGNATURES[name][1])).pack,
+           len(SIGNATURES[name][1]))
+    for i, name in enumerate(("mom_rope_append", "mom_decode_attn", "mom_rope_append_int4", "mom_decode_attn_int4",
+                              "mom_verify_drafts"))
 }
 
 _lock = threading.Lock()
@@ -141,6 +152,11 @@ def load(path: str = LIB_PATH):
         return lib
 
 
+def handle():
+    """load()'s handle, without its lock once it is there."""
+    return _lib or load()
+
+
 def last_error() -> str:
     return load().mom_last_error_string().decode(errors="replace")
 
@@ -165,12 +181,16 @@ def no_tangent(name: str, *tensors) -> None:
 def call_on(index: int, name: str, *args) -> None:
     """call() on CUDA device `index` with that device's current stream as the last
     argument: the short way for entry points whose call takes as long as their work
-    (the raw stream handle costs a tenth of a torch.cuda.Stream object)."""
-    lib = _lib or load()
-    if index == torch._C._cuda_getDevice():
-        status = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
+    (the raw stream handle costs a tenth of a torch.cuda.Stream object). A null pointer
+    is 0."""
+    if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
-            status = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(index))
+            return call_on(index, name, *args)
+    lib, stream = handle(), torch._C._cuda_getCurrentRawStream(index)
+    if name in _PACKED:
+        entry, pack, n = _PACKED[name]
+        status = lib.mom_call_packed(entry, pack(*args, stream), n)
+    else:
+        status = getattr(lib, name)(*args, stream)
     if status != OK:
         raise MomError(status, name, last_error())

@@ -143,7 +143,7 @@ def rope_append(qkv, cos, sin, positions, k_pages, v_pages, slots, *, n_heads: i
     k = torch.empty(T, Hk, hd, dtype=torch.bfloat16, device=dev) if want_k else None
     _lib.call_on(dev.index, "mom_rope_append", qkv.data_ptr(), qkv.stride(0) if T > 1 else qkv.shape[1], cos.data_ptr(),
           sin.data_ptr(), cos.shape[0], positions.data_ptr(), pcode, slots.data_ptr(), scode, T, H, Hk, hd, P, page,
-          k_pages.data_ptr(), v_pages.data_ptr(), q.data_ptr(), None if k is None else k.data_ptr())
+          k_pages.data_ptr(), v_pages.data_ptr(), q.data_ptr(), 0 if k is None else k.data_ptr())
     return q, k
 
 
@@ -263,11 +263,11 @@ def decode_attention(q, k_pages, v_pages, block_table, seq_lens, *, scale=None, 
     dev = q.device
     block_table, table_ld, seq_lens, max_len = _block_table("decode_attention", block_table, seq_lens, B, page, max_len, dev)
     out = torch.empty(B, H, hd, dtype=torch.bfloat16, device=dev)
-    need = _lib.load().mom_decode_attn_workspace_size(B, H, Hk, hd, max_len)
+    need = _lib.handle().mom_decode_attn_workspace_size(B, H, Hk, hd, max_len)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     _lib.call_on(dev.index, "mom_decode_attn", q.data_ptr(), q_ld, k_pages.data_ptr(), v_pages.data_ptr(), P, page,
           block_table.data_ptr(), table_ld, seq_lens.data_ptr(), max_len, B, H, Hk, hd,
-          hd ** -0.5 if scale is None else float(scale), out.data_ptr(), None if ws is None else ws.data_ptr(), need)
+          hd ** -0.5 if scale is None else float(scale), out.data_ptr(), 0 if ws is None else ws.data_ptr(), need)
     return out
 
 
@@ -324,7 +324,7 @@ def rope_append_int4(qkv, cos, sin, positions, k_pages, v_pages, scales, slots, 
     _lib.call_on(dev.index, "mom_rope_append_int4", qkv.data_ptr(), qkv.stride(0) if T > 1 else qkv.shape[1],
                  cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(), pcode, slots.data_ptr(), scode, T, H,
                  Hk, hd, P, page, k_pages.data_ptr(), v_pages.data_ptr(), scales.data_ptr(), q.data_ptr(),
-                 None if k is None else k.data_ptr(), None if v is None else v.data_ptr())
+                 0 if k is None else k.data_ptr(), 0 if v is None else v.data_ptr())
     return q, k, v
 
 
@@ -359,12 +359,12 @@ def decode_attention_int4(q, k_pages, v_pages, scales, block_table, seq_lens, *,
         new_lens = new_lens.contiguous()
     block_table, table_ld, seq_lens, max_len = _block_table(name, block_table, seq_lens, B, page, max_len, dev)
     out = torch.empty(B, n, H, hd, dtype=torch.bfloat16, device=dev)
-    need = _lib.load().mom_decode_attn_int4_workspace_size(B, n, H, Hk, hd, max_len)
+    need = _lib.handle().mom_decode_attn_int4_workspace_size(B, n, H, Hk, hd, max_len)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     _lib.call_on(dev.index, "mom_decode_attn_int4", q.data_ptr(), q_ld, k_pages.data_ptr(), v_pages.data_ptr(),
                  scales.data_ptr(), P, page, block_table.data_ptr(), table_ld, seq_lens.data_ptr(),
-                 None if new_lens is None else new_lens.data_ptr(), max_len, B, n, H, Hk, hd,
-                 hd ** -0.5 if scale is None else float(scale), out.data_ptr(), None if ws is None else ws.data_ptr(), need)
+                 0 if new_lens is None else new_lens.data_ptr(), max_len, B, n, H, Hk, hd,
+                 hd ** -0.5 if scale is None else float(scale), out.data_ptr(), 0 if ws is None else ws.data_ptr(), need)
     return out
 
 

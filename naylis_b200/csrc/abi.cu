@@ -11,6 +11,8 @@
 #include <atomic>
 #include <exception>
 #include <mutex>
+#include <type_traits>
+#include <utility>
 
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -1238,6 +1240,47 @@ int noalloc_scratch(void **ptr) {
     return MOM_OK;
 }
 }  // namespace
+
+}  // extern "C"
+
+namespace {
+template <typename A>
+A packed_arg(const void *args, size_t i) {
+    const char *at = static_cast<const char *>(args) + 8 * i;
+    if constexpr (std::is_floating_point_v<A>) {
+        double v;
+        std::memcpy(&v, at, 8);
+        return static_cast<A>(v);
+    } else {
+        int64_t v;
+        std::memcpy(&v, at, 8);
+        if constexpr (std::is_pointer_v<A>) return reinterpret_cast<A>(static_cast<uintptr_t>(v));
+        else return static_cast<A>(v);
+    }
+}
+template <typename... A, size_t... I>
+int call_with(int (*entry)(A...), const void *args, std::index_sequence<I...>) {
+    return entry(packed_arg<A>(args, I)...);
+}
+template <typename... A>
+int call_packed(int (*entry)(A...), const void *args, int n) {
+    MOM_REQUIRE(args && n == static_cast<int>(sizeof...(A)), "%d packed arguments, %d needed", n, static_cast<int>(sizeof...(A)));
+    return call_with(entry, args, std::index_sequence_for<A...>{});
+}
+}  // namespace
+
+extern "C" {
+
+int mom_call_packed(int entry, const void *args, int n) {
+    switch (entry) {
+        case MOM_CALL_ROPE_APPEND: return call_packed(mom_rope_append, args, n);
+        case MOM_CALL_DECODE_ATTN: return call_packed(mom_decode_attn, args, n);
+        case MOM_CALL_ROPE_APPEND_INT4: return call_packed(mom_rope_append_int4, args, n);
+        case MOM_CALL_DECODE_ATTN_INT4: return call_packed(mom_decode_attn_int4, args, n);
+        case MOM_CALL_VERIFY_DRAFTS: return call_packed(mom_verify_drafts, args, n);
+    }
+    return fail(MOM_ERR_INVALID_ARGUMENT, "no packed entry %d", entry);
+}
 
 size_t mom_read_bwd_noalloc_max_bytes(void) { return kNoAllocScratchBytes; }
 

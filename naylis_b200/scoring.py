@@ -181,8 +181,8 @@ def verify_drafts(logits, drafts, uniforms=None, *, draft_logits=None, temperatu
     tokens = torch.empty(B, K + 1, dtype=torch.int64, device=dev)
     accepted = torch.empty(B, dtype=torch.int64, device=dev)
     _lib.call_on(dev.index, "mom_verify_drafts", logits.data_ptr(), _code(logits), ld_seq, ld_row,
-                 None if draft_logits is None else draft_logits.data_ptr(), draft_ld_seq, draft_ld_row, drafts.data_ptr(),
-                 None if uniforms is None else uniforms.data_ptr(), None if draft_lens is None else draft_lens.data_ptr(),
+                 0 if draft_logits is None else draft_logits.data_ptr(), draft_ld_seq, draft_ld_row, drafts.data_ptr(),
+                 0 if uniforms is None else uniforms.data_ptr(), 0 if draft_lens is None else draft_lens.data_ptr(),
                  B, K, V, temperature, tokens.data_ptr(), accepted.data_ptr())
     return Verified(tokens, accepted)
 

@@ -1,6 +1,8 @@
 """CPU tests of the 4-bit cache's and the drafts' entry points of the C ABI: the arguments
 they reject before any device work, and the sizes that the host has to get right."""
 import ctypes
+import os
+import re
 
 import pytest
 
@@ -105,3 +107,21 @@ def test_the_python_calls_refuse_what_is_not_on_a_gpu():
         attention.rope_append_int4(q.view(1, 64), s, s, i, k, k, s, i, n_heads=1)
     with pytest.raises(RuntimeError, match="verify_drafts"):
         scoring.verify_drafts(torch.zeros(1, 2, 5), torch.zeros(1, 1, dtype=torch.int64), torch.zeros(1, 2))
+
+
+def test_packed_calls(lib):
+    """Entries of call_on()'s short way are the header's, and take all of their arguments."""
+    from naylis_b200 import _lib
+    header = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "naylis_mom.h")).read()
+    entries = {f"mom_{n.lower()}": int(i) for n, i in re.findall(r"MOM_CALL_(\w+) = (\d+)", header)}
+    assert entries == {name: i for name, (i, _, _) in _lib._PACKED.items()}
+    for name, (entry, pack, n) in _lib._PACKED.items():
+        kinds = _lib.SIGNATURES[name][1]
+        args = pack(*(0.5 if k is ctypes.c_double else 0 for k in kinds))
+        assert len(args) == 8 * n == 8 * len(kinds)
+        one = getattr(lib, name)(*(0.5 if k is ctypes.c_double else 0 for k in kinds))
+        error = _lib.last_error()
+        packed = lib.mom_call_packed(entry, args, n)
+        assert packed == one and one != 0 and _lib.last_error() == error
+        assert lib.mom_call_packed(entry, args, n - 1) == 1 and "packed arguments" in _lib.last_error()
+    assert lib.mom_call_packed(len(entries), b"", 0) == 1 and "no packed entry" in _lib.last_error()
