@@ -17,7 +17,7 @@
 // One cluster takes a sequence. Its warps share the rows out for the 32-bit sums, each some
 // contiguous part of one row at a time; in 64 bits each has a stretch of the vocabulary, whose
 // exponentials it keeps in shared memory where they fit (the search then reads them).
-// Rows of 32000, bf16: 1 sequence of 4 drafts 12 us, 48 of 4 23 us, 40 of 7 in fp32 17 us (drafts
+// Rows of 32000, bf16: 1 sequence of 4 drafts 12 us, 48 of 4 22 us, 40 of 7 in fp32 17 us (drafts
 // without logits), bound by the chain of phases (sums, decision, the row's terms, search), a barrier
 // behind each; 256 of 7 greedily 25 us, 5.2 TB/s, by memory.
 #include <algorithm>
@@ -38,8 +38,11 @@ constexpr int kRounds = 9;          // parts of rows that a warp takes, at most:
 constexpr int kTableBits = 7, kTable = 1 << kTableBits;
 constexpr int kMostKeep = 8300;     // doubles that a CTA keeps, for three CTAs an SM
 
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+    cluster_arrive();
+    cluster_wait();
 }
 // The same place in the shared memory of the cluster's CTA `rank`.
 __device__ __forceinline__ uint64_t ld_cluster(const void *p, int rank) {
@@ -114,7 +117,7 @@ __global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const 
     __shared__ uint64_t s_row[kRows];           // of whole rows
     __shared__ int s_verdict[kMaxDrafts];
     __shared__ double s_part[2][kWarps];        // the warps' sums in 64 bits, for the target and the draft
-    __shared__ double s_whole[2], s_left[kWarps], s_find[2], s_table[kTable];
+    __shared__ double s_left[kWarps], s_find[2], s_table[kTable];
     __shared__ int s_owner;
     const int b = static_cast<int>(blockIdx.y), me = static_cast<int>(blockIdx.x), ctas = P.ctas;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -153,8 +156,6 @@ __global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const 
             }
         }
     }
-    if constexpr (!Greedy)
-        if (threadIdx.x < kTable) s_table[threadIdx.x] = exp2(static_cast<double>(threadIdx.x) / kTable);
 
     // ---- every row's greatest logit and sum: parts of rows, as many as give each warp about the same
     int parts = 1;
@@ -258,17 +259,23 @@ __global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const 
         }
         if (lane == 0) s_unit[round][warp] = best;
     }
-    cluster_sync();
-    for (int r = warp; r < rows; r += kWarps) {
+    cluster_arrive();
+    if constexpr (!Greedy)      // while the others arrive
+        if (threadIdx.x < kTable) s_table[threadIdx.x] = exp2(static_cast<double>(threadIdx.x) / kTable);
+    cluster_wait();
+    // a row to a warp, or two where that takes the warps fewer turns: a turn is a read from another CTA
+    const int team = rows > kWarps ? 16 : 32, mate = lane & (team - 1);
+    for (int r0 = warp * 32 / team; r0 < rows; r0 += kWarps * 32 / team) {
+        const int r = r0 + lane / team;
         uint64_t got = kNothing;
-        for (int part = lane; part < parts; part += 32) {
+        for (int part = mate; part < parts && r < rows; part += team) {
             const int unit = r * parts + part, of = unit % W;
             got = join(got, ld_cluster(&s_unit[unit / W][of % kWarps], of / kWarps));
         }
-        got = join_lanes(got);
+        for (int o = team / 2; o > 0; o >>= 1) got = join(got, __shfl_xor_sync(0xffffffffu, got, o));
         // Greedy: the token, -1 for a row with a NaN
         if (Greedy) got = static_cast<uint32_t>(got >> 32) == 0xffffffffu ? ~0ull : static_cast<uint64_t>(rank_index(got));
-        if (lane == 0) s_row[r] = got;
+        if (mate == 0 && r < rows) s_row[r] = got;
     }
     __syncthreads();
 
@@ -419,17 +426,20 @@ __global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const 
             if (both) c = warp_sum(c);
             if (lane == 0) s_part[0][warp] = a, s_part[1][warp] = c;
             if (both || verdict == kUnsure) {
-                __syncthreads();
-                if (threadIdx.x < 2) {
-                    double s = 0.0;
-#pragma unroll
-                    for (int i = 0; i < kWarps; ++i) s += s_part[threadIdx.x][i];
-                    s_whole[threadIdx.x] = s;
-                }
                 cluster_sync();
-                // all CTAs' sums by the lanes at once, then the same sum in each
-                const double zp = warp_sum(lane < ctas ? ld_cluster(&s_whole[0], lane) : 0.0);
-                const double zq = both ? warp_sum(lane < ctas ? ld_cluster(&s_whole[1], lane) : 0.0) : 0.0;
+                // all warps' sums by the lanes at once, in the same order everywhere
+                const auto whole = [&](const double (&part)[kWarps]) {
+                    double x[kMostCtas * kWarps / 32], sum = 0.0;
+#pragma unroll
+                    for (int k = 0; k < kMostCtas * kWarps / 32; ++k) {
+                        const int i = lane + 32 * k;
+                        x[k] = i < W ? ld_cluster(&part[i % kWarps], i / kWarps) : 0.0;
+                    }
+#pragma unroll
+                    for (int k = 0; k < kMostCtas * kWarps / 32; ++k) sum += x[k];
+                    return warp_sum(sum);
+                };
+                const double zp = whole(s_part[0]), zq = both ? whole(s_part[1]) : 0.0;
                 if (verdict == kUnsure) {
                     const float u = P.uniforms[static_cast<int64_t>(b) * (P.K + 1) + stay];
                     bool near;
@@ -439,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const 
                     __syncthreads();
                     continue;
                 }
-                fp = 1.0 / zp, fq = 1.0 / zq;
+                fp = zq, fq = zp;      // p - q, times both sums
             }
             if (both) {
                 a = 0.0;
