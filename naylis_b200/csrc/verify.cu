@@ -17,7 +17,7 @@
 // One cluster takes a sequence. Its warps share the rows out for the 32-bit sums, each some
 // contiguous part of one row at a time; in 64 bits each has a stretch of the vocabulary, whose
 // exponentials it keeps in shared memory where they fit (the search then reads them).
-// Rows of 32000, bf16: 1 sequence of 4 drafts 12 us, 48 of 4 22 us, 40 of 7 in fp32 17 us (drafts
+// Rows of 32000, bf16: 1 sequence of 4 drafts 11 us, 48 of 4 22 us, 40 of 7 in fp32 17 us (drafts
 // without logits), bound by the chain of phases (sums, decision, the row's terms, search), a barrier
 // behind each; 256 of 7 greedily 25 us, 5.2 TB/s, by memory.
 #include <algorithm>
@@ -116,6 +116,7 @@ __global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const 
     __shared__ uint64_t s_unit[kRounds][kWarps];      // the greatest logit and the sum (Greedy: rank key) of a part of a row
     __shared__ uint64_t s_row[kRows];           // of whole rows
     __shared__ int s_verdict[kMaxDrafts];
+    __shared__ int64_t s_draft[Greedy ? 1 : kMaxDrafts];
     __shared__ double s_part[2][kWarps];        // the warps' sums in 64 bits, for the target and the draft
     __shared__ double s_left[kWarps], s_find[2], s_table[kTable];
     __shared__ int s_owner;
@@ -263,8 +264,9 @@ __global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const 
     if constexpr (!Greedy)      // while the others arrive
         if (threadIdx.x < kTable) s_table[threadIdx.x] = exp2(static_cast<double>(threadIdx.x) / kTable);
     cluster_wait();
-    // a row to a warp, or two where that takes the warps fewer turns: a turn is a read from another CTA
-    const int team = rows > kWarps ? 16 : 32, mate = lane & (team - 1);
+    // a row to a warp, or with the drafts' rows two where that takes fewer turns: a turn is a read from another CTA (0.4
+    // us of 1 x 4; at 8 rows without the drafts' the choice itself would cost as much)
+    const int team = Own && rows > kWarps ? 16 : 32, mate = lane & (team - 1);
     for (int r0 = warp * 32 / team; r0 < rows; r0 += kWarps * 32 / team) {
         const int r = r0 + lane / team;
         uint64_t got = kNothing;
@@ -282,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const 
     int64_t *tokens = P.tokens + static_cast<int64_t>(b) * (P.K + 1);
     auto finish = [&](int stay) {      // by the one CTA that knows the token: all but that
         for (int j = threadIdx.x; j <= P.K; j += kThreads)
-            if (j != stay) tokens[j] = j < stay ? drafts[j] : -1;
+            if (j != stay) tokens[j] = j >= stay ? -1 : Greedy ? drafts[j] : s_draft[j];
         if (threadIdx.x == 0) P.accepted[b] = stay;
     };
     if constexpr (Greedy) {
@@ -327,6 +329,7 @@ __global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const 
                 if (near) v = kUnsure;
             }
             s_verdict[j] = v;
+            s_draft[j] = draft;
         }
         __syncthreads();
         // where the running sum passes u times the whole: among the cluster's stretches
@@ -393,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const 
                 cluster_sync();
                 return;
             }
-            const int64_t d = stay < n ? drafts[stay] : -1;
+            const int64_t d = stay < n ? s_draft[stay] : -1;
             both = Own && stay < n && !own_alone;
             skip = !Own && verdict == kFalls && !own_alone && d >= 0 && d < P.V ? static_cast<int>(d) : -1;
             p = row_of(stay), q = both ? row_of(n + 1 + stay) : p;
@@ -402,11 +405,27 @@ __global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const 
             // a batch of both rows on its way together, and its terms side by side: each is a chain of a dozen operations
             for (int i = e0 + lane; i - lane < e1; i += 32 * kBatch) {
                 float x[2][kBatch];
+                if constexpr (Own) {
+                    // (unconditional, where there is nothing from the stretch's last place: under conditions 16 loads take turns,
+                    // 1 x 4 0.4 us; 8 did not)
 #pragma unroll
-                for (int k = 0; k < kBatch; ++k) {
-                    const int at = i + 32 * k;
-                    x[0][k] = at < e1 && at != skip ? Elem<DT>::load(p, at) : -INFINITY;
-                    x[1][k] = both && at < e1 ? Elem<DT>::load(q, at) : -INFINITY;
+                    for (int k = 0; k < kBatch; ++k) x[0][k] = Elem<DT>::load(p, min(i + 32 * k, e1 - 1));
+                    if (both) {
+#pragma unroll
+                        for (int k = 0; k < kBatch; ++k) x[1][k] = Elem<DT>::load(q, min(i + 32 * k, e1 - 1));
+                    }
+#pragma unroll
+                    for (int k = 0; k < kBatch; ++k) {
+                        const int at = i + 32 * k;
+                        if (at >= e1) x[0][k] = x[1][k] = -INFINITY;
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < kBatch; ++k) {
+                        const int at = i + 32 * k;
+                        x[0][k] = at < e1 && at != skip ? Elem<DT>::load(p, at) : -INFINITY;
+                        x[1][k] = -INFINITY;
+                    }
                 }
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
