@@ -305,7 +305,8 @@ def rope_append_int4(qkv, cos, sin, positions, k_pages, v_pages, scales, slots, 
     number n = round((x - zero) / scale), 0 to 15 (0 where scale is 0): it stands for
     zero + n scale. A group with a value that is not finite, or a range beyond fp32,
     stands for NaN. Two numbers share a byte, the even dimension's in the low half;
-    the last axis of scales is the key's scale and zero, then the value's.
+    the last axis of scales is the key's scale and zero, then the value's. Tokens of one
+    call have slots of their own: of two with the same one, parts of either may be kept.
 
     Returns (q (T, n_heads, hd) rotated, k, v): with want_kv what the filed keys and
     values stand for, rounded to bf16, (T, n_kv_heads, hd), so that a prefill attends

@@ -224,16 +224,16 @@ def test_wide_scores(hd):
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("H,n", [(2, 1), (8, 1), (2, 5), (8, 5)])
 @pytest.mark.parametrize("size", [1e3, 1e9, 1e25])
-def test_huge_scores(hd, H, n, size):
+@pytest.mark.parametrize("lens", [[9000, 300], [400, 130]], ids=str)
+def test_huge_scores(hd, H, n, size, lens):
     """Scores far beyond where fp32 has fractions, the greatest 1 % and more above all others: it has all the weight.
     Products and sums are within 2^-18 of a score, so no other comes near it."""
-    lens = [9000, 300]
     q, (k, v, s), table, sl = _case(hd, H, 2, 16, lens, n, seed=14)
     s = torch.nan_to_num(s.float(), nan=0.5)
     g = torch.Generator().manual_seed(15)
     s[..., 0] = 0
     s[..., 1] = (torch.rand(s.shape[:3], generator=g).to(DEV) * 150 + 30)[..., None]
-    for b, at in ((0, 7001), (1, 117)):
+    for b, at in ((0, 7 * lens[0] // 9), (1, 117)):
         s[int(table[b, at // 16]), :, at % 16, :, 1] = 187.0
     s = s.to(torch.bfloat16)
     q = torch.full_like(q, size) * (1 + torch.arange(H, device=DEV)[:, None] / 16).to(torch.bfloat16)
