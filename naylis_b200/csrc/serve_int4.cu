@@ -209,11 +209,12 @@ rope_append_int4_kernel(const uint16_t *__restrict__ qkv, int64_t ld, const floa
 // shared out over all lanes. More than 8 rows are lists of their own, which read the keys
 // again (from L2: 24 sequences of 1024 to 8191, 20 rows on each of 4 heads of 128: 52 us; up to 16
 // or 24 rows a list, whose sums leave room for 2 CTAs an SM: 56 and 59). The queries of a row are scaled by a power of two to 2^9 .. 2^10 at most, so that fp16
-// holds all their bits. The weights p_t s_t are fp16, scaled by a power of two above every
-// scale so far: 11 bits, a quarter of the output's own rounding; those below 2^-36 of the
-// largest lose bits. p is taken against a reference within 2^3 of the greatest so far, which
-// moves when that is passed: no search for the maximum in a tile that does not. Everything
-// else is fp32.
+// holds all their bits. The weights p_t s_t are fp16, against a unit for each row and group, a
+// power of two: 11 bits, a quarter of the output's own rounding; those below 2^-25 of the row's
+// greatest so far lose bits, below 2^-36 they vanish. p is taken against a reference within 2^3 of the greatest so far, which
+// moves when that is passed: no search for the maximum in a tile that does not. The unit likewise is lowered when a weight
+// passes 2^15, and rises with the reference: keys that a row does not see, or that have no weight, do not
+// count for it, whatever their scales. Everything else is fp32.
 //
 // A warp takes tiles of 64 keys (hd 128: 32) through a ring of its own, as the bf16 kernel
 // does, by bulk copies: a lane for each page's keys, values or scales (16-byte copies of
@@ -226,6 +227,8 @@ rope_append_int4_kernel(const uint16_t *__restrict__ qkv, int64_t ld, const floa
 // issue with many rows, by starts and ends of lists when these are short (48 of 64 to 4096, 16
 // heads of 64: 24 us; 1 of 577: 5 us).
 constexpr float kSlack = 3.0f;      // log2
+constexpr int kMostUnit = 120;      // log2 of the weights' greatest unit: 2^4 times it, the most that kSlack rounds to, is in fp32
+constexpr float kMostWeight = 32768.0f;      // what weights stay below, fp16 having 65504
 constexpr int kLeast = 4;           // tiles of a CTA's span, at least
 constexpr int kListCost = 6;        // tiles that a list's start and end cost
 constexpr int kMostRows = 8;        // of a list
@@ -521,13 +524,10 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
         float acc[NG][NA][4], m[2] = {-INFINITY, -INFINITY};
         float far[2] = {-INFINITY, -INFINITY};      // a score above moves the references
         uint64_t l2 = none2, z2[NG], ref = none2;   // ref: what is added to a score for its weight, -m or 0
-        int top[NG];                    // 2^(top - 127) is above every scale so far
-        float above[NG], unit[NG];      // that, and the weights' unit
+        uint64_t unit[NG];      // of each row's weights, a power of two
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-            top[g] = 15;
-            above[g] = pow2(15 - 127);
-            unit[g] = pow2(139 - 15);
+            unit[g] = tc::f2(pow2(kMostUnit), pow2(kMostUnit));
             z2[g] = none2;
 #pragma unroll
             for (int i = 0; i < NA; ++i)
@@ -551,36 +551,60 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                 }
             }
         };
-        // `most`, the greatest of the values' scales of this lane's keys: a finite one above the power of two so far raises it
-        auto raise = [&](int g, float most) {
-            if (__any_sync(0xffffffffu, most >= above[g])) {
-                const int to = static_cast<int>(__reduce_max_sync(0xffffffffu, __float_as_uint(most)) >> 23) + 1;
-                const float f = to - top[g] <= 126 ? pow2(top[g] - to) : 0.0f;
-                top[g] = to;
-                above[g] = to <= 254 ? pow2(to - 127) : INFINITY;
-                unit[g] = pow2(139 - to);
-                rescale(g, f, f);
+        // over the lanes that share a row
+        const auto most_of_row = [&](float x) {
+#pragma unroll
+            for (int o = ROWS == 1 ? 1 : 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+            return x;
+        };
+        const auto exponent = [](float x) { return (__float_as_int(x) >> 23) - 127; };      // of a positive one
+        // x0, x1: the greatest weights times scales of this lane's keys, times 2^-8 (finite where the scales are). Rows
+        // whose weights pass kMostWeight get the unit that brings the greatest to 2^11 .. 2^12.
+        auto lower = [&](int g, float x0, float x1) {
+            const float2 u = tc::f2_split(unit[g]);
+            float x[2] = {x0, x1}, from[2] = {u.x, u.y}, f[2];
+#pragma unroll
+            for (int e = 0; e < (ROWS == 8 ? 2 : 1); ++e) {
+                x[e] = most_of_row(x[e]);
+                const int was = exponent(from[e]);
+                const int to = x[e] * 256.0f * from[e] >= kMostWeight ? max(3 - exponent(x[e]), -126) : was;
+                f[e] = to - was < -126 ? 0.0f : pow2(to - was);
+                from[e] = pow2(to);
             }
+            if (ROWS < 8) f[1] = f[0], from[1] = from[0];
+            unit[g] = tc::f2(from[0], from[1]);
+            rescale(g, f[0], f[1]);
         };
         // the references to the greatest scores, over the lanes that share a row
         auto move = [&](float x0, float x1) {
-            float f[2], x[2] = {fmaxf(x0, m[0]), fmaxf(x1, m[1])};      // not NaN
+            float f[2], rise[2], x[2] = {fmaxf(x0, m[0]), fmaxf(x1, m[1])};      // not NaN
 #pragma unroll
             for (int e = 0; e < (ROWS == 8 ? 2 : 1); ++e) {
-#pragma unroll
-                for (int o = ROWS == 1 ? 1 : 4; o < 32; o <<= 1) x[e] = fmaxf(x[e], __shfl_xor_sync(0xffffffffu, x[e], o));
-                f[e] = x[e] > m[e] ? tc::ex2(m[e] - x[e]) : 1.0f;
+                x[e] = most_of_row(x[e]);
+                rise[e] = x[e] > m[e] ? x[e] - m[e] : 0.0f;      // (from -inf: inf)
+                f[e] = tc::ex2(-rise[e]);
                 m[e] = x[e];
                 far[e] = x[e] + kSlack;
             }
-            if (ROWS < 8) f[1] = f[0];
+            if (ROWS < 8) f[1] = f[0], rise[1] = rise[0];
             ref = tc::f2(m[0] == -INFINITY ? 0.0f : -m[0], m[1] == -INFINITY ? 0.0f : -m[1]);
             const uint64_t f2 = tc::f2(f[0], f[1]);
             l2 = tc::mul2(l2, f2);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 z2[g] = tc::mul2(z2[g], f2);
-                rescale(g, f[0], f[1]);
+                // weights that have become small get a larger unit, their sums so far keep theirs
+                const float2 u = tc::f2_split(unit[g]);
+                float from[2] = {u.x, u.y}, back[2];
+#pragma unroll
+                for (int e = 0; e < (ROWS == 8 ? 2 : 1); ++e) {
+                    const int was = exponent(from[e]), by = min(__float2int_rn(rise[e]), kMostUnit - was);
+                    back[e] = tc::ex2(static_cast<float>(by) - rise[e]);
+                    from[e] = pow2(was + by);
+                }
+                if (ROWS < 8) back[1] = back[0], from[1] = from[0];
+                unit[g] = tc::f2(from[0], from[1]);
+                rescale(g, back[0], back[1]);
             }
         };
         const auto low = [](uint64_t v) { return tc::f2_split(v).x; };
@@ -593,7 +617,7 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
         for (int i = (warp - taken) & (kDecWarps - 1); i < tiles; i += kDecWarps) {
             if (waits && !wait_phase(&s_full[warp][head], parity)) waits = false;
             lost |= (bad >> head & 1) || !waits;
-            const int key0 = (i0 + i) * kTile, there = len.n - key0;      // there: keys of the sequence from here on
+            const int key0 = (i0 + i) * kTile;
             const unsigned char *sk = dsm + (warp * C::kStages + head) * C::kStage, *sv = sk + C::kSide, *ss = sv + C::kSide;
             const bool masked = key0 + kTile > all_see;
             // the two words that a thread multiplies of a key's group
@@ -633,14 +657,9 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                 for (int k = 0; k < kKeys; ++k) t[k] = 0.0f;
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    float most = 0.0f;
 #pragma unroll
-                    for (int k = 0; k < kKeys; ++k) {
-                        const int key = 32 * k + 8 * c4 + r8;
-                        raw[g][k] = *reinterpret_cast<const uint2 *>(ss + key * C::kScaleBytes + 8 * g);
-                        if (key < there) most = fmaxf(most, bf_lo(raw[g][k].y));
-                    }
-                    raise(g, most);
+                    for (int k = 0; k < kKeys; ++k)
+                        raw[g][k] = *reinterpret_cast<const uint2 *>(ss + (32 * k + 8 * c4 + r8) * C::kScaleBytes + 8 * g);
                     float d[NB / 2][4];
 #pragma unroll
                     for (int mt = 0; mt < NB / 2; ++mt)
@@ -668,17 +687,42 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
 #pragma unroll
                 for (int k = 0; k < kKeys; ++k) mx = fmaxf(mx, t[k]);
                 if (__any_sync(0xffffffffu, mx * low(crow) > far[0])) move(mx * low(crow), -INFINITY);
+                float w[NG][kKeys];
+                const auto weigh = [&] {
+                    float most = 0.0f;
+#pragma unroll
+                    for (int g = 0; g < NG; ++g)
+#pragma unroll
+                        for (int k = 0; k < kKeys; ++k) {
+                            w[g][k] = t[k] * low(unit[g]) * bf_lo(raw[g][k].y);
+                            most = fmaxf(most, w[g][k]);
+                        }
+                    return most;
+                };
+#pragma unroll
+                for (int k = 0; k < kKeys; ++k) {
+                    t[k] = tc::ex2(weight_of(t[k], 0));
+                    l2 = tc::f2(low(l2) + t[k], 0.0f);
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) z2[g] = tc::f2(fmaf(t[k], bf_hi(raw[g][k].y), low(z2[g])), 0.0f);
+                }
+                if (__any_sync(0xffffffffu, weigh() >= kMostWeight)) {
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        float most = 0.0f;
+#pragma unroll
+                        for (int k = 0; k < kKeys; ++k) most = fmaxf(most, t[k] * (bf_lo(raw[g][k].y) * 0x1p-8f));
+                        lower(g, most, 0.0f);
+                    }
+                    weigh();
+                }
                 // weights to the lanes that multiply them: key t at (t mod 4, t / 4), once in the low half and once in the high one
 #pragma unroll
                 for (int k = 0; k < kKeys; ++k) {
                     const int key = 32 * k + 8 * c4 + r8;
-                    const float p = tc::ex2(weight_of(t[k], 0));
-                    l2 = tc::f2(low(l2) + p, 0.0f);
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
-                        const float w = p * (bf_lo(raw[g][k].y) * unit[g]);
-                        z2[g] = tc::f2(fmaf(p, bf_hi(raw[g][k].y), low(z2[g])), 0.0f);
-                        const uint32_t half = pack_f16x2(w, 0.0f);
+                        const uint32_t half = pack_f16x2(w[g][k], 0.0f);
                         uint32_t *to = s_w + 8 * C::kStride * g + (key & 3) * C::kStride + (key >> 2);
                         to[0] = half;
                         to[4 * C::kStride] = half << 16;
@@ -709,17 +753,8 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                 uint2 raw[NG][NB];
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    float most = 0.0f;
 #pragma unroll
                     for (int n = 0; n < NB; ++n) raw[g][n] = *reinterpret_cast<const uint2 *>(ss + (8 * n + mine) * C::kScaleBytes + 8 * g);
-                    if (there < kTile) {
-#pragma unroll
-                        for (int n = 0; n < NB; ++n)
-                            if (8 * n + mine >= there) raw[g][n].y = 0u;
-                    }
-#pragma unroll
-                    for (int n = 0; n < NB; n += 2) most = tc::fmax3(most, bf_lo(raw[g][n].y), bf_lo(raw[g][n + 1].y));
-                    raise(g, most);
 #pragma unroll
                     for (int mt = 0; mt < NB / 2; ++mt) {
                         float d[4];
@@ -746,6 +781,38 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
 #pragma unroll
                 for (int n = 0; n < NB; n += 2) mx = tc::fmax3(mx, t[n], t[n + 1]);
                 if (__any_sync(0xffffffffu, mx * low(crow) > far[0])) move(mx * low(crow), -INFINITY);
+                uint32_t pw[NG][NB];
+                const auto weigh = [&] {
+                    float most = 0.0f;
+#pragma unroll
+                    for (int g = 0; g < NG; ++g)
+#pragma unroll
+                        for (int n = 0; n < NB; n += 2) {
+                            const float w = t[n] * low(unit[g]) * bf_lo(raw[g][n].y);
+                            const float w2 = t[n + 1] * low(unit[g]) * bf_lo(raw[g][n + 1].y);
+                            pw[g][n] = pack_f16x2(w, w);
+                            pw[g][n + 1] = pack_f16x2(w2, w2);
+                            most = tc::fmax3(most, w, w2);
+                        }
+                    return most;
+                };
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    t[n] = tc::ex2(weight_of(t[n], 0));
+                    l2 = tc::f2(low(l2) + t[n], 0.0f);
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) z2[g] = tc::f2(fmaf(t[n], bf_hi(raw[g][n].y), low(z2[g])), 0.0f);
+                }
+                if (__any_sync(0xffffffffu, weigh() >= kMostWeight)) {
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        float most = 0.0f;
+#pragma unroll
+                        for (int n = 0; n < NB; ++n) most = fmaxf(most, t[n] * (bf_lo(raw[g][n].y) * 0x1p-8f));
+                        lower(g, most, 0.0f);
+                    }
+                    weigh();
+                }
                 // weights: transposed, a thread has those of keys in rows 2 c4 and 2 c4 + 1 of row r8 / 2: in an even column
                 // for the words' low halves, in an odd one for the high ones
                 const uint32_t first = r8 & 1 ? 0x1044u : 0x4410u, second = r8 & 1 ? 0x3244u : 0x4432u;
@@ -753,13 +820,9 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                 float d[NG][2][4];
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {
-                    const float p = tc::ex2(weight_of(t[n], 0));
-                    l2 = tc::f2(low(l2) + p, 0.0f);
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
-                        const float w = p * (bf_lo(raw[g][n].y) * unit[g]);
-                        z2[g] = tc::f2(fmaf(p, bf_hi(raw[g][n].y), low(z2[g])), 0.0f);
-                        const uint32_t both = transpose8(pack_f16x2(w, w));
+                        const uint32_t both = transpose8(pw[g][n]);
                         const int at = 8 * n * C::kRowBytes + 32 * g;
                         value_products(d[g], *reinterpret_cast<const uint32_t *>(v0 + at), *reinterpret_cast<const uint32_t *>(v1 + at),
                                        __byte_perm(both, 0, first), __byte_perm(both, 0, second), n == 0);
@@ -768,22 +831,14 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
 #pragma unroll
                 for (int g = 0; g < NG; ++g) add(g, d[g]);
             } else {
-                // [group][key's, value's][key]: scale, scale, zero, zero in fp32, once for the warp, each
-                // lane its keys'; the values' scales take the weights' unit along
+                // [group][key's, value's][key]: scale, scale, zero, zero in fp32, once for the warp, each lane its keys'
                 ulonglong2 *s_x = reinterpret_cast<ulonglong2 *>(s_w);
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    uint2 raw[kKeys];
-                    float most = 0.0f;
 #pragma unroll
                     for (int k = 0; k < kKeys; ++k) {
-                        raw[k] = *reinterpret_cast<const uint2 *>(ss + (lane + 32 * k) * C::kScaleBytes + 8 * g);
-                        if (lane + 32 * k < there) most = fmaxf(most, bf_lo(raw[k].y));
-                    }
-                    raise(g, most);
-#pragma unroll
-                    for (int k = 0; k < kKeys; ++k) {
-                        const float ks = bf_lo(raw[k].x), kz = bf_hi(raw[k].x), vs = bf_lo(raw[k].y) * unit[g], vz = bf_hi(raw[k].y);
+                        const uint2 raw = *reinterpret_cast<const uint2 *>(ss + (lane + 32 * k) * C::kScaleBytes + 8 * g);
+                        const float ks = bf_lo(raw.x), kz = bf_hi(raw.x), vs = bf_lo(raw.y), vz = bf_hi(raw.y);
                         s_x[(2 * g) * kTile + lane + 32 * k] = make_ulonglong2(tc::f2(ks, ks), tc::f2(kz, kz));
                         s_x[(2 * g + 1) * kTile + lane + 32 * k] = make_ulonglong2(tc::f2(vs, vs), tc::f2(vz, vz));
                     }
@@ -832,29 +887,53 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                 mx[0] *= c.x, mx[1] *= c.y;
                 if (__any_sync(0xffffffffu, mx[0] > far[0] || mx[1] > far[1])) move(mx[0], mx[1]);
                 uint32_t pw[NG][NB];
+                // a value's scale or zero for both rows; what a row does not see does not reach it: NaN scales neither
+                const auto seen = [&](uint64_t v, int n) {
+                    const int key = key0 + 8 * n + mine;
+                    return tc::f2(key < sees[0] ? low(v) : 0.0f, key < sees[1] ? low(v) : 0.0f);
+                };
+                float most = 0.0f;
                 auto weigh = [&](auto some_hidden) {
 #pragma unroll
                     for (int n = 0; n < NB; ++n) {
-                        const uint64_t p2 = tc::ex2_pair(tc::f2(weight_of(tc::f2_split(t[n]).x, 0), weight_of(tc::f2_split(t[n]).y, 1)));
-                        l2 = tc::add2(l2, p2);
+                        t[n] = tc::ex2_pair(tc::f2(weight_of(tc::f2_split(t[n]).x, 0), weight_of(tc::f2_split(t[n]).y, 1)));
+                        l2 = tc::add2(l2, t[n]);
 #pragma unroll
                         for (int g = 0; g < NG; ++g) {
                             ulonglong2 sz = s_x[(2 * g + 1) * kTile + 8 * n + mine];
-                            if constexpr (some_hidden.value) {
-                                // what a row does not see does not reach it: NaN scales neither
-                                const bool s0 = key0 + 8 * n + mine < sees[0], s1 = key0 + 8 * n + mine < sees[1];
-                                const float vs = low(sz.x), vz = low(sz.y);
-                                sz.x = tc::f2(s0 ? vs : 0.0f, s1 ? vs : 0.0f);
-                                sz.y = tc::f2(s0 ? vz : 0.0f, s1 ? vz : 0.0f);
-                            }
-                            z2[g] = tc::fma2(p2, sz.y, z2[g]);
-                            const float2 w = tc::f2_split(tc::mul2(p2, sz.x));
-                            pw[g][n] = transpose8(pack_f16x2(w.x, w.y));
+                            if constexpr (some_hidden.value) sz.x = seen(sz.x, n), sz.y = seen(sz.y, n);
+                            z2[g] = tc::fma2(t[n], sz.y, z2[g]);
+                            const float2 w = tc::f2_split(tc::mul2(tc::mul2(t[n], unit[g]), sz.x));
+                            pw[g][n] = pack_f16x2(w.x, w.y);
+                            most = tc::fmax3(most, w.x, w.y);
                         }
                     }
                 };
                 if (masked) weigh(std::true_type{});
                 else weigh(std::false_type{});
+                if (__any_sync(0xffffffffu, most >= kMostWeight)) {
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        const auto scale = [&](int n) { return seen(s_x[(2 * g + 1) * kTile + 8 * n + mine].x, n); };
+                        const uint64_t small = tc::f2(0x1p-8f, 0x1p-8f);
+                        float x[2] = {0.0f, 0.0f};
+#pragma unroll
+                        for (int n = 0; n < NB; ++n) {
+                            const float2 v = tc::f2_split(tc::mul2(t[n], tc::mul2(scale(n), small)));
+                            x[0] = fmaxf(x[0], v.x), x[1] = fmaxf(x[1], v.y);
+                        }
+                        lower(g, x[0], x[1]);
+#pragma unroll
+                        for (int n = 0; n < NB; ++n) {
+                            const float2 w = tc::f2_split(tc::mul2(tc::mul2(t[n], unit[g]), scale(n)));
+                            pw[g][n] = pack_f16x2(w.x, w.y);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int g = 0; g < NG; ++g)
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) pw[g][n] = transpose8(pw[g][n]);
                 const unsigned char *v0 = sv + key_of(2 * c4) * C::kRowBytes + 4 * r8, *v1 = sv + key_of(2 * c4 + 1) * C::kRowBytes + 4 * r8;
 #pragma unroll
                 for (int g = 0; g < NG; ++g)
@@ -949,20 +1028,21 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                 }
             __syncwarp();      // the warp's sums are read; their place takes its outputs
         }
-        // the numbers' 2^-24 and 2^-20 and the weights' unit taken out
-        const auto part_of = [&](int row, int g) {
+        // the numbers' 2^-24 and 2^-20 and the weights' unit taken out: that is 2^-119 (where scales are finite) to 2^120
+        const auto part_of = [&](int row, int g, int e) {
             const float f = s_m[warp][row] == -INFINITY ? 0.0f : tc::ex2(s_m[warp][row] - reference(row));
-            return pow2(min(top[g] - 127, 127)) * f;
+            const float2 u = tc::f2_split(unit[g]);
+            return pow2(min(8 - exponent(e ? u.y : u.x), 127)) * f;
         };
         const auto pair_of = [](const float (&x)[4], int e, float u) {
-            return make_float2(x[e] * 4096.0f * u, x[2 + e] * 256.0f * u);
+            return make_float2(x[e] * 65536.0f * u, x[2 + e] * 4096.0f * u);
         };
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             if constexpr (ROWS < 8) {
                 const int row = ROWS == 1 ? 0 : c4;
                 if (ROWS == 4 || c4 == 0) {
-                    const float u = part_of(row, g);
+                    const float u = part_of(row, g, 0);
                     float4 *to = reinterpret_cast<float4 *>(s_o + (warp * ROWS + row) * HD + 64 * g + 8 * r8);
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
@@ -973,7 +1053,7 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
             } else {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const float u = part_of(2 * c4 + e, g);
+                    const float u = part_of(2 * c4 + e, g, e);
                     float4 *to = reinterpret_cast<float4 *>(s_o + (warp * ROWS + 2 * c4 + e) * HD + 64 * g + 8 * r8);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
