@@ -209,7 +209,8 @@ rope_append_int4_kernel(const uint16_t *__restrict__ qkv, int64_t ld, const floa
 // shared out over all lanes. More than 8 rows are lists of their own, which read the keys
 // again (from L2: 24 sequences of 1024 to 8191, 20 rows on each of 4 heads of 128: 52 us; up to 16
 // or 24 rows a list, whose sums leave room for 2 CTAs an SM: 56 and 59). The queries of a row are scaled by a power of two to 2^9 .. 2^10 at most, so that fp16
-// holds all their bits. The weights p_t s_t are fp16, against a unit for each row and group, a
+// holds their bits: those 2^-31 of the greatest and smaller may lose some, 2^-39 of it. A score before
+// the scale is in units of that: of keys that stand for less than about 2^-100 it may lose bits. The weights p_t s_t are fp16, against a unit for each row and group, a
 // power of two: 11 bits, a quarter of the output's own rounding; those below 2^-25 of the row's
 // greatest so far lose bits, below 2^-36 they vanish. p is taken against a reference within 2^3 of the greatest so far, which
 // moves when that is passed: no search for the maximum in a tile that does not. The unit likewise is lowered when a weight
@@ -469,11 +470,13 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
             }
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // 2^up takes the greatest to 2^9 .. 2^10 (a row of tiny values not as far up: its scores are equal anyway)
-        const int up = min(136 - static_cast<int>(top >> 7), 100);
+        // 2^up takes the greatest to 2^9 .. 2^10 (from 2^-117 down not as far: multiples of 2^-133, which fp16 holds then)
+        const int up = min(136 - static_cast<int>(top >> 7), 126);
         const float f = pow2(up);
-        // positive and finite: beyond these bounds one key has all the weight, or all have the same
-        float c = fminf(fmaxf(P.scale_log2 * pow2(min(20 - up, 127)), 1e-37f), 3e38f);
+        // 2^(20 - up), up to 2^138, in two steps of one direction. Positive and finite: beyond these bounds one key has
+        // all the weight, or all have the same
+        const int back = 20 - up, half = back / 2;
+        float c = fminf(fmaxf(P.scale_log2 * pow2(half) * pow2(back - half), __int_as_float(1)), 3e38f);
         if (top >= 0x7f80u) c = __int_as_float(0x7fc00000);            // a query that is not finite
         crow = of_rows(c);
 #pragma unroll

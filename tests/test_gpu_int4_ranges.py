@@ -109,3 +109,43 @@ def test_scales_that_are_not_finite(H, Hk, n):
         hit[:, :, :H // Hk, 64:] = True
         _close(got[~hit], want[~hit], A[~hit])
         assert not bool(torch.isfinite(got[hit]).any())
+
+# ------------------------------------------------------------------ queries of any size
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("H,Hk,n", [(2, 2, 1), (2, 2, 4), (8, 2, 4)])
+@pytest.mark.parametrize("f", [3e37, 1e36, 1e34, 1e31, 1e-24, 1e-28, 1e-32, 1e-36, 1e-38, 2e-39])
+def test_queries_of_any_size(hd, H, Hk, n, f):
+    """Queries up to the greatest bf16 number and down to its subnormals, with scales that bring their
+    scores back to a few units."""
+    lens = [1000, 70]
+    q, cache, table, sl = _case(hd, H, Hk, 16, lens, n, seed=31)
+    q = (q.float() * f).clamp(-3e38, 3e38).to(torch.bfloat16)
+    scale = min(0.3 / f, 2e38)
+    got = _run(q, cache, table, sl, scale=scale)
+    want, A = _exact(q, cache, table, lens, [n] * 2, scale)
+    _close(got, want, A)
+    # the scores count: the mean of the values is something else
+    mean, _ = _exact(q * 0, cache, table, lens, [n] * 2, 1.0)
+    assert float((want - mean).abs().max()) > 0.05
+
+
+@pytest.mark.parametrize("H,Hk,n", [(2, 2, 1), (2, 2, 4), (8, 2, 4)])
+def test_queries_and_scales_at_opposite_ends(H, Hk, n):
+    """Scores far above 1 and far below it: one key has all the weight, or all have the same."""
+    lens = [1000, 70]
+    q, cache, table, sl = _case(64, H, Hk, 16, lens, n, seed=32)
+    for f, scale in ((1e-38, 1e-30), (1e-30, 1e-37), (1e-38, 1.0)):
+        x = (q.float() * f).to(torch.bfloat16)
+        _close(_run(x, cache, table, sl, scale=scale), *_exact(x, cache, table, lens, [n] * 2, scale))
+    # a key 10 % above all others, in every head
+    k, v, s = cache
+    s2 = torch.nan_to_num(s.float(), nan=0.5)
+    g = torch.Generator().manual_seed(33)
+    s2[..., 0] = 0
+    s2[..., 1] = (torch.rand(s2.shape[:3], generator=g).to(DEV) + 1)[..., None]
+    for b, at in ((0, 700), (1, 40)):
+        s2[int(table[b, at // 16]), :, at % 16, :, 1] = 2.25
+    cache = (k, v, s2.to(torch.bfloat16))
+    for f, scale in ((1e30, 1e4), (1e36, 0.1), (1e-2, 1e37), (1.0, 1e36)):
+        x = torch.full_like(q, f)
+        _close(_run(x, cache, table, sl, scale=scale), *_exact(x, cache, table, lens, [n] * 2, scale))
