@@ -622,7 +622,7 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
             lost |= (bad >> head & 1) || !waits;
             const int key0 = (i0 + i) * kTile;
             const unsigned char *sk = dsm + (warp * C::kStages + head) * C::kStage, *sv = sk + C::kSide, *ss = sv + C::kSide;
-            const bool masked = key0 + kTile > all_see;
+            const bool masked = all_see - key0 < kTile;
             // the two words that a thread multiplies of a key's group
             const auto key_words = [&](int key, int g) {
                 return *reinterpret_cast<const uint2 *>(sk + key * C::kRowBytes + 32 * g + 8 * c4);

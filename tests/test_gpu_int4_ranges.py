@@ -149,3 +149,23 @@ def test_queries_and_scales_at_opposite_ends(H, Hk, n):
     for f, scale in ((1e30, 1e4), (1e36, 0.1), (1e-2, 1e37), (1.0, 1e36)):
         x = torch.full_like(q, f)
         _close(_run(x, cache, table, sl, scale=scale), *_exact(x, cache, table, lens, [n] * 2, scale))
+
+# ------------------------------------------------------------------ the longest sequence
+@pytest.mark.parametrize("H,n", [(1, 1), (2, 2), (2, 4)])
+def test_the_longest_sequence(H, n):
+    """2^31 - 1 keys, of a few pages many times over: the place behind the last one stays hidden. Every
+    value is 1 and so is their mean, to fp32 sums of 2^31 terms over 2^16 threads (2^15 a thread, each addition
+    within 2^-24) and the result's rounding."""
+    page, longest = 256, (1 << 31) - 1
+    g = torch.Generator().manual_seed(41)
+    k = torch.randint(0, 256, (3, 1, page, 32), generator=g, dtype=torch.uint8).to(DEV)
+    v = torch.zeros_like(k)
+    s = torch.zeros(3, 1, page, 1, 4, dtype=torch.bfloat16, device=DEV)
+    s[..., 3] = 1.0
+    s[2, :, -1, :, 1], s[2, :, -1, :, 3] = 50.0, 1000.0      # behind the end, with all the weight
+    table = torch.arange((1 << 31) // page, device=DEV, dtype=torch.int32)[None] % 2
+    table[0, -1] = 2
+    q = torch.ones(1, n, H, 64, dtype=torch.bfloat16, device=DEV)
+    sl = torch.tensor([longest], dtype=torch.int32, device=DEV)
+    got = _run(q, (k, v, s), table, sl, max_len=longest)
+    assert float((got.double() - 1).abs().max()) <= 2.0 ** -7, got.flatten()[:4]
