@@ -106,6 +106,12 @@ __device__ __forceinline__ double sum_of_batch(double (&e)[kBatch]) {
     return e[0];
 }
 
+// What is left of the target for a term, max(a fa - c fc, 0). Both products are rounded, neither
+// goes into the difference whole: equal terms of equal rows leave nothing.
+__device__ __forceinline__ double left_of(double a, double fa, double c, double fc) {
+    return fmax(__dsub_rn(__dmul_rn(a, fa), __dmul_rn(c, fc)), 0.0);
+}
+
 // Greedy: a row's greatest logit, ties to the lowest index. Own: the drafts have logits.
 template <int DT, bool Greedy, bool Own>
 __global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const __grid_constant__ VerifyArgs P) {
@@ -381,9 +387,8 @@ __global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const 
         const T *p, *q;
         float mp, mq;
         auto left = [&](int i) {      // what the token is drawn from, where it is not kept
-            double v = i == skip ? 0.0 : term(Elem<DT>::load(p, i), mp);
-            if (both) v = v * fp - term(Elem<DT>::load(q, i), mq) * fq;
-            return v > 0.0 ? v : 0.0;
+            const double v = i == skip ? 0.0 : term(Elem<DT>::load(p, i), mp);
+            return both ? left_of(v, fp, term(Elem<DT>::load(q, i), mq), fq) : v;
         };
         while (true) {
             while (stay < n && s_verdict[stay] == kStays) ++stay;
@@ -478,8 +483,7 @@ __global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const 
 #pragma unroll
                         for (int k = 0; k < kBatch; ++k) {
                             const int at = i + 32 * k - c0;
-                            e[k] = i + 32 * k < e1 ? s_keep[at] * fp - s_keep[P.keep + at] * fq : 0.0;
-                            e[k] = e[k] > 0.0 ? e[k] : 0.0;
+                            e[k] = i + 32 * k < e1 ? left_of(s_keep[at], fp, s_keep[P.keep + at], fq) : 0.0;
                         }
 #pragma unroll
                         for (int k = 0; k < kBatch; ++k)

@@ -1,0 +1,35 @@
+"""GPU tests of scoring.verify_drafts where its parts meet: drafts that fall although both rows are
+one distribution, vocabularies whose terms are not kept, sums that 32 bits do not hold."""
+import pytest
+import torch
+
+from test_gpu_verify import DEV, INF, NAN, _check, _make  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ nothing left of the target
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,V", [(9, 1000), (40, 257), (9, 40000), (300, 4999)])
+@pytest.mark.parametrize("shift", [0.0, 8.0])
+def test_a_draft_falls_between_equal_rows(dtype, B, V, shift):
+    """The draft's distribution is the target's, and its draft falls all the same (outside the vocabulary, masked
+    in both rows, or a given number of 1): nothing is left, and the token is the target's own."""
+    K = 2
+    g = torch.Generator().manual_seed(V)
+    # quarters up to 16: a shift of 8 is exact in bf16
+    logits = (torch.randn(B, K + 1, V, generator=g) * 6).round().clamp(-28, 28) / 4
+    logits = logits.to(dtype).to(DEV)
+    drafts = torch.randint(0, V, (B, K), generator=g).to(DEV)
+    u = torch.rand(B, K + 1, generator=g).to(DEV)
+    u[0::4, 0] = 1.0
+    drafts[1::4, 0] = -1
+    drafts[2::4, 0] = V
+    for b in range(3, B, 4):
+        logits[b, 0, drafts[b, 0]] = -INF
+    u[4::5, 1] = 1.0
+    draft = logits[:, :K] + shift
+    want = _check(logits, drafts, u, draft, 1.0)
+    assert not want[1][:4].any() and len(set(want[0][:, 0].tolist())) > 4
+    if shift == 0.0:
+        _check(logits, drafts, u, draft, 0.7)
