@@ -11,8 +11,8 @@
 //
 // A running sum over the vocabulary decides between neighbours, so everything behind the
 // choice of the row is in 64 bits: exponentials, sums, the search. A draft's own test is a
-// comparison of two numbers: the rows' sums for it are 32-bit, and where u q and p are within
-// 2^-13 of one another, far above those sums' error, it is done again in 64 bits.
+// comparison of two numbers: the rows' sums for it are 32-bit, and where u q and p are as near one
+// another as those sums may be off, at least 2^-13, it is done again in 64 bits.
 //
 // One cluster takes a sequence. Its warps share the rows out for the 32-bit sums, each some
 // contiguous part of one row at a time; in 64 bits each has a stretch of the vocabulary, whose
@@ -70,6 +70,7 @@ struct VerifyArgs {
     int V, K, ctas;
     int keep;                           // elements of a CTA's stretch of a row that are kept, 0: none
     float c2;                           // log2(e) / T
+    double near;                        // what two 32-bit sums may be off by, of themselves
     double scale;                       // kTable log2(e) / T
     int64_t *tokens, *accepted;
 };
@@ -321,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const 
         auto test = [&](float u, float xp, float xq, int r, double zp, double zq, bool &near) {
             const double p = term(xp, greatest(r)), q = u * (Own ? term(xq, greatest(n + 1 + r)) : 1.0);      // times z
             const double l = q * zp, m = Own ? p * zq : p;
-            near = fabs(l - m) <= 0x1p-13 * fmax(fabs(l), m) && m > 0.0;
+            near = fabs(l - m) <= P.near * fmax(fabs(l), m) && m > 0.0;
             return l < m ? kStays : kFalls;
         };
         if (static_cast<int>(threadIdx.x) < n) {
@@ -603,6 +604,9 @@ cudaError_t launch_verify_drafts(const void *logits, int dt, int64_t ld_seq, int
     const double per = greedy ? 1.0 : 1.4426950408889634 / temperature;
     p.c2 = static_cast<float>(per);
     p.scale = kTable * per;
+    // a lane adds up to V / 64 terms to each of its two sums, which all may round the same way, by 2^-24 of the sum: twice that
+    // for the two rows; 2^-13 for exponentials and what joins the lanes (2^-18) and vocabularies up to 65536
+    p.near = std::max(0x1p-13, V * 0x1p-29);
     p.tokens = tokens;
     p.accepted = accepted;
     // as many CTAs a sequence as fit the GPU with those of all sequences

@@ -33,3 +33,26 @@ def test_a_draft_falls_between_equal_rows(dtype, B, V, shift):
     assert not want[1][:4].any() and len(set(want[0][:, 0].tolist())) > 4
     if shift == 0.0:
         _check(logits, drafts, u, draft, 0.7)
+
+# ------------------------------------------------------------------ sums that 32 bits do not hold
+def test_sums_of_very_large_vocabularies():
+    """Rows of two values: a lane's 32-bit sum of 32768 equal terms is off by up to 2^-11 of it, as every
+    addition rounds the same way. Drafts are tested at given numbers 2^-11.. 2^-13 beside p."""
+    from naylis_b200 import scoring
+    V, K, B, high = 1 << 21, 7, 256, 4096
+    gaps = torch.tensor([1.0, 1.25, 1.5, 2.0, 2.25, 3.0, 3.5, 0.75])
+    x = torch.zeros(K + 1, V) - gaps[:, None]
+    x[:, :high] = 0.0
+    logits = x.to(torch.bfloat16).to(DEV).expand(B, K + 1, V)
+    p = 1.0 / (high + (V - high) * torch.exp(-gaps.double()))
+    drafts = torch.arange(B * K).view(B, K) % high      # of the likely ones
+    u = torch.zeros(B, K + 1)
+    u[:, K] = 0.5
+    want = torch.empty(B, dtype=torch.int64)
+    for b in range(B):
+        j, f = b % K, 2.0 ** (-11 - (b // K) % 9 / 4) * (1 if b // (9 * K) % 2 else -1)
+        u[b, j] = float(p[j] * (1 + f))
+        u[b, j + 1:K] = 1.0
+        want[b] = j + int(float(u[b, j]) < float(p[j]))
+    got = scoring.verify_drafts(logits, drafts.to(DEV), u.to(DEV))
+    assert torch.equal(got.accepted.cpu(), want), (got.accepted.cpu() != want).nonzero()[:, 0].tolist()
