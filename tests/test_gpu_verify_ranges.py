@@ -56,3 +56,46 @@ def test_sums_of_very_large_vocabularies():
         want[b] = j + int(float(u[b, j]) < float(p[j]))
     got = scoring.verify_drafts(logits, drafts.to(DEV), u.to(DEV))
     assert torch.equal(got.accepted.cpu(), want), (got.accepted.cpu() != want).nonzero()[:, 0].tolist()
+
+# ------------------------------------------------------------------ terms that are not kept
+NOT_KEPT = [("sampled", 9, 2, 40000), ("sampled", 600, 2, 5001), ("lookup", 9, 2, 70001), ("lookup", 600, 1, 9001)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("mode,B,K,V", NOT_KEPT)
+def test_vocabularies_that_are_not_kept(dtype, mode, B, K, V):
+    """A CTA's stretch of the rows is more than its shared memory holds: terms are computed where they are needed."""
+    logits, drafts, u, draft = _make(B + V, B, K, V, dtype, mode, 0.8)
+    logits[0, 0, V // 3:] = -INF
+    logits[1, 0, :V - 5] = torch.finfo(dtype).min
+    logits[2, 0, 11] = NAN
+    logits[3, 0] = -INF
+    logits[4, 0] = 0.25
+    drafts[5, 0], drafts[6, 0] = -1, V
+    logits[7, 0, drafts[7, 0]] = -INF
+    if draft is not None:
+        draft[8, 0] = logits[8, 0]
+        draft[3, 1], draft[4, 0] = -INF, 0.25
+    want = _check(logits, drafts, u, draft, 0.8)
+    if B > 9:      # the inputs reach every end
+        assert len(set(want[1].tolist())) > 1
+    _check(logits, drafts, u, draft, 0.8, [(3 * i) % (K + 1) for i in range(B)])
+    for value in (0.0, 1 - 2.0 ** -24):
+        u2 = u.clone()
+        u2[:, K] = value
+        _check(logits, drafts, u2, draft, 0.8)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("own", [False, True])
+def test_borders_that_are_not_kept(dtype, own):
+    """Given numbers at p / q, where 32-bit sums leave the draft open."""
+    B, K, V = (9, 2, 40009) if own else (9, 2, 70001)
+    logits, drafts, u, draft = _make(5, B, K, V, dtype, "sampled" if own else "lookup", 1.0, noise=2.0)
+    r = torch.softmax(logits[:, :K].double(), -1).gather(2, drafts[..., None])[..., 0]
+    if own:
+        r = r / torch.softmax(draft.double(), -1).gather(2, drafts[..., None])[..., 0]
+    for f in (1.0, 1 - 2.0 ** -23, 1 + 2.0 ** -22, 1 - 1e-5, 1 + 1e-5):
+        u2 = u.clone()
+        u2[:, :K] = (r * f).clamp(0, 1 - 2.0 ** -24).float()
+        _check(logits, drafts, u2, draft, 1.0)
