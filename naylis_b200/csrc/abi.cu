@@ -962,6 +962,11 @@ int check_int4_cache(int64_t num_pages, int64_t Hk, int64_t page_size) {
     MOM_REQUIRE(num_pages <= (int64_t(1) << 31) / (Hk * page_size), "the cache has more than 2^31 rows");
     return MOM_OK;
 }
+bool int4_decode_fits(int64_t B, int64_t n_new, int64_t H, int64_t max_len) {
+    // a span, 1/444 of the tiles at most, is counted in 32 bits, and so is a list that ends behind it
+    return B <= 65535 && n_new >= 1 && n_new <= 64 && H <= 65535 && max_len >= 0 && max_len <= INT32_MAX &&
+           B * n_new * H <= (1 << 30) && B * n_new * H * (max_len / 32 + 8) <= (int64_t(1) << 37);
+}
 }  // namespace
 
 int mom_rope_append_int4(const void *qkv, int64_t qkv_ld, const float *cosv, const float *sinv, int64_t n_pos,
@@ -990,7 +995,8 @@ int mom_rope_append_int4(const void *qkv, int64_t qkv_ld, const float *cosv, con
 
 size_t mom_decode_attn_int4_workspace_size(int64_t B, int64_t n_new, int64_t H, int64_t Hk, int64_t hd,
                                            int64_t max_len) {
-    if (B <= 0 || n_new <= 0 || H <= 0 || Hk <= 0 || H < Hk || hd <= 0 || max_len < 0) return 0;
+    // 0 for what the call refuses: the split's arithmetic is for its sizes
+    if (B <= 0 || H <= 0 || Hk <= 0 || H % Hk || (hd != 64 && hd != 128) || !int4_decode_fits(B, n_new, H, max_len)) return 0;
     return mom::decode_int4_bytes(B, n_new * (H / Hk), Hk, hd, max_len);
 }
 
@@ -1005,9 +1011,7 @@ int mom_decode_attn_int4(const void *q, int64_t q_ld, const void *k_pages, const
     MOM_REQUIRE(B >= 0 && B <= 65535, "B must be in [0, 65535] (got %lld)", (long long)B);
     MOM_REQUIRE(n_new >= 1 && n_new <= 64, "n_new must be in [1, 64] (got %lld)", (long long)n_new);
     MOM_REQUIRE(max_len >= 0 && max_len <= INT32_MAX, "max_len out of range");
-    // a span, 1/444 of the tiles at most, is counted in 32 bits, and so is a list that ends behind it
-    MOM_REQUIRE(B * n_new * H <= (1 << 30) && B * n_new * H * (max_len / 32 + 8) <= (int64_t(1) << 37),
-                "too many sequences, new tokens, heads and keys (2^30, 2^42)");
+    MOM_REQUIRE(int4_decode_fits(B, n_new, H, max_len), "too many sequences, new tokens, heads and keys (2^30, 2^42)");
     MOM_REQUIRE(table_ld >= 0 && max_len <= table_ld * page_size, "max_len exceeds the block table (%lld pages of %lld)",
                 (long long)table_ld, (long long)page_size);
     MOM_REQUIRE(q_ld >= H * hd && q_ld % 8 == 0, "q row pitch must hold all heads and be a multiple of 8");
