@@ -424,6 +424,7 @@ def generate(model: NaylisForCausalLM, prompts, max_new_tokens: int, *, temperat
         most = min(attention.MAX_NEW - 1, scoring.MAX_DRAFTS)
         if not 1 <= draft_tokens <= most:
             raise RuntimeError(f"generate: draft_tokens {draft_tokens} must be in [1, {most}]")
+        _check_model(model)
         _check_model(draft_model)
         if draft_model.config.vocab_size != model.config.vocab_size:
             raise RuntimeError(f"generate: the draft model has {draft_model.config.vocab_size} tokens, the model "
