@@ -179,16 +179,18 @@ class Session:
                 h, sums, plan = self._prefill(prompts, positions, slots)
                 last = torch.tensor(lens, device=self.device).cumsum(0) - 1
                 logits = trunk.linear_f32grad(h[last], self.model.lm_head.weight)
+            past = [s.new_zeros(len(new), self.undo, s.shape[1]) for s in sums] if self.undo else None
+            if self.sums is not None:
+                sums = [torch.cat(p) for p in zip(self.sums, sums)]
+                past = past and [torch.cat(p) for p in zip(self._past, past)]
             plan.check()
         except BaseException:
             for s in new:
                 self.cache.free(s)
             raise
+        self.sums = sums
         if self.undo:
-            past = [s.new_zeros(len(new), self.undo, s.shape[1]) for s in sums]
-            self._past = past if self._past is None else [torch.cat(p) for p in zip(self._past, past)]
-            self._known += [0] * len(new)
-        self.sums = sums if self.sums is None else [torch.cat(p) for p in zip(self.sums, sums)]
+            self._past, self._known = past, self._known + [0] * len(new)
         self.seqs += new
         return logits
 
