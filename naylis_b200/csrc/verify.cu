@@ -31,7 +31,7 @@ namespace mom {
 namespace {
 
 constexpr int kWarps = 8, kThreads = kWarps * 32;
-constexpr int kMostCtas = 16;      // of a cluster: 16 where there are few sequences, else 8 at most
+constexpr int kMostCtas = 16;      // of a cluster: 16 where there are few sequences and the device places them, else 8 at most
 constexpr int kHold = 4;            // vectors of a lane in flight, twice
 constexpr int kBatch = 8;           // elements of a lane in flight, of each row
 constexpr int kRounds = 9;          // parts of rows that a warp takes, at most: all rows, one CTA
@@ -565,19 +565,50 @@ __global__ void __launch_bounds__(kThreads, Greedy ? 4 : 3) verify_kernel(const 
 }
 
 template <int DT, bool Greedy, bool Own>
-cudaError_t launch(cudaLaunchConfig_t &cfg, const VerifyArgs &p) {
-    static std::atomic<uint64_t> ready{0};      // devices whose kernel has its shared memory set
+cudaError_t launch(VerifyArgs &p, int64_t B, cudaStream_t st) {
+    static std::atomic<uint64_t> ready{0}, most{0};      // devices whose kernel has its shared memory set; that place kMostCtas
+    const auto kernel = verify_kernel<DT, Greedy, Own>;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
-        e = cudaFuncSetAttribute(verify_kernel<DT, Greedy, Own>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostKeep * 8);
-        if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(verify_kernel<DT, Greedy, Own>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess) return e;
-        if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = kMostCtas;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(kMostCtas, static_cast<unsigned>(B));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kMostKeep * sizeof(double);
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const uint64_t bit = uint64_t(1) << (dev & 63);
+    bool fits;
+    if (dev < 64 && ready.load(std::memory_order_acquire) & bit) {
+        fits = most.load(std::memory_order_relaxed) & bit;
+    } else {
+        if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostKeep * 8)) != cudaSuccess ||
+            (e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess)
+            return e;
+        // more than 8 CTAs a cluster are not promised: a part of a GPU may have no 16 processors side by side
+        int n = 0;
+        if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) n = 0, cudaGetLastError();
+        fits = n > 0;
+        if (dev < 64) {
+            if (fits) most.fetch_or(bit, std::memory_order_relaxed);
+            ready.fetch_or(bit, std::memory_order_release);
+        }
     }
-    e = cudaLaunchKernelEx(&cfg, verify_kernel<DT, Greedy, Own>, p);
+    // as many CTAs a sequence as fit the GPU with those of all sequences; 16 for few of them (4 sampled drafts of 32000, 16 and
+    // 8: 1 sequence 11.1 and 13.1 us, 4 12.4 and 14.8, 8 14.1 and 14.9, 20 17.0 and 16.7, 27 26.6 and 18.0)
+    p.ctas = B <= 8 && fits ? kMostCtas : 8;
+    while (p.ctas > 1 && B * p.ctas > (Greedy ? 4 : 3) * device_sm_count()) p.ctas /= 2;
+    const int keep = (p.V + p.ctas - 1) / p.ctas + 1, kept = Own ? 2 : 1;
+    if (!Greedy && static_cast<int64_t>(keep) * kept <= kMostKeep) p.keep = keep;
+    attr.val.clusterDim.x = static_cast<unsigned>(p.ctas);
+    cfg.gridDim.x = static_cast<unsigned>(p.ctas);
+    cfg.dynamicSmemBytes = static_cast<size_t>(p.keep) * kept * sizeof(double);
+    e = cudaLaunchKernelEx(&cfg, kernel, p);
     count_launch();
     return e;
 }
@@ -609,27 +640,11 @@ cudaError_t launch_verify_drafts(const void *logits, int dt, int64_t ld_seq, int
     p.near = std::max(0x1p-13, V * 0x1p-29);
     p.tokens = tokens;
     p.accepted = accepted;
-    // as many CTAs a sequence as fit the GPU with those of all sequences
-    p.ctas = B <= 8 ? kMostCtas : 8;
-    while (p.ctas > 1 && B * p.ctas > (greedy ? 4 : 3) * device_sm_count()) p.ctas /= 2;
-    const int keep = (V + p.ctas - 1) / p.ctas + 1;
-    if (!greedy && static_cast<int64_t>(keep) * (draft ? 2 : 1) <= kMostKeep) p.keep = keep;
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = static_cast<unsigned>(p.ctas);
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.gridDim = dim3(static_cast<unsigned>(p.ctas), static_cast<unsigned>(B));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = static_cast<size_t>(p.keep) * (draft ? 2 : 1) * sizeof(double);
-    cfg.stream = st;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
     if (dt == MOM_BF16)
-        return greedy ? launch<MOM_BF16, true, false>(cfg, p)
-                      : draft ? launch<MOM_BF16, false, true>(cfg, p) : launch<MOM_BF16, false, false>(cfg, p);
-    return greedy ? launch<MOM_F32, true, false>(cfg, p)
-                  : draft ? launch<MOM_F32, false, true>(cfg, p) : launch<MOM_F32, false, false>(cfg, p);
+        return greedy ? launch<MOM_BF16, true, false>(p, B, st)
+                      : draft ? launch<MOM_BF16, false, true>(p, B, st) : launch<MOM_BF16, false, false>(p, B, st);
+    return greedy ? launch<MOM_F32, true, false>(p, B, st)
+                  : draft ? launch<MOM_F32, false, true>(p, B, st) : launch<MOM_F32, false, false>(p, B, st);
 }
 
 }  // namespace mom

@@ -1,5 +1,9 @@
 """GPU tests of scoring.verify_drafts where its parts meet: drafts that fall although both rows are
 one distribution, vocabularies whose terms are not kept, sums that 32 bits do not hold."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -99,3 +103,45 @@ def test_borders_that_are_not_kept(dtype, own):
         u2 = u.clone()
         u2[:, :K] = (r * f).clamp(0, 1 - 2.0 ** -24).float()
         _check(logits, drafts, u2, draft, 1.0)
+
+
+# ------------------------------------------------------------------ clusters of either size
+@pytest.mark.parametrize("mode,T", [("sampled", 1.0), ("lookup", 1.0), ("greedy", 0.0)])
+@pytest.mark.parametrize("V", [5003, 40000])
+def test_a_sequence_alone_and_in_a_batch(mode, T, V):
+    """Clusters of 16 CTAs alone, of 8 and fewer among others: the same tokens."""
+    from naylis_b200 import scoring
+    logits, drafts, u, draft = _make(V, 70, 3, V, torch.bfloat16, mode, T)
+
+    def run(rows):
+        return scoring.verify_drafts(logits[rows], drafts[rows], None if u is None else u[rows], temperature=T,
+                                     draft_logits=None if draft is None else draft[rows])
+
+    every = run(slice(0, 70))
+    for n in (1, 8, 9, 30):
+        got = run(slice(0, n))
+        assert torch.equal(got.tokens, every.tokens[:n]) and torch.equal(got.accepted, every.accepted[:n])
+
+
+def test_a_first_call_that_is_captured():
+    """A process whose first calls are captured: what they ask of the device once does not disturb it."""
+    code = """
+import torch
+from naylis_b200 import scoring
+for dtype in (torch.bfloat16, torch.float32):
+    x, q = torch.randn(3, 3, 500, device="cuda").to(dtype), torch.randn(3, 2, 500, device="cuda").to(dtype)
+    d, u = torch.randint(0, 500, (3, 2), device="cuda"), torch.rand(3, 3, device="cuda")
+    torch.cuda.synchronize()
+    for args, kw in (((x, d, u), dict(draft_logits=q)), ((x, d, u), {}), ((x, d), dict(temperature=0.0))):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = scoring.verify_drafts(*args, **kw)
+        g.replay()
+        torch.cuda.synchronize()
+        now = scoring.verify_drafts(*args, **kw)
+        assert torch.equal(got.tokens, now.tokens) and torch.equal(got.accepted, now.accepted)
+print("fine")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=root)
+    assert r.returncode == 0 and r.stdout.strip() == "fine", r.stderr[-2000:]
