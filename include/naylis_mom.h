@@ -398,8 +398,9 @@ MOM_API int mom_decode_attn(const void *q, int64_t q_ld, const void *k_pages, co
 
 /* The same over a cache in 4 bits. A row (a token's key or value of one head) is cut into
  * groups of 64 values; a group keeps zero = its least value, scale = bf16((greatest -
- * least) / 15) and of each value x the number n = round((x - zero) / scale), 0 to 15 (0
- * where scale is 0): it stands for zero + n scale. A group with a value that is not
+ * least) s), s = 1 / 15 in fp32 and difference and product rounded to fp32, and of each
+ * value x the number n = round((x - zero) / scale), 0 to 15 (0 where scale is 0): it
+ * stands for zero + n scale. A group with a value that is not
  * finite, or a range beyond fp32, stands for NaN. k_pages, v_pages (num_pages, Hk,
  * page_size, hd / 2) bytes, the even dimension's number in a byte's low half; scales
  * (num_pages, Hk, page_size, hd / 64, 4) bf16, the key's scale and zero and the value's.

@@ -301,8 +301,8 @@ def rope_append_int4(qkv, cos, sin, positions, k_pages, v_pages, scales, slots, 
     bf16, written in place.
 
     Each 64 values of a key (rotated, rounded to bf16) or a value keep zero = the
-    least of them and scale = bf16((greatest - least) / 15), in fp32, and of each x the
-    number n = round((x - zero) / scale), 0 to 15 (0 where scale is 0): it stands for
+    least of them and scale = bf16((greatest - least) * fp32(1 / 15)), in fp32 (a product, not a
+    division: the two differ where bf16 rounds a tie), and of each x the number n = round((x - zero) / scale), 0 to 15 (0 where scale is 0): it stands for
     zero + n scale. A group with a value that is not finite, or a range beyond fp32,
     stands for NaN. Two numbers share a byte, the even dimension's in the low half;
     the last axis of scales is the key's scale and zero, then the value's. Tokens of one

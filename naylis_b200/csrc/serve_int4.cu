@@ -2,7 +2,7 @@
 // attention of one or several new tokens of each sequence over it.
 //
 // A row (a token's key or value of one head) is cut into groups of 64 values. A group
-// keeps zero = its least value and scale = bf16((greatest - least) / 15), and of each
+// keeps zero = its least value and scale = bf16((greatest - least) fp32(1 / 15)), and of each
 // value x the number n = round((x - zero) / scale), 0 .. 15; it stands for zero + n scale.
 // Pages (num_pages, Hk, page_size, hd / 2) bytes, the even dimension in a byte's low half;
 // scales (num_pages, Hk, page_size, hd / 64, 4) bf16: the key's scale and zero, the
