@@ -53,3 +53,13 @@ def test_a_prefill_whose_joins_fail_adds_nothing(session, monkeypatch):  # noqa:
     assert s._known == [1, 0, 0] and [len(t) for t in s.sums] == [len(p) for p in s._past] == [3] * len(s.sums)
     s.retract([1, 0, 0])
     assert [t[:, 0].tolist() for t in s.sums] == [[3.0, 9.0, 6.0]] * len(s.sums)
+
+
+def test_ragged_tokens_come_padded(session):  # noqa: F811
+    """Several tokens of each sequence: a tensor with a count for each row; lists of lists are refused."""
+    s = session
+    s.add([[1, 2], [3]])
+    logits = s.extend(torch.tensor([[4, 5, 6], [7, 8, 0]]), counts=[3, 2])
+    assert [s.cache.length(q) for q in s.seqs] == [5, 3] and not logits[1, 2].any() and bool(logits[0, 2].any())
+    with pytest.raises(RuntimeError, match="tokens must be"):
+        s.extend([[4, 5, 6], [7, 8]])
