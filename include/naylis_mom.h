@@ -421,7 +421,8 @@ MOM_API int mom_rope_append_int4(const void *qkv, int64_t qkv_ld, const float *c
  * behind new_len, gets zeros. A new_len outside [0, n_new] makes the sequence NaN. What a
  * token does not see does not reach it, NaN neither. Else as mom_decode_attn, with B n_new
  * H at most 2^30 and B n_new H (max_len / 32 + 8) at most 2^37. A weight below 2^-126 of its
- * row's greatest counts as 0; scales and zeros below 2^-100 may count with fewer bits. */
+ * row's greatest counts as 0; scales and zeros below 2^-100 may count with fewer bits; sums of
+ * weights (the greatest 1 to 8) times values have to stay within fp32. */
 MOM_API size_t mom_decode_attn_int4_workspace_size(int64_t B, int64_t n_new, int64_t H, int64_t Hk, int64_t head_dim,
                                                    int64_t max_len);
 MOM_API int mom_decode_attn_int4(const void *q, int64_t q_ld, const void *k_pages, const void *v_pages,

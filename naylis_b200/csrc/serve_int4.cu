@@ -211,8 +211,8 @@ rope_append_int4_kernel(const uint16_t *__restrict__ qkv, int64_t ld, const floa
 // or 24 rows a list, whose sums leave room for 2 CTAs an SM: 56 and 59). The queries of a row are scaled by a power of two to 2^9 .. 2^10 at most, so that fp16
 // holds their bits: those 2^-31 of the greatest and smaller may lose some, 2^-39 of it. A score before
 // the scale is in units of that: of keys that stand for less than about 2^-100 it may lose bits. The weights p_t s_t are fp16, against a unit for each row and group, a
-// power of two: 11 bits, a quarter of the output's own rounding; those below 2^-25 of the row's
-// greatest so far lose bits, below 2^-36 they vanish. p is taken against a reference within 2^3 of the greatest so far, which
+// power of two: 11 bits, a quarter of the output's own rounding; those below 2^-21 of the row's
+// greatest so far lose bits, below 2^-32 they vanish. p is taken against a reference within 2^3 of the greatest so far, which
 // moves when that is passed: no search for the maximum in a tile that does not. The unit likewise is lowered when a weight
 // passes 2^15, and rises with the reference: keys that a row does not see, or that have no weight, do not
 // count for it, whatever their scales. Everything else is fp32.
@@ -562,7 +562,8 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
         };
         const auto exponent = [](float x) { return (__float_as_int(x) >> 23) - 127; };      // of a positive one
         // x0, x1: the greatest weights times scales of this lane's keys, times 2^-8 (finite where the scales are). Rows
-        // whose weights pass kMostWeight get the unit that brings the greatest to 2^11 .. 2^12.
+        // whose weights pass kMostWeight get the unit that brings the greatest to 2^7 .. 2^8: room for what the next
+        // tiles bring (24 x 5 tokens 55.3 us; to 2^11 58.1, to 2^3 55.2).
         auto lower = [&](int g, float x0, float x1) {
             const float2 u = tc::f2_split(unit[g]);
             float x[2] = {x0, x1}, from[2] = {u.x, u.y}, f[2];
@@ -570,7 +571,7 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
             for (int e = 0; e < (ROWS == 8 ? 2 : 1); ++e) {
                 x[e] = most_of_row(x[e]);
                 const int was = exponent(from[e]);
-                const int to = x[e] * 256.0f * from[e] >= kMostWeight ? max(3 - exponent(x[e]), -126) : was;
+                const int to = x[e] * 256.0f * from[e] >= kMostWeight ? max(-1 - exponent(x[e]), -126) : was;
                 f[e] = to - was < -126 ? 0.0f : pow2(to - was);
                 from[e] = pow2(to);
             }
@@ -690,16 +691,22 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
 #pragma unroll
                 for (int k = 0; k < kKeys; ++k) mx = fmaxf(mx, t[k]);
                 if (__any_sync(0xffffffffu, mx * low(crow) > far[0])) move(mx * low(crow), -INFINITY);
-                float w[NG][kKeys];
+                // weights to the lanes that multiply them: key t at (t mod 4, t / 4), once in the low half and once in the high one
                 const auto weigh = [&] {
                     float most = 0.0f;
 #pragma unroll
-                    for (int g = 0; g < NG; ++g)
+                    for (int k = 0; k < kKeys; ++k) {
+                        const int key = 32 * k + 8 * c4 + r8;
 #pragma unroll
-                        for (int k = 0; k < kKeys; ++k) {
-                            w[g][k] = t[k] * low(unit[g]) * bf_lo(raw[g][k].y);
-                            most = fmaxf(most, w[g][k]);
+                        for (int g = 0; g < NG; ++g) {
+                            const float w = t[k] * low(unit[g]) * bf_lo(raw[g][k].y);
+                            most = fmaxf(most, w);
+                            const uint32_t half = pack_f16x2(w, 0.0f);
+                            uint32_t *to = s_w + 8 * C::kStride * g + (key & 3) * C::kStride + (key >> 2);
+                            to[0] = half;
+                            to[4 * C::kStride] = half << 16;
                         }
+                    }
                     return most;
                 };
 #pragma unroll
@@ -718,18 +725,6 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                         lower(g, most, 0.0f);
                     }
                     weigh();
-                }
-                // weights to the lanes that multiply them: key t at (t mod 4, t / 4), once in the low half and once in the high one
-#pragma unroll
-                for (int k = 0; k < kKeys; ++k) {
-                    const int key = 32 * k + 8 * c4 + r8;
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) {
-                        const uint32_t half = pack_f16x2(w[g][k], 0.0f);
-                        uint32_t *to = s_w + 8 * C::kStride * g + (key & 3) * C::kStride + (key >> 2);
-                        to[0] = half;
-                        to[4 * C::kStride] = half << 16;
-                    }
                 }
                 __syncwarp();
                 // outputs: words r8 of keys 4 j + c4; an even column has their low halves' products, an odd one the high ones'
@@ -907,7 +902,7 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                             if constexpr (some_hidden.value) sz.x = seen(sz.x, n), sz.y = seen(sz.y, n);
                             z2[g] = tc::fma2(t[n], sz.y, z2[g]);
                             const float2 w = tc::f2_split(tc::mul2(tc::mul2(t[n], unit[g]), sz.x));
-                            pw[g][n] = pack_f16x2(w.x, w.y);
+                            pw[g][n] = transpose8(pack_f16x2(w.x, w.y));
                             most = tc::fmax3(most, w.x, w.y);
                         }
                     }
@@ -929,14 +924,10 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
 #pragma unroll
                         for (int n = 0; n < NB; ++n) {
                             const float2 w = tc::f2_split(tc::mul2(tc::mul2(t[n], unit[g]), scale(n)));
-                            pw[g][n] = pack_f16x2(w.x, w.y);
+                            pw[g][n] = transpose8(pack_f16x2(w.x, w.y));
                         }
                     }
                 }
-#pragma unroll
-                for (int g = 0; g < NG; ++g)
-#pragma unroll
-                    for (int n = 0; n < NB; ++n) pw[g][n] = transpose8(pw[g][n]);
                 const unsigned char *v0 = sv + key_of(2 * c4) * C::kRowBytes + 4 * r8, *v1 = sv + key_of(2 * c4 + 1) * C::kRowBytes + 4 * r8;
 #pragma unroll
                 for (int g = 0; g < NG; ++g)
@@ -1031,14 +1022,14 @@ decode_int4_kernel(const __grid_constant__ Decode4Args P) {
                 }
             __syncwarp();      // the warp's sums are read; their place takes its outputs
         }
-        // the numbers' 2^-24 and 2^-20 and the weights' unit taken out: that is 2^-119 (where scales are finite) to 2^120
+        // the numbers' 2^-24 and 2^-20 and the weights' unit taken out: that is 2^-124 (where scales are finite) to 2^120
         const auto part_of = [&](int row, int g, int e) {
             const float f = s_m[warp][row] == -INFINITY ? 0.0f : tc::ex2(s_m[warp][row] - reference(row));
             const float2 u = tc::f2_split(unit[g]);
-            return pow2(min(8 - exponent(e ? u.y : u.x), 127)) * f;
+            return pow2(min(3 - exponent(e ? u.y : u.x), 127)) * f;
         };
         const auto pair_of = [](const float (&x)[4], int e, float u) {
-            return make_float2(x[e] * 65536.0f * u, x[2 + e] * 4096.0f * u);
+            return make_float2(x[e] * 0x1p21f * u, x[2 + e] * 0x1p17f * u);
         };
 #pragma unroll
         for (int g = 0; g < NG; ++g) {

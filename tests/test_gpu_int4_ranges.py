@@ -1,7 +1,7 @@
 """GPU tests of decode_attention_int4 at the ends of its range: scales, queries and lengths far
 from the usual ones. Tolerances, where not said otherwise, are test_gpu_int4_cache's: the
-weights' fp16 numbers lose bits below 2^-26 of the row's greatest product of weight and
-scale, 2^-36 of it and 15 numbers a key, which 2^-10 A contains up to 2^20 keys. (No floor
+weights' fp16 numbers lose bits below 2^-21 of the row's greatest product of weight and
+scale, 2^-32 of it and 15 numbers a key, which 2^-10 A contains up to 2^18 keys. (No floor
 under the tolerance: outputs may be as small as their values.)"""
 import pytest
 import torch
@@ -109,6 +109,21 @@ def test_scales_that_are_not_finite(H, Hk, n):
         hit[:, :, :H // Hk, 64:] = True
         _close(got[~hit], want[~hit], A[~hit])
         assert not bool(torch.isfinite(got[hit]).any())
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("H,Hk,n", [(2, 2, 1), (2, 2, 4), (8, 2, 4)])
+@pytest.mark.parametrize("size", [2.0 ** 124, 1e36, 1e-36, 2.0 ** -126])
+def test_scales_at_the_ends(hd, H, Hk, n, size):
+    """The greatest scale that a finite range has, and the least normal one; few keys, whose sums stay in fp32."""
+    lens = [2, 1, 0]
+    q, (k, v, s), table, sl = _case(hd, H, Hk, 16, lens, n, seed=26, qscale=0.1)
+    s2 = torch.nan_to_num(s.float(), nan=0.5)
+    s2[..., 2], s2[..., 3] = size, -3.75 * size
+    s2 = s2.to(torch.bfloat16)
+    v = v & 0x77      # numbers up to 7: values within 3.75 scales of 0
+    got = _run(q, (k, v, s2), table, sl)
+    _close(got, *_exact(q, (k, v, s2), table, lens, [n] * 3, hd ** -0.5))
+
 
 # ------------------------------------------------------------------ queries of any size
 @pytest.mark.parametrize("hd", [64, 128])
