@@ -337,8 +337,8 @@ def decode_attention_int4(q, k_pages, v_pages, scales, block_table, seq_lens, *,
     and rows behind new_len, get zeros. pages and scales as rope_append_int4 files
     them; block_table, seq_lens, scale and max_len as decode_attention takes them. A
     sequence longer than max_len, with a page outside the cache or with a new_len
-    outside [0, n]: NaN. What a token does not see does not reach it. Returns
-    (B, n, H, hd) bf16."""
+    outside [0, n]: NaN. What a token does not see does not reach it. A weight below
+    2^-126 of its row's greatest counts as 0. Returns (B, n, H, hd) bf16."""
     name = "decode_attention_int4"
     P, Hk, page, hd = _pages_int4(name, k_pages, v_pages, scales)
     _check(name, q, scales)

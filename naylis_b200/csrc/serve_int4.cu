@@ -202,31 +202,33 @@ rope_append_int4_kernel(const uint16_t *__restrict__ qkv, int64_t ld, const floa
 // bits 1.7e-3, a bf16 result's own 1.6e-3; with bytes and one accumulator it was 3.3e-3.
 //
 // Both products have the numbers as their first operand: scores are keys by rows (heads, new
-// tokens), outputs dimensions by rows, so that 8 rows cost half of what 16 do; the weights
-// turn from the one layout to the other by movmatrix. Up to 4 rows have two columns each,
-// which take the parts of a byte and of a word apart: neither masks nor pairs of keys to
-// make. One row alone (a head of keys for each of queries, one new token) has its softmax
-// shared out over all lanes. More than 8 rows are lists of their own, which read the keys
-// again (from L2: 24 sequences of 1024 to 8191, 20 rows on each of 4 heads of 128: 52 us; up to 16
-// or 24 rows a list, whose sums leave room for 2 CTAs an SM: 56 and 59). The queries of a row are scaled by a power of two to 2^9 .. 2^10 at most, so that fp16
-// holds their bits: those 2^-31 of the greatest and smaller may lose some, 2^-39 of it. A score before
-// the scale is in units of that: of keys that stand for less than about 2^-100 it may lose bits. The weights p_t s_t are fp16, against a unit for each row and group, a
-// power of two: 11 bits, a quarter of the output's own rounding; those below 2^-21 of the row's
-// greatest so far lose bits, below 2^-32 they vanish. p is taken against a reference within 2^3 of the greatest so far, which
-// moves when that is passed: no search for the maximum in a tile that does not. The unit likewise is lowered when a weight
-// passes 2^15, and rises with the reference: keys that a row does not see, or that have no weight, do not
-// count for it, whatever their scales. Everything else is fp32.
+// tokens), outputs dimensions by rows, so that 8 rows cost half of what 16 do; the weights turn
+// from the one layout to the other by movmatrix. Up to 4 rows have two columns each, which take
+// the parts of a byte and of a word apart: neither masks nor pairs of keys to make. One row alone
+// (a head of keys for each of queries, one new token) has its softmax shared out over all lanes.
+// More than 8 rows are lists of their own, which read the keys again (from L2: 24 sequences of
+// 1024 to 8191, 20 rows on each of 4 heads of 128: 55 us; up to 16 or 24 rows a list, whose sums
+// leave room for 2 CTAs an SM, 8 and 15 % more). The queries of a row are scaled by a power of two
+// to 2^9 .. 2^10 at most, so that fp16 holds their bits: those 2^-31 of the greatest and smaller
+// may lose some, 2^-39 of it. A score before the scale is in units of that: of keys that stand for
+// less than about 2^-100 it may lose bits. The weights p_t s_t are fp16, against a unit for each
+// row and group, a power of two: 11 bits, a quarter of the output's own rounding; those below
+// 2^-21 of the row's greatest so far lose bits, below 2^-32 they vanish. p is taken against a
+// reference within 2^3 of the greatest so far, which moves when that is passed: no search for the
+// maximum in a tile that does not. The unit likewise is lowered when a weight passes 2^15, and
+// rises with the reference: keys that a row does not see, or that have no weight, do not count for
+// it, whatever their scales. Everything else is fp32.
 //
 // A warp takes tiles of 64 keys (hd 128: 32) through a ring of its own, as the bf16 kernel
 // does, by bulk copies: a lane for each page's keys, values or scales (16-byte copies of
 // each row took 105 instructions a tile). What a page holds behind the sequence's end
 // comes along and is hidden like all that a row does not see.
 //
-// Bound by memory where there is much of it (16 sequences of 32768, 16 heads of 64: 103 us, 5.9
+// Bound by memory where there is much of it (16 sequences of 32768, 16 heads of 64: 103.5 us, 5.8
 // TB/s; the copies alone 96), by instruction issue and by memory alike for grouped heads (4 of
-// 87,000 to 131,072, 16 heads on 4 of 128: 59 us; the copies alone 45, the rest alone 47), by
+// 87,000 to 131,072, 16 heads on 4 of 128: 58 us; the copies alone 45, the rest alone 47), by
 // issue with many rows, by starts and ends of lists when these are short (48 of 64 to 4096, 16
-// heads of 64: 24 us; 1 of 577: 5 us).
+// heads of 64: 25 us; 1 of 577: 5 us).
 constexpr float kSlack = 3.0f;      // log2
 constexpr int kMostUnit = 120;      // log2 of the weights' greatest unit: 2^4 times it, the most that kSlack rounds to, is in fp32
 constexpr float kMostWeight = 32768.0f;      // what weights stay below, fp16 having 65504
